@@ -8,10 +8,11 @@ no CPU or framework fallback.
 from . import ffi
 from .inference import ModelOverrides, build_model_config
 from .kernel import BlockPattern1d, BlockPattern2d, BlockSparseConfig
-from .model import BDH, BDHConfig, FusedKernelConfig, LayerState, ModelState
+from .model import BDH, BDHConfig, FusedKernelConfig, LayerState, ModelState, SharedState
 from .positional import RotaryEmbedding
+from .rules import LogitRules
 from .tokenizer import ByteTokenizer, CharVocab, Tokenizer
 
 __all__ = ["ffi", "ModelOverrides", "build_model_config", "BlockPattern1d", "BlockPattern2d", "BlockSparseConfig",
-           "BDH", "BDHConfig", "FusedKernelConfig", "LayerState", "ModelState", "RotaryEmbedding",
-           "ByteTokenizer", "CharVocab", "Tokenizer"]
+           "BDH", "BDHConfig", "FusedKernelConfig", "LayerState", "ModelState", "SharedState", "RotaryEmbedding",
+           "LogitRules", "ByteTokenizer", "CharVocab", "Tokenizer"]

@@ -172,6 +172,28 @@ int bdh_launch_state_step_deferred(bdh_ctx *ctx, bdh_state_log *log, const float
                                    uint64_t *bitmask, int32_t *rows_touched);
 int bdh_launch_state_flush(bdh_ctx *ctx, bdh_state_log *log, void *rho);
 
+// shared_prefix.hip: T tokens of every sequence of a batch that continues shared prompts (bdh_shared_prefix_attention);
+// out_ln != nullptr: the readout is also written LayerNorm-ed (src/model/bdh.rs:359)
+struct SharedStepParams {
+  int G;
+  const int32_t *counts_host;
+  int B, h, T, N, d, rotary;
+  const float *x, *v, *freqs;
+  int64_t position;
+  const int32_t *positions_dev;
+  const float *slopes_host;  // resolved (never null for ALiBi)
+  const void *rho;
+  int rho_dtype, capacity;
+  const int32_t *lens_dev;
+  int longest;
+  float *keys, *values, *out, *out_ln;
+};
+int bdh_launch_shared_steps(bdh_ctx *ctx, const SharedStepParams &p);
+// what is checked of such a call's arguments (T = 0: a fork)
+int bdh_check_shared(bdh_ctx *ctx, int G, const int32_t *counts_host, int B, int h, int T, int Nq, int d, int rotary,
+                     const void *rho, int rho_dtype, int capacity, const int32_t *lens_dev, int longest, const float *keys,
+                     const float *values);
+
 struct ReluLowrankParams {
   int B, h_in, T, d, h, N;
   const float *in, *weight, *bias;

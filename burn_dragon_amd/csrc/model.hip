@@ -57,7 +57,7 @@ struct StateRefs {
 
 int model_forward_impl(bdh_model *m, const int64_t *tokens, int B, int T, StateRefs st, int rho_dtype, int64_t position,
                        const int32_t *positions_dev, float *logits, int64_t *next_tokens, float *x_tap, float *viz,
-                       bdh_model_logs *logs);
+                       bdh_model_logs *logs, const SharedStepParams *shared = nullptr);
 
 }  // namespace
 
@@ -203,7 +203,7 @@ namespace {
 
 int model_forward_impl(bdh_model *m, const int64_t *tokens, int B, int T, StateRefs st, int rho_dtype, int64_t position,
                        const int32_t *positions_dev, float *logits, int64_t *next_tokens, float *x_tap, float *viz,
-                       bdh_model_logs *logs) {
+                       bdh_model_logs *logs, const SharedStepParams *shared) {
   bdh_ctx *ctx = m->ctx;
   const bool has_stamps = st.stamps_base || st.stamps_layers;
   if (has_stamps && m->cfg.rotary != BDH_ALIBI)
@@ -218,7 +218,7 @@ int model_forward_impl(bdh_model *m, const int64_t *tokens, int B, int T, StateR
   const int d = c.n_embd, h = c.n_head, N = c.latent, V = c.vocab, L = c.n_layer;
   const size_t Nq = c.rotary == BDH_POPE ? 2 * (size_t)N : (size_t)N;
   const size_t M = (size_t)B * T;
-  st.layer_bytes = (size_t)B * h * Nq * d * (rho_dtype == BDH_BF16 ? 2 : 4);
+  st.layer_bytes = (size_t)(shared ? shared->G : B) * h * Nq * d * (rho_dtype == BDH_BF16 ? 2 : 4);
   st.stamps_layer = (size_t)B * h * N;
   // what passes between two visits of a layer's state: every layer's state and the weights, which all layers share
   const size_t walked = st.layer_bytes * L + sizeof(float) * 3 * (size_t)h * N * d;
@@ -237,7 +237,7 @@ int model_forward_impl(bdh_model *m, const int64_t *tokens, int B, int T, StateR
   // us per step, half the neurons firing, one launch | two per layer | kernel by kernel: W = 3 MiB 76|41|103 at B=1, 80|56|121
   // at B=42, 87|81|137 at B=127; 6.75 MiB 129|55|130 at B=1, 143|116|195 at B=64; 12 MiB 211|47|100 at B=1, 232|149|175 at
   // B=64; 96 MiB -|114|308 at B=1, -|309|470 at B=16, -|576|607 at B=32.
-  if (T == 1 && !x_tap && !viz && !logs && contiguous && ctx->opt_model_one_launch != 0) {
+  if (T == 1 && !x_tap && !viz && !logs && !shared && contiguous && ctx->opt_model_one_launch != 0) {
     const int one_from = bdh_model_one_launch_from(c);
     const bool small = has_phase_act(c);
     const bool forced = ctx->opt_model_one_launch == 2 && one_from > 0;
@@ -270,7 +270,7 @@ int model_forward_impl(bdh_model *m, const int64_t *tokens, int B, int T, StateR
   // partials per head (N/128 rows of d floats) and 128 KiB of encoder partials (h*N/KB rows); beyond that the redundant
   // sums cost more than the two launches they replace (measured at d=512, h=8, N=16384: 2.97 against 2.87 ms per token).
   const int fused_kb = ctx->opt_model_fused_kb;
-  if (B == 1 && T == 1 && !x_tap && !viz && !logs && ctx->opt_model_fused_rows != 0 && c.rotary == BDH_ROPE &&
+  if (B == 1 && T == 1 && !x_tap && !viz && !logs && !shared && ctx->opt_model_fused_rows != 0 && c.rotary == BDH_ROPE &&
       (d == 256 || d == 512) && N >= 2 && (N % 2) == 0 && (long)N * d <= (2L << 20) &&
       (long)h * N * d <= (long)fused_kb * (1L << 15)) {
     const int KB = fused_kb;
@@ -332,7 +332,17 @@ int model_forward_impl(bdh_model *m, const int64_t *tokens, int B, int T, StateR
     rc = bdh_launch_relu_lowrank(ctx, px);
     if (rc != BDH_OK) return rc;
     // :353-359  recurrent attention (value = cur) and LayerNorm of its output
-    if (logs) {  // the update of :298 goes to the layer's log, the state is only read
+    if (shared) {  // the prompt's state is only read, the tokens go to the sequences' own keys and values
+      SharedStepParams ps = *shared;
+      ps.x = x_l;
+      ps.v = cur;
+      ps.rho = st.rho(l);
+      ps.keys = shared->keys + (size_t)l * B * h * Nq * shared->capacity;
+      ps.values = shared->values + (size_t)l * B * shared->capacity * d;
+      ps.out = attn;
+      ps.out_ln = attn_ln;
+      rc = bdh_launch_shared_steps(ctx, ps);
+    } else if (logs) {  // the update of :298 goes to the layer's log, the state is only read
       rc = bdh_launch_state_step_deferred(ctx, logs->layer[l], x_l, cur, m->freqs, position, positions_dev, st.rho(l), attn,
                                           attn_ln, nullptr, nullptr);
     } else {
@@ -476,6 +486,49 @@ int bdh_model_flush(bdh_model *m, bdh_model_logs *logs, void *rho) {
   const size_t layer_bytes = (size_t)logs->B * c.n_head * c.latent * c.n_embd * (logs->rho_dtype == BDH_BF16 ? 2 : 4);
   for (int l = 0; l < c.n_layer; ++l) {
     const int rc = bdh_state_flush(ctx, logs->layer[l], static_cast<char *>(rho) + (size_t)l * layer_bytes);
+    if (rc != BDH_OK) return rc;
+  }
+  return BDH_OK;
+}
+
+int bdh_model_forward_shared(bdh_model *m, int G, const int32_t *counts_host, const int64_t *tokens, int B, int T,
+                             const void *rho, int rho_dtype, int capacity, const int32_t *lens_dev, int longest,
+                             float *keys, float *values, int64_t position, const int32_t *positions_dev, float *logits,
+                             int64_t *next_tokens) {
+  if (!m) return BDH_E_INVAL;
+  bdh_ctx *ctx = m->ctx;
+  const bdh_model_config &c = m->cfg;
+  if (B < 0 || T < 0) return bdh_fail(ctx, BDH_E_INVAL, "negative batch or time");
+  if (B > 0 && T > 0) {
+    const int Nq = c.rotary == BDH_POPE ? 2 * c.latent : c.latent;
+    const int rc = bdh_check_shared(ctx, G, counts_host, B, c.n_head, T, Nq, c.n_embd, c.rotary, rho, rho_dtype, capacity, lens_dev,
+                                    longest, keys, values);
+    if (rc != BDH_OK) return rc;
+  }
+  SharedStepParams p{G, counts_host, B, c.n_head, T, c.latent, c.n_embd, c.rotary, nullptr, nullptr, m->freqs, position,
+                     positions_dev, m->slopes, nullptr, rho_dtype, capacity, lens_dev, longest, keys, values, nullptr, nullptr};
+  StateRefs st;
+  st.rho_base = const_cast<void *>(rho);
+  return model_forward_impl(m, tokens, B, T, st, rho_dtype, position, positions_dev, logits, next_tokens, nullptr, nullptr,
+                            nullptr, &p);
+}
+
+int bdh_model_fork_shared(bdh_model *m, int G, const int32_t *counts_host, int B, const void *rho, int rho_dtype,
+                          int capacity, const int32_t *lens_dev, int longest, const float *keys, const float *values,
+                          void *rho_out) {
+  if (!m) return BDH_E_INVAL;
+  bdh_ctx *ctx = m->ctx;
+  const bdh_model_config &c = m->cfg;
+  const int Nq = c.rotary == BDH_POPE ? 2 * c.latent : c.latent;
+  if (B > 0 && (!rho || !keys || !values || !rho_out)) return bdh_fail(ctx, BDH_E_INVAL, "null data pointer");
+  const size_t state = (size_t)c.n_head * Nq * c.n_embd * (rho_dtype == BDH_BF16 ? 2 : 4);
+  for (int l = 0; l < c.n_layer; ++l) {
+    const int rc = bdh_shared_prefix_fork(ctx, G, counts_host, B, c.n_head, Nq, c.n_embd, c.rotary,
+                                          c.rotary == BDH_ALIBI ? m->slopes : nullptr,
+                                          static_cast<const char *>(rho) + (size_t)l * G * state, rho_dtype, capacity, lens_dev,
+                                          longest, keys + (size_t)l * B * c.n_head * Nq * capacity,
+                                          values + (size_t)l * B * capacity * c.n_embd,
+                                          static_cast<char *>(rho_out) + (size_t)l * B * state);
     if (rc != BDH_OK) return rc;
   }
   return BDH_OK;

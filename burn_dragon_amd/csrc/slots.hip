@@ -1,0 +1,196 @@
+// Sequences of a batch moved between the slots of the buffers that hold them: forked, compacted, freed.
+#include <algorithm>
+
+#include "bdh_internal.h"
+
+namespace {
+
+constexpr int kMaxBuffers = BDH_MAX_SLOT_BUFFERS;
+constexpr int kInPlaceSlots = 1024;
+constexpr int kStageBytes = 64 * 1024;  // of LDS: two workgroups a CU
+
+struct SlotBuffer {
+  char *dst;
+  const char *src;
+  size_t slot_bytes, pieces;  // pieces of `unit` bytes in a slot
+  long first;                 // number of this buffer's first task
+  long chunks;                // tasks a layer
+  int outer, unit;
+  unsigned chunk;             // pieces a task takes of each slot
+};
+struct SlotArgs {
+  SlotBuffer buf[kMaxBuffers];
+  int n_buf, n, m;  // slots of the destination, of the source
+  long tasks;
+  const int32_t *origin;
+};
+
+__device__ __forceinline__ const SlotBuffer &buffer_of(const SlotArgs &g, long task) {
+  int i = 0;
+  while (i + 1 < g.n_buf && task >= g.buf[i + 1].first) ++i;
+  return g.buf[i];
+}
+
+// One chunk of every destination slot: a source is read once for a run of slots that take it.
+template <typename P>
+__device__ __forceinline__ void copy_chunk(const SlotArgs &g, const SlotBuffer &f, long o, size_t p0, size_t p1) {
+  const P *src = reinterpret_cast<const P *>(f.src) + (size_t)o * g.m * f.pieces;
+  P *dst = reinterpret_cast<P *>(f.dst) + (size_t)o * g.n * f.pieces;
+  for (size_t p = p0 + threadIdx.x; p < p1; p += 256) {
+    P v = P{};
+    int held = -1;  // zeros
+    for (int i = 0; i < g.n; ++i) {
+      const int from = g.origin[i];
+      if (from < -1 || from >= g.m) continue;  // left as it is
+      if (from != held) {
+        v = from < 0 ? P{} : src[(size_t)from * f.pieces + p];
+        held = from;
+      }
+      dst[(size_t)i * f.pieces + p] = v;
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void k_copy_slots(SlotArgs g) {
+  for (long task = blockIdx.x; task < g.tasks; task += gridDim.x) {
+    const SlotBuffer &f = buffer_of(g, task);
+    const long at = task - f.first, o = at / f.chunks;
+    const size_t p0 = (size_t)(at - o * f.chunks) * f.chunk, p1 = p0 + f.chunk < f.pieces ? p0 + f.chunk : f.pieces;
+    if (f.unit == 16) copy_chunk<uint4>(g, f, o, p0, p1);
+    else if (f.unit == 4) copy_chunk<uint32_t>(g, f, o, p0, p1);
+    else if (f.unit == 2) copy_chunk<uint16_t>(g, f, o, p0, p1);
+    else copy_chunk<uint8_t>(g, f, o, p0, p1);
+  }
+}
+
+// In place: a chunk of every source that moves goes to LDS before any slot is written, so a slot may be read and
+// overwritten in one call, in any cycle.
+template <typename P>
+__device__ __forceinline__ void move_chunk(const SlotBuffer &f, int n, long o, size_t p0, size_t p1, char *stage, const short *read,
+                                           int n_read, const short *write, const short *from, int n_write) {
+  P *base = reinterpret_cast<P *>(f.dst) + (size_t)o * n * f.pieces;
+  P *st = reinterpret_cast<P *>(stage);
+  const unsigned w = (unsigned)(p1 - p0);
+  for (unsigned e = threadIdx.x; e < n_read * w; e += 256) {
+    const unsigned k = e / w, p = e - k * w;
+    st[e] = base[(size_t)read[k] * f.pieces + p0 + p];
+  }
+  __syncthreads();
+  for (unsigned e = threadIdx.x; e < n_write * w; e += 256) {
+    const unsigned k = e / w, p = e - k * w;
+    const int s = from[k];
+    base[(size_t)write[k] * f.pieces + p0 + p] = s < 0 ? P{} : st[s * w + p];
+  }
+  __syncthreads();
+}
+
+__global__ __launch_bounds__(256) void k_move_slots(SlotArgs g) {
+  __shared__ __attribute__((aligned(16))) char s_stage[kStageBytes];
+  __shared__ short s_place[kInPlaceSlots];  // of a source among those that are read; -1: not read
+  __shared__ short s_read[kInPlaceSlots], s_write[kInPlaceSlots], s_from[kInPlaceSlots];
+  __shared__ int s_n[2];
+  for (int i = threadIdx.x; i < g.n; i += 256) s_place[i] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < g.n; i += 256) {
+    const int from = g.origin[i];
+    if (from >= 0 && from < g.n && from != i) s_place[from] = 1;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int r = 0, w = 0;
+    for (int i = 0; i < g.n; ++i) {
+      if (s_place[i]) {
+        s_read[r] = (short)i;
+        s_place[i] = (short)r++;
+      }
+    }
+    for (int i = 0; i < g.n; ++i) {
+      const int from = g.origin[i];
+      if (from < -1 || from >= g.n || from == i) continue;
+      s_write[w] = (short)i;
+      s_from[w++] = from < 0 ? (short)-1 : s_place[from];
+    }
+    s_n[0] = r;
+    s_n[1] = w;
+  }
+  __syncthreads();
+  if (s_n[1] == 0) return;
+  for (long task = blockIdx.x; task < g.tasks; task += gridDim.x) {
+    const SlotBuffer &f = buffer_of(g, task);
+    const long at = task - f.first, o = at / f.chunks;
+    const size_t p0 = (size_t)(at - o * f.chunks) * f.chunk, p1 = p0 + f.chunk < f.pieces ? p0 + f.chunk : f.pieces;
+    if (f.unit == 16) move_chunk<uint4>(f, g.n, o, p0, p1, s_stage, s_read, s_n[0], s_write, s_from, s_n[1]);
+    else if (f.unit == 4) move_chunk<uint32_t>(f, g.n, o, p0, p1, s_stage, s_read, s_n[0], s_write, s_from, s_n[1]);
+    else if (f.unit == 2) move_chunk<uint16_t>(f, g.n, o, p0, p1, s_stage, s_read, s_n[0], s_write, s_from, s_n[1]);
+    else move_chunk<uint8_t>(f, g.n, o, p0, p1, s_stage, s_read, s_n[0], s_write, s_from, s_n[1]);
+  }
+}
+
+}  // namespace
+
+extern "C" int bdh_copy_slots(bdh_ctx *ctx, const bdh_slot_buffer *buffers_host, int n_buffers, int dst_slots, int src_slots,
+                              const int32_t *origin_dev) {
+  if (!ctx) return BDH_E_INVAL;
+  if (n_buffers < 0 || n_buffers > kMaxBuffers || (n_buffers > 0 && !buffers_host))
+    return bdh_fail(ctx, BDH_E_INVAL, "%d buffers: 0 to %d are moved in one call", n_buffers, kMaxBuffers);
+  if (dst_slots < 0 || src_slots < 0) return bdh_fail(ctx, BDH_E_INVAL, "negative number of slots");
+  if (n_buffers == 0 || dst_slots == 0) return BDH_OK;
+  if (!origin_dev) return bdh_fail(ctx, BDH_E_INVAL, "null data pointer");
+  SlotArgs g{};
+  g.n = dst_slots;
+  g.m = src_slots;
+  g.origin = origin_dev;
+  int in_place = 0;
+  for (int i = 0; i < n_buffers; ++i) {
+    const bdh_slot_buffer &u = buffers_host[i];
+    if (u.outer < 0) return bdh_fail(ctx, BDH_E_INVAL, "buffer %d: negative outer size", i);
+    if (u.outer == 0 || u.slot_bytes == 0) continue;
+    if (!u.dst || (!u.src && src_slots > 0)) return bdh_fail(ctx, BDH_E_INVAL, "buffer %d: null data pointer", i);
+    const size_t dst_bytes = (size_t)u.outer * dst_slots * u.slot_bytes, src_bytes = (size_t)u.outer * src_slots * u.slot_bytes;
+    const char *d = static_cast<const char *>(u.dst), *s = static_cast<const char *>(u.src);
+    if (d == s) {
+      if (dst_slots != src_slots) return bdh_fail(ctx, BDH_E_INVAL, "buffer %d: in place with %d and %d slots", i, dst_slots, src_slots);
+      ++in_place;
+    } else if (d < s + src_bytes && s < d + dst_bytes) {
+      return bdh_fail(ctx, BDH_E_INVAL, "buffer %d: destination overlaps the source without being it", i);
+    }
+    for (int k = 0; k < g.n_buf; ++k) {
+      const SlotBuffer &o = g.buf[k];
+      const size_t ob = (size_t)o.outer * dst_slots * o.slot_bytes, os = (size_t)o.outer * src_slots * o.slot_bytes;
+      if ((d < o.dst + ob && o.dst < d + dst_bytes) || (s < o.dst + ob && o.dst < s + src_bytes) ||
+          (d < o.src + os && o.src < d + dst_bytes))
+        return bdh_fail(ctx, BDH_E_INVAL, "buffer %d: what one buffer writes is part of another", i);
+    }
+    SlotBuffer &f = g.buf[g.n_buf++];
+    f.dst = static_cast<char *>(u.dst);
+    f.src = s;
+    f.slot_bytes = u.slot_bytes;
+    f.outer = u.outer;
+    f.unit = 1;
+    for (int unit : {16, 4, 2})
+      if (f.unit == 1 && u.slot_bytes % unit == 0 && bdh_aligned(u.dst, unit) && bdh_aligned(u.src, unit)) f.unit = unit;
+    f.pieces = u.slot_bytes / f.unit;
+  }
+  if (in_place && in_place != g.n_buf) return bdh_fail(ctx, BDH_E_INVAL, "buffers in place and others in one call");
+  if (in_place && dst_slots > kInPlaceSlots)
+    return bdh_fail(ctx, BDH_E_SHAPE, "%d slots in place: at most %d", dst_slots, kInPlaceSlots);
+  if (g.n_buf == 0) return BDH_OK;
+  for (int i = 0; i < g.n_buf; ++i) {
+    SlotBuffer &f = g.buf[i];
+    // in place: a chunk of every slot fits the stage
+    const size_t most = in_place ? (size_t)kStageBytes / f.unit / dst_slots : 1024;
+    f.chunk = (unsigned)std::max<size_t>(1, std::min(f.pieces, most));
+    f.chunks = (long)((f.pieces + f.chunk - 1) / f.chunk);
+    f.first = g.tasks;
+    g.tasks += f.chunks * f.outer;
+  }
+  const unsigned grid = (unsigned)std::min<long>(g.tasks, in_place ? 2L * ctx->n_cu : 8L * ctx->n_cu);
+  if (in_place) {
+    hipLaunchKernelGGL(k_move_slots, dim3(grid), dim3(256), 0, ctx->stream, g);
+    BDH_LAUNCH_CHECK(ctx, "k_move_slots");
+  } else {
+    hipLaunchKernelGGL(k_copy_slots, dim3(grid), dim3(256), 0, ctx->stream, g);
+    BDH_LAUNCH_CHECK(ctx, "k_copy_slots");
+  }
+  return BDH_OK;
+}

@@ -27,7 +27,8 @@ EXPORTS = [
     "bdh_recurrent_attention", "bdh_state_step", "bdh_relu_lowrank", "bdh_layer_norm",
     "bdh_fused_state_aligned", "bdh_prefill_chunked", "bdh_prefill_chunked_ex", "bdh_model_create", "bdh_model_destroy",
     "bdh_model_state_bytes", "bdh_model_forward", "bdh_model_forward_ex", "bdh_advance_positions",
-    "bdh_sample_top_k", "bdh_recurrent_attention_lazy_alibi", "bdh_alibi_materialize", "bdh_model_forward_lazy",
+    "bdh_sample_top_k", "bdh_shared_prefix_attention", "bdh_shared_prefix_fork", "bdh_model_forward_shared",
+    "bdh_model_fork_shared", "bdh_copy_slots", "bdh_logit_rules", "bdh_count_tokens", "bdh_recurrent_attention_lazy_alibi", "bdh_alibi_materialize", "bdh_model_forward_lazy",
     "bdh_rho_energy", "bdh_model_forward_viz", "bdh_rotate",
     "bdh_model_forward_fast", "bdh_model_forward_fast_ex", "bdh_state_step_noalloc", "bdh_probe_chunks",
     "bdh_state_log_create", "bdh_state_log_destroy", "bdh_state_log_pending", "bdh_state_log_bytes",
@@ -55,6 +56,13 @@ class ModelWeightsC(ctypes.Structure):
     _fields_ = [("embed", c_void_p), ("encoder", c_void_p), ("encoder_v", c_void_p), ("decoder", c_void_p),
                 ("lm_head", c_void_p)]
 
+
+
+class SlotBufferC(ctypes.Structure):
+    _fields_ = [("dst", c_void_p), ("src", c_void_p), ("slot_bytes", c_size_t), ("outer", c_int32)]
+
+
+MAX_SHARED_PROMPTS, MAX_SLOT_BUFFERS = 256, 8
 
 _lib = None
 
@@ -123,6 +131,15 @@ def load_library(path: Optional[str] = None) -> ctypes.CDLL:
     lib.bdh_model_forward_ex.argtypes = [P, P, c_int, c_int, P, c_int, c_int64, P, P, P, P]
     lib.bdh_advance_positions.argtypes = [P, P, c_int, c_int]
     lib.bdh_sample_top_k.argtypes = [P, c_int, c_int, P, c_int64, c_float, c_int, P, P]
+    lib.bdh_shared_prefix_attention.argtypes = [P, c_int, P, c_int, c_int, c_int, c_int, c_int, c_int, P, P, P, c_int64, P,
+                                                P, P, c_int, c_int, P, c_int, P, P, P]
+    lib.bdh_shared_prefix_fork.argtypes = [P, c_int, P, c_int, c_int, c_int, c_int, c_int, P, P, c_int, c_int, P, c_int, P,
+                                           P, P]
+    lib.bdh_model_forward_shared.argtypes = [P, c_int, P, P, c_int, c_int, P, c_int, c_int, P, c_int, P, P, c_int64, P, P, P]
+    lib.bdh_model_fork_shared.argtypes = [P, c_int, P, c_int, P, c_int, c_int, P, c_int, P, P, P]
+    lib.bdh_copy_slots.argtypes = [P, POINTER(SlotBufferC), c_int, c_int, c_int, P]
+    lib.bdh_logit_rules.argtypes = [P, c_int, c_int, P, c_int64, P, P, P, P, P, P, c_int64, P, c_int64, P, c_int64]
+    lib.bdh_count_tokens.argtypes = [P, c_int, c_int, c_int, P, c_int64, P, c_int, P]
     lib.bdh_recurrent_attention_lazy_alibi.argtypes = [P, c_int, c_int, c_int, c_int, c_int, P, P, c_int64, P, P, P,
                                                        c_int, P, P, P, P]
     lib.bdh_alibi_materialize.argtypes = [P, c_int, c_int, c_int, c_int, c_int64, P, P, P, c_int, P]

@@ -15,6 +15,7 @@ import torch
 
 from .model.bdh import BDH
 from .model.state import ModelState
+from .rules import LogitRules, apply_rules, count_tokens, token_counts
 from .tokenizer import Tokenizer
 
 
@@ -167,6 +168,72 @@ def generate_tokens(model: BDH, prompt_tokens: List[int], settings: GenerationSe
     if produced:
         full.extend(int(t) for t in torch.cat(produced).cpu())
     return full
+
+
+def generate_samples(model: BDH, prompt_tokens: List[int], n: int, settings: GenerationSettings,
+                     rules: Optional[LogitRules] = None, stop_token: Optional[int] = None, capacity: int = 64,
+                     generator: Optional[torch.Generator] = None) -> List[List[int]]:
+    """n continuations of one prompt, drawn together: the prompt is read once, its state is shared by all of them for the
+    first `capacity` tokens of their own (BDH.share_state) and copied for each only then.  `rules` apply to the logits of
+    every draw; a sequence ends with stop_token, which is part of it, or after settings.max_new_tokens, and the ended ones
+    leave the batch every few tokens.  Each sequence has its own variates: where others end does not change them.
+    Returns the new tokens of each (the reference generates one sequence at a time, src/generation.rs:158-203)."""
+    if settings.max_new_tokens is None or settings.max_new_tokens < 0:
+        raise ValueError("max_new_tokens says how long the samples may become")
+    if n < 1:
+        raise ValueError("at least one sample")
+    if settings.max_new_tokens == 0:
+        return [[] for _ in range(n)]
+    dev, V = model.device, model.vocab_size
+    state, last = prefill_state(model, prompt_tokens)
+    shared, own = model.share_state(state, [n], min(capacity, settings.max_new_tokens)), None
+    logits = last.reshape(1, V).repeat(n, 1)
+    seen = None
+    if rules is not None:
+        rules = rules.to(dev, n)
+        if rules.penalises:
+            seen = token_counts(n, V, dev)
+            said = torch.as_tensor(prompt_tokens, dtype=torch.int64).reshape(1, -1).to(dev).repeat(n, 1)
+            count_tokens(said, seen, prompt=True, ctx=model.ctx)
+    alive = list(range(n))  # the samples that the rows of the batch are
+    alive_dev = torch.arange(n, device=dev)
+    produced = []  # (rows, tokens) of every draw
+    newest, every = None, 16
+    for step in range(settings.max_new_tokens):
+        if rules is not None:
+            logits = apply_rules(logits, rules, seen, newest if seen is not None else None, ctx=model.ctx)
+        if step % every == 0:
+            variates = uniform_variates(every * n, dev, generator).reshape(every, n)
+        newest = sample_from_logits(model, logits, settings.temperature, settings.top_k,
+                                    variates[step % every].index_select(0, alive_dev))
+        produced.append((alive, newest))
+        if step + 1 == settings.max_new_tokens:
+            break
+        if stop_token is not None and step % every == every - 1:
+            recent = torch.stack([t for _, t in produced[-every:]])
+            live = [i for i, ended in enumerate((recent == stop_token).any(0).tolist()) if not ended]
+            if not live:
+                break
+            if len(live) < len(alive):
+                if own is None:
+                    shared = model.select_shared(shared, live)
+                else:
+                    own = model.select_sequences(own, live)
+                index = torch.tensor(live, device=dev)
+                newest, alive_dev = newest.index_select(0, index), alive_dev.index_select(0, index)
+                seen = None if seen is None else seen.index_select(0, index)
+                rules = None if rules is None else rules.select(index)
+                alive = [alive[i] for i in live]
+        if own is None and shared.room == 0:
+            own, shared = model.fork_shared(shared), None
+        tokens = newest.reshape(-1, 1)
+        logits = (model.forward_shared(tokens, shared) if own is None else model.forward_with_state(tokens, own))[:, -1]
+    out: List[List[int]] = [[] for _ in range(n)]
+    for rows, tokens in produced:
+        for i, t in zip(rows, tokens.tolist()):
+            if not out[i] or out[i][-1] != stop_token:
+                out[i].append(t)
+    return out
 
 
 def generate_text(model: BDH, tokenizer: Tokenizer, block_size: int, generation: GenerationConfig,

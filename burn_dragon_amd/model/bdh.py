@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import sys
-from typing import Optional
+from typing import Optional, Sequence
 
 import numpy as np
 import torch
@@ -16,7 +16,7 @@ import torch
 from .. import ffi
 from ..positional import RotaryEmbedding
 from .config import BDHConfig
-from .state import LayerState, LayerVizState, ModelState
+from .state import LayerState, LayerVizState, ModelState, SharedState
 
 UINT63_MAX = (1 << 63) - 1
 
@@ -169,6 +169,116 @@ class BDH:
                 layer.viz = LayerVizState(x_last=m[0], y_last=m[1], xy_last=m[2], rho_last=m[3])
         state.position = min(state.position + T, UINT63_MAX)  # saturating_add, :445
         return (logits, nxt) if want_next else logits
+
+    def share_state(self, state: ModelState, counts: Sequence[int], capacity: int = 64) -> SharedState:
+        """Many sequences for the prompts that `state` holds: counts[g] of them continue sequence g of it, up to `capacity`
+        tokens each (rounded up to a multiple of 4), with the prompts' states read once for all.  The state is taken
+        over: `state` is a fresh one afterwards."""
+        if state.storage is None or state.position == 0:
+            raise ValueError("run the prompts before sharing their state")
+        counts = [int(c) for c in counts]
+        L, G = state.storage.shape[:2]
+        if len(counts) != G or min(counts) < 0 or sum(counts) == 0:
+            raise ValueError(f"counts {counts} do not deal sequences to {G} prompts")
+        if capacity < 1:
+            raise ValueError("capacity must be positive")
+        self.materialize_state(state)
+        B, S = sum(counts), (capacity + 3) // 4 * 4
+        keys = torch.zeros((L, B, self.n_head, self.latent_q, S), device=self.device, dtype=torch.float32)
+        values = torch.zeros((L, B, S, self.n_embd), device=self.device, dtype=torch.float32)
+        lens = torch.zeros((B,), device=self.device, dtype=torch.int32)
+        positions = torch.full((B,), min(state.position, 0x7FFFFFFF), device=self.device, dtype=torch.int32)
+        shared = SharedState(state.storage, counts, keys, values, lens, positions, state.position)
+        state.reset()
+        return shared
+
+    def forward_shared(self, tokens: torch.Tensor, shared: SharedState, want_next: bool = False):
+        """forward_with_state for sequences that share their prompts' states: tokens [B,T] int64 -> logits [B,T,V] (and the
+        greedy next tokens, kept on the device, when want_next)."""
+        tokens = tokens.to(self.device, torch.int64).contiguous()
+        B, T = tokens.shape
+        if B != shared.batch:
+            raise ValueError(f"{B} rows of tokens for {shared.batch} sequences")
+        if T > shared.room:
+            raise ValueError(f"{T} tokens, room for {shared.room}: fork_shared gives the sequences states of their own")
+        L, G = shared.rho.shape[:2]
+        expected = (self.n_layer, B, self.n_head, self.latent_q, shared.capacity)
+        if tuple(shared.keys.shape) != expected or tuple(shared.rho.shape[2:]) != (self.n_head, self.latent_q, self.n_embd):
+            raise ValueError("the shared state belongs to another model")
+        counts = np.ascontiguousarray(shared.counts, np.int32)
+        logits = torch.empty((B, T, self.vocab_size), device=self.device, dtype=torch.float32)
+        nxt = torch.empty((B,), device=self.device, dtype=torch.int64) if want_next else None
+        lib = self.ctx.lib
+        self.ctx.check(lib.bdh_model_forward_shared(
+            self.handle, G, counts.ctypes.data, tokens.data_ptr(), B, T, shared.rho.data_ptr(), self.rho_dtype, shared.capacity,
+            shared.lens.data_ptr(), shared.length, shared.keys.data_ptr(), shared.values.data_ptr(), 0,
+            shared.positions.data_ptr(), logits.data_ptr(), ffi.ptr(nxt)))
+        self.ctx.check(lib.bdh_advance_positions(self.ctx.handle, shared.lens.data_ptr(), B, T))
+        self.ctx.check(lib.bdh_advance_positions(self.ctx.handle, shared.positions.data_ptr(), B, T))
+        shared.length += T
+        return (logits, nxt) if want_next else logits
+
+    def fork_shared(self, shared: SharedState) -> ModelState:
+        """States of their own for the sequences of a shared state: what forward_with_state would have left after the same
+        tokens.  The shared state is left as it is."""
+        L, G = shared.rho.shape[:2]
+        B = shared.batch
+        counts = np.ascontiguousarray(shared.counts, np.int32)
+        state = self.init_state()
+        state.storage = torch.empty((L, B, self.n_head, self.latent_q, self.n_embd), device=self.device, dtype=shared.rho.dtype)
+        self.ctx.check(self.ctx.lib.bdh_model_fork_shared(
+            self.handle, G, counts.ctypes.data, B, shared.rho.data_ptr(), self.rho_dtype, shared.capacity, shared.lens.data_ptr(),
+            shared.length, shared.keys.data_ptr(), shared.values.data_ptr(), state.storage.data_ptr()))
+        for i, layer in enumerate(state.layers):
+            layer.rho = state.storage[i]
+        state.position = shared.position
+        return state
+
+    def select_shared(self, shared: SharedState, origin: Sequence[int]) -> SharedState:
+        """The sequences `origin` of a shared state, in that order, as a state of as many sequences (compaction where some
+        are left out, a fork where one is named twice).  Sequences of one prompt stay together."""
+        from ..slots import copy_slots
+
+        owner = [g for g, n in enumerate(shared.counts) for _ in range(n)]
+        origin = [int(o) for o in origin]
+        if not origin or min(origin) < 0 or max(origin) >= len(owner):
+            raise ValueError(f"origin {origin} names sequences outside the {len(owner)}")
+        owners = [owner[o] for o in origin]
+        if owners != sorted(owners):
+            raise ValueError("the sequences of a prompt stay together, in the order of the prompts")
+        B = len(origin)
+        keys = torch.empty((shared.keys.shape[0], B, *shared.keys.shape[2:]), device=self.device, dtype=torch.float32)
+        values = torch.empty((shared.values.shape[0], B, *shared.values.shape[2:]), device=self.device, dtype=torch.float32)
+        lens, positions = shared.lens.new_empty((B,)), shared.positions.new_empty((B,))
+        copy_slots([(keys, shared.keys, 1), (values, shared.values, 1), (lens, shared.lens, 0), (positions, shared.positions, 0)],
+                   origin, self.ctx)
+        return SharedState(shared.rho, [owners.count(g) for g in range(len(shared.counts))], keys, values, lens, positions,
+                           shared.start, shared.length)
+
+    def select_sequences(self, state: ModelState, origin: Sequence[int]) -> ModelState:
+        """The sequences `origin` of a state, in that order; slots.FREE (-1) for a fresh one.  As many as the state has are
+        moved in place (and `state` is returned), another number gets a state of its own."""
+        from ..slots import copy_slots
+
+        if state.storage is None:
+            raise ValueError("the state holds no sequences")
+        self.flush_state(state)
+        n = len(origin)
+        B = state.storage.shape[1]
+        if n == 0 or any(not -1 <= int(o) < B for o in origin):
+            raise ValueError(f"origin {list(origin)} names sequences outside the {B}")
+        buffers = [state.storage] + ([state.stamps] if state.stamps is not None else [])
+        if n == B:
+            copy_slots([(t, t, 1) for t in buffers], origin, self.ctx)
+            return state
+        moved = [torch.empty((t.shape[0], n, *t.shape[2:]), device=self.device, dtype=t.dtype) for t in buffers]
+        copy_slots([(m, t, 1) for m, t in zip(moved, buffers)], origin, self.ctx)
+        new = self.init_state()
+        new.storage, new.position = moved[0], state.position
+        new.stamps = moved[1] if state.stamps is not None else None
+        for i, layer in enumerate(new.layers):
+            layer.rho = new.storage[i]
+        return new
 
     def capture_decode_step(self, state: ModelState, tokens: torch.Tensor) -> "DecodeGraph":
         """Captures ONE greedy decode step (forward_with_state on the last sampled token, argmax kept on

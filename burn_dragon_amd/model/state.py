@@ -30,6 +30,37 @@ class LayerState:
 
 
 @dataclass
+class SharedState:
+    """Sequences that continue the prompts of one ModelState (BDH.share_state): the prompts' states, which every sequence
+    reads and none writes, and beside them what each sequence has said."""
+
+    rho: torch.Tensor  # [L,G,h,Nq,d]
+    counts: List[int]  # sequences of each prompt, in order
+    keys: torch.Tensor  # [L,B,h,Nq,capacity]
+    values: torch.Tensor  # [L,B,capacity,d]
+    lens: torch.Tensor  # int32 [B], on the device
+    positions: torch.Tensor  # int32 [B], on the device
+    start: int  # tokens of the prompts
+    length: int = 0  # tokens every sequence has said
+
+    @property
+    def capacity(self) -> int:
+        return self.keys.shape[-1]
+
+    @property
+    def batch(self) -> int:
+        return self.keys.shape[1]
+
+    @property
+    def room(self) -> int:
+        return self.capacity - self.length
+
+    @property
+    def position(self) -> int:
+        return self.start + self.length
+
+
+@dataclass
 class ModelState:
     layers: List[LayerState] = field(default_factory=list)
     position: int = 0

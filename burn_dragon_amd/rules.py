@@ -1,0 +1,128 @@
+"""What a step's logits go through before a token is drawn from them (bdh_logit_rules, bdh_count_tokens): penalties for
+tokens that occurred, biases, and a mask of the tokens that a grammar allows.  The reference's sampler has a temperature
+and a top_k only (src/generation.rs:26-72)."""
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Optional, Union
+
+import torch
+
+from . import ffi
+
+Penalty = Union[None, float, torch.Tensor]
+
+
+@dataclass
+class LogitRules:
+    """repetition, presence, frequency: a float for all sequences or an f32 tensor [B]; bias: f32 [V] or [B,V]; allowed:
+    the words of pack_allowed, int32 [W] or [B,W].  None: no such rule."""
+
+    repetition: Penalty = None
+    presence: Penalty = None
+    frequency: Penalty = None
+    bias: Optional[torch.Tensor] = None
+    allowed: Optional[torch.Tensor] = None
+
+    @property
+    def penalises(self) -> bool:
+        return any(p is not None for p in (self.repetition, self.presence, self.frequency))
+
+    def to(self, device, batch: int) -> "LogitRules":
+        """The rules with their penalties as tensors on `device`: a loop makes them once."""
+
+        def row(p):
+            if p is None or torch.is_tensor(p):
+                return p
+            return torch.full((batch,), float(p), device=device, dtype=torch.float32)
+
+        return LogitRules(row(self.repetition), row(self.presence), row(self.frequency), self.bias, self.allowed)
+
+    def select(self, index: torch.Tensor) -> "LogitRules":
+        """The rules of the sequences `index` of the batch (rows that all share stay as they are)."""
+
+        def pick(t, per_row):
+            return t.index_select(0, index) if torch.is_tensor(t) and t.dim() == per_row else t
+
+        return LogitRules(pick(self.repetition, 1), pick(self.presence, 1), pick(self.frequency, 1), pick(self.bias, 2),
+                          pick(self.allowed, 2))
+
+
+def token_counts(batch: int, vocab: int, device) -> torch.Tensor:
+    """Empty counts [B,V] int32: bit 31 marks a token of the prompt, the others count how often it was produced."""
+    return torch.zeros((batch, vocab), device=device, dtype=torch.int32)
+
+
+def pack_allowed(allowed: torch.Tensor) -> torch.Tensor:
+    """A mask [..., V] of truth values as int32 words [..., ceil(V / 32)]: token v is bit v % 32 of word v / 32."""
+    V = allowed.shape[-1]
+    padded = torch.zeros((*allowed.shape[:-1], (V + 31) // 32 * 32), device=allowed.device, dtype=torch.int64)
+    padded[..., :V] = allowed.to(torch.int64)
+    weights = torch.ones(32, dtype=torch.int64, device=allowed.device) << torch.arange(32, device=allowed.device)
+    words = (padded.reshape(*allowed.shape[:-1], -1, 32) * weights).sum(-1)
+    return torch.where(words >= 2**31, words - 2**32, words).to(torch.int32)
+
+
+def _seen(seen: torch.Tensor, B: int, V: int, dev) -> None:
+    if tuple(seen.shape) != (B, V) or seen.dtype != torch.int32 or not seen.is_contiguous() or seen.device != dev:
+        raise ValueError(f"seen: expected a contiguous int32 tensor [{B}, {V}] on {dev}, got {seen.dtype} {tuple(seen.shape)}")
+
+
+def count_tokens(tokens: torch.Tensor, seen: torch.Tensor, lens: Optional[torch.Tensor] = None, prompt: bool = False,
+                 ctx: Optional[ffi.Context] = None) -> None:
+    """tokens [B,T] int64 (of row b the first lens[b]; lens int32 [B] on the device) into seen [B,V]: marked as tokens of
+    the prompt, or counted as produced.  Ids outside the vocabulary are skipped."""
+    B, T = tokens.shape
+    dev, V = tokens.device, seen.shape[-1]
+    _seen(seen, B, V, dev)
+    if tokens.dtype != torch.int64 or (T > 1 and tokens.stride(1) != 1):
+        raise ValueError("tokens: expected int64 rows")
+    if lens is not None and (tuple(lens.shape) != (B,) or lens.dtype != torch.int32 or lens.device != dev or not lens.is_contiguous()):
+        raise ValueError(f"lens: expected int32 [{B}] on {dev}")
+    ctx = ctx or ffi.default_context(dev.index or 0)
+    ctx.check(ctx.lib.bdh_count_tokens(ctx.handle, B, T, V, ffi.ptr(tokens), tokens.stride(0) if B > 1 else max(T, 1),
+                                       ffi.ptr(lens), int(bool(prompt)), ffi.ptr(seen)))
+
+
+def apply_rules(logits: torch.Tensor, rules: LogitRules, seen: Optional[torch.Tensor] = None,
+                newest: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                ctx: Optional[ffi.Context] = None) -> torch.Tensor:
+    """logits [B,V] f32 (rows may be strided) under the rules -> out [B,V] (a new tensor, or `out`, which may be logits).
+    seen [B,V]: the counts (token_counts) that penalties read; newest [B] int64: the tokens drawn last, counted first."""
+    if logits.dim() != 2 or logits.dtype != torch.float32 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("logits: expected f32 rows [B,V]")
+    B, V = logits.shape
+    dev = logits.device
+    if seen is not None:
+        _seen(seen, B, V, dev)
+    elif rules.penalises or newest is not None:
+        raise ValueError("penalties need the counts of the tokens seen")
+    if newest is not None:
+        newest = newest.reshape(-1)
+        if newest.numel() != B or newest.dtype != torch.int64 or newest.device != dev:
+            raise ValueError(f"newest: expected int64 [{B}] on {dev}")
+        newest = newest.contiguous()
+    rules = rules.to(dev, B)
+    for name in ("repetition", "presence", "frequency"):
+        p = getattr(rules, name)
+        if p is not None and (tuple(p.shape) != (B,) or p.dtype != torch.float32 or p.device != dev or not p.is_contiguous()):
+            raise ValueError(f"{name}: expected f32 [{B}] on {dev}")
+    rows = []
+    for name, t, width, dtype in (("bias", rules.bias, V, torch.float32), ("allowed", rules.allowed, (V + 31) // 32, torch.int32)):
+        if t is None:
+            rows.append(0)
+            continue
+        if t.dtype != dtype or t.device != dev or t.shape[-1] != width or t.dim() not in (1, 2) or \
+                (t.dim() == 2 and t.shape[0] != B) or (width > 1 and t.stride(-1) != 1):
+            raise ValueError(f"{name}: expected {dtype} [{width}] or [{B}, {width}] on {dev}, got {t.dtype} {tuple(t.shape)}")
+        rows.append(t.stride(0) if t.dim() == 2 and B > 1 else 0)
+    if out is None:
+        out = torch.empty((B, V), device=dev, dtype=torch.float32)
+    elif tuple(out.shape) != (B, V) or out.dtype != torch.float32 or out.device != dev or (V > 1 and out.stride(1) != 1):
+        raise ValueError(f"out: expected f32 rows [{B}, {V}] on {dev}")
+    ctx = ctx or ffi.default_context(dev.index or 0)
+    ctx.check(ctx.lib.bdh_logit_rules(ctx.handle, B, V, ffi.ptr(logits), logits.stride(0) if B > 1 else V, ffi.ptr(seen),
+                                      ffi.ptr(newest), ffi.ptr(rules.repetition), ffi.ptr(rules.presence),
+                                      ffi.ptr(rules.frequency), ffi.ptr(rules.bias), rows[0], ffi.ptr(rules.allowed), rows[1],
+                                      ffi.ptr(out), out.stride(0) if B > 1 else V))
+    return out

@@ -1,0 +1,110 @@
+"""Sequences that continue shared prompts, through the C ABI (bdh_shared_prefix_attention, bdh_shared_prefix_fork): the
+state a prompt left is read once for all the sequences that continue it, and what a sequence says itself is kept beside
+it as keys and values.  The sums are those of BDH::recurrent_attention (src/model/bdh.rs:288-302), cut where the prompt
+ends; the reference gives every sequence a state of its own."""
+from __future__ import annotations
+
+from typing import Optional, Sequence
+
+import numpy as np
+import torch
+
+from . import ffi
+from .positional import RotaryEmbedding
+
+_DTYPES = {torch.float32: ffi.F32, torch.bfloat16: ffi.BF16}
+
+
+def _check(name: str, t: torch.Tensor, shape, dtype, device) -> None:
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{name}: expected a contiguous {dtype} tensor {tuple(shape)} on {device}, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
+
+
+def _prompts(counts: Optional[Sequence[int]], G: int, B: int):
+    if counts is None:
+        if G != 1:
+            raise ValueError(f"{G} prompts need the numbers of their sequences")
+        counts = [B]
+    if len(counts) != G or sum(counts) != B or min(counts, default=0) < 0:
+        raise ValueError(f"counts {list(counts)} do not deal {B} sequences to {G} prompts")
+    return np.ascontiguousarray(counts, np.int32)
+
+
+def _slopes(alibi_slopes, h: int):
+    if alibi_slopes is None:
+        return None
+    s = np.ascontiguousarray(alibi_slopes, np.float32)
+    if s.size != h:
+        raise ValueError(f"{s.size} slopes for {h} heads")
+    return s
+
+
+def shared_prefix_attention(query: torch.Tensor, value: torch.Tensor, rho: torch.Tensor, keys: torch.Tensor,
+                            values: torch.Tensor, lens: torch.Tensor, freqs: Optional[torch.Tensor], position: int = 0,
+                            positions: Optional[torch.Tensor] = None,
+                            rotary_embedding: RotaryEmbedding = RotaryEmbedding.ROPE, alibi_slopes=None,
+                            counts: Optional[Sequence[int]] = None, longest: Optional[int] = None,
+                            ctx: Optional[ffi.Context] = None) -> torch.Tensor:
+    """query [B,h,T,N] (un-rotated), value [B,T,d]; rho [G,h,Nq,d] (f32 or bf16, read only) the states of G prompts, of
+    which prompt g is continued by counts[g] sequences in order; keys [B,h,Nq,S] and values [B,S,d] what each sequence
+    has said (zeros from place lens[b] on, lens int32 [B] on the device).  Returns out [B,h,T,d] and stores the new
+    tokens' keys and values at places lens[b] and on; lens itself is advanced by the caller.  position / positions: as in
+    recurrent_attention, the prompt's tokens counted.  longest: an upper bound of lens (default S - T)."""
+    B, h, T, N = query.shape
+    dev = query.device
+    rot = RotaryEmbedding.parse(rotary_embedding)
+    Nq = 2 * N if rot == RotaryEmbedding.POPE else N
+    d, S, G = value.shape[-1], keys.shape[-1], rho.shape[0]
+    if rho.dtype not in _DTYPES:
+        raise ValueError(f"rho is f32 or bf16, not {rho.dtype}")
+    _check("query", query, (B, h, T, N), torch.float32, dev)
+    value = value.reshape(B, T, d)
+    _check("value", value, (B, T, d), torch.float32, dev)
+    _check("rho", rho, (G, h, Nq, d), rho.dtype, dev)
+    _check("keys", keys, (B, h, Nq, S), torch.float32, dev)
+    _check("values", values, (B, S, d), torch.float32, dev)
+    _check("lens", lens, (B,), torch.int32, dev)
+    if positions is not None:
+        _check("positions", positions, (B,), torch.int32, dev)
+    if rot != RotaryEmbedding.ALIBI:
+        freqs = freqs.reshape(-1)
+        _check("freqs", freqs, (N,), torch.float32, dev)
+    n_of = _prompts(counts, G, B)
+    slopes = _slopes(alibi_slopes, h)
+    ctx = ctx or ffi.default_context(dev.index or 0)
+    out = torch.empty((B, h, T, d), device=dev, dtype=torch.float32)
+    ctx.check(ctx.lib.bdh_shared_prefix_attention(
+        ctx.handle, G, n_of.ctypes.data, B, h, T, N, d, int(rot), ffi.ptr(query), ffi.ptr(value),
+        None if rot == RotaryEmbedding.ALIBI else ffi.ptr(freqs), int(position), ffi.ptr(positions), ffi.ptr(slopes),
+        ffi.ptr(rho), _DTYPES[rho.dtype], S, ffi.ptr(lens), -1 if longest is None else int(longest), ffi.ptr(keys),
+        ffi.ptr(values), ffi.ptr(out)))
+    return out
+
+
+def shared_prefix_fork(rho: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, lens: torch.Tensor,
+                       rotary_embedding: RotaryEmbedding = RotaryEmbedding.ROPE, alibi_slopes=None,
+                       counts: Optional[Sequence[int]] = None, longest: Optional[int] = None,
+                       out: Optional[torch.Tensor] = None, ctx: Optional[ffi.Context] = None) -> torch.Tensor:
+    """The states [B,h,Nq,d] (of rho's type) that the sequences of shared_prefix_attention would have had to themselves:
+    the prompt's state with the sequence's own tokens added, as after the same recurrent_attention calls."""
+    B, h, Nq, S = keys.shape
+    dev = keys.device
+    G, d = rho.shape[0], rho.shape[-1]
+    if rho.dtype not in _DTYPES:
+        raise ValueError(f"rho is f32 or bf16, not {rho.dtype}")
+    _check("rho", rho, (G, h, Nq, d), rho.dtype, dev)
+    _check("keys", keys, (B, h, Nq, S), torch.float32, dev)
+    _check("values", values, (B, S, d), torch.float32, dev)
+    _check("lens", lens, (B,), torch.int32, dev)
+    if out is None:
+        out = torch.empty((B, h, Nq, d), device=dev, dtype=rho.dtype)
+    _check("out", out, (B, h, Nq, d), rho.dtype, dev)
+    n_of = _prompts(counts, G, B)
+    slopes = _slopes(alibi_slopes, h)
+    ctx = ctx or ffi.default_context(dev.index or 0)
+    ctx.check(ctx.lib.bdh_shared_prefix_fork(
+        ctx.handle, G, n_of.ctypes.data, B, h, Nq, d, int(RotaryEmbedding.parse(rotary_embedding)), ffi.ptr(slopes),
+        ffi.ptr(rho), _DTYPES[rho.dtype], S, ffi.ptr(lens), -1 if longest is None else int(longest), ffi.ptr(keys),
+        ffi.ptr(values), ffi.ptr(out)))
+    return out

@@ -1,0 +1,48 @@
+"""Sequences of a batch moved between the slots of the buffers that hold them (bdh_copy_slots): forked, compacted,
+freed, reordered; all buffers of a batch in one launch."""
+from __future__ import annotations
+
+from typing import Iterable, Optional, Sequence, Tuple, Union
+
+import torch
+
+from . import ffi
+
+FREE, KEEP = -1, -2
+
+
+def copy_slots(buffers: Iterable[Tuple[torch.Tensor, torch.Tensor, int]], origin: Union[torch.Tensor, Sequence[int]],
+               ctx: Optional[ffi.Context] = None) -> None:
+    """buffers: (destination, source, slot dimension) of each, the two alike but for the number of slots; the same tensor
+    twice moves its slots in place (every slot is read as it was before the call).  origin[i], for every slot of the
+    destinations: the source's slot that it takes, FREE (zeros) or KEEP (left as it is).  A list is checked here; an
+    int32 tensor on the device is not, entries that name no slot leave theirs as it is."""
+    buffers = list(buffers)
+    if not buffers:
+        return
+    dev = buffers[0][0].device
+    n, m = buffers[0][0].shape[buffers[0][2]], buffers[0][1].shape[buffers[0][2]]
+    table = (ffi.SlotBufferC * len(buffers))()
+    for k, (dst, src, dim) in enumerate(buffers):
+        if dst.dtype != src.dtype or dst.dim() != src.dim() or not (dst.is_contiguous() and src.is_contiguous()):
+            raise ValueError(f"buffer {k}: destination and source are contiguous tensors of one type and rank")
+        if dst.device != dev or src.device != dev:
+            raise ValueError(f"buffer {k}: every buffer is on {dev}")
+        if dst.shape[dim] != n or src.shape[dim] != m:
+            raise ValueError(f"buffer {k}: {dst.shape[dim]} and {src.shape[dim]} slots, the first has {n} and {m}")
+        dim %= dst.dim()
+        if dst.shape[:dim] != src.shape[:dim] or dst.shape[dim + 1:] != src.shape[dim + 1:]:
+            raise ValueError(f"buffer {k}: slots of {tuple(dst.shape)} and {tuple(src.shape)} differ")
+        outer = int(torch.Size(dst.shape[:dim]).numel())
+        table[k] = ffi.SlotBufferC(dst.data_ptr(), src.data_ptr(),
+                                   torch.Size(dst.shape[dim + 1:]).numel() * dst.element_size(), outer)
+    if not torch.is_tensor(origin):
+        origin = [int(o) for o in origin]
+        bad = [o for o in origin if not KEEP <= o < m]
+        if bad:
+            raise ValueError(f"origin names slots {bad} of {m}")
+        origin = torch.tensor(origin, dtype=torch.int32, device=dev)
+    if tuple(origin.shape) != (n,) or origin.dtype != torch.int32 or origin.device != dev or not origin.is_contiguous():
+        raise ValueError(f"origin: expected int32 [{n}] on {dev}, got {origin.dtype} {tuple(origin.shape)} on {origin.device}")
+    ctx = ctx or ffi.default_context(dev.index or 0)
+    ctx.check(ctx.lib.bdh_copy_slots(ctx.handle, table, len(buffers), n, m, origin.data_ptr()))

@@ -557,6 +557,102 @@ int bdh_model_forward_deferred_layers(bdh_model *model, bdh_model_logs *logs, co
                                       const int32_t *positions_dev, float *logits, int64_t *next_tokens);
 int bdh_model_flush_layers(bdh_model *model, bdh_model_logs *logs, void *const *rho_layers_host);
 
+/* ---- many sequences that continue shared prompts ------------------------------------- */
+/*
+ * A prompt's state is read by all the sequences that continue it and written by none: G prompts with states rho
+ * [G,h,Nq,d], and B sequences of which the first counts_host[0] continue prompt 0, the next counts_host[1] prompt 1, ...
+ * (counts may be zero; counts_host may be NULL with one prompt).  What a sequence says itself is kept beside the state:
+ *   keys   [B,h,Nq,capacity] f32   the rotated activation n of its token s at [b,h,n,s]
+ *   values [B,capacity,d]    f32   the layer input of token s at [b,s,:]
+ *   lens_dev int32 [B]             tokens held; keys and values at and after that place hold zeros
+ * The reference has no such form: each sequence owns a state (src/model/state.rs:5-15).  The sums are those of
+ * src/model/bdh.rs:288-302, cut where the prompt ends:
+ *   q_t = rot(x_t),  k = lens[b] + t,
+ *   out_t = a^k q_t rho[g] + sum_{s < k} a^(k-s) (q_t . k_s) v_s   with a = exp(-slope_h) for BDH_ALIBI, else 1
+ * (f32 reassociation; the powers of a as exp(k * log(a_f32)) like a lazily decayed state).
+ *
+ * bdh_shared_prefix_attention: T tokens of every sequence; keys and values of the T tokens are stored at places lens[b] ..
+ *   lens[b] + T - 1, and lens_dev is left as it is: after the last layer of a step the caller advances it and the
+ *   positions with bdh_advance_positions.  x [B,h,T,N], v [B,T,d], freqs, position, positions_dev, alibi_slopes_host,
+ *   out [B,h,T,d] as in bdh_recurrent_attention; rho f32 or bf16 (eagerly decayed: bdh_alibi_materialize first).
+ *   T = 1 stores a key only where it is not zero.
+ *   longest: an upper bound of lens_dev that the host knows (keys past longest + T are not looked at by a call of many
+ *   tokens), or -1 for capacity - T.  A sequence whose len is negative, above longest or beyond capacity - T gets NaN
+ *   as its output, and nothing of it is stored.
+ * bdh_shared_prefix_fork: rho_out [B,h,Nq,d] = a^len rho[g] + sum_{s < len} a^(len-s) k_s (x) v_s, of rho's type, rounded
+ *   once: states of their own, as after the same tokens through bdh_recurrent_attention (f32 reassociation).  A len
+ *   outside 0 .. longest gives a state of NaN.  rho_out must not overlap rho.
+ *
+ * d a multiple of 4, at most 1024; capacity a multiple of 4; at most BDH_MAX_SHARED_PROMPTS prompts and B * h <= 65535 a call.
+ * Inputs are assumed finite.  Nothing is copied to or from the host, no result depends on the order of atomics.
+ */
+#define BDH_MAX_SHARED_PROMPTS 256
+int bdh_shared_prefix_attention(bdh_ctx *ctx, int G, const int32_t *counts_host, int B, int h, int T, int N, int d,
+                                int rotary, const float *x, const float *v, const float *freqs, int64_t position,
+                                const int32_t *positions_dev, const float *alibi_slopes_host, const void *rho,
+                                int rho_dtype, int capacity, const int32_t *lens_dev, int longest, float *keys,
+                                float *values, float *out);
+int bdh_shared_prefix_fork(bdh_ctx *ctx, int G, const int32_t *counts_host, int B, int h, int Nq, int d, int rotary,
+                           const float *alibi_slopes_host, const void *rho, int rho_dtype, int capacity,
+                           const int32_t *lens_dev, int longest, const float *keys, const float *values, void *rho_out);
+
+/*
+ * bdh_model_forward_ex for sequences that continue shared prompts: rho [L,G,h,Nq,d] (read only), keys
+ * [L,B,h,Nq,capacity], values [L,B,capacity,d], lens_dev, longest and counts_host as above.  position / positions_dev:
+ * place of the call's first token, the prompt's and the sequence's own tokens counted.  The caller advances lens_dev and
+ * positions_dev afterwards.
+ * bdh_model_fork_shared: the states rho_out [L,B,h,Nq,d] of the sequences, as bdh_model_forward* take them.
+ */
+int bdh_model_forward_shared(bdh_model *model, int G, const int32_t *counts_host, const int64_t *tokens, int B, int T,
+                             const void *rho, int rho_dtype, int capacity, const int32_t *lens_dev, int longest,
+                             float *keys, float *values, int64_t position, const int32_t *positions_dev, float *logits,
+                             int64_t *next_tokens);
+int bdh_model_fork_shared(bdh_model *model, int G, const int32_t *counts_host, int B, const void *rho, int rho_dtype,
+                          int capacity, const int32_t *lens_dev, int longest, const float *keys, const float *values,
+                          void *rho_out);
+
+/*
+ * Sequences moved between the slots of the buffers that hold them: forked, compacted, freed, reordered.  The buffers of a
+ * batch (states of all layers, decay stamps, keys, values, counts, positions) go in one call, one launch.  A buffer is
+ * src [outer, src_slots, slot_bytes] and dst [outer, dst_slots, slot_bytes]; for every slot i of dst
+ *   origin_dev[i] = s >= 0  dst[:, i] = src[:, s]
+ *                  -1       dst[:, i] = 0 (a fresh state, empty counts)
+ *                  else     (-2, or no slot of src) dst[:, i] is left as it is
+ * src may be dst (of every buffer of the call; src_slots = dst_slots <= 1024): all slots are then read as they were before
+ * the call, so origin may hold any permutation or fork.  Otherwise no destination may overlap a source.
+ */
+#define BDH_MAX_SLOT_BUFFERS 8
+typedef struct bdh_slot_buffer {
+  void *dst;
+  const void *src;
+  size_t slot_bytes;
+  int32_t outer;
+} bdh_slot_buffer;
+int bdh_copy_slots(bdh_ctx *ctx, const bdh_slot_buffer *buffers_host, int n_buffers, int dst_slots, int src_slots,
+                   const int32_t *origin_dev);
+
+/*
+ * What a step's logits go through before bdh_sample_top_k draws from them (the reference divides by a temperature and
+ * keeps the top_k, src/generation.rs:26-72, and has no such rules).  seen int32 [B,V]: bit 31 is set for a token of the
+ * prompt, bits 0..30 count how often the sequence produced it.  newest[b] (int64, optional; an id outside [0,V) counts as
+ * none) is counted first; then for every token
+ *   z = logits[b,v];  if seen: z = z > 0 ? z / repetition[b] : z * repetition[b]
+ *   z = z - (frequency[b] * times + (times > 0 ? presence[b] : 0)) + bias[b,v]
+ *   out[b,v] = z, or -inf where bit v % 32 of word v / 32 of allowed[b] is clear, whatever z is
+ * repetition, presence, frequency: device float [B] or NULL (1, 0, 0); they need seen.  bias and allowed: NULL, or rows
+ * bias_stride floats / allowed_stride words apart, 0 for one row that all sequences share.  logits: row b starts at
+ * logits + b*row_stride; out may be logits (same stride).  A row of which nothing is allowed is all -inf:
+ * bdh_sample_top_k draws from it uniformly, so a caller that may run out of allowed tokens ends such a sequence.
+ * bdh_count_tokens: seen[b, tokens[b,t]] for t < lens_dev[b] (NULL: T) is marked as the prompt's (prompt = 1) or counted
+ * once more (0); ids outside [0,V) are skipped; lens are taken into 0..T.
+ */
+int bdh_logit_rules(bdh_ctx *ctx, int B, int V, const float *logits, int64_t row_stride, int32_t *seen,
+                    const int64_t *newest, const float *repetition, const float *presence, const float *frequency,
+                    const float *bias, int64_t bias_stride, const int32_t *allowed, int64_t allowed_stride, float *out,
+                    int64_t out_stride);
+int bdh_count_tokens(bdh_ctx *ctx, int B, int T, int V, const int64_t *tokens, int64_t row_stride,
+                     const int32_t *lens_dev, int prompt, int32_t *seen);
+
 /* Draws the next token of every sequence on the device.  Replaces the temperature division of
  * sample_next_token (src/generation.rs:117) and sample_from_logits_values (src/generation.rs:26-72),
  * which copy the logits to the host for every token: values = logits / temperature; with

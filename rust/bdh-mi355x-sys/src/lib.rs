@@ -37,6 +37,15 @@ pub struct bdh_model_logs {
     _private: [u8; 0],
 }
 
+/// one buffer of `bdh_copy_slots`: [outer, slots, slot_bytes]
+#[repr(C)]
+pub struct bdh_slot_buffer {
+    pub dst: *mut c_void,
+    pub src: *const c_void,
+    pub slot_bytes: usize,
+    pub outer: i32,
+}
+
 pub const BDH_OK: c_int = 0;
 pub const BDH_E_INVAL: c_int = -1;
 pub const BDH_E_SHAPE: c_int = -2;
@@ -181,6 +190,27 @@ extern "C" {
         logits: *mut f32, next_tokens: *mut i64) -> c_int;
     pub fn bdh_model_flush_layers(model: *mut bdh_model, logs: *mut bdh_model_logs,
         rho_layers_host: *const *mut c_void) -> c_int;
+    pub fn bdh_shared_prefix_attention(ctx: *mut bdh_ctx, g: c_int, counts_host: *const i32, b: c_int, h: c_int,
+        t: c_int, n: c_int, d: c_int, rotary: c_int, x: *const f32, v: *const f32, freqs: *const f32, position: i64,
+        positions_dev: *const i32, alibi_slopes_host: *const f32, rho: *const c_void, rho_dtype: c_int, capacity: c_int,
+        lens_dev: *const i32, longest: c_int, keys: *mut f32, values: *mut f32, out: *mut f32) -> c_int;
+    pub fn bdh_shared_prefix_fork(ctx: *mut bdh_ctx, g: c_int, counts_host: *const i32, b: c_int, h: c_int, nq: c_int,
+        d: c_int, rotary: c_int, alibi_slopes_host: *const f32, rho: *const c_void, rho_dtype: c_int, capacity: c_int,
+        lens_dev: *const i32, longest: c_int, keys: *const f32, values: *const f32, rho_out: *mut c_void) -> c_int;
+    pub fn bdh_model_forward_shared(model: *mut bdh_model, g: c_int, counts_host: *const i32, tokens: *const i64,
+        b: c_int, t: c_int, rho: *const c_void, rho_dtype: c_int, capacity: c_int, lens_dev: *const i32, longest: c_int,
+        keys: *mut f32, values: *mut f32, position: i64, positions_dev: *const i32, logits: *mut f32,
+        next_tokens: *mut i64) -> c_int;
+    pub fn bdh_model_fork_shared(model: *mut bdh_model, g: c_int, counts_host: *const i32, b: c_int,
+        rho: *const c_void, rho_dtype: c_int, capacity: c_int, lens_dev: *const i32, longest: c_int, keys: *const f32,
+        values: *const f32, rho_out: *mut c_void) -> c_int;
+    pub fn bdh_copy_slots(ctx: *mut bdh_ctx, buffers_host: *const bdh_slot_buffer, n_buffers: c_int, dst_slots: c_int,
+        src_slots: c_int, origin_dev: *const i32) -> c_int;
+    pub fn bdh_logit_rules(ctx: *mut bdh_ctx, b: c_int, v: c_int, logits: *const f32, row_stride: i64, seen: *mut i32,
+        newest: *const i64, repetition: *const f32, presence: *const f32, frequency: *const f32, bias: *const f32,
+        bias_stride: i64, allowed: *const i32, allowed_stride: i64, out: *mut f32, out_stride: i64) -> c_int;
+    pub fn bdh_count_tokens(ctx: *mut bdh_ctx, b: c_int, t: c_int, v: c_int, tokens: *const i64, row_stride: i64,
+        lens_dev: *const i32, prompt: c_int, seen: *mut i32) -> c_int;
     pub fn bdh_sample_top_k(ctx: *mut bdh_ctx, b: c_int, v: c_int, logits: *const f32, row_stride: i64,
         temperature: f32, top_k: c_int, uniforms: *const f32, next_tokens: *mut i64) -> c_int;
     pub fn bdh_probe_chunks(ctx: *mut bdh_ctx, region: *mut c_void, region_bytes: usize,

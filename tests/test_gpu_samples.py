@@ -1,0 +1,141 @@
+"""Many sequences of one prompt through a whole model: forward_shared and fork_shared next to forward_with_state on states
+of their own, the sequences selected in between, and generate_samples, which runs all of it together.
+
+Tolerance of the logits: 1e-3 of their largest magnitude, the bound of every f32 form of the model step here (a neuron
+whose pre-activation is within rounding of the threshold may fire in one form and not in the other)."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+@pytest.fixture(scope="module")
+def bda():
+    if not torch.cuda.is_available():
+        pytest.fail("no HIP device: the GPU tests must run on the MI355X box")
+    import burn_dragon_amd
+
+    return burn_dragon_amd
+
+
+def _model(bda, rotary, dtype=0, d=128, mult=8, **more):
+    cfg = bda.BDHConfig(n_layer=3, n_embd=d, n_head=4, mlp_internal_dim_multiplier=mult, vocab_size=69)
+    cfg.fused_kernels.set_rotary_embedding(rotary)
+    return bda.BDH(cfg, DEV, seed=3, rho_dtype=dtype, **more)
+
+
+def _close(a, b, tol):
+    assert (a - b).abs().max().item() <= tol * b.abs().max().item()
+
+
+@pytest.mark.parametrize("rotary,lazy,dtype", [("rope", False, 0), ("alibi", False, 0), ("alibi", True, 0), ("pope", False, 0),
+                                               ("rope", False, 1)])
+def test_shared_sequences_equal_sequences_of_their_own(bda, rotary, lazy, dtype):
+    model = _model(bda, rotary, dtype, alibi_lazy=lazy)
+    tol = 1e-3 if dtype == 0 else 2e-2
+    rng = np.random.default_rng(1)
+    prompts = torch.from_numpy(rng.integers(0, 69, (2, 19)))
+    counts, owner = [3, 1], [0, 0, 0, 1]
+    state = model.init_state()
+    model.forward_with_state(prompts, state)
+    own = model.init_state()
+    model.forward_with_state(prompts[owner], own)
+    shared = model.share_state(state, counts, 14)
+    assert shared.capacity == 16 and state.storage is None and state.position == 0
+    for T in (5, 1, 1, 4, 1):
+        tokens = torch.from_numpy(rng.integers(0, 69, (4, T)))
+        logits, nxt = model.forward_shared(tokens, shared, want_next=True)
+        want = model.forward_with_state(tokens, own)
+        _close(logits, want, tol)
+        assert torch.equal(nxt, logits[:, -1].argmax(-1))
+    assert shared.position == own.position == 31 and shared.room == 4
+    with pytest.raises(ValueError):
+        model.forward_shared(torch.zeros((4, 5), dtype=torch.int64), shared)
+    forked = model.fork_shared(shared)
+    model.materialize_state(own)
+    _close(forked.storage.float(), own.storage.float(), tol)
+    tokens = torch.from_numpy(rng.integers(0, 69, (4, 3)))
+    _close(model.forward_with_state(tokens, forked), model.forward_with_state(tokens, own), tol)
+
+
+def test_selected_sequences_go_on_alike(bda):
+    model = _model(bda, "rope")
+    rng = np.random.default_rng(2)
+    state = model.init_state()
+    model.forward_with_state(torch.from_numpy(rng.integers(0, 69, (2, 8))), state)
+    shared = model.share_state(state, [3, 2], 8)
+    model.forward_shared(torch.from_numpy(rng.integers(0, 69, (5, 2))), shared)
+    picked = model.select_shared(shared, [2, 0, 0, 4])
+    assert picked.counts == [3, 1]
+    with pytest.raises(ValueError):
+        model.select_shared(shared, [3, 0])
+    own = model.fork_shared(shared)
+    few = model.select_sequences(own, [2, 0, 0, 4])
+    tokens = torch.from_numpy(rng.integers(0, 69, (4, 1)))
+    a, b = model.forward_shared(tokens, picked), model.forward_with_state(tokens, few)
+    _close(a, b, 1e-3)
+    before = own.storage.clone()
+    assert model.select_sequences(own, [4, 3, -1, 1, 0]) is own
+    assert torch.equal(own.storage[:, [0, 1, 3, 4]], before[:, [4, 3, 1, 0]]) and not own.storage[:, 2].any()
+
+
+@pytest.mark.parametrize("rotary", ["rope", "alibi"])
+def test_greedy_samples_equal_the_single_sequence(bda, rotary):
+    """Greedy tokens of every sample against generate_tokens; runs past the shared capacity and through the fork.  The two
+    may only part where the two largest logits are within rounding of each other, which the test looks up."""
+    from burn_dragon_amd.generation import GenerationSettings, generate_samples, generate_tokens
+
+    model = _model(bda, rotary, d=256, mult=4)
+    prompt = [int(t) for t in np.random.default_rng(4).integers(0, 69, 21)]
+    settings = GenerationSettings(max_new_tokens=30, top_k=1)
+    want = generate_tokens(model, prompt, settings)[21:]
+    got = generate_samples(model, prompt, 3, settings, capacity=12)
+    for sample in got:
+        assert len(sample) == 30
+        if sample != want:
+            i = next(i for i, (a, b) in enumerate(zip(sample, want)) if a != b)
+            logits = model.forward(torch.tensor([prompt + want[:i]]))[0, -1]
+            assert (logits[want[i]] - logits[sample[i]]).abs().item() <= 2e-3 * logits.abs().max().item()
+
+
+def test_samples_with_rules_and_a_stop_token(bda):
+    from burn_dragon_amd.generation import GenerationSettings, generate_samples
+    from burn_dragon_amd.rules import pack_allowed
+
+    model = _model(bda, "alibi", d=256, mult=4)
+    prompt = list(range(10))
+    allowed = torch.zeros(69, dtype=torch.bool)
+    allowed[20:60] = True
+    settings = GenerationSettings(max_new_tokens=50, temperature=1.0, top_k=None)
+
+    def run(n, stop):
+        rules = bda.LogitRules(repetition=1.3, presence=0.1, frequency=0.2, allowed=pack_allowed(allowed.to(DEV)))
+        return generate_samples(model, prompt, n, settings, rules, stop, capacity=24,
+                                generator=torch.Generator().manual_seed(5))
+
+    free = run(6, None)
+    assert all(len(s) == 50 and all(20 <= t < 60 for t in s) for s in free)
+    assert len({tuple(s) for s in free}) > 1
+    stop = free[0][9]  # a token that some samples draw
+    ended = run(6, stop)
+    for a, b in zip(ended, free):
+        cut = b[:b.index(stop) + 1] if stop in b else b
+        n = min(len(a), len(cut))
+        same = sum(x == y for x, y in zip(a, cut))
+        assert stop not in a[:-1] and same >= n - 0 if n <= 16 else a[:16] == cut[:16]  # alike until the batch changes
+    # never twice the same token under a frequency penalty that outweighs every logit
+    rules = bda.LogitRules(frequency=1e6)
+    for s in generate_samples(model, prompt, 4, GenerationSettings(max_new_tokens=40), rules, capacity=16):
+        assert len(set(s)) == 40
+
+
+def test_one_sample_one_token(bda):
+    from burn_dragon_amd.generation import GenerationSettings, generate_samples
+
+    model = _model(bda, "rope")
+    for n in (1, 2):
+        got = generate_samples(model, [3], n, GenerationSettings(max_new_tokens=1, top_k=1))
+        assert [len(s) for s in got] == [1] * n
+    assert generate_samples(model, [3], 2, GenerationSettings(max_new_tokens=0)) == [[], []]

@@ -1,0 +1,326 @@
+"""Attention of sequences that continue shared prompts (shared_prefix_attention), and the states of their own that they
+get (shared_prefix_fork), against the definition in 64 bits, against the sequences' own recurrent states, and under
+what serving does with them: calls in a row, graphs, other streams.
+
+Tolerances.  With u = 2^-24 (f32 rounds to nearest), every term q_n rho_nc and (q.k_s) v_sc of an output carries the
+roundings of its query and key (the angle and its sine: 8 steps, softplus 4 more; two factors: 24 in all), of its
+decay (8), of its products (3) and of the additions it passes through.  One token: at most 256 in a chain of a block of
+rows, `parts` and `blocks` <= Nq / 64 + 1 of them, 48 in a block's score, and len for the values.  Many tokens: every sum
+in some order of at most Nq, then span.  So |error| <= u * depth * (sum of the terms' magnitudes), depth as written in
+`_depth`; the magnitudes come from the same definition with absolute values."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import bdh_oracle as orc
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+U = 2.0**-24
+ROT = {"rope": orc.ROPE, "alibi": orc.ALIBI, "pope": orc.POPE}
+
+
+@pytest.fixture(scope="module")
+def gpu():
+    if not torch.cuda.is_available():
+        pytest.fail("no HIP device: the GPU tests must run on the MI355X box")
+    from burn_dragon_amd import ffi, recurrent, shared
+
+    return ffi, recurrent, shared
+
+
+def _turn(x, freqs, pos, rotary):
+    """x [...,N] at position pos, in 64 bits (the product of position and frequency is rounded to f32 by definition)."""
+    x = x.astype(np.float64)
+    if rotary == "alibi":
+        return x
+    raw = (np.float32(pos) * freqs).astype(np.float32)
+    ang = 2 * np.pi * (raw.astype(np.float64) - np.floor(raw.astype(np.float64)))
+    if rotary == "pope":
+        m = np.log(np.exp(x) + 1)
+        return np.concatenate([m * np.cos(ang), m * np.sin(ang)], -1)
+    y = np.empty_like(x)
+    y[..., 0::2] = x[..., 0::2] * np.cos(ang[0::2]) - x[..., 1::2] * np.sin(ang[0::2])
+    y[..., 1::2] = x[..., 1::2] * np.cos(ang[1::2]) + x[..., 0::2] * np.sin(ang[1::2])
+    return y
+
+
+class Case:
+    def __init__(self, seed, counts, h, N, d, S, lens, T, rotary, dtype, density=0.3):
+        rng = np.random.default_rng(seed)
+        self.counts, self.rotary, self.T, self.dtype = list(counts), rotary, T, dtype
+        self.B, self.h, self.N, self.d, self.S = sum(counts), h, N, d, S
+        self.Nq = 2 * N if rotary == "pope" else N
+        self.owner = [g for g, n in enumerate(counts) for _ in range(n)]
+        self.lens = np.array([lens[b % len(lens)] for b in range(self.B)], np.int32)
+        self.slopes = [2.0 ** (-(i + 1.0)) for i in range(h)] if rotary == "alibi" else None
+        self.rate = np.log(np.exp(-np.array(self.slopes, np.float32)).astype(np.float64)) if self.slopes else np.zeros(h)
+        from burn_dragon_amd.kernel.linear_attention import build_freqs
+
+        self.freqs = build_freqs(N, 65536.0, ROT[rotary]).numpy().reshape(-1)
+        self.start = rng.integers(0, 3000, len(counts))[self.owner]
+        rho = torch.from_numpy(rng.standard_normal((len(counts), h, self.Nq, d)).astype(np.float32)).to(dtype)
+        self.rho_t, self.rho = rho, rho.to(torch.float64).numpy()
+
+        def act(*shape):
+            return (np.maximum(rng.standard_normal(shape) * 2, 0) * (rng.random(shape) < density)).astype(np.float32)
+
+        self.past = act(self.B, h, max(1, int(self.lens.max(initial=0))), N)
+        self.x = act(self.B, h, T, N)
+        self.v = rng.standard_normal((self.B, T, d)).astype(np.float32)
+        self.keys = np.zeros((self.B, h, self.Nq, S), np.float32)
+        self.values = np.zeros((self.B, S, d), np.float32)
+        for b in range(self.B):
+            n = int(self.lens[b])
+            self.values[b, :n] = rng.standard_normal((n, d))
+            for s in range(n):
+                self.keys[b, :, :, s] = _turn(self.past[b, :, s], self.freqs, self.start[b] + s, rotary)
+
+    def device(self, dev=DEV):
+        t = {n: torch.from_numpy(getattr(self, n)).to(dev) for n in ("x", "v", "keys", "values", "lens", "freqs")}
+        t["rho"] = self.rho_t.to(dev)
+        t["positions"] = torch.from_numpy((self.start + self.lens).astype(np.int32)).to(dev)
+        return t
+
+    def call(self, shared, t, **more):
+        return shared.shared_prefix_attention(t["x"], t["v"], t["rho"], t["keys"], t["values"], t["lens"], t["freqs"],
+                                              positions=t["positions"], rotary_embedding=self.rotary,
+                                              alibi_slopes=self.slopes, counts=self.counts, **more)
+
+    def exact(self):
+        """out, its terms' magnitudes, keys, values"""
+        out = np.zeros((self.B, self.h, self.T, self.d))
+        mag = np.zeros_like(out)
+        keys, values = self.keys.astype(np.float64), self.values.astype(np.float64)
+        for b in range(self.B):
+            rho = self.rho[self.owner[b]]
+            for t in range(self.T):
+                k = int(self.lens[b]) + t
+                q = _turn(self.x[b, :, t], self.freqs, self.start[b] + k, self.rotary)
+                a = np.exp(self.rate * k)[:, None]
+                back = np.exp(self.rate[:, None] * (k - np.arange(k)))
+                out[b, :, t] = a * np.einsum("hn,hnd->hd", q, rho)
+                out[b, :, t] += (np.einsum("hn,hns->hs", q, keys[b, :, :, :k]) * back) @ values[b, :k]
+                mag[b, :, t] = a * np.einsum("hn,hnd->hd", np.abs(q), np.abs(rho))
+                mag[b, :, t] += (np.einsum("hn,hns->hs", np.abs(q), np.abs(keys[b, :, :, :k])) * back) @ np.abs(values[b, :k])
+                keys[b, :, :, k] = q
+                values[b, k] = self.v[b, t]
+        return out, mag, keys, values
+
+
+def _depth(c):
+    extra = 24 + 8 + 3
+    if c.T == 1:
+        return extra + 256 + 2 * (c.Nq // 64 + 5) + 48 + int(c.lens.max())
+    return extra + c.Nq + int(c.lens.max()) + c.T
+
+
+def _check_read(gpu, c):
+    _, _, shared = gpu
+    t = c.device()
+    out = c.call(shared, t, longest=int(c.lens.max()))
+    torch.cuda.synchronize()
+    ref, mag, keys, values = c.exact()
+    err = np.abs(out.double().cpu().numpy() - ref)
+    assert (err <= U * _depth(c) * mag + 1e-37).all(), (err / (mag + 1e-300)).max() / U
+    got = t["keys"].double().cpu().numpy()
+    new = np.zeros(keys.shape, bool)
+    for b in range(c.B):
+        new[b, :, :, c.lens[b]:c.lens[b] + c.T] = True
+    assert np.array_equal(got[~new], keys[~new])  # what was there stays, the room behind stays zero
+    big = np.abs(c.x).max() * 2 + 1
+    assert np.abs(got - keys)[new].max(initial=0) <= U * 12 * big
+    assert ((got != 0) <= (keys != 0))[new].all()
+    assert np.array_equal(t["values"].double().cpu().numpy(), values)
+    return out
+
+
+F32, BF16 = torch.float32, torch.bfloat16
+READ = [
+    # counts, h, N, d, S, lens, T, rotary, dtype
+    ((1,), 1, 2, 4, 4, (0,), 1, "rope", F32),
+    ((4,), 4, 256, 256, 32, (3, 21, 0, 31), 1, "alibi", F32),
+    ((3, 0, 2), 2, 70, 68, 8, (7, 0, 4), 1, "rope", F32),
+    ((2, 1), 3, 33, 12, 12, (5, 11), 1, "alibi", F32),
+    ((5,), 2, 31, 132, 16, (9, 15, 0), 1, "pope", F32),
+    ((17,), 1, 600, 64, 72, (64, 65, 70, 63), 1, "rope", F32),
+    ((16, 1), 2, 514, 128, 8, (2, 7), 1, "rope", BF16),
+    ((40,), 1, 130, 192, 4, (1, 3, 0), 1, "rope", F32),
+    ((70, 3), 1, 66, 260, 4, (2,), 1, "alibi", BF16),
+    ((2,), 1, 300, 1024, 8, (6, 1), 1, "pope", BF16),
+    ((2,), 1, 8, 8, 1100, (1060, 1099), 1, "rope", F32),
+    ((3,), 5, 1030, 320, 20, (13, 2, 19), 1, "rope", BF16),
+    ((1,), 1, 2, 4, 4, (0, 2), 2, "rope", F32),
+    ((4, 2), 2, 130, 68, 64, (0, 13, 7), 45, "rope", F32),
+    ((3, 3), 2, 64, 128, 40, (8, 1), 32, "alibi", F32),
+    ((1, 0, 2), 3, 35, 20, 40, (6, 3, 2), 33, "pope", F32),
+    ((2, 1), 1, 258, 64, 12, (4, 9), 3, "rope", BF16),
+    ((5,), 1, 129, 36, 132, (100, 3), 29, "alibi", BF16),
+]
+
+
+@pytest.mark.parametrize("counts,h,N,d,S,lens,T,rotary,dtype", READ)
+def test_attention_equals_the_definition(gpu, counts, h, N, d, S, lens, T, rotary, dtype):
+    _check_read(gpu, Case(hash((sum(counts), h, N, d, T)) % 2**31, counts, h, N, d, S, lens, T, rotary, dtype))
+
+
+@pytest.mark.parametrize("density", [0.0, 1.0])
+@pytest.mark.parametrize("T", [1, 6])
+def test_silent_and_fully_firing_tokens(gpu, density, T):
+    out = _check_read(gpu, Case(7, (3, 2), 2, 200, 64, 24, (0, 11, 18), T, "rope", F32, density))
+    if density == 0.0:
+        assert not out.any()
+
+
+def _check_fork(gpu, c, out):
+    """u * (len additions + decays 8 + products 3) of the magnitudes; a bf16 state is rounded once more, by half a step."""
+    ref = np.zeros((c.B, c.h, c.Nq, c.d))
+    mag = np.zeros_like(ref)
+    for b in range(c.B):
+        n = int(c.lens[b])
+        a, back = np.exp(c.rate * n)[:, None, None], np.exp(c.rate[:, None] * (n - np.arange(n)))
+        k = c.keys[b, :, :, :n].astype(np.float64) * back[:, None]
+        ref[b] = a * c.rho[c.owner[b]] + k @ c.values[b, :n].astype(np.float64)
+        mag[b] = a * np.abs(c.rho[c.owner[b]]) + np.abs(k) @ np.abs(c.values[b, :n].astype(np.float64))
+    bound = U * (int(c.lens.max()) + 12) * mag
+    if c.dtype == BF16:
+        bound = bound * (1 + 2.0**-8) + 2.0**-8 * np.abs(ref)
+    err = np.abs(out.double().cpu().numpy() - ref)
+    assert (err <= bound + 1e-37).all(), (err / (mag + 1e-300)).max() / U
+
+
+FORK = [
+    ((1,), 1, 2, 4, 4, (0,), "rope", F32),
+    ((4,), 4, 256, 256, 32, (5, 32, 17), "alibi", F32),
+    ((3, 0, 2), 2, 70, 68, 8, (8, 0, 3), "rope", BF16),
+    ((2, 1), 3, 33, 12, 12, (5, 11, 12), "alibi", BF16),
+    ((2,), 1, 31, 132, 20, (9, 19), "pope", F32),
+    ((3,), 1, 260, 1024, 64, (63, 64, 1), "rope", F32),
+    ((2,), 2, 9, 64, 1028, (1025, 3), "alibi", F32),
+]
+
+
+@pytest.mark.parametrize("counts,h,N,d,S,lens,rotary,dtype", FORK)
+def test_fork_equals_the_definition(gpu, counts, h, N, d, S, lens, rotary, dtype):
+    _, _, shared = gpu
+    c = Case(hash((h, N, d)) % 2**31, counts, h, N, d, S, lens, 1, rotary, dtype)
+    t = c.device()
+    before = t["rho"].clone()
+    out = shared.shared_prefix_fork(t["rho"], t["keys"], t["values"], t["lens"], rotary_embedding=rotary,
+                                    alibi_slopes=c.slopes, counts=c.counts)
+    _check_fork(gpu, c, out)
+    assert torch.equal(before, t["rho"])
+
+
+@pytest.mark.parametrize("rotary", ["rope", "alibi", "pope"])
+def test_steps_equal_those_of_own_states(gpu, rotary):
+    """5 tokens at once, then 6 one by one, next to recurrent_attention on a copy of the prompt's state for each sequence:
+    both within their bounds of the definition, so of each other within twice the bound of the longer sums."""
+    _, recurrent, shared = gpu
+    c = Case(11, (3, 2), 2, 96, 64, 16, (0,), 5, rotary, F32)
+    t = c.device()
+    rho = t["rho"][c.owner].clone()
+    rng = np.random.default_rng(3)
+    lens, pos = t["lens"], t["positions"]
+    scale = 0.0
+    for n in [5] + [1] * 6:
+        x = torch.from_numpy(np.maximum(rng.standard_normal((5, 2, n, 96)), 0).astype(np.float32)).to(DEV)
+        v = torch.from_numpy(rng.standard_normal((5, n, 64)).astype(np.float32)).to(DEV)
+        own = recurrent.recurrent_attention(x, v, rho, t["freqs"], 0, rotary_embedding=shared.RotaryEmbedding.parse(rotary),
+                                            alibi_slopes=c.slopes, positions=pos)
+        out = shared.shared_prefix_attention(x, v, t["rho"], t["keys"], t["values"], lens, t["freqs"], positions=pos,
+                                             rotary_embedding=rotary, alibi_slopes=c.slopes, counts=c.counts)
+        lens += n
+        pos += n
+        scale = max(scale, own.abs().max().item())
+        assert (out - own).abs().max().item() <= 1e-5 * scale  # u * depth (400) * cancellation (terms over their sum, < 1/2)
+    state = shared.shared_prefix_fork(t["rho"], t["keys"], t["values"], lens, rotary_embedding=rotary, alibi_slopes=c.slopes,
+                                      counts=c.counts)
+    assert (state - rho).abs().max().item() <= 1e-5 * rho.abs().max().item()
+
+
+@pytest.mark.parametrize("T", [1, 4])
+def test_a_sequence_without_room_gets_nan_and_others_their_output(gpu, T):
+    _, _, shared = gpu
+    c = Case(5, (4,), 2, 40, 64, 16, (3, 8, 5, 2), T, "rope", F32)
+    t = c.device()
+    good = c.call(shared, t)
+    t = c.device()
+    t["lens"][1] = 17
+    t["lens"][2] = -1
+    keys, values = t["keys"].clone(), t["values"].clone()
+    out = c.call(shared, t)
+    assert torch.isnan(out[1]).all() and torch.isnan(out[2]).all()
+    assert torch.equal(out[0], good[0]) and torch.equal(out[3], good[3])
+    assert torch.equal(t["keys"][1:3], keys[1:3]) and torch.equal(t["values"][1:3], values[1:3])
+    state = shared.shared_prefix_fork(t["rho"], t["keys"], t["values"], t["lens"], counts=c.counts)
+    assert torch.isnan(state[1]).all() and torch.isnan(state[2]).all() and torch.isfinite(state[[0, 3]]).all()
+
+
+def test_equal_calls_give_equal_bits(gpu):
+    _, _, shared = gpu
+    for T in (1, 7):
+        c = Case(9, (33, 4), 2, 300, 128, 24, (13, 2), T, "rope", F32)
+        outs = []
+        for _ in range(3):
+            t = c.device()
+            outs.append((c.call(shared, t), t["keys"]))
+        assert all(torch.equal(o, outs[0][0]) and torch.equal(k, outs[0][1]) for o, k in outs)
+
+
+def test_graph_replays_walk_on(gpu):
+    """A step and the advance of lens and positions in one graph: every replay is the next token, checked against eager
+    steps, with eager work of another shape between the replays."""
+    ffi, _, shared = gpu
+    c = Case(21, (6,), 2, 128, 64, 16, (2, 5), 1, "rope", F32)
+    other = Case(22, (2,), 1, 64, 32, 8, (1,), 3, "alibi", F32)
+    ctx = ffi.Context(0)
+    rng = np.random.default_rng(8)
+    xs = torch.from_numpy(np.maximum(rng.standard_normal((7, 6, 2, 1, 128)), 0).astype(np.float32)).to(DEV)
+    vs = torch.from_numpy(rng.standard_normal((7, 6, 1, 64)).astype(np.float32)).to(DEV)
+
+    def step(t, x, v):
+        o = shared.shared_prefix_attention(x, v, t["rho"], t["keys"], t["values"], t["lens"], t["freqs"],
+                                           positions=t["positions"], counts=c.counts, ctx=ctx)
+        for p in ("lens", "positions"):
+            ctx.check(ctx.lib.bdh_advance_positions(ctx.handle, t[p].data_ptr(), 6, 1))
+        return o
+
+    t = c.device()
+    want = [step(t, x, v).clone() for x, v in zip(xs, vs)]
+    end = t["keys"].clone()
+    t = c.device()
+    x, v = xs[0].clone(), vs[0].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        out = step(t, x, v)
+    for i in range(7):
+        x.copy_(xs[i])
+        v.copy_(vs[i])
+        graph.replay()
+        assert torch.equal(out, want[i]), i
+        o = other.device()
+        other.call(shared, o)
+        torch.cuda.synchronize()
+    assert torch.equal(t["keys"], end)
+
+
+def test_another_stream_and_two_contexts(gpu):
+    ffi, _, shared = gpu
+    c = Case(31, (8,), 2, 128, 64, 16, (2, 5), 1, "rope", F32)
+    t = c.device()
+    want = c.call(shared, t)
+    torch.cuda.synchronize()
+    a, b = ffi.Context(0), ffi.Context(0)
+    sa, sb = torch.cuda.Stream(), torch.cuda.Stream()
+    ta, tb = c.device(), c.device()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(sa):
+        oa = c.call(shared, ta, ctx=a)
+    with torch.cuda.stream(sb):
+        ob = c.call(shared, tb, ctx=b)
+    torch.cuda.synchronize()
+    assert torch.equal(oa, want) and torch.equal(ob, want)

@@ -1,0 +1,96 @@
+"""What the operators of many sequences refuse, without a GPU: the C entry points (shared_refusal_test.cpp) and the checks
+of the Python functions, which come before a context is asked for."""
+import os
+import subprocess
+
+import pytest
+import torch
+
+from burn_dragon_amd import build
+from burn_dragon_amd.rules import LogitRules, apply_rules, count_tokens, pack_allowed, token_counts
+from burn_dragon_amd.shared import shared_prefix_attention, shared_prefix_fork
+from burn_dragon_amd.slots import copy_slots
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+
+
+def test_the_c_entry_points_refuse_before_they_touch_a_device(tmp_path):
+    exe = str(tmp_path / "shared_refusal_test")
+    subprocess.run([build.HIPCC, *build.FLAGS, "-x", "hip", os.path.join(HERE, "shared_refusal_test.cpp"), "-x", "none", "-o", exe,
+                    "-L" + build.PKG, "-lbdh_mi355x", "-Wl,-rpath," + build.PKG], check=True, capture_output=True)
+    done = subprocess.run([exe], capture_output=True, text=True)
+    assert done.returncode == 0 and done.stdout == "ok\n", (done.returncode, done.stdout, done.stderr)
+
+
+def _read_args():
+    return {"query": torch.zeros(5, 2, 1, 6), "value": torch.zeros(5, 1, 8), "rho": torch.zeros(2, 2, 6, 8),
+            "keys": torch.zeros(5, 2, 6, 8), "values": torch.zeros(5, 8, 8), "lens": torch.zeros(5, dtype=torch.int32),
+            "freqs": torch.zeros(6), "counts": [3, 2]}
+
+
+@pytest.mark.parametrize("name,bad", [
+    ("query", torch.zeros(5, 2, 1, 6, dtype=torch.float64)), ("query", torch.zeros(5, 2, 1, 12)[..., ::2]),
+    ("value", torch.zeros(5, 1, 8, dtype=torch.bfloat16)), ("rho", torch.zeros(2, 2, 6, 8, dtype=torch.float16)),
+    ("rho", torch.zeros(2, 2, 5, 8)), ("rho", torch.zeros(2, 2, 8, 6).transpose(2, 3)), ("keys", torch.zeros(5, 2, 7, 8)),
+    ("keys", torch.zeros(5, 2, 6, 8, dtype=torch.bfloat16)), ("values", torch.zeros(5, 7, 8)),
+    ("lens", torch.zeros(5, dtype=torch.int64)), ("lens", torch.zeros(4, dtype=torch.int32)), ("freqs", torch.zeros(5)),
+    ("positions", torch.zeros(5)), ("counts", [3, 3]), ("counts", None), ("counts", [6, -1]), ("counts", [5]),
+    ("alibi_slopes", [1.0])])
+def test_attention_checks_its_arguments(name, bad):
+    args = _read_args()
+    args[name] = bad
+    with pytest.raises(ValueError):
+        shared_prefix_attention(**args)
+
+
+@pytest.mark.parametrize("name,bad", [
+    ("rho", torch.zeros(2, 2, 5, 8)), ("keys", torch.zeros(5, 2, 6, 9)), ("values", torch.zeros(4, 8, 8)),
+    ("lens", torch.zeros(5)), ("counts", [1, 1]), ("out", torch.zeros(5, 2, 6, 8, dtype=torch.bfloat16)),
+    ("out", torch.zeros(4, 2, 6, 8))])
+def test_fork_checks_its_arguments(name, bad):
+    args = {k: v for k, v in _read_args().items() if k in ("rho", "keys", "values", "lens", "counts")}
+    args[name] = bad
+    with pytest.raises(ValueError):
+        shared_prefix_fork(**args)
+
+
+def test_slots_check_their_arguments():
+    a, b = torch.zeros(3, 4, 5), torch.zeros(3, 6, 5)
+    for buffers, origin in [([(a, b.to(torch.int32), 1)], [0] * 4), ([(a, b, 0)], [0] * 3), ([(a, b, 1), (a, a, 1)], [0] * 4),
+                            ([(a, b, 1)], [0] * 5), ([(a, b, 1)], [6, 0, 0, 0]), ([(a, b, 1)], [-3, 0, 0, 0]),
+                            ([(a, b.transpose(0, 2).contiguous().transpose(0, 2), 1)], [0] * 4),
+                            ([(a, b, 1)], torch.zeros(4, dtype=torch.int64)), ([(a, b[0], 1)], [0] * 4)]:
+        with pytest.raises(ValueError):
+            copy_slots(buffers, origin)
+    copy_slots([], [])
+
+
+def test_rules_check_their_arguments():
+    z, seen = torch.zeros(2, 40), torch.zeros(2, 40, dtype=torch.int32)
+    for rules, more in [(LogitRules(repetition=1.1), {}), (LogitRules(), {"newest": torch.zeros(2, dtype=torch.int64)}),
+                        (LogitRules(1.1), {"seen": seen.long()}), (LogitRules(1.1), {"seen": seen[:1]}),
+                        (LogitRules(1.1), {"seen": seen, "newest": torch.zeros(3, dtype=torch.int64)}),
+                        (LogitRules(1.1), {"seen": seen, "newest": torch.zeros(2, dtype=torch.int32)}),
+                        (LogitRules(torch.zeros(3)), {"seen": seen}), (LogitRules(bias=torch.zeros(39)), {}),
+                        (LogitRules(bias=torch.zeros(3, 40)), {}), (LogitRules(allowed=torch.zeros(2, dtype=torch.int64)), {}),
+                        (LogitRules(allowed=torch.zeros(3, dtype=torch.int32)), {}), (LogitRules(), {"out": torch.zeros(2, 41)})]:
+        with pytest.raises(ValueError):
+            apply_rules(z, rules, **more)
+    with pytest.raises(ValueError):
+        apply_rules(z.double(), LogitRules())
+    with pytest.raises(ValueError):
+        apply_rules(torch.zeros(40, 2).t(), LogitRules())
+    for tokens, kw in [(torch.zeros(2, 3, dtype=torch.int32), {}), (torch.zeros(3, 3, dtype=torch.int64), {}),
+                       (torch.zeros(3, 2, dtype=torch.int64).t(), {}), (torch.zeros(2, 3, dtype=torch.int64), {"lens": torch.zeros(2)})]:
+        with pytest.raises(ValueError):
+            count_tokens(tokens, seen, **kw)
+
+
+def test_packed_masks_and_empty_counts():
+    mask = torch.rand(3, 70, generator=torch.Generator().manual_seed(1)) < 0.5
+    words = pack_allowed(mask)
+    assert words.shape == (3, 3) and words.dtype == torch.int32
+    for b in range(3):
+        for v in range(96):
+            assert (int(words[b, v // 32]) >> (v % 32)) & 1 == (int(mask[b, v]) if v < 70 else 0)
+    assert not token_counts(2, 9, "cpu").any()
