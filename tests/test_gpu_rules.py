@@ -1,7 +1,8 @@
 """Penalties, biases and masks on logits (apply_rules) and the counts they read (count_tokens) against numpy in 64 bits.
 
 Tolerance: a division or product, frequency * n, its sum with presence, two subtractions / additions: 5 roundings, each of
-at most u = 2^-24 of the magnitudes that pass through it; and the factors n <= 2^24 are exact: 6 u (|z| r + f n + p + |bias|)."""
+at most u = 2^-24 of the magnitudes that pass through it; and the factors n <= 2^24 are exact: 6 u (|z r| + |f| n + |p| + |bias|), magnitudes also
+of the negative penalties."""
 import numpy as np
 import pytest
 import torch
@@ -34,7 +35,7 @@ def _reference(logits, seen, newest, rep, pres, freq, bias, allowed):
         f = np.zeros((B, 1)) if freq is None else freq.astype(np.float64)[:, None]
         met = seen != 0
         z = np.where(met, np.where(z > 0, z / r, z * r), z)
-        mag = np.abs(z) + f * n + p
+        mag = np.abs(z) + np.abs(f) * n + np.abs(p)
         z = z - (f * n + p * (n > 0))
     if bias is not None:
         z = z + bias
