@@ -5,6 +5,7 @@
 // with a = exp(-slope_h) for ALiBi, else 1: src/model/bdh.rs:288-302 with the sum over tokens cut where the prompt ends.
 // The keys of a neuron lie side by side, so the neurons that are silent now are not read.
 #include <algorithm>
+#include <type_traits>
 
 #include "bdh_internal.h"
 #include "gemm_f32.h"
@@ -16,130 +17,23 @@ constexpr int kMaxPrompts = BDH_MAX_SHARED_PROMPTS;
 constexpr float kLnEps = 1e-5f;  // src/model/bdh.rs:17
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2u __attribute__((ext_vector_type(2), aligned(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
 
 struct Prompts {
   int G;
-  int begin[kMaxPrompts + 1];  // sequences of prompt g: begin[g] .. begin[g + 1] - 1
+  int begin[kMaxPrompts + 1];         // sequences of prompt g: begin[g] .. begin[g + 1] - 1
+  unsigned char by_size[kMaxPrompts];  // the prompts, those with most sequences first
 };
 struct HeadRates {
   float log_decay[64];
 };
 
 __device__ __forceinline__ bool valid_len(int len, int T, int longest, int S) { return len >= 0 && len <= longest && len + T <= S; }
-
-// ---- one token per sequence ------------------------------------------------------------------------------------------
-
-struct SuffixArgs {
-  const float *x, *freqs;
-  float *q;     // [B,h,Nq]
-  float *keys;  // [B,h,Nq,S]
-  float *score_parts;  // [B*h][blocks][S]
-  const int32_t *lens, *positions;
-  long position;
-  int h, N, Nq, S, rotary, blocks, longest;
-};
-
-// The queries of a block of neurons of one (sequence, head), their place among the keys, and the block's part of the scores.
-__global__ __launch_bounds__(256) void k_suffix_scores(SuffixArgs g) {
-  __shared__ int s_row[512];
-  __shared__ float s_q[512];
-  __shared__ int s_cnt[8];
-  __shared__ float4 s_acc[16][16];
-  const int blk = blockIdx.x, bh = blockIdx.y, b = bh / g.h, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int len = g.lens[b];
-  const bool valid = valid_len(len, 1, g.longest, g.S);
-  const float pos = (float)(g.positions ? (long)g.positions[b] : g.position);
-  const int p = blk * 256 + tid;  // RoPE, ALiBi: neurons 2p and 2p + 1; PoPE: neuron p, rows p and N + p
-  const float *x = g.x + (long)bh * g.N;
-  int row[2] = {-1, -1};
-  float q[2] = {0.0f, 0.0f};
-  if (g.rotary == BDH_POPE) {
-    if (p < g.N) {
-      float s, c;
-      sincosf(rope_phase(pos, g.freqs[p]), &s, &c);
-      const float m = softplus1(x[p]);
-      row[0] = p;
-      row[1] = g.N + p;
-      q[0] = m * c;
-      q[1] = m * s;
-    }
-  } else {
-    const int n = 2 * p;
-    if (n < g.N) { row[0] = n; q[0] = x[n]; }
-    if (n + 1 < g.N) { row[1] = n + 1; q[1] = x[n + 1]; }
-    if (g.rotary == BDH_ROPE && (q[0] != 0.0f || q[1] != 0.0f)) {
-      const float x0 = q[0], x1 = q[1];
-      float s0, c0, s1, c1;
-      sincosf(rope_phase(pos, g.freqs[n]), &s0, &c0);
-      sincosf(rope_phase(pos, g.freqs[n + 1]), &s1, &c1);
-      const float a0 = x0 * c0, r0 = (-x1) * s0, a1 = x1 * c1, r1 = x0 * s1;
-      q[0] = a0 + r0;
-      q[1] = a1 + r1;
-    }
-  }
-  float *K = g.keys + (long)bh * g.Nq * g.S;
-  unsigned long long mask[2];
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    if (row[e] >= 0) g.q[(long)bh * g.Nq + row[e]] = q[e];
-    mask[e] = __ballot(q[e] != 0.0f);
-  }
-  if (lane == 0) s_cnt[wave] = __popcll(mask[0]) + __popcll(mask[1]);
-  __syncthreads();
-  int at = 0, cnt = 0;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    if (w < wave) at += s_cnt[w];
-    cnt += s_cnt[w];
-  }
-  const unsigned long long below = (1ull << lane) - 1;
-  at += __popcll(mask[0] & below) + __popcll(mask[1] & below);
-#pragma unroll
-  for (int e = 0; e < 2; ++e)
-    if (q[e] != 0.0f) {
-      s_row[at] = row[e];
-      s_q[at++] = q[e];
-      if (valid) K[(long)row[e] * g.S + len] = q[e];
-    }
-  __syncthreads();
-  if (!valid) return;
-  // sixteen groups of sixteen lanes; a group takes every sixteenth active row, a lane four neighbouring keys of it
-  const int grp = tid >> 4, li = tid & 15;
-  float *parts = g.score_parts + ((long)bh * g.blocks + blk) * g.S;
-  for (int s0 = 0; s0 < len; s0 += 64) {
-    const int s = s0 + li * 4;
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (s < len) {
-      int e = grp;
-      for (; e + 48 < cnt; e += 64) {
-        f32x4 k[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) k[u] = *reinterpret_cast<const f32x4 *>(K + (long)s_row[e + 16 * u] * g.S + s);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) acc += s_q[e + 16 * u] * k[u];
-      }
-      for (; e < cnt; e += 16) acc += s_q[e] * *reinterpret_cast<const f32x4 *>(K + (long)s_row[e] * g.S + s);
-    }
-    __syncthreads();
-    s_acc[grp][li] = make_float4(acc.x, acc.y, acc.z, acc.w);
-    __syncthreads();
-    if (tid < 64 && s0 + tid < len) {
-      const float *col = reinterpret_cast<const float *>(&s_acc[0][0]) + tid;
-      float t = 0.0f;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) t += col[64 * r];
-      parts[s0 + tid] = t;
-    }
-  }
-}
-
-struct ReadArgs {
-  const float *q;    // [B,h,Nq]
-  const void *rho;   // [G,h,Nq,d]
-  float *partial;    // [parts][B*h][d]
-  int B, h, Nq, d, rows;  // rows of the state a workgroup takes (64, 128 or 256)
-  int kw;                 // wavefronts that share the rows of one column group
-};
 
 __device__ __forceinline__ f32x4 load_state4(const float *p) { return *reinterpret_cast<const f32x4 *>(p); }
 __device__ __forceinline__ f32x4 load_state4(const unsigned short *p) {
@@ -148,98 +42,529 @@ __device__ __forceinline__ f32x4 load_state4(const unsigned short *p) {
                __uint_as_float(v.y & 0xffff0000u)};
 }
 
-// The product of up to 16 * RT sequences' queries with a block of rows of their prompt's state, on the f32 matrix cores.  The
-// rows that some of them uses are listed first; v_mfma_f32_16x16x4_f32 takes four listed rows at a time, a lane's 16-byte
-// load being one row of four column tiles (columns 4 * (lane % 16) + c of tile c).
-template <typename R, int RT>
-__global__ __launch_bounds__(256) void k_shared_read(ReadArgs g, Prompts pr) {
-  extern __shared__ __attribute__((aligned(16))) float s_dyn[];
-  __shared__ unsigned short s_list[256 + 16];
-  __shared__ int s_used[256];
-  __shared__ int s_cnt[4];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, blk = blockIdx.x, hh = blockIdx.y;
-  int tile = blockIdx.z, grp = 0;
-  for (; grp < pr.G; ++grp) {
-    const int tiles = (pr.begin[grp + 1] - pr.begin[grp] + 16 * RT - 1) / (16 * RT);
-    if (tile < tiles) break;
-    tile -= tiles;
-  }
-  if (grp >= pr.G) return;
-  const int b0 = pr.begin[grp] + tile * 16 * RT, nb = min(16 * RT, pr.begin[grp + 1] - b0);
-  const int n0 = blk * g.rows, rows = min(g.rows, g.Nq - n0);
-  const int ldq = g.rows + 4;
-  float *s_q = s_dyn;  // [16 * RT][ldq]
-  const int r = tid & (g.rows - 1), part = tid / g.rows, n_part = 256 / g.rows;
-  if (tid < g.rows) s_used[tid] = 0;
-  __syncthreads();
-  const float *q = g.q + ((long)b0 * g.h + hh) * g.Nq + n0 + r;
-  const long q_seq = (long)g.h * g.Nq;
-  if (r < rows) {
-    bool used = false;
-    for (int i = part; i < nb; i += n_part) used |= q[i * q_seq] != 0.0f;
-    if (used) s_used[r] = 1;
-  }
-  __syncthreads();
-  const bool mine = tid < g.rows && s_used[tid];
-  const unsigned long long mask = __ballot(mine);
-  if (lane == 0) s_cnt[wave] = __popcll(mask);
-  __syncthreads();
-  int at = 0, cnt = 0;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    if (w < wave) at += s_cnt[w];
-    cnt += s_cnt[w];
-  }
-  at += __popcll(mask & ((1ull << lane) - 1));
-  if (mine) {
-    s_list[at] = (unsigned short)tid;
-    s_used[tid] = at + 1;  // its place in the list, from 1 on
-  }
-  __syncthreads();
-  const int steps = (cnt + 15) / 16;
-  if (tid < 16 && cnt + tid < steps * 16) s_list[cnt + tid] = s_list[0];  // the last step's spare rows: queries of zero
-  for (int e = tid; e < (steps * 16 - cnt) * 16 * RT; e += 256) s_q[(e % (16 * RT)) * ldq + cnt + e / (16 * RT)] = 0.0f;
-  if (r < rows && s_used[r]) {
-    const int place = s_used[r] - 1;
-    for (int i = part; i < 16 * RT; i += n_part) s_q[i * ldq + place] = i < nb ? q[i * q_seq] : 0.0f;
-  }
-  __syncthreads();
-  const R *rho = static_cast<const R *>(g.rho) + (((long)grp * g.h + hh) * g.Nq + n0) * g.d;
-  const int groups = (g.d + 63) / 64, cols = 4 / g.kw;  // column groups the wavefronts take at a time
-  const int k4 = lane >> 4, li = lane & 15, sub = wave / cols;
-  for (int cg = wave % cols; cg < groups; cg += cols) {
-    const int col = cg * 64 + li * 4;
-    const R *base = rho + (col < g.d ? col : 0);
-    f32x4 acc[RT][4];
+// sin and cos of 2 pi f, 0 <= f < 1 (the phase of src/model/attention.rs:342-343 before its factor 2 pi): f is taken to the
+// nearest quarter turn, which is exact, and the rest to the polynomials of least largest error on an eighth of a turn either
+// side (3e-9 and 3e-10; 1.7 steps of the result with the roundings).  Twenty operations where sincosf takes some sixty.
+__device__ __forceinline__ void sincos_turns(float f, float &s, float &c) {
+  const float y = f * 4.0f, k = rintf(y), t = y - k, u = t * t;
+  const float a = t * fmaf(fmaf(fmaf(-0.004602177f, u, 0.07968023f), u, -0.6459635f), u, 1.5707964f);
+  const float b = fmaf(fmaf(fmaf(fmaf(0.00090752944f, u, -0.020861866f), u, 0.25366944f), u, -1.2337005f), u, 1.0f);
+  const int quarter = (int)k;
+  const float p = (quarter & 1) ? b : a, r = (quarter & 1) ? a : b;
+  s = (quarter & 2) ? -p : p;
+  c = ((quarter + 1) & 2) ? -r : r;
+}
+__device__ __forceinline__ float turns(float pos, float f) {
+  const float raw = pos * f;
+  return raw - floorf(raw);
+}
+// both neurons of a RoPE pair (src/model/attention.rs:305-321)
+__device__ __forceinline__ void rotate_pair(float pos, float f0, float f1, float &x0, float &x1) {
+  float s0, c0, s1, c1;
+  sincos_turns(turns(pos, f0), s0, c0);
+  sincos_turns(turns(pos, f1), s1, c1);
+  const float a0 = x0 * c0, r0 = (-x1) * s0, a1 = x1 * c1, r1 = x0 * s1;
+  x0 = a0 + r0;
+  x1 = a1 + r1;
+}
+
+// ---- queries times rows of a matrix -----------------------------------------------------------------------------------
+
+constexpr int kDenseTokens = 64;  // from here on: dense products
+constexpr int kRowsMost = 256;    // rows of the matrix a workgroup takes at a time
+
+struct PassArgs {
+  const float *x, *freqs;  // one token a sequence: its activations, turned here
+  const float *q;          // several: the queries [B,h,T,Nq]
+  const int32_t *lens, *positions;
+  long position;
+  const void *rho;     // [G,h,Nq,d]
+  float *keys;         // [B,h,Nq,S]
+  float *partial;      // [parts][B*h*T][d]
+  float *score_parts;  // [score_parts_n][B*h*T][span]
+  int B, h, T, N, Nq, d, S, rotary, longest;
+  int rows, cg, row_blocks;      // rows and column groups a workgroup takes at a time, blocks of rows in all
+  int parts, per, longer;        // of a sum: the blocks of rows are dealt to so many workgroups, per or (the first `longer`) per + 1
+  int col_blocks;                // the columns' workgroups
+  int span, score_parts_n;       // columns and parts of the scores
+  int score_per, score_longer, score_cols;  // several tokens: as per, longer, col_blocks
+};
+
+// How a product is made: see Product.
+enum { kF32 = 0, kHalf = 1, kSplit = 2 };
+
+// the wavefront of a thread, as a number that all of its lanes are known to share: what follows from it stays in scalar registers
+__device__ __forceinline__ int wave_of_thread() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
+struct TileShared {
+  __attribute__((aligned(16))) unsigned short list[kRowsMost + 32];
+  int used[kRowsMost];
+  int cnt[4];
+  int row[64];                              // query i is row[i] of [B,h,T]
+  float pos[64];
+  int len[64];                              // of the tile's sequences; -1: no room
+  unsigned long long fires[64][kRowsMost / 64];  // one token: what of a sequence is active, a bit for a pair of rows (or a row)
+  unsigned short item[4][1024 + 64];        // a wavefront's active (sequence, pair)s, and room for what is none
+  unsigned short own[8][kRowsMost];         // half a wavefront's sequence: its active pairs (or rows), listed
+};
+
+// Queries of up to 16 * RT sequences (or tokens) times the rows n0 .. n0 + rows - 1 of a matrix [*, cols].  The rows that
+// some query uses are listed, the queries go to LDS in the list's order, and a wavefront takes 64 (kHalf: 128) columns:
+//  kF32    v_mfma_f32_16x16x4_f32 takes four listed rows; a lane's load is one row of four column tiles (columns
+//          4 * (lane % 16) + c of tile c).
+//  kHalf   a bf16 matrix times the three bf16 terms of the queries on v_mfma_f32_16x16x32_bf16: products are exact, sums f32.
+//          A lane loads eight columns of eight listed rows and swaps them by v_perm into one operand a column.
+//  kSplit  an f32 matrix taken as three bf16 terms too, six of the nine products (what is left out is below 2^-23 of one).
+// The wavefronts that share the rows of a column group add their sums in LDS in a fixed order.
+template <typename R, int RT, int MODE>
+struct Product {
+  static constexpr int kQ = 16 * RT, C = MODE == kHalf ? 8 : 4, kCols = 16 * C, kStep = MODE == kF32 ? 16 : 32;
+  static constexpr int kDepth = MODE == kF32 ? 4 : 2;
+  TileShared &sh;
+  char *tile;  // the queries: f32 [query][ld], or three planes [query][ld] of bf16
+  int ld, cnt = 0;
+  f32x4 acc[RT][C];
+
+  __device__ __forceinline__ Product(TileShared &shared, char *lds, int rows) : sh(shared), tile(lds), ld(rows + (MODE == kF32 ? 4 : 8)) {
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) acc[i][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int st = sub; st < steps; st += g.kw) {
-      const int k0 = st * 16 + k4 * 4;
-      f32x4 bv[4];
+      for (int c = 0; c < C; ++c) acc[i][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  __device__ __forceinline__ void put(int i, int place, float v) const {
+    if constexpr (MODE == kF32) {
+      reinterpret_cast<float *>(tile)[i * ld + place] = v;
+    } else {  // hi + mid + lo is v itself
+      unsigned short *p = reinterpret_cast<unsigned short *>(tile) + i * ld + place;
+      const unsigned short hi = f32_to_bf16(v);
+      const float r = v - bf16_to_f32(hi);
+      const unsigned short mid = f32_to_bf16(r);
+      p[0] = hi;
+      p[kQ * ld] = mid;
+      p[2 * kQ * ld] = f32_to_bf16(r - bf16_to_f32(mid));
+    }
+  }
+  __device__ __forceinline__ float get(int i, int place) const {
+    if constexpr (MODE == kF32) {
+      return reinterpret_cast<const float *>(tile)[i * ld + place];
+    } else {
+      const unsigned short *p = reinterpret_cast<const unsigned short *>(tile) + i * ld + place;
+      return bf16_to_f32(p[0]) + bf16_to_f32(p[kQ * ld]) + bf16_to_f32(p[2 * kQ * ld]);
+    }
+  }
+
+  // the list of the rows in use: the place of row r is used[r] - 1; the spare rows of the last step are row 0 of the list
+  // with queries of zero
+  __device__ __forceinline__ int list_rows(int rows) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const bool mine = tid < rows && sh.used[tid] != 0;
+    const unsigned long long mask = __ballot(mine);
+    if (lane == 0) sh.cnt[wave] = __popcll(mask);
+    __syncthreads();
+    int at = __popcll(mask & ((1ull << lane) - 1));
+    cnt = 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) bv[j] = load_state4(base + (long)s_list[k0 + j] * g.d);
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) at += sh.cnt[w];
+      cnt += sh.cnt[w];
+    }
+    if (mine) {
+      sh.list[at] = (unsigned short)tid;
+      sh.used[tid] = at + 1;
+    }
+    __syncthreads();
+    const int pad = (cnt + kStep - 1) / kStep * kStep - cnt;
+    if (tid < pad) sh.list[cnt + tid] = sh.list[0];
+    return pad;
+  }
+
+  // queries in memory: row n0 and those behind it, `have` of them.  A thread takes one row of every parts-th query.
+  template <bool MASKS>
+  __device__ __forceinline__ void load_queries(const float *q, unsigned ld_q, int nb, int rows, int have) {
+    const int tid = threadIdx.x, r = tid & (rows - 1), wave = wave_of_thread();
+    const int part = rows == 256 ? 0 : wave >> 1, parts = rows == 256 ? 1 : 2;  // rows is 128 or 256
+    const bool exists = r < have;
+    const unsigned at = min(r, have - 1);
+    const bool all = RT == 4;  // next to nothing of a row is silent in all of so many queries: no list
+    if (tid < rows) sh.used[tid] = all && exists ? tid + 1 : 0;
+    __syncthreads();
+    if (all) {
+      cnt = have;
+      sh.list[tid] = (unsigned short)(tid < have ? tid : 0);
+    }
+    if (!all || MASKS) {
+      bool used = false;
+#pragma unroll 1
+      for (int i0 = part; i0 < nb; i0 += 8 * parts) {
+        float v[8];
 #pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        const f32x4 av = *reinterpret_cast<const f32x4 *>(s_q + (i * 16 + li) * ldq + k0);
+        for (int k = 0; k < 8; ++k) v[k] = q[sh.row[min(i0 + k * parts, nb - 1)] * (long)ld_q + at];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[j], bv[j][c], acc[i][c], 0, 0, 0);
+        for (int k = 0; k < 8; ++k) {
+          const bool fires = v[k] != 0.0f && i0 + k * parts < nb && exists;
+          used |= fires;
+          if constexpr (MASKS) {
+            const unsigned long long mask = __ballot(fires);
+            if ((tid & 63) == 0 && i0 + k * parts < nb) sh.fires[i0 + k * parts][r >> 6] = mask;
+          }
+        }
+      }
+      if (!all) {
+        if (used) sh.used[r] = 1;
+        __syncthreads();
+        list_rows(rows);
       }
     }
-    float *out = g.partial + (long)(blk * g.kw + sub) * g.B * g.h * g.d;
+    const int width = (cnt + kStep - 1) / kStep * kStep;
+    for (int e = tid; e < (width - cnt) * kQ; e += 256) put(e % kQ, cnt + e / kQ, 0.0f);
+    const int place = sh.used[r] - 1;
+#pragma unroll 1
+    for (int i0 = part; i0 < kQ; i0 += 8 * parts) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = q[sh.row[min(i0 + k * parts, nb - 1)] * (long)ld_q + at];
+      if (place >= 0)
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (i0 + k * parts < kQ) put(i0 + k * parts, place, i0 + k * parts < nb ? v[k] : 0.0f);
+    }
+    __syncthreads();
+  }
+
+  // one token a sequence, RoPE or ALiBi: activations, turned here, and stored as the new keys of sequences own0 .. own1 - 1.  A
+  // thread looks at one pair of rows of every parts-th sequence; the pairs that fire are listed, so that the sines are taken
+  // for those and by full wavefronts.  (Short loops on purpose, here and below: code that a workgroup runs once waits for its
+  // instructions, some 100 cycles for every 64 bytes.  Unrolled, with the activations in registers, this kernel was 28 KB
+  // and took twice its time.)
+  __device__ __forceinline__ void turn_queries(const PassArgs &g, int row0, int nb, int n0, int own0, int own1, int my_len, float my_pos) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_of_thread();
+    const int pairs = g.rows / 2, p = tid & (pairs - 1), part = g.rows == 256 ? wave >> 1 : wave, parts = g.rows == 256 ? 2 : 4;
+    const int n = n0 + 2 * p;
+    const bool in0 = n < g.N, in1 = n + 1 < g.N, rope = g.rotary == BDH_ROPE;
+    const float *x = g.x + (long)row0 * g.N;
+    const unsigned c0 = min(n, g.N - 1), c1 = min(n + 1, g.N - 1);
+    const long step = (long)g.h * g.N;
+    if (tid < g.rows) sh.used[tid] = 0;
+    __syncthreads();
+    bool u0 = false, u1 = false;
+    int items = 0;
+#pragma unroll 1
+    for (int i0 = part; i0 < nb; i0 += 8 * parts) {
+      f32x2u v[8];  // loads without a condition, from places that exist: all are on their way at once
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float *at = x + min(i0 + k * parts, nb - 1) * step;
+        v[k] = f32x2u{at[c0], at[c1]};
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int i = i0 + k * parts;
+        const bool f0 = v[k].x != 0.0f && in0 && i < nb, f1 = v[k].y != 0.0f && in1 && i < nb;
+        u0 |= f0;
+        u1 |= f1;
+        const unsigned long long mask = __ballot(f0 || f1);
+        if (lane == 0 && i < nb) sh.fires[i][p >> 6] = mask;
+        sh.item[wave][f0 || f1 ? items + __popcll(mask & ((1ull << lane) - 1)) : 1024 + lane] = (unsigned short)(i << 8 | p);
+        items += __popcll(mask);
+      }
+    }
+    if (rope) u0 = u1 = u0 || u1;
+    if (u0) sh.used[2 * p] = 1;
+    if (u1) sh.used[2 * p + 1] = 1;
+    if (tid < 64) {
+      sh.len[tid] = my_len;
+      sh.pos[tid] = my_pos;
+    }
+    // an item's operands are on their way while the rows are listed, then while the one before it is turned
+    const float *f = g.freqs;
+    int it = sh.item[wave][min(lane, max(items - 1, 0))];
+    float x0 = 0.0f, x1 = 0.0f, t0 = 0.0f, t1 = 0.0f;
+    auto fetch = [&] {
+      const unsigned m = n0 + 2 * (it & 255), m1 = min(m + 1, (unsigned)g.N - 1), seq = (unsigned)((it >> 8) * g.h) * g.N;
+      x0 = x[seq + m];
+      x1 = x[seq + m1];
+      if (rope) {
+        t0 = f[m];
+        t1 = f[m1];
+      }
+    };
+    if (items > 0) fetch();
+    __syncthreads();
+    list_rows(g.rows);
+    {  // zeros, 16 bytes at a time (a query's room is a multiple of that)
+      const int width = (cnt + kStep - 1) / kStep * kStep * (MODE == kF32 ? 4 : 2), room = ld * (MODE == kF32 ? 4 : 2);
+#pragma unroll 1
+      for (int q = tid >> 4; q < (MODE == kF32 ? 1 : 3) * kQ; q += 16)
+        for (int o = (tid & 15) * 16; o < width; o += 256) *reinterpret_cast<u32x4 *>(tile + q * room + o) = u32x4{0, 0, 0, 0};
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int e = lane; e < items; e += 64) {
+      const int i = it >> 8, r = 2 * (it & 255), m = n0 + r;
+      float q0 = x0, q1 = m + 1 < g.N ? x1 : 0.0f;
+      const float a0 = t0, a1 = t1;
+      it = sh.item[wave][min(e + 64, items - 1)];
+      fetch();
+      if (rope) rotate_pair(sh.pos[i], a0, a1, q0, q1);
+      const int at0 = sh.used[r] - 1, at1 = sh.used[r + 1] - 1;
+      if (at0 >= 0) put(i, at0, q0);
+      if (at1 >= 0) put(i, at1, q1);
+      if (i >= own0 && i < own1 && sh.len[i] >= 0) {
+        float *key = g.keys + ((row0 + i * g.h) * (long)g.Nq + m) * g.S + sh.len[i];
+        if (q0 != 0.0f) key[0] = q0;
+        if (q1 != 0.0f) key[g.S] = q1;
+      }
+    }
+    __syncthreads();
+  }
+
+  __device__ __forceinline__ void multiply(const R *matrix, int ld_m, int cols, int col0, int cg, int nb) {
+    const int lane = threadIdx.x & 63, wave = wave_of_thread(), k4 = lane >> 4, li = lane & 15;
+    const int kw = 4 / cg, sub = wave / cg, steps = (cnt + kStep - 1) / kStep, col = col0 + (wave % cg) * kCols + li * C;
+    const unsigned from = col < cols ? col : 0;  // offsets from a scalar base: a block of rows is less than 4 GiB
+    constexpr int L = kStep / 4;  // rows a lane loads of a step
+    using V = typename std::conditional<MODE == kHalf, u32x4, f32x4>::type;
+    V buf[kDepth][L];
+    auto load = [&](V(&v)[L], int st) {
+      unsigned short r[L];
+      __builtin_memcpy(r, __builtin_assume_aligned(sh.list + min(st, steps - 1) * kStep + k4 * L, 2 * L), sizeof(r));
+#pragma unroll
+      for (int j = 0; j < L; ++j) {
+        if constexpr (MODE == kHalf) v[j] = *reinterpret_cast<const u32x4 *>(matrix + (r[j] * (unsigned)ld_m + from));
+        else v[j] = load_state4(matrix + (r[j] * (unsigned)ld_m + from));
+      }
+    };
+    auto product = [&](const V(&v)[L], int st) {
+      if constexpr (MODE == kF32) {
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+          if (i == 0 || i * 16 < nb) {
+            const f32x4 a = *reinterpret_cast<const f32x4 *>(reinterpret_cast<const float *>(tile) + (i * 16 + li) * ld + st * 16 + k4 * 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], v[j][c], acc[i][c], 0, 0, 0);
+          }
+      } else {
+        bf16x8 a[RT][3];
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int t = 0; t < 3; ++t)
+            a[i][t] = *reinterpret_cast<const bf16x8 *>(reinterpret_cast<const unsigned short *>(tile) + (t * kQ + i * 16 + li) * ld +
+                                                        st * 32 + k4 * 8);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          u32x4 o[3];
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            if constexpr (MODE == kHalf) {
+              o[0][m] = __builtin_amdgcn_perm(v[2 * m + 1][c >> 1], v[2 * m][c >> 1], (c & 1) ? 0x07060302u : 0x05040100u);
+            } else {
+              const float e0 = v[2 * m][c], e1 = v[2 * m + 1][c];
+              o[0][m] = pack_bf16_rne(e0, e1);
+              const float r0 = e0 - __uint_as_float(o[0][m] << 16), r1 = e1 - __uint_as_float(o[0][m] & 0xffff0000u);
+              o[1][m] = pack_bf16_rne(r0, r1);
+              o[2][m] = pack_bf16_rne(r0 - __uint_as_float(o[1][m] << 16), r1 - __uint_as_float(o[1][m] & 0xffff0000u));
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < RT; ++i)
+            if (i == 0 || i * 16 < nb) {
+              auto mac = [&](int ta, int tb) {
+                acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i][ta], __builtin_bit_cast(bf16x8, o[tb]), acc[i][c], 0, 0, 0);
+              };
+              if constexpr (MODE == kSplit) {
+                mac(0, 2);
+                mac(1, 1);
+              }
+              mac(2, 0);
+              if constexpr (MODE == kSplit) mac(0, 1);
+              mac(1, 0);
+              mac(0, 0);
+            }
+        }
+      }
+    };
+    if (steps == 0) return;
+#pragma unroll
+    for (int u = 0; u < kDepth; ++u) load(buf[u], sub + u * kw);
+    int st = sub;
+#pragma unroll 1
+    for (; st + kDepth * kw < steps; st += kDepth * kw) {
+#pragma unroll
+      for (int u = 0; u < kDepth; ++u) {
+        product(buf[u], st + u * kw);
+        load(buf[u], st + (kDepth + u) * kw);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kDepth; ++u)
+      if (st + u * kw < steps) product(buf[u], st + u * kw);
+  }
+
+  // The scores of these rows for sequences own0 .. own1 - 1: half a wavefront lists what of a sequence is active (PAIR: pairs of
+  // rows), then sixteen lanes take four neighbouring keys each of every other listed one.
+  template <bool PAIR>
+  __device__ __forceinline__ void own_keys(const PassArgs &g, int rb, int own0, int own1) {
+    constexpr int PER = PAIR ? 2 : 1, U = 8 / PER;
+    const int tid = threadIdx.x, half = tid >> 5, hl = tid & 31, k2 = hl >> 4, li = tid & 15;
+    const int last = g.Nq - 1 - rb * g.rows;
+    unsigned short *own = sh.own[half];
+#pragma unroll 1
+    for (int i = own0 + half; i < own1; i += 8) {
+      const int len = sh.len[i], row = sh.row[i];
+      int n = 0;
+#pragma unroll 1
+      for (int w = 0; w < g.rows / PER / 32; ++w) {
+        const unsigned mask = reinterpret_cast<const unsigned *>(sh.fires[i])[w];
+        if ((mask >> hl) & 1) own[n + __popc(mask & ((1u << hl) - 1))] = (unsigned short)(w * 32 + hl);
+        n += __popc(mask);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      const float *keys = g.keys + ((long)row * g.Nq + rb * g.rows) * g.S;
+      float *parts = g.score_parts + ((long)rb * g.B * g.h + row) * g.span;
+#pragma unroll 1
+      for (int s0 = 0; s0 < len; s0 += 64) {
+        const int s = s0 + li * 4;
+        f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (s < len)
+#pragma unroll 1
+          for (int e = k2; e < n; e += 2 * U) {
+            f32x4 k[U][PER];
+            int r[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              r[u] = own[min(e + 2 * u, n - 1)] * PER;
+#pragma unroll
+              for (int j = 0; j < PER; ++j) k[u][j] = *reinterpret_cast<const f32x4 *>(keys + (unsigned)(min(r[u] + j, last) * g.S + s));
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+              for (int j = 0; j < PER; ++j) {
+                const int place = sh.used[r[u] + j] - 1;  // a row of the pair may be nobody's (ALiBi)
+                const float q = get(i, max(place, 0));
+                sum += (e + 2 * u < n && place >= 0 ? q : 0.0f) * k[u][j];
+              }
+          }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sum[c] += __shfl_xor(sum[c], 16, 64);
+        if (k2 == 0 && s < len) *reinterpret_cast<f32x4 *>(parts + s) = sum;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+  }
+
+  // the sums of query i go to row sh.row[i] of out [B*h*T, cols]
+  __device__ __forceinline__ void finish(float *out, int cols, int col0, int cg, int nb) {
+    const int lane = threadIdx.x & 63, wave = wave_of_thread(), k4 = lane >> 4, li = lane & 15;
+    const int kw = 4 / cg, group = wave % cg, sub = wave / cg, col = col0 + group * kCols + li * C;
+    f32x4 *s = reinterpret_cast<f32x4 *>(tile);  // the queries are used up: their place takes the sums, and each wavefront of a
+    if (kw > 1) {                                // column group adds those of a share of the rows
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int c = 0; c < C; c += 4)
+            s[((wave * RT + i) * 4 + e) * (C * 16) + (c / 4) * 64 + lane] = f32x4{acc[i][c][e], acc[i][c + 1][e], acc[i][c + 2][e], acc[i][c + 3][e]};
+      __syncthreads();
+      if (col >= cols) return;
+#pragma unroll 1
+      for (int i = 0; i < RT; ++i)
+#pragma unroll 1
+        for (int e = sub * cg; e < (sub + 1) * cg; ++e) {  // 4 / kw = cg of the four
+          const int at = i * 16 + k4 * 4 + e;
+          if (at >= nb) continue;
+          float *o = out + (long)sh.row[at] * cols + col;
+#pragma unroll
+          for (int c = 0; c < C; c += 4) {
+            f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int w = group; w < 4; w += cg) sum += s[((w * RT + i) * 4 + e) * (C * 16) + (c / 4) * 64 + lane];
+            *reinterpret_cast<f32x4 *>(o + c) = sum;
+          }
+        }
+      return;
+    }
+    if (col >= cols) return;
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int seq = i * 16 + k4 * 4 + e;
-        if (seq < nb && col < g.d)
-          *reinterpret_cast<f32x4 *>(out + ((long)(b0 + seq) * g.h + hh) * g.d + col) =
-              f32x4{acc[i][0][e], acc[i][1][e], acc[i][2][e], acc[i][3][e]};
+        const int at = i * 16 + k4 * 4 + e;
+        if (at >= nb) continue;
+        float *o = out + (long)sh.row[at] * cols + col;
+#pragma unroll
+        for (int c = 0; c < C; c += 4)
+          *reinterpret_cast<f32x4 *>(o + c) = f32x4{acc[i][c][e], acc[i][c + 1][e], acc[i][c + 2][e], acc[i][c + 3][e]};
       }
   }
+};
+
+// The queries of a tile times a part of their prompt's state; one token: also their scores with what their sequences said.
+// Grid: (tile, column block), part, (prompt, head), the prompts with most sequences first.  Tiles of the same rows start together: they read them from memory once.
+template <typename R, int RT, bool ROT, int MODE>
+__global__ __launch_bounds__(256, RT == 4 && MODE == kHalf ? 1 : 2) void k_shared_pass(PassArgs g, Prompts pr) {
+  extern __shared__ __attribute__((aligned(16))) char s_dyn[];
+  __shared__ TileShared sh;
+  const unsigned tid = threadIdx.x, z = blockIdx.z / (unsigned)g.h, grp = pr.by_size[z], hh = blockIdx.z - z * g.h;
+  const unsigned tile = blockIdx.x / (unsigned)g.col_blocks, cb = blockIdx.x - tile * g.col_blocks, part = blockIdx.y;
+  const int first = pr.begin[grp], m0 = tile * 16 * RT, nb = min(16 * RT, (pr.begin[grp + 1] - first) * g.T - m0);
+  if (nb <= 0) return;
+  int my_len = -1;  // of sequence tid; one token's go to LDS with its activations on their way
+  float my_pos = 0.0f;
+  if ((int)tid < nb) {
+    const unsigned m = m0 + tid, b = first + (g.T == 1 ? m : m / (unsigned)g.T), t = g.T == 1 ? 0 : m % (unsigned)g.T;
+    sh.row[tid] = (b * g.h + hh) * g.T + t;
+    if (g.T == 1) {
+      const int len = g.lens[b];
+      my_len = valid_len(len, 1, g.longest, g.S) ? len : -1;
+      my_pos = (float)(g.positions ? (long)g.positions[b] : g.position);
+    }
+  }
+  if (!ROT && tid < 64) sh.len[tid] = my_len;
+  Product<R, RT, MODE> p(sh, s_dyn, g.rows);
+  const int col0 = cb * g.cg * p.kCols;
+  const int own0 = cb * nb / g.col_blocks, own1 = (cb + 1) * nb / g.col_blocks;  // the column blocks share the tile's sequences
+  int rb = part * g.per + min((int)part, g.longer);
+  const int end = rb + g.per + ((int)part < g.longer ? 1 : 0);
+#pragma unroll 1
+  for (; rb < end; ++rb) {
+    const int n0 = rb * g.rows;
+    if constexpr (ROT) p.turn_queries(g, (first + m0) * g.h + hh, nb, n0, own0, own1, my_len, my_pos);
+    else p.template load_queries<true>(g.q + n0, g.Nq, nb, g.rows, min(g.rows, g.Nq - n0));
+    p.multiply(static_cast<const R *>(g.rho) + (((long)grp * g.h + hh) * g.Nq + n0) * g.d, g.d, g.d, col0, g.cg, nb);
+    if (ROT || g.T == 1) p.template own_keys<ROT>(g, rb, own0, own1);
+    __syncthreads();  // the next block's list takes the place of what is still read here
+  }
+  p.finish(g.partial + (long)part * g.B * g.h * g.T * g.d, g.d, col0, g.cg, nb);
+}
+
+// Several tokens: the queries of a tile of a sequence's tokens times a part of its own keys.  Grid: (tile, column block), part,
+// (sequence, head).
+template <int RT>
+__global__ __launch_bounds__(256, 2) void k_suffix_scores(PassArgs g) {
+  extern __shared__ __attribute__((aligned(16))) char s_dyn[];
+  __shared__ TileShared sh;
+  const unsigned tid = threadIdx.x, bh = blockIdx.z, b = bh / (unsigned)g.h, part = blockIdx.y;
+  const unsigned tile = blockIdx.x / (unsigned)g.score_cols, cb = blockIdx.x - tile * g.score_cols;
+  const int len = g.lens[b], t0 = tile * 16 * RT, nb = min(16 * RT, g.T - t0), col0 = cb * g.cg * 64;
+  // keys behind the tile's last token are of no use to it
+  if (!valid_len(len, g.T, g.longest, g.S) || col0 >= len + t0 + nb - 1) return;
+  if (tid < 64) sh.row[tid] = (int)tid < nb ? bh * g.T + t0 + tid : 0;
+  Product<float, RT, RT == 4 ? kSplit : kF32> p(sh, s_dyn, g.rows);
+  int rb = part * g.score_per + min((int)part, g.score_longer);
+  const int end = rb + g.score_per + ((int)part < g.score_longer ? 1 : 0);
+#pragma unroll 1
+  for (; rb < end; ++rb) {
+    const int n0 = rb * g.rows;
+    p.template load_queries<false>(g.q + n0, g.Nq, nb, g.rows, min(g.rows, g.Nq - n0));
+    p.multiply(g.keys + ((long)bh * g.Nq + n0) * g.S, g.S, g.span, col0, g.cg, nb);
+    __syncthreads();
+  }
+  p.finish(g.score_parts + (long)part * g.B * g.h * g.T * g.span, g.span, col0, g.cg, nb);
 }
 
 struct JoinArgs {
@@ -247,86 +572,151 @@ struct JoinArgs {
   float *values;  // [B,S,d]
   float *out, *out_ln;
   const int32_t *lens;
-  int B, h, d, S, parts, blocks, longest;
+  int B, h, T, d, S, parts, blocks, longest;
+  long block_step, row_step;  // of the scores' parts
   bool decays;
 };
 
-// out = a^len * (the parts of q rho) + sum_s a^(len-s) score_s v_s, in the order of the parts and of the tokens; the value
-// of the new token goes to its place.
-template <bool LN>
-__global__ __launch_bounds__(256) void k_shared_join(JoinArgs g, HeadRates rates) {
-  __shared__ float s_sc[1024];
-  __shared__ float s_red[2][4];
-  const int bh = blockIdx.x, b = bh / g.h, hh = bh - b * g.h, tid = threadIdx.x;
-  const int len = g.lens[b];
-  const bool valid = valid_len(len, 1, g.longest, g.S);
-  const float ld = g.decays ? rates.log_decay[hh] : 0.0f;
-  float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  const long step = (long)g.B * g.h * g.d;
+// p[0] + p[step] + ... in order, eight of the n on their way at a time
+__device__ __forceinline__ float sum8(const float *p, long step, int n) {
+  float s = 0.0f;
+#pragma unroll 1
+  for (int q = 0; q < n; q += 8) {
+    float t[8];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int c = tid + j * 256;
-    if (c >= g.d) continue;
-    o[j] = bdh_sum_in_order(g.partial + (long)bh * g.d + c, step, g.parts);
-    if (g.decays) o[j] *= expf((float)len * ld);
-    if (hh == 0 && valid) g.values[((long)b * g.S + len) * g.d + c] = g.v[(long)b * g.d + c];
+    for (int u = 0; u < 8; ++u) t[u] = p[min(q + u, n - 1) * step];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s += q + u < n ? t[u] : 0.0f;
   }
-  if (valid)
-    for (int s0 = 0; s0 < len; s0 += 1024) {
-      const int n = min(1024, len - s0);
-      __syncthreads();
-      for (int s = tid; s < n; s += 256) {
-        float t = bdh_sum_in_order(g.score_parts + (long)bh * g.blocks * g.S + s0 + s, (long)g.S, g.blocks);
-        if (g.decays) t *= expf((float)(len - s0 - s) * ld);
-        s_sc[s] = t;
-      }
-      __syncthreads();
+  return s;
+}
+
+// out = a^k * (the parts of q rho) + sum_s a^(k-s) score_s v_s, in the order of the parts and of the tokens, for TT tokens of a
+// (sequence, head); a column's parts and values are dealt to as many threads as a workgroup of 1024 has for it.  One token: its
+// value goes to its place.
+template <int TT, bool LN>
+__global__ __launch_bounds__(1024) void k_shared_join(JoinArgs g, HeadRates rates) {
+  __shared__ float s_sc[TT][512];
+  __shared__ float s_sum[TT][1024];  // also the groups' sums of one token's scores [16][64]
+  __shared__ float s_red[2][16];
+  const int t0 = blockIdx.x * TT, bh = blockIdx.y, b = bh / g.h, hh = bh - b * g.h, tid = threadIdx.x;
+  const int len = g.lens[b], nt = min(TT, g.T - t0);
+  const bool valid = valid_len(len, g.T, g.longest, g.S);
+  const float ld = g.decays ? rates.log_decay[hh] : 0.0f;
+  const int dc = (g.d + 63) & ~63, slices = 1024 / dc, c = tid % dc, sl = tid / dc;
+  const bool mine = sl < slices && c < g.d;
+  const long row = (long)bh * g.T + t0, step = (long)g.B * g.h * g.T * g.d;
+  float o[TT];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int c = tid + j * 256;
-        if (c >= g.d) continue;
-        const float *v = g.values + ((long)b * g.S + s0) * g.d + c;
-        int s = 0;
-        for (; s + 8 <= n; s += 8) {
-          float t[8];
+  for (int t = 0; t < TT; ++t) o[t] = 0.0f;
+  if (mine && valid) {
+    const int p0 = sl * g.parts / slices, p1 = (sl + 1) * g.parts / slices;
+    if constexpr (TT == 1) {
+      o[0] = sum8(g.partial + p0 * step + row * g.d + c, step, p1 - p0);
+    } else {
+      const float *at = g.partial + p0 * step + row * g.d + c;
+#pragma unroll 4
+      for (int q = p0; q < p1; ++q, at += step)
 #pragma unroll
-          for (int u = 0; u < 8; ++u) t[u] = v[(long)(s + u) * g.d];
+        for (int t = 0; t < TT; ++t)
+          if (t < nt) o[t] += at[(long)t * g.d];
+    }
+    if (g.decays)
 #pragma unroll
-          for (int u = 0; u < 8; ++u) o[j] = fmaf(s_sc[s + u], t[u], o[j]);
+      for (int t = 0; t < TT; ++t) o[t] *= expf((float)(len + t0 + t) * ld);
+    if (g.T == 1 && hh == 0 && sl == 0) g.values[((long)b * g.S + len) * g.d + c] = g.v[(long)b * g.d + c];
+  }
+  const int end = valid ? len + t0 + nt - 1 : 0;  // the keys before the last token
+  for (int s0 = 0; s0 < end; s0 += 512) {
+    const int n = min(512, end - s0);
+    if (s0) __syncthreads();
+    if constexpr (TT == 1) {  // 64 scores at a time, a wavefront adds every sixteenth block's parts
+      for (int c0 = 0; c0 < n; c0 += 64) {
+        const int s = c0 + (tid & 63), wave = tid >> 6, mine_n = (g.blocks - wave + 15) / 16;
+        if (c0) __syncthreads();
+        s_sum[0][tid] = s < n && mine_n > 0 ? sum8(g.score_parts + row * g.row_step + s0 + s + wave * g.block_step, 16 * g.block_step, mine_n) : 0.0f;
+        __syncthreads();
+        if (tid < 64 && s < n) {
+          float w = 0.0f;
+#pragma unroll
+          for (int u = 0; u < 16; ++u) w += s_sum[0][u * 64 + tid];
+          if (g.decays) w *= expf((float)(len - s0 - s) * ld);
+          s_sc[0][s] = w;
         }
-        for (; s < n; ++s) o[j] = fmaf(s_sc[s], v[(long)s * g.d], o[j]);
+      }
+    } else {
+      for (int e = tid; e < TT * n; e += 1024) {
+        const int t = e / n, s = e - t * n, k = len + t0 + t;
+        float w = 0.0f;
+        if (t < nt && s0 + s < k) {
+          const float *at = g.score_parts + (row + t) * g.row_step + s0 + s;
+#pragma unroll 4
+          for (int q = 0; q < g.blocks; ++q) w += at[q * g.block_step];
+          if (g.decays) w *= expf((float)(k - s0 - s) * ld);
+        }
+        s_sc[t][s] = w;
       }
     }
-  if (!valid)
-    for (int j = 0; j < 4; ++j) o[j] = __uint_as_float(0x7fc00000u);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int c = tid + j * 256;
-    if (c < g.d) g.out[(long)bh * g.d + c] = o[j];
-  }
-  if (!LN) return;
-  auto block_sum = [&](float t, int slot) {
-    t = bdh_wave_sum(t);
-    if ((tid & 63) == 0) s_red[slot][tid >> 6] = t;
     __syncthreads();
-    return (s_red[slot][0] + s_red[slot][1]) + (s_red[slot][2] + s_red[slot][3]);
-  };
-  float sum = 0.0f;
-  for (int j = 0; j < 4; ++j) sum += tid + j * 256 < g.d ? o[j] : 0.0f;
-  const float mean = block_sum(sum, 0) / (float)g.d;
-  float sq = 0.0f;
-  for (int j = 0; j < 4; ++j) {
-    const float t = o[j] - mean;
-    sq += tid + j * 256 < g.d ? t * t : 0.0f;
+    if (mine) {
+      const float *v = g.values + ((long)b * g.S + s0) * g.d + c;
+      const int e1 = (sl + 1) * n / slices;
+      int s = sl * n / slices;
+      for (; s + 8 <= e1; s += 8) {
+        float y[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) y[u] = v[(long)(s + u) * g.d];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+#pragma unroll
+          for (int t = 0; t < TT; ++t) o[t] = fmaf(s_sc[t][s + u], y[u], o[t]);
+      }
+      for (; s < e1; ++s) {
+        const float y = v[(long)s * g.d];
+#pragma unroll
+        for (int t = 0; t < TT; ++t) o[t] = fmaf(s_sc[t][s], y, o[t]);
+      }
+    }
   }
-  const float den = sqrtf(block_sum(sq, 1) / (float)g.d + kLnEps);
-  for (int j = 0; j < 4; ++j) {
-    const int c = tid + j * 256;
-    if (c < g.d) g.out_ln[(long)bh * g.d + c] = (o[j] - mean) / den;
+  if (slices > 1) {
+#pragma unroll
+    for (int t = 0; t < TT; ++t) s_sum[t][tid] = o[t];
+    __syncthreads();
+    if (sl == 0)
+      for (int w = 1; w < slices; ++w)
+#pragma unroll
+        for (int t = 0; t < TT; ++t) o[t] += s_sum[t][w * dc + c];
+  }
+  if (!valid)
+#pragma unroll
+    for (int t = 0; t < TT; ++t) o[t] = __uint_as_float(0x7fc00000u);
+  const bool last = mine && sl == 0;
+#pragma unroll
+  for (int t = 0; t < TT; ++t)
+    if (last && t < nt) g.out[(row + t) * g.d + c] = o[t];
+  if (!LN) return;
+  // LayerNorm of the row (src/model/bdh.rs:359); the threads of slice 0 hold it, whole wavefronts of them
+  const int waves = dc / 64;
+#pragma unroll
+  for (int t = 0; t < TT; ++t) {
+    if (t >= nt) break;
+    auto row_sum = [&](float y, int slot) {
+      y = bdh_wave_sum(y);
+      if ((tid & 63) == 0) s_red[slot][tid >> 6] = y;
+      __syncthreads();
+      float sum = 0.0f;
+      for (int w = 0; w < waves; ++w) sum += s_red[slot][w];
+      return sum;
+    };
+    const float mean = row_sum(last ? o[t] : 0.0f, 0) / (float)g.d;
+    const float e = last ? o[t] - mean : 0.0f;
+    const float den = sqrtf(row_sum(e * e, 1) / (float)g.d + kLnEps);
+    if (last) g.out_ln[(row + t) * g.d + c] = e / den;
+    __syncthreads();
   }
 }
 
-// ---- several tokens per sequence --------------------------------------------------------------------------------------
+// ---- queries of several tokens ------------------------------------------------------------------------------------------
 
 struct AppendArgs {
   const float *x, *freqs, *v;
@@ -336,53 +726,70 @@ struct AppendArgs {
   int h, T, N, Nq, S, d, rotary, longest;
 };
 
-// Queries of all tokens [B,h,T,Nq], and their places among the keys: 32 tokens x 64 rows through LDS.
+// Queries of all tokens [B,h,T,Nq], and their places among the keys: 32 tokens x 64 neurons through LDS.  A thread turns the
+// two neurons of a pair for four tokens; with PoPE a neuron gives two rows.
 __global__ __launch_bounds__(256) void k_suffix_append(AppendArgs g) {
-  __shared__ float s_t[64][33];
+  __shared__ float s_t[128][33];
   const int n0 = blockIdx.x * 64, t0 = blockIdx.y * 32, bh = blockIdx.z, b = bh / g.h, tid = threadIdx.x;
-  const int len = g.lens[b];
-  const bool valid = valid_len(len, g.T, g.longest, g.S);
-  const int i = tid & 63, n = n0 + i;  // a row of the queries
-  const int src = n < g.N ? n : n - g.N;
-  const float f = g.rotary == BDH_ALIBI || n >= g.Nq ? 0.0f : g.freqs[src];
-  for (int t = tid >> 6; t < 32; t += 4) {
-    float q = 0.0f;
-    if (n < g.Nq && t0 + t < g.T) {
-      const float *x = g.x + ((long)bh * g.T + t0 + t) * g.N;
-      const float pos = (float)((g.positions ? (long)g.positions[b] : g.position) + t0 + t);
-      if (g.rotary == BDH_ALIBI) {
-        q = x[n];
-      } else if (g.rotary == BDH_ROPE) {
-        const float own = x[n], other = x[n ^ 1];
-        if (own != 0.0f || other != 0.0f) {
-          float s, c;
-          sincosf(rope_phase(pos, f), &s, &c);
-          const float a = own * c, r = ((n & 1) ? other : -other) * s;
-          q = a + r;
-        }
-      } else {
-        float s, c;
-        sincosf(rope_phase(pos, f), &s, &c);
-        q = softplus1(x[src]) * (n < g.N ? c : s);
-      }
-      if (g.q) g.q[((long)bh * g.T + t0 + t) * g.Nq + n] = q;
+  const int len = g.lens[b], i = 2 * (tid & 31), n = n0 + i, tq = tid >> 5;
+  const bool valid = valid_len(len, g.T, g.longest, g.S), in0 = n < g.N, in1 = n + 1 < g.N, pope = g.rotary == BDH_POPE;
+  const int c0 = min(n, g.N - 1), c1 = min(n + 1, g.N - 1);
+  const long pos0 = g.positions ? (long)g.positions[b] : g.position;
+  float x[4][2];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const float *at = g.x + ((long)bh * g.T + min(t0 + tq + 8 * u, g.T - 1)) * g.N;
+    x[u][0] = at[c0];
+    x[u][1] = at[c1];
+  }
+  const float f0 = g.rotary == BDH_ALIBI ? 0.0f : g.freqs[c0], f1 = g.rotary == BDH_ALIBI ? 0.0f : g.freqs[c1];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int t = t0 + tq + 8 * u;
+    const float pos = (float)(pos0 + t);
+    float q0 = x[u][0], q1 = x[u][1], r0 = 0.0f, r1 = 0.0f;
+    if (pope) {
+      float s, c, m = softplus1(q0);
+      sincos_turns(turns(pos, f0), s, c);
+      q0 = m * c;
+      r0 = m * s;
+      m = softplus1(q1);
+      sincos_turns(turns(pos, f1), s, c);
+      q1 = m * c;
+      r1 = m * s;
+    } else if (g.rotary == BDH_ROPE && (q0 != 0.0f || q1 != 0.0f)) {
+      rotate_pair(pos, f0, f1, q0, q1);
     }
-    s_t[i][t] = q;
+    if (t < g.T && g.q) {
+      float *q = g.q + ((long)bh * g.T + t) * g.Nq + n;
+      if (in1) *reinterpret_cast<f32x2u *>(q) = f32x2u{q0, q1};
+      else if (in0) q[0] = q0;
+      if (pope && in0) q[g.N] = r0;
+      if (pope && in1) q[g.N + 1] = r1;
+    }
+    s_t[i][tq + 8 * u] = q0;
+    s_t[i + 1][tq + 8 * u] = q1;
+    if (pope) {
+      s_t[64 + i][tq + 8 * u] = r0;
+      s_t[65 + i][tq + 8 * u] = r1;
+    }
   }
   __syncthreads();
-  if (valid)
-    for (int e = tid; e < 64 * 32; e += 256) {
-      const int t = e & 31, r = e >> 5;
-      if (t0 + t < g.T && n0 + r < g.Nq) g.keys[((long)bh * g.Nq + n0 + r) * g.S + len + t0 + t] = s_t[r][t];
-    }
-  if (valid && blockIdx.x == 0 && bh % g.h == 0) {
+  if (!valid) return;
+  const int t = t0 + (tid & 31);
+  for (int r = tid >> 5; r < (pope ? 128 : 64); r += 8) {
+    const int m = n0 + (r & 63);
+    if (t < g.T && m < g.N) g.keys[((long)bh * g.Nq + (r < 64 ? m : g.N + m)) * g.S + len + t] = s_t[r][tid & 31];
+  }
+  if (g.T > 1 && blockIdx.x == 0 && bh % g.h == 0) {
     const long last = min(t0 + 32, g.T);
     for (long e = (long)t0 * g.d + tid; e < last * g.d; e += 256)
       g.values[((long)b * g.S + len) * g.d + e] = g.v[(long)b * g.T * g.d + e];
   }
 }
 
-// Parts of a product added in order: dst [rows][cols] += nothing, = sum of parts [ks][rows][cols] (4 columns a thread).
+// ---- many tokens: dense products ----------------------------------------------------------------------------------------
+
 struct MaskArgs {
   const float *score_parts;  // [ks][B*h][T][span]
   float *scores;             // [B*h][T][lds]
@@ -528,70 +935,36 @@ int check_prompts(bdh_ctx *ctx, int G, const int32_t *counts_host, int B, Prompt
     pr.begin[i + 1] = (int)sum;
   }
   if (sum != B) return bdh_fail(ctx, BDH_E_INVAL, "the prompts' sequences are not the batch of %d", B);
+  for (int i = 0; i < G; ++i) pr.by_size[i] = (unsigned char)i;
+  std::stable_sort(pr.by_size, pr.by_size + G, [&](int a, int b) { return pr.begin[a + 1] - pr.begin[a] > pr.begin[b + 1] - pr.begin[b]; });
   return BDH_OK;
 }
 
 }  // namespace
 
-int bdh_launch_shared_steps(bdh_ctx *ctx, const SharedStepParams &p) {
-  Prompts pr;
-  int rc = check_prompts(ctx, p.G, p.counts_host, p.B, pr);
-  if (rc != BDH_OK) return rc;
+namespace {
+
+template <typename R, bool ROT, int MODE, int MODE4>
+const void *pass_kernel(int rt) {
+  return rt == 1   ? reinterpret_cast<const void *>(k_shared_pass<R, 1, ROT, MODE>)
+         : rt == 2 ? reinterpret_cast<const void *>(k_shared_pass<R, 2, ROT, MODE>)
+                   : reinterpret_cast<const void *>(k_shared_pass<R, 4, ROT, MODE4>);
+}
+
+int launch_pass(bdh_ctx *ctx, const void *kernel, const char *name, dim3 grid, size_t lds, void **args) {
+  if (lds > 48 * 1024) BDH_HIP_CHECK(ctx, hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+  const hipError_t e = hipLaunchKernel(kernel, grid, dim3(256), args, lds, ctx->stream);
+  if (e != hipSuccess) return bdh_fail(ctx, BDH_E_HIP, "launch of %s failed: %s", name, hipGetErrorString(e));
+  return BDH_OK;
+}
+
+int launch_dense(bdh_ctx *ctx, const SharedStepParams &p, const Prompts &pr, const HeadRates &rates, int longest) {
   const int B = p.B, h = p.h, T = p.T, N = p.N, d = p.d, S = p.capacity;
   const int Nq = p.rotary == BDH_POPE ? 2 * N : N;
   const bool alibi = p.rotary == BDH_ALIBI;
   const long BH = (long)B * h;
-  HeadRates rates{};
-  if (alibi)
-    for (int i = 0; i < h; ++i) rates.log_decay[i] = bdh_log_decay(p.slopes_host[i]);
-  const int longest = p.longest < 0 ? S - T : p.longest;
-  if (T == 1) {
-    const int pairs = p.rotary == BDH_POPE ? N : (N + 1) / 2, blocks = (pairs + 255) / 256;
-    int most = 1;
-    for (int i = 0; i < p.G; ++i) most = std::max(most, pr.begin[i + 1] - pr.begin[i]);
-    const int rt = most <= 16 ? 1 : most <= 32 ? 2 : 4;
-    int tiles = 0;
-    for (int i = 0; i < p.G; ++i) tiles += (pr.begin[i + 1] - pr.begin[i] + 16 * rt - 1) / (16 * rt);
-    // rows a workgroup: as many as leave two workgroups for every CU
-    int rows = 256;
-    while (rows > 64 && (long)((Nq + rows - 1) / rows) * h * tiles < 2L * ctx->n_cu) rows /= 2;
-    const int groups = (d + 63) / 64, kw = groups == 1 ? 4 : groups == 2 ? 2 : 1;
-    const int nblk = (Nq + rows - 1) / rows, parts = nblk * kw;
-    if (tiles > 65535) return bdh_fail(ctx, BDH_E_SHAPE, "too many sequences");
-    const size_t q_bytes = bdh_align_up(sizeof(float) * (size_t)BH * Nq, 256);
-    const size_t sc_bytes = bdh_align_up(sizeof(float) * (size_t)BH * blocks * S, 256);
-    const size_t pt_bytes = sizeof(float) * (size_t)BH * parts * d;
-    rc = bdh_ws_reserve(ctx, q_bytes + sc_bytes + pt_bytes);
-    if (rc != BDH_OK) return rc;
-    char *ws = static_cast<char *>(ctx->ws);
-    float *q = reinterpret_cast<float *>(ws), *score_parts = reinterpret_cast<float *>(ws + q_bytes);
-    float *partial = reinterpret_cast<float *>(ws + q_bytes + sc_bytes);
-    const SuffixArgs sa{p.x, p.freqs, q, p.keys, score_parts, p.lens_dev, p.positions_dev, (long)p.position, h, N, Nq, S,
-                        p.rotary, blocks, longest};
-    hipLaunchKernelGGL(k_suffix_scores, dim3(blocks, (unsigned)BH), dim3(256), 0, ctx->stream, sa);
-    BDH_LAUNCH_CHECK(ctx, "k_suffix_scores");
-    const ReadArgs ra{q, p.rho, partial, B, h, Nq, d, rows, kw};
-    const dim3 grid(nblk, h, tiles);
-    const size_t lds = sizeof(float) * 16 * rt * (rows + 4);
-    const bool wide = p.rho_dtype == BDH_F32;
-    auto *kernel = rt == 1 ? (wide ? k_shared_read<float, 1> : k_shared_read<unsigned short, 1>)
-                   : rt == 2 ? (wide ? k_shared_read<float, 2> : k_shared_read<unsigned short, 2>)
-                             : (wide ? k_shared_read<float, 4> : k_shared_read<unsigned short, 4>);
-    if (lds > 60 * 1024)
-      BDH_HIP_CHECK(ctx, hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    hipLaunchKernelGGL(kernel, grid, dim3(256), lds, ctx->stream, ra, pr);
-    BDH_LAUNCH_CHECK(ctx, "k_shared_read");
-    const JoinArgs ja{partial, score_parts, p.v, p.values, p.out, p.out_ln, p.lens_dev, B, h, d, S, parts, blocks, longest, alibi};
-    if (p.out_ln)
-      hipLaunchKernelGGL(k_shared_join<true>, dim3((unsigned)BH), dim3(256), 0, ctx->stream, ja, rates);
-    else
-      hipLaunchKernelGGL(k_shared_join<false>, dim3((unsigned)BH), dim3(256), 0, ctx->stream, ja, rates);
-    BDH_LAUNCH_CHECK(ctx, "k_shared_join");
-    return BDH_OK;
-  }
-  // many tokens: the queries once, then three dense products on the matrix cores
+  int rc = BDH_OK;
   const int span = std::min(S, longest + T), lds = (span + 3) & ~3;
-  if (BH * T > 0x7fffffffL / 4) return bdh_fail(ctx, BDH_E_SHAPE, "B*h*T too large");
   GemmF32 o, s, w;
   bool even = true;  // every prompt has as many sequences: one launch
   for (int i = 1; i < p.G; ++i) even &= pr.begin[i + 1] - pr.begin[i] == pr.begin[1];
@@ -630,7 +1003,7 @@ int bdh_launch_shared_steps(bdh_ctx *ctx, const SharedStepParams &p) {
   }
   const AppendArgs aa{p.x, p.freqs, p.v, q, p.keys, p.values, p.lens_dev, p.positions_dev, (long)p.position, h, T, N, Nq, S, d,
                       p.rotary, longest};
-  hipLaunchKernelGGL(k_suffix_append, dim3((Nq + 63) / 64, (T + 31) / 32, (unsigned)BH), dim3(256), 0, ctx->stream, aa);
+  hipLaunchKernelGGL(k_suffix_append, dim3((N + 63) / 64, (T + 31) / 32, (unsigned)BH), dim3(256), 0, ctx->stream, aa);
   BDH_LAUNCH_CHECK(ctx, "k_suffix_append");
   const float *queries = alibi ? p.x : q;
   for (int i = 0; i < launches; ++i) {
@@ -655,6 +1028,111 @@ int bdh_launch_shared_steps(bdh_ctx *ctx, const SharedStepParams &p) {
   rc = bdh_launch_gemm_f32(ctx, w, false, true, pw, nullptr);
   if (rc != BDH_OK) return rc;
   if (p.out_ln) return bdh_launch_layer_norm_rows(ctx, (int64_t)BH * T, d, p.out, p.out_ln);
+  return BDH_OK;
+}
+
+}  // namespace
+
+int bdh_launch_shared_steps(bdh_ctx *ctx, const SharedStepParams &p) {
+  Prompts pr;
+  int rc = check_prompts(ctx, p.G, p.counts_host, p.B, pr);
+  if (rc != BDH_OK) return rc;
+  const int B = p.B, h = p.h, T = p.T, N = p.N, d = p.d, S = p.capacity;
+  const int Nq = p.rotary == BDH_POPE ? 2 * N : N;
+  const bool alibi = p.rotary == BDH_ALIBI;
+  const long BH = (long)B * h;
+  HeadRates rates{};
+  if (alibi)
+    for (int i = 0; i < h; ++i) rates.log_decay[i] = bdh_log_decay(p.slopes_host[i]);
+  const int longest = p.longest < 0 ? S - T : p.longest;
+  if (BH * T > 0x7fffffffL / 1024) return bdh_fail(ctx, BDH_E_SHAPE, "B*h*T too large");
+  if (T >= kDenseTokens) return launch_dense(ctx, p, pr, rates, longest);
+  const bool rot = T == 1 && p.rotary != BDH_POPE;        // the queries are made where they are used
+  const bool half = p.rho_dtype == BDH_BF16 && d % 8 == 0;
+  PassArgs g{};
+  g.x = p.x; g.freqs = p.freqs; g.lens = p.lens_dev; g.positions = p.positions_dev; g.position = (long)p.position;
+  g.rho = p.rho; g.keys = p.keys;
+  g.B = B; g.h = h; g.T = T; g.N = N; g.Nq = Nq; g.d = d; g.S = S; g.rotary = p.rotary; g.longest = longest;
+  long most = 1;  // queries of a prompt
+  for (int i = 0; i < p.G; ++i) most = std::max(most, (long)(pr.begin[i + 1] - pr.begin[i]) * T);
+  const int rt = most <= 16 ? 1 : most <= 32 ? 2 : 4;
+  const long tiles = (most + 16 * rt - 1) / (16 * rt);
+  // rows and columns of a workgroup: as many as leave two workgroups for every CU
+  const int group = half ? 128 : 64, groups = (d + group - 1) / group;
+  g.rows = rt == 4 ? 128 : kRowsMost;
+  g.cg = groups >= 4 ? 4 : groups >= 2 ? 2 : 1;
+  auto count = [&] {
+    g.row_blocks = (Nq + g.rows - 1) / g.rows;
+    g.col_blocks = (groups + g.cg - 1) / g.cg;
+    return (long)p.G * h * g.row_blocks * g.col_blocks * tiles;
+  };
+  while (count() < 2L * ctx->n_cu && (g.cg > 1 || g.rows > 128)) {
+    if (g.rows > 128) g.rows /= 2;
+    else g.cg /= 2;
+  }
+  // more than fit the chip at once: blocks of rows one after the other in a workgroup, so that all run together; or twice as many
+  // where the prompts' workgroups take their own times
+  bool even = true;
+  for (int i = 1; i < p.G; ++i) even &= pr.begin[i + 1] - pr.begin[i] == pr.begin[1];
+  const long slots = (long)ctx->n_cu * (half || rt == 4 ? 2 : 3) * (even ? 1 : 2);
+  auto deal = [&](long others, int &parts, int &per, int &longer) {
+    parts = (int)std::max<long>(1, std::min<long>(g.row_blocks, slots / std::max<long>(1, others)));
+    per = g.row_blocks / parts;
+    longer = g.row_blocks % parts;
+  };
+  deal(count() / g.row_blocks, g.parts, g.per, g.longer);
+  g.span = (std::min(S, longest + T) + 3) & ~3;
+  g.score_parts_n = g.row_blocks;
+  const long score_tiles = (T + 16 * rt - 1) / (16 * rt);
+  if (T > 1) {
+    g.score_cols = ((g.span + 63) / 64 + g.cg - 1) / g.cg;
+    deal(BH * g.score_cols * score_tiles, g.score_parts_n, g.score_per, g.score_longer);
+  }
+  if (g.row_blocks > 65535 || (long)p.G * h > 65535 || (long)h * Nq * 64 * 4 > 0xffffffffL)
+    return bdh_fail(ctx, BDH_E_SHAPE, "h * Nq %ld too large", (long)h * Nq);
+  const size_t q_bytes = rot || alibi ? 0 : bdh_align_up(sizeof(float) * (size_t)BH * T * Nq, 256);
+  const size_t pt_bytes = bdh_align_up(sizeof(float) * (size_t)g.parts * BH * T * d, 256);
+  const size_t sc_bytes = sizeof(float) * (size_t)g.score_parts_n * BH * T * g.span;
+  rc = bdh_ws_reserve(ctx, q_bytes + pt_bytes + sc_bytes);
+  if (rc != BDH_OK) return rc;
+  char *ws = static_cast<char *>(ctx->ws);
+  g.partial = reinterpret_cast<float *>(ws + q_bytes);
+  g.score_parts = reinterpret_cast<float *>(ws + q_bytes + pt_bytes);
+  g.q = q_bytes ? reinterpret_cast<float *>(ws) : p.x;
+  if (!rot) {
+    const AppendArgs aa{p.x, p.freqs, p.v, q_bytes ? reinterpret_cast<float *>(ws) : nullptr, p.keys, p.values, p.lens_dev,
+                        p.positions_dev, (long)p.position, h, T, N, Nq, S, d, p.rotary, longest};
+    hipLaunchKernelGGL(k_suffix_append, dim3((N + 63) / 64, (T + 31) / 32, (unsigned)BH), dim3(256), 0, ctx->stream, aa);
+    BDH_LAUNCH_CHECK(ctx, "k_suffix_append");
+  }
+  // the queries, or the sums of the four wavefronts
+  auto room = [&](bool split, int cols) {
+    return std::max((size_t)16 * rt * (split ? 6 * (g.rows + 8) : 4 * (g.rows + 4)), g.cg == 4 ? 0 : 4 * sizeof(float) * 16 * rt * cols);
+  };
+  using h16 = unsigned short;
+  const void *kernel = p.rho_dtype == BDH_F32 ? (rot ? pass_kernel<float, true, kF32, kSplit>(rt) : pass_kernel<float, false, kF32, kSplit>(rt))
+                       : half                 ? (rot ? pass_kernel<h16, true, kHalf, kHalf>(rt) : pass_kernel<h16, false, kHalf, kHalf>(rt))
+                                              : (rot ? pass_kernel<h16, true, kF32, kF32>(rt) : pass_kernel<h16, false, kF32, kF32>(rt));
+  void *args[] = {&g, &pr};
+  rc = launch_pass(ctx, kernel, "k_shared_pass", dim3((unsigned)(tiles * g.col_blocks), g.parts, p.G * h),
+                   room(half || (rt == 4 && p.rho_dtype == BDH_F32), group), args);
+  if (rc != BDH_OK) return rc;
+  if (T > 1) {
+    const void *scores = rt == 1   ? reinterpret_cast<const void *>(k_suffix_scores<1>)
+                         : rt == 2 ? reinterpret_cast<const void *>(k_suffix_scores<2>)
+                                   : reinterpret_cast<const void *>(k_suffix_scores<4>);
+    rc = launch_pass(ctx, scores, "k_suffix_scores", dim3((unsigned)(score_tiles * g.score_cols), g.score_parts_n, (unsigned)BH),
+                     room(rt == 4, 64), args);
+    if (rc != BDH_OK) return rc;
+  }
+  const long rows = BH * T;
+  const JoinArgs ja{g.partial, g.score_parts, p.v, p.values, p.out, p.out_ln, p.lens_dev, B, h, T, d, S, g.parts, g.score_parts_n,
+                    longest, rows * g.span, (long)g.span, alibi};
+  const dim3 grid(T == 1 ? 1 : (T + 3) / 4, (unsigned)BH);
+  auto *join = T == 1 ? (p.out_ln ? k_shared_join<1, true> : k_shared_join<1, false>)
+                      : (p.out_ln ? k_shared_join<4, true> : k_shared_join<4, false>);
+  hipLaunchKernelGGL(join, grid, dim3(1024), 0, ctx->stream, ja, rates);
+  BDH_LAUNCH_CHECK(ctx, "k_shared_join");
   return BDH_OK;
 }
 

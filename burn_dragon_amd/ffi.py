@@ -196,9 +196,10 @@ class Context:
         if self._follow and getattr(self, "handle", None) and not sys.is_finalizing():
             import torch
 
-            cur = torch.cuda.current_stream(self.device_id)
-            current = cur.cuda_stream
+            # the raw handle: a Stream object costs a microsecond, and this runs before every call
+            current = torch._C._cuda_getCurrentRawStream(self.device_id)
             if current != self._stream:
+                cur = torch.cuda.current_stream(self.device_id)
                 # The context's workspace and the model's activation scratch are shared by every call: work queued on
                 # the old stream may still use them, so the new stream waits for it (not under graph capture, where
                 # an event recorded outside the capture must not be waited on; a capture orders its own work).

@@ -4,7 +4,7 @@ what serving does with them: calls in a row, graphs, other streams.
 
 Tolerances.  With u = 2^-24 (f32 rounds to nearest), every term q_n rho_nc and (q.k_s) v_sc of an output carries the
 roundings of its query and key (the angle and its sine: 8 steps, softplus 4 more; two factors: 24 in all), of its
-decay (8), of its products (3) and of the additions it passes through.  One token: at most 256 in a chain of a block of
+decay (8), of its products (3) and of the additions it passes through.  One token: at most Nq in the chain of a workgroup's
 rows, `parts` and `blocks` <= Nq / 64 + 1 of them, 48 in a block's score, and len for the values.  Many tokens: every sum
 in some order of at most Nq, then span.  So |error| <= u * depth * (sum of the terms' magnitudes), depth as written in
 `_depth`; the magnitudes come from the same definition with absolute values."""
@@ -111,7 +111,7 @@ class Case:
 def _depth(c):
     extra = 24 + 8 + 3
     if c.T == 1:
-        return extra + 256 + 2 * (c.Nq // 64 + 5) + 48 + int(c.lens.max())
+        return extra + c.Nq + 2 * (c.Nq // 64 + 5) + 48 + int(c.lens.max())
     return extra + c.Nq + int(c.lens.max()) + c.T
 
 
@@ -150,6 +150,12 @@ READ = [
     ((2,), 1, 300, 1024, 8, (6, 1), 1, "pope", BF16),
     ((2,), 1, 8, 8, 1100, (1060, 1099), 1, "rope", F32),
     ((3,), 5, 1030, 320, 20, (13, 2, 19), 1, "rope", BF16),
+    # more blocks of rows than workgroups: several blocks one after the other
+    ((20, 3), 16, 16384, 8, 8, (3, 0, 7), 1, "rope", BF16),
+    ((18,), 16, 16384, 4, 8, (5, 1), 1, "rope", F32),
+    ((40,), 8, 16384, 8, 4, (3, 2), 1, "alibi", F32),
+    ((3,), 16, 8192, 12, 8, (7, 2), 1, "pope", BF16),
+    ((9, 2), 16, 8192, 16, 16, (3, 5), 7, "rope", BF16),
     ((1,), 1, 2, 4, 4, (0, 2), 2, "rope", F32),
     ((4, 2), 2, 130, 68, 64, (0, 13, 7), 45, "rope", F32),
     ((3, 3), 2, 64, 128, 40, (8, 1), 32, "alibi", F32),
