@@ -838,80 +838,146 @@ struct ForkArgs {
   const float *keys, *values;
   const int32_t *lens;
   int B, h, Nq, d, S, longest;
+  int rows, row_blocks, col_blocks;  // rows a workgroup makes
   bool decays;
 };
 
 __device__ __forceinline__ void store_state4(float *p, f32x4 v) { *reinterpret_cast<f32x4 *>(p) = v; }
 __device__ __forceinline__ void store_state4(unsigned short *p, f32x4 v) {
-  uint2 o;
-  o.x = bdh_bf16_rne(v.x) | (bdh_bf16_rne(v.y) << 16);
-  o.y = bdh_bf16_rne(v.z) | (bdh_bf16_rne(v.w) << 16);
-  *reinterpret_cast<uint2 *>(p) = o;
+  *reinterpret_cast<uint2 *>(p) = make_uint2(pack_bf16_rne(v.x, v.y), pack_bf16_rne(v.z, v.w));
 }
 
-// A wavefront makes 64 rows x 64 columns of one (sequence, head): a^len rho + sum_s a^(len-s) k_s (x) v_s, 16 tokens at a time
-// on v_mfma_f32_16x16x4_f32.
-template <typename R>
-__global__ __launch_bounds__(256) void k_shared_fork(ForkArgs g, Prompts pr, HeadRates rates) {
-  constexpr int RT = 4;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, k4 = lane >> 4, li = lane & 15;
-  const int bh = blockIdx.z, b = bh / g.h, hh = bh - b * g.h;
-  const int col = blockIdx.y * 64 + li * 4, n0 = (blockIdx.x * 4 + wave) * 64;
-  if (n0 >= g.Nq) return;
+// a^len rho + sum_s a^(len-s) k_s (x) v_s for `rows` rows and CB columns of one (sequence, head).  The (decayed) values stand in
+// LDS as three bf16 terms, token by token of a column, TK tokens at a time; a wavefront makes RW rows at a time: it takes the
+// keys of 32 tokens as they lie in memory, splits them in registers and multiplies six of the nine products of terms on
+// v_mfma_f32_16x16x32_bf16 (what is left out is below 2^-23 of a product), on top of the prompt's row.  Bound by the bytes of
+// the states written and the keys read; columns are dealt so that a lane has four neighbouring ones.
+template <typename R, int CB>
+__global__ __launch_bounds__(512, 2) void k_shared_fork(ForkArgs g, Prompts pr, HeadRates rates) {
+  constexpr int TK = 64 * 256 / CB, LDV = TK + 8, RT = 256 / CB, RW = 16 * RT, CT = CB / 16;
+  extern __shared__ __attribute__((aligned(16))) char s_dyn[];
+  unsigned short *s_v = reinterpret_cast<unsigned short *>(s_dyn);  // [3][CB][LDV]
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_of_thread(), k4 = lane >> 4, li = lane & 15;
+  const unsigned rb = blockIdx.x / (unsigned)g.col_blocks, cb = blockIdx.x - rb * g.col_blocks, b = blockIdx.y, hh = blockIdx.z;
   int grp = 0;
-  while (grp + 1 < pr.G && b >= pr.begin[grp + 1]) ++grp;
+  while (grp + 1 < pr.G && (int)b >= pr.begin[grp + 1]) ++grp;
   const int len = g.lens[b];
   const bool valid = len >= 0 && len <= g.longest && len <= g.S;
-  const float ld = g.decays ? rates.log_decay[hh] : 0.0f, base = g.decays ? expf((float)len * ld) : 1.0f;
+  const int end = valid ? len : 0, first = rb * g.rows, last = min(first + g.rows, g.Nq), col0 = cb * CB;
+  const float ld = g.decays ? rates.log_decay[hh] : 0.0f;
+  const float base = !valid ? __uint_as_float(0x7fc00000u) : g.decays ? expf((float)len * ld) : 1.0f;
   const R *rho = static_cast<const R *>(g.rho) + ((long)grp * g.h + hh) * g.Nq * g.d;
-  R *out = static_cast<R *>(g.out) + (long)bh * g.Nq * g.d;
-  const float *K = g.keys + (long)bh * g.Nq * g.S, *V = g.values + (long)b * g.S * g.d;
-  const bool inside = col < g.d;
-  f32x4 acc[RT][4];
+  const long bh = (long)b * g.h + hh;
+  R *out = static_cast<R *>(g.out) + bh * g.Nq * g.d;
+  const float *K = g.keys + bh * g.Nq * g.S, *V = g.values + (long)b * g.S * g.d;
+  // values of tokens s0 .. s0 + TK - 1; column 64 j + 4 i + c of the block stands at place 64 j + 16 c + i
+  auto stage = [&](int s0) {
+    const int tokens = min((end - s0 + 31) & ~31, TK);
+    for (int e = tid; e < tokens / 8 * CB; e += 512) {
+      const int c = e % CB, t = e / CB * 8, place = (c & ~63) + ((c & 3) << 4) + ((c >> 2) & 15);
+      float v[8];
 #pragma unroll
-  for (int i = 0; i < RT; ++i)
+      for (int u = 0; u < 8; ++u) v[u] = V[(long)min(s0 + t + u, end - 1) * g.d + min(col0 + c, g.d - 1)];
+      u32x4 o[3];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int n = n0 + i * 16 + k4 * 4 + e;
-      f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (n < g.Nq && inside) v = load_state4(rho + (long)n * g.d + col);
+      for (int u = 0; u < 8; u += 2) {
+        float x[2];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) acc[i][c][e] = v[c] * base;
+        for (int w = 0; w < 2; ++w) {
+          const int s = s0 + t + u + w;
+          x[w] = s < end && col0 + c < g.d ? (g.decays ? v[u + w] * expf((float)(len - s) * ld) : v[u + w]) : 0.0f;
+        }
+        o[0][u / 2] = pack_bf16_rne(x[0], x[1]);
+        const float r0 = x[0] - __uint_as_float(o[0][u / 2] << 16), r1 = x[1] - __uint_as_float(o[0][u / 2] & 0xffff0000u);
+        o[1][u / 2] = pack_bf16_rne(r0, r1);
+        o[2][u / 2] = pack_bf16_rne(r0 - __uint_as_float(o[1][u / 2] << 16), r1 - __uint_as_float(o[1][u / 2] & 0xffff0000u));
+      }
+#pragma unroll
+      for (int q = 0; q < 3; ++q) *reinterpret_cast<u32x4 *>(s_v + (q * CB + place) * LDV + t) = o[q];
     }
-  const int end = valid ? len : 0;
-  for (int s0 = 0; s0 < end; s0 += 16) {
-    const int s = s0 + k4 * 4;  // this lane's four tokens
-    f32x4 bv[4], av[RT];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      bv[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      if (s + j < end && inside) bv[j] = *reinterpret_cast<const f32x4 *>(V + (long)(s + j) * g.d + col);
-      if (g.decays) bv[j] *= expf((float)(len - s - j) * ld);
-    }
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      const int n = n0 + i * 16 + li;
-      av[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      if (n < g.Nq && s < end) av[i] = *reinterpret_cast<const f32x4 *>(K + (long)n * g.S + s);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) av[i][j] = s + j < end ? av[i][j] : 0.0f;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[i][j], bv[j][c], acc[i][c], 0, 0, 0);
+  };
+  if (end > 0 && end <= TK) {
+    stage(0);
+    __syncthreads();
   }
+#pragma unroll 1
+  for (int m0 = first; m0 < last; m0 += 8 * RW) {
+    const int n0 = m0 + wave * RW;
+    f32x4 acc[RT][CT];
 #pragma unroll
-  for (int i = 0; i < RT; ++i)
+    for (int i = 0; i < RT; ++i)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int n = n0 + i * 16 + k4 * 4 + e;
-      f32x4 v = {acc[i][0][e], acc[i][1][e], acc[i][2][e], acc[i][3][e]};
-      if (!valid) v = __uint_as_float(0x7fc00000u) - f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      if (n < g.Nq && inside) store_state4(out + (long)n * g.d + col, v);
+      for (int j = 0; j < CT; j += 4)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int n = min(n0 + i * 16 + k4 * 4 + e, g.Nq - 1), col = col0 + j * 16 + li * 4;
+          const f32x4 v = load_state4(rho + (long)n * g.d + (col < g.d ? col : 0));
+#pragma unroll
+          for (int c = 0; c < 4; ++c) acc[i][j + c][e] = v[c] * base;
+        }
+#pragma unroll 1
+    for (int s0 = 0; s0 < end; s0 += TK) {
+      if (end > TK) {
+        __syncthreads();
+        stage(s0);
+        __syncthreads();
+      }
+      const int stop = min(end - s0, TK);
+#pragma unroll 1
+      for (int t = 0; t < stop; t += 32) {
+        bf16x8 a[RT][3];
+        f32x4 k[RT][2];
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int n = min(n0 + i * 16 + li, g.Nq - 1), s = s0 + t + k4 * 8 + u * 4;
+            k[i][u] = *reinterpret_cast<const f32x4 *>(K + (long)n * g.S + (s < end ? s : 0));
+            if (s >= end) k[i][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          }
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+          u32x4 o[3];
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            const float e0 = k[i][m >> 1][(m & 1) * 2], e1 = k[i][m >> 1][(m & 1) * 2 + 1];
+            o[0][m] = pack_bf16_rne(e0, e1);
+            const float r0 = e0 - __uint_as_float(o[0][m] << 16), r1 = e1 - __uint_as_float(o[0][m] & 0xffff0000u);
+            o[1][m] = pack_bf16_rne(r0, r1);
+            o[2][m] = pack_bf16_rne(r0 - __uint_as_float(o[1][m] << 16), r1 - __uint_as_float(o[1][m] & 0xffff0000u));
+          }
+#pragma unroll
+          for (int q = 0; q < 3; ++q) a[i][q] = __builtin_bit_cast(bf16x8, o[q]);
+        }
+#pragma unroll
+        for (int j = 0; j < CT; ++j) {
+          bf16x8 v[3];
+#pragma unroll
+          for (int q = 0; q < 3; ++q) v[q] = *reinterpret_cast<const bf16x8 *>(s_v + (q * CB + j * 16 + li) * LDV + t + k4 * 8);
+#pragma unroll
+          for (int i = 0; i < RT; ++i) {
+            auto mac = [&](int ta, int tb) { acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i][ta], v[tb], acc[i][j], 0, 0, 0); };
+            mac(0, 2);
+            mac(1, 1);
+            mac(2, 0);
+            mac(0, 1);
+            mac(1, 0);
+            mac(0, 0);
+          }
+        }
+      }
     }
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int j = 0; j < CT; j += 4)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int n = n0 + i * 16 + k4 * 4 + e, col = col0 + j * 16 + li * 4;
+          if (n < last && col < g.d)
+            store_state4(out + (long)n * g.d + col, f32x4{acc[i][j][e], acc[i][j + 1][e], acc[i][j + 2][e], acc[i][j + 3][e]});
+        }
+  }
 }
 
 bool disjoint(const void *a, size_t na, const void *b, size_t nb) {
@@ -1208,13 +1274,23 @@ int bdh_shared_prefix_fork(bdh_ctx *ctx, int G, const int32_t *counts_host, int 
     else bdh_default_alibi_slopes(h, slopes);
     for (int i = 0; i < h; ++i) rates.log_decay[i] = bdh_log_decay(slopes[i]);
   }
-  const ForkArgs g{rho, rho_out, keys, values, lens_dev, B, h, Nq, d, capacity, longest < 0 ? capacity : longest, rotary == BDH_ALIBI};
-  const dim3 grid((Nq + 255) / 256, (d + 63) / 64, B * h);
-  if (rho_dtype == BDH_F32)
-    hipLaunchKernelGGL(k_shared_fork<float>, grid, dim3(256), 0, ctx->stream, g, pr, rates);
-  else
-    hipLaunchKernelGGL(k_shared_fork<unsigned short>, grid, dim3(256), 0, ctx->stream, g, pr, rates);
-  BDH_LAUNCH_CHECK(ctx, "k_shared_fork");
+  ForkArgs g{rho, rho_out, keys, values, lens_dev, B, h, Nq, d, capacity, longest < 0 ? capacity : longest, 0, 0, 0, rotary == BDH_ALIBI};
+  // columns of a workgroup: as many as leave its LDS room for every token; a wavefront's tile is 16 x 256, 32 x 128 or 64 x 64
+  const int cols = g.longest <= 64 && d > 128 ? 256 : g.longest <= 128 && d > 64 ? 128 : 64;
+  const int tile = 8 * 16 * 256 / cols;  // rows that the eight wavefronts make at a time
+  g.col_blocks = (d + cols - 1) / cols;
+  g.rows = tile;
+  while ((long)B * h * g.col_blocks * ((Nq + 2 * g.rows - 1) / (2 * g.rows)) >= 4L * ctx->n_cu) g.rows *= 2;
+  g.row_blocks = (Nq + g.rows - 1) / g.rows;
+  const size_t lds = (size_t)6 * cols * (64 * 256 / cols + 8);
+  using h16 = unsigned short;
+  const bool wide = rho_dtype == BDH_F32;
+  const void *kernel = cols == 256   ? (wide ? reinterpret_cast<const void *>(k_shared_fork<float, 256>) : reinterpret_cast<const void *>(k_shared_fork<h16, 256>))
+                       : cols == 128 ? (wide ? reinterpret_cast<const void *>(k_shared_fork<float, 128>) : reinterpret_cast<const void *>(k_shared_fork<h16, 128>))
+                                     : (wide ? reinterpret_cast<const void *>(k_shared_fork<float, 64>) : reinterpret_cast<const void *>(k_shared_fork<h16, 64>));
+  BDH_HIP_CHECK(ctx, hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+  void *args[] = {&g, &pr, &rates};
+  BDH_HIP_CHECK(ctx, hipLaunchKernel(kernel, dim3(g.row_blocks * g.col_blocks, B, h), dim3(512), args, lds, ctx->stream));
   return BDH_OK;
 }
 

@@ -16,7 +16,7 @@ struct SlotBuffer {
   long first;                 // number of this buffer's first task
   long chunks;                // tasks a layer
   int outer, unit;
-  unsigned chunk;             // pieces a task takes of each slot
+  unsigned chunk, shift;      // pieces a task takes of each slot (in place: 2^shift)
 };
 struct SlotArgs {
   SlotBuffer buf[kMaxBuffers];
@@ -31,23 +31,28 @@ __device__ __forceinline__ const SlotBuffer &buffer_of(const SlotArgs &g, long t
   return g.buf[i];
 }
 
-// One chunk of every destination slot: a source is read once for a run of slots that take it.
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+// One chunk of every destination slot: a source is read once for a run of slots that take it.  What is written passes the
+// caches by (a state is larger than they are).
 template <typename P>
 __device__ __forceinline__ void copy_chunk(const SlotArgs &g, const SlotBuffer &f, long o, size_t p0, size_t p1) {
   const P *src = reinterpret_cast<const P *>(f.src) + (size_t)o * g.m * f.pieces;
   P *dst = reinterpret_cast<P *>(f.dst) + (size_t)o * g.n * f.pieces;
-  for (size_t p = p0 + threadIdx.x; p < p1; p += 256) {
-    P v = P{};
-    int held = -1;  // zeros
-    for (int i = 0; i < g.n; ++i) {
-      const int from = g.origin[i];
-      if (from < -1 || from >= g.m) continue;  // left as it is
-      if (from != held) {
-        v = from < 0 ? P{} : src[(size_t)from * f.pieces + p];
-        held = from;
-      }
-      dst[(size_t)i * f.pieces + p] = v;
+  const size_t p = p0 + threadIdx.x;
+  P v[4];
+  int held = -2;
+  for (int i = 0; i < g.n; ++i) {
+    const int from = g.origin[i];
+    if (from < -1 || from >= g.m) continue;  // left as it is
+    if (from != held) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = from < 0 ? P{} : src[(size_t)from * f.pieces + (p + 256 * u < p1 ? p + 256 * u : p0)];
+      held = from;
     }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (p + 256 * u < p1) __builtin_nontemporal_store(v[u], dst + (size_t)i * f.pieces + p + 256 * u);
   }
 }
 
@@ -56,7 +61,7 @@ __global__ __launch_bounds__(256) void k_copy_slots(SlotArgs g) {
     const SlotBuffer &f = buffer_of(g, task);
     const long at = task - f.first, o = at / f.chunks;
     const size_t p0 = (size_t)(at - o * f.chunks) * f.chunk, p1 = p0 + f.chunk < f.pieces ? p0 + f.chunk : f.pieces;
-    if (f.unit == 16) copy_chunk<uint4>(g, f, o, p0, p1);
+    if (f.unit == 16) copy_chunk<u32x4>(g, f, o, p0, p1);
     else if (f.unit == 4) copy_chunk<uint32_t>(g, f, o, p0, p1);
     else if (f.unit == 2) copy_chunk<uint16_t>(g, f, o, p0, p1);
     else copy_chunk<uint8_t>(g, f, o, p0, p1);
@@ -64,65 +69,87 @@ __global__ __launch_bounds__(256) void k_copy_slots(SlotArgs g) {
 }
 
 // In place: a chunk of every source that moves goes to LDS before any slot is written, so a slot may be read and
-// overwritten in one call, in any cycle.
+// overwritten in one call, in any cycle.  A chunk is a power of two of pieces: 2^shift lanes take one slot's.
 template <typename P>
 __device__ __forceinline__ void move_chunk(const SlotBuffer &f, int n, long o, size_t p0, size_t p1, char *stage, const short *read,
                                            int n_read, const short *write, const short *from, int n_write) {
-  P *base = reinterpret_cast<P *>(f.dst) + (size_t)o * n * f.pieces;
+  P *base = reinterpret_cast<P *>(f.dst) + (size_t)o * n * f.pieces + p0;
   P *st = reinterpret_cast<P *>(stage);
-  const unsigned w = (unsigned)(p1 - p0);
-  for (unsigned e = threadIdx.x; e < n_read * w; e += 256) {
-    const unsigned k = e / w, p = e - k * w;
-    st[e] = base[(size_t)read[k] * f.pieces + p0 + p];
+  const unsigned shift = f.shift, w = (unsigned)(p1 - p0), mask = (1u << shift) - 1;
+#pragma unroll 4
+  for (unsigned e = threadIdx.x; e < (unsigned)n_read << shift; e += 256) {
+    const unsigned p = e & mask;
+    st[e] = base[(size_t)read[e >> shift] * f.pieces + (p < w ? p : 0)];
   }
   __syncthreads();
-  for (unsigned e = threadIdx.x; e < n_write * w; e += 256) {
-    const unsigned k = e / w, p = e - k * w;
+#pragma unroll 4
+  for (unsigned e = threadIdx.x; e < (unsigned)n_write << shift; e += 256) {
+    const unsigned k = e >> shift, p = e & mask;
     const int s = from[k];
-    base[(size_t)write[k] * f.pieces + p0 + p] = s < 0 ? P{} : st[s * w + p];
+    const P v = s < 0 ? P{} : st[(s << shift) + p];
+    if (p < w) base[(size_t)write[k] * f.pieces + p] = v;
   }
   __syncthreads();
 }
 
 __global__ __launch_bounds__(256) void k_move_slots(SlotArgs g) {
   __shared__ __attribute__((aligned(16))) char s_stage[kStageBytes];
-  __shared__ short s_place[kInPlaceSlots];  // of a source among those that are read; -1: not read
+  __shared__ int s_origin[kInPlaceSlots];
+  __shared__ short s_place[kInPlaceSlots];  // of a source among those that are read
   __shared__ short s_read[kInPlaceSlots], s_write[kInPlaceSlots], s_from[kInPlaceSlots];
   __shared__ int s_n[2];
-  for (int i = threadIdx.x; i < g.n; i += 256) s_place[i] = 0;
+  const int lane = threadIdx.x & 63;
+  for (int i = threadIdx.x; i < g.n; i += 256) {
+    s_origin[i] = g.origin[i];
+    s_place[i] = 0;
+  }
   __syncthreads();
   for (int i = threadIdx.x; i < g.n; i += 256) {
-    const int from = g.origin[i];
+    const int from = s_origin[i];
     if (from >= 0 && from < g.n && from != i) s_place[from] = 1;
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
+  if (threadIdx.x < 64) {  // one wavefront lists what is read and what is written, 64 slots at a time
+    const unsigned long long below = (1ull << lane) - 1;
     int r = 0, w = 0;
-    for (int i = 0; i < g.n; ++i) {
-      if (s_place[i]) {
-        s_read[r] = (short)i;
-        s_place[i] = (short)r++;
+    for (int c = 0; c < g.n; c += 64) {
+      const int i = c + lane;
+      const bool reads = i < g.n && s_place[i];
+      const unsigned long long mask = __ballot(reads);
+      if (reads) {
+        const int at = r + __popcll(mask & below);
+        s_read[at] = (short)i;
+        s_place[i] = (short)at;
       }
+      r += __popcll(mask);
     }
-    for (int i = 0; i < g.n; ++i) {
-      const int from = g.origin[i];
-      if (from < -1 || from >= g.n || from == i) continue;
-      s_write[w] = (short)i;
-      s_from[w++] = from < 0 ? (short)-1 : s_place[from];
+    for (int c = 0; c < g.n; c += 64) {
+      const int i = c + lane, from = i < g.n ? s_origin[i] : -2;
+      const bool writes = from >= -1 && from < g.n && from != i;
+      const unsigned long long mask = __ballot(writes);
+      if (writes) {
+        const int at = w + __popcll(mask & below);
+        s_write[at] = (short)i;
+        s_from[at] = from < 0 ? (short)-1 : s_place[from];
+      }
+      w += __popcll(mask);
     }
-    s_n[0] = r;
-    s_n[1] = w;
+    if (lane == 0) {
+      s_n[0] = r;
+      s_n[1] = w;
+    }
   }
   __syncthreads();
-  if (s_n[1] == 0) return;
+  const int n_read = s_n[0], n_write = s_n[1];
+  if (n_write == 0) return;
   for (long task = blockIdx.x; task < g.tasks; task += gridDim.x) {
     const SlotBuffer &f = buffer_of(g, task);
     const long at = task - f.first, o = at / f.chunks;
     const size_t p0 = (size_t)(at - o * f.chunks) * f.chunk, p1 = p0 + f.chunk < f.pieces ? p0 + f.chunk : f.pieces;
-    if (f.unit == 16) move_chunk<uint4>(f, g.n, o, p0, p1, s_stage, s_read, s_n[0], s_write, s_from, s_n[1]);
-    else if (f.unit == 4) move_chunk<uint32_t>(f, g.n, o, p0, p1, s_stage, s_read, s_n[0], s_write, s_from, s_n[1]);
-    else if (f.unit == 2) move_chunk<uint16_t>(f, g.n, o, p0, p1, s_stage, s_read, s_n[0], s_write, s_from, s_n[1]);
-    else move_chunk<uint8_t>(f, g.n, o, p0, p1, s_stage, s_read, s_n[0], s_write, s_from, s_n[1]);
+    if (f.unit == 16) move_chunk<u32x4>(f, g.n, o, p0, p1, s_stage, s_read, n_read, s_write, s_from, n_write);
+    else if (f.unit == 4) move_chunk<uint32_t>(f, g.n, o, p0, p1, s_stage, s_read, n_read, s_write, s_from, n_write);
+    else if (f.unit == 2) move_chunk<uint16_t>(f, g.n, o, p0, p1, s_stage, s_read, n_read, s_write, s_from, n_write);
+    else move_chunk<uint8_t>(f, g.n, o, p0, p1, s_stage, s_read, n_read, s_write, s_from, n_write);
   }
 }
 
@@ -177,9 +204,11 @@ extern "C" int bdh_copy_slots(bdh_ctx *ctx, const bdh_slot_buffer *buffers_host,
   if (g.n_buf == 0) return BDH_OK;
   for (int i = 0; i < g.n_buf; ++i) {
     SlotBuffer &f = g.buf[i];
-    // in place: a chunk of every slot fits the stage
-    const size_t most = in_place ? (size_t)kStageBytes / f.unit / dst_slots : 1024;
-    f.chunk = (unsigned)std::max<size_t>(1, std::min(f.pieces, most));
+    f.chunk = 1024;
+    if (in_place) {  // a chunk of every slot fits the stage
+      while ((size_t)f.chunk * f.unit * dst_slots > (size_t)kStageBytes || (f.chunk > 1 && f.chunk / 2 >= f.pieces)) f.chunk /= 2;
+      f.shift = (unsigned)__builtin_ctz(f.chunk);
+    }
     f.chunks = (long)((f.pieces + f.chunk - 1) / f.chunk);
     f.first = g.tasks;
     g.tasks += f.chunks * f.outer;

@@ -64,8 +64,16 @@ def pack_allowed(allowed: torch.Tensor) -> torch.Tensor:
 
 
 def _seen(seen: torch.Tensor, B: int, V: int, dev) -> None:
-    if tuple(seen.shape) != (B, V) or seen.dtype != torch.int32 or not seen.is_contiguous() or seen.device != dev:
+    if seen.shape != (B, V) or seen.dtype is not torch.int32 or not seen.is_contiguous() or seen.device != dev:
         raise ValueError(f"seen: expected a contiguous int32 tensor [{B}, {V}] on {dev}, got {seen.dtype} {tuple(seen.shape)}")
+
+
+def _row_stride(name: str, t: torch.Tensor, B: int, width: int, dtype, dev) -> int:
+    """Elements between the rows of a bias or mask: 0 for one row that all sequences share."""
+    if t.dtype is not dtype or t.device != dev or t.dim() not in (1, 2) or t.shape[-1] != width or \
+            (t.dim() == 2 and t.shape[0] != B) or (width > 1 and t.stride(-1) != 1):
+        raise ValueError(f"{name}: expected {dtype} [{width}] or [{B}, {width}] on {dev}, got {t.dtype} {tuple(t.shape)}")
+    return t.stride(0) if t.dim() == 2 and B > 1 else 0
 
 
 def count_tokens(tokens: torch.Tensor, seen: torch.Tensor, lens: Optional[torch.Tensor] = None, prompt: bool = False,
@@ -75,9 +83,9 @@ def count_tokens(tokens: torch.Tensor, seen: torch.Tensor, lens: Optional[torch.
     B, T = tokens.shape
     dev, V = tokens.device, seen.shape[-1]
     _seen(seen, B, V, dev)
-    if tokens.dtype != torch.int64 or (T > 1 and tokens.stride(1) != 1):
+    if tokens.dtype is not torch.int64 or (T > 1 and tokens.stride(1) != 1):
         raise ValueError("tokens: expected int64 rows")
-    if lens is not None and (tuple(lens.shape) != (B,) or lens.dtype != torch.int32 or lens.device != dev or not lens.is_contiguous()):
+    if lens is not None and (lens.shape != (B,) or lens.dtype is not torch.int32 or lens.device != dev or not lens.is_contiguous()):
         raise ValueError(f"lens: expected int32 [{B}] on {dev}")
     ctx = ctx or ffi.default_context(dev.index or 0)
     ctx.check(ctx.lib.bdh_count_tokens(ctx.handle, B, T, V, ffi.ptr(tokens), tokens.stride(0) if B > 1 else max(T, 1),
@@ -98,31 +106,30 @@ def apply_rules(logits: torch.Tensor, rules: LogitRules, seen: Optional[torch.Te
     elif rules.penalises or newest is not None:
         raise ValueError("penalties need the counts of the tokens seen")
     if newest is not None:
-        newest = newest.reshape(-1)
-        if newest.numel() != B or newest.dtype != torch.int64 or newest.device != dev:
+        if newest.dim() != 1:
+            newest = newest.reshape(-1)
+        if newest.shape != (B,) or newest.dtype is not torch.int64 or newest.device != dev:
             raise ValueError(f"newest: expected int64 [{B}] on {dev}")
         newest = newest.contiguous()
-    rules = rules.to(dev, B)
-    for name in ("repetition", "presence", "frequency"):
-        p = getattr(rules, name)
-        if p is not None and (tuple(p.shape) != (B,) or p.dtype != torch.float32 or p.device != dev or not p.is_contiguous()):
-            raise ValueError(f"{name}: expected f32 [{B}] on {dev}")
-    rows = []
-    for name, t, width, dtype in (("bias", rules.bias, V, torch.float32), ("allowed", rules.allowed, (V + 31) // 32, torch.int32)):
-        if t is None:
-            rows.append(0)
-            continue
-        if t.dtype != dtype or t.device != dev or t.shape[-1] != width or t.dim() not in (1, 2) or \
-                (t.dim() == 2 and t.shape[0] != B) or (width > 1 and t.stride(-1) != 1):
-            raise ValueError(f"{name}: expected {dtype} [{width}] or [{B}, {width}] on {dev}, got {t.dtype} {tuple(t.shape)}")
-        rows.append(t.stride(0) if t.dim() == 2 and B > 1 else 0)
+    penalties = []
+    for name, p in (("repetition", rules.repetition), ("presence", rules.presence), ("frequency", rules.frequency)):
+        if p is not None:
+            if not torch.is_tensor(p):
+                p = torch.full((B,), float(p), device=dev, dtype=torch.float32)
+            elif p.shape != (B,) or p.dtype is not torch.float32 or p.device != dev or not p.is_contiguous():
+                raise ValueError(f"{name}: expected f32 [{B}] on {dev}")
+        penalties.append(p)
+    bias, allowed = rules.bias, rules.allowed
+    bias_stride = 0 if bias is None else _row_stride("bias", bias, B, V, torch.float32, dev)
+    allowed_stride = 0 if allowed is None else _row_stride("allowed", allowed, B, (V + 31) // 32, torch.int32, dev)
     if out is None:
-        out = torch.empty((B, V), device=dev, dtype=torch.float32)
-    elif tuple(out.shape) != (B, V) or out.dtype != torch.float32 or out.device != dev or (V > 1 and out.stride(1) != 1):
+        out = torch.empty_like(logits) if logits.is_contiguous() else torch.empty((B, V), device=dev, dtype=torch.float32)
+    elif out.shape != (B, V) or out.dtype is not torch.float32 or out.device != dev or (V > 1 and out.stride(1) != 1):
         raise ValueError(f"out: expected f32 rows [{B}, {V}] on {dev}")
     ctx = ctx or ffi.default_context(dev.index or 0)
-    ctx.check(ctx.lib.bdh_logit_rules(ctx.handle, B, V, ffi.ptr(logits), logits.stride(0) if B > 1 else V, ffi.ptr(seen),
-                                      ffi.ptr(newest), ffi.ptr(rules.repetition), ffi.ptr(rules.presence),
-                                      ffi.ptr(rules.frequency), ffi.ptr(rules.bias), rows[0], ffi.ptr(rules.allowed), rows[1],
-                                      ffi.ptr(out), out.stride(0) if B > 1 else V))
+    ctx.check(ctx.lib.bdh_logit_rules(
+        ctx.handle, B, V, logits.data_ptr(), logits.stride(0) if B > 1 else V, None if seen is None else seen.data_ptr(),
+        None if newest is None else newest.data_ptr(), *[None if p is None else p.data_ptr() for p in penalties],
+        None if bias is None else bias.data_ptr(), bias_stride, None if allowed is None else allowed.data_ptr(), allowed_stride,
+        out.data_ptr(), out.stride(0) if B > 1 else V))
     return out

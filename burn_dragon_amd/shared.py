@@ -4,9 +4,9 @@ it as keys and values.  The sums are those of BDH::recurrent_attention (src/mode
 ends; the reference gives every sequence a state of its own."""
 from __future__ import annotations
 
+import ctypes
 from typing import Optional, Sequence
 
-import numpy as np
 import torch
 
 from . import ffi
@@ -16,7 +16,7 @@ _DTYPES = {torch.float32: ffi.F32, torch.bfloat16: ffi.BF16}
 
 
 def _check(name: str, t: torch.Tensor, shape, dtype, device) -> None:
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous() or t.device != device:
+    if t.shape != shape or t.dtype is not dtype or not t.is_contiguous() or t.device != device:
         raise ValueError(f"{name}: expected a contiguous {dtype} tensor {tuple(shape)} on {device}, got {t.dtype} "
                          f"{tuple(t.shape)} on {t.device}")
 
@@ -28,16 +28,15 @@ def _prompts(counts: Optional[Sequence[int]], G: int, B: int):
         counts = [B]
     if len(counts) != G or sum(counts) != B or min(counts, default=0) < 0:
         raise ValueError(f"counts {list(counts)} do not deal {B} sequences to {G} prompts")
-    return np.ascontiguousarray(counts, np.int32)
+    return (ctypes.c_int32 * G)(*counts)
 
 
 def _slopes(alibi_slopes, h: int):
     if alibi_slopes is None:
         return None
-    s = np.ascontiguousarray(alibi_slopes, np.float32)
-    if s.size != h:
-        raise ValueError(f"{s.size} slopes for {h} heads")
-    return s
+    if len(alibi_slopes) != h:
+        raise ValueError(f"{len(alibi_slopes)} slopes for {h} heads")
+    return (ctypes.c_float * h)(*[float(s) for s in alibi_slopes])
 
 
 def shared_prefix_attention(query: torch.Tensor, value: torch.Tensor, rho: torch.Tensor, keys: torch.Tensor,
@@ -75,10 +74,10 @@ def shared_prefix_attention(query: torch.Tensor, value: torch.Tensor, rho: torch
     ctx = ctx or ffi.default_context(dev.index or 0)
     out = torch.empty((B, h, T, d), device=dev, dtype=torch.float32)
     ctx.check(ctx.lib.bdh_shared_prefix_attention(
-        ctx.handle, G, n_of.ctypes.data, B, h, T, N, d, int(rot), ffi.ptr(query), ffi.ptr(value),
-        None if rot == RotaryEmbedding.ALIBI else ffi.ptr(freqs), int(position), ffi.ptr(positions), ffi.ptr(slopes),
-        ffi.ptr(rho), _DTYPES[rho.dtype], S, ffi.ptr(lens), -1 if longest is None else int(longest), ffi.ptr(keys),
-        ffi.ptr(values), ffi.ptr(out)))
+        ctx.handle, G, n_of, B, h, T, N, d, int(rot), query.data_ptr(), value.data_ptr(),
+        None if rot == RotaryEmbedding.ALIBI else freqs.data_ptr(), int(position), ffi.ptr(positions), slopes,
+        rho.data_ptr(), _DTYPES[rho.dtype], S, lens.data_ptr(), -1 if longest is None else int(longest), keys.data_ptr(),
+        values.data_ptr(), out.data_ptr()))
     return out
 
 
@@ -104,7 +103,7 @@ def shared_prefix_fork(rho: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     slopes = _slopes(alibi_slopes, h)
     ctx = ctx or ffi.default_context(dev.index or 0)
     ctx.check(ctx.lib.bdh_shared_prefix_fork(
-        ctx.handle, G, n_of.ctypes.data, B, h, Nq, d, int(RotaryEmbedding.parse(rotary_embedding)), ffi.ptr(slopes),
-        ffi.ptr(rho), _DTYPES[rho.dtype], S, ffi.ptr(lens), -1 if longest is None else int(longest), ffi.ptr(keys),
-        ffi.ptr(values), ffi.ptr(out)))
+        ctx.handle, G, n_of, B, h, Nq, d, int(RotaryEmbedding.parse(rotary_embedding)), slopes,
+        rho.data_ptr(), _DTYPES[rho.dtype], S, lens.data_ptr(), -1 if longest is None else int(longest), keys.data_ptr(),
+        values.data_ptr(), out.data_ptr()))
     return out

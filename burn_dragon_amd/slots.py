@@ -2,6 +2,7 @@
 freed, reordered; all buffers of a batch in one launch."""
 from __future__ import annotations
 
+import math
 from typing import Iterable, Optional, Sequence, Tuple, Union
 
 import torch
@@ -33,16 +34,17 @@ def copy_slots(buffers: Iterable[Tuple[torch.Tensor, torch.Tensor, int]], origin
         dim %= dst.dim()
         if dst.shape[:dim] != src.shape[:dim] or dst.shape[dim + 1:] != src.shape[dim + 1:]:
             raise ValueError(f"buffer {k}: slots of {tuple(dst.shape)} and {tuple(src.shape)} differ")
-        outer = int(torch.Size(dst.shape[:dim]).numel())
-        table[k] = ffi.SlotBufferC(dst.data_ptr(), src.data_ptr(),
-                                   torch.Size(dst.shape[dim + 1:]).numel() * dst.element_size(), outer)
+        row = table[k]
+        row.dst, row.src = dst.data_ptr(), src.data_ptr()
+        row.outer = math.prod(dst.shape[:dim])
+        row.slot_bytes = math.prod(dst.shape[dim + 1:]) * dst.element_size()
     if not torch.is_tensor(origin):
         origin = [int(o) for o in origin]
         bad = [o for o in origin if not KEEP <= o < m]
         if bad:
             raise ValueError(f"origin names slots {bad} of {m}")
         origin = torch.tensor(origin, dtype=torch.int32, device=dev)
-    if tuple(origin.shape) != (n,) or origin.dtype != torch.int32 or origin.device != dev or not origin.is_contiguous():
+    if origin.shape != (n,) or origin.dtype != torch.int32 or origin.device != dev or not origin.is_contiguous():
         raise ValueError(f"origin: expected int32 [{n}] on {dev}, got {origin.dtype} {tuple(origin.shape)} on {origin.device}")
     ctx = ctx or ffi.default_context(dev.index or 0)
     ctx.check(ctx.lib.bdh_copy_slots(ctx.handle, table, len(buffers), n, m, origin.data_ptr()))
