@@ -136,12 +136,12 @@ struct Product {
       reinterpret_cast<float *>(tile)[i * ld + place] = v;
     } else {  // hi + mid + lo is v itself
       unsigned short *p = reinterpret_cast<unsigned short *>(tile) + i * ld + place;
-      const unsigned short hi = f32_to_bf16(v);
-      const float r = v - bf16_to_f32(hi);
-      const unsigned short mid = f32_to_bf16(r);
-      p[0] = hi;
-      p[kQ * ld] = mid;
-      p[2 * kQ * ld] = f32_to_bf16(r - bf16_to_f32(mid));
+      const unsigned int hi = pack_bf16_rne(v, 0.0f);
+      const float r = v - __uint_as_float(hi << 16);
+      const unsigned int mid = pack_bf16_rne(r, 0.0f);
+      p[0] = (unsigned short)hi;
+      p[kQ * ld] = (unsigned short)mid;
+      p[2 * kQ * ld] = (unsigned short)pack_bf16_rne(r - __uint_as_float(mid << 16), 0.0f);
     }
   }
   __device__ __forceinline__ float get(int i, int place) const {
@@ -179,8 +179,9 @@ struct Product {
   }
 
   // queries in memory: row n0 and those behind it, `have` of them.  A thread takes one row of every parts-th query.
-  template <bool MASKS>
-  __device__ __forceinline__ void load_queries(const float *q, unsigned ld_q, int nb, int rows, int have) {
+  // masks: also which of them fire, for own_keys.
+  __device__ __forceinline__ void load_queries(const float *q, unsigned ld_q, int nb, int rows, int have, bool masks) {
+    constexpr int U = 16;  // loads on their way
     const int tid = threadIdx.x, r = tid & (rows - 1), wave = wave_of_thread();
     const int part = rows == 256 ? 0 : wave >> 1, parts = rows == 256 ? 1 : 2;  // rows is 128 or 256
     const bool exists = r < have;
@@ -192,18 +193,18 @@ struct Product {
       cnt = have;
       sh.list[tid] = (unsigned short)(tid < have ? tid : 0);
     }
-    if (!all || MASKS) {
+    if (!all || masks) {
       bool used = false;
 #pragma unroll 1
-      for (int i0 = part; i0 < nb; i0 += 8 * parts) {
-        float v[8];
+      for (int i0 = part; i0 < nb; i0 += U * parts) {
+        float v[U];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = q[sh.row[min(i0 + k * parts, nb - 1)] * (long)ld_q + at];
+        for (int k = 0; k < U; ++k) v[k] = q[sh.row[min(i0 + k * parts, nb - 1)] * (long)ld_q + at];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < U; ++k) {
           const bool fires = v[k] != 0.0f && i0 + k * parts < nb && exists;
           used |= fires;
-          if constexpr (MASKS) {
+          if (masks) {
             const unsigned long long mask = __ballot(fires);
             if ((tid & 63) == 0 && i0 + k * parts < nb) sh.fires[i0 + k * parts][r >> 6] = mask;
           }
@@ -219,13 +220,13 @@ struct Product {
     for (int e = tid; e < (width - cnt) * kQ; e += 256) put(e % kQ, cnt + e / kQ, 0.0f);
     const int place = sh.used[r] - 1;
 #pragma unroll 1
-    for (int i0 = part; i0 < kQ; i0 += 8 * parts) {
-      float v[8];
+    for (int i0 = part; i0 < kQ; i0 += U * parts) {
+      float v[U];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = q[sh.row[min(i0 + k * parts, nb - 1)] * (long)ld_q + at];
+      for (int k = 0; k < U; ++k) v[k] = q[sh.row[min(i0 + k * parts, nb - 1)] * (long)ld_q + at];
       if (place >= 0)
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
+        for (int k = 0; k < U; ++k)
           if (i0 + k * parts < kQ) put(i0 + k * parts, place, i0 + k * parts < nb ? v[k] : 0.0f);
     }
     __syncthreads();
@@ -403,16 +404,19 @@ struct Product {
       if (st + u * kw < steps) product(buf[u], st + u * kw);
   }
 
-  // The scores of these rows for sequences own0 .. own1 - 1: half a wavefront lists what of a sequence is active (PAIR: pairs of
-  // rows), then sixteen lanes take four neighbouring keys each of every other listed one.
+  // The scores of these rows for sequences own0 .. own1 - 1: half a wavefront (of up to four sequences a whole one) lists what of
+  // a sequence is active (PAIR: pairs of rows), then sixteen lanes take four neighbouring keys each of every other (every
+  // fourth) listed one.
   template <bool PAIR>
   __device__ __forceinline__ void own_keys(const PassArgs &g, int rb, int own0, int own1) {
     constexpr int PER = PAIR ? 2 : 1, U = 8 / PER;
-    const int tid = threadIdx.x, half = tid >> 5, hl = tid & 31, k2 = hl >> 4, li = tid & 15;
+    const int tid = threadIdx.x, half = tid >> 5, hl = tid & 31, li = tid & 15;
+    const bool whole = own1 - own0 <= 4;
+    const int k2 = whole ? (tid & 63) >> 4 : hl >> 4, stride = whole ? 4 : 2;
     const int last = g.Nq - 1 - rb * g.rows;
     unsigned short *own = sh.own[half];
 #pragma unroll 1
-    for (int i = own0 + half; i < own1; i += 8) {
+    for (int i = own0 + (whole ? half >> 1 : half); i < own1; i += whole ? 4 : 8) {
       const int len = sh.len[i], row = sh.row[i];
       int n = 0;
 #pragma unroll 1
@@ -430,12 +434,12 @@ struct Product {
         f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
         if (s < len)
 #pragma unroll 1
-          for (int e = k2; e < n; e += 2 * U) {
+          for (int e = k2; e < n; e += stride * U) {
             f32x4 k[U][PER];
             int r[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-              r[u] = own[min(e + 2 * u, n - 1)] * PER;
+              r[u] = own[min(e + stride * u, n - 1)] * PER;
 #pragma unroll
               for (int j = 0; j < PER; ++j) k[u][j] = *reinterpret_cast<const f32x4 *>(keys + (unsigned)(min(r[u] + j, last) * g.S + s));
             }
@@ -445,11 +449,14 @@ struct Product {
               for (int j = 0; j < PER; ++j) {
                 const int place = sh.used[r[u] + j] - 1;  // a row of the pair may be nobody's (ALiBi)
                 const float q = get(i, max(place, 0));
-                sum += (e + 2 * u < n && place >= 0 ? q : 0.0f) * k[u][j];
+                sum += (e + stride * u < n && place >= 0 ? q : 0.0f) * k[u][j];
               }
           }
 #pragma unroll
-        for (int c = 0; c < 4; ++c) sum[c] += __shfl_xor(sum[c], 16, 64);
+        for (int c = 0; c < 4; ++c) {
+          sum[c] += __shfl_xor(sum[c], 16, 64);
+          if (whole) sum[c] += __shfl_xor(sum[c], 32, 64);
+        }
         if (k2 == 0 && s < len) *reinterpret_cast<f32x4 *>(parts + s) = sum;
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -534,7 +541,7 @@ __global__ __launch_bounds__(256, RT == 4 && MODE == kHalf ? 1 : 2) void k_share
   for (; rb < end; ++rb) {
     const int n0 = rb * g.rows;
     if constexpr (ROT) p.turn_queries(g, (first + m0) * g.h + hh, nb, n0, own0, own1, my_len, my_pos);
-    else p.template load_queries<true>(g.q + n0, g.Nq, nb, g.rows, min(g.rows, g.Nq - n0));
+    else p.load_queries(g.q + n0, g.Nq, nb, g.rows, min(g.rows, g.Nq - n0), g.T == 1);
     p.multiply(static_cast<const R *>(g.rho) + (((long)grp * g.h + hh) * g.Nq + n0) * g.d, g.d, g.d, col0, g.cg, nb);
     if (ROT || g.T == 1) p.template own_keys<ROT>(g, rb, own0, own1);
     __syncthreads();  // the next block's list takes the place of what is still read here
@@ -560,7 +567,7 @@ __global__ __launch_bounds__(256, 2) void k_suffix_scores(PassArgs g) {
 #pragma unroll 1
   for (; rb < end; ++rb) {
     const int n0 = rb * g.rows;
-    p.template load_queries<false>(g.q + n0, g.Nq, nb, g.rows, min(g.rows, g.Nq - n0));
+    p.load_queries(g.q + n0, g.Nq, nb, g.rows, min(g.rows, g.Nq - n0), false);
     p.multiply(g.keys + ((long)bh * g.Nq + n0) * g.S, g.S, g.span, col0, g.cg, nb);
     __syncthreads();
   }
@@ -649,9 +656,7 @@ __global__ __launch_bounds__(1024) void k_shared_join(JoinArgs g, HeadRates rate
         const int t = e / n, s = e - t * n, k = len + t0 + t;
         float w = 0.0f;
         if (t < nt && s0 + s < k) {
-          const float *at = g.score_parts + (row + t) * g.row_step + s0 + s;
-#pragma unroll 4
-          for (int q = 0; q < g.blocks; ++q) w += at[q * g.block_step];
+          w = sum8(g.score_parts + (row + t) * g.row_step + s0 + s, g.block_step, g.blocks);
           if (g.decays) w *= expf((float)(k - s0 - s) * ld);
         }
         s_sc[t][s] = w;
@@ -838,13 +843,14 @@ struct ForkArgs {
   const float *keys, *values;
   const int32_t *lens;
   int B, h, Nq, d, S, longest;
-  int rows, row_blocks, col_blocks;  // rows a workgroup makes
+  int rows, row_blocks, col_blocks, groups;  // rows a workgroup makes; row blocks * column blocks * heads
   bool decays;
 };
 
-__device__ __forceinline__ void store_state4(float *p, f32x4 v) { *reinterpret_cast<f32x4 *>(p) = v; }
+__device__ __forceinline__ void store_state4(float *p, f32x4 v) { __builtin_nontemporal_store(v, reinterpret_cast<f32x4 *>(p)); }
 __device__ __forceinline__ void store_state4(unsigned short *p, f32x4 v) {
-  *reinterpret_cast<uint2 *>(p) = make_uint2(pack_bf16_rne(v.x, v.y), pack_bf16_rne(v.z, v.w));
+  typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+  __builtin_nontemporal_store(u32x2{pack_bf16_rne(v.x, v.y), pack_bf16_rne(v.z, v.w)}, reinterpret_cast<u32x2 *>(p));
 }
 
 // a^len rho + sum_s a^(len-s) k_s (x) v_s for `rows` rows and CB columns of one (sequence, head).  The (decayed) values stand in
@@ -852,13 +858,20 @@ __device__ __forceinline__ void store_state4(unsigned short *p, f32x4 v) {
 // keys of 32 tokens as they lie in memory, splits them in registers and multiplies six of the nine products of terms on
 // v_mfma_f32_16x16x32_bf16 (what is left out is below 2^-23 of a product), on top of the prompt's row.  Bound by the bytes of
 // the states written and the keys read; columns are dealt so that a lane has four neighbouring ones.
+constexpr int fork_waves(int cb) { return cb == 64 ? 8 : 12; }
 template <typename R, int CB>
-__global__ __launch_bounds__(512, 2) void k_shared_fork(ForkArgs g, Prompts pr, HeadRates rates) {
-  constexpr int TK = 64 * 256 / CB, LDV = TK + 8, RT = 256 / CB, RW = 16 * RT, CT = CB / 16;
+__global__ __launch_bounds__(64 * fork_waves(CB)) void k_shared_fork(ForkArgs g, Prompts pr, HeadRates rates) {
+  constexpr int NW = fork_waves(CB), TK = 64 * 256 / CB, LDV = TK + 8, RT = 256 / CB, RW = 16 * RT, CT = CB / 16;
   extern __shared__ __attribute__((aligned(16))) char s_dyn[];
   unsigned short *s_v = reinterpret_cast<unsigned short *>(s_dyn);  // [3][CB][LDV]
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_of_thread(), k4 = lane >> 4, li = lane & 15;
-  const unsigned rb = blockIdx.x / (unsigned)g.col_blocks, cb = blockIdx.x - rb * g.col_blocks, b = blockIdx.y, hh = blockIdx.z;
+  // the same rows of all sequences eight apart: they run on one XCD, and its L2 has the prompt's rows for all but the first
+  const unsigned round = blockIdx.x / (unsigned)(8 * g.B), in = blockIdx.x - round * 8 * g.B, b = in >> 3;
+  unsigned w = round * 8 + (in & 7);
+  if (w >= (unsigned)g.groups) return;
+  const unsigned cb = w % (unsigned)g.col_blocks;
+  w /= (unsigned)g.col_blocks;
+  const unsigned rb = w % (unsigned)g.row_blocks, hh = w / (unsigned)g.row_blocks;
   int grp = 0;
   while (grp + 1 < pr.G && (int)b >= pr.begin[grp + 1]) ++grp;
   const int len = g.lens[b];
@@ -873,7 +886,7 @@ __global__ __launch_bounds__(512, 2) void k_shared_fork(ForkArgs g, Prompts pr, 
   // values of tokens s0 .. s0 + TK - 1; column 64 j + 4 i + c of the block stands at place 64 j + 16 c + i
   auto stage = [&](int s0) {
     const int tokens = min((end - s0 + 31) & ~31, TK);
-    for (int e = tid; e < tokens / 8 * CB; e += 512) {
+    for (int e = tid; e < tokens / 8 * CB; e += 64 * NW) {
       const int c = e % CB, t = e / CB * 8, place = (c & ~63) + ((c & 3) << 4) + ((c >> 2) & 15);
       float v[8];
 #pragma unroll
@@ -901,8 +914,22 @@ __global__ __launch_bounds__(512, 2) void k_shared_fork(ForkArgs g, Prompts pr, 
     __syncthreads();
   }
 #pragma unroll 1
-  for (int m0 = first; m0 < last; m0 += 8 * RW) {
+  for (int m0 = first; m0 < last; m0 += NW * RW) {
     const int n0 = m0 + wave * RW;
+    constexpr int PRE = RT == 4 ? 1 : 2;  // times 32 tokens whose keys are asked for ahead
+    f32x4 ahead[PRE][RT][2];
+    auto fetch = [&](f32x4(&k)[RT][2], int s) {
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int n = min(n0 + i * 16 + li, g.Nq - 1), at = s + k4 * 8 + u * 4;
+          k[i][u] = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(K + (long)n * g.S + (at < end ? at : 0)));
+        }
+    };
+    if (end > 0)
+#pragma unroll
+      for (int u = 0; u < PRE; ++u) fetch(ahead[u], 32 * u);
     f32x4 acc[RT][CT];
 #pragma unroll
     for (int i = 0; i < RT; ++i)
@@ -931,10 +958,11 @@ __global__ __launch_bounds__(512, 2) void k_shared_fork(ForkArgs g, Prompts pr, 
         for (int i = 0; i < RT; ++i)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const int n = min(n0 + i * 16 + li, g.Nq - 1), s = s0 + t + k4 * 8 + u * 4;
-            k[i][u] = *reinterpret_cast<const f32x4 *>(K + (long)n * g.S + (s < end ? s : 0));
-            if (s >= end) k[i][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            k[i][u] = ahead[0][i][u];
+            if (s0 + t + k4 * 8 + u * 4 >= end) k[i][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (PRE == 2) ahead[0][i][u] = ahead[1][i][u];
           }
+        if (s0 + t + 32 * PRE < end) fetch(ahead[PRE - 1], s0 + t + 32 * PRE);
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
           u32x4 o[3];
@@ -1139,7 +1167,7 @@ int bdh_launch_shared_steps(bdh_ctx *ctx, const SharedStepParams &p) {
   // more than fit the chip at once: blocks of rows one after the other in a workgroup, so that all run together; or twice as many
   // where the prompts' workgroups take their own times
   bool even = true;
-  for (int i = 1; i < p.G; ++i) even &= pr.begin[i + 1] - pr.begin[i] == pr.begin[1];
+  for (int i = 1; i < p.G && T == 1; ++i) even &= pr.begin[i + 1] - pr.begin[i] == pr.begin[1];
   const long slots = (long)ctx->n_cu * (half || rt == 4 ? 2 : 3) * (even ? 1 : 2);
   auto deal = [&](long others, int &parts, int &per, int &longer) {
     parts = (int)std::max<long>(1, std::min<long>(g.row_blocks, slots / std::max<long>(1, others)));
@@ -1274,14 +1302,16 @@ int bdh_shared_prefix_fork(bdh_ctx *ctx, int G, const int32_t *counts_host, int 
     else bdh_default_alibi_slopes(h, slopes);
     for (int i = 0; i < h; ++i) rates.log_decay[i] = bdh_log_decay(slopes[i]);
   }
-  ForkArgs g{rho, rho_out, keys, values, lens_dev, B, h, Nq, d, capacity, longest < 0 ? capacity : longest, 0, 0, 0, rotary == BDH_ALIBI};
+  ForkArgs g{rho, rho_out, keys, values, lens_dev, B, h, Nq, d, capacity, longest < 0 ? capacity : longest, 0, 0, 0, 0, rotary == BDH_ALIBI};
   // columns of a workgroup: as many as leave its LDS room for every token; a wavefront's tile is 16 x 256, 32 x 128 or 64 x 64
   const int cols = g.longest <= 64 && d > 128 ? 256 : g.longest <= 128 && d > 64 ? 128 : 64;
-  const int tile = 8 * 16 * 256 / cols;  // rows that the eight wavefronts make at a time
+  const int tile = fork_waves(cols) * 16 * 256 / cols;  // rows that its wavefronts make at a time
   g.col_blocks = (d + cols - 1) / cols;
   g.rows = tile;
   while ((long)B * h * g.col_blocks * ((Nq + 2 * g.rows - 1) / (2 * g.rows)) >= 4L * ctx->n_cu) g.rows *= 2;
   g.row_blocks = (Nq + g.rows - 1) / g.rows;
+  g.groups = g.row_blocks * g.col_blocks * h;
+  if ((g.groups + 7L) / 8 * 8 * B > 0x7fffffffL) return bdh_fail(ctx, BDH_E_SHAPE, "too many tiles");
   const size_t lds = (size_t)6 * cols * (64 * 256 / cols + 8);
   using h16 = unsigned short;
   const bool wide = rho_dtype == BDH_F32;
@@ -1290,7 +1320,7 @@ int bdh_shared_prefix_fork(bdh_ctx *ctx, int G, const int32_t *counts_host, int 
                                      : (wide ? reinterpret_cast<const void *>(k_shared_fork<float, 64>) : reinterpret_cast<const void *>(k_shared_fork<h16, 64>));
   BDH_HIP_CHECK(ctx, hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
   void *args[] = {&g, &pr, &rates};
-  BDH_HIP_CHECK(ctx, hipLaunchKernel(kernel, dim3(g.row_blocks * g.col_blocks, B, h), dim3(512), args, lds, ctx->stream));
+  BDH_HIP_CHECK(ctx, hipLaunchKernel(kernel, dim3((unsigned)((g.groups + 7) / 8 * 8 * B)), dim3(64 * fork_waves(cols)), args, lds, ctx->stream));
   return BDH_OK;
 }
 
