@@ -42,6 +42,16 @@ __device__ __forceinline__ f32x4 load_state4(const unsigned short *p) {
                __uint_as_float(v.y & 0xffff0000u)};
 }
 
+// two floats as pairs (number m) of three bf16 terms, each rounded to the nearest: hi + mid + lo is the float
+__device__ __forceinline__ void split_pair(float a, float b, u32x4 (&terms)[3], int m) {
+  const unsigned int hi = pack_bf16_rne(a, b);
+  const float ra = a - __uint_as_float(hi << 16), rb = b - __uint_as_float(hi & 0xffff0000u);
+  const unsigned int mid = pack_bf16_rne(ra, rb);
+  terms[0][m] = hi;
+  terms[1][m] = mid;
+  terms[2][m] = pack_bf16_rne(ra - __uint_as_float(mid << 16), rb - __uint_as_float(mid & 0xffff0000u));
+}
+
 // sin and cos of 2 pi f, 0 <= f < 1 (the phase of src/model/attention.rs:342-343 before its factor 2 pi): f is taken to the
 // nearest quarter turn, which is exact, and the rest to the polynomials of least largest error on an eighth of a turn either
 // side (3e-9 and 3e-10; 1.7 steps of the result with the roundings).  Twenty operations where sincosf takes some sixty.
@@ -74,7 +84,7 @@ constexpr int kDenseTokens = 64;  // from here on: dense products
 constexpr int kRowsMost = 256;    // rows of the matrix a workgroup takes at a time
 
 struct PassArgs {
-  const float *x, *freqs;  // one token a sequence: its activations, turned here
+  const float *x, *freqs;  // one token a sequence (STEP): its activations, turned here
   const float *q;          // several: the queries [B,h,T,Nq]
   const int32_t *lens, *positions;
   long position;
@@ -178,22 +188,21 @@ struct Product {
     return pad;
   }
 
-  // queries in memory: row n0 and those behind it, `have` of them.  A thread takes one row of every parts-th query.
-  // masks: also which of them fire, for own_keys.
-  __device__ __forceinline__ void load_queries(const float *q, unsigned ld_q, int nb, int rows, int have, bool masks) {
+  // several tokens: their queries in memory, row n0 and those behind it, `have` of them.  A thread takes one row of every
+  // parts-th query.
+  __device__ __forceinline__ void load_queries(const float *q, unsigned ld_q, int nb, int rows, int have) {
     constexpr int U = 16;  // loads on their way
     const int tid = threadIdx.x, r = tid & (rows - 1), wave = wave_of_thread();
     const int part = rows == 256 ? 0 : wave >> 1, parts = rows == 256 ? 1 : 2;  // rows is 128 or 256
     const bool exists = r < have;
     const unsigned at = min(r, have - 1);
-    const bool all = RT == 4;  // next to nothing of a row is silent in all of so many queries: no list
+    constexpr bool all = RT == 4;  // next to nothing of a row is silent in all of so many queries: no list
     if (tid < rows) sh.used[tid] = all && exists ? tid + 1 : 0;
     __syncthreads();
-    if (all) {
+    if constexpr (all) {
       cnt = have;
       sh.list[tid] = (unsigned short)(tid < have ? tid : 0);
-    }
-    if (!all || masks) {
+    } else {
       bool used = false;
 #pragma unroll 1
       for (int i0 = part; i0 < nb; i0 += U * parts) {
@@ -201,20 +210,11 @@ struct Product {
 #pragma unroll
         for (int k = 0; k < U; ++k) v[k] = q[sh.row[min(i0 + k * parts, nb - 1)] * (long)ld_q + at];
 #pragma unroll
-        for (int k = 0; k < U; ++k) {
-          const bool fires = v[k] != 0.0f && i0 + k * parts < nb && exists;
-          used |= fires;
-          if (masks) {
-            const unsigned long long mask = __ballot(fires);
-            if ((tid & 63) == 0 && i0 + k * parts < nb) sh.fires[i0 + k * parts][r >> 6] = mask;
-          }
-        }
+        for (int k = 0; k < U; ++k) used |= v[k] != 0.0f;
       }
-      if (!all) {
-        if (used) sh.used[r] = 1;
-        __syncthreads();
-        list_rows(rows);
-      }
+      if (used && exists) sh.used[r] = 1;
+      __syncthreads();
+      list_rows(rows);
     }
     const int width = (cnt + kStep - 1) / kStep * kStep;
     for (int e = tid; e < (width - cnt) * kQ; e += 256) put(e % kQ, cnt + e / kQ, 0.0f);
@@ -228,6 +228,50 @@ struct Product {
 #pragma unroll
         for (int k = 0; k < U; ++k)
           if (i0 + k * parts < kQ) put(i0 + k * parts, place, i0 + k * parts < nb ? v[k] : 0.0f);
+    }
+    __syncthreads();
+  }
+
+  // one token a sequence, PoPE: nothing is silent (src/model/attention.rs:323-330).  Neuron n gives rows n and N + n; a thread makes
+  // one row of every parts-th sequence, and stores it as a new key for sequences own0 .. own1 - 1.
+  __device__ __forceinline__ void pope_queries(const PassArgs &g, int row0, int nb, int n0, int own0, int own1, int my_len, float my_pos) {
+    constexpr int U = 8;
+    const int tid = threadIdx.x, rows = g.rows, r = tid & (rows - 1), wave = wave_of_thread(), have = min(rows, g.Nq - n0);
+    const int part = rows == 256 ? 0 : wave >> 1, parts = rows == 256 ? 1 : 2;
+    const unsigned n = n0 + min(r, have - 1), src = n < (unsigned)g.N ? n : n - g.N;
+    const float *x = g.x + (long)row0 * g.N;
+    const float f = g.freqs[src];
+    if (tid < 64) {
+      sh.len[tid] = my_len;
+      sh.pos[tid] = my_pos;
+      const int pairs = (have + 1) / 2;
+      for (int w = 0; w < rows / 2; w += 64) sh.fires[tid][w >> 6] = pairs - w >= 64 ? ~0ull : pairs > w ? (1ull << (pairs - w)) - 1 : 0ull;
+    }
+    cnt = have;
+    sh.list[tid] = (unsigned short)(tid < have ? tid : 0);
+    sh.used[tid] = tid < have ? tid + 1 : 0;
+    __syncthreads();
+    const int width = (cnt + kStep - 1) / kStep * kStep;
+#pragma unroll 1
+    for (int i0 = part; i0 < kQ; i0 += U * parts) {
+      float v[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) v[k] = x[min(i0 + k * parts, nb - 1) * (unsigned)g.h * (unsigned)g.N + src];
+#pragma unroll 1
+      for (int k = 0; k < U; ++k) {
+        const int i = i0 + k * parts;
+        if (i >= kQ || r >= width) continue;
+        float q = 0.0f;
+        if (i < nb && r < have) {
+          float s, c;
+          sincos_turns(turns(sh.pos[i], f), s, c);
+          q = softplus1(v[0]) * (n < (unsigned)g.N ? c : s);
+          if (i >= own0 && i < own1 && sh.len[i] >= 0) g.keys[((row0 + i * g.h) * (long)g.Nq + n) * g.S + sh.len[i]] = q;
+        }
+        put(i, r, q);
+#pragma unroll
+        for (int u = 0; u + 1 < U; ++u) v[u] = v[u + 1];
+      }
     }
     __syncthreads();
   }
@@ -322,7 +366,10 @@ struct Product {
   __device__ __forceinline__ void multiply(const R *matrix, int ld_m, int cols, int col0, int cg, int nb) {
     const int lane = threadIdx.x & 63, wave = wave_of_thread(), k4 = lane >> 4, li = lane & 15;
     const int kw = 4 / cg, sub = wave / cg, steps = (cnt + kStep - 1) / kStep, col = col0 + (wave % cg) * kCols + li * C;
-    const unsigned from = col < cols ? col : 0;  // offsets from a scalar base: a block of rows is less than 4 GiB
+    // offsets from a scalar base: a block of rows is less than 4 GiB.  kHalf: a row's last piece may be four columns, it is then
+    // taken with the four before it
+    const bool short_piece = MODE == kHalf && col + 4 == cols;
+    const unsigned from = col >= cols ? 0 : short_piece ? col - 4 : col;
     constexpr int L = kStep / 4;  // rows a lane loads of a step
     using V = typename std::conditional<MODE == kHalf, u32x4, f32x4>::type;
     V buf[kDepth][L];
@@ -331,7 +378,7 @@ struct Product {
       __builtin_memcpy(r, __builtin_assume_aligned(sh.list + min(st, steps - 1) * kStep + k4 * L, 2 * L), sizeof(r));
 #pragma unroll
       for (int j = 0; j < L; ++j) {
-        if constexpr (MODE == kHalf) v[j] = *reinterpret_cast<const u32x4 *>(matrix + (r[j] * (unsigned)ld_m + from));
+        if constexpr (MODE == kHalf) v[j] = *reinterpret_cast<const u32x4u *>(matrix + (r[j] * (unsigned)ld_m + from));
         else v[j] = load_state4(matrix + (r[j] * (unsigned)ld_m + from));
       }
     };
@@ -360,13 +407,14 @@ struct Product {
 #pragma unroll
           for (int m = 0; m < 4; ++m) {
             if constexpr (MODE == kHalf) {
-              o[0][m] = __builtin_amdgcn_perm(v[2 * m + 1][c >> 1], v[2 * m][c >> 1], (c & 1) ? 0x07060302u : 0x05040100u);
+              unsigned int hi = v[2 * m + 1][c >> 1], lo = v[2 * m][c >> 1];
+              if (c < 4 && short_piece) {
+                hi = v[2 * m + 1][2 + (c >> 1)];
+                lo = v[2 * m][2 + (c >> 1)];
+              }
+              o[0][m] = __builtin_amdgcn_perm(hi, lo, (c & 1) ? 0x07060302u : 0x05040100u);
             } else {
-              const float e0 = v[2 * m][c], e1 = v[2 * m + 1][c];
-              o[0][m] = pack_bf16_rne(e0, e1);
-              const float r0 = e0 - __uint_as_float(o[0][m] << 16), r1 = e1 - __uint_as_float(o[0][m] & 0xffff0000u);
-              o[1][m] = pack_bf16_rne(r0, r1);
-              o[2][m] = pack_bf16_rne(r0 - __uint_as_float(o[1][m] << 16), r1 - __uint_as_float(o[1][m] & 0xffff0000u));
+              split_pair(v[2 * m][c], v[2 * m + 1][c], o, m);
             }
           }
 #pragma unroll
@@ -405,11 +453,10 @@ struct Product {
   }
 
   // The scores of these rows for sequences own0 .. own1 - 1: half a wavefront (of up to four sequences a whole one) lists what of
-  // a sequence is active (PAIR: pairs of rows), then sixteen lanes take four neighbouring keys each of every other (every
+  // a sequence is active (pairs of rows; with PoPE all of them), then sixteen lanes take four neighbouring keys each of every other (every
   // fourth) listed one.
-  template <bool PAIR>
   __device__ __forceinline__ void own_keys(const PassArgs &g, int rb, int own0, int own1) {
-    constexpr int PER = PAIR ? 2 : 1, U = 8 / PER;
+    constexpr int PER = 2, U = 4;
     const int tid = threadIdx.x, half = tid >> 5, hl = tid & 31, li = tid & 15;
     const bool whole = own1 - own0 <= 4;
     const int k2 = whole ? (tid & 63) >> 4 : hl >> 4, stride = whole ? 4 : 2;
@@ -490,7 +537,7 @@ struct Product {
           for (int c = 0; c < C; c += 4) {
             f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
             for (int w = group; w < 4; w += cg) sum += s[((w * RT + i) * 4 + e) * (C * 16) + (c / 4) * 64 + lane];
-            *reinterpret_cast<f32x4 *>(o + c) = sum;
+            if (c == 0 || col + 4 < cols) *reinterpret_cast<f32x4 *>(o + c) = sum;
           }
         }
       return;
@@ -505,14 +552,14 @@ struct Product {
         float *o = out + (long)sh.row[at] * cols + col;
 #pragma unroll
         for (int c = 0; c < C; c += 4)
-          *reinterpret_cast<f32x4 *>(o + c) = f32x4{acc[i][c][e], acc[i][c + 1][e], acc[i][c + 2][e], acc[i][c + 3][e]};
+          if (c == 0 || col + 4 < cols) *reinterpret_cast<f32x4 *>(o + c) = f32x4{acc[i][c][e], acc[i][c + 1][e], acc[i][c + 2][e], acc[i][c + 3][e]};
       }
   }
 };
 
 // The queries of a tile times a part of their prompt's state; one token: also their scores with what their sequences said.
 // Grid: (tile, column block), part, (prompt, head), the prompts with most sequences first.  Tiles of the same rows start together: they read them from memory once.
-template <typename R, int RT, bool ROT, int MODE>
+template <typename R, int RT, bool STEP, int MODE>
 __global__ __launch_bounds__(256, RT == 4 && MODE == kHalf ? 1 : 2) void k_shared_pass(PassArgs g, Prompts pr) {
   extern __shared__ __attribute__((aligned(16))) char s_dyn[];
   __shared__ TileShared sh;
@@ -531,7 +578,6 @@ __global__ __launch_bounds__(256, RT == 4 && MODE == kHalf ? 1 : 2) void k_share
       my_pos = (float)(g.positions ? (long)g.positions[b] : g.position);
     }
   }
-  if (!ROT && tid < 64) sh.len[tid] = my_len;
   Product<R, RT, MODE> p(sh, s_dyn, g.rows);
   const int col0 = cb * g.cg * p.kCols;
   const int own0 = cb * nb / g.col_blocks, own1 = (cb + 1) * nb / g.col_blocks;  // the column blocks share the tile's sequences
@@ -540,10 +586,14 @@ __global__ __launch_bounds__(256, RT == 4 && MODE == kHalf ? 1 : 2) void k_share
 #pragma unroll 1
   for (; rb < end; ++rb) {
     const int n0 = rb * g.rows;
-    if constexpr (ROT) p.turn_queries(g, (first + m0) * g.h + hh, nb, n0, own0, own1, my_len, my_pos);
-    else p.load_queries(g.q + n0, g.Nq, nb, g.rows, min(g.rows, g.Nq - n0), g.T == 1);
+    if constexpr (STEP) {
+      if (g.rotary == BDH_POPE) p.pope_queries(g, (first + m0) * g.h + hh, nb, n0, own0, own1, my_len, my_pos);
+      else p.turn_queries(g, (first + m0) * g.h + hh, nb, n0, own0, own1, my_len, my_pos);
+    } else {
+      p.load_queries(g.q + n0, g.Nq, nb, g.rows, min(g.rows, g.Nq - n0));
+    }
     p.multiply(static_cast<const R *>(g.rho) + (((long)grp * g.h + hh) * g.Nq + n0) * g.d, g.d, g.d, col0, g.cg, nb);
-    if (ROT || g.T == 1) p.template own_keys<ROT>(g, rb, own0, own1);
+    if constexpr (STEP) p.own_keys(g, rb, own0, own1);
     __syncthreads();  // the next block's list takes the place of what is still read here
   }
   p.finish(g.partial + (long)part * g.B * g.h * g.T * g.d, g.d, col0, g.cg, nb);
@@ -567,7 +617,7 @@ __global__ __launch_bounds__(256, 2) void k_suffix_scores(PassArgs g) {
 #pragma unroll 1
   for (; rb < end; ++rb) {
     const int n0 = rb * g.rows;
-    p.load_queries(g.q + n0, g.Nq, nb, g.rows, min(g.rows, g.Nq - n0), false);
+    p.load_queries(g.q + n0, g.Nq, nb, g.rows, min(g.rows, g.Nq - n0));
     p.multiply(g.keys + ((long)bh * g.Nq + n0) * g.S, g.S, g.span, col0, g.cg, nb);
     __syncthreads();
   }
@@ -786,7 +836,7 @@ __global__ __launch_bounds__(256) void k_suffix_append(AppendArgs g) {
     const int m = n0 + (r & 63);
     if (t < g.T && m < g.N) g.keys[((long)bh * g.Nq + (r < 64 ? m : g.N + m)) * g.S + len + t] = s_t[r][tid & 31];
   }
-  if (g.T > 1 && blockIdx.x == 0 && bh % g.h == 0) {
+  if (blockIdx.x == 0 && bh % g.h == 0) {
     const long last = min(t0 + 32, g.T);
     for (long e = (long)t0 * g.d + tid; e < last * g.d; e += 256)
       g.values[((long)b * g.S + len) * g.d + e] = g.v[(long)b * g.T * g.d + e];
@@ -843,169 +893,183 @@ struct ForkArgs {
   const float *keys, *values;
   const int32_t *lens;
   int B, h, Nq, d, S, longest;
-  int rows, row_blocks, col_blocks, groups;  // rows a workgroup makes; row blocks * column blocks * heads
-  bool decays;
+  int rows, row_blocks, col_blocks, groups;  // rows a workgroup makes; row blocks * heads
+  bool decays, whole_lines;                  // rows of whole cache lines
 };
 
-__device__ __forceinline__ void store_state4(float *p, f32x4 v) { __builtin_nontemporal_store(v, reinterpret_cast<f32x4 *>(p)); }
-__device__ __forceinline__ void store_state4(unsigned short *p, f32x4 v) {
+__device__ __forceinline__ void store_state4(float *p, f32x4 v, bool past) {
+  if (past) __builtin_nontemporal_store(v, reinterpret_cast<f32x4 *>(p));
+  else *reinterpret_cast<f32x4 *>(p) = v;
+}
+__device__ __forceinline__ void store_state4(unsigned short *p, f32x4 v, bool past) {
   typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
-  __builtin_nontemporal_store(u32x2{pack_bf16_rne(v.x, v.y), pack_bf16_rne(v.z, v.w)}, reinterpret_cast<u32x2 *>(p));
+  const u32x2 o = {pack_bf16_rne(v.x, v.y), pack_bf16_rne(v.z, v.w)};
+  if (past) __builtin_nontemporal_store(o, reinterpret_cast<u32x2 *>(p));
+  else *reinterpret_cast<u32x2 *>(p) = o;
 }
 
-// a^len rho + sum_s a^(len-s) k_s (x) v_s for `rows` rows and CB columns of one (sequence, head).  The (decayed) values stand in
-// LDS as three bf16 terms, token by token of a column, TK tokens at a time; a wavefront makes RW rows at a time: it takes the
-// keys of 32 tokens as they lie in memory, splits them in registers and multiplies six of the nine products of terms on
-// v_mfma_f32_16x16x32_bf16 (what is left out is below 2^-23 of a product), on top of the prompt's row.  Bound by the bytes of
-// the states written and the keys read; columns are dealt so that a lane has four neighbouring ones.
-constexpr int fork_waves(int cb) { return cb == 64 ? 8 : 12; }
+constexpr int fork_waves(int cb) { return cb == 320 ? 8 : 12; }  // as many as its registers leave room for
+
+// What a workgroup of a fork works on.
+struct ForkTile {
+  int first, last, col0, len, end, grp;
+  long bh;
+  float log_decay, base;
+  bool valid;
+  const float *V;
+  // the same rows of all sequences eight apart: they run on one XCD, and its L2 has the prompt's rows for all but the first
+  __device__ __forceinline__ bool find(const ForkArgs &g, const Prompts &pr, const HeadRates &rates, int cb_size) {
+    const unsigned each = 8 * g.B * g.col_blocks, round = blockIdx.x / each, in = blockIdx.x - round * each;
+    const unsigned b = (in >> 3) / (unsigned)g.col_blocks, cb = (in >> 3) - b * g.col_blocks, w = round * 8 + (in & 7);
+    if (w >= (unsigned)g.groups) return false;
+    const unsigned hh = w / (unsigned)g.row_blocks, rb = w - hh * g.row_blocks;
+    grp = 0;
+    while (grp + 1 < pr.G && (int)b >= pr.begin[grp + 1]) ++grp;
+    grp = grp * g.h + hh;
+    len = g.lens[b];
+    valid = len >= 0 && len <= g.longest && len <= g.S;
+    end = valid ? len : 0;
+    first = rb * g.rows;
+    last = min(first + g.rows, g.Nq);
+    col0 = cb * cb_size;
+    log_decay = g.decays ? rates.log_decay[hh] : 0.0f;
+    base = !valid ? __uint_as_float(0x7fc00000u) : g.decays ? expf((float)len * log_decay) : 1.0f;
+    bh = (long)b * g.h + hh;
+    V = g.values + (long)b * g.S * g.d;
+    return true;
+  }
+};
+
+constexpr int kForkTokens = 64;  // whose values stand in LDS at a time
+
+// The (decayed) values of tokens s0 .. s0 + 63, up to the last one, as three bf16 terms [3][CB][72]: token by token of a column,
+// column 64 j + 4 i + c of the block at place 64 j + 16 c + i, so that a lane gets four neighbouring columns of a row.
+template <int CB, int THREADS>
+__device__ __forceinline__ void stage_values(const ForkArgs &g, const ForkTile &w, int s0, unsigned short *s_v) {
+  constexpr int LDV = kForkTokens + 8;
+  const int tokens = min((w.end - s0 + 31) & ~31, kForkTokens);
+#pragma unroll 1
+  for (int e = threadIdx.x; e < tokens / 8 * CB; e += THREADS) {
+    const int c = e % CB, t = e / CB * 8, place = (c & ~63) + ((c & 3) << 4) + ((c >> 2) & 15);
+    float v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = w.V[(long)min(s0 + t + u, w.end - 1) * g.d + min(w.col0 + c, g.d - 1)];
+    u32x4 o[3];
+#pragma unroll
+    for (int u = 0; u < 8; u += 2) {
+      float x[2];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int s = s0 + t + u + q;
+        x[q] = s < w.end && w.col0 + c < g.d ? (g.decays ? v[u + q] * expf((float)(w.len - s) * w.log_decay) : v[u + q]) : 0.0f;
+      }
+      split_pair(x[0], x[1], o, u / 2);
+    }
+#pragma unroll
+    for (int q = 0; q < 3; ++q) *reinterpret_cast<u32x4 *>(s_v + (q * CB + place) * LDV + t) = o[q];
+  }
+}
+
+// a^len rho + sum_s a^(len-s) k_s (x) v_s for `rows` rows and CB columns of one (sequence, head).  A wavefront makes 16 rows at a
+// time on top of the prompt's rows: it splits the rows' keys into bf16 terms as they lie in memory and multiplies six of the
+// nine products with the terms of the values on v_mfma_f32_16x16x32_bf16 (what is left out is below 2^-23 of a product).  The
+// values of 64 tokens stand in LDS; those of more pass through it 64 at a time, for every 192 (128) rows again.
+// Bound by memory: without the products the largest case (32 sequences, 64 tokens, 4 heads of 8192, d = 256: 1 GiB written,
+// 256 MiB of keys) takes 9 % less, without reading the prompt's rows (from L2: a workgroup's neighbours on the XCD make the
+// same rows of other sequences) 17 %; what is written and the keys alone go at 4.0 TB/s.  A workgroup takes whole rows of up
+// to 320 columns, and the column blocks of wider ones stay on one XCD: a cache line that two XCDs write a part of goes to
+// memory twice (rows of 1200 bytes: 523 -> 426 us).
 template <typename R, int CB>
 __global__ __launch_bounds__(64 * fork_waves(CB)) void k_shared_fork(ForkArgs g, Prompts pr, HeadRates rates) {
-  constexpr int NW = fork_waves(CB), TK = 64 * 256 / CB, LDV = TK + 8, RT = 256 / CB, RW = 16 * RT, CT = CB / 16;
+  constexpr int NW = fork_waves(CB), TK = kForkTokens, LDV = TK + 8, CT = CB / 16;
   extern __shared__ __attribute__((aligned(16))) char s_dyn[];
-  unsigned short *s_v = reinterpret_cast<unsigned short *>(s_dyn);  // [3][CB][LDV]
-  const int tid = threadIdx.x, lane = tid & 63, wave = wave_of_thread(), k4 = lane >> 4, li = lane & 15;
-  // the same rows of all sequences eight apart: they run on one XCD, and its L2 has the prompt's rows for all but the first
-  const unsigned round = blockIdx.x / (unsigned)(8 * g.B), in = blockIdx.x - round * 8 * g.B, b = in >> 3;
-  unsigned w = round * 8 + (in & 7);
-  if (w >= (unsigned)g.groups) return;
-  const unsigned cb = w % (unsigned)g.col_blocks;
-  w /= (unsigned)g.col_blocks;
-  const unsigned rb = w % (unsigned)g.row_blocks, hh = w / (unsigned)g.row_blocks;
-  int grp = 0;
-  while (grp + 1 < pr.G && (int)b >= pr.begin[grp + 1]) ++grp;
-  const int len = g.lens[b];
-  const bool valid = len >= 0 && len <= g.longest && len <= g.S;
-  const int end = valid ? len : 0, first = rb * g.rows, last = min(first + g.rows, g.Nq), col0 = cb * CB;
-  const float ld = g.decays ? rates.log_decay[hh] : 0.0f;
-  const float base = !valid ? __uint_as_float(0x7fc00000u) : g.decays ? expf((float)len * ld) : 1.0f;
-  const R *rho = static_cast<const R *>(g.rho) + ((long)grp * g.h + hh) * g.Nq * g.d;
-  const long bh = (long)b * g.h + hh;
-  R *out = static_cast<R *>(g.out) + bh * g.Nq * g.d;
-  const float *K = g.keys + bh * g.Nq * g.S, *V = g.values + (long)b * g.S * g.d;
-  // values of tokens s0 .. s0 + TK - 1; column 64 j + 4 i + c of the block stands at place 64 j + 16 c + i
-  auto stage = [&](int s0) {
-    const int tokens = min((end - s0 + 31) & ~31, TK);
-    for (int e = tid; e < tokens / 8 * CB; e += 64 * NW) {
-      const int c = e % CB, t = e / CB * 8, place = (c & ~63) + ((c & 3) << 4) + ((c >> 2) & 15);
-      float v[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) v[u] = V[(long)min(s0 + t + u, end - 1) * g.d + min(col0 + c, g.d - 1)];
-      u32x4 o[3];
-#pragma unroll
-      for (int u = 0; u < 8; u += 2) {
-        float x[2];
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const int s = s0 + t + u + w;
-          x[w] = s < end && col0 + c < g.d ? (g.decays ? v[u + w] * expf((float)(len - s) * ld) : v[u + w]) : 0.0f;
-        }
-        o[0][u / 2] = pack_bf16_rne(x[0], x[1]);
-        const float r0 = x[0] - __uint_as_float(o[0][u / 2] << 16), r1 = x[1] - __uint_as_float(o[0][u / 2] & 0xffff0000u);
-        o[1][u / 2] = pack_bf16_rne(r0, r1);
-        o[2][u / 2] = pack_bf16_rne(r0 - __uint_as_float(o[1][u / 2] << 16), r1 - __uint_as_float(o[1][u / 2] & 0xffff0000u));
-      }
-#pragma unroll
-      for (int q = 0; q < 3; ++q) *reinterpret_cast<u32x4 *>(s_v + (q * CB + place) * LDV + t) = o[q];
-    }
-  };
-  if (end > 0 && end <= TK) {
-    stage(0);
-    __syncthreads();
-  }
+  unsigned short *s_v = reinterpret_cast<unsigned short *>(s_dyn);
+  const int lane = threadIdx.x & 63, wave = wave_of_thread(), k4 = lane >> 4, li = lane & 15;
+  ForkTile w;
+  if (!w.find(g, pr, rates, CB)) return;
+  const R *rho = static_cast<const R *>(g.rho) + (long)w.grp * g.Nq * g.d;
+  R *out = static_cast<R *>(g.out) + w.bh * g.Nq * g.d;
+  const float *K = g.keys + w.bh * g.Nq * g.S;
+  const int end = w.end;
+  if (end > 0 && end <= TK) stage_values<CB, 64 * NW>(g, w, 0, s_v);
+  __syncthreads();
 #pragma unroll 1
-  for (int m0 = first; m0 < last; m0 += NW * RW) {
-    const int n0 = m0 + wave * RW;
-    constexpr int PRE = RT == 4 ? 1 : 2;  // times 32 tokens whose keys are asked for ahead
-    f32x4 ahead[PRE][RT][2];
-    auto fetch = [&](f32x4(&k)[RT][2], int s) {
+  for (int m0 = w.first; m0 < w.last; m0 += NW * 16) {
+    const int n0 = m0 + wave * 16;
+    const float *key = K + (long)min(n0 + li, g.Nq - 1) * g.S;
+    f32x4 ahead[2][2];  // keys of twice 32 tokens
+    auto fetch = [&](f32x4(&k)[2], int s) {
 #pragma unroll
-      for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int n = min(n0 + i * 16 + li, g.Nq - 1), at = s + k4 * 8 + u * 4;
-          k[i][u] = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(K + (long)n * g.S + (at < end ? at : 0)));
-        }
+      for (int q = 0; q < 2; ++q) {
+        const int at = s + k4 * 8 + q * 4;
+        k[q] = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(key + (at < end ? at : 0)));
+      }
     };
-    if (end > 0)
+    if (end > 0) {
+      fetch(ahead[0], 0);
+      fetch(ahead[1], 32);
+    }
+    f32x4 acc[CT];
 #pragma unroll
-      for (int u = 0; u < PRE; ++u) fetch(ahead[u], 32 * u);
-    f32x4 acc[RT][CT];
+    for (int j = 0; j < CT; j += 4)
 #pragma unroll
-    for (int i = 0; i < RT; ++i)
+      for (int e = 0; e < 4; ++e) {
+        const int n = min(n0 + k4 * 4 + e, g.Nq - 1), col = w.col0 + j * 16 + li * 4;
+        const f32x4 v = load_state4(rho + (long)n * g.d + (col < g.d ? col : 0));
 #pragma unroll
-      for (int j = 0; j < CT; j += 4)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int n = min(n0 + i * 16 + k4 * 4 + e, g.Nq - 1), col = col0 + j * 16 + li * 4;
-          const f32x4 v = load_state4(rho + (long)n * g.d + (col < g.d ? col : 0));
-#pragma unroll
-          for (int c = 0; c < 4; ++c) acc[i][j + c][e] = v[c] * base;
-        }
+        for (int c = 0; c < 4; ++c) acc[j + c][e] = v[c] * w.base;
+      }
 #pragma unroll 1
     for (int s0 = 0; s0 < end; s0 += TK) {
       if (end > TK) {
         __syncthreads();
-        stage(s0);
+        stage_values<CB, 64 * NW>(g, w, s0, s_v);
         __syncthreads();
       }
       const int stop = min(end - s0, TK);
 #pragma unroll 1
       for (int t = 0; t < stop; t += 32) {
-        bf16x8 a[RT][3];
-        f32x4 k[RT][2];
+        u32x4 o[3];
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            k[i][u] = ahead[0][i][u];
-            if (s0 + t + k4 * 8 + u * 4 >= end) k[i][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            if constexpr (PRE == 2) ahead[0][i][u] = ahead[1][i][u];
-          }
-        if (s0 + t + 32 * PRE < end) fetch(ahead[PRE - 1], s0 + t + 32 * PRE);
-#pragma unroll
-        for (int i = 0; i < RT; ++i) {
-          u32x4 o[3];
-#pragma unroll
-          for (int m = 0; m < 4; ++m) {
-            const float e0 = k[i][m >> 1][(m & 1) * 2], e1 = k[i][m >> 1][(m & 1) * 2 + 1];
-            o[0][m] = pack_bf16_rne(e0, e1);
-            const float r0 = e0 - __uint_as_float(o[0][m] << 16), r1 = e1 - __uint_as_float(o[0][m] & 0xffff0000u);
-            o[1][m] = pack_bf16_rne(r0, r1);
-            o[2][m] = pack_bf16_rne(r0 - __uint_as_float(o[1][m] << 16), r1 - __uint_as_float(o[1][m] & 0xffff0000u));
-          }
-#pragma unroll
-          for (int q = 0; q < 3; ++q) a[i][q] = __builtin_bit_cast(bf16x8, o[q]);
+        for (int m = 0; m < 4; ++m) {
+          const bool in = s0 + t + k4 * 8 + (m >> 1) * 4 < end;
+          split_pair(in ? ahead[0][m >> 1][(m & 1) * 2] : 0.0f, in ? ahead[0][m >> 1][(m & 1) * 2 + 1] : 0.0f, o, m);
         }
+        bf16x8 a[3];
+#pragma unroll
+        for (int q = 0; q < 3; ++q) a[q] = __builtin_bit_cast(bf16x8, o[q]);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) ahead[0][q] = ahead[1][q];
+        if (s0 + t + 64 < end) fetch(ahead[1], s0 + t + 64);
 #pragma unroll
         for (int j = 0; j < CT; ++j) {
           bf16x8 v[3];
 #pragma unroll
           for (int q = 0; q < 3; ++q) v[q] = *reinterpret_cast<const bf16x8 *>(s_v + (q * CB + j * 16 + li) * LDV + t + k4 * 8);
-#pragma unroll
-          for (int i = 0; i < RT; ++i) {
-            auto mac = [&](int ta, int tb) { acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i][ta], v[tb], acc[i][j], 0, 0, 0); };
-            mac(0, 2);
-            mac(1, 1);
-            mac(2, 0);
-            mac(0, 1);
-            mac(1, 0);
-            mac(0, 0);
-          }
+          auto mac = [&](int ta, int tb) { acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[ta], v[tb], acc[j], 0, 0, 0); };
+          mac(0, 2);
+          mac(1, 1);
+          mac(2, 0);
+          mac(0, 1);
+          mac(1, 0);
+          mac(0, 0);
         }
       }
     }
 #pragma unroll
-    for (int i = 0; i < RT; ++i)
+    for (int j = 0; j < CT; j += 4)
 #pragma unroll
-      for (int j = 0; j < CT; j += 4)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int n = n0 + i * 16 + k4 * 4 + e, col = col0 + j * 16 + li * 4;
-          if (n < last && col < g.d)
-            store_state4(out + (long)n * g.d + col, f32x4{acc[i][j][e], acc[i][j + 1][e], acc[i][j + 2][e], acc[i][j + 3][e]});
-        }
+      for (int e = 0; e < 4; ++e) {
+        const int n = n0 + k4 * 4 + e, col = w.col0 + j * 16 + li * 4;
+        if (n < w.last && col < g.d)
+          store_state4(out + (long)n * g.d + col, f32x4{acc[j][e], acc[j + 1][e], acc[j + 2][e], acc[j + 3][e]}, g.whole_lines);
+      }
   }
+}
+
+template <typename R, int CB>
+const void *fork_kernel() {
+  return reinterpret_cast<const void *>(k_shared_fork<R, CB>);
 }
 
 bool disjoint(const void *a, size_t na, const void *b, size_t nb) {
@@ -1038,11 +1102,11 @@ int check_prompts(bdh_ctx *ctx, int G, const int32_t *counts_host, int B, Prompt
 
 namespace {
 
-template <typename R, bool ROT, int MODE, int MODE4>
+template <typename R, bool STEP, int MODE, int MODE4>
 const void *pass_kernel(int rt) {
-  return rt == 1   ? reinterpret_cast<const void *>(k_shared_pass<R, 1, ROT, MODE>)
-         : rt == 2 ? reinterpret_cast<const void *>(k_shared_pass<R, 2, ROT, MODE>)
-                   : reinterpret_cast<const void *>(k_shared_pass<R, 4, ROT, MODE4>);
+  return rt == 1   ? reinterpret_cast<const void *>(k_shared_pass<R, 1, STEP, MODE>)
+         : rt == 2 ? reinterpret_cast<const void *>(k_shared_pass<R, 2, STEP, MODE>)
+                   : reinterpret_cast<const void *>(k_shared_pass<R, 4, STEP, MODE4>);
 }
 
 int launch_pass(bdh_ctx *ctx, const void *kernel, const char *name, dim3 grid, size_t lds, void **args) {
@@ -1141,8 +1205,7 @@ int bdh_launch_shared_steps(bdh_ctx *ctx, const SharedStepParams &p) {
   const int longest = p.longest < 0 ? S - T : p.longest;
   if (BH * T > 0x7fffffffL / 1024) return bdh_fail(ctx, BDH_E_SHAPE, "B*h*T too large");
   if (T >= kDenseTokens) return launch_dense(ctx, p, pr, rates, longest);
-  const bool rot = T == 1 && p.rotary != BDH_POPE;        // the queries are made where they are used
-  const bool half = p.rho_dtype == BDH_BF16 && d % 8 == 0;
+  const bool half = p.rho_dtype == BDH_BF16 && d >= 8;
   PassArgs g{};
   g.x = p.x; g.freqs = p.freqs; g.lens = p.lens_dev; g.positions = p.positions_dev; g.position = (long)p.position;
   g.rho = p.rho; g.keys = p.keys;
@@ -1184,7 +1247,7 @@ int bdh_launch_shared_steps(bdh_ctx *ctx, const SharedStepParams &p) {
   }
   if (g.row_blocks > 65535 || (long)p.G * h > 65535 || (long)h * Nq * 64 * 4 > 0xffffffffL)
     return bdh_fail(ctx, BDH_E_SHAPE, "h * Nq %ld too large", (long)h * Nq);
-  const size_t q_bytes = rot || alibi ? 0 : bdh_align_up(sizeof(float) * (size_t)BH * T * Nq, 256);
+  const size_t q_bytes = T == 1 || alibi ? 0 : bdh_align_up(sizeof(float) * (size_t)BH * T * Nq, 256);
   const size_t pt_bytes = bdh_align_up(sizeof(float) * (size_t)g.parts * BH * T * d, 256);
   const size_t sc_bytes = sizeof(float) * (size_t)g.score_parts_n * BH * T * g.span;
   rc = bdh_ws_reserve(ctx, q_bytes + pt_bytes + sc_bytes);
@@ -1193,7 +1256,7 @@ int bdh_launch_shared_steps(bdh_ctx *ctx, const SharedStepParams &p) {
   g.partial = reinterpret_cast<float *>(ws + q_bytes);
   g.score_parts = reinterpret_cast<float *>(ws + q_bytes + pt_bytes);
   g.q = q_bytes ? reinterpret_cast<float *>(ws) : p.x;
-  if (!rot) {
+  if (T > 1) {
     const AppendArgs aa{p.x, p.freqs, p.v, q_bytes ? reinterpret_cast<float *>(ws) : nullptr, p.keys, p.values, p.lens_dev,
                         p.positions_dev, (long)p.position, h, T, N, Nq, S, d, p.rotary, longest};
     hipLaunchKernelGGL(k_suffix_append, dim3((N + 63) / 64, (T + 31) / 32, (unsigned)BH), dim3(256), 0, ctx->stream, aa);
@@ -1204,9 +1267,9 @@ int bdh_launch_shared_steps(bdh_ctx *ctx, const SharedStepParams &p) {
     return std::max((size_t)16 * rt * (split ? 6 * (g.rows + 8) : 4 * (g.rows + 4)), g.cg == 4 ? 0 : 4 * sizeof(float) * 16 * rt * cols);
   };
   using h16 = unsigned short;
-  const void *kernel = p.rho_dtype == BDH_F32 ? (rot ? pass_kernel<float, true, kF32, kSplit>(rt) : pass_kernel<float, false, kF32, kSplit>(rt))
-                       : half                 ? (rot ? pass_kernel<h16, true, kHalf, kHalf>(rt) : pass_kernel<h16, false, kHalf, kHalf>(rt))
-                                              : (rot ? pass_kernel<h16, true, kF32, kF32>(rt) : pass_kernel<h16, false, kF32, kF32>(rt));
+  const void *kernel = p.rho_dtype == BDH_F32 ? (T == 1 ? pass_kernel<float, true, kF32, kSplit>(rt) : pass_kernel<float, false, kF32, kSplit>(rt))
+                       : half                 ? (T == 1 ? pass_kernel<h16, true, kHalf, kHalf>(rt) : pass_kernel<h16, false, kHalf, kHalf>(rt))
+                                              : (T == 1 ? pass_kernel<h16, true, kF32, kF32>(rt) : pass_kernel<h16, false, kF32, kF32>(rt));
   void *args[] = {&g, &pr};
   rc = launch_pass(ctx, kernel, "k_shared_pass", dim3((unsigned)(tiles * g.col_blocks), g.parts, p.G * h),
                    room(half || (rt == 4 && p.rho_dtype == BDH_F32), group), args);
@@ -1242,6 +1305,7 @@ int bdh_check_shared(bdh_ctx *ctx, int G, const int32_t *counts_host, int B, int
   if (rho_dtype != BDH_F32 && rho_dtype != BDH_BF16) return bdh_fail(ctx, BDH_E_INVAL, "rho_dtype %d is not a bdh_dtype value", rho_dtype);
   if (h > 64) return bdh_fail(ctx, BDH_E_SHAPE, "n_head %d > 64", h);
   if ((d & 3) || d > 1024) return bdh_fail(ctx, BDH_E_SHAPE, "d must be a multiple of 4 and <= 1024, got %d", d);
+  if ((long)Nq * capacity > 0x7fffffffL) return bdh_fail(ctx, BDH_E_SHAPE, "Nq * capacity %ld too large", (long)Nq * capacity);
   if ((capacity & 3) || capacity > (1 << 20)) return bdh_fail(ctx, BDH_E_SHAPE, "capacity must be a multiple of 4 and <= 2^20, got %d", capacity);
   if (longest > capacity) return bdh_fail(ctx, BDH_E_INVAL, "longest %d > capacity %d", longest, capacity);
   if ((long)T + std::max(longest, 0) > capacity)
@@ -1302,25 +1366,26 @@ int bdh_shared_prefix_fork(bdh_ctx *ctx, int G, const int32_t *counts_host, int 
     else bdh_default_alibi_slopes(h, slopes);
     for (int i = 0; i < h; ++i) rates.log_decay[i] = bdh_log_decay(slopes[i]);
   }
-  ForkArgs g{rho, rho_out, keys, values, lens_dev, B, h, Nq, d, capacity, longest < 0 ? capacity : longest, 0, 0, 0, 0, rotary == BDH_ALIBI};
-  // columns of a workgroup: as many as leave its LDS room for every token; a wavefront's tile is 16 x 256, 32 x 128 or 64 x 64
-  const int cols = g.longest <= 64 && d > 128 ? 256 : g.longest <= 128 && d > 64 ? 128 : 64;
-  const int tile = fork_waves(cols) * 16 * 256 / cols;  // rows that its wavefronts make at a time
+  ForkArgs g{rho, rho_out, keys, values, lens_dev, B, h, Nq, d, capacity, longest < 0 ? capacity : longest, 0, 0, 0, 0, rotary == BDH_ALIBI, false};
+  // columns of a workgroup: all, or equal shares of at most 320 (what its LDS has room for)
+  const int shares = (d + 319) / 320, cols = ((d + shares - 1) / shares + 63) / 64 * 64;
   g.col_blocks = (d + cols - 1) / cols;
-  g.rows = tile;
+  g.rows = fork_waves(cols) * 16;  // that its wavefronts make at a time
   while ((long)B * h * g.col_blocks * ((Nq + 2 * g.rows - 1) / (2 * g.rows)) >= 4L * ctx->n_cu) g.rows *= 2;
   g.row_blocks = (Nq + g.rows - 1) / g.rows;
-  g.groups = g.row_blocks * g.col_blocks * h;
-  if ((g.groups + 7L) / 8 * 8 * B > 0x7fffffffL) return bdh_fail(ctx, BDH_E_SHAPE, "too many tiles");
-  const size_t lds = (size_t)6 * cols * (64 * 256 / cols + 8);
-  using h16 = unsigned short;
+  g.groups = g.row_blocks * h;
+  g.whole_lines = (size_t)d * (rho_dtype == BDH_BF16 ? 2 : 4) % 128 == 0 && bdh_aligned(rho_out, 128);
+  if ((g.groups + 7L) / 8 * 8 * B * g.col_blocks > 0x7fffffffL) return bdh_fail(ctx, BDH_E_SHAPE, "too many tiles");
+  const size_t lds = (size_t)6 * cols * (kForkTokens + 8);
   const bool wide = rho_dtype == BDH_F32;
-  const void *kernel = cols == 256   ? (wide ? reinterpret_cast<const void *>(k_shared_fork<float, 256>) : reinterpret_cast<const void *>(k_shared_fork<h16, 256>))
-                       : cols == 128 ? (wide ? reinterpret_cast<const void *>(k_shared_fork<float, 128>) : reinterpret_cast<const void *>(k_shared_fork<h16, 128>))
-                                     : (wide ? reinterpret_cast<const void *>(k_shared_fork<float, 64>) : reinterpret_cast<const void *>(k_shared_fork<h16, 64>));
+  const void *kernel = cols == 64    ? (wide ? fork_kernel<float, 64>() : fork_kernel<unsigned short, 64>())
+                       : cols == 128 ? (wide ? fork_kernel<float, 128>() : fork_kernel<unsigned short, 128>())
+                       : cols == 192 ? (wide ? fork_kernel<float, 192>() : fork_kernel<unsigned short, 192>())
+                       : cols == 256 ? (wide ? fork_kernel<float, 256>() : fork_kernel<unsigned short, 256>())
+                                     : (wide ? fork_kernel<float, 320>() : fork_kernel<unsigned short, 320>());
   BDH_HIP_CHECK(ctx, hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
   void *args[] = {&g, &pr, &rates};
-  BDH_HIP_CHECK(ctx, hipLaunchKernel(kernel, dim3((unsigned)((g.groups + 7) / 8 * 8 * B)), dim3(64 * fork_waves(cols)), args, lds, ctx->stream));
+  BDH_HIP_CHECK(ctx, hipLaunchKernel(kernel, dim3((unsigned)((g.groups + 7) / 8 * 8 * B * g.col_blocks)), dim3(64 * fork_waves(cols)), args, lds, ctx->stream));
   return BDH_OK;
 }
 

@@ -7,6 +7,7 @@ namespace {
 
 constexpr int kMaxBuffers = BDH_MAX_SLOT_BUFFERS;
 constexpr int kInPlaceSlots = 1024;
+constexpr int kRun = 256;
 constexpr int kStageBytes = 64 * 1024;  // of LDS: two workgroups a CU
 
 struct SlotBuffer {
@@ -21,6 +22,7 @@ struct SlotBuffer {
 struct SlotArgs {
   SlotBuffer buf[kMaxBuffers];
   int n_buf, n, m;  // slots of the destination, of the source
+  int run;          // slots a workgroup takes (not in place)
   long tasks;
   const int32_t *origin;
 };
@@ -36,14 +38,14 @@ typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 // One chunk of every destination slot: a source is read once for a run of slots that take it.  What is written passes the
 // caches by (a state is larger than they are).
 template <typename P>
-__device__ __forceinline__ void copy_chunk(const SlotArgs &g, const SlotBuffer &f, long o, size_t p0, size_t p1) {
+__device__ __forceinline__ void copy_chunk(const SlotArgs &g, const SlotBuffer &f, long o, size_t p0, size_t p1, int i0, int i1, const int *origin) {
   const P *src = reinterpret_cast<const P *>(f.src) + (size_t)o * g.m * f.pieces;
   P *dst = reinterpret_cast<P *>(f.dst) + (size_t)o * g.n * f.pieces;
   const size_t p = p0 + threadIdx.x;
   P v[4];
   int held = -2;
-  for (int i = 0; i < g.n; ++i) {
-    const int from = g.origin[i];
+  for (int i = i0; i < i1; ++i) {
+    const int from = origin[i - i0];
     if (from < -1 || from >= g.m) continue;  // left as it is
     if (from != held) {
 #pragma unroll
@@ -56,15 +58,20 @@ __device__ __forceinline__ void copy_chunk(const SlotArgs &g, const SlotBuffer &
   }
 }
 
+// Grid: tasks, runs of slots.
 __global__ __launch_bounds__(256) void k_copy_slots(SlotArgs g) {
+  __shared__ int s_origin[kRun];
+  const int i0 = blockIdx.y * g.run, i1 = min(i0 + g.run, g.n);
+  if ((int)threadIdx.x < i1 - i0) s_origin[threadIdx.x] = g.origin[i0 + threadIdx.x];
+  __syncthreads();
   for (long task = blockIdx.x; task < g.tasks; task += gridDim.x) {
     const SlotBuffer &f = buffer_of(g, task);
     const long at = task - f.first, o = at / f.chunks;
     const size_t p0 = (size_t)(at - o * f.chunks) * f.chunk, p1 = p0 + f.chunk < f.pieces ? p0 + f.chunk : f.pieces;
-    if (f.unit == 16) copy_chunk<u32x4>(g, f, o, p0, p1);
-    else if (f.unit == 4) copy_chunk<uint32_t>(g, f, o, p0, p1);
-    else if (f.unit == 2) copy_chunk<uint16_t>(g, f, o, p0, p1);
-    else copy_chunk<uint8_t>(g, f, o, p0, p1);
+    if (f.unit == 16) copy_chunk<u32x4>(g, f, o, p0, p1, i0, i1, s_origin);
+    else if (f.unit == 4) copy_chunk<uint32_t>(g, f, o, p0, p1, i0, i1, s_origin);
+    else if (f.unit == 2) copy_chunk<uint16_t>(g, f, o, p0, p1, i0, i1, s_origin);
+    else copy_chunk<uint8_t>(g, f, o, p0, p1, i0, i1, s_origin);
   }
 }
 
@@ -214,11 +221,15 @@ extern "C" int bdh_copy_slots(bdh_ctx *ctx, const bdh_slot_buffer *buffers_host,
     g.tasks += f.chunks * f.outer;
   }
   const unsigned grid = (unsigned)std::min<long>(g.tasks, in_place ? 2L * ctx->n_cu : 8L * ctx->n_cu);
+  // few tasks: a source is read by several workgroups, so that the slots are written side by side
+  g.run = std::min(kRun, dst_slots);
+  while (g.run > 1 && (long)grid * ((dst_slots + g.run - 1) / g.run) < 2L * ctx->n_cu) g.run = (g.run + 1) / 2;
+  if ((dst_slots + g.run - 1) / g.run > 65535) return bdh_fail(ctx, BDH_E_SHAPE, "%d slots: too many", dst_slots);
   if (in_place) {
     hipLaunchKernelGGL(k_move_slots, dim3(grid), dim3(256), 0, ctx->stream, g);
     BDH_LAUNCH_CHECK(ctx, "k_move_slots");
   } else {
-    hipLaunchKernelGGL(k_copy_slots, dim3(grid), dim3(256), 0, ctx->stream, g);
+    hipLaunchKernelGGL(k_copy_slots, dim3(grid, (dst_slots + g.run - 1) / g.run), dim3(256), 0, ctx->stream, g);
     BDH_LAUNCH_CHECK(ctx, "k_copy_slots");
   }
   return BDH_OK;
