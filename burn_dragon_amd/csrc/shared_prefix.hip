@@ -42,6 +42,20 @@ __device__ __forceinline__ f32x4 load_state4(const unsigned short *p) {
                __uint_as_float(v.y & 0xffff0000u)};
 }
 
+// p[0] + p[step] + ... in order, eight of the n on their way at a time
+__device__ __forceinline__ float sum8(const float *p, long step, int n) {
+  float s = 0.0f;
+#pragma unroll 1
+  for (int q = 0; q < n; q += 8) {
+    float t[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) t[u] = p[min(q + u, n - 1) * step];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s += q + u < n ? t[u] : 0.0f;
+  }
+  return s;
+}
+
 // two floats as pairs (number m) of three bf16 terms, each rounded to the nearest: hi + mid + lo is the float
 __device__ __forceinline__ void split_pair(float a, float b, u32x4 (&terms)[3], int m) {
   const unsigned int hi = pack_bf16_rne(a, b);
@@ -80,7 +94,6 @@ __device__ __forceinline__ void rotate_pair(float pos, float f0, float f1, float
 
 // ---- queries times rows of a matrix -----------------------------------------------------------------------------------
 
-constexpr int kDenseTokens = 64;  // from here on: dense products
 constexpr int kRowsMost = 256;    // rows of the matrix a workgroup takes at a time
 
 struct PassArgs {
@@ -196,26 +209,20 @@ struct Product {
     const int part = rows == 256 ? 0 : wave >> 1, parts = rows == 256 ? 1 : 2;  // rows is 128 or 256
     const bool exists = r < have;
     const unsigned at = min(r, have - 1);
-    constexpr bool all = RT == 4;  // next to nothing of a row is silent in all of so many queries: no list
-    if (tid < rows) sh.used[tid] = all && exists ? tid + 1 : 0;
+    if (tid < rows) sh.used[tid] = 0;
     __syncthreads();
-    if constexpr (all) {
-      cnt = have;
-      sh.list[tid] = (unsigned short)(tid < have ? tid : 0);
-    } else {
-      bool used = false;
+    bool used = false;
 #pragma unroll 1
-      for (int i0 = part; i0 < nb; i0 += U * parts) {
-        float v[U];
+    for (int i0 = part; i0 < nb; i0 += U * parts) {
+      float v[U];
 #pragma unroll
-        for (int k = 0; k < U; ++k) v[k] = q[sh.row[min(i0 + k * parts, nb - 1)] * (long)ld_q + at];
+      for (int k = 0; k < U; ++k) v[k] = q[sh.row[min(i0 + k * parts, nb - 1)] * (long)ld_q + at];
 #pragma unroll
-        for (int k = 0; k < U; ++k) used |= v[k] != 0.0f;
-      }
-      if (used && exists) sh.used[r] = 1;
-      __syncthreads();
-      list_rows(rows);
+      for (int k = 0; k < U; ++k) used |= v[k] != 0.0f;
     }
+    if (used && exists) sh.used[r] = 1;
+    __syncthreads();
+    list_rows(rows);
     const int width = (cnt + kStep - 1) / kStep * kStep;
     for (int e = tid; e < (width - cnt) * kQ; e += 256) put(e % kQ, cnt + e / kQ, 0.0f);
     const int place = sh.used[r] - 1;
@@ -611,7 +618,7 @@ __global__ __launch_bounds__(256, 2) void k_suffix_scores(PassArgs g) {
   // keys behind the tile's last token are of no use to it
   if (!valid_len(len, g.T, g.longest, g.S) || col0 >= len + t0 + nb - 1) return;
   if (tid < 64) sh.row[tid] = (int)tid < nb ? bh * g.T + t0 + tid : 0;
-  Product<float, RT, RT == 4 ? kSplit : kF32> p(sh, s_dyn, g.rows);
+  Product<float, RT, kF32> p(sh, s_dyn, g.rows);
   int rb = part * g.score_per + min((int)part, g.score_longer);
   const int end = rb + g.score_per + ((int)part < g.score_longer ? 1 : 0);
 #pragma unroll 1
@@ -633,20 +640,6 @@ struct JoinArgs {
   long block_step, row_step;  // of the scores' parts
   bool decays;
 };
-
-// p[0] + p[step] + ... in order, eight of the n on their way at a time
-__device__ __forceinline__ float sum8(const float *p, long step, int n) {
-  float s = 0.0f;
-#pragma unroll 1
-  for (int q = 0; q < n; q += 8) {
-    float t[8];
-#pragma unroll
-    for (int u = 0; u < 8; ++u) t[u] = p[min(q + u, n - 1) * step];
-#pragma unroll
-    for (int u = 0; u < 8; ++u) s += q + u < n ? t[u] : 0.0f;
-  }
-  return s;
-}
 
 // out = a^k * (the parts of q rho) + sum_s a^(k-s) score_s v_s, in the order of the parts and of the tokens, for TT tokens of a
 // (sequence, head); a column's parts and values are dealt to as many threads as a workgroup of 1024 has for it.  One token: its
@@ -848,15 +841,15 @@ __global__ __launch_bounds__(256) void k_suffix_append(AppendArgs g) {
 struct MaskArgs {
   const float *score_parts;  // [ks][B*h][T][span]
   float *scores;             // [B*h][T][lds]
-  const float *out_parts;    // [ko][rows in the order of the products][d]
+  const float *out_parts;    // of each launch [ko][slices][queries of a slice][d]
   float *out;                // [B*h][T][d]
   const int32_t *lens;
   int B, h, T, d, S, span, lds, ks, ko, longest;
-  bool decays;
+  bool decays, even;  // even: one launch for all prompts
 };
 
 // Scores of a token with the keys before its own, decayed; and its readout of the prompt's state, decayed.  A workgroup a token.
-__global__ __launch_bounds__(256) void k_shared_scores(MaskArgs g, HeadRates rates) {
+__global__ __launch_bounds__(256) void k_shared_scores(MaskArgs g, HeadRates rates, Prompts pr) {
   const long row = blockIdx.x;
   const int t = (int)(row % g.T), bh = (int)(row / g.T), b = bh / g.h, hh = bh - b * g.h, tid = threadIdx.x;
   const int len = g.lens[b], k = len + t;
@@ -867,15 +860,25 @@ __global__ __launch_bounds__(256) void k_shared_scores(MaskArgs g, HeadRates rat
   for (int s = tid; s < g.lds; s += 256) {
     float v = 0.0f;
     if (valid && s < k) {
-      v = g.ks > 1 ? bdh_sum_in_order(g.score_parts + row * g.span + s, step, g.ks) : sc[s];
+      v = g.ks > 1 ? sum8(g.score_parts + row * g.span + s, step, g.ks) : sc[s];
       if (g.decays) v *= expf((float)(k - s) * ld);
     }
     sc[s] = v;
   }
   const float scale = !valid ? __uint_as_float(0x7fc00000u) : g.decays ? expf((float)k * ld) : 1.0f;
   float *out = g.out + row * g.d;
+  const float *parts = g.out_parts;
+  long step_o = 0;
+  if (g.ko > 1) {
+    int grp = 0;
+    while (grp + 1 < pr.G && b >= pr.begin[grp + 1]) ++grp;
+    const int first = pr.begin[grp];
+    const long m = (long)(pr.begin[grp + 1] - first) * g.T, slices = g.even ? (long)pr.G * g.h : g.h;
+    step_o = slices * m * g.d;
+    parts += (g.even ? 0 : (long)g.ko * g.h * first * g.T * g.d) + (((g.even ? grp * g.h : 0) + hh) * m + (long)(b - first) * g.T + t) * g.d;
+  }
   for (int c = tid; c < g.d; c += 256) {
-    const float v = g.ko > 1 ? bdh_sum_in_order(g.out_parts + row * g.d + c, (long)g.B * g.h * g.T * g.d, g.ko) : out[c];
+    const float v = g.ko > 1 ? sum8(parts + c, step_o, g.ko) : out[c];
     out[c] = v * scale;
   }
 }
@@ -1102,11 +1105,13 @@ int check_prompts(bdh_ctx *ctx, int G, const int32_t *counts_host, int B, Prompt
 
 namespace {
 
-template <typename R, bool STEP, int MODE, int MODE4>
-const void *pass_kernel(int rt) {
-  return rt == 1   ? reinterpret_cast<const void *>(k_shared_pass<R, 1, STEP, MODE>)
-         : rt == 2 ? reinterpret_cast<const void *>(k_shared_pass<R, 2, STEP, MODE>)
-                   : reinterpret_cast<const void *>(k_shared_pass<R, 4, STEP, MODE4>);
+// one token: tiles of 64 sequences where a prompt has more than 32
+template <typename R, int MODE, int MODE4>
+const void *pass_kernel(int T, int rt) {
+  if (T > 1) return rt == 1 ? reinterpret_cast<const void *>(k_shared_pass<R, 1, false, MODE>) : reinterpret_cast<const void *>(k_shared_pass<R, 2, false, MODE>);
+  return rt == 1   ? reinterpret_cast<const void *>(k_shared_pass<R, 1, true, MODE>)
+         : rt == 2 ? reinterpret_cast<const void *>(k_shared_pass<R, 2, true, MODE>)
+                   : reinterpret_cast<const void *>(k_shared_pass<R, 4, true, MODE4>);
 }
 
 int launch_pass(bdh_ctx *ctx, const void *kernel, const char *name, dim3 grid, size_t lds, void **args) {
@@ -1141,19 +1146,28 @@ int launch_dense(bdh_ctx *ctx, const SharedStepParams &p, const Prompts &pr, con
   const size_t most = size_t(256) << 20, one_s = sizeof(float) * (size_t)BH * T * span;
   const GemmPlan ps = bdh_gemm_f32_plan(ctx, s, (int)std::min<size_t>(32, std::max<size_t>(1, most / one_s)));
   const GemmPlan pw = bdh_gemm_f32_plan(ctx, w, 1);
+  // one plan for all prompts, made for the one with most sequences
+  int widest = 0;
+  for (int i = 0; i < p.G; ++i) widest = std::max(widest, pr.begin[i + 1] - pr.begin[i]);
+  o.M = widest * T;
+  o.n_slices = even ? p.G * h : h;
+  const size_t one_o = sizeof(float) * (size_t)BH * T * d;
+  const GemmPlan po = bdh_gemm_f32_plan(ctx, o, (int)std::min<size_t>(32, std::max<size_t>(1, most / one_o)));
   const size_t n_state = (size_t)p.G * h * Nq * d;
   const size_t q_bytes = alibi ? 0 : bdh_align_up(sizeof(float) * (size_t)BH * T * Nq, 256);
   const size_t sc_bytes = bdh_align_up(sizeof(float) * (size_t)BH * T * lds, 256);
   const size_t parts_bytes = ps.ks > 1 ? bdh_align_up(one_s * ps.ks, 256) : 0;
+  const size_t out_bytes = po.ks > 1 ? bdh_align_up(one_o * po.ks, 256) : 0;
   const size_t wide_bytes = p.rho_dtype == BDH_BF16 ? bdh_align_up(sizeof(float) * n_state, 256) : 0;
-  rc = bdh_ws_reserve(ctx, q_bytes + sc_bytes + parts_bytes + wide_bytes);
+  rc = bdh_ws_reserve(ctx, q_bytes + sc_bytes + parts_bytes + out_bytes + wide_bytes);
   if (rc != BDH_OK) return rc;
   char *ws = static_cast<char *>(ctx->ws);
   float *q = alibi ? nullptr : reinterpret_cast<float *>(ws);
   float *scores = reinterpret_cast<float *>(ws + q_bytes), *parts = reinterpret_cast<float *>(ws + q_bytes + sc_bytes);
+  float *out_parts = reinterpret_cast<float *>(ws + q_bytes + sc_bytes + parts_bytes);
   const float *rho = static_cast<const float *>(p.rho);
   if (wide_bytes) {
-    float *wide = reinterpret_cast<float *>(ws + q_bytes + sc_bytes + parts_bytes);
+    float *wide = reinterpret_cast<float *>(ws + q_bytes + sc_bytes + parts_bytes + out_bytes);
     hipLaunchKernelGGL(k_widen_state, dim3((unsigned)std::min<size_t>((n_state / 4 + 255) / 256, 16384)), dim3(256), 0, ctx->stream,
                        static_cast<const unsigned short *>(p.rho), wide, n_state / 4);
     BDH_LAUNCH_CHECK(ctx, "k_widen_state");
@@ -1173,14 +1187,14 @@ int launch_dense(bdh_ctx *ctx, const SharedStepParams &p, const Prompts &pr, con
     g.A = queries + (long)first * h * T * Nq;
     g.B = rho + (even ? 0 : (long)i * h * Nq * d);
     g.C = p.out + (long)first * h * T * d;
-    rc = bdh_launch_gemm_f32(ctx, g, false, true, bdh_gemm_f32_plan(ctx, g, 1), nullptr);
+    rc = bdh_launch_gemm_f32(ctx, g, false, true, po, out_parts + (size_t)po.ks * h * first * T * d);
     if (rc != BDH_OK) return rc;
   }
   s.A = queries; s.B = p.keys; s.C = scores;
   rc = bdh_launch_gemm_f32(ctx, s, false, true, ps, parts);
   if (rc != BDH_OK) return rc;
-  const MaskArgs ma{parts, scores, nullptr, p.out, p.lens_dev, B, h, T, d, S, span, lds, ps.ks, 1, longest, alibi};
-  hipLaunchKernelGGL(k_shared_scores, dim3((unsigned)(BH * T)), dim3(256), 0, ctx->stream, ma, rates);
+  const MaskArgs ma{parts, scores, out_parts, p.out, p.lens_dev, B, h, T, d, S, span, lds, ps.ks, po.ks, longest, alibi, even};
+  hipLaunchKernelGGL(k_shared_scores, dim3((unsigned)(BH * T)), dim3(256), 0, ctx->stream, ma, rates, pr);
   BDH_LAUNCH_CHECK(ctx, "k_shared_scores");
   w.A = scores; w.B = p.values; w.C = p.out;
   rc = bdh_launch_gemm_f32(ctx, w, false, true, pw, nullptr);
@@ -1204,7 +1218,6 @@ int bdh_launch_shared_steps(bdh_ctx *ctx, const SharedStepParams &p) {
     for (int i = 0; i < h; ++i) rates.log_decay[i] = bdh_log_decay(p.slopes_host[i]);
   const int longest = p.longest < 0 ? S - T : p.longest;
   if (BH * T > 0x7fffffffL / 1024) return bdh_fail(ctx, BDH_E_SHAPE, "B*h*T too large");
-  if (T >= kDenseTokens) return launch_dense(ctx, p, pr, rates, longest);
   const bool half = p.rho_dtype == BDH_BF16 && d >= 8;
   PassArgs g{};
   g.x = p.x; g.freqs = p.freqs; g.lens = p.lens_dev; g.positions = p.positions_dev; g.position = (long)p.position;
@@ -1212,6 +1225,10 @@ int bdh_launch_shared_steps(bdh_ctx *ctx, const SharedStepParams &p) {
   g.B = B; g.h = h; g.T = T; g.N = N; g.Nq = Nq; g.d = d; g.S = S; g.rotary = p.rotary; g.longest = longest;
   long most = 1;  // queries of a prompt
   for (int i = 0; i < p.G; ++i) most = std::max(most, (long)(pr.begin[i + 1] - pr.begin[i]) * T);
+  // Several tokens: more than 32 queries of a prompt go through dense products (us, here | there: 6 sequences of one prompt, 4
+  // heads of 8192, d = 256, 2 tokens 57 | 95, 4 tokens 73 | 94, 8 tokens 118 | 98, 63 tokens 198 | 202; 4 sequences, 4 heads of
+  // 256, 8 tokens 27 | 36, 24 tokens 36 | 35; 16 sequences, 8 heads of 4096, d = 512, 2 tokens 102 | 112, 4 tokens 171 | 117)
+  if (T > 1 && most > 32) return launch_dense(ctx, p, pr, rates, longest);
   const int rt = most <= 16 ? 1 : most <= 32 ? 2 : 4;
   const long tiles = (most + 16 * rt - 1) / (16 * rt);
   // rows and columns of a workgroup: as many as leave two workgroups for every CU
@@ -1266,20 +1283,17 @@ int bdh_launch_shared_steps(bdh_ctx *ctx, const SharedStepParams &p) {
   auto room = [&](bool split, int cols) {
     return std::max((size_t)16 * rt * (split ? 6 * (g.rows + 8) : 4 * (g.rows + 4)), g.cg == 4 ? 0 : 4 * sizeof(float) * 16 * rt * cols);
   };
-  using h16 = unsigned short;
-  const void *kernel = p.rho_dtype == BDH_F32 ? (T == 1 ? pass_kernel<float, true, kF32, kSplit>(rt) : pass_kernel<float, false, kF32, kSplit>(rt))
-                       : half                 ? (T == 1 ? pass_kernel<h16, true, kHalf, kHalf>(rt) : pass_kernel<h16, false, kHalf, kHalf>(rt))
-                                              : (T == 1 ? pass_kernel<h16, true, kF32, kF32>(rt) : pass_kernel<h16, false, kF32, kF32>(rt));
+  const void *kernel = p.rho_dtype == BDH_F32 ? pass_kernel<float, kF32, kSplit>(T, rt)
+                       : half                 ? pass_kernel<unsigned short, kHalf, kHalf>(T, rt)
+                                              : pass_kernel<unsigned short, kF32, kF32>(T, rt);
   void *args[] = {&g, &pr};
   rc = launch_pass(ctx, kernel, "k_shared_pass", dim3((unsigned)(tiles * g.col_blocks), g.parts, p.G * h),
                    room(half || (rt == 4 && p.rho_dtype == BDH_F32), group), args);
   if (rc != BDH_OK) return rc;
   if (T > 1) {
-    const void *scores = rt == 1   ? reinterpret_cast<const void *>(k_suffix_scores<1>)
-                         : rt == 2 ? reinterpret_cast<const void *>(k_suffix_scores<2>)
-                                   : reinterpret_cast<const void *>(k_suffix_scores<4>);
+    const void *scores = rt == 1 ? reinterpret_cast<const void *>(k_suffix_scores<1>) : reinterpret_cast<const void *>(k_suffix_scores<2>);
     rc = launch_pass(ctx, scores, "k_suffix_scores", dim3((unsigned)(score_tiles * g.score_cols), g.score_parts_n, (unsigned)BH),
-                     room(rt == 4, 64), args);
+                     room(false, 64), args);
     if (rc != BDH_OK) return rc;
   }
   const long rows = BH * T;
