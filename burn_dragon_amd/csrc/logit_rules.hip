@@ -30,7 +30,7 @@ __device__ __forceinline__ float ruled(float z, int seen, const RowRules &r, flo
   if (r.counted) {
     const float times = (float)(seen & 0x7fffffff);
     if (seen != 0) z = z > 0.0f ? z / r.repetition : z * r.repetition;
-    z = z - (r.frequency * times + (times > 0.0f ? r.presence : 0.0f));
+    if (times > 0.0f) z = z - (r.frequency * times + r.presence);
   }
   return allowed ? z + bias : -INFINITY;
 }
@@ -84,8 +84,14 @@ __global__ __launch_bounds__(256) void k_count_tokens(const int64_t *__restrict_
     if (v < 0 || v >= V) continue;
     if (prompt) {
       if (row[v] >= 0) atomicOr(row + v, kInPrompt);  // a stale value only asks for the mark once more
-    } else {
+    } else if (!(row[v] & 0x40000000)) {
       atomicAdd(row + v, 1);
+    } else {  // counts end at 2^31 - 1: the bit above them is the prompt's
+      for (int32_t had = row[v]; (had & 0x7fffffff) != 0x7fffffff;) {
+        const int32_t now = atomicCAS(row + v, had, had + 1);
+        if (now == had) break;
+        had = now;
+      }
     }
   }
 }
@@ -120,6 +126,17 @@ int bdh_logit_rules(bdh_ctx *ctx, int B, int V, const float *logits, int64_t row
   const size_t in_bytes = sizeof(float) * ((size_t)(B - 1) * row_stride + V), out_bytes = sizeof(float) * ((size_t)(B - 1) * out_stride + V);
   if (!(logits == out && (row_stride == out_stride || B == 1)) && overlap(logits, in_bytes, out, out_bytes))
     return bdh_fail(ctx, BDH_E_INVAL, "out overlaps the logits without being them");
+  const size_t row = sizeof(float) * (size_t)B, counts = sizeof(int32_t) * (size_t)B * V;
+  const struct {
+    const void *p;
+    size_t bytes;
+  } reads[] = {{newest, sizeof(int64_t) * (size_t)B}, {repetition, row}, {presence, row}, {frequency, row},
+               {bias, sizeof(float) * ((size_t)(B - 1) * bias_stride + V)}, {allowed, sizeof(int32_t) * ((size_t)(B - 1) * allowed_stride + words)}};
+  for (const auto &r : reads)
+    if (r.p && (overlap(r.p, r.bytes, out, out_bytes) || (seen && overlap(r.p, r.bytes, seen, counts))))
+      return bdh_fail(ctx, BDH_E_INVAL, "out or seen overlaps what the rules read");
+  if (seen && (overlap(seen, counts, out, out_bytes) || overlap(seen, counts, logits, in_bytes)))
+    return bdh_fail(ctx, BDH_E_INVAL, "seen overlaps the logits or out");
   const RulesArgs g{logits, out, (long)row_stride, (long)out_stride, (long)bias_stride, (long)allowed_stride, V, seen, newest,
                     repetition, presence, frequency, bias, allowed};
   hipLaunchKernelGGL(k_logit_rules, dim3((V + 1023) / 1024, B), dim3(256), 0, ctx->stream, g);

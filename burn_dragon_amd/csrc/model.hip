@@ -522,6 +522,15 @@ int bdh_model_fork_shared(bdh_model *m, int G, const int32_t *counts_host, int B
   const int Nq = c.rotary == BDH_POPE ? 2 * c.latent : c.latent;
   if (B > 0 && (!rho || !keys || !values || !rho_out)) return bdh_fail(ctx, BDH_E_INVAL, "null data pointer");
   const size_t state = (size_t)c.n_head * Nq * c.n_embd * (rho_dtype == BDH_BF16 ? 2 : 4);
+  if (B > 0 && G > 0 && c.n_layer > 0) {  // a layer's states are written before the next one's prompts and keys are read
+    const size_t L = c.n_layer, key_bytes = sizeof(float) * L * B * c.n_head * Nq * std::max(capacity, 0);
+    auto apart = [&](const void *p, size_t n) {
+      const char *a = static_cast<const char *>(p), *o = static_cast<const char *>(rho_out);
+      return a >= o + L * B * state || o >= a + n;
+    };
+    if (!apart(rho, L * G * state) || !apart(keys, key_bytes) || !apart(values, sizeof(float) * L * B * std::max(capacity, 0) * c.n_embd))
+      return bdh_fail(ctx, BDH_E_INVAL, "rho_out overlaps what the forks read");
+  }
   for (int l = 0; l < c.n_layer; ++l) {
     const int rc = bdh_shared_prefix_fork(ctx, G, counts_host, B, c.n_head, Nq, c.n_embd, c.rotary,
                                           c.rotary == BDH_ALIBI ? m->slopes : nullptr,

@@ -1035,8 +1035,8 @@ __global__ __launch_bounds__(64 * fork_waves(CB)) void k_shared_fork(ForkArgs g,
         u32x4 o[3];
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-          const bool in = s0 + t + k4 * 8 + (m >> 1) * 4 < end;
-          split_pair(in ? ahead[0][m >> 1][(m & 1) * 2] : 0.0f, in ? ahead[0][m >> 1][(m & 1) * 2 + 1] : 0.0f, o, m);
+          const int s = s0 + t + k4 * 8 + m * 2;  // what lies behind the last token is not looked at
+          split_pair(s < end ? ahead[0][m >> 1][(m & 1) * 2] : 0.0f, s + 1 < end ? ahead[0][m >> 1][(m & 1) * 2 + 1] : 0.0f, o, m);
         }
         bf16x8 a[3];
 #pragma unroll
@@ -1321,6 +1321,7 @@ int bdh_check_shared(bdh_ctx *ctx, int G, const int32_t *counts_host, int B, int
   if ((d & 3) || d > 1024) return bdh_fail(ctx, BDH_E_SHAPE, "d must be a multiple of 4 and <= 1024, got %d", d);
   if ((long)Nq * capacity > 0x7fffffffL) return bdh_fail(ctx, BDH_E_SHAPE, "Nq * capacity %ld too large", (long)Nq * capacity);
   if ((capacity & 3) || capacity > (1 << 20)) return bdh_fail(ctx, BDH_E_SHAPE, "capacity must be a multiple of 4 and <= 2^20, got %d", capacity);
+  if (longest < -1) return bdh_fail(ctx, BDH_E_INVAL, "longest %d is neither a length nor -1", longest);
   if (longest > capacity) return bdh_fail(ctx, BDH_E_INVAL, "longest %d > capacity %d", longest, capacity);
   if ((long)T + std::max(longest, 0) > capacity)
     return bdh_fail(ctx, BDH_E_INVAL, "%d tokens after %d do not fit a capacity of %d", T, std::max(longest, 0), capacity);
@@ -1373,6 +1374,8 @@ int bdh_shared_prefix_fork(bdh_ctx *ctx, int G, const int32_t *counts_host, int 
   if (!bdh_aligned(rho_out, 16)) return bdh_fail(ctx, BDH_E_ALIGN, "rho_out needs 16-byte alignment");
   const size_t slot = (size_t)h * Nq * d * (rho_dtype == BDH_BF16 ? 2 : 4);
   if (!disjoint(rho, slot * G, rho_out, slot * B)) return bdh_fail(ctx, BDH_E_INVAL, "rho_out overlaps the prompts' states");
+  if (!disjoint(keys, sizeof(float) * B * h * Nq * capacity, rho_out, slot * B) || !disjoint(values, sizeof(float) * B * capacity * d, rho_out, slot * B))
+    return bdh_fail(ctx, BDH_E_INVAL, "rho_out overlaps the keys or values");
   HeadRates rates{};
   if (rotary == BDH_ALIBI) {
     float slopes[64];

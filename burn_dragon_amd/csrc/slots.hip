@@ -188,6 +188,9 @@ extern "C" int bdh_copy_slots(bdh_ctx *ctx, const bdh_slot_buffer *buffers_host,
     } else if (d < s + src_bytes && s < d + dst_bytes) {
       return bdh_fail(ctx, BDH_E_INVAL, "buffer %d: destination overlaps the source without being it", i);
     }
+    const char *map = reinterpret_cast<const char *>(origin_dev);
+    if (d < map + sizeof(int32_t) * (size_t)dst_slots && map < d + dst_bytes)
+      return bdh_fail(ctx, BDH_E_INVAL, "buffer %d: origin is part of the destination", i);
     for (int k = 0; k < g.n_buf; ++k) {
       const SlotBuffer &o = g.buf[k];
       const size_t ob = (size_t)o.outer * dst_slots * o.slot_bytes, os = (size_t)o.outer * src_slots * o.slot_bytes;

@@ -243,6 +243,21 @@ class Context:
             pass
 
 
+def context_on(device, ctx: Optional[Context] = None) -> Context:
+    """The context for tensors on `device` (ctx, or the device's default one).  Refuses what no kernel may be given: tensors
+    in host memory, a context of another device, a device that is not the current one."""
+    import torch
+
+    if device.type != "cuda":
+        raise ValueError(f"tensors on {device}: this operator runs on a HIP device")
+    if torch.cuda.current_device() != device.index:
+        raise ValueError(f"tensors on {device}, the current device is cuda:{torch.cuda.current_device()}")
+    ctx = ctx or default_context(device.index)
+    if ctx.device_id != device.index:
+        raise ValueError(f"tensors on {device}, the context is on cuda:{ctx.device_id}")
+    return ctx
+
+
 _default_ctx = {}
 
 

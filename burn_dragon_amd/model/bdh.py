@@ -192,6 +192,18 @@ class BDH:
         state.reset()
         return shared
 
+    def _check_shared(self, shared: SharedState) -> int:
+        """The number of prompts of a shared state that is this model's."""
+        L, h, Nq, d, S, B, G = (self.n_layer, self.n_head, self.latent_q, self.n_embd, shared.capacity, shared.batch,
+                                len(shared.counts))
+        rho_dtype = torch.bfloat16 if self.rho_dtype == ffi.BF16 else torch.float32
+        for t, shape, dtype in [(shared.rho, (L, G, h, Nq, d), rho_dtype), (shared.keys, (L, B, h, Nq, S), torch.float32),
+                                (shared.values, (L, B, S, d), torch.float32), (shared.lens, (B,), torch.int32),
+                                (shared.positions, (B,), torch.int32)]:
+            if tuple(t.shape) != shape or t.dtype is not dtype or t.device != self.params["embed"].device or not t.is_contiguous():
+                raise ValueError("the shared state belongs to another model")
+        return G
+
     def forward_shared(self, tokens: torch.Tensor, shared: SharedState, want_next: bool = False):
         """forward_with_state for sequences that share their prompts' states: tokens [B,T] int64 -> logits [B,T,V] (and the
         greedy next tokens, kept on the device, when want_next)."""
@@ -201,10 +213,9 @@ class BDH:
             raise ValueError(f"{B} rows of tokens for {shared.batch} sequences")
         if T > shared.room:
             raise ValueError(f"{T} tokens, room for {shared.room}: fork_shared gives the sequences states of their own")
-        L, G = shared.rho.shape[:2]
-        expected = (self.n_layer, B, self.n_head, self.latent_q, shared.capacity)
-        if tuple(shared.keys.shape) != expected or tuple(shared.rho.shape[2:]) != (self.n_head, self.latent_q, self.n_embd):
-            raise ValueError("the shared state belongs to another model")
+        if torch.cuda.is_current_stream_capturing():
+            raise ValueError("forward_shared counts the tokens on the host: capture shared_prefix_attention instead")
+        G = self._check_shared(shared)
         counts = np.ascontiguousarray(shared.counts, np.int32)
         logits = torch.empty((B, T, self.vocab_size), device=self.device, dtype=torch.float32)
         nxt = torch.empty((B,), device=self.device, dtype=torch.int64) if want_next else None
@@ -221,8 +232,7 @@ class BDH:
     def fork_shared(self, shared: SharedState) -> ModelState:
         """States of their own for the sequences of a shared state: what forward_with_state would have left after the same
         tokens.  The shared state is left as it is."""
-        L, G = shared.rho.shape[:2]
-        B = shared.batch
+        G, L, B = self._check_shared(shared), self.n_layer, shared.batch
         counts = np.ascontiguousarray(shared.counts, np.int32)
         state = self.init_state()
         state.storage = torch.empty((L, B, self.n_head, self.latent_q, self.n_embd), device=self.device, dtype=shared.rho.dtype)

@@ -24,6 +24,10 @@ class LogitRules:
     bias: Optional[torch.Tensor] = None
     allowed: Optional[torch.Tensor] = None
 
+    def __post_init__(self):
+        if self.repetition is not None and not torch.is_tensor(self.repetition) and not self.repetition > 0:
+            raise ValueError(f"repetition divides and multiplies logits: it is positive, not {self.repetition}")
+
     @property
     def penalises(self) -> bool:
         return any(p is not None for p in (self.repetition, self.presence, self.frequency))
@@ -87,7 +91,7 @@ def count_tokens(tokens: torch.Tensor, seen: torch.Tensor, lens: Optional[torch.
         raise ValueError("tokens: expected int64 rows")
     if lens is not None and (lens.shape != (B,) or lens.dtype is not torch.int32 or lens.device != dev or not lens.is_contiguous()):
         raise ValueError(f"lens: expected int32 [{B}] on {dev}")
-    ctx = ctx or ffi.default_context(dev.index or 0)
+    ctx = ffi.context_on(dev, ctx)
     ctx.check(ctx.lib.bdh_count_tokens(ctx.handle, B, T, V, ffi.ptr(tokens), tokens.stride(0) if B > 1 else max(T, 1),
                                        ffi.ptr(lens), int(bool(prompt)), ffi.ptr(seen)))
 
@@ -126,7 +130,7 @@ def apply_rules(logits: torch.Tensor, rules: LogitRules, seen: Optional[torch.Te
         out = torch.empty_like(logits) if logits.is_contiguous() else torch.empty((B, V), device=dev, dtype=torch.float32)
     elif out.shape != (B, V) or out.dtype is not torch.float32 or out.device != dev or (V > 1 and out.stride(1) != 1):
         raise ValueError(f"out: expected f32 rows [{B}, {V}] on {dev}")
-    ctx = ctx or ffi.default_context(dev.index or 0)
+    ctx = ffi.context_on(dev, ctx)
     ctx.check(ctx.lib.bdh_logit_rules(
         ctx.handle, B, V, logits.data_ptr(), logits.stride(0) if B > 1 else V, None if seen is None else seen.data_ptr(),
         None if newest is None else newest.data_ptr(), *[None if p is None else p.data_ptr() for p in penalties],

@@ -67,11 +67,13 @@ def shared_prefix_attention(query: torch.Tensor, value: torch.Tensor, rho: torch
     if positions is not None:
         _check("positions", positions, (B,), torch.int32, dev)
     if rot != RotaryEmbedding.ALIBI:
+        if freqs is None:
+            raise ValueError(f"{rot.name} needs its frequencies")
         freqs = freqs.reshape(-1)
         _check("freqs", freqs, (N,), torch.float32, dev)
     n_of = _prompts(counts, G, B)
     slopes = _slopes(alibi_slopes, h)
-    ctx = ctx or ffi.default_context(dev.index or 0)
+    ctx = ffi.context_on(dev, ctx)
     out = torch.empty((B, h, T, d), device=dev, dtype=torch.float32)
     ctx.check(ctx.lib.bdh_shared_prefix_attention(
         ctx.handle, G, n_of, B, h, T, N, d, int(rot), query.data_ptr(), value.data_ptr(),
@@ -101,7 +103,7 @@ def shared_prefix_fork(rho: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     _check("out", out, (B, h, Nq, d), rho.dtype, dev)
     n_of = _prompts(counts, G, B)
     slopes = _slopes(alibi_slopes, h)
-    ctx = ctx or ffi.default_context(dev.index or 0)
+    ctx = ffi.context_on(dev, ctx)
     ctx.check(ctx.lib.bdh_shared_prefix_fork(
         ctx.handle, G, n_of, B, h, Nq, d, int(RotaryEmbedding.parse(rotary_embedding)), slopes,
         rho.data_ptr(), _DTYPES[rho.dtype], S, lens.data_ptr(), -1 if longest is None else int(longest), keys.data_ptr(),

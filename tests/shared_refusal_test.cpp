@@ -69,6 +69,7 @@ int main() {
   READ(BDH_E_INVAL, r.longest = 8);
   READ(BDH_E_INVAL, r.longest = 0x7fffffff);
   READ(BDH_E_INVAL, r.T = 4; r.longest = 5);
+  READ(BDH_E_INVAL, r.longest = -2);
   READ(BDH_E_INVAL, r.position = -1);
   READ(BDH_E_INVAL, r.x = nullptr);
   READ(BDH_E_INVAL, r.v = nullptr);
@@ -98,6 +99,8 @@ int main() {
   FORK(BDH_E_INVAL, 2, 5, 6, 8, BDH_ROPE, buf, 8, -1, nullptr);
   FORK(BDH_E_ALIGN, 2, 5, 6, 8, BDH_ROPE, buf, 8, -1, buf + 2049);
   FORK(BDH_E_INVAL, 2, 5, 6, 8, BDH_ROPE, buf, 8, -1, buf + 64);
+  EXPECT(BDH_E_INVAL, bdh_shared_prefix_fork(&ctx, 2, counts, 5, 2, 6, 8, BDH_ROPE, nullptr, buf, BDH_F32, 8, ints, -1, buf + 1024, f, buf + 1000));
+  EXPECT(BDH_E_INVAL, bdh_shared_prefix_fork(&ctx, 2, counts, 5, 2, 6, 8, BDH_ROPE, nullptr, buf, BDH_F32, 8, ints, -1, f, buf + 1304, buf + 1000));
   // slots
   auto slots = [&](bdh_slot_buffer a, bdh_slot_buffer b, int n, int m, int count = 2) {
     const bdh_slot_buffer t[2] = {a, b};
@@ -122,6 +125,8 @@ int main() {
   EXPECT(BDH_E_INVAL, slots({buf, buf + 64, 16, 1}, {buf + 128, buf + 4, 16, 1}, 4, 4));    // one reads what the other writes
   EXPECT(BDH_E_INVAL, slots({buf, buf + 64, 16, 1}, {buf + 68, buf + 128, 16, 1}, 4, 4));
   EXPECT(BDH_E_SHAPE, slots({buf, buf, 1, 1}, none, 1025, 1025));
+  EXPECT(BDH_E_INVAL, slots({ints, buf, 4, 1}, none, 4, 4));      // what is written holds the map
+  EXPECT(BDH_E_INVAL, slots({ints, ints, 16, 1}, none, 4, 4));
   // rules
   int64_t toks[4];
 #define RULES(want, B, V, ld, seen, newest, pen, bias, bs, al, as, in, out, os) \
@@ -141,6 +146,13 @@ int main() {
   RULES(BDH_E_INVAL, 2, 8, 8, ints, toks, f, f, 0, ints, 0, buf, nullptr, 8);
   RULES(BDH_E_INVAL, 2, 8, 8, ints, toks, f, f, 0, ints, 0, buf, buf + 4, 8);
   RULES(BDH_E_INVAL, 2, 8, 8, ints, toks, f, f, 0, ints, 0, buf, buf, 9);
+  float *seen_f = reinterpret_cast<float *>(ints);
+  RULES(BDH_E_INVAL, 2, 8, 8, ints, toks, f, buf + 68, 8, nullptr, 0, buf, buf + 64, 8);             // out is part of the bias
+  RULES(BDH_E_INVAL, 1, 8, 8, nullptr, nullptr, nullptr, nullptr, 0, ints + 7, 0, buf, seen_f, 8);   // of the mask
+  RULES(BDH_E_INVAL, 2, 8, 8, ints, toks, buf + 65, nullptr, 0, nullptr, 0, buf, buf + 64, 8);       // of a penalty
+  RULES(BDH_E_INVAL, 2, 8, 8, ints, toks, f, nullptr, 0, nullptr, 0, buf + 64, seen_f + 15, 8);      // of the counts
+  RULES(BDH_E_INVAL, 2, 8, 8, ints, toks, f, nullptr, 0, nullptr, 0, seen_f, buf + 64, 8);           // the logits are
+  RULES(BDH_E_INVAL, 2, 8, 8, ints, reinterpret_cast<int64_t *>(ints + 12), f, nullptr, 0, nullptr, 0, buf + 64, buf + 64, 8);
   EXPECT(BDH_E_INVAL, bdh_logit_rules(nullptr, 1, 8, buf, 8, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 0, nullptr, 0, buf, 8));
   EXPECT(BDH_E_INVAL, bdh_count_tokens(nullptr, 1, 1, 8, toks, 1, nullptr, 0, ints));
   EXPECT(BDH_E_INVAL, bdh_count_tokens(&ctx, -1, 1, 8, toks, 1, nullptr, 0, ints));
@@ -165,6 +177,10 @@ int main() {
   EXPECT(BDH_E_INVAL, bdh_model_fork_shared(nullptr, 2, counts, 5, buf, 0, 8, ints, -1, buf, buf, buf + 2048));
   EXPECT(BDH_E_INVAL, bdh_model_fork_shared(&m, 2, counts, 5, buf, 0, 8, ints, -1, buf, buf, nullptr));
   EXPECT(BDH_E_INVAL, bdh_model_fork_shared(&m, 2, counts, 5, buf, 0, 8, ints, -1, buf, buf, buf + 16));
+  // layers: the first one's states would be written over the second one's keys
+  m.cfg.n_layer = 2;
+  EXPECT(BDH_E_INVAL, bdh_model_fork_shared(&m, 2, counts, 5, buf, 0, 8, ints, -1, buf + 1600, buf, buf + 2400));
+  EXPECT(BDH_E_INVAL, bdh_model_fork_shared(&m, 2, counts, 5, buf + 2048, 0, 8, ints, -1, buf, buf, buf + 2048 + 300));
   if (failures) return 1;
   std::puts("ok");
   return 0;

@@ -170,3 +170,15 @@ def test_a_captured_step_counts_every_replay(rules):
         graph.replay()
         want = rules.apply_rules(logits, r, eager, newest)
         assert torch.equal(out, want) and torch.equal(seen, eager)
+
+
+def test_full_counts_stay_and_endless_penalties_leave_what_was_not_said(rules):
+    tokens = torch.tensor([[0, 1, 1, 1, 2, 3] * 300], device=DEV)
+    seen = torch.tensor([[2**31 - 2, -2, 2**30 - 5, -2**31 + 2**30 - 1]], dtype=torch.int32, device=DEV)  # 1, -2: marked, one to go
+    rules.count_tokens(tokens, seen)
+    assert seen.tolist() == [[2**31 - 1, -1, 2**30 - 5 + 300, -2**31 + 2**30 - 1 + 300]]
+    inf = float("inf")
+    z = torch.tensor([[1.0, -2.0, 0.5]], device=DEV)
+    seen = torch.tensor([[0, -2**31, 3]], dtype=torch.int32, device=DEV)
+    out = rules.apply_rules(z, rules.LogitRules(frequency=inf, presence=inf), seen)
+    assert out.tolist() == [[1.0, -2.0, -inf]]

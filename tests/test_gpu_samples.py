@@ -139,3 +139,21 @@ def test_one_sample_one_token(bda):
         got = generate_samples(model, [3], n, GenerationSettings(max_new_tokens=1, top_k=1))
         assert [len(s) for s in got] == [1] * n
     assert generate_samples(model, [3], 2, GenerationSettings(max_new_tokens=0)) == [[], []]
+
+
+def test_states_of_other_models_and_captures_are_refused(bda, monkeypatch):
+    model, half, other = _model(bda, "rope"), _model(bda, "rope", 1), _model(bda, "rope", d=64)
+    state = model.init_state()
+    model.forward_with_state(torch.tensor([[1, 2, 3]]), state)
+    shared = model.share_state(state, [2], 8)
+    tokens = torch.tensor([[4], [5]])
+    for m in (half, other):
+        with pytest.raises(ValueError, match="another model"):
+            m.forward_shared(tokens, shared)
+        with pytest.raises(ValueError, match="another model"):
+            m.fork_shared(shared)
+    with monkeypatch.context() as p:
+        p.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with pytest.raises(ValueError, match="capture"):
+            model.forward_shared(tokens, shared)
+    assert shared.length == 0 and model.forward_shared(tokens, shared).shape == (2, 1, 69)

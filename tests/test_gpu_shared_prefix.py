@@ -330,3 +330,76 @@ def test_another_stream_and_two_contexts(gpu):
         ob = c.call(shared, tb, ctx=b)
     torch.cuda.synchronize()
     assert torch.equal(oa, want) and torch.equal(ob, want)
+
+
+# more than 32 tokens of a prompt's sequences: dense products, their sums dealt to several workgroups; even and uneven prompts
+DENSE = [
+    ((2, 2), 2, 8192, 64, 32, (3, 9, 0), 20, "rope", F32),
+    ((3, 0, 1), 2, 8190, 72, 24, (5, 1), 14, "rope", F32),
+    ((1, 4), 1, 5001, 36, 48, (7, 0, 11), 35, "pope", BF16),
+    ((7,), 3, 2048, 128, 12, (2, 4, 0), 5, "alibi", BF16),
+    ((17,), 1, 4000, 64, 4, (1, 2), 2, "rope", F32),
+    ((5, 28), 2, 512, 256, 8, (0, 5, 3), 3, "alibi", F32),
+    ((2,), 1, 300, 64, 132, (0,), 129, "rope", F32),
+]
+
+
+@pytest.mark.parametrize("counts,h,N,d,S,lens,T,rotary,dtype", DENSE)
+def test_many_tokens_equal_the_definition(gpu, counts, h, N, d, S, lens, T, rotary, dtype):
+    _check_read(gpu, Case(hash((sum(counts), h, N, d, T)) % 2**31, counts, h, N, d, S, lens, T, rotary, dtype, 0.1))
+
+
+@pytest.mark.parametrize("T", [2, 7])
+def test_a_sequence_without_room_among_dense_products(gpu, T):
+    _, _, shared = gpu
+    c = Case(6, (20, 3), 2, 700, 64, 16, (3, 8, 5, 2), T, "rope", F32)
+    t = c.device()
+    good = c.call(shared, t)
+    t = c.device()
+    t["lens"][1], t["lens"][21] = 17, -1
+    keys, values = t["keys"].clone(), t["values"].clone()
+    out = c.call(shared, t)
+    bad = [1, 21]
+    rest = [b for b in range(23) if b not in bad]
+    assert torch.isnan(out[bad]).all() and torch.equal(out[rest], good[rest])
+    assert torch.equal(t["keys"][bad], keys[bad]) and torch.equal(t["values"][bad], values[bad])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_fork_does_not_look_behind_the_last_token(gpu, dtype):
+    _, _, shared = gpu
+    c = Case(41, (4,), 2, 70, 68, 72, (5, 0, 66, 31), 1, "rope", dtype)
+    t = c.device()
+    for b in range(4):
+        t["keys"][b, :, :, c.lens[b]:] = float("nan")
+        t["values"][b, c.lens[b]:] = float("inf")
+    _check_fork(gpu, c, shared.shared_prefix_fork(t["rho"], t["keys"], t["values"], t["lens"], counts=c.counts))
+
+
+def test_two_graphs_of_one_workspace(gpu):
+    """Steps of two shapes captured on one context, replayed in turns with eager calls of a third between them: each leaves
+    what its eager call leaves."""
+    ffi, _, shared = gpu
+    cases = [Case(51, (9,), 2, 256, 64, 16, (2, 5), 1, "rope", F32), Case(52, (3, 2), 2, 130, 128, 24, (4, 9), 12, "alibi", BF16)]
+    between = Case(53, (2, 4), 1, 64, 32, 8, (1,), 3, "pope", F32)
+    ctx = ffi.Context(0)
+    want, held, graphs = [], [], []
+    for c in cases + [between]:
+        t = c.device()
+        want.append((c.call(shared, t, ctx=ctx), t["keys"]))
+    torch.cuda.synchronize()
+    for c in cases:
+        t = c.device()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = c.call(shared, t, ctx=ctx)
+        held.append((t, out))
+        graphs.append(graph)
+    for i in range(6):
+        k = i % 2
+        held[k][1].fill_(-1.0)
+        graphs[k].replay()
+        assert torch.equal(held[k][1], want[k][0]) and torch.equal(held[k][0]["keys"], want[k][1]), i
+        t = between.device()
+        assert torch.equal(between.call(shared, t, ctx=ctx), want[2][0])

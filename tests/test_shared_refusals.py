@@ -86,6 +86,28 @@ def test_rules_check_their_arguments():
             count_tokens(tokens, seen, **kw)
 
 
+def test_tensors_in_host_memory_are_refused():
+    """The last check before a context is asked for: no address of host memory reaches a kernel."""
+    z, seen, toks = torch.zeros(2, 40), torch.zeros(2, 40, dtype=torch.int32), torch.zeros(2, 3, dtype=torch.int64)
+    args = _read_args()
+    fork = {k: v for k, v in args.items() if k in ("rho", "keys", "values", "lens", "counts")}
+    for call in (lambda: shared_prefix_attention(**args), lambda: shared_prefix_fork(**fork), lambda: count_tokens(toks, seen),
+                 lambda: apply_rules(z, LogitRules(1.5), seen), lambda: copy_slots([(z, z, 0)], [0, 1]),
+                 lambda: copy_slots([(z, z, 0)], torch.zeros(2, dtype=torch.int32))):
+        with pytest.raises(ValueError, match="HIP device"):
+            call()
+
+
+def test_penalties_that_mean_nothing_and_missing_frequencies():
+    for r in (0.0, -1.5, float("nan")):
+        with pytest.raises(ValueError):
+            LogitRules(repetition=r)
+    args = _read_args()
+    args["freqs"] = None
+    with pytest.raises(ValueError):
+        shared_prefix_attention(**args)
+
+
 def test_packed_masks_and_empty_counts():
     mask = torch.rand(3, 70, generator=torch.Generator().manual_seed(1)) < 0.5
     words = pack_allowed(mask)
