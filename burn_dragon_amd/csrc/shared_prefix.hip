@@ -18,6 +18,7 @@ constexpr float kLnEps = 1e-5f;  // src/model/bdh.rs:17
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2u __attribute__((ext_vector_type(2), aligned(4)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x4u __attribute__((ext_vector_type(4), aligned(4)));
@@ -460,18 +461,19 @@ struct Product {
   }
 
   // The scores of these rows for sequences own0 .. own1 - 1: half a wavefront (of up to four sequences a whole one) lists what of
-  // a sequence is active (pairs of rows; with PoPE all of them), then sixteen lanes take four neighbouring keys each of every other (every
-  // fourth) listed one.
+  // a sequence is active (pairs of rows; with PoPE all of them), then sixteen lanes (four, where all keys are 16 at most) take four
+  // neighbouring keys each of every other (every fourth, ...) listed one.
   __device__ __forceinline__ void own_keys(const PassArgs &g, int rb, int own0, int own1) {
     constexpr int PER = 2, U = 4;
-    const int tid = threadIdx.x, half = tid >> 5, hl = tid & 31, li = tid & 15;
+    const int tid = threadIdx.x, half = tid >> 5, hl = tid & 31;
     const bool whole = own1 - own0 <= 4;
-    const int k2 = whole ? (tid & 63) >> 4 : hl >> 4, stride = whole ? 4 : 2;
+    const int lanes = whole ? 64 : 32, lane = tid & (lanes - 1);
     const int last = g.Nq - 1 - rb * g.rows;
     unsigned short *own = sh.own[half];
 #pragma unroll 1
     for (int i = own0 + (whole ? half >> 1 : half); i < own1; i += whole ? 4 : 8) {
-      const int len = sh.len[i], row = sh.row[i];
+      const int len = sh.len[i], row = sh.row[i], bits = len <= 16 ? 2 : 4;
+      const int li = tid & ((1 << bits) - 1), k2 = lane >> bits, stride = lanes >> bits;
       int n = 0;
 #pragma unroll 1
       for (int w = 0; w < g.rows / PER / 32; ++w) {
@@ -484,7 +486,7 @@ struct Product {
       float *parts = g.score_parts + ((long)rb * g.B * g.h + row) * g.span;
 #pragma unroll 1
       for (int s0 = 0; s0 < len; s0 += 64) {
-        const int s = s0 + li * 4;
+        const int s = s0 + li * 4;  // four lanes: len is 16 at most
         f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
         if (s < len)
 #pragma unroll 1
@@ -506,11 +508,10 @@ struct Product {
                 sum += (e + stride * u < n && place >= 0 ? q : 0.0f) * k[u][j];
               }
           }
+#pragma unroll 1
+        for (int m = 1 << bits; m < lanes; m <<= 1)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          sum[c] += __shfl_xor(sum[c], 16, 64);
-          if (whole) sum[c] += __shfl_xor(sum[c], 32, 64);
-        }
+          for (int c = 0; c < 4; ++c) sum[c] += __shfl_xor(sum[c], m, 64);
         if (k2 == 0 && s < len) *reinterpret_cast<f32x4 *>(parts + s) = sum;
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -829,11 +830,12 @@ __global__ __launch_bounds__(256) void k_suffix_append(AppendArgs g) {
     const int m = n0 + (r & 63);
     if (t < g.T && m < g.N) g.keys[((long)bh * g.Nq + (r < 64 ? m : g.N + m)) * g.S + len + t] = s_t[r][tid & 31];
   }
-  if (blockIdx.x == 0 && bh % g.h == 0) {
-    const long last = min(t0 + 32, g.T);
-    for (long e = (long)t0 * g.d + tid; e < last * g.d; e += 256)
-      g.values[((long)b * g.S + len) * g.d + e] = g.v[(long)b * g.T * g.d + e];
-  }
+  // the values, shared out to all workgroups of the sequence
+  const unsigned groups = gridDim.x * gridDim.y * g.h, mine = ((bh - b * g.h) * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
+  const float *from = g.v + (long)b * g.T * g.d;
+  float *to = g.values + ((long)b * g.S + len) * g.d;
+  for (long e = ((long)mine * 256 + tid) * 4; e < (long)g.T * g.d; e += (long)groups * 1024)
+    *reinterpret_cast<f32x4u *>(to + e) = *reinterpret_cast<const f32x4u *>(from + e);
 }
 
 // ---- many tokens: dense products ----------------------------------------------------------------------------------------

@@ -248,12 +248,14 @@ def context_on(device, ctx: Optional[Context] = None) -> Context:
     in host memory, a context of another device, a device that is not the current one."""
     import torch
 
+    index = device.index
     if device.type != "cuda":
         raise ValueError(f"tensors on {device}: this operator runs on a HIP device")
-    if torch.cuda.current_device() != device.index:
+    if torch._C._cuda_getDevice() != index:  # current_device() without its look at whether CUDA is initialised: it is
         raise ValueError(f"tensors on {device}, the current device is cuda:{torch.cuda.current_device()}")
-    ctx = ctx or default_context(device.index)
-    if ctx.device_id != device.index:
+    if ctx is None:
+        ctx = _default_ctx.get(index) or default_context(index)
+    if ctx.device_id != index:
         raise ValueError(f"tensors on {device}, the context is on cuda:{ctx.device_id}")
     return ctx
 

@@ -67,16 +67,18 @@ def pack_allowed(allowed: torch.Tensor) -> torch.Tensor:
     return torch.where(words >= 2**31, words - 2**32, words).to(torch.int32)
 
 
-def _seen(seen: torch.Tensor, B: int, V: int, dev) -> None:
-    if seen.shape != (B, V) or seen.dtype is not torch.int32 or not seen.is_contiguous() or seen.device != dev:
-        raise ValueError(f"seen: expected a contiguous int32 tensor [{B}, {V}] on {dev}, got {seen.dtype} {tuple(seen.shape)}")
+def _seen(seen: torch.Tensor, B: int, V: int, on: int) -> None:
+    if seen.shape != (B, V) or seen.dtype is not torch.int32 or seen.get_device() != on or not seen.is_contiguous():
+        raise ValueError(f"seen: expected a contiguous int32 tensor [{B}, {V}] on device {on}, got {seen.dtype} {tuple(seen.shape)} "
+                         f"on {seen.device}")
 
 
-def _row_stride(name: str, t: torch.Tensor, B: int, width: int, dtype, dev) -> int:
+def _row_stride(name: str, t: torch.Tensor, B: int, width: int, dtype, on: int) -> int:
     """Elements between the rows of a bias or mask: 0 for one row that all sequences share."""
-    if t.dtype is not dtype or t.device != dev or t.dim() not in (1, 2) or t.shape[-1] != width or \
+    if t.dtype is not dtype or t.get_device() != on or t.dim() not in (1, 2) or t.shape[-1] != width or \
             (t.dim() == 2 and t.shape[0] != B) or (width > 1 and t.stride(-1) != 1):
-        raise ValueError(f"{name}: expected {dtype} [{width}] or [{B}, {width}] on {dev}, got {t.dtype} {tuple(t.shape)}")
+        raise ValueError(f"{name}: expected {dtype} [{width}] or [{B}, {width}] on device {on}, got {t.dtype} {tuple(t.shape)} "
+                         f"on {t.device}")
     return t.stride(0) if t.dim() == 2 and B > 1 else 0
 
 
@@ -85,11 +87,11 @@ def count_tokens(tokens: torch.Tensor, seen: torch.Tensor, lens: Optional[torch.
     """tokens [B,T] int64 (of row b the first lens[b]; lens int32 [B] on the device) into seen [B,V]: marked as tokens of
     the prompt, or counted as produced.  Ids outside the vocabulary are skipped."""
     B, T = tokens.shape
-    dev, V = tokens.device, seen.shape[-1]
-    _seen(seen, B, V, dev)
+    dev, on, V = tokens.device, tokens.get_device(), seen.shape[-1]
+    _seen(seen, B, V, on)
     if tokens.dtype is not torch.int64 or (T > 1 and tokens.stride(1) != 1):
         raise ValueError("tokens: expected int64 rows")
-    if lens is not None and (lens.shape != (B,) or lens.dtype is not torch.int32 or lens.device != dev or not lens.is_contiguous()):
+    if lens is not None and (lens.shape != (B,) or lens.dtype is not torch.int32 or lens.get_device() != on or not lens.is_contiguous()):
         raise ValueError(f"lens: expected int32 [{B}] on {dev}")
     ctx = ffi.context_on(dev, ctx)
     ctx.check(ctx.lib.bdh_count_tokens(ctx.handle, B, T, V, ffi.ptr(tokens), tokens.stride(0) if B > 1 else max(T, 1),
@@ -104,31 +106,32 @@ def apply_rules(logits: torch.Tensor, rules: LogitRules, seen: Optional[torch.Te
     if logits.dim() != 2 or logits.dtype != torch.float32 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError("logits: expected f32 rows [B,V]")
     B, V = logits.shape
-    dev = logits.device
+    dev, on = logits.device, logits.get_device()
     if seen is not None:
-        _seen(seen, B, V, dev)
+        _seen(seen, B, V, on)
     elif rules.penalises or newest is not None:
         raise ValueError("penalties need the counts of the tokens seen")
     if newest is not None:
         if newest.dim() != 1:
             newest = newest.reshape(-1)
-        if newest.shape != (B,) or newest.dtype is not torch.int64 or newest.device != dev:
+        if newest.shape != (B,) or newest.dtype is not torch.int64 or newest.get_device() != on:
             raise ValueError(f"newest: expected int64 [{B}] on {dev}")
-        newest = newest.contiguous()
+        if not newest.is_contiguous():
+            newest = newest.contiguous()
     penalties = []
     for name, p in (("repetition", rules.repetition), ("presence", rules.presence), ("frequency", rules.frequency)):
         if p is not None:
             if not torch.is_tensor(p):
                 p = torch.full((B,), float(p), device=dev, dtype=torch.float32)
-            elif p.shape != (B,) or p.dtype is not torch.float32 or p.device != dev or not p.is_contiguous():
+            elif p.shape != (B,) or p.dtype is not torch.float32 or p.get_device() != on or not p.is_contiguous():
                 raise ValueError(f"{name}: expected f32 [{B}] on {dev}")
-        penalties.append(p)
+        penalties.append(p)  # held until the call: one made here has no other owner
     bias, allowed = rules.bias, rules.allowed
-    bias_stride = 0 if bias is None else _row_stride("bias", bias, B, V, torch.float32, dev)
-    allowed_stride = 0 if allowed is None else _row_stride("allowed", allowed, B, (V + 31) // 32, torch.int32, dev)
+    bias_stride = 0 if bias is None else _row_stride("bias", bias, B, V, torch.float32, on)
+    allowed_stride = 0 if allowed is None else _row_stride("allowed", allowed, B, (V + 31) // 32, torch.int32, on)
     if out is None:
-        out = torch.empty_like(logits) if logits.is_contiguous() else torch.empty((B, V), device=dev, dtype=torch.float32)
-    elif out.shape != (B, V) or out.dtype is not torch.float32 or out.device != dev or (V > 1 and out.stride(1) != 1):
+        out = logits.new_empty(B, V)
+    elif out.shape != (B, V) or out.dtype is not torch.float32 or out.get_device() != on or (V > 1 and out.stride(1) != 1):
         raise ValueError(f"out: expected f32 rows [{B}, {V}] on {dev}")
     ctx = ffi.context_on(dev, ctx)
     ctx.check(ctx.lib.bdh_logit_rules(

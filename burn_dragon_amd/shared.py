@@ -15,17 +15,20 @@ from .positional import RotaryEmbedding
 _DTYPES = {torch.float32: ffi.F32, torch.bfloat16: ffi.BF16}
 
 
-def _check(name: str, t: torch.Tensor, shape, dtype, device) -> None:
-    if t.shape != shape or t.dtype is not dtype or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{name}: expected a contiguous {dtype} tensor {tuple(shape)} on {device}, got {t.dtype} "
+def _check(name: str, t: torch.Tensor, shape, dtype, device: int) -> None:
+    """device: the index, -1 for host memory (an int is compared in half the time of a torch.device; a call of one token
+    takes the GPU as long as the host, so these checks count)"""
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous {dtype} tensor {tuple(shape)} on device {device}, got {t.dtype} "
                          f"{tuple(t.shape)} on {t.device}")
 
 
 def _prompts(counts: Optional[Sequence[int]], G: int, B: int):
+    """The numbers of the prompts' sequences for the C ABI: None is all of one prompt."""
+    if G == 1 and (counts is None or (len(counts) == 1 and counts[0] == B)):
+        return None
     if counts is None:
-        if G != 1:
-            raise ValueError(f"{G} prompts need the numbers of their sequences")
-        counts = [B]
+        raise ValueError(f"{G} prompts need the numbers of their sequences")
     if len(counts) != G or sum(counts) != B or min(counts, default=0) < 0:
         raise ValueError(f"counts {list(counts)} do not deal {B} sequences to {G} prompts")
     return (ctypes.c_int32 * G)(*counts)
@@ -36,7 +39,7 @@ def _slopes(alibi_slopes, h: int):
         return None
     if len(alibi_slopes) != h:
         raise ValueError(f"{len(alibi_slopes)} slopes for {h} heads")
-    return (ctypes.c_float * h)(*[float(s) for s in alibi_slopes])
+    return (ctypes.c_float * h)(*map(float, alibi_slopes))
 
 
 def shared_prefix_attention(query: torch.Tensor, value: torch.Tensor, rho: torch.Tensor, keys: torch.Tensor,
@@ -51,33 +54,36 @@ def shared_prefix_attention(query: torch.Tensor, value: torch.Tensor, rho: torch
     tokens' keys and values at places lens[b] and on; lens itself is advanced by the caller.  position / positions: as in
     recurrent_attention, the prompt's tokens counted.  longest: an upper bound of lens (default S - T)."""
     B, h, T, N = query.shape
-    dev = query.device
+    dev, on = query.device, query.get_device()
     rot = RotaryEmbedding.parse(rotary_embedding)
     Nq = 2 * N if rot == RotaryEmbedding.POPE else N
     d, S, G = value.shape[-1], keys.shape[-1], rho.shape[0]
     if rho.dtype not in _DTYPES:
         raise ValueError(f"rho is f32 or bf16, not {rho.dtype}")
-    _check("query", query, (B, h, T, N), torch.float32, dev)
-    value = value.reshape(B, T, d)
-    _check("value", value, (B, T, d), torch.float32, dev)
-    _check("rho", rho, (G, h, Nq, d), rho.dtype, dev)
-    _check("keys", keys, (B, h, Nq, S), torch.float32, dev)
-    _check("values", values, (B, S, d), torch.float32, dev)
-    _check("lens", lens, (B,), torch.int32, dev)
+    f32, int32 = torch.float32, torch.int32
+    _check("query", query, (B, h, T, N), f32, on)
+    if value.dim() != 3:
+        value = value.reshape(B, T, d)
+    _check("value", value, (B, T, d), f32, on)
+    _check("rho", rho, (G, h, Nq, d), rho.dtype, on)
+    _check("keys", keys, (B, h, Nq, S), f32, on)
+    _check("values", values, (B, S, d), f32, on)
+    _check("lens", lens, (B,), int32, on)
     if positions is not None:
-        _check("positions", positions, (B,), torch.int32, dev)
+        _check("positions", positions, (B,), int32, on)
     if rot != RotaryEmbedding.ALIBI:
         if freqs is None:
             raise ValueError(f"{rot.name} needs its frequencies")
-        freqs = freqs.reshape(-1)
-        _check("freqs", freqs, (N,), torch.float32, dev)
+        if freqs.dim() != 1:
+            freqs = freqs.reshape(-1)
+        _check("freqs", freqs, (N,), f32, on)
     n_of = _prompts(counts, G, B)
     slopes = _slopes(alibi_slopes, h)
     ctx = ffi.context_on(dev, ctx)
-    out = torch.empty((B, h, T, d), device=dev, dtype=torch.float32)
+    out = query.new_empty(B, h, T, d)
     ctx.check(ctx.lib.bdh_shared_prefix_attention(
-        ctx.handle, G, n_of, B, h, T, N, d, int(rot), query.data_ptr(), value.data_ptr(),
-        None if rot == RotaryEmbedding.ALIBI else freqs.data_ptr(), int(position), ffi.ptr(positions), slopes,
+        ctx.handle, G, n_of, B, h, T, N, d, rot, query.data_ptr(), value.data_ptr(),
+        None if rot == RotaryEmbedding.ALIBI else freqs.data_ptr(), int(position), None if positions is None else positions.data_ptr(), slopes,
         rho.data_ptr(), _DTYPES[rho.dtype], S, lens.data_ptr(), -1 if longest is None else int(longest), keys.data_ptr(),
         values.data_ptr(), out.data_ptr()))
     return out
@@ -90,17 +96,18 @@ def shared_prefix_fork(rho: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     """The states [B,h,Nq,d] (of rho's type) that the sequences of shared_prefix_attention would have had to themselves:
     the prompt's state with the sequence's own tokens added, as after the same recurrent_attention calls."""
     B, h, Nq, S = keys.shape
-    dev = keys.device
+    dev, on = keys.device, keys.get_device()
     G, d = rho.shape[0], rho.shape[-1]
     if rho.dtype not in _DTYPES:
         raise ValueError(f"rho is f32 or bf16, not {rho.dtype}")
-    _check("rho", rho, (G, h, Nq, d), rho.dtype, dev)
-    _check("keys", keys, (B, h, Nq, S), torch.float32, dev)
-    _check("values", values, (B, S, d), torch.float32, dev)
-    _check("lens", lens, (B,), torch.int32, dev)
+    _check("rho", rho, (G, h, Nq, d), rho.dtype, on)
+    _check("keys", keys, (B, h, Nq, S), torch.float32, on)
+    _check("values", values, (B, S, d), torch.float32, on)
+    _check("lens", lens, (B,), torch.int32, on)
     if out is None:
-        out = torch.empty((B, h, Nq, d), device=dev, dtype=rho.dtype)
-    _check("out", out, (B, h, Nq, d), rho.dtype, dev)
+        out = rho.new_empty(B, h, Nq, d)
+    else:
+        _check("out", out, (B, h, Nq, d), rho.dtype, on)
     n_of = _prompts(counts, G, B)
     slopes = _slopes(alibi_slopes, h)
     ctx = ffi.context_on(dev, ctx)

@@ -21,23 +21,24 @@ def copy_slots(buffers: Iterable[Tuple[torch.Tensor, torch.Tensor, int]], origin
     buffers = list(buffers)
     if not buffers:
         return
-    dev = buffers[0][0].device
-    n, m = buffers[0][0].shape[buffers[0][2]], buffers[0][1].shape[buffers[0][2]]
+    dst, src, dim = buffers[0]
+    dev, on, n, m = dst.device, dst.get_device(), dst.shape[dim], src.shape[dim]
     table = (ffi.SlotBufferC * len(buffers))()
     for k, (dst, src, dim) in enumerate(buffers):
-        if dst.dtype != src.dtype or dst.dim() != src.dim() or not (dst.is_contiguous() and src.is_contiguous()):
-            raise ValueError(f"buffer {k}: destination and source are contiguous tensors of one type and rank")
-        if dst.device != dev or src.device != dev:
-            raise ValueError(f"buffer {k}: every buffer is on {dev}")
-        if dst.shape[dim] != n or src.shape[dim] != m:
-            raise ValueError(f"buffer {k}: {dst.shape[dim]} and {src.shape[dim]} slots, the first has {n} and {m}")
-        dim %= dst.dim()
-        if dst.shape[:dim] != src.shape[:dim] or dst.shape[dim + 1:] != src.shape[dim + 1:]:
-            raise ValueError(f"buffer {k}: slots of {tuple(dst.shape)} and {tuple(src.shape)} differ")
+        shape, rank = dst.shape, dst.dim()
+        if not dst.is_contiguous() or dst.get_device() != on:
+            raise ValueError(f"buffer {k}: every buffer is contiguous and on {dev}")
+        if src is not dst and not (dst.dtype is src.dtype and rank == src.dim() and src.is_contiguous() and src.get_device() == on):
+            raise ValueError(f"buffer {k}: destination and source are contiguous tensors of one type and rank on {dev}")
+        if shape[dim] != n or src.shape[dim] != m:
+            raise ValueError(f"buffer {k}: {shape[dim]} and {src.shape[dim]} slots, the first has {n} and {m}")
+        dim %= rank
+        outer, inner = shape[:dim], shape[dim + 1:]
+        if src is not dst and (outer != src.shape[:dim] or inner != src.shape[dim + 1:]):
+            raise ValueError(f"buffer {k}: slots of {tuple(shape)} and {tuple(src.shape)} differ")
         row = table[k]
         row.dst, row.src = dst.data_ptr(), src.data_ptr()
-        row.outer = math.prod(dst.shape[:dim])
-        row.slot_bytes = math.prod(dst.shape[dim + 1:]) * dst.element_size()
+        row.outer, row.slot_bytes = math.prod(outer), math.prod(inner) * dst.element_size()
     if not torch.is_tensor(origin):
         origin = [int(o) for o in origin]
         bad = [o for o in origin if not KEEP <= o < m]
@@ -45,7 +46,7 @@ def copy_slots(buffers: Iterable[Tuple[torch.Tensor, torch.Tensor, int]], origin
             raise ValueError(f"origin: {len(origin)} entries for {n} slots, naming slots {bad} of {m}")
         ctx = ffi.context_on(dev, ctx)
         origin = torch.tensor(origin, dtype=torch.int32, device=dev)
-    if origin.shape != (n,) or origin.dtype != torch.int32 or origin.device != dev or not origin.is_contiguous():
+    if origin.shape != (n,) or origin.dtype != torch.int32 or origin.get_device() != on or not origin.is_contiguous():
         raise ValueError(f"origin: expected int32 [{n}] on {dev}, got {origin.dtype} {tuple(origin.shape)} on {origin.device}")
     ctx = ffi.context_on(dev, ctx)
     ctx.check(ctx.lib.bdh_copy_slots(ctx.handle, table, len(buffers), n, m, origin.data_ptr()))
