@@ -600,8 +600,19 @@ __global__ __launch_bounds__(256, RT == 4 && MODE == kHalf ? 1 : 2) void k_share
     } else {
       p.load_queries(g.q + n0, g.Nq, nb, g.rows, min(g.rows, g.Nq - n0));
     }
-    p.multiply(static_cast<const R *>(g.rho) + (((long)grp * g.h + hh) * g.Nq + n0) * g.d, g.d, g.d, col0, g.cg, nb);
-    if constexpr (STEP) p.own_keys(g, rb, own0, own1);
+    if constexpr (STEP) {
+      // All workgroups start together; every other one of a CU reads the keys first, so that they are not all at the same thing (three
+      // prompts of 14, 14 and 12 sequences, 8 heads of 16384, d = 512, bf16: 132 -> 127 us; one of 32, 4 of 8192, f32: 30.5 -> 30.1)
+      const unsigned id = blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z);
+      const bool keys_first = (id >> 8) & 1;
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
+        if ((half == 0) == keys_first) p.own_keys(g, rb, own0, own1);
+        else p.multiply(static_cast<const R *>(g.rho) + (((long)grp * g.h + hh) * g.Nq + n0) * g.d, g.d, g.d, col0, g.cg, nb);
+      }
+    } else {
+      p.multiply(static_cast<const R *>(g.rho) + (((long)grp * g.h + hh) * g.Nq + n0) * g.d, g.d, g.d, col0, g.cg, nb);
+    }
     __syncthreads();  // the next block's list takes the place of what is still read here
   }
   p.finish(g.partial + (long)part * g.B * g.h * g.T * g.d, g.d, col0, g.cg, nb);
@@ -1247,10 +1258,11 @@ int bdh_launch_shared_steps(bdh_ctx *ctx, const SharedStepParams &p) {
     else g.cg /= 2;
   }
   // more than fit the chip at once: blocks of rows one after the other in a workgroup, so that all run together; or twice as many
-  // where the prompts' workgroups take their own times
+  // where the prompts' workgroups take their own times.  A CU has room for three (bf16 or 64 queries: two; both: one, where 40
+  // sequences of 8 heads of 16384, d = 512, take 112 us, dealt to twice as many 123)
   bool even = true;
   for (int i = 1; i < p.G && T == 1; ++i) even &= pr.begin[i + 1] - pr.begin[i] == pr.begin[1];
-  const long slots = (long)ctx->n_cu * (half || rt == 4 ? 2 : 3) * (even ? 1 : 2);
+  const long slots = (long)ctx->n_cu * (half && rt == 4 ? 1 : half || rt == 4 ? 2 : 3) * (even ? 1 : 2);
   auto deal = [&](long others, int &parts, int &per, int &longer) {
     parts = (int)std::max<long>(1, std::min<long>(g.row_blocks, slots / std::max<long>(1, others)));
     per = g.row_blocks / parts;
