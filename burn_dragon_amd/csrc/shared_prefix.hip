@@ -96,6 +96,7 @@ __device__ __forceinline__ void rotate_pair(float pos, float f0, float f1, float
 // ---- queries times rows of a matrix -----------------------------------------------------------------------------------
 
 constexpr int kRowsMost = 256;    // rows of the matrix a workgroup takes at a time
+constexpr int kQueriesMost = 32;  // and queries
 
 struct PassArgs {
   const float *x, *freqs;  // one token a sequence (STEP): its activations, turned here
@@ -110,6 +111,7 @@ struct PassArgs {
   int rows, cg, row_blocks;      // rows and column groups a workgroup takes at a time, blocks of rows in all
   int parts, per, longer;        // of a sum: the blocks of rows are dealt to so many workgroups, per or (the first `longer`) per + 1
   int col_blocks;                // the columns' workgroups
+  int tile;                      // queries of a workgroup, 16 * RT at most
   int span, score_parts_n;       // columns and parts of the scores
   int score_per, score_longer, score_cols;  // several tokens: as per, longer, col_blocks
 };
@@ -124,10 +126,10 @@ struct TileShared {
   __attribute__((aligned(16))) unsigned short list[kRowsMost + 32];
   int used[kRowsMost];
   int cnt[4];
-  int row[64];                              // query i is row[i] of [B,h,T]
-  float pos[64];
-  int len[64];                              // of the tile's sequences; -1: no room
-  unsigned long long fires[64][kRowsMost / 64];  // one token: what of a sequence is active, a bit for a pair of rows (or a row)
+  int row[kQueriesMost];                    // query i is row[i] of [B,h,T]
+  float pos[kQueriesMost];
+  int len[kQueriesMost];                    // of the tile's sequences; -1: no room
+  unsigned long long fires[kQueriesMost][kRowsMost / 64];  // one token: what of a sequence is active, a bit for a pair of rows (or a row)
   unsigned short item[4][1024 + 64];        // a wavefront's active (sequence, pair)s, and room for what is none
   unsigned short own[8][kRowsMost];         // half a wavefront's sequence: its active pairs (or rows), listed
 };
@@ -249,7 +251,7 @@ struct Product {
     const unsigned n = n0 + min(r, have - 1), src = n < (unsigned)g.N ? n : n - g.N;
     const float *x = g.x + (long)row0 * g.N;
     const float f = g.freqs[src];
-    if (tid < 64) {
+    if (tid < kQueriesMost) {
       sh.len[tid] = my_len;
       sh.pos[tid] = my_pos;
       const int pairs = (have + 1) / 2;
@@ -324,7 +326,7 @@ struct Product {
     if (rope) u0 = u1 = u0 || u1;
     if (u0) sh.used[2 * p] = 1;
     if (u1) sh.used[2 * p + 1] = 1;
-    if (tid < 64) {
+    if (tid < kQueriesMost) {
       sh.len[tid] = my_len;
       sh.pos[tid] = my_pos;
     }
@@ -568,12 +570,12 @@ struct Product {
 // The queries of a tile times a part of their prompt's state; one token: also their scores with what their sequences said.
 // Grid: (tile, column block), part, (prompt, head), the prompts with most sequences first.  Tiles of the same rows start together: they read them from memory once.
 template <typename R, int RT, bool STEP, int MODE>
-__global__ __launch_bounds__(256, RT == 4 && MODE == kHalf ? 1 : 2) void k_shared_pass(PassArgs g, Prompts pr) {
+__global__ __launch_bounds__(256, 2) void k_shared_pass(PassArgs g, Prompts pr) {
   extern __shared__ __attribute__((aligned(16))) char s_dyn[];
   __shared__ TileShared sh;
   const unsigned tid = threadIdx.x, z = blockIdx.z / (unsigned)g.h, grp = pr.by_size[z], hh = blockIdx.z - z * g.h;
   const unsigned tile = blockIdx.x / (unsigned)g.col_blocks, cb = blockIdx.x - tile * g.col_blocks, part = blockIdx.y;
-  const int first = pr.begin[grp], m0 = tile * 16 * RT, nb = min(16 * RT, (pr.begin[grp + 1] - first) * g.T - m0);
+  const int first = pr.begin[grp], m0 = tile * g.tile, nb = min(g.tile, (pr.begin[grp + 1] - first) * g.T - m0);
   if (nb <= 0) return;
   int my_len = -1;  // of sequence tid; one token's go to LDS with its activations on their way
   float my_pos = 0.0f;
@@ -629,7 +631,7 @@ __global__ __launch_bounds__(256, 2) void k_suffix_scores(PassArgs g) {
   const int len = g.lens[b], t0 = tile * 16 * RT, nb = min(16 * RT, g.T - t0), col0 = cb * g.cg * 64;
   // keys behind the tile's last token are of no use to it
   if (!valid_len(len, g.T, g.longest, g.S) || col0 >= len + t0 + nb - 1) return;
-  if (tid < 64) sh.row[tid] = (int)tid < nb ? bh * g.T + t0 + tid : 0;
+  if (tid < kQueriesMost) sh.row[tid] = (int)tid < nb ? bh * g.T + t0 + tid : 0;
   Product<float, RT, kF32> p(sh, s_dyn, g.rows);
   int rb = part * g.score_per + min((int)part, g.score_longer);
   const int end = rb + g.score_per + ((int)part < g.score_longer ? 1 : 0);
@@ -1118,13 +1120,11 @@ int check_prompts(bdh_ctx *ctx, int G, const int32_t *counts_host, int B, Prompt
 
 namespace {
 
-// one token: tiles of 64 sequences where a prompt has more than 32
-template <typename R, int MODE, int MODE4>
+// FEW: how 16 queries at a time are made, MANY: how 32 are
+template <typename R, int FEW, int MANY>
 const void *pass_kernel(int T, int rt) {
-  if (T > 1) return rt == 1 ? reinterpret_cast<const void *>(k_shared_pass<R, 1, false, MODE>) : reinterpret_cast<const void *>(k_shared_pass<R, 2, false, MODE>);
-  return rt == 1   ? reinterpret_cast<const void *>(k_shared_pass<R, 1, true, MODE>)
-         : rt == 2 ? reinterpret_cast<const void *>(k_shared_pass<R, 2, true, MODE>)
-                   : reinterpret_cast<const void *>(k_shared_pass<R, 4, true, MODE4>);
+  if (rt == 1) return T > 1 ? reinterpret_cast<const void *>(k_shared_pass<R, 1, false, FEW>) : reinterpret_cast<const void *>(k_shared_pass<R, 1, true, FEW>);
+  return T > 1 ? reinterpret_cast<const void *>(k_shared_pass<R, 2, false, MANY>) : reinterpret_cast<const void *>(k_shared_pass<R, 2, true, MANY>);
 }
 
 int launch_pass(bdh_ctx *ctx, const void *kernel, const char *name, dim3 grid, size_t lds, void **args) {
@@ -1238,15 +1238,21 @@ int bdh_launch_shared_steps(bdh_ctx *ctx, const SharedStepParams &p) {
   g.B = B; g.h = h; g.T = T; g.N = N; g.Nq = Nq; g.d = d; g.S = S; g.rotary = p.rotary; g.longest = longest;
   long most = 1;  // queries of a prompt
   for (int i = 0; i < p.G; ++i) most = std::max(most, (long)(pr.begin[i + 1] - pr.begin[i]) * T);
-  // Several tokens: more than 32 queries of a prompt go through dense products (us, here | there: 6 sequences of one prompt, 4
-  // heads of 8192, d = 256, 2 tokens 57 | 95, 4 tokens 73 | 94, 8 tokens 118 | 98, 63 tokens 198 | 202; 4 sequences, 4 heads of
-  // 256, 8 tokens 27 | 36, 24 tokens 36 | 35; 16 sequences, 8 heads of 4096, d = 512, 2 tokens 102 | 112, 4 tokens 171 | 117)
-  if (T > 1 && most > 32) return launch_dense(ctx, p, pr, rates, longest);
-  const int rt = most <= 16 ? 1 : most <= 32 ? 2 : 4;
+  // Several tokens go through dense products from 33 queries a prompt on (us, here | there, f32: 6 sequences of one prompt, 4 heads
+  // of 8192, d = 256, 3 tokens 68 | 64, 7 tokens 83 | 65, 32 tokens 128 | 80; prompts of 4, 9 and 6, 8 heads of 4096, d = 512, 2
+  // tokens 95 | 136, 5 tokens 187 | 217, 10 tokens 241 | 217; 4 sequences of 4 heads of 256, 4 tokens 25 | 35), with a bf16 state of
+  // more than 2^24 numbers from 161 on, as it is widened for them (8 heads of 16384, d = 512, one sequence, 48 tokens 149 | 205,
+  // 100 tokens 254 | 267, 200 tokens 643 | 490; 6 sequences of 4 heads of 8192, d = 256, 8 tokens 86 | 68)
+  const bool large = p.rho_dtype == BDH_BF16 && (long)p.G * h * Nq * d > (1L << 24);
+  if (T > 1 && (long)B * T > (large ? 160L : 32L) * p.G) return launch_dense(ctx, p, pr, rates, longest);
+  // 32 queries a workgroup at most; of more, tiles of equal size
+  const int rt = most <= 16 ? 1 : 2;
+  const bool planes = half || (rt == 2 && p.rho_dtype == BDH_F32);  // the queries stand in LDS as three planes of bf16
   const long tiles = (most + 16 * rt - 1) / (16 * rt);
+  g.tile = (int)((most + tiles - 1) / tiles);
   // rows and columns of a workgroup: as many as leave two workgroups for every CU
   const int group = half ? 128 : 64, groups = (d + group - 1) / group;
-  g.rows = rt == 4 ? 128 : kRowsMost;
+  g.rows = kRowsMost;
   g.cg = groups >= 4 ? 4 : groups >= 2 ? 2 : 1;
   auto count = [&] {
     g.row_blocks = (Nq + g.rows - 1) / g.rows;
@@ -1258,11 +1264,10 @@ int bdh_launch_shared_steps(bdh_ctx *ctx, const SharedStepParams &p) {
     else g.cg /= 2;
   }
   // more than fit the chip at once: blocks of rows one after the other in a workgroup, so that all run together; or twice as many
-  // where the prompts' workgroups take their own times.  A CU has room for three (bf16 or 64 queries: two; both: one, where 40
-  // sequences of 8 heads of 16384, d = 512, take 112 us, dealt to twice as many 123)
+  // where the prompts' workgroups take their own times.  A CU has room for three (two of those with planes).
   bool even = true;
   for (int i = 1; i < p.G && T == 1; ++i) even &= pr.begin[i + 1] - pr.begin[i] == pr.begin[1];
-  const long slots = (long)ctx->n_cu * (half && rt == 4 ? 1 : half || rt == 4 ? 2 : 3) * (even ? 1 : 2);
+  const long slots = (long)ctx->n_cu * (planes ? 2 : 3) * (even ? 1 : 2);
   auto deal = [&](long others, int &parts, int &per, int &longer) {
     parts = (int)std::max<long>(1, std::min<long>(g.row_blocks, slots / std::max<long>(1, others)));
     per = g.row_blocks / parts;
@@ -1302,7 +1307,7 @@ int bdh_launch_shared_steps(bdh_ctx *ctx, const SharedStepParams &p) {
                                               : pass_kernel<unsigned short, kF32, kF32>(T, rt);
   void *args[] = {&g, &pr};
   rc = launch_pass(ctx, kernel, "k_shared_pass", dim3((unsigned)(tiles * g.col_blocks), g.parts, p.G * h),
-                   room(half || (rt == 4 && p.rho_dtype == BDH_F32), group), args);
+                   room(planes, group), args);
   if (rc != BDH_OK) return rc;
   if (T > 1) {
     const void *scores = rt == 1 ? reinterpret_cast<const void *>(k_suffix_scores<1>) : reinterpret_cast<const void *>(k_suffix_scores<2>);

@@ -332,8 +332,14 @@ def test_another_stream_and_two_contexts(gpu):
     assert torch.equal(oa, want) and torch.equal(ob, want)
 
 
-# more than 32 tokens of a prompt's sequences: dense products, their sums dealt to several workgroups; even and uneven prompts
+# more than 32 tokens of a prompt's sequences: dense products, their sums dealt to several workgroups, even and uneven prompts;
+# a large bf16 state, and prompts most of which have few, take tiles of 32
 DENSE = [
+    ((2,), 16, 16384, 68, 24, (3, 0), 18, "rope", BF16),
+    ((20, 1, 1), 1, 512, 64, 8, (3, 0), 3, "rope", F32),
+    ((9, 30), 2, 1025, 72, 8, (3, 0, 4), 1, "pope", BF16),
+    ((9, 65), 2, 1024, 72, 24, (3, 20, 17), 1, "rope", F32),
+    ((33,), 4, 256, 256, 32, (16, 20, 15, 31), 1, "alibi", F32),
     ((2, 2), 2, 8192, 64, 32, (3, 9, 0), 20, "rope", F32),
     ((3, 0, 1), 2, 8190, 72, 24, (5, 1), 14, "rope", F32),
     ((1, 4), 1, 5001, 36, 48, (7, 0, 11), 35, "pope", BF16),
