@@ -4,6 +4,12 @@
 //   q_t = rot(x_t),  k = len_b + t,  out_t = a^k q_t rho[g(b)] + sum_{s < k} a^(k-s) (q_t . k_s) v_s,  k_k = q_t, v_k = v_t
 // with a = exp(-slope_h) for ALiBi, else 1: src/model/bdh.rs:288-302 with the sum over tokens cut where the prompt ends.
 // The keys of a neuron lie side by side, so the neurons that are silent now are not read.
+//
+// One token of every sequence takes two launches: k_shared_pass multiplies the queries with the prompt's rows and with the
+// sequences' own keys, in parts, and k_shared_join adds the parts and the values.  (One launch, whose last workgroup of a
+// prompt and head joins, would leave the joining of all its sequences to four workgroups in the smallest case and in the
+// one of 32 sequences alike.)  Several tokens: k_suffix_append turns them and stores them as keys and values, then the same
+// pass, k_suffix_scores and the join for few queries, and dense products for many (bdh_launch_shared_steps says from where).
 #include <algorithm>
 #include <type_traits>
 
@@ -568,7 +574,19 @@ struct Product {
 };
 
 // The queries of a tile times a part of their prompt's state; one token: also their scores with what their sequences said.
-// Grid: (tile, column block), part, (prompt, head), the prompts with most sequences first.  Tiles of the same rows start together: they read them from memory once.
+// Grid: (tile, column block), part, (prompt, head), the prompts with most sequences first.  Tiles of the same rows start
+// together: they read them from memory once.
+// The rows that some query of the tile uses are read once and nothing else is: 32 sequences that each use 5 % of the neurons
+// use 96 % of the pairs between them (one: 10 %).  Bound by memory where the state is large: 40 sequences of three prompts,
+// 8 heads of 16384, d = 512, bf16: 110 us for 341 MB of rows, keys and activations, 3.1 TB/s where a sum over a large tensor
+// reads 4.0; registers and LDS leave room for two workgroups a CU, and one lists and turns its queries while the other multiplies.
+// Below that the steps of one workgroup after the other: 32 sequences of one prompt, 4 heads of 8192, d = 256, f32: 20.5 us
+// for 54 MB, of which a workgroup spends 1.2 on its arguments, 2.7 on the activations, 2.8 on listing and turning what
+// fires, 4.2 on rows and products, 5.1 on keys, 1.3 on its sums; 4 sequences, 4 heads of 256: 10.5 us, all of it waiting.
+// f32 states of 17 to 32 queries are split on the way (kSplit): the f32 instructions take 256 cycles for 32 rows, six bf16 ones 96
+// (24 sequences of 8192: 47 -> 45.6 us, 32: 30.1 -> 29.7).  With
+// tiles of 64 queries a CU has fewer workgroups (us, 64 at a time | 32: 40 sequences of 4 heads of 8192, d = 256, f32 50 |
+// 34, bf16 44 | 45; of 8 heads of 16384, d = 512, f32 133 | 138, bf16 112 | 83; 100 of them 258 | 263, bf16 282 | 184).
 template <typename R, int RT, bool STEP, int MODE>
 __global__ __launch_bounds__(256, 2) void k_shared_pass(PassArgs g, Prompts pr) {
   extern __shared__ __attribute__((aligned(16))) char s_dyn[];
@@ -621,7 +639,7 @@ __global__ __launch_bounds__(256, 2) void k_shared_pass(PassArgs g, Prompts pr) 
 }
 
 // Several tokens: the queries of a tile of a sequence's tokens times a part of its own keys.  Grid: (tile, column block), part,
-// (sequence, head).
+// (sequence, head).  Six tokens of 4 sequences, 2 heads of 160 rows: 5.7 us, the steps of a workgroup one after the other.
 template <int RT>
 __global__ __launch_bounds__(256, 2) void k_suffix_scores(PassArgs g) {
   extern __shared__ __attribute__((aligned(16))) char s_dyn[];
@@ -657,7 +675,9 @@ struct JoinArgs {
 
 // out = a^k * (the parts of q rho) + sum_s a^(k-s) score_s v_s, in the order of the parts and of the tokens, for TT tokens of a
 // (sequence, head); a column's parts and values are dealt to as many threads as a workgroup of 1024 has for it.  One token: its
-// value goes to its place.
+// value goes to its place.  What it reads comes from the caches and in three waits of one another (parts, scores, values), so
+// a workgroup has as many loads on their way as it can: 4.4 us for 16 workgroups, 7.9 for 128 with up to 60 tokens each, 13.3
+// for 320 with up to 31 and rows of 512.
 template <int TT, bool LN>
 __global__ __launch_bounds__(1024) void k_shared_join(JoinArgs g, HeadRates rates) {
   __shared__ float s_sc[TT][512];
@@ -789,7 +809,9 @@ struct AppendArgs {
 };
 
 // Queries of all tokens [B,h,T,Nq], and their places among the keys: 32 tokens x 64 neurons through LDS.  A thread turns the
-// two neurons of a pair for four tokens; with PoPE a neuron gives two rows.
+// two neurons of a pair for four tokens; with PoPE a neuron gives two rows.  Bound by memory: 45 tokens of 6 sequences, 4 heads
+// of 8192: 105 MB in 28-30 us, of which a third are the keys' runs of 180 bytes that begin and end inside cache lines.  Tiles of 64
+// tokens, which write such a run at once, took 27.5-31.7 us there and 24 for 20 at 22 tokens.
 __global__ __launch_bounds__(256) void k_suffix_append(AppendArgs g) {
   __shared__ float s_t[128][33];
   const int n0 = blockIdx.x * 64, t0 = blockIdx.y * 32, bh = blockIdx.z, b = bh / g.h, tid = threadIdx.x;
@@ -863,7 +885,11 @@ struct MaskArgs {
   bool decays, even;  // even: one launch for all prompts
 };
 
-// Scores of a token with the keys before its own, decayed; and its readout of the prompt's state, decayed.  A workgroup a token.
+// Scores of a token with the keys before its own, decayed; and its readout of the prompt's state, decayed: the parts of both
+// products added in order.  A workgroup a token (270 tokens of 4 heads: 7.2 us).  The products are the framework's own dense f32
+// ones: of 144 us for 45 tokens of prompts of 4 and 2 sequences, 4 heads of 8192, d = 256, those with the prompts' states take 81
+// (5.4 GFLOP as dealt, 66 TFLOP/s: 180 and 90 queries leave tiles of 64 short, and 16 parts of the sum are written and read), those
+// with the keys 23, with the values 7.6; k_suffix_append 29.
 __global__ __launch_bounds__(256) void k_shared_scores(MaskArgs g, HeadRates rates, Prompts pr) {
   const long row = blockIdx.x;
   const int t = (int)(row % g.T), bh = (int)(row / g.T), b = bh / g.h, hh = bh - b * g.h, tid = threadIdx.x;

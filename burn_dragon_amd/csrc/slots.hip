@@ -36,7 +36,9 @@ __device__ __forceinline__ const SlotBuffer &buffer_of(const SlotArgs &g, long t
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
 // One chunk of every destination slot: a source is read once for a run of slots that take it.  What is written passes the
-// caches by (a state is larger than they are).
+// caches by (a state is larger than they are; forking one to 16 slots of 64 MiB took 252 us through them).  Bound by memory: 16 slots forked from one,
+// 1.14 GB read and written, 205 us, 5.6 TB/s; 24 slots compacted to 11, bf16, 1.1 GB in 200 us; a copy of a large tensor
+// reaches 5.2 TB/s.  A piece is 16 bytes where sizes and addresses allow it, a thread has four on their way.
 template <typename P>
 __device__ __forceinline__ void copy_chunk(const SlotArgs &g, const SlotBuffer &f, long o, size_t p0, size_t p1, int i0, int i1, const int *origin) {
   const P *src = reinterpret_cast<const P *>(f.src) + (size_t)o * g.m * f.pieces;
@@ -76,7 +78,9 @@ __global__ __launch_bounds__(256) void k_copy_slots(SlotArgs g) {
 }
 
 // In place: a chunk of every source that moves goes to LDS before any slot is written, so a slot may be read and
-// overwritten in one call, in any cycle.  A chunk is a power of two of pieces: 2^shift lanes take one slot's.
+// overwritten in one call, in any cycle.  A chunk is a power of two of pieces: 2^shift lanes take one slot's.  Bound by memory:
+// 16 slots of 6 layers of 1 MiB, 76 MB read and written in 15.4 us, 4.9 TB/s.  The stage is 64 KiB, so that two workgroups of a CU
+// read and write in turns.
 template <typename P>
 __device__ __forceinline__ void move_chunk(const SlotBuffer &f, int n, long o, size_t p0, size_t p1, char *stage, const short *read,
                                            int n_read, const short *write, const short *from, int n_write) {

@@ -243,20 +243,21 @@ class Context:
             pass
 
 
-def context_on(device, ctx: Optional[Context] = None) -> Context:
-    """The context for tensors on `device` (ctx, or the device's default one).  Refuses what no kernel may be given: tensors
-    in host memory, a context of another device, a device that is not the current one."""
+def context_on(device: int, ctx: Optional[Context] = None) -> Context:
+    """The context for tensors on device `device` (Tensor.get_device(); -1 is host memory): ctx, or the device's default
+    one.  Refuses what no kernel may be given: tensors in host memory, a device that is not the current one, a context of
+    another device."""
     import torch
 
-    index = device.index
-    if device.type != "cuda":
-        raise ValueError(f"tensors on {device}: this operator runs on a HIP device")
-    if torch._C._cuda_getDevice() != index:  # current_device() without its look at whether CUDA is initialised: it is
-        raise ValueError(f"tensors on {device}, the current device is cuda:{torch.cuda.current_device()}")
+    if device < 0:
+        raise ValueError("tensors in host memory: this operator runs on a HIP device")
+    current = torch._C._cuda_getDevice()  # current_device() without its look at whether CUDA is initialised: it is
+    if current != device:
+        raise ValueError(f"tensors on cuda:{device}, the current device is cuda:{current}")
     if ctx is None:
-        ctx = _default_ctx.get(index) or default_context(index)
-    if ctx.device_id != index:
-        raise ValueError(f"tensors on {device}, the context is on cuda:{ctx.device_id}")
+        return _default_ctx.get(device) or default_context(device)
+    if ctx.device_id != device:
+        raise ValueError(f"tensors on cuda:{device}, the context is on cuda:{ctx.device_id}")
     return ctx
 
 

@@ -82,18 +82,28 @@ def _row_stride(name: str, t: torch.Tensor, B: int, width: int, dtype, on: int) 
     return t.stride(0) if t.dim() == 2 and B > 1 else 0
 
 
+def _per_row(name: str, p: Penalty, B: int, like: torch.Tensor, on: int) -> Optional[torch.Tensor]:
+    if p is None:
+        return None
+    if not isinstance(p, torch.Tensor):
+        return torch.full((B,), float(p), device=like.device, dtype=torch.float32)
+    if p.shape != (B,) or p.dtype is not torch.float32 or p.get_device() != on or not p.is_contiguous():
+        raise ValueError(f"{name}: expected f32 [{B}] on {like.device}")
+    return p
+
+
 def count_tokens(tokens: torch.Tensor, seen: torch.Tensor, lens: Optional[torch.Tensor] = None, prompt: bool = False,
                  ctx: Optional[ffi.Context] = None) -> None:
     """tokens [B,T] int64 (of row b the first lens[b]; lens int32 [B] on the device) into seen [B,V]: marked as tokens of
     the prompt, or counted as produced.  Ids outside the vocabulary are skipped."""
     B, T = tokens.shape
-    dev, on, V = tokens.device, tokens.get_device(), seen.shape[-1]
+    on, V = tokens.get_device(), seen.shape[-1]
     _seen(seen, B, V, on)
     if tokens.dtype is not torch.int64 or (T > 1 and tokens.stride(1) != 1):
         raise ValueError("tokens: expected int64 rows")
     if lens is not None and (lens.shape != (B,) or lens.dtype is not torch.int32 or lens.get_device() != on or not lens.is_contiguous()):
-        raise ValueError(f"lens: expected int32 [{B}] on {dev}")
-    ctx = ffi.context_on(dev, ctx)
+        raise ValueError(f"lens: expected int32 [{B}] on {tokens.device}")
+    ctx = ffi.context_on(on, ctx)
     ctx.check(ctx.lib.bdh_count_tokens(ctx.handle, B, T, V, ffi.ptr(tokens), tokens.stride(0) if B > 1 else max(T, 1),
                                        ffi.ptr(lens), int(bool(prompt)), ffi.ptr(seen)))
 
@@ -103,40 +113,46 @@ def apply_rules(logits: torch.Tensor, rules: LogitRules, seen: Optional[torch.Te
                 ctx: Optional[ffi.Context] = None) -> torch.Tensor:
     """logits [B,V] f32 (rows may be strided) under the rules -> out [B,V] (a new tensor, or `out`, which may be logits).
     seen [B,V]: the counts (token_counts) that penalties read; newest [B] int64: the tokens drawn last, counted first."""
-    if logits.dim() != 2 or logits.dtype != torch.float32 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+    shape, f32 = logits.shape, torch.float32
+    if len(shape) != 2 or logits.dtype is not f32:
         raise ValueError("logits: expected f32 rows [B,V]")
-    B, V = logits.shape
-    dev, on = logits.device, logits.get_device()
+    B, V = shape
+    on, dense = logits.get_device(), logits.is_contiguous()
+    if not dense and V > 1 and logits.stride(1) != 1:
+        raise ValueError("logits: expected f32 rows [B,V]")
     if seen is not None:
         _seen(seen, B, V, on)
+        seen_ptr = seen.data_ptr()
     elif rules.penalises or newest is not None:
         raise ValueError("penalties need the counts of the tokens seen")
+    else:
+        seen_ptr = None
+    newest_ptr = None
     if newest is not None:
         if newest.dim() != 1:
             newest = newest.reshape(-1)
         if newest.shape != (B,) or newest.dtype is not torch.int64 or newest.get_device() != on:
-            raise ValueError(f"newest: expected int64 [{B}] on {dev}")
+            raise ValueError(f"newest: expected int64 [{B}] on {logits.device}")
         if not newest.is_contiguous():
             newest = newest.contiguous()
-    penalties = []
-    for name, p in (("repetition", rules.repetition), ("presence", rules.presence), ("frequency", rules.frequency)):
-        if p is not None:
-            if not torch.is_tensor(p):
-                p = torch.full((B,), float(p), device=dev, dtype=torch.float32)
-            elif p.shape != (B,) or p.dtype is not torch.float32 or p.get_device() != on or not p.is_contiguous():
-                raise ValueError(f"{name}: expected f32 [{B}] on {dev}")
-        penalties.append(p)  # held until the call: one made here has no other owner
+        newest_ptr = newest.data_ptr()
+    repetition = _per_row("repetition", rules.repetition, B, logits, on)  # held until the call: a tensor made here has no
+    presence = _per_row("presence", rules.presence, B, logits, on)        # other owner
+    frequency = _per_row("frequency", rules.frequency, B, logits, on)
     bias, allowed = rules.bias, rules.allowed
-    bias_stride = 0 if bias is None else _row_stride("bias", bias, B, V, torch.float32, on)
+    bias_stride = 0 if bias is None else _row_stride("bias", bias, B, V, f32, on)
     allowed_stride = 0 if allowed is None else _row_stride("allowed", allowed, B, (V + 31) // 32, torch.int32, on)
     if out is None:
-        out = logits.new_empty(B, V)
-    elif out.shape != (B, V) or out.dtype is not torch.float32 or out.get_device() != on or (V > 1 and out.stride(1) != 1):
-        raise ValueError(f"out: expected f32 rows [{B}, {V}] on {dev}")
-    ctx = ffi.context_on(dev, ctx)
+        out = torch.empty_like(logits) if dense else logits.new_empty(B, V)
+        out_stride = V
+    else:
+        if out.shape != shape or out.dtype is not f32 or out.get_device() != on or (V > 1 and out.stride(1) != 1):
+            raise ValueError(f"out: expected f32 rows [{B}, {V}] on {logits.device}")
+        out_stride = out.stride(0) if B > 1 else V
+    ctx = ffi.context_on(on, ctx)
     ctx.check(ctx.lib.bdh_logit_rules(
-        ctx.handle, B, V, logits.data_ptr(), logits.stride(0) if B > 1 else V, None if seen is None else seen.data_ptr(),
-        None if newest is None else newest.data_ptr(), *[None if p is None else p.data_ptr() for p in penalties],
-        None if bias is None else bias.data_ptr(), bias_stride, None if allowed is None else allowed.data_ptr(), allowed_stride,
-        out.data_ptr(), out.stride(0) if B > 1 else V))
+        ctx.handle, B, V, logits.data_ptr(), logits.stride(0) if B > 1 else V, seen_ptr, newest_ptr,
+        None if repetition is None else repetition.data_ptr(), None if presence is None else presence.data_ptr(),
+        None if frequency is None else frequency.data_ptr(), None if bias is None else bias.data_ptr(), bias_stride,
+        None if allowed is None else allowed.data_ptr(), allowed_stride, out.data_ptr(), out_stride))
     return out

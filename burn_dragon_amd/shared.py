@@ -54,7 +54,7 @@ def shared_prefix_attention(query: torch.Tensor, value: torch.Tensor, rho: torch
     tokens' keys and values at places lens[b] and on; lens itself is advanced by the caller.  position / positions: as in
     recurrent_attention, the prompt's tokens counted.  longest: an upper bound of lens (default S - T)."""
     B, h, T, N = query.shape
-    dev, on = query.device, query.get_device()
+    on = query.get_device()
     rot = RotaryEmbedding.parse(rotary_embedding)
     Nq = 2 * N if rot == RotaryEmbedding.POPE else N
     d, S, G = value.shape[-1], keys.shape[-1], rho.shape[0]
@@ -79,7 +79,7 @@ def shared_prefix_attention(query: torch.Tensor, value: torch.Tensor, rho: torch
         _check("freqs", freqs, (N,), f32, on)
     n_of = _prompts(counts, G, B)
     slopes = _slopes(alibi_slopes, h)
-    ctx = ffi.context_on(dev, ctx)
+    ctx = ffi.context_on(on, ctx)
     out = query.new_empty(B, h, T, d)
     ctx.check(ctx.lib.bdh_shared_prefix_attention(
         ctx.handle, G, n_of, B, h, T, N, d, rot, query.data_ptr(), value.data_ptr(),
@@ -96,7 +96,7 @@ def shared_prefix_fork(rho: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     """The states [B,h,Nq,d] (of rho's type) that the sequences of shared_prefix_attention would have had to themselves:
     the prompt's state with the sequence's own tokens added, as after the same recurrent_attention calls."""
     B, h, Nq, S = keys.shape
-    dev, on = keys.device, keys.get_device()
+    on = keys.get_device()
     G, d = rho.shape[0], rho.shape[-1]
     if rho.dtype not in _DTYPES:
         raise ValueError(f"rho is f32 or bf16, not {rho.dtype}")
@@ -110,7 +110,7 @@ def shared_prefix_fork(rho: torch.Tensor, keys: torch.Tensor, values: torch.Tens
         _check("out", out, (B, h, Nq, d), rho.dtype, on)
     n_of = _prompts(counts, G, B)
     slopes = _slopes(alibi_slopes, h)
-    ctx = ffi.context_on(dev, ctx)
+    ctx = ffi.context_on(on, ctx)
     ctx.check(ctx.lib.bdh_shared_prefix_fork(
         ctx.handle, G, n_of, B, h, Nq, d, int(RotaryEmbedding.parse(rotary_embedding)), slopes,
         rho.data_ptr(), _DTYPES[rho.dtype], S, lens.data_ptr(), -1 if longest is None else int(longest), keys.data_ptr(),

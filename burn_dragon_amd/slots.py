@@ -44,9 +44,9 @@ def copy_slots(buffers: Iterable[Tuple[torch.Tensor, torch.Tensor, int]], origin
         bad = [o for o in origin if not KEEP <= o < m]
         if bad or len(origin) != n:
             raise ValueError(f"origin: {len(origin)} entries for {n} slots, naming slots {bad} of {m}")
-        ctx = ffi.context_on(dev, ctx)
+        ctx = ffi.context_on(on, ctx)
         origin = torch.tensor(origin, dtype=torch.int32, device=dev)
     if origin.shape != (n,) or origin.dtype != torch.int32 or origin.get_device() != on or not origin.is_contiguous():
         raise ValueError(f"origin: expected int32 [{n}] on {dev}, got {origin.dtype} {tuple(origin.shape)} on {origin.device}")
-    ctx = ffi.context_on(dev, ctx)
+    ctx = ffi.context_on(on, ctx)
     ctx.check(ctx.lib.bdh_copy_slots(ctx.handle, table, len(buffers), n, m, origin.data_ptr()))
