@@ -2,7 +2,7 @@
 
 The package is a thin host-side mirror of the reference's interface for that path
 (`kernel`, `model`, `positional`, `inference`, `generation`, `tokenizer`, `record`) over the C ABI of libbdh_mi355x.so
-(include/bdh_mi355x.h).  All computation happens in hand-written HIP kernels; there is
+(include/bdh_mi355x.h), and beside it what many answers of one prompt need (`shared`, `slots`, `rules`).  All computation happens in hand-written HIP kernels; there is
 no CPU or framework fallback.
 """
 from . import ffi

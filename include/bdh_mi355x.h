@@ -564,7 +564,8 @@ int bdh_model_flush_layers(bdh_model *model, bdh_model_logs *logs, void *const *
  * (counts may be zero; counts_host may be NULL with one prompt).  What a sequence says itself is kept beside the state:
  *   keys   [B,h,Nq,capacity] f32   the rotated activation n of its token s at [b,h,n,s]
  *   values [B,capacity,d]    f32   the layer input of token s at [b,s,:]
- *   lens_dev int32 [B]             tokens held; keys and values at and after that place hold zeros
+ *   lens_dev int32 [B]             tokens held; keys and values at and after that place hold zeros (a caller that takes a
+ *                                  length back clears what lay behind it)
  * The reference has no such form: each sequence owns a state (src/model/state.rs:5-15).  The sums are those of
  * src/model/bdh.rs:288-302, cut where the prompt ends:
  *   q_t = rot(x_t),  k = lens[b] + t,
@@ -583,7 +584,9 @@ int bdh_model_flush_layers(bdh_model *model, bdh_model_logs *logs, void *const *
  *   once: states of their own, as after the same tokens through bdh_recurrent_attention (f32 reassociation).  A len
  *   outside 0 .. longest gives a state of NaN.  rho_out must not overlap rho.
  *
- * d a multiple of 4, at most 1024; capacity a multiple of 4; at most BDH_MAX_SHARED_PROMPTS prompts and B * h <= 65535 a call.
+ * d a multiple of 4, at most 1024; capacity a multiple of 4, at most 2^20; h at most 64; at most BDH_MAX_SHARED_PROMPTS prompts
+ * and B * h <= 65535 a call; Nq * capacity < 2^31, B * h * T < 2^21.  rho, keys, values, out and rho_out on 16 bytes.  A call in a
+ * HIP graph takes longest = -1 (a replay's lengths are the device's).
  * Inputs are assumed finite.  Nothing is copied to or from the host, no result depends on the order of atomics.
  */
 #define BDH_MAX_SHARED_PROMPTS 256
@@ -619,7 +622,8 @@ int bdh_model_fork_shared(bdh_model *model, int G, const int32_t *counts_host, i
  *                  -1       dst[:, i] = 0 (a fresh state, empty counts)
  *                  else     (-2, or no slot of src) dst[:, i] is left as it is
  * src may be dst (of every buffer of the call; src_slots = dst_slots <= 1024): all slots are then read as they were before
- * the call, so origin may hold any permutation or fork.  Otherwise no destination may overlap a source.
+ * the call, so origin may hold any permutation or fork.  Otherwise no destination may overlap a source; none may hold
+ * origin_dev.
  */
 #define BDH_MAX_SLOT_BUFFERS 8
 typedef struct bdh_slot_buffer {
@@ -637,11 +641,12 @@ int bdh_copy_slots(bdh_ctx *ctx, const bdh_slot_buffer *buffers_host, int n_buff
  * prompt, bits 0..30 count how often the sequence produced it.  newest[b] (int64, optional; an id outside [0,V) counts as
  * none) is counted first; then for every token
  *   z = logits[b,v];  if seen: z = z > 0 ? z / repetition[b] : z * repetition[b]
- *   z = z - (frequency[b] * times + (times > 0 ? presence[b] : 0)) + bias[b,v]
+ *   z = z - (times > 0 ? frequency[b] * times + presence[b] : 0) + bias[b,v]
  *   out[b,v] = z, or -inf where bit v % 32 of word v / 32 of allowed[b] is clear, whatever z is
  * repetition, presence, frequency: device float [B] or NULL (1, 0, 0); they need seen.  bias and allowed: NULL, or rows
  * bias_stride floats / allowed_stride words apart, 0 for one row that all sequences share.  logits: row b starts at
- * logits + b*row_stride; out may be logits (same stride).  A row of which nothing is allowed is all -inf:
+ * logits + b*row_stride; out may be logits (same stride), and else overlaps nothing that is read; nor does seen.  A count
+ * ends at 2^31 - 1.  A row of which nothing is allowed is all -inf:
  * bdh_sample_top_k draws from it uniformly, so a caller that may run out of allowed tokens ends such a sequence.
  * bdh_count_tokens: seen[b, tokens[b,t]] for t < lens_dev[b] (NULL: T) is marked as the prompt's (prompt = 1) or counted
  * once more (0); ids outside [0,V) are skipped; lens are taken into 0..T.
