@@ -583,9 +583,8 @@ struct Product {
 // Below that the steps of one workgroup after the other: 32 sequences of one prompt, 4 heads of 8192, d = 256, f32: 20.5 us
 // for 54 MB, of which a workgroup spends 1.2 on its arguments, 2.7 on the activations, 2.8 on listing and turning what
 // fires, 4.2 on rows and products, 5.1 on keys, 1.3 on its sums; 4 sequences, 4 heads of 256: 10.5 us, all of it waiting.
-// f32 states of 17 to 32 queries are split on the way (kSplit): the f32 instructions take 256 cycles for 32 rows, six bf16 ones 96
-// (24 sequences of 8192: 47 -> 45.6 us, 32: 30.1 -> 29.7).  With
-// tiles of 64 queries a CU has fewer workgroups (us, 64 at a time | 32: 40 sequences of 4 heads of 8192, d = 256, f32 50 |
+// f32 states of 17 to 32 queries are split on the way (kSplit): the f32 instructions take 256 cycles for 32 rows, six bf16 ones 96.
+// With tiles of 64 queries a CU has fewer workgroups (us, 64 at a time | 32: 40 sequences of 4 heads of 8192, d = 256, f32 50 |
 // 34, bf16 44 | 45; of 8 heads of 16384, d = 512, f32 133 | 138, bf16 112 | 83; 100 of them 258 | 263, bf16 282 | 184).
 template <typename R, int RT, bool STEP, int MODE>
 __global__ __launch_bounds__(256, 2) void k_shared_pass(PassArgs g, Prompts pr) {
@@ -1146,11 +1145,9 @@ int check_prompts(bdh_ctx *ctx, int G, const int32_t *counts_host, int B, Prompt
 
 namespace {
 
-// FEW: how 16 queries at a time are made, MANY: how 32 are
-template <typename R, int FEW, int MANY>
-const void *pass_kernel(int T, int rt) {
-  if (rt == 1) return T > 1 ? reinterpret_cast<const void *>(k_shared_pass<R, 1, false, FEW>) : reinterpret_cast<const void *>(k_shared_pass<R, 1, true, FEW>);
-  return T > 1 ? reinterpret_cast<const void *>(k_shared_pass<R, 2, false, MANY>) : reinterpret_cast<const void *>(k_shared_pass<R, 2, true, MANY>);
+template <typename R, int RT, int MODE>
+const void *pass_kernel(int T) {
+  return T > 1 ? reinterpret_cast<const void *>(k_shared_pass<R, RT, false, MODE>) : reinterpret_cast<const void *>(k_shared_pass<R, RT, true, MODE>);
 }
 
 int launch_pass(bdh_ctx *ctx, const void *kernel, const char *name, dim3 grid, size_t lds, void **args) {
@@ -1273,7 +1270,10 @@ int bdh_launch_shared_steps(bdh_ctx *ctx, const SharedStepParams &p) {
   if (T > 1 && (long)B * T > (large ? 160L : 32L) * p.G) return launch_dense(ctx, p, pr, rates, longest);
   // 32 queries a workgroup at most; of more, tiles of equal size
   const int rt = most <= 16 ? 1 : 2;
-  const bool planes = half || (rt == 2 && p.rho_dtype == BDH_F32);  // the queries stand in LDS as three planes of bf16
+  // An f32 state is split where its prompts have more than 16 queries on average: splitting costs the same for few (prompts of 20, 7
+  // and 13 sequences, 8 heads of 16384, d = 512: 191 us split, 179 not; of 40: 138 and 144; of 24, 4 heads of 8192, d = 256: 45.6, 47)
+  const bool split = rt == 2 && p.rho_dtype == BDH_F32 && (long)B * T > 16L * p.G;
+  const bool planes = half || split;  // the queries stand in LDS as three planes of bf16
   const long tiles = (most + 16 * rt - 1) / (16 * rt);
   g.tile = (int)((most + tiles - 1) / tiles);
   // rows and columns of a workgroup: as many as leave two workgroups for every CU
@@ -1328,9 +1328,11 @@ int bdh_launch_shared_steps(bdh_ctx *ctx, const SharedStepParams &p) {
   auto room = [&](bool split, int cols) {
     return std::max((size_t)16 * rt * (split ? 6 * (g.rows + 8) : 4 * (g.rows + 4)), g.cg == 4 ? 0 : 4 * sizeof(float) * 16 * rt * cols);
   };
-  const void *kernel = p.rho_dtype == BDH_F32 ? pass_kernel<float, kF32, kSplit>(T, rt)
-                       : half                 ? pass_kernel<unsigned short, kHalf, kHalf>(T, rt)
-                                              : pass_kernel<unsigned short, kF32, kF32>(T, rt);
+  using u16 = unsigned short;
+  const void *kernel = half                     ? (rt == 1 ? pass_kernel<u16, 1, kHalf>(T) : pass_kernel<u16, 2, kHalf>(T))
+                       : split                  ? pass_kernel<float, 2, kSplit>(T)
+                       : p.rho_dtype == BDH_F32 ? (rt == 1 ? pass_kernel<float, 1, kF32>(T) : pass_kernel<float, 2, kF32>(T))
+                                                : (rt == 1 ? pass_kernel<u16, 1, kF32>(T) : pass_kernel<u16, 2, kF32>(T));
   void *args[] = {&g, &pr};
   rc = launch_pass(ctx, kernel, "k_shared_pass", dim3((unsigned)(tiles * g.col_blocks), g.parts, p.G * h),
                    room(planes, group), args);

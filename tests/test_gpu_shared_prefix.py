@@ -409,3 +409,65 @@ def test_two_graphs_of_one_workspace(gpu):
         assert torch.equal(held[k][1], want[k][0]) and torch.equal(held[k][0]["keys"], want[k][1]), i
         t = between.device()
         assert torch.equal(between.call(shared, t, ctx=ctx), want[2][0])
+
+
+# rows of four numbers; 17 to 32 tokens of a prompt's sequences, alone and next to prompts of few
+FORMS = [
+    ((2,), 1, 6, 4, 8, (1, 3), 1, "rope", BF16),
+    ((20,), 2, 130, 4, 4, (1, 0), 1, "alibi", BF16),
+    ((5,), 1, 33, 4, 12, (2, 7), 5, "pope", BF16),
+    ((3,), 1, 10, 4, 8, (2, 0), 3, "rope", BF16),
+    ((4,), 2, 300, 64, 16, (3, 0), 7, "rope", F32),
+    ((10, 1, 1), 2, 513, 100, 12, (3, 0, 6), 2, "alibi", F32),
+    ((22, 2, 3), 1, 1030, 72, 8, (3, 0, 6), 1, "rope", F32),
+    ((10, 1), 2, 140, 136, 12, (3, 0, 6), 3, "pope", BF16),
+]
+
+
+@pytest.mark.parametrize("counts,h,N,d,S,lens,T,rotary,dtype", FORMS)
+def test_every_form_equals_the_definition(gpu, counts, h, N, d, S, lens, T, rotary, dtype):
+    _check_read(gpu, Case(hash((sum(counts), h, N, d, T)) % 2**31, counts, h, N, d, S, lens, T, rotary, dtype))
+
+
+@pytest.mark.parametrize("T", [1, 20])
+def test_caches_beyond_32_bits_of_places(gpu, T):
+    """Three sequences of 2 heads of 8192 neurons with room for 131072 tokens: 26 GB of keys.  The last sequence is nearly full;
+    its last head, and the fork of it, against the definition in 64 bits."""
+    _, _, shared = gpu
+    B, h, N, d, S = 3, 2, 8192, 64, 131072
+    n = S - T - 1
+    gen = torch.Generator(DEV).manual_seed(5)
+    rand = lambda *shape: torch.randn(shape, device=DEV, generator=gen)
+    keys = torch.zeros((B, h, N, S), device=DEV)
+    keys[2, 1, :, :n] = rand(N, n)
+    values = torch.zeros((B, S, d), device=DEV)
+    values[2, :n] = rand(n, d)
+    lens = torch.tensor([0, 3, n], dtype=torch.int32, device=DEV)
+    x = rand(B, h, T, N).relu() * (torch.rand((B, h, T, N), device=DEV, generator=gen) < 0.05)
+    v, rho = rand(B, T, d), rand(1, h, N, d)
+    state = shared.shared_prefix_fork(rho, keys, values, lens, rotary_embedding="alibi", alibi_slopes=[1e-5, 1e-5])
+    out = shared.shared_prefix_attention(x, v, rho, keys, values, lens, None, rotary_embedding="alibi", alibi_slopes=[1e-5, 1e-5])
+    rate = float(np.log(np.exp(-np.float32(1e-5)).astype(np.float64)))
+    q, K, V = x[2, 1].double(), keys[2, 1, :, :n + T], values[2, :n + T].double()
+    scores = torch.zeros((T, n + T), dtype=torch.float64, device=DEV)
+    size = torch.zeros_like(scores)
+    ref, mag = torch.zeros((N, d), dtype=torch.float64, device=DEV), torch.zeros((N, d), dtype=torch.float64, device=DEV)
+    back = torch.exp(rate * (n - torch.arange(n, device=DEV, dtype=torch.float64)))[:, None]
+    for a in range(0, N, 1024):
+        part = K[a:a + 1024].double()
+        scores += q[:, a:a + 1024] @ part
+        size += q[:, a:a + 1024].abs() @ part.abs()
+        ref[a:a + 1024] = part[:, :n] @ (V[:n] * back)
+        mag[a:a + 1024] = part[:, :n].abs() @ (V[:n] * back).abs()
+    k = n + torch.arange(T, device=DEV)[:, None]
+    decay = torch.exp(rate * (k - torch.arange(n + T, device=DEV)).double()) * (torch.arange(n + T, device=DEV) < k)
+    grown = torch.exp(rate * k.double())
+    want = grown * (q @ rho[0, 1].double()) + (scores * decay) @ V
+    terms = grown * (q.abs() @ rho[0, 1].double().abs()) + (size * decay) @ V.abs()
+    depth = 35 + N + 2 * (N // 64 + 5) + 48 + n + T
+    assert ((out[2, 1].double() - want).abs() <= U * depth * terms).all()
+    assert torch.equal(keys[2, 1, :, n:n + T], x[2, 1].t()) and torch.equal(values[2, n:n + T], v[2])
+    assert not keys[2, 1, :, n + T:].any() and not keys[1, 1, :, 3 + T:].any()
+    start = float(np.exp(rate * n)) * rho[0, 1].double()
+    assert ((state[2, 1].double() - ref - start).abs() <= U * (n + 12) * (mag + start.abs())).all()
+    assert torch.equal(state[0], rho[0])
