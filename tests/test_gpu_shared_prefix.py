@@ -471,3 +471,31 @@ def test_caches_beyond_32_bits_of_places(gpu, T):
     start = float(np.exp(rate * n)) * rho[0, 1].double()
     assert ((state[2, 1].double() - ref - start).abs() <= U * (n + 12) * (mag + start.abs())).all()
     assert torch.equal(state[0], rho[0])
+
+
+def test_captured_forks_and_dense_products(gpu):
+    """Many tokens, then the fork of what they left, in one graph: replays on other inputs equal eager calls, with eager work
+    between them."""
+    ffi, _, shared = gpu
+    ctx = ffi.Context(0)
+    c = Case(61, (4, 2), 2, 514, 64, 32, (3, 0, 9), 14, "rope", F32)
+
+    def run(t, x):
+        out = shared.shared_prefix_attention(x, t["v"], t["rho"], t["keys"], t["values"], t["lens"], t["freqs"],
+                                             positions=t["positions"], counts=c.counts, ctx=ctx)
+        return out, shared.shared_prefix_fork(t["rho"], t["keys"], t["values"], t["lens"] + 14, counts=c.counts, ctx=ctx)
+
+    xs = [c.device()["x"] * (1 + 0.25 * i) for i in range(4)]
+    want = [run(c.device(), x) for x in xs]
+    t, x = c.device(), xs[0].clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, state = run(t, x)
+    for i in (0, 1, 2, 3, 1, 0):
+        x.copy_(xs[i])
+        graph.replay()
+        assert torch.equal(out, want[i][0]) and torch.equal(state, want[i][1]), i
+        again = run(c.device(), xs[3])
+        torch.cuda.synchronize()
+        assert torch.equal(again[0], want[3][0])
