@@ -1017,9 +1017,11 @@ __device__ __forceinline__ void stage_values(const ForkArgs &g, const ForkTile &
 // time on top of the prompt's rows: it splits the rows' keys into bf16 terms as they lie in memory and multiplies six of the
 // nine products with the terms of the values on v_mfma_f32_16x16x32_bf16 (what is left out is below 2^-23 of a product).  The
 // values of 64 tokens stand in LDS; those of more pass through it 64 at a time, for every 192 (128) rows again.
-// Bound by memory: without the products the largest case (32 sequences, 64 tokens, 4 heads of 8192, d = 256: 1 GiB written,
-// 256 MiB of keys) takes 9 % less, without reading the prompt's rows (from L2: a workgroup's neighbours on the XCD make the
-// same rows of other sequences) 17 %; what is written and the keys alone go at 4.0 TB/s.  A workgroup takes whole rows of up
+// Bound by the way to memory and to L2: the largest case (32 sequences, 64 tokens, 4 heads of 8192, d = 256: 1 GiB written, 256 MiB of
+// keys, the prompt's rows 32 times from L2, which misses 11 % of them: a workgroup's neighbours on the XCD make the same rows
+// of other sequences) takes 350 us; its writes alone take 204, with the keys 291, with the prompt's rows 352 (in shorter
+// workgroups, where all of it took 394 and all but the products 365).  Rows and keys asked for one step ahead, with
+// no wait for the stores between: 356.  A workgroup takes whole rows of up
 // to 320 columns, and the column blocks of wider ones stay on one XCD: a cache line that two XCDs write a part of goes to
 // memory twice (rows of 1200 bytes: 523 -> 426 us).
 template <typename R, int CB>
@@ -1434,11 +1436,24 @@ int bdh_shared_prefix_fork(bdh_ctx *ctx, int G, const int32_t *counts_host, int 
   // columns of a workgroup: all, or equal shares of at most 320 (what its LDS has room for)
   const int shares = (d + 319) / 320, cols = ((d + shares - 1) / shares + 63) / 64 * 64;
   g.col_blocks = (d + cols - 1) / cols;
-  g.rows = fork_waves(cols) * 16;  // that its wavefronts make at a time
-  while ((long)B * h * g.col_blocks * ((Nq + 2 * g.rows - 1) / (2 * g.rows)) >= 4L * ctx->n_cu) g.rows *= 2;
+  // Rows of a workgroup: so many times those its wavefronts make at a time that the rounds of workgroups an XCD takes are fewest in
+  // sum, with the values' way into LDS counted as one time more, and the rows that its L2 holds for all of its sequences are at
+  // most 2.25 MiB of the 4 (us, as many workgroups as four a CU need | so: 32 sequences, 64 tokens, 4 heads of 8192, d = 256 392 | 352,
+  // 16 tokens, 4 heads of 6620, d = 292 388 | 400, d = 320 333 | 313; 16 sequences, 48 tokens, 8 heads of 4096, d = 512, bf16 285 | 246)
+  const int step = fork_waves(cols) * 16, times = (Nq + step - 1) / step;
+  const size_t row_bytes = (size_t)d * (rho_dtype == BDH_BF16 ? 2 : 4);
+  long best = -1;
+  for (int t = 1; t <= times && (t == 1 || t * step * row_bytes <= (size_t)9 << 18); ++t) {
+    const long groups = (long)h * ((times + t - 1) / t), on_xcd = (groups + 7) / 8 * B * g.col_blocks, cus = std::max(1, ctx->n_cu / 8);
+    const long cost = (on_xcd + cus - 1) / cus * (t + 1);
+    if (best < 0 || cost < best) {
+      best = cost;
+      g.rows = t * step;
+    }
+  }
   g.row_blocks = (Nq + g.rows - 1) / g.rows;
   g.groups = g.row_blocks * h;
-  g.whole_lines = (size_t)d * (rho_dtype == BDH_BF16 ? 2 : 4) % 128 == 0 && bdh_aligned(rho_out, 128);
+  g.whole_lines = row_bytes % 128 == 0 && bdh_aligned(rho_out, 128);
   if ((g.groups + 7L) / 8 * 8 * B * g.col_blocks > 0x7fffffffL) return bdh_fail(ctx, BDH_E_SHAPE, "too many tiles");
   const size_t lds = (size_t)6 * cols * (kForkTokens + 8);
   const bool wide = rho_dtype == BDH_F32;

@@ -203,6 +203,9 @@ FORK = [
     ((2,), 1, 31, 132, 20, (9, 19), "pope", F32),
     ((3,), 1, 260, 1024, 64, (63, 64, 1), "rope", F32),
     ((2,), 2, 9, 64, 1028, (1025, 3), "alibi", F32),
+    # several times the rows that a workgroup makes at a time
+    ((40, 24), 16, 1000, 8, 12, (7, 12, 0), "rope", F32),
+    ((70,), 8, 1010, 8, 72, (71, 64, 0, 33), "alibi", BF16),
 ]
 
 
