@@ -469,8 +469,9 @@ struct Product {
   }
 
   // The scores of these rows for sequences own0 .. own1 - 1: half a wavefront (of up to four sequences a whole one) lists what of
-  // a sequence is active (pairs of rows; with PoPE all of them), then sixteen lanes (four, where all keys are 16 at most) take four
-  // neighbouring keys each of every other (every fourth, ...) listed one.
+  // a sequence is active (pairs of rows; with PoPE all of them), then sixteen lanes (eight or four, where all keys are 32 or 16 at most) take four
+  // neighbouring keys each of every other (every fourth, ...) listed one (30 sequences of up to 21 keys, 4 heads of 256, PoPE: 26.6 us
+  // by sixteen, 22 by eight).
   __device__ __forceinline__ void own_keys(const PassArgs &g, int rb, int own0, int own1) {
     constexpr int PER = 2, U = 4;
     const int tid = threadIdx.x, half = tid >> 5, hl = tid & 31;
@@ -480,7 +481,7 @@ struct Product {
     unsigned short *own = sh.own[half];
 #pragma unroll 1
     for (int i = own0 + (whole ? half >> 1 : half); i < own1; i += whole ? 4 : 8) {
-      const int len = sh.len[i], row = sh.row[i], bits = len <= 16 ? 2 : 4;
+      const int len = sh.len[i], row = sh.row[i], bits = len <= 16 ? 2 : len <= 32 ? 3 : 4;
       const int li = tid & ((1 << bits) - 1), k2 = lane >> bits, stride = lanes >> bits;
       int n = 0;
 #pragma unroll 1
@@ -494,7 +495,7 @@ struct Product {
       float *parts = g.score_parts + ((long)rb * g.B * g.h + row) * g.span;
 #pragma unroll 1
       for (int s0 = 0; s0 < len; s0 += 64) {
-        const int s = s0 + li * 4;  // four lanes: len is 16 at most
+        const int s = s0 + li * 4;  // fewer than sixteen lanes: they are enough for all keys
         f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
         if (s < len)
 #pragma unroll 1
