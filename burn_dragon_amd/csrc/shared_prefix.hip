@@ -579,11 +579,11 @@ struct Product {
 // together: they read them from memory once.
 // The rows that some query of the tile uses are read once and nothing else is: 32 sequences that each use 5 % of the neurons
 // use 96 % of the pairs between them (one: 10 %).  Bound by memory where the state is large: 40 sequences of three prompts,
-// 8 heads of 16384, d = 512, bf16: 110 us for 341 MB of rows, keys and activations, 3.1 TB/s where a sum over a large tensor
+// 8 heads of 16384, d = 512, bf16: 108 us for 341 MB of rows, keys and activations, 3.2 TB/s where a sum over a large tensor
 // reads 4.0; registers and LDS leave room for two workgroups a CU, and one lists and turns its queries while the other multiplies.
 // Below that the steps of one workgroup after the other: 32 sequences of one prompt, 4 heads of 8192, d = 256, f32: 20.5 us
 // for 54 MB, of which a workgroup spends 1.2 on its arguments, 2.7 on the activations, 2.8 on listing and turning what
-// fires, 4.2 on rows and products, 5.1 on keys, 1.3 on its sums; 4 sequences, 4 heads of 256: 10.5 us, all of it waiting.
+// fires, 4.2 on rows and products, 5.1 on keys, 1.3 on its sums; 4 sequences, 4 heads of 256: 9.6 us, all of it waiting.
 // f32 states of 17 to 32 queries are split on the way (kSplit): the f32 instructions take 256 cycles for 32 rows, six bf16 ones 96.
 // With tiles of 64 queries a CU has fewer workgroups (us, 64 at a time | 32: 40 sequences of 4 heads of 8192, d = 256, f32 50 |
 // 34, bf16 44 | 45; of 8 heads of 16384, d = 512, f32 133 | 138, bf16 112 | 83; 100 of them 258 | 263, bf16 282 | 184).
