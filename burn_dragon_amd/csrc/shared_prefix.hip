@@ -1269,8 +1269,14 @@ int bdh_launch_shared_steps(bdh_ctx *ctx, const SharedStepParams &p) {
   // tokens 95 | 136, 5 tokens 187 | 217, 10 tokens 241 | 217; 4 sequences of 4 heads of 256, 4 tokens 25 | 35), with a bf16 state of
   // more than 2^24 numbers from 161 on, as it is widened for them (8 heads of 16384, d = 512, one sequence, 48 tokens 149 | 205,
   // 100 tokens 254 | 267, 200 tokens 643 | 490; 6 sequences of 4 heads of 8192, d = 256, 8 tokens 86 | 68)
+  // The products with the prompts' states are to be worth the more launches, of which prompts of other sizes take one each
+  // (2^25 multiplications, 2^27; prompts of 1, 4 and 6, one head of 320, d = 124, 40 tokens 29 | 45; of 4 and 18, 4 heads of 524, d =
+  // 340, 8 tokens 43 | 43, 38 tokens 128 | 68; 22 sequences of one, 4 heads of 256, d = 256, 5 tokens 26 | 29, 6 of 512, 45 tokens 46 | 38)
   const bool large = p.rho_dtype == BDH_BF16 && (long)p.G * h * Nq * d > (1L << 24);
-  if (T > 1 && (long)B * T > (large ? 160L : 32L) * p.G) return launch_dense(ctx, p, pr, rates, longest);
+  bool even = true;
+  for (int i = 1; i < p.G; ++i) even &= pr.begin[i + 1] - pr.begin[i] == pr.begin[1];
+  if (T > 1 && (long)B * T > (large ? 160L : 32L) * p.G && (long)B * T * h * Nq * d > (even ? 1L << 25 : 1L << 27))
+    return launch_dense(ctx, p, pr, rates, longest);
   // 32 queries a workgroup at most; of more, tiles of equal size
   const int rt = most <= 16 ? 1 : 2;
   // An f32 state is split where its prompts have more than 16 queries on average: splitting costs the same for few (prompts of 20, 7
@@ -1294,9 +1300,7 @@ int bdh_launch_shared_steps(bdh_ctx *ctx, const SharedStepParams &p) {
   }
   // more than fit the chip at once: blocks of rows one after the other in a workgroup, so that all run together; or twice as many
   // where the prompts' workgroups take their own times.  A CU has room for three (two of those with planes).
-  bool even = true;
-  for (int i = 1; i < p.G && T == 1; ++i) even &= pr.begin[i + 1] - pr.begin[i] == pr.begin[1];
-  const long slots = (long)ctx->n_cu * (planes ? 2 : 3) * (even ? 1 : 2);
+  const long slots = (long)ctx->n_cu * (planes ? 2 : 3) * (even || T > 1 ? 1 : 2);
   auto deal = [&](long others, int &parts, int &per, int &longer) {
     parts = (int)std::max<long>(1, std::min<long>(g.row_blocks, slots / std::max<long>(1, others)));
     per = g.row_blocks / parts;

@@ -350,6 +350,9 @@ DENSE = [
     ((17,), 1, 4000, 64, 4, (1, 2), 2, "rope", F32),
     ((5, 28), 2, 512, 256, 8, (0, 5, 3), 3, "alibi", F32),
     ((2,), 1, 300, 64, 132, (0,), 129, "rope", F32),
+    ((2, 5), 2, 8192, 64, 32, (3, 8, 0), 24, "rope", F32),
+    ((1, 0, 6), 2, 4101, 68, 48, (3, 18, 0), 30, "pope", BF16),
+    ((3, 3), 4, 2047, 128, 16, (6, 0), 10, "alibi", BF16),
 ]
 
 
@@ -358,10 +361,10 @@ def test_many_tokens_equal_the_definition(gpu, counts, h, N, d, S, lens, T, rota
     _check_read(gpu, Case(hash((sum(counts), h, N, d, T)) % 2**31, counts, h, N, d, S, lens, T, rotary, dtype, 0.1))
 
 
-@pytest.mark.parametrize("T", [2, 7])
-def test_a_sequence_without_room_among_dense_products(gpu, T):
+@pytest.mark.parametrize("counts,N,T", [((20, 3), 700, 2), ((20, 3), 700, 7), ((11, 11), 4096, 7), ((20, 3), 8192, 7)])
+def test_a_sequence_without_room_among_many_tokens(gpu, counts, N, T):
     _, _, shared = gpu
-    c = Case(6, (20, 3), 2, 700, 64, 16, (3, 8, 5, 2), T, "rope", F32)
+    c = Case(6, counts, 2, N, 64, 16, (3, 8, 5, 2), T, "rope", F32)
     t = c.device()
     good = c.call(shared, t)
     t = c.device()
@@ -369,7 +372,7 @@ def test_a_sequence_without_room_among_dense_products(gpu, T):
     keys, values = t["keys"].clone(), t["values"].clone()
     out = c.call(shared, t)
     bad = [1, 21]
-    rest = [b for b in range(23) if b not in bad]
+    rest = [b for b in range(c.B) if b not in bad]
     assert torch.isnan(out[bad]).all() and torch.equal(out[rest], good[rest])
     assert torch.equal(t["keys"][bad], keys[bad]) and torch.equal(t["values"][bad], values[bad])
 
@@ -476,12 +479,13 @@ def test_caches_beyond_32_bits_of_places(gpu, T):
     assert torch.equal(state[0], rho[0])
 
 
-def test_captured_forks_and_dense_products(gpu):
+@pytest.mark.parametrize("counts,h,N", [((4, 2), 2, 514), ((3, 3), 4, 4096), ((4, 2), 4, 8192)])
+def test_captured_forks_and_reads_of_many_tokens(gpu, counts, h, N):
     """Many tokens, then the fork of what they left, in one graph: replays on other inputs equal eager calls, with eager work
     between them."""
     ffi, _, shared = gpu
     ctx = ffi.Context(0)
-    c = Case(61, (4, 2), 2, 514, 64, 32, (3, 0, 9), 14, "rope", F32)
+    c = Case(61, counts, h, N, 64, 32, (3, 0, 9), 14, "rope", F32)
 
     def run(t, x):
         out = shared.shared_prefix_attention(x, t["v"], t["rho"], t["keys"], t["values"], t["lens"], t["freqs"],
