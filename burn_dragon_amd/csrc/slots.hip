@@ -9,6 +9,7 @@ constexpr int kMaxBuffers = BDH_MAX_SLOT_BUFFERS;
 constexpr int kInPlaceSlots = 1024;
 constexpr int kRun = 256;
 constexpr int kStageBytes = 64 * 1024;  // of LDS: two workgroups a CU
+constexpr int kMoveThreads = 512;
 
 struct SlotBuffer {
   char *dst;
@@ -79,8 +80,9 @@ __global__ __launch_bounds__(256) void k_copy_slots(SlotArgs g) {
 
 // In place: a chunk of every source that moves goes to LDS before any slot is written, so a slot may be read and
 // overwritten in one call, in any cycle.  A chunk is a power of two of pieces: 2^shift lanes take one slot's.  Bound by memory:
-// 16 slots of 6 layers of 1 MiB, 76 MB read and written in 15.4 us, 4.9 TB/s.  The stage is 64 KiB, so that two workgroups of a CU
-// read and write in turns.
+// 16 slots of 6 layers of 1 MiB, 76 MB read and written in 11.2 us where they are in the caches, in 24 where they are not.  The stage is 64 KiB, so that
+// two workgroups of a CU read and write in turns; 512 threads each have enough on their way (256 and 1024: 12.5 and 11.4 us; 17 slots of
+// 4 layers of 7.3 MiB 80, 67 and 69).
 template <typename P>
 __device__ __forceinline__ void move_chunk(const SlotBuffer &f, int n, long o, size_t p0, size_t p1, char *stage, const short *read,
                                            int n_read, const short *write, const short *from, int n_write) {
@@ -88,13 +90,13 @@ __device__ __forceinline__ void move_chunk(const SlotBuffer &f, int n, long o, s
   P *st = reinterpret_cast<P *>(stage);
   const unsigned shift = f.shift, w = (unsigned)(p1 - p0), mask = (1u << shift) - 1;
 #pragma unroll 4
-  for (unsigned e = threadIdx.x; e < (unsigned)n_read << shift; e += 256) {
+  for (unsigned e = threadIdx.x; e < (unsigned)n_read << shift; e += kMoveThreads) {
     const unsigned p = e & mask;
     st[e] = base[(size_t)read[e >> shift] * f.pieces + (p < w ? p : 0)];
   }
   __syncthreads();
 #pragma unroll 4
-  for (unsigned e = threadIdx.x; e < (unsigned)n_write << shift; e += 256) {
+  for (unsigned e = threadIdx.x; e < (unsigned)n_write << shift; e += kMoveThreads) {
     const unsigned k = e >> shift, p = e & mask;
     const int s = from[k];
     const P v = s < 0 ? P{} : st[(s << shift) + p];
@@ -103,19 +105,19 @@ __device__ __forceinline__ void move_chunk(const SlotBuffer &f, int n, long o, s
   __syncthreads();
 }
 
-__global__ __launch_bounds__(256) void k_move_slots(SlotArgs g) {
+__global__ __launch_bounds__(kMoveThreads) void k_move_slots(SlotArgs g) {
   __shared__ __attribute__((aligned(16))) char s_stage[kStageBytes];
   __shared__ int s_origin[kInPlaceSlots];
   __shared__ short s_place[kInPlaceSlots];  // of a source among those that are read
   __shared__ short s_read[kInPlaceSlots], s_write[kInPlaceSlots], s_from[kInPlaceSlots];
   __shared__ int s_n[2];
   const int lane = threadIdx.x & 63;
-  for (int i = threadIdx.x; i < g.n; i += 256) {
+  for (int i = threadIdx.x; i < g.n; i += kMoveThreads) {
     s_origin[i] = g.origin[i];
     s_place[i] = 0;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < g.n; i += 256) {
+  for (int i = threadIdx.x; i < g.n; i += kMoveThreads) {
     const int from = s_origin[i];
     if (from >= 0 && from < g.n && from != i) s_place[from] = 1;
   }
@@ -233,7 +235,7 @@ extern "C" int bdh_copy_slots(bdh_ctx *ctx, const bdh_slot_buffer *buffers_host,
   while (g.run > 1 && (long)grid * ((dst_slots + g.run - 1) / g.run) < 2L * ctx->n_cu) g.run = (g.run + 1) / 2;
   if ((dst_slots + g.run - 1) / g.run > 65535) return bdh_fail(ctx, BDH_E_SHAPE, "%d slots: too many", dst_slots);
   if (in_place) {
-    hipLaunchKernelGGL(k_move_slots, dim3(grid), dim3(256), 0, ctx->stream, g);
+    hipLaunchKernelGGL(k_move_slots, dim3(grid), dim3(kMoveThreads), 0, ctx->stream, g);
     BDH_LAUNCH_CHECK(ctx, "k_move_slots");
   } else {
     hipLaunchKernelGGL(k_copy_slots, dim3(grid, (dst_slots + g.run - 1) / g.run), dim3(256), 0, ctx->stream, g);
