@@ -506,3 +506,30 @@ def test_captured_forks_and_reads_of_many_tokens(gpu, counts, h, N):
         again = run(c.device(), xs[3])
         torch.cuda.synchronize()
         assert torch.equal(again[0], want[3][0])
+
+
+@pytest.mark.parametrize("counts,h,N,d,S,lens,T,rotary,dtype", [
+    ((1,), 1, 64, 16, 1004, (3,), 1000, "rope", F32), ((1,), 1, 512, 128, 1004, (3,), 1000, "alibi", F32),
+    ((1,) * 256, 1, 34, 12, 8, (3, 0, 5), 1, "rope", BF16), ((1, 0) * 128, 2, 20, 8, 12, (3, 0, 5), 4, "pope", F32),
+    ((9,), 64, 16, 4, 8, (2, 5), 1, "alibi", F32), ((2, 1), 64, 18, 8, 8, (2, 5), 3, "alibi", BF16)])
+def test_long_calls_many_prompts_and_many_heads(gpu, counts, h, N, d, S, lens, T, rotary, dtype):
+    _check_read(gpu, Case(77, counts, h, N, d, S, lens, T, rotary, dtype))
+
+
+@pytest.mark.parametrize("T", [1, 3])
+def test_as_many_sequences_as_a_call_takes(gpu, T):
+    """65535 sequences alike: each within the bound of the definition."""
+    _, _, shared = gpu
+    one, B = Case(78, (1,), 1, 20, 8, 8, (3,), T, "rope", F32), 65535
+    t = one.device()
+    many = {n: t[n][:1].expand(B, *t[n].shape[1:]).contiguous() for n in ("x", "v", "keys", "values", "lens", "positions")}
+    many.update(rho=t["rho"], freqs=t["freqs"])
+    ref, mag, keys, _ = one.exact()
+    one.counts = [B]
+    got = one.call(shared, many)
+    bound = torch.from_numpy(U * _depth(one) * mag[:1]).to(DEV)
+    assert ((got.double() - torch.from_numpy(ref[:1]).to(DEV)).abs() <= bound).all()
+    assert torch.equal(many["keys"], many["keys"][:1].expand_as(many["keys"]))
+    assert np.array_equal(many["keys"][0].cpu().numpy() != 0, keys[0] != 0)
+    state = shared.shared_prefix_fork(t["rho"], many["keys"], many["values"], many["lens"] + T, counts=[B])
+    assert torch.equal(state, state[:1].expand_as(state)) and torch.isfinite(state[0]).all()
