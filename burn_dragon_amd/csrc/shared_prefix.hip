@@ -1275,8 +1275,10 @@ int bdh_launch_shared_steps(bdh_ctx *ctx, const SharedStepParams &p) {
   const bool large = p.rho_dtype == BDH_BF16 && (long)p.G * h * Nq * d > (1L << 24);
   bool even = true;
   for (int i = 1; i < p.G; ++i) even &= pr.begin[i + 1] - pr.begin[i] == pr.begin[1];
-  if (T > 1 && (long)B * T > (large ? 160L : 32L) * p.G && (long)B * T * h * Nq * d > (even ? 1L << 25 : 1L << 27))
-    return launch_dense(ctx, p, pr, rates, longest);
+  if (T > 1 && (long)B * T > (large ? 160L : 32L) * p.G && (long)B * T * h * Nq * d > (even ? 1L << 25 : 1L << 27)) {
+    rc = launch_dense(ctx, p, pr, rates, longest);
+    if (rc != BDH_E_NOMEM) return rc;  // without room for its workspace (asked for before anything is launched): as few tokens are
+  }
   // 32 queries a workgroup at most; of more, tiles of equal size
   const int rt = most <= 16 ? 1 : 2;
   // An f32 state is split where its prompts have more than 16 queries on average: splitting costs the same for few (prompts of 20, 7

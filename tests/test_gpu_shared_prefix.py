@@ -533,3 +533,24 @@ def test_as_many_sequences_as_a_call_takes(gpu, T):
     assert np.array_equal(many["keys"][0].cpu().numpy() != 0, keys[0] != 0)
     state = shared.shared_prefix_fork(t["rho"], many["keys"], many["values"], many["lens"] + T, counts=[B])
     assert torch.equal(state, state[:1].expand_as(state)) and torch.isfinite(state[0]).all()
+
+
+def test_many_tokens_without_room_for_dense_products(gpu):
+    """A context whose workspace may not hold the state in f32 makes the call as it makes one of few tokens, and refuses what
+    it has no room for at all."""
+    ffi, _, shared = gpu
+    c = Case(91, (3, 3), 4, 2047, 128, 16, (6, 0), 10, "alibi", BF16)
+    ref, mag, keys, _ = c.exact()
+    for mib in (0, 7):
+        ctx = ffi.Context(0)
+        ctx.set_option("workspace.max_mib", mib)
+        t = c.device()
+        out = c.call(shared, t, ctx=ctx)
+        assert (np.abs(out.double().cpu().numpy() - ref) <= U * _depth(c) * mag).all()
+        assert np.array_equal(t["keys"].double().cpu().numpy(), keys)
+    ctx.close()
+    ctx = ffi.Context(0)
+    ctx.set_option("workspace.max_mib", 1)
+    with pytest.raises(ffi.BdhError, match="workspace"):
+        c.call(shared, c.device(), ctx=ctx)
+    ctx.close()
