@@ -988,12 +988,12 @@ constexpr int kForkTokens = 64;  // whose values stand in LDS at a time
 
 // The (decayed) values of tokens s0 .. s0 + 63, up to the last one, as three bf16 terms [3][CB][72]: token by token of a column,
 // column 64 j + 4 i + c of the block at place 64 j + 16 c + i, so that a lane gets four neighbouring columns of a row.
-template <int CB, int THREADS>
+template <int CB>
 __device__ __forceinline__ void stage_values(const ForkArgs &g, const ForkTile &w, int s0, unsigned short *s_v) {
   constexpr int LDV = kForkTokens + 8;
   const int tokens = min((w.end - s0 + 31) & ~31, kForkTokens);
 #pragma unroll 1
-  for (int e = threadIdx.x; e < tokens / 8 * CB; e += THREADS) {
+  for (int e = threadIdx.x; e < tokens / 8 * CB; e += (int)blockDim.x) {
     const int c = e % CB, t = e / CB * 8, place = (c & ~63) + ((c & 3) << 4) + ((c >> 2) & 15);
     float v[8];
 #pragma unroll
@@ -1027,7 +1027,8 @@ __device__ __forceinline__ void stage_values(const ForkArgs &g, const ForkTile &
 // memory twice (rows of 1200 bytes: 523 -> 426 us).
 template <typename R, int CB>
 __global__ __launch_bounds__(64 * fork_waves(CB)) void k_shared_fork(ForkArgs g, Prompts pr, HeadRates rates) {
-  constexpr int NW = fork_waves(CB), TK = kForkTokens, LDV = TK + 8, CT = CB / 16;
+  constexpr int TK = kForkTokens, LDV = TK + 8, CT = CB / 16;
+  const int step = blockDim.x / 4;  // 16 rows a wavefront
   extern __shared__ __attribute__((aligned(16))) char s_dyn[];
   unsigned short *s_v = reinterpret_cast<unsigned short *>(s_dyn);
   const int lane = threadIdx.x & 63, wave = wave_of_thread(), k4 = lane >> 4, li = lane & 15;
@@ -1037,10 +1038,10 @@ __global__ __launch_bounds__(64 * fork_waves(CB)) void k_shared_fork(ForkArgs g,
   R *out = static_cast<R *>(g.out) + w.bh * g.Nq * g.d;
   const float *K = g.keys + w.bh * g.Nq * g.S;
   const int end = w.end;
-  if (end > 0 && end <= TK) stage_values<CB, 64 * NW>(g, w, 0, s_v);
+  if (end > 0 && end <= TK) stage_values<CB>(g, w, 0, s_v);
   __syncthreads();
 #pragma unroll 1
-  for (int m0 = w.first; m0 < w.last; m0 += NW * 16) {
+  for (int m0 = w.first; m0 < w.last; m0 += step) {
     const int n0 = m0 + wave * 16;
     const float *key = K + (long)min(n0 + li, g.Nq - 1) * g.S;
     f32x4 ahead[2][2];  // keys of twice 32 tokens
@@ -1069,7 +1070,7 @@ __global__ __launch_bounds__(64 * fork_waves(CB)) void k_shared_fork(ForkArgs g,
     for (int s0 = 0; s0 < end; s0 += TK) {
       if (end > TK) {
         __syncthreads();
-        stage_values<CB, 64 * NW>(g, w, s0, s_v);
+        stage_values<CB>(g, w, s0, s_v);
         __syncthreads();
       }
       const int stop = min(end - s0, TK);
@@ -1441,13 +1442,20 @@ int bdh_shared_prefix_fork(bdh_ctx *ctx, int G, const int32_t *counts_host, int 
   }
   ForkArgs g{rho, rho_out, keys, values, lens_dev, B, h, Nq, d, capacity, longest < 0 ? capacity : longest, 0, 0, 0, 0, rotary == BDH_ALIBI, false};
   // columns of a workgroup: all, or equal shares of at most 320 (what its LDS has room for)
-  const int shares = (d + 319) / 320, cols = ((d + shares - 1) / shares + 63) / 64 * 64;
+  const int shares = (d + 319) / 320;
+  int cols = ((d + shares - 1) / shares + 63) / 64 * 64;
+  // few rows: narrower blocks of columns, and then fewer wavefronts a workgroup, for workgroups on all CUs (4 sequences of 4 heads of
+  // 256, d = 256: 10.4 -> 5.5 us; one of 4 heads of 968, d = 244: 19 -> 8; where half of them have work, blocks of half the width
+  // cost more than they give: 7 of 4 heads of 148 rows, d = 452, 118 tokens 22.7 -> 24.7)
+  while (cols > 64 && (long)B * h * ((d + cols - 1) / cols) * ((Nq + 63) / 64) * 2 <= ctx->n_cu) cols -= 64;
   g.col_blocks = (d + cols - 1) / cols;
   // Rows of a workgroup: so many times those its wavefronts make at a time that the rounds of workgroups an XCD takes are fewest in
   // sum, with the values' way into LDS counted as one time more, and the rows that its L2 holds for all of its sequences are at
   // most 2.25 MiB of the 4 (us, as many workgroups as four a CU need | so: 32 sequences, 64 tokens, 4 heads of 8192, d = 256 392 | 352,
   // 16 tokens, 4 heads of 6620, d = 292 388 | 400, d = 320 333 | 313; 16 sequences, 48 tokens, 8 heads of 4096, d = 512, bf16 285 | 246)
-  const int step = fork_waves(cols) * 16, times = (Nq + step - 1) / step;
+  int waves = fork_waves(cols);
+  while (waves > 4 && (long)B * h * g.col_blocks * ((Nq + 16 * waves - 1) / (16 * waves)) < ctx->n_cu) waves -= 4;
+  const int step = waves * 16, times = (Nq + step - 1) / step;
   const size_t row_bytes = (size_t)d * (rho_dtype == BDH_BF16 ? 2 : 4);
   long best = -1;
   for (int t = 1; t <= times && (t == 1 || t * step * row_bytes <= (size_t)9 << 18); ++t) {
@@ -1469,9 +1477,9 @@ int bdh_shared_prefix_fork(bdh_ctx *ctx, int G, const int32_t *counts_host, int 
                        : cols == 192 ? (wide ? fork_kernel<float, 192>() : fork_kernel<unsigned short, 192>())
                        : cols == 256 ? (wide ? fork_kernel<float, 256>() : fork_kernel<unsigned short, 256>())
                                      : (wide ? fork_kernel<float, 320>() : fork_kernel<unsigned short, 320>());
-  BDH_HIP_CHECK(ctx, hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+  if (lds > 48 * 1024) BDH_HIP_CHECK(ctx, hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
   void *args[] = {&g, &pr, &rates};
-  BDH_HIP_CHECK(ctx, hipLaunchKernel(kernel, dim3((unsigned)((g.groups + 7) / 8 * 8 * B * g.col_blocks)), dim3(64 * fork_waves(cols)), args, lds, ctx->stream));
+  BDH_HIP_CHECK(ctx, hipLaunchKernel(kernel, dim3((unsigned)((g.groups + 7) / 8 * 8 * B * g.col_blocks)), dim3(64 * waves), args, lds, ctx->stream));
   return BDH_OK;
 }
 
