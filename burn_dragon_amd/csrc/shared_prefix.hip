@@ -317,16 +317,17 @@ struct Product {
         const float *at = x + min(i0 + k * parts, nb - 1) * step;
         v[k] = f32x2u{at[c0], at[c1]};
       }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int i = i0 + k * parts;
-        const bool f0 = v[k].x != 0.0f && in0 && i < nb, f1 = v[k].y != 0.0f && in1 && i < nb;
+#pragma unroll 1
+      for (int i = i0; i < min(i0 + 8 * parts, nb); i += parts) {
+        const bool f0 = v[0].x != 0.0f && in0, f1 = v[0].y != 0.0f && in1;
         u0 |= f0;
         u1 |= f1;
         const unsigned long long mask = __ballot(f0 || f1);
-        if (lane == 0 && i < nb) sh.fires[i][p >> 6] = mask;
+        if (lane == 0) sh.fires[i][p >> 6] = mask;
         sh.item[wave][f0 || f1 ? items + __popcll(mask & ((1ull << lane) - 1)) : 1024 + lane] = (unsigned short)(i << 8 | p);
         items += __popcll(mask);
+#pragma unroll
+        for (int k = 0; k < 7; ++k) v[k] = v[k + 1];
       }
     }
     if (rope) u0 = u1 = u0 || u1;
