@@ -151,7 +151,7 @@ struct TileShared {
 template <typename R, int RT, int MODE>
 struct Product {
   static constexpr int kQ = 16 * RT, C = MODE == kHalf ? 8 : 4, kCols = 16 * C, kStep = MODE == kF32 ? 16 : 32;
-  static constexpr int kDepth = MODE == kF32 ? 4 : 2;
+  static constexpr int kDepth = 2;
   TileShared &sh;
   char *tile;  // the queries: f32 [query][ld], or three planes [query][ld] of bf16
   int ld, cnt = 0;
@@ -583,8 +583,9 @@ struct Product {
 // 8 heads of 16384, d = 512, bf16: 108 us for 341 MB of rows, keys and activations, 3.2 TB/s where a sum over a large tensor
 // reads 4.0; registers and LDS leave room for two workgroups a CU, and one lists and turns its queries while the other multiplies.
 // Below that the steps of one workgroup after the other: 32 sequences of one prompt, 4 heads of 8192, d = 256, f32: 20.5 us
-// for 54 MB, of which a workgroup spends 1.2 on its arguments, 2.7 on the activations, 2.8 on listing and turning what
-// fires, 4.2 on rows and products, 5.1 on keys, 1.3 on its sums; 4 sequences, 4 heads of 256: 9.6 us, all of it waiting.
+// for 54 MB, of which a workgroup spends 0.8 on its arguments, 2.8 on the activations, 2.5 on listing and turning what
+// fires, 3.4 on rows and products, 4.8 on keys, 1.6 on its sums; 4 sequences, 4 heads of 256: 8.3 us, all of it waiting
+// (9.6 with the look at the activations unrolled and twice as many steps of a product on their way: both are instructions to wait for).
 // f32 states of 17 to 32 queries are split on the way (kSplit): the f32 instructions take 256 cycles for 32 rows, six bf16 ones 96.
 // With tiles of 64 queries a CU has fewer workgroups (us, 64 at a time | 32: 40 sequences of 4 heads of 8192, d = 256, f32 50 |
 // 34, bf16 44 | 45; of 8 heads of 16384, d = 512, f32 133 | 138, bf16 112 | 83; 100 of them 258 | 263, bf16 282 | 184).
