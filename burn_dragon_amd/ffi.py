@@ -245,8 +245,8 @@ class Context:
 
 def context_on(device: int, ctx: Optional[Context] = None) -> Context:
     """The context for tensors on device `device` (Tensor.get_device(); -1 is host memory): ctx, or the device's default
-    one.  Refuses what no kernel may be given: tensors in host memory, a device that is not the current one, a context of
-    another device."""
+    one, bound to the stream it follows, so that its `_lib` may be called as it is.  Refuses what no kernel may be given:
+    tensors in host memory, a device that is not the current one, a context of another device."""
     import torch
 
     if device < 0:
@@ -255,9 +255,11 @@ def context_on(device: int, ctx: Optional[Context] = None) -> Context:
     if current != device:
         raise ValueError(f"tensors on cuda:{device}, the current device is cuda:{current}")
     if ctx is None:
-        return _default_ctx.get(device) or default_context(device)
-    if ctx.device_id != device:
+        ctx = _default_ctx.get(device) or default_context(device)
+    elif ctx.device_id != device:
         raise ValueError(f"tensors on cuda:{device}, the context is on cuda:{ctx.device_id}")
+    if ctx._follow and torch._C._cuda_getCurrentRawStream(device) != ctx._stream:
+        ctx.lib  # re-binds it
     return ctx
 
 

@@ -82,9 +82,7 @@ def _row_stride(name: str, t: torch.Tensor, B: int, width: int, dtype, on: int) 
     return t.stride(0) if t.dim() == 2 and B > 1 else 0
 
 
-def _per_row(name: str, p: Penalty, B: int, like: torch.Tensor, on: int) -> Optional[torch.Tensor]:
-    if p is None:
-        return None
+def _per_row(name: str, p: Union[float, torch.Tensor], B: int, like: torch.Tensor, on: int) -> torch.Tensor:
     if not isinstance(p, torch.Tensor):
         return torch.full((B,), float(p), device=like.device, dtype=torch.float32)
     if p.shape != (B,) or p.dtype is not torch.float32 or p.get_device() != on or not p.is_contiguous():
@@ -104,8 +102,8 @@ def count_tokens(tokens: torch.Tensor, seen: torch.Tensor, lens: Optional[torch.
     if lens is not None and (lens.shape != (B,) or lens.dtype is not torch.int32 or lens.get_device() != on or not lens.is_contiguous()):
         raise ValueError(f"lens: expected int32 [{B}] on {tokens.device}")
     ctx = ffi.context_on(on, ctx)
-    ctx.check(ctx.lib.bdh_count_tokens(ctx.handle, B, T, V, ffi.ptr(tokens), tokens.stride(0) if B > 1 else max(T, 1),
-                                       ffi.ptr(lens), int(bool(prompt)), ffi.ptr(seen)))
+    ctx.check(ctx._lib.bdh_count_tokens(ctx.handle, B, T, V, tokens.data_ptr(), tokens.stride(0) if B > 1 else max(T, 1),
+                                        None if lens is None else lens.data_ptr(), 1 if prompt else 0, seen.data_ptr()))
 
 
 def apply_rules(logits: torch.Tensor, rules: LogitRules, seen: Optional[torch.Tensor] = None,
@@ -136,9 +134,13 @@ def apply_rules(logits: torch.Tensor, rules: LogitRules, seen: Optional[torch.Te
         if not newest.is_contiguous():
             newest = newest.contiguous()
         newest_ptr = newest.data_ptr()
-    repetition = _per_row("repetition", rules.repetition, B, logits, on)  # held until the call: a tensor made here has no
-    presence = _per_row("presence", rules.presence, B, logits, on)        # other owner
-    frequency = _per_row("frequency", rules.frequency, B, logits, on)
+    repetition, presence, frequency = rules.repetition, rules.presence, rules.frequency
+    if repetition is not None:  # held until the call: a tensor made here has no other owner
+        repetition = _per_row("repetition", repetition, B, logits, on)
+    if presence is not None:
+        presence = _per_row("presence", presence, B, logits, on)
+    if frequency is not None:
+        frequency = _per_row("frequency", frequency, B, logits, on)
     bias, allowed = rules.bias, rules.allowed
     bias_stride = 0 if bias is None else _row_stride("bias", bias, B, V, f32, on)
     allowed_stride = 0 if allowed is None else _row_stride("allowed", allowed, B, (V + 31) // 32, torch.int32, on)
@@ -150,7 +152,7 @@ def apply_rules(logits: torch.Tensor, rules: LogitRules, seen: Optional[torch.Te
             raise ValueError(f"out: expected f32 rows [{B}, {V}] on {logits.device}")
         out_stride = out.stride(0) if B > 1 else V
     ctx = ffi.context_on(on, ctx)
-    ctx.check(ctx.lib.bdh_logit_rules(
+    ctx.check(ctx._lib.bdh_logit_rules(
         ctx.handle, B, V, logits.data_ptr(), logits.stride(0) if B > 1 else V, seen_ptr, newest_ptr,
         None if repetition is None else repetition.data_ptr(), None if presence is None else presence.data_ptr(),
         None if frequency is None else frequency.data_ptr(), None if bias is None else bias.data_ptr(), bias_stride,

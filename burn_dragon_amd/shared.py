@@ -81,7 +81,7 @@ def shared_prefix_attention(query: torch.Tensor, value: torch.Tensor, rho: torch
     slopes = _slopes(alibi_slopes, h)
     ctx = ffi.context_on(on, ctx)
     out = query.new_empty(B, h, T, d)
-    ctx.check(ctx.lib.bdh_shared_prefix_attention(
+    ctx.check(ctx._lib.bdh_shared_prefix_attention(
         ctx.handle, G, n_of, B, h, T, N, d, rot, query.data_ptr(), value.data_ptr(),
         None if rot == RotaryEmbedding.ALIBI else freqs.data_ptr(), int(position), None if positions is None else positions.data_ptr(), slopes,
         rho.data_ptr(), _DTYPES[rho.dtype], S, lens.data_ptr(), -1 if longest is None else int(longest), keys.data_ptr(),
@@ -111,7 +111,7 @@ def shared_prefix_fork(rho: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     n_of = _prompts(counts, G, B)
     slopes = _slopes(alibi_slopes, h)
     ctx = ffi.context_on(on, ctx)
-    ctx.check(ctx.lib.bdh_shared_prefix_fork(
+    ctx.check(ctx._lib.bdh_shared_prefix_fork(
         ctx.handle, G, n_of, B, h, Nq, d, int(RotaryEmbedding.parse(rotary_embedding)), slopes,
         rho.data_ptr(), _DTYPES[rho.dtype], S, lens.data_ptr(), -1 if longest is None else int(longest), keys.data_ptr(),
         values.data_ptr(), out.data_ptr()))

@@ -49,4 +49,4 @@ def copy_slots(buffers: Iterable[Tuple[torch.Tensor, torch.Tensor, int]], origin
     if origin.shape != (n,) or origin.dtype != torch.int32 or origin.get_device() != on or not origin.is_contiguous():
         raise ValueError(f"origin: expected int32 [{n}] on {dev}, got {origin.dtype} {tuple(origin.shape)} on {origin.device}")
     ctx = ffi.context_on(on, ctx)
-    ctx.check(ctx.lib.bdh_copy_slots(ctx.handle, table, len(buffers), n, m, origin.data_ptr()))
+    ctx.check(ctx._lib.bdh_copy_slots(ctx.handle, table, len(buffers), n, m, origin.data_ptr()))
