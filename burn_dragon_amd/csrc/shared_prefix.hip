@@ -986,14 +986,12 @@ struct ForkTile {
   }
 };
 
-constexpr int kForkTokens = 64;  // whose values stand in LDS at a time
-
-// The (decayed) values of tokens s0 .. s0 + 63, up to the last one, as three bf16 terms [3][CB][72]: token by token of a column,
+// The (decayed) values of TK tokens from s0 on, up to the last one, as three bf16 terms [3][CB][TK + 8]: token by token of a column,
 // column 64 j + 4 i + c of the block at place 64 j + 16 c + i, so that a lane gets four neighbouring columns of a row.
-template <int CB>
+template <int CB, int TK>
 __device__ __forceinline__ void stage_values(const ForkArgs &g, const ForkTile &w, int s0, unsigned short *s_v) {
-  constexpr int LDV = kForkTokens + 8;
-  const int tokens = min((w.end - s0 + 31) & ~31, kForkTokens);
+  constexpr int LDV = TK + 8;
+  const int tokens = min((w.end - s0 + 31) & ~31, TK);
 #pragma unroll 1
   for (int e = threadIdx.x; e < tokens / 8 * CB; e += (int)blockDim.x) {
     const int c = e % CB, t = e / CB * 8, place = (c & ~63) + ((c & 3) << 4) + ((c >> 2) & 15);
@@ -1019,7 +1017,8 @@ __device__ __forceinline__ void stage_values(const ForkArgs &g, const ForkTile &
 // a^len rho + sum_s a^(len-s) k_s (x) v_s for `rows` rows and CB columns of one (sequence, head).  A wavefront makes 16 rows at a
 // time on top of the prompt's rows: it splits the rows' keys into bf16 terms as they lie in memory and multiplies six of the
 // nine products with the terms of the values on v_mfma_f32_16x16x32_bf16 (what is left out is below 2^-23 of a product).  The
-// values of 64 tokens stand in LDS; those of more pass through it 64 at a time, for every 192 (128) rows again.
+// values of TK tokens stand in LDS: 64, or 128 of up to 192 columns where a call has 65 to 128 (32 sequences of up to 100, 4
+// heads of 8192, d = 256: 582 -> 483 us); those of more pass through it 64 at a time, for every 192 (128) rows again.
 // Bound by the way to memory and to L2: the largest case (32 sequences, 64 tokens, 4 heads of 8192, d = 256: 1 GiB written, 256 MiB of
 // keys, the prompt's rows 32 times from L2, which misses 11 % of them: a workgroup's neighbours on the XCD make the same rows
 // of other sequences) takes 350 us; its writes alone take 204, with the keys 291, with the prompt's rows 352 (in shorter
@@ -1027,9 +1026,9 @@ __device__ __forceinline__ void stage_values(const ForkArgs &g, const ForkTile &
 // no wait for the stores between: 356.  A workgroup takes whole rows of up
 // to 320 columns, and the column blocks of wider ones stay on one XCD: a cache line that two XCDs write a part of goes to
 // memory twice (rows of 1200 bytes: 523 -> 426 us).
-template <typename R, int CB>
+template <typename R, int CB, int TK>
 __global__ __launch_bounds__(64 * fork_waves(CB)) void k_shared_fork(ForkArgs g, Prompts pr, HeadRates rates) {
-  constexpr int TK = kForkTokens, LDV = TK + 8, CT = CB / 16;
+  constexpr int LDV = TK + 8, CT = CB / 16;
   const int step = blockDim.x / 4;  // 16 rows a wavefront
   extern __shared__ __attribute__((aligned(16))) char s_dyn[];
   unsigned short *s_v = reinterpret_cast<unsigned short *>(s_dyn);
@@ -1040,7 +1039,7 @@ __global__ __launch_bounds__(64 * fork_waves(CB)) void k_shared_fork(ForkArgs g,
   R *out = static_cast<R *>(g.out) + w.bh * g.Nq * g.d;
   const float *K = g.keys + w.bh * g.Nq * g.S;
   const int end = w.end;
-  if (end > 0 && end <= TK) stage_values<CB>(g, w, 0, s_v);
+  if (end > 0 && end <= TK) stage_values<CB, TK>(g, w, 0, s_v);
   __syncthreads();
 #pragma unroll 1
   for (int m0 = w.first; m0 < w.last; m0 += step) {
@@ -1072,7 +1071,7 @@ __global__ __launch_bounds__(64 * fork_waves(CB)) void k_shared_fork(ForkArgs g,
     for (int s0 = 0; s0 < end; s0 += TK) {
       if (end > TK) {
         __syncthreads();
-        stage_values<CB>(g, w, s0, s_v);
+        stage_values<CB, TK>(g, w, s0, s_v);
         __syncthreads();
       }
       const int stop = min(end - s0, TK);
@@ -1116,9 +1115,17 @@ __global__ __launch_bounds__(64 * fork_waves(CB)) void k_shared_fork(ForkArgs g,
   }
 }
 
-template <typename R, int CB>
-const void *fork_kernel() {
-  return reinterpret_cast<const void *>(k_shared_fork<R, CB>);
+template <typename R>
+const void *fork_kernel(int cols, int tokens) {
+  if (tokens == 128)
+    return cols == 64    ? reinterpret_cast<const void *>(k_shared_fork<R, 64, 128>)
+           : cols == 128 ? reinterpret_cast<const void *>(k_shared_fork<R, 128, 128>)
+                         : reinterpret_cast<const void *>(k_shared_fork<R, 192, 128>);
+  return cols == 64    ? reinterpret_cast<const void *>(k_shared_fork<R, 64, 64>)
+         : cols == 128 ? reinterpret_cast<const void *>(k_shared_fork<R, 128, 64>)
+         : cols == 192 ? reinterpret_cast<const void *>(k_shared_fork<R, 192, 64>)
+         : cols == 256 ? reinterpret_cast<const void *>(k_shared_fork<R, 256, 64>)
+                       : reinterpret_cast<const void *>(k_shared_fork<R, 320, 64>);
 }
 
 bool disjoint(const void *a, size_t na, const void *b, size_t nb) {
@@ -1444,7 +1451,9 @@ int bdh_shared_prefix_fork(bdh_ctx *ctx, int G, const int32_t *counts_host, int 
   }
   ForkArgs g{rho, rho_out, keys, values, lens_dev, B, h, Nq, d, capacity, longest < 0 ? capacity : longest, 0, 0, 0, 0, rotary == BDH_ALIBI, false};
   // columns of a workgroup: all, or equal shares of at most 320 (what its LDS has room for)
-  const int shares = (d + 319) / 320;
+  const int tokens = g.longest > 64 && g.longest <= 128 ? 128 : 64;  // whose values stand in LDS at a time
+  const int widest = tokens == 128 ? 192 : 320;  // columns LDS has room for
+  const int shares = (d + widest - 1) / widest;
   int cols = ((d + shares - 1) / shares + 63) / 64 * 64;
   // few rows: narrower blocks of columns, and then fewer wavefronts a workgroup, for workgroups on all CUs (4 sequences of 4 heads of
   // 256, d = 256: 10.4 -> 5.5 us; one of 4 heads of 968, d = 244: 19 -> 8; where half of them have work, blocks of half the width
@@ -1472,13 +1481,8 @@ int bdh_shared_prefix_fork(bdh_ctx *ctx, int G, const int32_t *counts_host, int 
   g.groups = g.row_blocks * h;
   g.whole_lines = row_bytes % 128 == 0 && bdh_aligned(rho_out, 128);
   if ((g.groups + 7L) / 8 * 8 * B * g.col_blocks > 0x7fffffffL) return bdh_fail(ctx, BDH_E_SHAPE, "too many tiles");
-  const size_t lds = (size_t)6 * cols * (kForkTokens + 8);
-  const bool wide = rho_dtype == BDH_F32;
-  const void *kernel = cols == 64    ? (wide ? fork_kernel<float, 64>() : fork_kernel<unsigned short, 64>())
-                       : cols == 128 ? (wide ? fork_kernel<float, 128>() : fork_kernel<unsigned short, 128>())
-                       : cols == 192 ? (wide ? fork_kernel<float, 192>() : fork_kernel<unsigned short, 192>())
-                       : cols == 256 ? (wide ? fork_kernel<float, 256>() : fork_kernel<unsigned short, 256>())
-                                     : (wide ? fork_kernel<float, 320>() : fork_kernel<unsigned short, 320>());
+  const size_t lds = (size_t)6 * cols * (tokens + 8);
+  const void *kernel = rho_dtype == BDH_F32 ? fork_kernel<float>(cols, tokens) : fork_kernel<unsigned short>(cols, tokens);
   if (lds > 48 * 1024) BDH_HIP_CHECK(ctx, hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
   void *args[] = {&g, &pr, &rates};
   BDH_HIP_CHECK(ctx, hipLaunchKernel(kernel, dim3((unsigned)((g.groups + 7) / 8 * 8 * B * g.col_blocks)), dim3(64 * waves), args, lds, ctx->stream));

@@ -206,6 +206,12 @@ FORK = [
     # several times the rows that a workgroup makes at a time
     ((40, 24), 16, 1000, 8, 12, (7, 12, 0), "rope", F32),
     ((70,), 8, 1010, 8, 72, (71, 64, 0, 33), "alibi", BF16),
+    # 65 to 128 tokens, and more, in blocks of 64, 128 and 192 columns
+    ((3, 1), 2, 70, 60, 128, (128, 65, 0), "rope", F32),
+    ((4, 6), 4, 600, 180, 112, (100, 3, 112, 64), "pope", F32),
+    ((9,), 4, 610, 200, 100, (97, 100, 65), "alibi", BF16),
+    ((4,), 4, 640, 184, 96, (96, 33), "rope", BF16),
+    ((5,), 4, 600, 180, 160, (130, 3, 159), "rope", F32),
 ]
 
 
