@@ -175,8 +175,9 @@ def generate_samples(model: BDH, prompt_tokens: List[int], n: int, settings: Gen
                      generator: Optional[torch.Generator] = None) -> List[List[int]]:
     """n continuations of one prompt, drawn together: the prompt is read once, its state is shared by all of them for the
     first `capacity` tokens of their own (BDH.share_state) and copied for each only then.  `rules` apply to the logits of
-    every draw; a sequence ends with stop_token, which is part of it, or after settings.max_new_tokens, and the ended ones
-    leave the batch every few tokens.  Each sequence has its own variates: where others end does not change them.
+    every draw; a sequence ends with stop_token, which is part of it, where the rules allow nothing more (its logits are all
+    -inf: nothing is drawn from them), or after settings.max_new_tokens, and the ended ones leave the batch every few tokens.
+    Each sequence has its own variates: where others end does not change them.
     Returns the new tokens of each (the reference generates one sequence at a time, src/generation.rs:158-203)."""
     if settings.max_new_tokens is None or settings.max_new_tokens < 0:
         raise ValueError("max_new_tokens says how long the samples may become")
@@ -197,21 +198,26 @@ def generate_samples(model: BDH, prompt_tokens: List[int], n: int, settings: Gen
             count_tokens(said, seen, prompt=True, ctx=model.ctx)
     alive = list(range(n))  # the samples that the rows of the batch are
     alive_dev = torch.arange(n, device=dev)
-    produced = []  # (rows, tokens) of every draw
-    newest, every = None, 16
+    produced = []  # (rows, tokens, largest logits or None) of every draw
+    newest, every, largest = None, 16, None
     for step in range(settings.max_new_tokens):
         if rules is not None:
             logits = apply_rules(logits, rules, seen, newest if seen is not None else None, ctx=model.ctx)
+            largest = logits.amax(1)  # looked at with the tokens: what is drawn meanwhile from a row of -inf is dropped
         if step % every == 0:
             variates = uniform_variates(every * n, dev, generator).reshape(every, n)
         newest = sample_from_logits(model, logits, settings.temperature, settings.top_k,
                                     variates[step % every].index_select(0, alive_dev))
-        produced.append((alive, newest))
+        produced.append((alive, newest, largest))
         if step + 1 == settings.max_new_tokens:
             break
-        if stop_token is not None and step % every == every - 1:
-            recent = torch.stack([t for _, t in produced[-every:]])
-            live = [i for i, ended in enumerate((recent == stop_token).any(0).tolist()) if not ended]
+        if (stop_token is not None or rules is not None) and step % every == every - 1:
+            ended = torch.zeros_like(newest, dtype=torch.bool)
+            if stop_token is not None:
+                ended |= (torch.stack([t for _, t, _ in produced[-every:]]) == stop_token).any(0)
+            if rules is not None:
+                ended |= torch.isneginf(torch.stack([m for _, _, m in produced[-every:]])).any(0)
+            live = [i for i, e in enumerate(ended.tolist()) if not e]
             if not live:
                 break
             if len(live) < len(alive):
@@ -229,10 +235,12 @@ def generate_samples(model: BDH, prompt_tokens: List[int], n: int, settings: Gen
         tokens = newest.reshape(-1, 1)
         logits = (model.forward_shared(tokens, shared) if own is None else model.forward_with_state(tokens, own))[:, -1]
     out: List[List[int]] = [[] for _ in range(n)]
-    for rows, tokens in produced:
-        for i, t in zip(rows, tokens.tolist()):
-            if not out[i] or out[i][-1] != stop_token:
+    going = [True] * n
+    for rows, tokens, most in produced:
+        for i, t, empty in zip(rows, tokens.tolist(), [False] * len(rows) if most is None else torch.isneginf(most).tolist()):
+            if going[i] and not empty:
                 out[i].append(t)
+            going[i] = going[i] and not empty and t != stop_token
     return out
 
 

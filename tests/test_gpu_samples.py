@@ -176,3 +176,24 @@ def test_states_with_logged_updates_are_flushed_before_they_are_shared_or_moved(
     tokens = torch.from_numpy(rng.integers(0, 69, (4, 1)))
     _close(*[m.forward_shared(tokens, s) for m, s in zip((model, plain), shared)], 1e-3)
     _close(*[m.forward_with_state(tokens[:2], s) for m, s in zip((model, plain), moved)], 1e-3)
+
+
+def test_a_sample_of_which_the_rules_allow_nothing_ends(bda):
+    """A row whose mask is empty from the start, one that a bias takes everything from, and rows that run out of allowed tokens
+    as none may be said twice: each ends with what it was allowed, the others go on."""
+    from burn_dragon_amd.generation import GenerationSettings, generate_samples
+    from burn_dragon_amd.rules import pack_allowed
+
+    model = _model(bda, "rope")
+    allowed = torch.zeros((5, 69), dtype=torch.bool)
+    for row, n in enumerate((0, 40, 5, 19, 69)):
+        allowed[row, :n] = True
+    bias = torch.zeros((5, 69))
+    bias[4] = float("-inf")
+    sizes = [0, 40, 5, 19, 0]
+    for stop in (None, 68):
+        rules = bda.LogitRules(frequency=float("inf"), bias=bias.to(DEV), allowed=pack_allowed(allowed.to(DEV)))
+        got = generate_samples(model, [3, 1, 4], 5, GenerationSettings(max_new_tokens=60), rules, stop, capacity=12)
+        assert [sorted(s) for s in got] == [list(range(n)) for n in sizes]
+    one = bda.LogitRules(allowed=torch.zeros(3, dtype=torch.int32, device=DEV))
+    assert generate_samples(model, [3], 2, GenerationSettings(max_new_tokens=3), one) == [[], []]
