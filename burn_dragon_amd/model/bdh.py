@@ -173,7 +173,8 @@ class BDH:
     def share_state(self, state: ModelState, counts: Sequence[int], capacity: int = 64) -> SharedState:
         """Many sequences for the prompts that `state` holds: counts[g] of them continue sequence g of it, up to `capacity`
         tokens each (rounded up to a multiple of 4), with the prompts' states read once for all.  The state is taken
-        over: `state` is a fresh one afterwards."""
+        over: `state` is a fresh one afterwards.  Positions are int32 on the device: where they rotate, prompts and
+        capacity that go beyond them are refused (forward_with_state takes such positions)."""
         if state.storage is None or state.position == 0:
             raise ValueError("run the prompts before sharing their state")
         counts = [int(c) for c in counts]
@@ -182,8 +183,10 @@ class BDH:
             raise ValueError(f"counts {counts} do not deal sequences to {G} prompts")
         if capacity < 1:
             raise ValueError("capacity must be positive")
-        self.materialize_state(state)
         B, S = sum(counts), (capacity + 3) // 4 * 4
+        if state.position + S > 0x7FFFFFFF and RotaryEmbedding.parse(self.kernel.rotary_embedding) != RotaryEmbedding.ALIBI:
+            raise ValueError(f"{state.position} tokens and room for {S} more go beyond the int32 positions of a shared state")
+        self.materialize_state(state)
         keys = torch.zeros((L, B, self.n_head, self.latent_q, S), device=self.device, dtype=torch.float32)
         values = torch.zeros((L, B, S, self.n_embd), device=self.device, dtype=torch.float32)
         lens = torch.zeros((B,), device=self.device, dtype=torch.int32)

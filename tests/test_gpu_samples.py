@@ -197,3 +197,31 @@ def test_a_sample_of_which_the_rules_allow_nothing_ends(bda):
         assert [sorted(s) for s in got] == [list(range(n)) for n in sizes]
     one = bda.LogitRules(allowed=torch.zeros(3, dtype=torch.int32, device=DEV))
     assert generate_samples(model, [3], 2, GenerationSettings(max_new_tokens=3), one) == [[], []]
+
+
+def test_positions_beyond_31_bits_are_refused(bda):
+    """Positions are held in 32 bits beside a shared state: the last one that fits is rotated as sequences of their own rotate it, one
+    more is refused and the state is not taken over.  Nothing is rotated by ALiBi."""
+    model = _model(bda, "rope")
+    state, own = model.init_state(), model.init_state()
+    model.forward_with_state(torch.tensor([[1, 2, 3]]), state)
+    model.forward_with_state(torch.tensor([[1, 2, 3], [1, 2, 3]]), own)
+    state.position = own.position = 2**31 - 9
+    for capacity in (9, 12, 100):
+        with pytest.raises(ValueError, match="position"):
+            model.share_state(state, [2], capacity)
+    assert state.storage is not None and state.position == 2**31 - 9
+    shared = model.share_state(state, [2], 8)
+    for t in range(8):
+        tokens = torch.tensor([[t], [9 - t]])
+        _close(model.forward_shared(tokens, shared), model.forward_with_state(tokens, own), 1e-3)
+    assert shared.position == own.position == 2**31 - 1 and shared.positions.tolist() == [2**31 - 1] * 2
+    decaying = _model(bda, "alibi")
+    state, own = decaying.init_state(), decaying.init_state()
+    for s in (state, own):
+        decaying.forward_with_state(torch.tensor([[1, 2, 3]]), s)
+        s.position = 2**31 + 5
+    shared = decaying.share_state(state, [1], 4)
+    for t in range(3):
+        _close(decaying.forward_shared(torch.tensor([[t]]), shared), decaying.forward_with_state(torch.tensor([[t]]), own), 1e-3)
+    assert shared.position == 2**31 + 8
