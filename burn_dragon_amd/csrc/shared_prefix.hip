@@ -63,9 +63,13 @@ __device__ __forceinline__ float sum8(const float *p, long step, int n) {
   return s;
 }
 
+// the largest bf16 (0x1.fep127, 3.3895e38) for what is above it, so that the leading term of a finite number is never infinite: what
+// is missing is exact in the other two
+__device__ __forceinline__ float in_bf16_range(float v) { return __builtin_amdgcn_fmed3f(v, -0x1.fep127f, 0x1.fep127f); }
+
 // two floats as pairs (number m) of three bf16 terms, each rounded to the nearest: hi + mid + lo is the float
 __device__ __forceinline__ void split_pair(float a, float b, u32x4 (&terms)[3], int m) {
-  const unsigned int hi = pack_bf16_rne(a, b);
+  const unsigned int hi = pack_bf16_rne(in_bf16_range(a), in_bf16_range(b));
   const float ra = a - __uint_as_float(hi << 16), rb = b - __uint_as_float(hi & 0xffff0000u);
   const unsigned int mid = pack_bf16_rne(ra, rb);
   terms[0][m] = hi;
@@ -168,7 +172,7 @@ struct Product {
       reinterpret_cast<float *>(tile)[i * ld + place] = v;
     } else {  // hi + mid + lo is v itself
       unsigned short *p = reinterpret_cast<unsigned short *>(tile) + i * ld + place;
-      const unsigned int hi = pack_bf16_rne(v, 0.0f);
+      const unsigned int hi = pack_bf16_rne(in_bf16_range(v), 0.0f);
       const float r = v - __uint_as_float(hi << 16);
       const unsigned int mid = pack_bf16_rne(r, 0.0f);
       p[0] = (unsigned short)hi;

@@ -587,7 +587,8 @@ int bdh_model_flush_layers(bdh_model *model, bdh_model_logs *logs, void *const *
  * d a multiple of 4, at most 1024; capacity a multiple of 4, at most 2^20; h at most 64; at most BDH_MAX_SHARED_PROMPTS prompts
  * and B * h <= 65535 a call; Nq * capacity < 2^31, B * h * T < 2^21.  rho, keys, values, out and rho_out on 16 bytes.  A call in a
  * HIP graph takes longest = -1 (a replay's lengths are the device's).
- * Inputs are assumed finite.  Nothing is copied to or from the host, no result depends on the order of atomics.
+ * Inputs are assumed finite; where many tokens go through dense products (more than 32 of a prompt), also below 3.389e38 in
+ * magnitude, as in the other forms that use those.  Nothing is copied to or from the host, no result depends on the order of atomics.
  */
 #define BDH_MAX_SHARED_PROMPTS 256
 int bdh_shared_prefix_attention(bdh_ctx *ctx, int G, const int32_t *counts_host, int B, int h, int T, int N, int d,

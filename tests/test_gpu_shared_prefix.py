@@ -560,3 +560,50 @@ def test_many_tokens_without_room_for_dense_products(gpu):
     with pytest.raises(ffi.BdhError, match="workspace"):
         c.call(shared, c.device(), ctx=ctx)
     ctx.close()
+
+
+# sequences, tokens, columns, state: the f32 cores, split f32 states, bf16 states, several tokens of few
+@pytest.mark.parametrize("B,T,d,dtype", [(4, 1, 64, F32), (20, 1, 64, F32), (4, 1, 64, BF16), (20, 1, 132, BF16), (3, 9, 64, F32),
+                                         (2, 3, 64, BF16)])
+def test_the_largest_numbers_of_f32(gpu, B, T, d, dtype):
+    """Numbers between the largest of bf16 (3.3895e38) and the largest of f32, in the prompt's state (f32) or among the activations:
+    sums that f32 holds are what the definition gives, to the bound of one product (24 + 8 + 3 roundings and one term)."""
+    _, _, shared = gpu
+    rng = np.random.default_rng(13)
+    N, h, top = 130, 2, float(np.finfo(np.float32).max)
+    many = np.float32(top) * np.float32(1) - np.float32(2.0**104) * rng.integers(0, 2**15, (h, N, d)).astype(np.float32)
+    assert (many > 3.3895e38).all() and np.isfinite(many).all()
+    small = (rng.integers(1, 4, (h, N, d)) / 8).astype(np.float32)
+    for large_state in ([True, False] if dtype == F32 else [False]):
+        x = np.zeros((B, h, T, N), np.float32)
+        for b in range(B):
+            for i in range(h):
+                x[b, i, np.arange(T), rng.choice(N, T, replace=False)] = 0.25 if large_state else many[i, 0, 0]
+        rho = torch.from_numpy(many if large_state else small).to(dtype)[None]
+        keys, values = torch.zeros((B, h, N, 12), device=DEV), torch.zeros((B, 12, d), device=DEV)
+        lens = torch.zeros(B, dtype=torch.int32, device=DEV)
+        out = shared.shared_prefix_attention(torch.from_numpy(x).to(DEV), torch.zeros((B, T, d), device=DEV), rho.to(DEV), keys, values,
+                                             lens, None, rotary_embedding="alibi", alibi_slopes=[0.0] * h)
+        want = np.einsum("bhtn,hnd->bhtd", x.astype(np.float64), rho[0].double().numpy())
+        assert (np.abs(out.double().cpu().numpy() - want) <= U * 36 * want).all()
+        assert torch.equal(keys[:, :, :, :T].permute(0, 1, 3, 2).cpu(), torch.from_numpy(x))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_the_largest_numbers_of_f32_in_a_fork(gpu, dtype):
+    """As above, in keys and in values; a token of keys 0 is of no use to the others."""
+    _, _, shared = gpu
+    N, d, S = 34, 68, 8
+    top = np.float32(np.finfo(np.float32).max)
+    keys, values = np.zeros((2, 1, N, S), np.float32), np.zeros((2, S, d), np.float32)
+    keys[0, 0, :17, 2], values[0, 2] = 0.25, top  # values, and further down keys
+    keys[0, 0, 17:, 5], values[0, 5] = -top, 0.125
+    keys[1, 0, 5, 0], values[1, 0] = -top, -0.25
+    rho = torch.ones((1, 1, N, d), device=DEV, dtype=dtype)
+    lens = torch.tensor([8, 3], dtype=torch.int32, device=DEV)
+    out = shared.shared_prefix_fork(rho, torch.from_numpy(keys).to(DEV), torch.from_numpy(values).to(DEV), lens)
+    want = 1 + np.einsum("bhns,bsd->bhnd", keys.astype(np.float64), values.astype(np.float64))
+    bound = U * 20 * np.abs(want)
+    if dtype == BF16:
+        bound = bound * (1 + 2.0**-8) + 2.0**-8 * np.abs(want)
+    assert (np.abs(out.double().cpu().numpy() - want) <= bound).all()
