@@ -96,6 +96,8 @@ def count_tokens(tokens: torch.Tensor, seen: torch.Tensor, lens: Optional[torch.
     the prompt, or counted as produced.  Ids outside the vocabulary are skipped."""
     B, T = tokens.shape
     on, V = tokens.get_device(), seen.shape[-1]
+    if (B | T | V) >> 31:
+        raise ValueError(f"sizes {B}, {T}, {V}: a call carries sizes below 2^31")
     _seen(seen, B, V, on)
     if tokens.dtype is not torch.int64 or (T > 1 and tokens.stride(1) != 1):
         raise ValueError("tokens: expected int64 rows")
@@ -115,6 +117,8 @@ def apply_rules(logits: torch.Tensor, rules: LogitRules, seen: Optional[torch.Te
     if len(shape) != 2 or logits.dtype is not f32:
         raise ValueError("logits: expected f32 rows [B,V]")
     B, V = shape
+    if (B | V) >> 31:
+        raise ValueError(f"sizes {B}, {V}: a call carries sizes below 2^31")
     on, dense = logits.get_device(), logits.is_contiguous()
     if not dense and V > 1 and logits.stride(1) != 1:
         raise ValueError("logits: expected f32 rows [B,V]")

@@ -23,6 +23,10 @@ def _check(name: str, t: torch.Tensor, shape, dtype, device: int) -> None:
                          f"{tuple(t.shape)} on {t.device}")
 
 
+def _refuse_sizes(*sizes: int) -> None:
+    raise ValueError(f"sizes {sizes}: a call carries sizes below 2^31")
+
+
 def _prompts(counts: Optional[Sequence[int]], G: int, B: int):
     """The numbers of the prompts' sequences for the C ABI: None is all of one prompt."""
     if G == 1 and (counts is None or (len(counts) == 1 and counts[0] == B)):
@@ -58,6 +62,8 @@ def shared_prefix_attention(query: torch.Tensor, value: torch.Tensor, rho: torch
     rot = RotaryEmbedding.parse(rotary_embedding)
     Nq = 2 * N if rot == RotaryEmbedding.POPE else N
     d, S, G = value.shape[-1], keys.shape[-1], rho.shape[0]
+    if (B | h | T | Nq | d | S | G) >> 31:
+        _refuse_sizes(B, h, T, Nq, d, S, G)
     if rho.dtype not in _DTYPES:
         raise ValueError(f"rho is f32 or bf16, not {rho.dtype}")
     f32, int32 = torch.float32, torch.int32
@@ -98,6 +104,8 @@ def shared_prefix_fork(rho: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     B, h, Nq, S = keys.shape
     on = keys.get_device()
     G, d = rho.shape[0], rho.shape[-1]
+    if (B | h | Nq | S | G | d) >> 31:
+        _refuse_sizes(B, h, Nq, S, G, d)
     if rho.dtype not in _DTYPES:
         raise ValueError(f"rho is f32 or bf16, not {rho.dtype}")
     _check("rho", rho, (G, h, Nq, d), rho.dtype, on)

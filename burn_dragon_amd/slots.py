@@ -23,6 +23,8 @@ def copy_slots(buffers: Iterable[Tuple[torch.Tensor, torch.Tensor, int]], origin
         return
     dst, src, dim = buffers[0]
     dev, on, n, m = dst.device, dst.get_device(), dst.shape[dim], src.shape[dim]
+    if (n | m) >> 31:
+        raise ValueError(f"{n} and {m} slots: a call carries numbers below 2^31")
     table = (ffi.SlotBufferC * len(buffers))()
     for k, (dst, src, dim) in enumerate(buffers):
         shape, rank = dst.shape, dst.dim()
@@ -38,7 +40,10 @@ def copy_slots(buffers: Iterable[Tuple[torch.Tensor, torch.Tensor, int]], origin
             raise ValueError(f"buffer {k}: slots of {tuple(shape)} and {tuple(src.shape)} differ")
         row = table[k]
         row.dst, row.src = dst.data_ptr(), src.data_ptr()
-        row.outer, row.slot_bytes = math.prod(outer), math.prod(inner) * dst.element_size()
+        before = math.prod(outer)
+        if before >> 31:
+            raise ValueError(f"buffer {k}: {before} rows of slots before the slot dimension: a call carries numbers below 2^31")
+        row.outer, row.slot_bytes = before, math.prod(inner) * dst.element_size()
     if not torch.is_tensor(origin):
         origin = [int(o) for o in origin]
         bad = [o for o in origin if not KEEP <= o < m]

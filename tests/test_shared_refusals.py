@@ -116,3 +116,37 @@ def test_packed_masks_and_empty_counts():
         for v in range(96):
             assert (int(words[b, v // 32]) >> (v % 32)) & 1 == (int(mask[b, v]) if v < 70 else 0)
     assert not token_counts(2, 9, "cpu").any()
+
+
+def test_sizes_that_a_call_cannot_carry_are_refused():
+    """Sizes of 2^31 and more, of which a C entry point would see the low 32 bits and serve those; tensors without memory."""
+    big = 2**32 + 8
+
+    def empty(*shape, dtype=torch.float32):
+        return torch.empty(shape, dtype=dtype, device="meta")
+
+    def read(B=1, h=1, T=1, N=2, d=4, S=4, G=1):
+        return {"query": empty(B, h, T, N), "value": empty(B, T, d), "rho": empty(G, h, N, d), "keys": empty(B, h, N, S),
+                "values": empty(B, S, d), "lens": empty(B, dtype=torch.int32), "freqs": empty(N), "counts": [B]}
+
+    for size in ("B", "h", "T", "N", "d", "S"):
+        args = read(**{size: big})
+        with pytest.raises(ValueError, match="2\\^31"):
+            shared_prefix_attention(**args)
+        if size != "T":
+            with pytest.raises(ValueError, match="2\\^31"):
+                shared_prefix_fork(**{k: v for k, v in args.items() if k in ("rho", "keys", "values", "lens", "counts")})
+    with pytest.raises(ValueError, match="2\\^31"):  # N fits, the 2 N rows of PoPE do not
+        shared_prefix_attention(**read(N=2**30), rotary_embedding="pope")
+    u8 = torch.uint8
+    for dst, src, dim in [((big, 2), (big, 3), 1), ((2**16, 2**16, 2, 3), (2**16, 2**16, 2, 3), 2), ((big, 2), (4, 2), 0), ((4, 2), (big, 2), 0)]:
+        with pytest.raises(ValueError, match="2\\^31"):
+            copy_slots([(empty(*dst, dtype=u8), empty(*src, dtype=u8), dim)], [0] * min(dst[dim], 4))
+    for B, V in [(1, big), (big, 1)]:
+        seen = empty(B, V, dtype=torch.int32)
+        with pytest.raises(ValueError, match="2\\^31"):
+            apply_rules(empty(B, V), LogitRules(), seen)
+        with pytest.raises(ValueError, match="2\\^31"):
+            count_tokens(empty(B, 3, dtype=torch.int64), seen)
+    with pytest.raises(ValueError, match="2\\^31"):
+        count_tokens(empty(1, big, dtype=torch.int64), empty(1, 9, dtype=torch.int32))
