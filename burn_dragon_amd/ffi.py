@@ -6,6 +6,7 @@ built, or no HIP device is present, loading or context creation raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import sys
@@ -223,6 +224,17 @@ class Context:
         self._stream = stream or 0
         if pin:
             self._follow = False
+
+    def torch_stream(self):
+        """Torch's current stream while a wrapper fills or copies what its call reads: the stream of a context that keeps
+        one, so that the call comes after that work and what it allocated is not given to anyone before the call has read it.
+        (The caller orders its own tensors, and cannot order what is made inside a wrapper.)"""
+        if self._follow:
+            return contextlib.nullcontext()
+        import torch
+
+        return torch.cuda.stream(torch.cuda.ExternalStream(self._stream, device=self.device_id) if self._stream
+                                 else torch.cuda.default_stream(self.device_id))
 
     def set_option(self, name: str, value: int):
         self.check(self._lib.bdh_ctx_set_option(self.handle, name.encode(), int(value)))

@@ -185,6 +185,12 @@ def generate_samples(model: BDH, prompt_tokens: List[int], n: int, settings: Gen
         raise ValueError("at least one sample")
     if settings.max_new_tokens == 0:
         return [[] for _ in range(n)]
+    with model.ctx.torch_stream():
+        return _generate_samples(model, prompt_tokens, n, settings, rules, stop_token, capacity, generator)
+
+
+def _generate_samples(model: BDH, prompt_tokens: List[int], n: int, settings: GenerationSettings, rules: Optional[LogitRules],
+                      stop_token: Optional[int], capacity: int, generator: Optional[torch.Generator]) -> List[List[int]]:
     dev, V = model.device, model.vocab_size
     state, last = prefill_state(model, prompt_tokens)
     shared, own = model.share_state(state, [n], min(capacity, settings.max_new_tokens)), None

@@ -210,7 +210,8 @@ class BDH:
     def forward_shared(self, tokens: torch.Tensor, shared: SharedState, want_next: bool = False):
         """forward_with_state for sequences that share their prompts' states: tokens [B,T] int64 -> logits [B,T,V] (and the
         greedy next tokens, kept on the device, when want_next)."""
-        tokens = tokens.to(self.device, torch.int64).contiguous()
+        with self.ctx.torch_stream():
+            tokens = tokens.to(self.device, torch.int64).contiguous()
         B, T = tokens.shape
         if B != shared.batch:
             raise ValueError(f"{B} rows of tokens for {shared.batch} sequences")

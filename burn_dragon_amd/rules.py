@@ -82,12 +82,14 @@ def _row_stride(name: str, t: torch.Tensor, B: int, width: int, dtype, on: int) 
     return t.stride(0) if t.dim() == 2 and B > 1 else 0
 
 
-def _per_row(name: str, p: Union[float, torch.Tensor], B: int, like: torch.Tensor, on: int) -> torch.Tensor:
-    if not isinstance(p, torch.Tensor):
-        return torch.full((B,), float(p), device=like.device, dtype=torch.float32)
-    if p.shape != (B,) or p.dtype is not torch.float32 or p.get_device() != on or not p.is_contiguous():
+def _check_row(name: str, p: Union[float, torch.Tensor], B: int, like: torch.Tensor, on: int) -> None:
+    if isinstance(p, torch.Tensor) and (p.shape != (B,) or p.dtype is not torch.float32 or p.get_device() != on or not p.is_contiguous()):
         raise ValueError(f"{name}: expected f32 [{B}] on {like.device}")
-    return p
+
+
+def _row(p: float, B: int, like: torch.Tensor, ctx: ffi.Context) -> torch.Tensor:
+    with ctx.torch_stream():
+        return torch.full((B,), float(p), device=like.device, dtype=torch.float32)
 
 
 def count_tokens(tokens: torch.Tensor, seen: torch.Tensor, lens: Optional[torch.Tensor] = None, prompt: bool = False,
@@ -129,22 +131,15 @@ def apply_rules(logits: torch.Tensor, rules: LogitRules, seen: Optional[torch.Te
         raise ValueError("penalties need the counts of the tokens seen")
     else:
         seen_ptr = None
-    newest_ptr = None
-    if newest is not None:
-        if newest.dim() != 1:
-            newest = newest.reshape(-1)
-        if newest.shape != (B,) or newest.dtype is not torch.int64 or newest.get_device() != on:
-            raise ValueError(f"newest: expected int64 [{B}] on {logits.device}")
-        if not newest.is_contiguous():
-            newest = newest.contiguous()
-        newest_ptr = newest.data_ptr()
+    if newest is not None and (newest.numel() != B or newest.dtype is not torch.int64 or newest.get_device() != on):
+        raise ValueError(f"newest: expected int64 [{B}] on {logits.device}")
     repetition, presence, frequency = rules.repetition, rules.presence, rules.frequency
-    if repetition is not None:  # held until the call: a tensor made here has no other owner
-        repetition = _per_row("repetition", repetition, B, logits, on)
+    if repetition is not None:
+        _check_row("repetition", repetition, B, logits, on)
     if presence is not None:
-        presence = _per_row("presence", presence, B, logits, on)
+        _check_row("presence", presence, B, logits, on)
     if frequency is not None:
-        frequency = _per_row("frequency", frequency, B, logits, on)
+        _check_row("frequency", frequency, B, logits, on)
     bias, allowed = rules.bias, rules.allowed
     bias_stride = 0 if bias is None else _row_stride("bias", bias, B, V, f32, on)
     allowed_stride = 0 if allowed is None else _row_stride("allowed", allowed, B, (V + 31) // 32, torch.int32, on)
@@ -156,8 +151,18 @@ def apply_rules(logits: torch.Tensor, rules: LogitRules, seen: Optional[torch.Te
             raise ValueError(f"out: expected f32 rows [{B}, {V}] on {logits.device}")
         out_stride = out.stride(0) if B > 1 else V
     ctx = ffi.context_on(on, ctx)
+    if newest is not None and (newest.dim() != 1 or not newest.is_contiguous()):
+        with ctx.torch_stream():
+            newest = newest.reshape(-1).contiguous()
+    if repetition is not None and not isinstance(repetition, torch.Tensor):  # held until the call: a tensor made here has no other owner
+        repetition = _row(repetition, B, logits, ctx)
+    if presence is not None and not isinstance(presence, torch.Tensor):
+        presence = _row(presence, B, logits, ctx)
+    if frequency is not None and not isinstance(frequency, torch.Tensor):
+        frequency = _row(frequency, B, logits, ctx)
     ctx.check(ctx._lib.bdh_logit_rules(
-        ctx.handle, B, V, logits.data_ptr(), logits.stride(0) if B > 1 else V, seen_ptr, newest_ptr,
+        ctx.handle, B, V, logits.data_ptr(), logits.stride(0) if B > 1 else V, seen_ptr,
+        None if newest is None else newest.data_ptr(),
         None if repetition is None else repetition.data_ptr(), None if presence is None else presence.data_ptr(),
         None if frequency is None else frequency.data_ptr(), None if bias is None else bias.data_ptr(), bias_stride,
         None if allowed is None else allowed.data_ptr(), allowed_stride, out.data_ptr(), out_stride))

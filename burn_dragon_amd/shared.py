@@ -23,6 +23,11 @@ def _check(name: str, t: torch.Tensor, shape, dtype, device: int) -> None:
                          f"{tuple(t.shape)} on {t.device}")
 
 
+def _reshaped(t: torch.Tensor, shape, on: int, ctx: Optional[ffi.Context]) -> torch.Tensor:
+    with ffi.context_on(on, ctx).torch_stream():  # it may be a copy
+        return t.reshape(shape)
+
+
 def _refuse_sizes(*sizes: int) -> None:
     raise ValueError(f"sizes {sizes}: a call carries sizes below 2^31")
 
@@ -69,7 +74,7 @@ def shared_prefix_attention(query: torch.Tensor, value: torch.Tensor, rho: torch
     f32, int32 = torch.float32, torch.int32
     _check("query", query, (B, h, T, N), f32, on)
     if value.dim() != 3:
-        value = value.reshape(B, T, d)
+        value = _reshaped(value, (B, T, d), on, ctx)
     _check("value", value, (B, T, d), f32, on)
     _check("rho", rho, (G, h, Nq, d), rho.dtype, on)
     _check("keys", keys, (B, h, Nq, S), f32, on)
@@ -81,7 +86,7 @@ def shared_prefix_attention(query: torch.Tensor, value: torch.Tensor, rho: torch
         if freqs is None:
             raise ValueError(f"{rot.name} needs its frequencies")
         if freqs.dim() != 1:
-            freqs = freqs.reshape(-1)
+            freqs = _reshaped(freqs, (-1,), on, ctx)
         _check("freqs", freqs, (N,), f32, on)
     n_of = _prompts(counts, G, B)
     slopes = _slopes(alibi_slopes, h)

@@ -50,7 +50,8 @@ def copy_slots(buffers: Iterable[Tuple[torch.Tensor, torch.Tensor, int]], origin
         if bad or len(origin) != n:
             raise ValueError(f"origin: {len(origin)} entries for {n} slots, naming slots {bad} of {m}")
         ctx = ffi.context_on(on, ctx)
-        origin = torch.tensor(origin, dtype=torch.int32, device=dev)
+        with ctx.torch_stream():
+            origin = torch.tensor(origin, dtype=torch.int32, device=dev)
     if origin.shape != (n,) or origin.dtype != torch.int32 or origin.get_device() != on or not origin.is_contiguous():
         raise ValueError(f"origin: expected int32 [{n}] on {dev}, got {origin.dtype} {tuple(origin.shape)} on {origin.device}")
     ctx = ffi.context_on(on, ctx)
