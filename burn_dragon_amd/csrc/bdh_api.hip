@@ -34,6 +34,30 @@ int bdh_ws_reserve(bdh_ctx *ctx, size_t bytes) {
   return BDH_OK;
 }
 
+int bdh_ws_reserve_room(bdh_ctx *ctx, size_t bytes, size_t most) {
+  most = bdh_align_up(most, size_t(1) << 20);
+  if (most > ctx->ws_bytes && (ctx->ws_refused == 0 || most < ctx->ws_refused) &&
+      (ctx->opt_ws_max_mib == 0 || most <= (size_t)ctx->opt_ws_max_mib << 20)) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusActive;  // a call that is captured takes what is there, if it is enough
+    const bool known = hipStreamIsCapturing(ctx->stream, &status) == hipSuccess;
+    if (!known) (void)hipGetLastError();
+    void *larger = nullptr;
+    if (!known || status != hipStreamCaptureStatusNone) return bdh_ws_reserve(ctx, bytes);
+    if (hipMalloc(&larger, most) == hipSuccess) {
+      if (ctx->ws) {
+        BDH_HIP_CHECK(ctx, hipStreamSynchronize(ctx->stream));
+        BDH_HIP_CHECK(ctx, hipFree(ctx->ws));
+      }
+      ctx->ws = larger;
+      ctx->ws_bytes = most;
+    } else {
+      (void)hipGetLastError();
+      ctx->ws_refused = most;
+    }
+  }
+  return bdh_ws_reserve(ctx, bytes);
+}
+
 int bdh_stage_reserve(bdh_ctx *ctx, size_t bytes) {
   if (bytes <= ctx->stage_bytes) return BDH_OK;
   bytes = bdh_align_up(bytes, size_t(1) << 20);

@@ -18,6 +18,7 @@ struct bdh_ctx {
   // growable device workspace (partials, counters); owned by the context
   void *ws = nullptr;
   size_t ws_bytes = 0;
+  size_t ws_refused = 0;  // what bdh_ws_reserve_room last asked for in vain
   // a second growable buffer for inputs a launcher converts before it calls a path that sizes ctx->ws itself
   void *stage = nullptr;
   size_t stage_bytes = 0;
@@ -87,7 +88,11 @@ int bdh_launch_model_small(bdh_model *m, const int64_t *tokens, int B, void *rho
 
 // Grows ctx->ws to at least `bytes` (synchronises the stream before freeing the old one).
 int bdh_ws_reserve(bdh_ctx *ctx, size_t bytes);
-// The same for ctx->stage.
+// The same for a call that needs `bytes` now, and `most` at the most where it is repeated with other arguments of the same shape:
+// room for all of them is made at once, so that the workspace stays where it is (a captured graph may hold its address).  Where
+// there is no memory for `most`, what is needed now is enough, and so much is not asked for again.
+int bdh_ws_reserve_room(bdh_ctx *ctx, size_t bytes, size_t most);
+// The same as bdh_ws_reserve for ctx->stage.
 int bdh_stage_reserve(bdh_ctx *ctx, size_t bytes);
 
 #define BDH_HIP_CHECK(ctx, call)                                                        \

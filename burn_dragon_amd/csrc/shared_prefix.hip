@@ -1212,7 +1212,11 @@ int launch_dense(bdh_ctx *ctx, const SharedStepParams &p, const Prompts &pr, con
   const size_t parts_bytes = ps.ks > 1 ? bdh_align_up(one_s * ps.ks, 256) : 0;
   const size_t out_bytes = po.ks > 1 ? bdh_align_up(one_o * po.ks, 256) : 0;
   const size_t wide_bytes = p.rho_dtype == BDH_BF16 ? bdh_align_up(sizeof(float) * n_state, 256) : 0;
-  rc = bdh_ws_reserve(ctx, q_bytes + sc_bytes + parts_bytes + out_bytes + wide_bytes);
+  // room for the scores of every length that fits the capacity: ps deals K to at most one part for every 128 of it (and 32), and its
+  // parts are at most `most` bytes
+  const size_t one_room = sizeof(float) * (size_t)BH * T * S, part_room = (size_t)std::min(32, (Nq + 127) / 128);
+  const size_t room = bdh_align_up(one_room, 256) + bdh_align_up(std::max(one_room, std::min(part_room * one_room, most)), 256);
+  rc = bdh_ws_reserve_room(ctx, q_bytes + sc_bytes + parts_bytes + out_bytes + wide_bytes, q_bytes + room + out_bytes + wide_bytes);
   if (rc != BDH_OK) return rc;
   char *ws = static_cast<char *>(ctx->ws);
   float *q = alibi ? nullptr : reinterpret_cast<float *>(ws);
@@ -1335,7 +1339,12 @@ int bdh_launch_shared_steps(bdh_ctx *ctx, const SharedStepParams &p) {
   const size_t q_bytes = T == 1 || alibi ? 0 : bdh_align_up(sizeof(float) * (size_t)BH * T * Nq, 256);
   const size_t pt_bytes = bdh_align_up(sizeof(float) * (size_t)g.parts * BH * T * d, 256);
   const size_t sc_bytes = sizeof(float) * (size_t)g.score_parts_n * BH * T * g.span;
-  rc = bdh_ws_reserve(ctx, q_bytes + pt_bytes + sc_bytes);
+  // room for the scores of every length that fits the capacity: one token has a part a block of rows; of several, the parts times
+  // their blocks of columns are at most what `deal` has workgroups for, or one part of all columns
+  const long block_cols = 64L * g.cg, cols_most = (S + block_cols - 1) / block_cols;
+  const long places = T == 1 ? (long)g.row_blocks * S
+                             : block_cols * std::max(cols_most, std::min(slots / std::max<long>(1, BH * score_tiles), g.row_blocks * cols_most));
+  rc = bdh_ws_reserve_room(ctx, q_bytes + pt_bytes + sc_bytes, q_bytes + pt_bytes + sizeof(float) * (size_t)BH * T * (size_t)places);
   if (rc != BDH_OK) return rc;
   char *ws = static_cast<char *>(ctx->ws);
   g.partial = reinterpret_cast<float *>(ws + q_bytes);

@@ -578,7 +578,8 @@ int bdh_model_flush_layers(bdh_model *model, bdh_model_logs *logs, void *const *
  *   out [B,h,T,d] as in bdh_recurrent_attention; rho f32 or bf16 (eagerly decayed: bdh_alibi_materialize first).
  *   T = 1 stores a key only where it is not zero.
  *   longest: an upper bound of lens_dev that the host knows (keys past longest + T are not looked at by a call of many
- *   tokens), or -1 for capacity - T.  A sequence whose len is negative, above longest or beyond capacity - T gets NaN
+ *   tokens), or -1 for capacity - T.  The workspace of a call is that of its shape whatever longest is (where the memory for
+ *   that is not there, it grows with longest).  A sequence whose len is negative, above longest or beyond capacity - T gets NaN
  *   as its output, and nothing of it is stored.
  * bdh_shared_prefix_fork: rho_out [B,h,Nq,d] = a^len rho[g] + sum_{s < len} a^(len-s) k_s (x) v_s, of rho's type, rounded
  *   once: states of their own, as after the same tokens through bdh_recurrent_attention (f32 reassociation).  A len

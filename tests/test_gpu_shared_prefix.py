@@ -607,3 +607,34 @@ def test_the_largest_numbers_of_f32_in_a_fork(gpu, dtype):
     if dtype == BF16:
         bound = bound * (1 + 2.0**-8) + 2.0**-8 * np.abs(want)
     assert (np.abs(out.double().cpu().numpy() - want) <= bound).all()
+
+
+@pytest.mark.parametrize("counts,h,N,d,S,T", [((32,), 4, 256, 64, 2048, 1), ((20, 1, 3), 2, 512, 128, 2048, 1), ((2,), 4, 256, 64, 4096, 8),
+                                              ((3,), 2, 1030, 512, 2048, 5), ((3,), 4, 1024, 256, 2048, 20), ((1, 4), 4, 2048, 128, 1024, 30)])
+def test_the_workspace_does_not_grow_with_the_answers(gpu, counts, h, N, d, S, T):
+    """Calls of one shape on a context of their own, longest from 0 to what the capacity takes: after the first one the workspace
+    may not grow any more (a limit of 1 MiB refuses every growth), and what comes out is what a context without a past gives."""
+    ffi, _, shared = gpu
+    B = sum(counts)
+    gen = torch.Generator(DEV).manual_seed(6)
+    x = torch.randn((B, h, T, N), device=DEV, generator=gen).relu() * (torch.rand((B, h, T, N), device=DEV, generator=gen) < 0.05)
+    v, rho = torch.randn((B, T, d), device=DEV, generator=gen), torch.randn((len(counts), h, N, d), device=DEV, generator=gen)
+    keys, values = torch.zeros((B, h, N, S), device=DEV), torch.zeros((B, S, d), device=DEV)
+    lens = torch.zeros(B, dtype=torch.int32, device=DEV)
+
+    def call(ctx, longest):
+        return shared.shared_prefix_attention(x, v, rho, keys, values, lens, None, rotary_embedding="alibi", alibi_slopes=[0.1] * h,
+                                              counts=counts, longest=longest, ctx=ctx)
+
+    walker = ffi.Context(0)
+    call(walker, 0)
+    walker.set_option("workspace.max_mib", 1)
+    for longest in (0, 1, 60, 64, 200, S // 3, S // 2 + 1, S - T):
+        got = call(walker, longest)
+        fresh = ffi.Context(0)
+        assert torch.equal(got, call(fresh, longest)), longest
+        torch.cuda.synchronize()
+        fresh.close()
+    call(walker, None)
+    torch.cuda.synchronize()
+    walker.close()
