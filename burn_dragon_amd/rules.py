@@ -3,6 +3,7 @@ tokens that occurred, biases, and a mask of the tokens that a grammar allows.  T
 and a top_k only (src/generation.rs:26-72)."""
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 from typing import Optional, Union
 
@@ -25,8 +26,12 @@ class LogitRules:
     allowed: Optional[torch.Tensor] = None
 
     def __post_init__(self):
-        if self.repetition is not None and not torch.is_tensor(self.repetition) and not self.repetition > 0:
-            raise ValueError(f"repetition divides and multiplies logits: it is positive, not {self.repetition}")
+        r, p, f = self.repetition, self.presence, self.frequency
+        if r is not None and not isinstance(r, torch.Tensor) and not 2.0**-126 <= r < 2.0**128:
+            raise ValueError(f"repetition divides and multiplies logits: it is positive and finite in f32, not {r}")
+        if (p is not None and not isinstance(p, torch.Tensor) and not p > -math.inf) or \
+                (f is not None and not isinstance(f, torch.Tensor) and not f > -math.inf):
+            raise ValueError(f"a penalty is a number, or infinite where no token is said twice: presence {p}, frequency {f}")
 
     @property
     def penalises(self) -> bool:

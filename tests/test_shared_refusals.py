@@ -150,3 +150,16 @@ def test_sizes_that_a_call_cannot_carry_are_refused():
             count_tokens(empty(B, 3, dtype=torch.int64), seen)
     with pytest.raises(ValueError, match="2\\^31"):
         count_tokens(empty(1, big, dtype=torch.int64), empty(1, 9, dtype=torch.int32))
+
+
+def test_penalties_that_would_make_logits_nan():
+    """0 times an infinite repetition, 0 divided by one that f32 rounds to 0, and penalties that are no numbers."""
+    for r in (float("inf"), 1e39, 1e-46):
+        with pytest.raises(ValueError):
+            LogitRules(repetition=r)
+    for p in (float("nan"), float("-inf")):
+        with pytest.raises(ValueError):
+            LogitRules(presence=p)
+        with pytest.raises(ValueError):
+            LogitRules(frequency=p)
+    assert LogitRules(0.5, -1.0, float("inf")).penalises and LogitRules(3, 1, 0).penalises
