@@ -225,3 +225,65 @@ def test_positions_beyond_31_bits_are_refused(bda):
     for t in range(3):
         _close(decaying.forward_shared(torch.tensor([[t]]), shared), decaying.forward_with_state(torch.tensor([[t]]), own), 1e-3)
     assert shared.position == 2**31 + 8
+
+
+def _row_sets(n):
+    """Tokens of a vocabulary of 300 that row i may say, disjoint, and the stop token"""
+    sizes = [10, 25, 40, 55, 70, 12][:n]
+    ends = np.cumsum(sizes)
+    return [list(range(e - s, e)) for s, e in zip(sizes, ends)], 299
+
+
+def _row_rules(bda, sets, stop):
+    """Each row says its tokens once (a second time costs 1e6) and then, as its bias is lower than any logit, the stop token."""
+    from burn_dragon_amd.rules import pack_allowed
+
+    allowed = torch.zeros((len(sets), 300), dtype=torch.bool)
+    for row, tokens in enumerate(sets):
+        allowed[row, tokens] = allowed[row, stop] = True
+    bias = torch.zeros(300)
+    bias[stop] = -1e4
+    return bda.LogitRules(frequency=1e6, bias=bias.to(DEV), allowed=pack_allowed(allowed.to(DEV)))
+
+
+@pytest.mark.parametrize("rotary,lazy", [("rope", False), ("alibi", True)])
+@pytest.mark.parametrize("capacity", [20, 4, 96])
+@pytest.mark.parametrize("top_k", [1, None])
+def test_rows_stay_their_own_as_others_leave(bda, rotary, lazy, capacity, top_k):
+    """Six samples that may say disjoint sets of tokens, of six sizes: they leave the batch after 16, 32, 48, 64 and 80 draws, with
+    shared states (capacity 96), with states of their own (4) and with both (20).  Every sample says exactly its set and the stop
+    token; and walked again alone, with its own counts and its own variates, it draws the same tokens: greedy ones up to logits
+    that are within the bound of each other (2e-3 of the largest), drawn ones between the tokens of its variate moved by twice that
+    much either way (weights are then off by as much, relatively, and their sums too)."""
+    from burn_dragon_amd.generation import (GenerationSettings, generate_samples, prefill_state, sample_from_logits,
+                                            uniform_variates)
+
+    cfg = bda.BDHConfig(n_layer=2, n_embd=128, n_head=4, mlp_internal_dim_multiplier=8, vocab_size=300)
+    cfg.fused_kernels.set_rotary_embedding(rotary)
+    model = bda.BDH(cfg, DEV, seed=3, alibi_lazy=lazy)
+    sets, stop = _row_sets(6)
+    prompt = [7, 250, 31, 8]
+    settings = GenerationSettings(max_new_tokens=100, temperature=1.0, top_k=top_k)
+    got = generate_samples(model, prompt, 6, settings, _row_rules(bda, sets, stop), stop, capacity,
+                           torch.Generator().manual_seed(11))
+    for sample, tokens in zip(got, sets):
+        assert sample[-1] == stop and sorted(sample[:-1]) == tokens
+    source = torch.Generator().manual_seed(11)
+    variates = torch.cat([uniform_variates(96, DEV, source).reshape(16, 6) for _ in range(5)])
+    for row, sample in enumerate(got):
+        state, logits = prefill_state(model, prompt)
+        left = set(sets[row])
+        for step, token in enumerate(sample[:-1]):
+            slack = 1e-3 * logits.abs().max().item()
+            ruled = torch.full_like(logits, float("-inf"))
+            index = torch.tensor(sorted(left), device=DEV)
+            ruled[index] = logits[index]
+            if top_k == 1:
+                assert ruled[token] >= ruled.max() - 2 * slack
+            else:
+                u = variates[step, row]
+                at = [sample_from_logits(model, ruled[None], 1.0, None, (u + m).clamp(0, 1 - 2**-24)[None]).item()
+                      for m in (-4 * slack, 4 * slack)]
+                assert at[0] <= token <= at[1], (row, step)
+            left.remove(token)
+            logits = model.forward_with_state(torch.tensor([[token]]), state)[0, -1]
