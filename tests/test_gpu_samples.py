@@ -287,3 +287,27 @@ def test_rows_stay_their_own_as_others_leave(bda, rotary, lazy, capacity, top_k)
                 assert at[0] <= token <= at[1], (row, step)
             left.remove(token)
             logits = model.forward_with_state(torch.tensor([[token]]), state)[0, -1]
+
+
+@pytest.mark.parametrize("rotary,dtype,counts,T", [("rope", 0, [2, 1], 45), ("rope", 0, [2, 2], 20), ("alibi", 0, [4], 30),
+                                                   ("pope", 0, [1, 2], 45), ("rope", 1, [2, 2], 20), ("rope", 1, [1, 2], 45)])
+def test_a_follow_up_prompt_through_dense_products(bda, rotary, dtype, counts, T):
+    """So many tokens that their products are dense ones, with the LayerNorm that a model takes of them: 4 heads of 1024 rows (PoPE
+    2048) of 256 numbers, 2^20 multiplications a query; more than 32 queries a prompt and 2^25 multiplications, 2^27 where the
+    prompts' counts differ.  Then single tokens, another such call, and the fork, next to states of their own."""
+    model = _model(bda, rotary, dtype, d=256, mult=16)
+    assert model.latent == 1024 and sum(counts) * T > 32 * len(counts) and sum(counts) * T > (32 if len(set(counts)) == 1 else 128)
+    tol = 1e-3 if dtype == 0 else 2e-2
+    rng = np.random.default_rng(12)
+    B, owner = sum(counts), [g for g, n in enumerate(counts) for _ in range(n)]
+    prompts = torch.from_numpy(rng.integers(0, 69, (len(counts), 11)))
+    state, own = model.init_state(), model.init_state()
+    model.forward_with_state(prompts, state)
+    model.forward_with_state(prompts[owner], own)
+    shared = model.share_state(state, counts, 2 * T + 3)
+    for n in (T, 1, 1, T):
+        tokens = torch.from_numpy(rng.integers(0, 69, (B, n)))
+        logits, nxt = model.forward_shared(tokens, shared, want_next=True)
+        _close(logits, model.forward_with_state(tokens, own), tol)
+        assert torch.equal(nxt, logits[:, -1].argmax(-1))
+    _close(model.fork_shared(shared).storage.float(), own.storage.float(), tol)
