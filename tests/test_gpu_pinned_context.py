@@ -6,7 +6,7 @@ import torch
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
-WAIT = 200_000_000
+WAIT = 1_000_000_000  # cycles, 0.4 s: a call takes less than a millisecond
 
 
 @pytest.fixture(scope="module")
