@@ -14,7 +14,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libbdh_mi355x.so")
 SOURCES = ["bdh_api.hip", "state_step.hip", "state_deferred.hip", "projections.hip", "model.hip", "gemm_f32.hip", "attention_parallel.hip", "prefill.hip",
-           "sampling.hip", "viz_taps.hip", "shared_prefix.hip", "slots.hip", "logit_rules.hip", "model_small.hip", "model_phase.hip", "probe.hip"]
+           "sampling.hip", "viz_taps.hip", "shared_prefix.hip", "slots.hip", "logit_rules.hip", "packed.hip", "model_small.hip", "model_phase.hip", "probe.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [
     "--offload-arch=gfx950",

@@ -18,7 +18,7 @@ LIB_PATH = os.path.join(PKG, "libbdh_mi355x.so")
 
 OK, E_INVAL, E_SHAPE, E_ALIGN, E_HIP, E_NOMEM, E_UNSUPPORTED = 0, -1, -2, -3, -4, -5, -6
 ROPE, ALIBI, POPE = 0, 1, 2
-F32, BF16 = 0, 1
+F32, BF16, INT8 = 0, 1, 2
 PREFILL_STATE_IS_ZERO, PREFILL_STATE_HILO, PREFILL_ALL_SCORES, PREFILL_ROW_NORMALIZE = 1, 2, 4, 8
 
 # every symbol include/bdh_mi355x.h declares
@@ -36,6 +36,8 @@ EXPORTS = [
     "bdh_state_step_deferred", "bdh_state_flush", "bdh_model_forward_layers",
     "bdh_model_logs_create", "bdh_model_logs_destroy", "bdh_model_logs_pending", "bdh_model_forward_deferred",
     "bdh_model_flush", "bdh_model_forward_deferred_layers", "bdh_model_flush_layers",
+    "bdh_packed_bytes", "bdh_pack_weights", "bdh_packed_workspace", "bdh_packed_product", "bdh_packed_relu_lowrank",
+    "bdh_grouped_product",
 ]
 
 
@@ -61,6 +63,11 @@ class ModelWeightsC(ctypes.Structure):
 
 class SlotBufferC(ctypes.Structure):
     _fields_ = [("dst", c_void_p), ("src", c_void_p), ("slot_bytes", c_size_t), ("outer", c_int32)]
+
+
+class PackedWeightsC(ctypes.Structure):
+    _fields_ = [("type", c_int32), ("groups", c_int32), ("inner", c_int32), ("outer", c_int32), ("data", c_void_p),
+                ("scales", c_void_p)]
 
 
 MAX_SHARED_PROMPTS, MAX_SLOT_BUFFERS = 256, 8
@@ -150,6 +157,15 @@ def load_library(path: Optional[str] = None) -> ctypes.CDLL:
     lib.bdh_rotate.argtypes = [P, c_int, c_int, c_int, c_int, c_int, P, P, c_int64, P, P]
     lib.bdh_rho_energy.argtypes = [P, c_int, c_int, c_int, c_int, P, c_int, P, c_int64, P, P, P]
     lib.bdh_model_forward_viz.argtypes = [P, P, c_int, c_int, P, c_int, P, c_int64, P, P, P, P, P]
+    W = POINTER(PackedWeightsC)
+    lib.bdh_packed_bytes.restype = c_size_t
+    lib.bdh_packed_bytes.argtypes = [c_int, c_int, c_int, c_int]
+    lib.bdh_pack_weights.argtypes = [P, c_int, c_int, c_int, c_int, P, c_int, P, P]
+    lib.bdh_packed_workspace.restype = c_size_t
+    lib.bdh_packed_workspace.argtypes = [P, W, c_int64, c_int64, P, c_int, c_int64]
+    lib.bdh_packed_product.argtypes = [P, W, c_int64, P, c_int, c_int64, P, c_int, c_int64, P, c_size_t]
+    lib.bdh_packed_relu_lowrank.argtypes = [P, W, c_int, c_int, c_int, P, c_int, P, c_float, P, c_int, P, c_int, P, c_size_t]
+    lib.bdh_grouped_product.argtypes = [P, W, c_int64, P, P, c_int, c_int64, P, c_int, c_int64, P, c_size_t]
     for name in EXPORTS:
         fn = getattr(lib, name)
         if fn.restype is c_int and name not in ("bdh_version",):

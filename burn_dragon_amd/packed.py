@@ -1,0 +1,132 @@
+"""Projections through weights that are packed for the matrix cores (bdh_pack_weights, bdh_packed_product,
+bdh_grouped_product; the ReLU low-rank form is kernel.relu_lowrank.packed_forward): 8-bit integers with a scale for each
+output channel, the rows brought to 8-bit integers with a scale each on their way, or bf16.  The reference keeps its
+projections in f32 (src/model/bdh.rs:346-384, 446-449)."""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Sequence, Union
+
+import torch
+
+from . import ffi
+
+_ROWS = {torch.float32: ffi.F32, torch.bfloat16: ffi.BF16}
+_WEIGHTS = {torch.int8: ffi.INT8, torch.bfloat16: ffi.BF16}
+MOST_INNER, MOST_OUTER, MOST_GROUPS = 131072, 1 << 24, 65535
+
+
+class PackedWeights:
+    """weight [K,N] or [G,K,N] (f32 or bf16, on the device) as weights of G groups for rows of K values: dtype torch.int8 or
+    torch.bfloat16.  Laid out once; the tensor it was made from is not kept."""
+
+    def __init__(self, weight: torch.Tensor, dtype: torch.dtype = torch.int8, ctx: Optional[ffi.Context] = None):
+        if dtype not in _WEIGHTS:
+            raise ValueError(f"packed weights are int8 or bf16, not {dtype}")
+        if weight.dim() not in (2, 3) or weight.dtype not in _ROWS or not weight.is_contiguous():
+            raise ValueError(f"weight: expected a contiguous f32 or bf16 tensor [K,N] or [G,K,N], got {weight.dtype} {tuple(weight.shape)}")
+        self.groups, self.inner, self.outer = (1, *weight.shape) if weight.dim() == 2 else weight.shape
+        if not (0 < self.inner <= MOST_INNER and 0 < self.outer <= MOST_OUTER and self.groups <= MOST_GROUPS):
+            raise ValueError(f"weights [{self.groups}, {self.inner}, {self.outer}]: at most {MOST_GROUPS} groups of {MOST_INNER} x {MOST_OUTER}")
+        self.dtype, self.device, self.on = dtype, weight.device, weight.get_device()
+        ctx = ffi.context_on(self.on, ctx)
+        lib, kind = ctx._lib, _WEIGHTS[dtype]
+        with ctx.torch_stream():
+            self.data = torch.empty((lib.bdh_packed_bytes(kind, self.groups, self.inner, self.outer),), device=self.device, dtype=torch.uint8)
+            self.scales = torch.empty((self.groups, self.outer), device=self.device, dtype=torch.float32) if kind == ffi.INT8 else None
+        ctx.check(lib.bdh_pack_weights(ctx.handle, kind, self.groups, self.inner, self.outer, weight.data_ptr(), _ROWS[weight.dtype],
+                                       self.data.data_ptr(), ffi.ptr(self.scales)))
+        self._c = ffi.PackedWeightsC(kind, self.groups, self.inner, self.outer, self.data.data_ptr(), ffi.ptr(self.scales))
+        self._ref = ctypes.byref(self._c)
+
+    @property
+    def nbytes(self) -> int:
+        return self.data.numel() + (0 if self.scales is None else 4 * self.scales.numel())
+
+
+def _rows_type(name: str, t: torch.Tensor, on: int) -> int:
+    if t.dtype not in _ROWS or t.get_device() != on:
+        raise ValueError(f"{name}: expected f32 or bf16 on device {on}, got {t.dtype} on {t.device}")
+    return _ROWS[t.dtype]
+
+
+def _workspace(ctx: ffi.Context, weights: PackedWeights, rows: int, of_group: int, x: torch.Tensor, kind: int, stride: int):
+    """What the call needs beside its arguments, from torch's allocator: a captured call keeps its own."""
+    size = ctx._lib.bdh_packed_workspace(ctx.handle, weights._ref, rows, of_group, x.data_ptr(), kind, stride)
+    if size == 0:
+        return None, None, 0
+    with ctx.torch_stream():
+        held = torch.empty((size,), device=x.device, dtype=torch.uint8)
+    return held, held.data_ptr(), size
+
+
+def _as_rows(x: torch.Tensor, K: int, ctx: ffi.Context) -> torch.Tensor:
+    """x as [M,K] rows of neighbouring values."""
+    if x.dim() == 2 and (K == 1 or x.stride(1) == 1) and (x.shape[0] < 2 or x.stride(0) >= K):
+        return x
+    with ctx.torch_stream():  # it may be a copy
+        return x.reshape(-1, K).contiguous()
+
+
+def _call(name: str, x: torch.Tensor, weights: PackedWeights, offsets, out_dtype, out, ctx):
+    K, N, on = weights.inner, weights.outer, weights.on
+    kind = _rows_type("x", x, on)
+    if x.dim() < 1 or x.shape[-1] != K:
+        raise ValueError(f"x: expected rows of {K} values, got {tuple(x.shape)}")
+    ctx = ffi.context_on(on, ctx)
+    rows = _as_rows(x, K, ctx)
+    M = rows.shape[0]
+    if M >> 31:
+        raise ValueError(f"{M} rows: a call carries numbers below 2^31")
+    shape = (*x.shape[:-1], N)
+    if out is None:
+        if out_dtype not in _ROWS:
+            raise ValueError(f"out_dtype: f32 or bf16, not {out_dtype}")
+        with ctx.torch_stream():
+            out = torch.empty(shape, device=x.device, dtype=out_dtype)
+        out_stride = N
+    else:
+        _rows_type("out", out, on)
+        dense = out.is_contiguous()
+        if out.shape != shape or not (dense or (out.dim() == 2 and out.stride(1) == 1 and out.stride(0) >= N)):
+            raise ValueError(f"out: expected rows {shape}, got {tuple(out.shape)} with strides {out.stride()}")
+        out_stride = N if dense else out.stride(0)
+    stride = rows.stride(0) if M > 1 else K
+    held, workspace, size = _workspace(ctx, weights, M, M if offsets is None else -1, rows, kind, stride)
+    if offsets is None:
+        ctx.check(ctx._lib.bdh_packed_product(ctx.handle, weights._ref, M, rows.data_ptr(), kind, stride, out.data_ptr(), _ROWS[out.dtype],
+                                              out_stride, workspace, size))
+    else:
+        ctx.check(ctx._lib.bdh_grouped_product(ctx.handle, weights._ref, M, offsets.data_ptr(), rows.data_ptr(), kind, stride,
+                                               out.data_ptr(), _ROWS[out.dtype], out_stride, workspace, size))
+    return out
+
+
+def product(x: torch.Tensor, weights: PackedWeights, out_dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None,
+            ctx: Optional[ffi.Context] = None) -> torch.Tensor:
+    """x [..., K] (f32 or bf16) times weights of one group -> [..., N], a new tensor of out_dtype (f32 or bf16) or `out`."""
+    if weights.groups != 1:
+        raise ValueError(f"weights of {weights.groups} groups: a product takes one (grouped_product takes them all)")
+    return _call("product", x, weights, None, out_dtype, out, ctx)
+
+
+def grouped_product(x: torch.Tensor, weights: PackedWeights, offsets: Union[torch.Tensor, Sequence[int]],
+                    out_dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None,
+                    ctx: Optional[ffi.Context] = None) -> torch.Tensor:
+    """x [M,K] (f32 or bf16), rows sorted by the group of weights they meet: rows offsets[g] .. offsets[g+1] - 1 meet group g
+    -> [M,N], a new tensor of out_dtype or `out`, in which rows of no group are left as they are (uninitialised in a new one).
+    offsets: G + 1 numbers that do not decrease; a list is checked here, an int32 tensor on the device is not (what decreases or
+    leaves 0 .. M counts as the running maximum within 0 .. M)."""
+    G = weights.groups
+    if x.dim() != 2:
+        raise ValueError(f"x: expected rows [M, {weights.inner}], got {tuple(x.shape)}")
+    if not torch.is_tensor(offsets):
+        offsets = [int(o) for o in offsets]
+        if len(offsets) != G + 1 or offsets[0] < 0 or offsets[-1] > x.shape[0] or any(a > b for a, b in zip(offsets, offsets[1:])):
+            raise ValueError(f"offsets: {len(offsets)} numbers for {G} groups of {x.shape[0]} rows that start at 0 or later and do not decrease")
+        _rows_type("x", x, weights.on)
+        with ffi.context_on(weights.on, ctx).torch_stream():
+            offsets = torch.tensor(offsets, dtype=torch.int32, device=x.device)
+    if offsets.shape != (G + 1,) or offsets.dtype is not torch.int32 or offsets.get_device() != weights.on or not offsets.is_contiguous():
+        raise ValueError(f"offsets: expected int32 [{G + 1}] on {weights.device}, got {offsets.dtype} {tuple(offsets.shape)} on {offsets.device}")
+    return _call("grouped_product", x, weights, offsets, out_dtype, out, ctx)

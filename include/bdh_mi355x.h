@@ -60,6 +60,8 @@ enum bdh_rotary { BDH_ROPE = 0, BDH_ALIBI = 1, BDH_POPE = 2 };
 /* storage type of the recurrent state rho.  The reference keeps it in f32; bf16 storage
  * with f32 accumulation is an extension of this library. */
 enum bdh_dtype { BDH_F32 = 0, BDH_BF16 = 1 };
+/* the other type of packed weights (BDH_BF16 is one as well) */
+enum bdh_packed_type { BDH_INT8 = 2 };
 
 /* ---- library / context ------------------------------------------------------------ */
 const char *bdh_version(void);
@@ -661,6 +663,52 @@ int bdh_logit_rules(bdh_ctx *ctx, int B, int V, const float *logits, int64_t row
                     int64_t out_stride);
 int bdh_count_tokens(bdh_ctx *ctx, int B, int T, int V, const int64_t *tokens, int64_t row_stride,
                      const int32_t *lens_dev, int prompt, int32_t *seen);
+
+/* ---- projections through packed weights ----------------------------------------------- */
+/*
+ * Weights [groups, inner, outer] laid out once for the matrix cores, in 8-bit integers with a scale for each output channel
+ * or in bf16, and the products of rows with them.  The reference has no such form; its projections are those of
+ * src/model/bdh.rs:346-350, 370-384 and 446-449.
+ *   BDH_INT8  a row x_m of largest magnitude a has the scale s_m = a / 127 and the whole numbers q_mk = rint(x_mk * (127 / a)),
+ *             each operation rounded to f32; channel n of the weights t_n and p_kn by the same rule along k.  Then
+ *             out_mn = (sum_k q_mk p_kn) s_m t_n; the sums are exact.  A row or channel with a < 2^-118 counts as zeros; one that
+ *             holds an infinity or a NaN gives NaN.
+ *   BDH_BF16  out_mn = sum_k bf16(x_mk) bf16(w_kn), sums in f32.  Finite values stay finite when they are rounded.
+ * bdh_packed_bytes: the size of `data` for these weights (0 for sizes that are refused); scales: float [groups, outer], for
+ *   BDH_INT8 only.  inner at most 131072, outer at most 2^24, at most 65535 groups.
+ * bdh_pack_weights: weight [groups, inner, outer] (BDH_F32 or BDH_BF16) into data (on 16 bytes) and scales.
+ * bdh_packed_product: x [rows, inner] -> out [rows, outer] with weights of one group.
+ * bdh_packed_relu_lowrank: bdh_relu_lowrank through packed weights of h = groups heads: in [B,h_in,T,inner], h_in = 1 or h,
+ *   bias [h,outer] or NULL, gate [B,h,T,outer] or NULL, out [B,h,T,outer] = gate * relu(in . weight + bias - threshold); a sum
+ *   that is NaN is not above the threshold.
+ * bdh_grouped_product: rows sorted by the weights they meet: rows offsets_dev[g] .. offsets_dev[g + 1] - 1 of x meet group g
+ *   (int32 [groups + 1] on the device; a group may be empty).  Rows before the first and behind the last offset are left as they
+ *   are in out.  Offsets that decrease or leave 0 .. rows count as their running maximum within 0 .. rows.
+ * x, in, gate and out are BDH_F32 or BDH_BF16 each, strides in values; an f32 result is rounded once where out is BDH_BF16.  out
+ * overlaps nothing that is read.  The workspace is the caller's, bdh_packed_workspace bytes of it (0: none; on 16 bytes) for the
+ * same weights, rows and place of the rows: rows_in = the rows of x or in, rows_of_group = rows that meet each group (B * T of
+ * bdh_packed_relu_lowrank), -1 for bdh_grouped_product.  Nothing is copied to or from the host, no result depends on the order of
+ * atomics, and a call in a HIP graph uses the workspace it was captured with.
+ */
+typedef struct bdh_packed_weights {
+  int32_t type, groups, inner, outer;
+  const void *data;
+  const float *scales;
+} bdh_packed_weights;
+size_t bdh_packed_bytes(int type, int groups, int inner, int outer);
+int bdh_pack_weights(bdh_ctx *ctx, int type, int groups, int inner, int outer, const void *weight, int weight_dtype,
+                     void *data, float *scales);
+size_t bdh_packed_workspace(const bdh_ctx *ctx, const bdh_packed_weights *weights, int64_t rows_in, int64_t rows_of_group,
+                            const void *x, int x_dtype, int64_t x_stride);
+int bdh_packed_product(bdh_ctx *ctx, const bdh_packed_weights *weights, int64_t rows, const void *x, int x_dtype,
+                       int64_t x_stride, void *out, int out_dtype, int64_t out_stride, void *workspace,
+                       size_t workspace_bytes);
+int bdh_packed_relu_lowrank(bdh_ctx *ctx, const bdh_packed_weights *weights, int B, int h_in, int T, const void *in,
+                            int in_dtype, const float *bias, float threshold, const void *gate, int gate_dtype, void *out,
+                            int out_dtype, void *workspace, size_t workspace_bytes);
+int bdh_grouped_product(bdh_ctx *ctx, const bdh_packed_weights *weights, int64_t rows, const int32_t *offsets_dev,
+                        const void *x, int x_dtype, int64_t x_stride, void *out, int out_dtype, int64_t out_stride,
+                        void *workspace, size_t workspace_bytes);
 
 /* Draws the next token of every sequence on the device.  Replaces the temperature division of
  * sample_next_token (src/generation.rs:117) and sample_from_logits_values (src/generation.rs:26-72),

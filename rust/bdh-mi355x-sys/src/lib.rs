@@ -46,6 +46,17 @@ pub struct bdh_slot_buffer {
     pub outer: i32,
 }
 
+/// weights of `bdh_packed_product` and its kin: [groups, inner, outer]
+#[repr(C)]
+pub struct bdh_packed_weights {
+    pub r#type: i32,
+    pub groups: i32,
+    pub inner: i32,
+    pub outer: i32,
+    pub data: *const c_void,
+    pub scales: *const f32,
+}
+
 pub const BDH_OK: c_int = 0;
 pub const BDH_E_INVAL: c_int = -1;
 pub const BDH_E_SHAPE: c_int = -2;
@@ -62,6 +73,9 @@ pub const BDH_POPE: c_int = 2;
 /// storage type of the recurrent state
 pub const BDH_F32: c_int = 0;
 pub const BDH_BF16: c_int = 1;
+
+/// the other type of packed weights
+pub const BDH_INT8: c_int = 2;
 
 /// flags of bdh_prefill_chunked
 pub const BDH_PREFILL_STATE_IS_ZERO: c_int = 1;
@@ -211,6 +225,20 @@ extern "C" {
         bias_stride: i64, allowed: *const i32, allowed_stride: i64, out: *mut f32, out_stride: i64) -> c_int;
     pub fn bdh_count_tokens(ctx: *mut bdh_ctx, b: c_int, t: c_int, v: c_int, tokens: *const i64, row_stride: i64,
         lens_dev: *const i32, prompt: c_int, seen: *mut i32) -> c_int;
+    pub fn bdh_packed_bytes(r#type: c_int, groups: c_int, inner: c_int, outer: c_int) -> usize;
+    pub fn bdh_pack_weights(ctx: *mut bdh_ctx, r#type: c_int, groups: c_int, inner: c_int, outer: c_int,
+        weight: *const c_void, weight_dtype: c_int, data: *mut c_void, scales: *mut f32) -> c_int;
+    pub fn bdh_packed_workspace(ctx: *const bdh_ctx, weights: *const bdh_packed_weights, rows_in: i64, rows_of_group: i64,
+        x: *const c_void, x_dtype: c_int, x_stride: i64) -> usize;
+    pub fn bdh_packed_product(ctx: *mut bdh_ctx, weights: *const bdh_packed_weights, rows: i64, x: *const c_void,
+        x_dtype: c_int, x_stride: i64, out: *mut c_void, out_dtype: c_int, out_stride: i64, workspace: *mut c_void,
+        workspace_bytes: usize) -> c_int;
+    pub fn bdh_packed_relu_lowrank(ctx: *mut bdh_ctx, weights: *const bdh_packed_weights, b: c_int, h_in: c_int, t: c_int,
+        input: *const c_void, in_dtype: c_int, bias: *const f32, threshold: f32, gate: *const c_void, gate_dtype: c_int,
+        out: *mut c_void, out_dtype: c_int, workspace: *mut c_void, workspace_bytes: usize) -> c_int;
+    pub fn bdh_grouped_product(ctx: *mut bdh_ctx, weights: *const bdh_packed_weights, rows: i64, offsets_dev: *const i32,
+        x: *const c_void, x_dtype: c_int, x_stride: i64, out: *mut c_void, out_dtype: c_int, out_stride: i64,
+        workspace: *mut c_void, workspace_bytes: usize) -> c_int;
     pub fn bdh_sample_top_k(ctx: *mut bdh_ctx, b: c_int, v: c_int, logits: *const f32, row_stride: i64,
         temperature: f32, top_k: c_int, uniforms: *const f32, next_tokens: *mut i64) -> c_int;
     pub fn bdh_probe_chunks(ctx: *mut bdh_ctx, region: *mut c_void, region_bytes: usize,
