@@ -17,6 +17,7 @@
 #include "lds_copy.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -52,6 +53,13 @@ __device__ __forceinline__ unsigned int whole(float x, float up) {
 __device__ __forceinline__ unsigned int to_bf16(float x) {
   const unsigned int r = bdh_bf16_rne(x);
   return (r & 0x7fffu) == 0x7f80u && (__float_as_uint(x) & 0x7fffffffu) < 0x7f800000u ? r - 1 : r;
+}
+
+// The same without the clamp (results are not brought back into range), two at a time.
+__device__ __forceinline__ unsigned int half2(float a, float b) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(unsigned int, __builtin_convertvector((f32x2){a, b}, bf16x2));
 }
 
 // ---- weights ------------------------------------------------------------------------------------
@@ -120,14 +128,15 @@ struct RowsIn {
   long rows, stride;
 };
 
-// 16 neighbouring values of a row from k on; what lies past the end is 0.
-__device__ __forceinline__ void load16(const RowsIn &in, long row, int k, float (&v)[16]) {
+// PER (8 or 16) neighbouring values of a row from k on; what lies past the end is 0.
+template <int PER>
+__device__ __forceinline__ void load_values(const RowsIn &in, long row, int k, float (&v)[PER]) {
   const long at = row * in.stride + k;
-  if (k + 16 <= in.K) {
+  if (k + PER <= in.K) {
     if (in.dtype == BDH_F32) {
       const float *p = static_cast<const float *>(in.x) + at;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < PER / 4; ++j) {
         const f32x4 t = *reinterpret_cast<const f32x4u *>(p + 4 * j);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[4 * j + e] = t[e];
@@ -135,7 +144,7 @@ __device__ __forceinline__ void load16(const RowsIn &in, long row, int k, float 
     } else {
       const unsigned short *p = static_cast<const unsigned short *>(in.x) + at;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < PER / 8; ++j) {
         const u32x4u t = *reinterpret_cast<const u32x4u *>(p + 8 * j);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -146,44 +155,43 @@ __device__ __forceinline__ void load16(const RowsIn &in, long row, int k, float 
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) v[e] = k + e < in.K ? load_value(in.x, in.dtype, at + e) : 0.0f;
+    for (int e = 0; e < PER; ++e) v[e] = k + e < in.K ? load_value(in.x, in.dtype, at + e) : 0.0f;
   }
 }
-__device__ __forceinline__ unsigned int top_of(const float (&v)[16], unsigned int top) {
+template <int PER>
+__device__ __forceinline__ unsigned int top_of(const float (&v)[PER], unsigned int top) {
 #pragma unroll
-  for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+  for (int e = 0; e < PER; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
   return top;
 }
-__device__ __forceinline__ uint4 whole16(const float (&v)[16], float up) {
+// The 16 bytes that 16 values make in 8 bits, or 8 in bf16.
+template <int TYPE, int PER>
+__device__ __forceinline__ uint4 packed16(const float (&v)[PER], float up) {
   unsigned int w[4] = {0, 0, 0, 0};
 #pragma unroll
-  for (int e = 0; e < 16; ++e) w[e >> 2] |= whole(v[e], up) << (8 * (e & 3));
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-__device__ __forceinline__ uint4 half8(const float (&v)[16], int from) {
-  unsigned int w[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) w[e] = to_bf16(v[from + 2 * e]) | to_bf16(v[from + 2 * e + 1]) << 16;
+  for (int e = 0; e < PER; ++e) {
+    if (TYPE == BDH_INT8) w[e >> 2] |= whole(v[e], up) << (8 * (e & 3));
+    else w[e >> 1] |= to_bf16(v[e]) << (16 * (e & 1));
+  }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Rows as the product takes them: [rows][Kb * 64 bytes], zeros behind K, and the scales of 8-bit rows.  THR threads a row, 16
-// values a thread at a time; 8-bit rows are read twice, the second time from a cache.
+// Rows as the product takes them: [rows][Kb * 64 bytes], zeros behind K, and the scales of 8-bit rows.  THR threads a row, 16 bytes
+// a thread at a time; 8-bit rows are read twice, the second time from a cache.
 template <int TYPE, int THR>
 __global__ __launch_bounds__(THR < 256 ? 256 : THR) void k_prepare_rows(RowsIn in, int Kb, uint4 *__restrict__ q, float *__restrict__ scales) {
-  constexpr int ROWS = THR < 256 ? 256 / THR : 1;
+  constexpr int ROWS = THR < 256 ? 256 / THR : 1, PER = TYPE == BDH_INT8 ? 16 : 8;
   __shared__ unsigned int s_top[THR < 256 ? 4 : THR / 64];
   const long row = (long)blockIdx.x * ROWS + threadIdx.x / THR;
   const int t = threadIdx.x % THR, padded = Kb * (TYPE == BDH_INT8 ? 64 : 32);
   const bool live = row < in.rows;
-  float v[16];
-  float scale = 1.0f, up = 1.0f;
+  float v[PER], scale = 1.0f, up = 1.0f;
   if (TYPE == BDH_INT8) {
     unsigned int top = 0;
     if (live)
-      for (int k = t * 16; k < in.K; k += THR * 16) {
-        load16(in, row, k, v);
-        top = top_of(v, top);
+      for (int k = t * PER; k < in.K; k += THR * PER) {
+        load_values<PER>(in, row, k, v);
+        top = top_of<PER>(v, top);
       }
     for (int o = 32; o > 0; o >>= 1) top = max(top, (unsigned int)__shfl_xor((int)top, o));
     if (THR > 64) {
@@ -197,19 +205,9 @@ __global__ __launch_bounds__(THR < 256 ? 256 : THR) void k_prepare_rows(RowsIn i
   }
   if (!live) return;
   uint4 *out = q + row * Kb * 4;
-  for (int k = t * 16; k < padded; k += THR * 16) {
-    if (k < in.K) {
-      load16(in, row, k, v);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) v[e] = 0.0f;
-    }
-    if (TYPE == BDH_INT8) {
-      out[k >> 4] = whole16(v, up);
-    } else {
-      out[k >> 3] = half8(v, 0);
-      out[(k >> 3) + 1] = half8(v, 8);
-    }
+  for (int k = t * PER; k < padded; k += THR * PER) {
+    load_values<PER>(in, row, min(k, in.K), v);
+    out[k / PER] = packed16<TYPE>(v, up);
   }
 }
 
@@ -236,24 +234,28 @@ struct Product {
   int out_dtype;
   long out_stride;
   int m_tiles, n_tiles;  // of a head, or of all groups
+  // k cut into `splits` parts of kb_each blocks: sums of part i at parts[i][row of out][Nb * 64], each 32 bits
+  int splits, kb_each;
+  void *parts;
+  long rows_out;
 };
 
-// The rows [first, last) of group g are those between the running maximum of the offsets up to g and up to g + 1, both within
-// 0 .. rows: groups never overlap, whatever the offsets hold.  Tile number `tile` of the groups' tiles of BM rows; false: there are
-// fewer.  Uniform over the wavefront, which looks at 64 groups at a time.
-__device__ __forceinline__ bool find_tile(const int32_t *offsets, int G, long rows, int BM, int tile, int &group, long &first, long &last) {
+// The rows [first, last) of tile number `tile` of the groups' tiles of BM rows, the tile's first row and the end of its group's; false:
+// there are fewer tiles.  Group g has the rows between the running maximum of the offsets up to g and up to g + 1, both within
+// 0 .. rows: groups never overlap, whatever the offsets hold, and there are at most rows / BM + G tiles.  Every wavefront finds its
+// tile by itself, 64 groups at a time: a table made by a launch before cost as much as it saved.
+__device__ __forceinline__ bool find_tile(const int32_t *__restrict__ offsets, int G, int rows, int BM, int tile, int &group, long &first,
+                                          long &last) {
   const int lane = threadIdx.x & 63;
-  long reached = min(max((long)offsets[0], 0L), rows);  // the running maximum so far
-  int before = 0;                                       // tiles of the groups so far
+  int reached = min(max(offsets[0], 0), rows), before = 0;  // the running maximum and the number of tiles so far
   for (int g0 = 0; g0 < G; g0 += 64) {
-    long end = g0 + lane < G ? min(max((long)offsets[g0 + lane + 1], 0L), rows) : 0;
-    end = max(end, reached);
+    int end = max(g0 + lane < G ? min(max(offsets[g0 + lane + 1], 0), rows) : 0, reached);
     for (int o = 1; o < 64; o <<= 1) {
-      const long other = __shfl_up(end, o);
+      const int other = __shfl_up(end, o);
       if (lane >= o) end = max(end, other);
     }
-    const long below = __shfl_up(end, 1), start = lane == 0 ? reached : below;
-    int tiles = (int)((end - start + BM - 1) / BM);
+    const int below = __shfl_up(end, 1), start = lane == 0 ? reached : below;
+    const int tiles = (int)(((unsigned int)(end - start) + BM - 1) / BM);
     int sum = tiles;
     for (int o = 1; o < 64; o <<= 1) {
       const int other = __shfl_up(sum, o);
@@ -262,14 +264,13 @@ __device__ __forceinline__ bool find_tile(const int32_t *offsets, int G, long ro
     const unsigned long long has = __ballot(before + sum > tile);
     if (has) {
       const int l = __builtin_ctzll(has);
-      group = __builtin_amdgcn_readfirstlane(g0 + l);
-      const long s = __shfl(start, l), e = __shfl(end, l);
-      first = s + (long)(tile - (before + __shfl(sum - tiles, l))) * BM;
-      last = e;
+      group = g0 + l;
+      first = __builtin_amdgcn_readlane(start, l) + (long)(tile - before - __builtin_amdgcn_readlane(sum - tiles, l)) * BM;
+      last = __builtin_amdgcn_readlane(end, l);
       return true;
     }
-    before += __shfl(sum, 63);
-    reached = __shfl(end, 63);
+    before += __builtin_amdgcn_readlane(sum, 63);
+    reached = __builtin_amdgcn_readlane(end, 63);
   }
   return false;
 }
@@ -291,61 +292,165 @@ struct Acc<BDH_BF16> {
 
 // sum s t, the smaller scale first: what is in between neither leaves the range of f32 where the result does not, nor is subnormal.
 __device__ __forceinline__ float scaled(float sum, float s, float t) { return sum * (t < s ? t : s) * (t < s ? s : t); }
+// Where the scales are like these, (sum s) t does as well, for half the operations.
+__device__ __forceinline__ bool plain_scale(float s) { return s == 0.0f || (s > 0x1p-60f && s < 0x1p60f); }
 
-// 8 neighbouring channels of a row from n on: scales, bias, threshold, gate, and the one rounding where out is bf16.
-template <int TYPE>
-__device__ __forceinline__ void finish8(const Product &g, int group, long out_row, int n, const typename Acc<TYPE>::type &lo,
-                                        const typename Acc<TYPE>::type &hi, float row_scale) {
-  float v[8];
-  const int left = g.N - n;
-  const long c0 = (long)group * g.N + n, at = out_row * g.out_stride + n;
+// What comes behind the sums: nothing but the scales; ReLU alone; bias, threshold, ReLU and gate as they are given; nothing, where
+// the sums are parts of a longer k.
+enum Behind { kScales, kRelu, kAll, kParts };
+
+// What a lane needs of the 8 neighbouring channels n .. that it holds of every row; channels past the end repeat the last one.
+template <int TYPE, int BEHIND>
+struct Channels {
+  int n, left;  // left <= 0: none of them exists
+  float scale[8], bias[8];
+  __device__ __forceinline__ Channels(const Product &g, int group, int first) : n(first), left(g.N - first) {
+    const long c0 = (long)group * g.N;
+    if (TYPE == BDH_INT8) values(g.scales + c0, scale);
+    if (BEHIND == kAll) {
+      if (g.bias) {
+        values(g.bias + c0, bias);
+      } else {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    v[e] = (float)(e < 4 ? lo[e] : hi[e - 4]);
-    if (e < left) {
-      if (TYPE == BDH_INT8) v[e] = scaled(v[e], row_scale, g.scales[c0 + e]);
-      if (g.bias) v[e] += g.bias[c0 + e];
-      if (g.relu) {
-        v[e] -= g.threshold;
-        v[e] = v[e] > 0.0f ? v[e] : 0.0f;  // a NaN is not above the threshold
-        if (g.gate) v[e] *= load_value(g.gate, g.gate_dtype, at + e);
+        for (int e = 0; e < 8; ++e) bias[e] = 0.0f;
       }
     }
   }
+  __device__ __forceinline__ void values(const float *p, float (&v)[8]) const {
+    if (left >= 8) {
+      const f32x4 a = *reinterpret_cast<const f32x4u *>(p + n), b = *reinterpret_cast<const f32x4u *>(p + n + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = p[min(n + e, n + left - 1 < 0 ? 0 : n + left - 1)];
+    }
+  }
+  __device__ __forceinline__ bool plain() const {
+    bool all = true;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) all = all && plain_scale(scale[e]);
+    return all;
+  }
+};
+
+__device__ __forceinline__ void load8(const void *p, int dtype, long at, float (&v)[8]) {
+  if (dtype == BDH_F32) {
+    const f32x4u *f = reinterpret_cast<const f32x4u *>(static_cast<const float *>(p) + at);
+    const f32x4 a = f[0], b = f[1];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
+  } else {
+    const u32x4u t = *reinterpret_cast<const u32x4u *>(static_cast<const unsigned short *>(p) + at);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[2 * e] = __uint_as_float(t[e] << 16);
+      v[2 * e + 1] = __uint_as_float(t[e] & 0xffff0000u);
+    }
+  }
+}
+// Results are stored with the streaming hint where every row starts on 16 bytes: they are written once and, where they are many,
+// gone from the caches before anyone reads them (1554 rows of 4 heads of 8192 in f32, gated, 122 -> 91 us; 8191 rows of 2816 in
+// bf16 47 -> 43).  Rows that start anywhere share their lines' ends: there the hint costs (192 rows of 65601 33 -> 59 us).
+template <bool PAST, typename V>
+__device__ __forceinline__ void store(V v, void *p) {
+  if (PAST) __builtin_nontemporal_store(v, static_cast<V *>(p));
+  else *static_cast<V *>(p) = v;
+}
+
+// 8 neighbouring channels of a row, whose first value is number `at` of out (and gate): scales, bias, threshold, gate, and the one
+// rounding where out is bf16.  plain: plain_scale holds for all of them (uniform over the wavefront).  A large output counts by the
+// operations here: each one a value costs 5 us where 1500 rows of 131072 are written in 100.
+template <int TYPE, int BEHIND, bool PAST>
+__device__ __forceinline__ void finish8(const Product &g, const Channels<TYPE, BEHIND> &c, long at, const typename Acc<TYPE>::type &lo,
+                                        const typename Acc<TYPE>::type &hi, float row_scale, bool plain) {
+  if (c.left <= 0) return;
+  float v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = (float)(e < 4 ? lo[e] : hi[e - 4]);
+  if (TYPE == BDH_INT8) {
+    if (plain) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = v[e] * row_scale * c.scale[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = scaled(v[e], row_scale, c.scale[e]);
+    }
+  }
+  if (BEHIND == kAll) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = v[e] + c.bias[e] - g.threshold;
+  }
+  if (BEHIND != kScales) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = fmaxf(v[e], 0.0f);  // 0 for a NaN: it is not above the threshold
+  }
+  if (BEHIND == kAll && g.gate) {
+    float m[8];
+    if (c.left >= 8) {
+      load8(g.gate, g.gate_dtype, at, m);
+    } else {
+      for (int e = 0; e < 8; ++e) m[e] = load_value(g.gate, g.gate_dtype, at + min(e, c.left - 1));
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] *= m[e];
+  }
   if (g.out_dtype == BDH_F32) {
     float *o = static_cast<float *>(g.out) + at;
-    if (left >= 8) {
-      *reinterpret_cast<f32x4u *>(o) = f32x4u{v[0], v[1], v[2], v[3]};
-      *reinterpret_cast<f32x4u *>(o + 4) = f32x4u{v[4], v[5], v[6], v[7]};
+    if (c.left >= 8) {
+      store<PAST>(f32x4u{v[0], v[1], v[2], v[3]}, o);
+      store<PAST>(f32x4u{v[4], v[5], v[6], v[7]}, o + 4);
     } else {
-      for (int e = 0; e < left; ++e) o[e] = v[e];
+      for (int e = 0; e < c.left; ++e) o[e] = v[e];
     }
   } else {
+    unsigned int w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = half2(v[2 * e], v[2 * e + 1]);
     unsigned short *o = static_cast<unsigned short *>(g.out) + at;
-    if (left >= 8) {
-      *reinterpret_cast<u32x4u *>(o) = u32x4u{bdh_bf16_rne(v[0]) | bdh_bf16_rne(v[1]) << 16, bdh_bf16_rne(v[2]) | bdh_bf16_rne(v[3]) << 16,
-                                              bdh_bf16_rne(v[4]) | bdh_bf16_rne(v[5]) << 16, bdh_bf16_rne(v[6]) | bdh_bf16_rne(v[7]) << 16};
+    if (c.left >= 8) {
+      store<PAST>(u32x4u{w[0], w[1], w[2], w[3]}, o);
     } else {
-      for (int e = 0; e < left; ++e) o[e] = (unsigned short)bdh_bf16_rne(v[e]);
+      for (int e = 0; e < c.left; ++e) o[e] = (unsigned short)(w[e >> 1] >> (16 * (e & 1)));
     }
   }
 }
 
-// A tile of BM rows x BN channels, WM x WN wavefronts.  Blocks of 64 bytes of k come through a ring of NS stages in LDS, copied
-// past the registers and waited for by count.
-template <int TYPE, int BM, int BN, int WM, int WN, int NS>
-__global__ __launch_bounds__(64 * WM * WN) void k_packed_tile(Product g) {
-  constexpr int W = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, CB = BN / 16, RB = BM / 16, COPIES = (CB + RB) / W;
-  static_assert((CB + RB) % W == 0 && TN % 2 == 0 && BN % 64 == 0);
-  __shared__ __attribute__((aligned(1024))) unsigned char s_ring[NS][(CB + RB) * 1024];
+// Which tile a workgroup takes: workgroups go to the eight XCDs in turn, so XCD i gets every eighth; it takes the i-th eighth of
+// the tiles, which go through the channels by panels of kPanel tiles of rows, so that what an XCD works on at a time shares its
+// rows and weights in the XCD's L2.
+constexpr unsigned int kPanel = 4;
+__device__ __forceinline__ void place_of(const Product &g, int &m_tile, int &n_tile, int &split) {
+  const unsigned int total = gridDim.x, xcd = blockIdx.x & 7, each = total >> 3, rest = total & 7;
+  unsigned int tile = xcd * each + min(xcd, rest) + (blockIdx.x >> 3);
+  const unsigned int tiles = total / g.splits, m_tiles = tiles / g.n_tiles;
+  split = tile / tiles;  // an XCD works on one part of k at a time
+  tile -= split * tiles;
+  const unsigned int panel = tile / (kPanel * g.n_tiles), at = tile - panel * kPanel * g.n_tiles;
+  const unsigned int wide = min(kPanel, m_tiles - panel * kPanel);
+  n_tile = at / wide;
+  m_tile = panel * kPanel + (at - n_tile * wide);
+}
+
+// A tile of BM rows x BN channels, WM x WN wavefronts.  The weights of 64 bytes of k come through a ring of three stages in LDS,
+// the rows' 128 bytes of k (whole lines of memory: half lines cost up to a fifth) through one of two; both are copied past the
+// registers and waited for by count.  A copy takes 128 bytes of 8 rows; piece p of row r lies at place p ^ (r & 7), so that the
+// reads of a fragment, rows 128 bytes apart, meet no bank twice.
+constexpr int tile_lds(int BM, int BN) { return (3 * BN / 16 + 2 * BM / 8) * 1024; }
+constexpr int tiles_a_cu(int BM, int BN) { return 160 * 1024 / tile_lds(BM, BN); }
+template <int TYPE, int BEHIND, bool PAST, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, tiles_a_cu(BM, BN) * WM * WN / 4) void k_packed_tile(Product g) {
+  constexpr int W = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, CB = BN / 16, RB = BM / 8, CW = CB / W, CR = RB / W;
+  static_assert(CB % W == 0 && RB % W == 0 && TN % 2 == 0 && BN % 64 == 0);
+  __shared__ __attribute__((aligned(1024))) unsigned char s_w[3][CB * 1024], s_r[2][RB * 1024];
   typedef typename Acc<TYPE>::type acc_t;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % WM, wn = wave / WM;
-  const int n_tile = blockIdx.x % g.n_tiles, m_tile = blockIdx.x / g.n_tiles;
-  int group = 0;
+  int m_tile, n_tile, split, group = 0;
+  place_of(g, m_tile, n_tile, split);
   long first, last;
   if (g.offsets) {
-    if (!find_tile(g.offsets, g.G, g.rows, BM, m_tile, group, first, last)) return;
+    if (!find_tile(g.offsets, g.G, (int)g.rows, BM, m_tile, group, first, last)) return;
   } else {
     group = m_tile / g.m_tiles;
     first = (long)(m_tile - group * g.m_tiles) * BM;
@@ -355,26 +460,29 @@ __global__ __launch_bounds__(64 * WM * WN) void k_packed_tile(Product g) {
     if (g.offsets || g.h_in == 1) return r;
     return (r / g.T * g.h_in + group) * g.T + r % g.T;
   };
-  const unsigned char *src[COPIES];
-  int step[COPIES];
+  const unsigned char *from_w[CW], *from_r[CR];
 #pragma unroll
-  for (int c = 0; c < COPIES; ++c) {
-    const int piece = wave + c * W;
-    if (piece < CB) {
-      const int nb = min(n_tile * (BN / 64) + piece / 4, g.Nb - 1);
-      src[c] = g.w + (((long)group * g.Nb + nb) * g.Kb * 4 + piece % 4) * 1024 + lane * 16;
-      step[c] = 4096;
-    } else {
-      const long r = min(first + (piece - CB) * 16 + (lane & 15), last - 1);
-      src[c] = g.q + row_in(r) * g.pitch + (lane >> 4) * 16;
-      step[c] = 64;
-    }
+  for (int c = 0; c < CW; ++c) {
+    const int piece = wave + c * W, nb = min(n_tile * (BN / 64) + piece / 4, g.Nb - 1);
+    from_w[c] = g.w + ((((long)group * g.Nb + nb) * g.Kb + split * g.kb_each) * 4 + piece % 4) * 1024 + lane * 16;
   }
-  auto issue = [&](int stage) {
 #pragma unroll
-    for (int c = 0; c < COPIES; ++c) {
-      bdh_copy_to_lds(src[c], &s_ring[stage][(wave + c * W) * 1024]);
-      src[c] += step[c];
+  for (int c = 0; c < CR; ++c) {
+    const long r = min(first + (wave + c * W) * 8 + (lane >> 3), last - 1);
+    from_r[c] = g.q + row_in(r) * g.pitch + split * g.kb_each * 64 + ((lane & 7) ^ (lane >> 3)) * 16;
+  }
+  auto copy_w = [&](int stage) {
+#pragma unroll
+    for (int c = 0; c < CW; ++c) {
+      bdh_copy_to_lds(from_w[c], &s_w[stage][(wave + c * W) * 1024]);
+      from_w[c] += 4096;
+    }
+  };
+  auto copy_r = [&](int stage) {
+#pragma unroll
+    for (int c = 0; c < CR; ++c) {
+      bdh_copy_to_lds(from_r[c], &s_r[stage][(wave + c * W) * 1024]);
+      from_r[c] += 128;
     }
   };
   acc_t acc[TM][TN];
@@ -382,45 +490,240 @@ __global__ __launch_bounds__(64 * WM * WN) void k_packed_tile(Product g) {
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = acc_t{};
-  const int n = g.Kb;
-  for (int s = 0; s < NS - 1; ++s)
-    if (s < n) issue(s);
-  int stage = 0, ahead = NS - 1;
-  for (int kb = 0; kb < n; ++kb) {
-    bdh_wait_for_stage<COPIES, NS - 2>(n - 1 - kb);
-    asm volatile("s_barrier" ::: "memory");  // every wave's copies of this stage are there, and its reads of the one before are done
-    if (kb + NS - 1 < n) issue(ahead);
+  // where a lane finds its 16 bytes of row block 0 of the first 64 bytes of k; those of the second lie at ^ 64
+  const int at_r = (lane & 15) * 128 + ((lane >> 4) ^ (lane & 7)) * 16;
+  const int n = min(g.kb_each, g.Kb - split * g.kb_each);  // even
+  copy_w(0);
+  copy_r(0);
+  copy_w(1);
+  int stage = 0, ahead = 2;
+  auto step = [&](int half, int rows) {
     i32x4 fw[TN], fr[TM];
 #pragma unroll
-    for (int j = 0; j < TN; ++j) fw[j] = *reinterpret_cast<const i32x4 *>(&s_ring[stage][(wn * TN + j) * 1024 + lane * 16]);
+    for (int j = 0; j < TN; ++j) fw[j] = *reinterpret_cast<const i32x4 *>(&s_w[stage][(wn * TN + j) * 1024 + lane * 16]);
 #pragma unroll
-    for (int i = 0; i < TM; ++i) fr[i] = *reinterpret_cast<const i32x4 *>(&s_ring[stage][(CB + wm * TM + i) * 1024 + lane * 16]);
+    for (int i = 0; i < TM; ++i)
+      fr[i] = *reinterpret_cast<const i32x4 *>(&s_r[rows][(wm * TM + i) * 2048 + (half ? at_r ^ 64 : at_r)]);
 #pragma unroll
     for (int j = 0; j < TN; ++j)
 #pragma unroll
       for (int i = 0; i < TM; ++i) acc[i][j] = Acc<TYPE>::mac(fw[j], fr[i], acc[i][j]);
-    stage = stage + 1 == NS ? 0 : stage + 1;
-    ahead = ahead + 1 == NS ? 0 : ahead + 1;
+    stage = stage == 2 ? 0 : stage + 1;
+    ahead = ahead == 2 ? 0 : ahead + 1;
+  };
+  for (int kb = 0, rows = 0; kb < n; kb += 2, rows ^= 1) {
+    const bool more = kb + 2 < n;
+    bdh_wait_for_stage<CW, 1>(1);  // issued after what this half needs: the weights of the other half
+    asm volatile("s_barrier" ::: "memory");  // every wave's copies are there, and its reads of what is overwritten now are done
+    if (more) {
+      copy_w(ahead);
+      copy_r(rows ^ 1);
+    }
+    step(0, rows);
+    bdh_wait_for_stage<CW + CR, 1>(more ? 1 : 0);  // issued after what this half needs: the next rows and half
+    asm volatile("s_barrier" ::: "memory");
+    if (more) copy_w(ahead);
+    step(1, rows);
   }
+  long at[TM];
+  float row_scale[TM];
+  bool plain = true;
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
-    const long r = first + (wm * TM + i) * 16 + (lane & 15);
-    if (r >= last) continue;
-    const long out_row = g.offsets ? r : (r / g.T * g.G + group) * g.T + r % g.T;
-    const float row_scale = TYPE == BDH_INT8 ? g.row_scales[row_in(r)] : 1.0f;
-#pragma unroll
-    for (int j = 0; j < TN; j += 2) {
-      const int channel = n_tile * BN + (wn * TN + j) * 16 + 8 * (lane >> 4);
-      if (channel < g.N) finish8<TYPE>(g, group, out_row, channel, acc[i][j], acc[i][j + 1], row_scale);
-    }
+    const long r = min(first + (wm * TM + i) * 16 + (lane & 15), last - 1);
+    at[i] = (g.offsets || g.G == 1 ? r : (r / g.T * g.G + group) * g.T + r % g.T) * (BEHIND == kParts ? g.Nb * 64L : g.out_stride);
+    if (BEHIND == kParts) continue;
+    row_scale[i] = TYPE == BDH_INT8 ? g.row_scales[row_in(r)] : 1.0f;
+    plain = plain && plain_scale(row_scale[i]);
   }
+  if (BEHIND == kParts) {
+    acc_t *out = reinterpret_cast<acc_t *>(static_cast<char *>(g.parts) + 4 * split * g.rows_out * g.Nb * 64);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int channel = n_tile * BN + (wn * TN + (j & ~1)) * 16 + 8 * (lane >> 4) + 4 * (j & 1);
+      if (channel >= g.Nb * 64) continue;
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+        if (first + (wm * TM + i) * 16 + (lane & 15) < last) out[(at[i] + channel) >> 2] = acc[i][j];
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < TN; j += 2) {
+    const Channels<TYPE, BEHIND> c(g, group, n_tile * BN + (wn * TN + j) * 16 + 8 * (lane >> 4));
+    const bool simple = TYPE != BDH_INT8 || __ballot(plain && c.plain()) == ~0ull;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+      if (first + (wm * TM + i) * 16 + (lane & 15) < last)
+        finish8<TYPE, BEHIND, PAST>(g, c, at[i] + c.n, acc[i][j], acc[i][j + 1], row_scale[i], simple);
+  }
+}
+
+// Few rows meet many weights: the weights are streamed, past LDS, and the rows are brought to 8 bits (or bf16) on their way.  A
+// workgroup takes 64 channels of a group, its W wavefronts every W-th block of k; 16 * MT rows at a time.  All that a wavefront has
+// of k, up to U blocks of weights and rows, is asked for at once, and the largest magnitude of a row is a maximum over the
+// wavefronts in LDS; the wavefronts' sums are added up in LDS in their order.  PRE: the rows are prepared ones, for k so long that a row's
+// largest magnitude is looked for by a launch of its own and k is cut into parts.
+template <int TYPE, int BEHIND, int MT, int W, bool PRE>
+__global__ __launch_bounds__(64 * W) void k_packed_few(Product g, RowsIn in) {
+  constexpr int U = MT == 1 ? 4 : MT == 2 ? 2 : 1, PER = TYPE == BDH_INT8 ? 16 : 8, LD = 68;
+  typedef typename Acc<TYPE>::type acc_t;
+  __shared__ unsigned int s_top[16 * MT];
+  __shared__ __attribute__((aligned(16))) int s_sum[W][16 * MT][LD];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int nb = blockIdx.x % g.Nb, rest = blockIdx.x / g.Nb, group = rest % g.G, split = rest / g.G;
+  long first = 0, last = g.rows;
+  if (g.offsets) {  // the running maximum of the offsets up to the group's first and last row
+    int a = 0, b = 0;
+    for (int i = lane; i <= group + 1; i += 64) {
+      const int o = min(max(g.offsets[i], 0), (int)g.rows);
+      b = max(b, o);
+      if (i <= group) a = max(a, o);
+    }
+    for (int o = 32; o > 0; o >>= 1) {
+      a = max(a, __shfl_xor(a, o));
+      b = max(b, __shfl_xor(b, o));
+    }
+    first = __builtin_amdgcn_readfirstlane(a);
+    last = __builtin_amdgcn_readfirstlane(b);
+  }
+  auto row_in = [&](long r) {
+    if (g.offsets || g.h_in == 1) return r;
+    return (r / g.T * g.h_in + group) * g.T + r % g.T;
+  };
+  const int kb0 = split * g.kb_each, kb1 = min(kb0 + g.kb_each, g.Kb);
+  const i32x4 *w = reinterpret_cast<const i32x4 *>(g.w) + ((long)group * g.Nb + nb) * g.Kb * 256 + lane;
+  for (; first < last; first += 16 * MT) {
+    long row[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) row[i] = row_in(min(first + i * 16 + (lane & 15), last - 1));
+    i32x4 fw[U][4], fr[U][MT];
+    float v[PRE ? 1 : U][PRE ? 1 : MT][PER];
+    auto ask = [&](int b, int u) {  // block b of the weights and rows
+#pragma unroll
+      for (int j = 0; j < 4; ++j) fw[u][j] = w[(long)b * 256 + j * 64];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        if constexpr (PRE) fr[u][i] = *reinterpret_cast<const i32x4 *>(g.q + row[i] * g.pitch + b * 64 + (lane >> 4) * 16);
+        else load_values<PER>(in, row[i], (b * 4 + (lane >> 4)) * PER, v[u][i]);
+      }
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (kb0 + wave + u * W < kb1) ask(kb0 + wave + u * W, u);
+    float up[MT];
+    if constexpr (TYPE == BDH_INT8 && !PRE) {
+      if (threadIdx.x < 16 * MT) s_top[threadIdx.x] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        unsigned int top = 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (kb0 + wave + u * W < kb1) top = top_of<PER>(v[u][i], top);
+        for (int kb = kb0 + wave + U * W; kb < kb1; kb += W) {
+          float more[PER];
+          load_values<PER>(in, row[i], (kb * 4 + (lane >> 4)) * PER, more);
+          top = top_of<PER>(more, top);
+        }
+        top = max(top, (unsigned int)__shfl_xor((int)top, 16));
+        top = max(top, (unsigned int)__shfl_xor((int)top, 32));
+        if (lane < 16) atomicMax(&s_top[i * 16 + lane], top);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        float scale;
+        scale_of(s_top[i * 16 + (lane & 15)], scale, up[i]);
+      }
+    }
+    acc_t acc[MT][4];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = acc_t{};
+    for (int kb = kb0 + wave; kb < kb1; kb += U * W) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (kb + u * W < kb1) {
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            i32x4 r;
+            if constexpr (PRE) r = fr[u][i];
+            else r = __builtin_bit_cast(i32x4, packed16<TYPE>(v[u][i], up[i]));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = Acc<TYPE>::mac(fw[u][j], r, acc[i][j]);
+          }
+        }
+        if (kb + (u + U) * W < kb1) ask(kb + (u + U) * W, u);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<acc_t *>(&s_sum[wave][i * 16 + (lane & 15)][32 * (j >> 1) + 8 * (lane >> 4) + 4 * (j & 1)]) = acc[i][j];
+    __syncthreads();
+    for (int t = threadIdx.x; t < 16 * MT * 8; t += 64 * W) {
+      const int r = t >> 3, c8 = (t & 7) * 8;
+      if (first + r >= last) break;
+      acc_t lo = acc_t{}, hi = acc_t{};
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        lo += *reinterpret_cast<const acc_t *>(&s_sum[k][r][c8]);
+        hi += *reinterpret_cast<const acc_t *>(&s_sum[k][r][c8 + 4]);
+      }
+      const long q = first + r, out_row = g.offsets || g.G == 1 ? q : (q / g.T * g.G + group) * g.T + q % g.T;
+      if constexpr (BEHIND == kParts) {
+        acc_t *out = reinterpret_cast<acc_t *>(static_cast<char *>(g.parts) + 4 * ((split * g.rows_out + out_row) * g.Nb + nb) * 64);
+        out[c8 / 4] = lo;
+        out[c8 / 4 + 1] = hi;
+      } else {
+        float scale = 1.0f, unused;
+        if constexpr (TYPE == BDH_INT8) {
+          if constexpr (PRE) scale = g.row_scales[row_in(q)];
+          else scale_of(s_top[r], scale, unused);
+        }
+        const Channels<TYPE, BEHIND> c(g, group, nb * 64 + c8);
+        finish8<TYPE, BEHIND, false>(g, c, out_row * g.out_stride + c.n, lo, hi, scale, false);
+      }
+    }
+    if (first + 16 * MT < last) __syncthreads();
+  }
+}
+
+// The sums of the parts of k, and what comes behind them: 8 channels of a row a thread.
+template <int TYPE, int BEHIND>
+__global__ __launch_bounds__(256) void k_packed_finish(Product g) {
+  typedef typename Acc<TYPE>::type acc_t;
+  const int eighths = (g.N + 7) / 8;
+  const long t = (long)blockIdx.x * 256 + threadIdx.x, row = t / eighths;
+  if (row >= g.rows_out) return;
+  const int n = (int)(t - row * eighths) * 8;
+  const long part = g.rows_out * g.Nb * 16;
+  const acc_t *p = static_cast<const acc_t *>(g.parts) + (row * g.Nb * 64 + n) / 4;
+  acc_t lo = acc_t{}, hi = acc_t{};
+  int i = 0;
+  for (; i + 8 <= g.splits; i += 8) {  // eight parts on their way at a time
+    acc_t a[8], b[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) a[u] = p[(i + u) * part], b[u] = p[(i + u) * part + 1];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) lo += a[u], hi += b[u];
+  }
+  for (; i < g.splits; ++i) lo += p[i * part], hi += p[i * part + 1];
+  const int group = (int)(row / g.T % g.G);
+  const long row_in = g.h_in == 1 ? row / ((long)g.T * g.G) * g.T + row % g.T : row;
+  const Channels<TYPE, BEHIND> c(g, group, n);
+  finish8<TYPE, BEHIND, false>(g, c, row * g.out_stride + n, lo, hi, TYPE == BDH_INT8 ? g.row_scales[row_in] : 1.0f, false);
 }
 
 // ---- host ---------------------------------------------------------------------------------------
 
 constexpr int kMostGroups = 65535;
 
-int blocks_of_k(int type, long K) { return (int)((K * (type == BDH_INT8 ? 1 : 2) + 63) / 64); }
+// blocks of 64 bytes, an even number of them: rows are copied by 128 bytes
+int blocks_of_k(int type, long K) { return (int)((K * (type == BDH_INT8 ? 1 : 2) + 127) / 128 * 2); }
 
 int check_weights(bdh_ctx *ctx, const bdh_packed_weights *w) {
   if (!w) return bdh_fail(ctx, BDH_E_INVAL, "null weights");
@@ -438,12 +741,67 @@ size_t value_bytes(int dtype) { return dtype == BDH_F32 ? 4 : 2; }
 
 // Whether the product can read the rows where they are.
 bool rows_as_they_are(int type, int K, const void *x, int x_dtype, int64_t x_stride) {
-  return type == BDH_BF16 && x_dtype == BDH_BF16 && K % 32 == 0 && x_stride % 8 == 0 && bdh_aligned(x, 16);
+  return type == BDH_BF16 && x_dtype == BDH_BF16 && K % 64 == 0 && x_stride % 8 == 0 && bdh_aligned(x, 16);
 }
 
-size_t workspace_of(int type, int K, int64_t rows, const void *x, int x_dtype, int64_t x_stride) {
-  if (rows_as_they_are(type, K, x, x_dtype, x_stride)) return 0;
-  return (size_t)rows * blocks_of_k(type, K) * 64 + bdh_align_up(sizeof(float) * (size_t)rows, 64);
+// How a call is done.
+struct Plan {
+  bool few;       // the weights are streamed by k_packed_few, for 16 * mt rows at a time by `waves` wavefronts
+  int mt, waves;
+  int bm, bn;     // else tiles
+  bool prepared, direct;  // the rows are prepared by a launch of their own; the product reads them where they are
+  int splits, kb_each;
+  size_t scales, parts, bytes;  // where in the workspace the prepared rows' scales and the parts' sums lie, and its size
+};
+
+Plan plan_of(const bdh_ctx *ctx, const bdh_packed_weights &w, int64_t rows_in, int64_t rows_of_group, const void *x, int x_dtype,
+             int64_t x_stride) {
+  Plan p{};
+  const bool grouped = rows_of_group < 0;
+  p.direct = rows_as_they_are(w.type, w.inner, x, x_dtype, x_stride);
+  const int64_t rows = grouped ? rows_in : rows_of_group;
+  const int Kb = blocks_of_k(w.type, w.inner);
+  const int64_t Nb = (w.outer + 63) / 64, blocks = Nb * w.groups;
+  p.splits = 1;
+  p.kb_each = Kb;
+  p.few = rows <= 64;
+  if (p.few) {
+    const int64_t a_group = grouped ? (rows + std::max(w.groups, 1) - 1) / std::max(w.groups, 1) : rows;
+    p.mt = a_group <= 16 ? 1 : a_group <= 32 ? 2 : 4;
+    p.waves = p.mt < 4 && blocks < ctx->n_cu && Kb > 8 ? 8 : 4;
+    if (!grouped && Kb > 16 * p.waves && blocks < ctx->n_cu) {  // fewer workgroups than CUs, and more of k than they have on their way
+      const int64_t most = (Kb + p.waves - 1) / p.waves, want = (2 * ctx->n_cu + blocks - 1) / blocks;
+      p.waves = 4;
+      p.kb_each = (int)((Kb + std::min(most, want) - 1) / std::min(most, want) + 7) / 8 * 8;
+      p.splits = (Kb + p.kb_each - 1) / p.kb_each;
+      p.prepared = !p.direct;
+    }
+  } else {
+    p.prepared = !p.direct;
+    const int64_t heads = grouped ? 1 : w.groups;
+    auto tiles = [&](int bm, int bn) { return (rows + bm - 1) / bm * heads * ((w.outer + bn - 1) / bn); };
+    if (tiles(128, 256) >= 2 * ctx->n_cu) p.bm = 128, p.bn = 256;
+    else if (tiles(64, 128) >= 2 * ctx->n_cu) p.bm = 64, p.bn = 128;
+    else p.bm = 64, p.bn = 64;
+    if (!grouped && tiles(64, 64) < 2 * ctx->n_cu && Kb >= 32) {
+      if (tiles(128, 256) * (Kb / 16) >= 2 * ctx->n_cu) p.bm = 128, p.bn = 256;
+      const int64_t each = p.bm == 128 ? 2 : 5, want = (each * ctx->n_cu) / tiles(p.bm, p.bn), most = Kb / 16;
+      const int64_t splits = std::max<int64_t>(1, std::min(want, most));
+      p.kb_each = (int)((Kb + splits - 1) / splits + 1) / 2 * 2;
+      p.splits = (Kb + p.kb_each - 1) / p.kb_each;
+    }
+  }
+  size_t at = 0;
+  if (p.prepared) {
+    p.scales = (size_t)rows_in * Kb * 64;
+    at = p.scales + bdh_align_up(sizeof(float) * (size_t)rows_in, 64);
+  }
+  if (p.splits > 1) {
+    p.parts = at;
+    at += (size_t)p.splits * rows * w.groups * Nb * 256;
+  }
+  p.bytes = at;
+  return p;
 }
 
 template <int TYPE>
@@ -458,14 +816,47 @@ int launch_prepare(bdh_ctx *ctx, const RowsIn &in, int Kb, uint4 *q, float *scal
   return BDH_OK;
 }
 
-template <int TYPE, int BM, int BN, int WM, int WN, int NS>
+// What comes behind the sums of a product, as the kernels' parameter.
+template <typename F>
+void with_behind(const Product &p, F launch) {
+  if (!p.relu) launch(std::integral_constant<int, kScales>{});
+  else if (!p.bias && !p.gate && p.threshold == 0.0f) launch(std::integral_constant<int, kRelu>{});
+  else launch(std::integral_constant<int, kAll>{});
+}
+
+template <int TYPE, int BM, int BN, int WM, int WN>
 int launch_tiles(bdh_ctx *ctx, Product p) {
   p.n_tiles = (p.N + BN - 1) / BN;
-  const long per_head = (p.rows + BM - 1) / BM, tiles = p.offsets ? per_head + p.G : per_head * p.G;
-  if (tiles * p.n_tiles > 0x7fffffffL) return bdh_fail(ctx, BDH_E_SHAPE, "%ld tiles: the call is too large", tiles * p.n_tiles);
-  p.m_tiles = (int)(p.offsets ? tiles : per_head);
-  hipLaunchKernelGGL((k_packed_tile<TYPE, BM, BN, WM, WN, NS>), dim3((unsigned)(tiles * p.n_tiles)), dim3(64 * WM * WN), 0, ctx->stream, p);
+  const long per_head = (p.rows + BM - 1) / BM, tiles = (p.offsets ? per_head + p.G : per_head * p.G) * p.n_tiles * p.splits;
+  if (tiles > 0x7fffffffL) return bdh_fail(ctx, BDH_E_SHAPE, "%ld tiles: the call is too large", tiles);
+  p.m_tiles = (int)per_head;
+  const dim3 grid((unsigned)tiles), threads(64 * WM * WN);
+  const bool past = bdh_aligned(p.out, 16) && p.out_stride * value_bytes(p.out_dtype) % 16 == 0;
+  if (p.splits > 1)
+    hipLaunchKernelGGL((k_packed_tile<TYPE, kParts, false, BM, BN, WM, WN>), grid, threads, 0, ctx->stream, p);
+  else
+    with_behind(p, [&](auto behind) {
+      constexpr int BEHIND = decltype(behind)::value;
+      if (past) hipLaunchKernelGGL((k_packed_tile<TYPE, BEHIND, true, BM, BN, WM, WN>), grid, threads, 0, ctx->stream, p);
+      else hipLaunchKernelGGL((k_packed_tile<TYPE, BEHIND, false, BM, BN, WM, WN>), grid, threads, 0, ctx->stream, p);
+    });
   BDH_LAUNCH_CHECK(ctx, "k_packed_tile");
+  return BDH_OK;
+}
+
+template <int TYPE, int MT, int W, bool PRE>
+int launch_few(bdh_ctx *ctx, const Product &p, const RowsIn &in) {
+  const long blocks = (long)p.Nb * p.G * p.splits;
+  if (blocks > 0x7fffffffL) return bdh_fail(ctx, BDH_E_SHAPE, "%ld workgroups: the call is too large", blocks);
+  const dim3 grid((unsigned)blocks), threads(64 * W);
+  if (p.splits > 1) {
+    if constexpr (PRE && W == 4) hipLaunchKernelGGL((k_packed_few<TYPE, kParts, MT, W, true>), grid, threads, 0, ctx->stream, p, in);
+  } else if constexpr (!PRE || TYPE == BDH_BF16) {
+    with_behind(p, [&](auto behind) {
+      hipLaunchKernelGGL((k_packed_few<TYPE, decltype(behind)::value, MT, W, PRE>), grid, threads, 0, ctx->stream, p, in);
+    });
+  }
+  BDH_LAUNCH_CHECK(ctx, "k_packed_few");
   return BDH_OK;
 }
 
@@ -480,7 +871,7 @@ struct Call {
 };
 
 template <int TYPE>
-int launch_product(bdh_ctx *ctx, const Call &c, Product p) {
+int launch_product(bdh_ctx *ctx, const Call &c, const Plan &plan, Product p) {
   p.w = static_cast<const unsigned char *>(c.w->data);
   p.scales = c.w->scales;
   p.G = c.w->groups;
@@ -488,21 +879,47 @@ int launch_product(bdh_ctx *ctx, const Call &c, Product p) {
   p.N = c.w->outer;
   p.Kb = blocks_of_k(TYPE, p.K);
   p.Nb = (p.N + 63) / 64;
-  if (rows_as_they_are(TYPE, p.K, c.x, c.x_dtype, c.x_stride)) {
-    p.q = static_cast<const unsigned char *>(c.x);
-    p.pitch = 2 * c.x_stride;
-    p.row_scales = nullptr;
-  } else {
-    uint4 *q = static_cast<uint4 *>(c.workspace);
-    p.pitch = (long)p.Kb * 64;
-    float *scales = reinterpret_cast<float *>(static_cast<char *>(c.workspace) + (size_t)c.rows_in * p.pitch);
-    const RowsIn in{c.x, c.x_dtype, p.K, (long)c.rows_in, (long)c.x_stride};
+  p.splits = plan.splits;
+  p.kb_each = plan.kb_each;
+  char *workspace = static_cast<char *>(c.workspace);
+  p.parts = workspace + plan.parts;
+  p.rows_out = p.rows * p.G;
+  const RowsIn in{c.x, c.x_dtype, p.K, (long)c.rows_in, (long)c.x_stride};
+  if (plan.prepared) {
+    uint4 *q = reinterpret_cast<uint4 *>(workspace);
+    float *scales = reinterpret_cast<float *>(workspace + plan.scales);
     const int rc = launch_prepare<TYPE>(ctx, in, p.Kb, q, scales);
     if (rc != BDH_OK) return rc;
+    p.pitch = (long)p.Kb * 64;
     p.q = reinterpret_cast<const unsigned char *>(q);
     p.row_scales = scales;
+  } else {
+    p.pitch = 2 * c.x_stride;
+    p.q = static_cast<const unsigned char *>(c.x);
   }
-  return launch_tiles<TYPE, 64, 64, 2, 2, 4>(ctx, p);
+  int rc;
+  if (plan.few) {
+    auto launch = [&](auto pre) {
+      constexpr bool PRE = decltype(pre)::value;
+      return plan.waves == 8 ? (plan.mt == 1 ? launch_few<TYPE, 1, 8, PRE>(ctx, p, in) : launch_few<TYPE, 2, 8, PRE>(ctx, p, in))
+             : plan.mt == 1  ? launch_few<TYPE, 1, 4, PRE>(ctx, p, in)
+             : plan.mt == 2  ? launch_few<TYPE, 2, 4, PRE>(ctx, p, in)
+                             : launch_few<TYPE, 4, 4, PRE>(ctx, p, in);
+    };
+    rc = plan.splits > 1 || plan.direct ? launch(std::true_type{}) : launch(std::false_type{});
+  } else {
+    rc = plan.bm == 128  ? launch_tiles<TYPE, 128, 256, 2, 4>(ctx, p)
+         : plan.bn == 128 ? launch_tiles<TYPE, 64, 128, 2, 2>(ctx, p)
+                          : launch_tiles<TYPE, 64, 64, 2, 2>(ctx, p);
+  }
+  if (rc != BDH_OK || plan.splits == 1) return rc;
+  const long blocks = (p.rows_out * ((p.N + 7) / 8) + 255) / 256;
+  if (blocks > 0x7fffffffL) return bdh_fail(ctx, BDH_E_SHAPE, "%ld workgroups: the call is too large", blocks);
+  with_behind(p, [&](auto behind) {
+    hipLaunchKernelGGL((k_packed_finish<TYPE, decltype(behind)::value>), dim3((unsigned)blocks), dim3(256), 0, ctx->stream, p);
+  });
+  BDH_LAUNCH_CHECK(ctx, "k_packed_finish");
+  return BDH_OK;
 }
 
 bool overlap(const void *a, size_t na, const void *b, size_t nb) {
@@ -523,7 +940,8 @@ int run_product(bdh_ctx *ctx, const Call &c, const Product &p, int64_t rows_out)
   if (!bdh_aligned(c.x, value_bytes(c.x_dtype)) || !bdh_aligned(p.out, value_bytes(p.out_dtype)) ||
       (p.gate && !bdh_aligned(p.gate, value_bytes(p.gate_dtype))))
     return bdh_fail(ctx, BDH_E_ALIGN, "rows, gate and out need the alignment of their values");
-  const size_t need = workspace_of(w.type, w.inner, c.rows_in, c.x, c.x_dtype, c.x_stride);
+  const Plan plan = plan_of(ctx, w, c.rows_in, p.offsets ? -1 : p.rows, c.x, c.x_dtype, c.x_stride);
+  const size_t need = plan.bytes;
   if (need > 0 && (!c.workspace || c.workspace_bytes < need))
     return bdh_fail(ctx, BDH_E_INVAL, "workspace of %zu bytes, %zu are needed", c.workspace ? c.workspace_bytes : 0, need);
   if (need > 0 && !bdh_aligned(c.workspace, 16)) return bdh_fail(ctx, BDH_E_ALIGN, "the workspace needs 16-byte alignment");
@@ -540,7 +958,7 @@ int run_product(bdh_ctx *ctx, const Call &c, const Product &p, int64_t rows_out)
     if (overlap(r.p, r.bytes, p.out, out_bytes) || (need > 0 && overlap(r.p, r.bytes, c.workspace, need)))
       return bdh_fail(ctx, BDH_E_INVAL, "out or the workspace overlaps what the product reads");
   if (need > 0 && overlap(p.out, out_bytes, c.workspace, need)) return bdh_fail(ctx, BDH_E_INVAL, "out overlaps the workspace");
-  return w.type == BDH_INT8 ? launch_product<BDH_INT8>(ctx, c, p) : launch_product<BDH_BF16>(ctx, c, p);
+  return w.type == BDH_INT8 ? launch_product<BDH_INT8>(ctx, c, plan, p) : launch_product<BDH_BF16>(ctx, c, plan, p);
 }
 
 }  // namespace
@@ -582,9 +1000,10 @@ int bdh_pack_weights(bdh_ctx *ctx, int type, int groups, int inner, int outer, c
 
 size_t bdh_packed_workspace(const bdh_ctx *ctx, const bdh_packed_weights *w, int64_t rows_in, int64_t rows_of_group, const void *x,
                             int x_dtype, int64_t x_stride) {
-  if (!ctx || !w || (w->type != BDH_INT8 && w->type != BDH_BF16) || w->inner < 1 || rows_in <= 0 || !is_rows_type(x_dtype)) return 0;
-  (void)rows_of_group;
-  return workspace_of(w->type, w->inner, rows_in, x, x_dtype, x_stride);
+  if (!ctx || !w || (w->type != BDH_INT8 && w->type != BDH_BF16) || w->inner < 1 || w->outer < 1 || w->groups < 1 || rows_in <= 0 ||
+      rows_of_group == 0 || !is_rows_type(x_dtype))
+    return 0;
+  return plan_of(ctx, *w, rows_in, rows_of_group, x, x_dtype, x_stride).bytes;
 }
 
 int bdh_packed_product(bdh_ctx *ctx, const bdh_packed_weights *w, int64_t rows, const void *x, int x_dtype, int64_t x_stride, void *out,
