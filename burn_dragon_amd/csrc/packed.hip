@@ -26,6 +26,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // rows start at any multiple of their values' size
 typedef unsigned int u32x4u __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned int u32x2u __attribute__((ext_vector_type(2), aligned(2)));
 
 constexpr float kLeast = 0x1p-118f;  // below it a scale would be subnormal: such a row or channel counts as zeros
 constexpr int kMostInner = 131072;   // 127^2 K < 2^31
@@ -46,8 +47,11 @@ __device__ __forceinline__ void scale_of(unsigned int top, float &scale, float &
   scale = top >= 0x7f800000u ? NAN : fits ? a / 127.0f : 0.0f;
   up = fits ? 127.0f / a : 0.0f;
 }
-__device__ __forceinline__ unsigned int whole(float x, float up) {
-  return up != 0.0f ? (unsigned int)(int)__builtin_rintf(x * up) & 0xffu : 0u;  // |x up| < 127.5
+// The whole number nearest to x up (|x up| < 127.5), in the low byte: 1.5 * 2^23 is added, whose last place is 1, so the sum is rounded as
+// rint rounds.  The upper bytes are not cleared.  (What a row or channel that holds no numbers makes does not matter: its scale is NaN.)
+__device__ __forceinline__ unsigned int whole(float x, float up) { return __float_as_uint(x * up + 12582912.0f); }
+__device__ __forceinline__ unsigned int low_bytes(unsigned int a, unsigned int b, unsigned int c, unsigned int d) {
+  return __builtin_amdgcn_perm(b, a, 0x0c0c0400u) | __builtin_amdgcn_perm(d, c, 0x04000c0cu);
 }
 // Rounded to nearest even; a finite value stays finite (the largest bf16 is within half a step of what rounds above it).
 __device__ __forceinline__ unsigned int to_bf16(float x) {
@@ -64,55 +68,52 @@ __device__ __forceinline__ unsigned int half2(float a, float b) {
 
 // ---- weights ------------------------------------------------------------------------------------
 
-// The scales of 64 channels of a group: 16 threads a channel walk k.
-__global__ __launch_bounds__(1024) void k_pack_scales(const void *__restrict__ w, int dtype, int K, int N, float *__restrict__ scales) {
-  __shared__ unsigned int s_top[16][64];
-  const int n = blockIdx.x * 64 + (threadIdx.x & 63), part = threadIdx.x >> 6;
-  const long base = (long)blockIdx.y * K * N;
+// Scales are made in three steps, each over many workgroups: cleared; the bits of the channels' largest magnitudes (their order is that
+// of the magnitudes, and a maximum does not depend on the order of the atomics); the scales of those, after the weights are packed.
+__global__ __launch_bounds__(256) void k_pack_scales(unsigned int *__restrict__ scales, long n, int clear) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float scale = 0.0f, up;
+  if (!clear) scale_of(scales[i], scale, up);
+  scales[i] = __float_as_uint(scale);
+}
+
+constexpr int kPackBlocks = 16;  // blocks of k that a workgroup of the two kernels below takes
+
+__global__ __launch_bounds__(256) void k_pack_tops(const void *__restrict__ w, int dtype, int K, int N, unsigned int *__restrict__ tops) {
+  __shared__ unsigned int s_top[4][64];
+  const int lane = threadIdx.x & 63, part = threadIdx.x >> 6, n = blockIdx.x * 64 + lane, group = blockIdx.y;
+  const int k0 = blockIdx.z * kPackBlocks * 64, k1 = min(K, k0 + kPackBlocks * 64);
   unsigned int top = 0;
   if (n < N)
-    for (int k = part; k < K; k += 16) top = max(top, __float_as_uint(load_value(w, dtype, base + (long)k * N + n)) & 0x7fffffffu);
-  s_top[part][threadIdx.x & 63] = top;
+    for (int k = k0 + part; k < k1; k += 4) top = max(top, __float_as_uint(load_value(w, dtype, ((long)group * K + k) * N + n)) & 0x7fffffffu);
+  s_top[part][lane] = top;
   __syncthreads();
   if (part == 0 && n < N) {
-    for (int p = 1; p < 16; ++p) top = max(top, s_top[p][threadIdx.x]);
-    float scale, up;
-    scale_of(top, scale, up);
-    scales[(long)blockIdx.y * N + n] = scale;
-    s_top[0][threadIdx.x] = top;
+    for (int p = 1; p < 4; ++p) top = max(top, s_top[p][lane]);
+    atomicMax(&tops[(long)group * N + n], top);
   }
 }
 
-// A thread makes the 16 bytes of one lane of a fragment.  The factor 127 / a is that of the largest magnitude itself, which is
-// looked for once more: the scale alone does not give it back.
+// A thread makes the 16 bytes of one lane of a fragment.
 template <int TYPE>
-__global__ __launch_bounds__(256) void k_pack(const void *__restrict__ w, int dtype, int K, int N, int Kb, uint4 *__restrict__ data) {
+__global__ __launch_bounds__(256) void k_pack(const void *__restrict__ w, int dtype, int K, int N, int Kb, const unsigned int *__restrict__ tops,
+                                              uint4 *__restrict__ data) {
   constexpr int PER = TYPE == BDH_INT8 ? 16 : 8;  // values of k in a piece
-  __shared__ unsigned int s_top[64];
-  const int lane = threadIdx.x & 63, frag = threadIdx.x >> 6, nb = blockIdx.x;
-  const int channel = channel_of(frag, lane & 15), n = nb * 64 + channel;
-  const long base = (long)blockIdx.y * K * N;
-  float up = 0.0f;
-  if (TYPE == BDH_INT8) {
-    if (threadIdx.x < 64) s_top[threadIdx.x] = 0;
-    __syncthreads();
-    const int c = nb * 64 + lane;
-    unsigned int top = 0;
-    if (c < N)
-      for (int k = frag; k < K; k += 4) top = max(top, __float_as_uint(load_value(w, dtype, base + (long)k * N + c)) & 0x7fffffffu);
-    atomicMax(&s_top[lane], top);
-    __syncthreads();
-    float scale;
-    scale_of(s_top[channel], scale, up);
-  }
-  uint4 *out = data + (((long)blockIdx.y * gridDim.x + nb) * Kb * 4 + frag) * 64 + lane;
-  for (int kb = 0; kb < Kb; ++kb) {
+  const int lane = threadIdx.x & 63, frag = threadIdx.x >> 6, nb = blockIdx.x, group = blockIdx.y;
+  const int n = nb * 64 + channel_of(frag, lane & 15);
+  float up = 0.0f, scale;
+  if (TYPE == BDH_INT8 && n < N) scale_of(tops[(long)group * N + n], scale, up);
+  uint4 *out = data + (((long)group * gridDim.x + nb) * Kb * 4 + frag) * 64 + lane;
+  const int kb1 = min(Kb, (int)(blockIdx.z + 1) * kPackBlocks);
+  for (int kb = blockIdx.z * kPackBlocks; kb < kb1; ++kb) {
     const int k0 = kb * 4 * PER + (lane >> 4) * PER;
     unsigned int words[4] = {0, 0, 0, 0};
+#pragma unroll
     for (int e = 0; e < PER; ++e) {
       const int k = k0 + e;
-      const float v = n < N && k < K ? load_value(w, dtype, base + (long)k * N + n) : 0.0f;
-      if (TYPE == BDH_INT8) words[e >> 2] |= whole(v, up) << (8 * (e & 3));
+      const float v = n < N && k < K ? load_value(w, dtype, ((long)group * K + k) * N + n) : 0.0f;
+      if (TYPE == BDH_INT8) words[e >> 2] |= (whole(v, up) & 0xffu) << (8 * (e & 3));
       else words[e >> 1] |= to_bf16(v) << (16 * (e & 1));
     }
     out[(long)kb * 256] = make_uint4(words[0], words[1], words[2], words[3]);
@@ -167,11 +168,11 @@ __device__ __forceinline__ unsigned int top_of(const float (&v)[PER], unsigned i
 // The 16 bytes that 16 values make in 8 bits, or 8 in bf16.
 template <int TYPE, int PER>
 __device__ __forceinline__ uint4 packed16(const float (&v)[PER], float up) {
-  unsigned int w[4] = {0, 0, 0, 0};
+  unsigned int w[4];
 #pragma unroll
-  for (int e = 0; e < PER; ++e) {
-    if (TYPE == BDH_INT8) w[e >> 2] |= whole(v[e], up) << (8 * (e & 3));
-    else w[e >> 1] |= to_bf16(v[e]) << (16 * (e & 1));
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (TYPE == BDH_INT8) w[e] = low_bytes(whole(v[4 * e], up), whole(v[4 * e + 1], up), whole(v[4 * e + 2], up), whole(v[4 * e + 3], up));
+    else w[e] = to_bf16(v[2 * e]) | to_bf16(v[2 * e + 1]) << 16;
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
@@ -222,7 +223,7 @@ struct Product {
   long pitch;
   // dense: G heads of B * T rows each; row r of head g is row (r / T * h_in + (h_in > 1 ? g : 0)) * T + r % T of q and row
   // (r / T * G + g) * T + r % T of out.  grouped (offsets): rows offsets[g] .. offsets[g + 1] of both.
-  long rows;  // of a head, or of all groups
+  int rows;  // of a head, or of all groups
   int T, h_in;
   const int32_t *offsets;
   const float *bias;  // [G][N]
@@ -244,8 +245,8 @@ struct Product {
 // there are fewer tiles.  Group g has the rows between the running maximum of the offsets up to g and up to g + 1, both within
 // 0 .. rows: groups never overlap, whatever the offsets hold, and there are at most rows / BM + G tiles.  Every wavefront finds its
 // tile by itself, 64 groups at a time: a table made by a launch before cost as much as it saved.
-__device__ __forceinline__ bool find_tile(const int32_t *__restrict__ offsets, int G, int rows, int BM, int tile, int &group, long &first,
-                                          long &last) {
+__device__ __forceinline__ bool find_tile(const int32_t *__restrict__ offsets, int G, int rows, int BM, int tile, int &group, int &first,
+                                          int &last) {
   const int lane = threadIdx.x & 63;
   int reached = min(max(offsets[0], 0), rows), before = 0;  // the running maximum and the number of tiles so far
   for (int g0 = 0; g0 < G; g0 += 64) {
@@ -265,7 +266,7 @@ __device__ __forceinline__ bool find_tile(const int32_t *__restrict__ offsets, i
     if (has) {
       const int l = __builtin_ctzll(has);
       group = g0 + l;
-      first = __builtin_amdgcn_readlane(start, l) + (long)(tile - before - __builtin_amdgcn_readlane(sum - tiles, l)) * BM;
+      first = __builtin_amdgcn_readlane(start, l) + (tile - before - __builtin_amdgcn_readlane(sum - tiles, l)) * BM;
       last = __builtin_amdgcn_readlane(end, l);
       return true;
     }
@@ -299,11 +300,11 @@ __device__ __forceinline__ bool plain_scale(float s) { return s == 0.0f || (s > 
 // the sums are parts of a longer k.
 enum Behind { kScales, kRelu, kAll, kParts };
 
-// What a lane needs of the 8 neighbouring channels n .. that it holds of every row; channels past the end repeat the last one.
-template <int TYPE, int BEHIND>
+// What a lane needs of the E (4 or 8) neighbouring channels n .. that it holds of every row; channels past the end repeat the last one.
+template <int TYPE, int BEHIND, int E>
 struct Channels {
   int n, left;  // left <= 0: none of them exists
-  float scale[8], bias[8];
+  float scale[E], bias[E];
   __device__ __forceinline__ Channels(const Product &g, int group, int first) : n(first), left(g.N - first) {
     const long c0 = (long)group * g.N;
     if (TYPE == BDH_INT8) values(g.scales + c0, scale);
@@ -312,40 +313,54 @@ struct Channels {
         values(g.bias + c0, bias);
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) bias[e] = 0.0f;
+        for (int e = 0; e < E; ++e) bias[e] = 0.0f;
       }
     }
   }
-  __device__ __forceinline__ void values(const float *p, float (&v)[8]) const {
-    if (left >= 8) {
-      const f32x4 a = *reinterpret_cast<const f32x4u *>(p + n), b = *reinterpret_cast<const f32x4u *>(p + n + 4);
+  __device__ __forceinline__ void values(const float *p, float (&v)[E]) const {
+    if (left >= E) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
+      for (int q = 0; q < E; q += 4) {
+        const f32x4 a = *reinterpret_cast<const f32x4u *>(p + n + q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[q + e] = a[e];
+      }
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = p[min(n + e, n + left - 1 < 0 ? 0 : n + left - 1)];
+      for (int e = 0; e < E; ++e) v[e] = p[min(n + e, n + left - 1)];  // left <= 0: the group's last channel
     }
   }
   __device__ __forceinline__ bool plain() const {
     bool all = true;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) all = all && plain_scale(scale[e]);
+    for (int e = 0; e < E; ++e) all = all && plain_scale(scale[e]);
     return all;
   }
 };
 
-__device__ __forceinline__ void load8(const void *p, int dtype, long at, float (&v)[8]) {
-  if (dtype == BDH_F32) {
+// E neighbouring values of which `left` > 0 exist; the others repeat the last one.
+template <int E>
+__device__ __forceinline__ void load_some(const void *p, int dtype, long at, int left, float (&v)[E]) {
+  if (left < E) {
+    for (int e = 0; e < E; ++e) v[e] = load_value(p, dtype, at + min(e, left - 1));
+  } else if (dtype == BDH_F32) {
     const f32x4u *f = reinterpret_cast<const f32x4u *>(static_cast<const float *>(p) + at);
-    const f32x4 a = f[0], b = f[1];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
+    for (int q = 0; q < E / 4; ++q) {
+      const f32x4 a = f[q];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 * q + e] = a[e];
+    }
   } else {
-    const u32x4u t = *reinterpret_cast<const u32x4u *>(static_cast<const unsigned short *>(p) + at);
+    const u32x2u *h = reinterpret_cast<const u32x2u *>(static_cast<const unsigned short *>(p) + at);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[2 * e] = __uint_as_float(t[e] << 16);
-      v[2 * e + 1] = __uint_as_float(t[e] & 0xffff0000u);
+    for (int q = 0; q < E / 4; ++q) {
+      const u32x2u t = h[q];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        v[4 * q + 2 * e] = __uint_as_float(t[e] << 16);
+        v[4 * q + 2 * e + 1] = __uint_as_float(t[e] & 0xffff0000u);
+      }
     }
   }
 }
@@ -358,62 +373,68 @@ __device__ __forceinline__ void store(V v, void *p) {
   else *static_cast<V *>(p) = v;
 }
 
-// 8 neighbouring channels of a row, whose first value is number `at` of out (and gate): scales, bias, threshold, gate, and the one
-// rounding where out is bf16.  plain: plain_scale holds for all of them (uniform over the wavefront).  A large output counts by the
-// operations here: each one a value costs 5 us where 1500 rows of 131072 are written in 100.
-template <int TYPE, int BEHIND, bool PAST>
-__device__ __forceinline__ void finish8(const Product &g, const Channels<TYPE, BEHIND> &c, long at, const typename Acc<TYPE>::type &lo,
-                                        const typename Acc<TYPE>::type &hi, float row_scale, bool plain) {
+// E neighbouring channels of a row, whose first value is number `at` of out (and gate): scales, bias, threshold, gate (m, where there is
+// one), and the one rounding where out is bf16.  plain: plain_scale holds for all of them (uniform over the wavefront).  A large output
+// counts by the operations here: each one a value costs 5 us where 1500 rows of 131072 are written in 165.
+template <int TYPE, int BEHIND, bool PAST, int E>
+__device__ __forceinline__ void finish(const Product &g, const Channels<TYPE, BEHIND, E> &c, long at, float (&v)[E], const float (&m)[E],
+                                       float row_scale, bool plain) {
   if (c.left <= 0) return;
-  float v[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = (float)(e < 4 ? lo[e] : hi[e - 4]);
   if (TYPE == BDH_INT8) {
     if (plain) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = v[e] * row_scale * c.scale[e];
+      for (int e = 0; e < E; ++e) v[e] = v[e] * row_scale * c.scale[e];
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = scaled(v[e], row_scale, c.scale[e]);
+      for (int e = 0; e < E; ++e) v[e] = scaled(v[e], row_scale, c.scale[e]);
     }
   }
   if (BEHIND == kAll) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = v[e] + c.bias[e] - g.threshold;
+    for (int e = 0; e < E; ++e) v[e] = v[e] + c.bias[e] - g.threshold;
   }
   if (BEHIND != kScales) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = fmaxf(v[e], 0.0f);  // 0 for a NaN: it is not above the threshold
+    for (int e = 0; e < E; ++e) v[e] = fmaxf(v[e], 0.0f);  // 0 for a NaN: it is not above the threshold
   }
   if (BEHIND == kAll && g.gate) {
-    float m[8];
-    if (c.left >= 8) {
-      load8(g.gate, g.gate_dtype, at, m);
-    } else {
-      for (int e = 0; e < 8; ++e) m[e] = load_value(g.gate, g.gate_dtype, at + min(e, c.left - 1));
-    }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] *= m[e];
+    for (int e = 0; e < E; ++e) v[e] *= m[e];
   }
   if (g.out_dtype == BDH_F32) {
     float *o = static_cast<float *>(g.out) + at;
-    if (c.left >= 8) {
-      store<PAST>(f32x4u{v[0], v[1], v[2], v[3]}, o);
-      store<PAST>(f32x4u{v[4], v[5], v[6], v[7]}, o + 4);
+    if (c.left >= E) {
+#pragma unroll
+      for (int q = 0; q < E; q += 4) store<PAST>(f32x4u{v[q], v[q + 1], v[q + 2], v[q + 3]}, o + q);
     } else {
       for (int e = 0; e < c.left; ++e) o[e] = v[e];
     }
   } else {
-    unsigned int w[4];
+    unsigned int w[E / 2];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = half2(v[2 * e], v[2 * e + 1]);
+    for (int e = 0; e < E / 2; ++e) w[e] = half2(v[2 * e], v[2 * e + 1]);
     unsigned short *o = static_cast<unsigned short *>(g.out) + at;
-    if (c.left >= 8) {
-      store<PAST>(u32x4u{w[0], w[1], w[2], w[3]}, o);
+    if (c.left >= E) {
+      if constexpr (E == 8) store<PAST>(u32x4u{w[0], w[1], w[2], w[3]}, o);
+      else store<PAST>(u32x2u{w[0], w[1]}, o);
     } else {
       for (int e = 0; e < c.left; ++e) o[e] = (unsigned short)(w[e >> 1] >> (16 * (e & 1)));
     }
   }
+}
+
+// Rows of a head in q and in out; all row numbers are below 2^31.
+__device__ __forceinline__ unsigned int row_of(unsigned int r, unsigned int T, unsigned int heads, unsigned int head) {
+  if (heads == 1) return r;
+  if (T == 1) return r * heads + head;
+  const unsigned int b = r / T;
+  return (b * heads + head) * T + (r - b * T);
+}
+__device__ __forceinline__ unsigned int row_in_of(const Product &g, unsigned int r, int group) {
+  return g.offsets ? r : row_of(r, g.T, g.h_in, g.h_in == 1 ? 0 : group);
+}
+__device__ __forceinline__ unsigned int row_out_of(const Product &g, unsigned int r, int group) {
+  return g.offsets ? r : row_of(r, g.T, g.G, group);
 }
 
 // Which tile a workgroup takes: workgroups go to the eight XCDs in turn, so XCD i gets every eighth; it takes the i-th eighth of
@@ -448,18 +469,14 @@ __global__ __launch_bounds__(64 * WM * WN, tiles_a_cu(BM, BN) * WM * WN / 4) voi
   const int wm = wave % WM, wn = wave / WM;
   int m_tile, n_tile, split, group = 0;
   place_of(g, m_tile, n_tile, split);
-  long first, last;
+  int first, last;
   if (g.offsets) {
-    if (!find_tile(g.offsets, g.G, (int)g.rows, BM, m_tile, group, first, last)) return;
+    if (!find_tile(g.offsets, g.G, g.rows, BM, m_tile, group, first, last)) return;
   } else {
     group = m_tile / g.m_tiles;
-    first = (long)(m_tile - group * g.m_tiles) * BM;
+    first = (m_tile - group * g.m_tiles) * BM;
     last = g.rows;
   }
-  auto row_in = [&](long r) {
-    if (g.offsets || g.h_in == 1) return r;
-    return (r / g.T * g.h_in + group) * g.T + r % g.T;
-  };
   const unsigned char *from_w[CW], *from_r[CR];
 #pragma unroll
   for (int c = 0; c < CW; ++c) {
@@ -468,8 +485,8 @@ __global__ __launch_bounds__(64 * WM * WN, tiles_a_cu(BM, BN) * WM * WN / 4) voi
   }
 #pragma unroll
   for (int c = 0; c < CR; ++c) {
-    const long r = min(first + (wave + c * W) * 8 + (lane >> 3), last - 1);
-    from_r[c] = g.q + row_in(r) * g.pitch + split * g.kb_each * 64 + ((lane & 7) ^ (lane >> 3)) * 16;
+    const int r = min(first + (wave + c * W) * 8 + (lane >> 3), last - 1);
+    from_r[c] = g.q + row_in_of(g, r, group) * g.pitch + split * g.kb_each * 64 + ((lane & 7) ^ (lane >> 3)) * 16;
   }
   auto copy_w = [&](int stage) {
 #pragma unroll
@@ -530,10 +547,10 @@ __global__ __launch_bounds__(64 * WM * WN, tiles_a_cu(BM, BN) * WM * WN / 4) voi
   bool plain = true;
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
-    const long r = min(first + (wm * TM + i) * 16 + (lane & 15), last - 1);
-    at[i] = (g.offsets || g.G == 1 ? r : (r / g.T * g.G + group) * g.T + r % g.T) * (BEHIND == kParts ? g.Nb * 64L : g.out_stride);
+    const int r = min(first + (wm * TM + i) * 16 + (lane & 15), last - 1);
+    at[i] = row_out_of(g, r, group) * (BEHIND == kParts ? g.Nb * 64L : g.out_stride);
     if (BEHIND == kParts) continue;
-    row_scale[i] = TYPE == BDH_INT8 ? g.row_scales[row_in(r)] : 1.0f;
+    row_scale[i] = TYPE == BDH_INT8 ? g.row_scales[row_in_of(g, r, group)] : 1.0f;
     plain = plain && plain_scale(row_scale[i]);
   }
   if (BEHIND == kParts) {
@@ -550,12 +567,17 @@ __global__ __launch_bounds__(64 * WM * WN, tiles_a_cu(BM, BN) * WM * WN / 4) voi
   }
 #pragma unroll
   for (int j = 0; j < TN; j += 2) {
-    const Channels<TYPE, BEHIND> c(g, group, n_tile * BN + (wn * TN + j) * 16 + 8 * (lane >> 4));
+    const Channels<TYPE, BEHIND, 8> c(g, group, n_tile * BN + (wn * TN + j) * 16 + 8 * (lane >> 4));
     const bool simple = TYPE != BDH_INT8 || __ballot(plain && c.plain()) == ~0ull;
 #pragma unroll
     for (int i = 0; i < TM; ++i)
-      if (first + (wm * TM + i) * 16 + (lane & 15) < last)
-        finish8<TYPE, BEHIND, PAST>(g, c, at[i] + c.n, acc[i][j], acc[i][j + 1], row_scale[i], simple);
+      if (first + (wm * TM + i) * 16 + (lane & 15) < last) {
+        float v[8], m[8];
+        if (BEHIND == kAll && g.gate && c.left > 0) load_some(g.gate, g.gate_dtype, at[i] + c.n, c.left, m);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (float)acc[i][j + (e >> 2)][e & 3];
+        finish<TYPE, BEHIND, PAST>(g, c, at[i] + c.n, v, m, row_scale[i], simple);
+      }
   }
 }
 
@@ -566,17 +588,20 @@ __global__ __launch_bounds__(64 * WM * WN, tiles_a_cu(BM, BN) * WM * WN / 4) voi
 // largest magnitude is looked for by a launch of its own and k is cut into parts.
 template <int TYPE, int BEHIND, int MT, int W, bool PRE>
 __global__ __launch_bounds__(64 * W) void k_packed_few(Product g, RowsIn in) {
-  constexpr int U = MT == 1 ? 4 : MT == 2 ? 2 : 1, PER = TYPE == BDH_INT8 ? 16 : 8, LD = 68;
+  constexpr int U = MT == 1 ? 4 : MT == 2 ? 2 : 1, PER = TYPE == BDH_INT8 ? 16 : 8, LD = 68, ROUNDS = 16 * MT * 16 / (64 * W);
+  static_assert(ROUNDS * 64 * W == 16 * MT * 16 || ROUNDS == 0);
+  constexpr int R = ROUNDS ? ROUNDS : 1;
   typedef typename Acc<TYPE>::type acc_t;
   __shared__ unsigned int s_top[16 * MT];
   __shared__ __attribute__((aligned(16))) int s_sum[W][16 * MT][LD];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int nb = blockIdx.x % g.Nb, rest = blockIdx.x / g.Nb, group = rest % g.G, split = rest / g.G;
-  long first = 0, last = g.rows;
+  const unsigned int rest = blockIdx.x / (unsigned int)g.Nb;
+  const int nb = blockIdx.x - rest * g.Nb, split = rest / (unsigned int)g.G, group = rest - split * g.G;
+  int first = 0, last = g.rows;
   if (g.offsets) {  // the running maximum of the offsets up to the group's first and last row
     int a = 0, b = 0;
     for (int i = lane; i <= group + 1; i += 64) {
-      const int o = min(max(g.offsets[i], 0), (int)g.rows);
+      const int o = min(max(g.offsets[i], 0), g.rows);
       b = max(b, o);
       if (i <= group) a = max(a, o);
     }
@@ -587,30 +612,37 @@ __global__ __launch_bounds__(64 * W) void k_packed_few(Product g, RowsIn in) {
     first = __builtin_amdgcn_readfirstlane(a);
     last = __builtin_amdgcn_readfirstlane(b);
   }
-  auto row_in = [&](long r) {
-    if (g.offsets || g.h_in == 1) return r;
-    return (r / g.T * g.h_in + group) * g.T + r % g.T;
-  };
   const int kb0 = split * g.kb_each, kb1 = min(kb0 + g.kb_each, g.Kb);
   const i32x4 *w = reinterpret_cast<const i32x4 *>(g.w) + ((long)group * g.Nb + nb) * g.Kb * 256 + lane;
   for (; first < last; first += 16 * MT) {
-    long row[MT];
+    unsigned int row[MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) row[i] = row_in(min(first + i * 16 + (lane & 15), last - 1));
+    for (int i = 0; i < MT; ++i) row[i] = row_in_of(g, min(first + i * 16 + (lane & 15), last - 1), group);
     i32x4 fw[U][4], fr[U][MT];
     float v[PRE ? 1 : U][PRE ? 1 : MT][PER];
     auto ask = [&](int b, int u) {  // block b of the weights and rows
-#pragma unroll
-      for (int j = 0; j < 4; ++j) fw[u][j] = w[(long)b * 256 + j * 64];
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         if constexpr (PRE) fr[u][i] = *reinterpret_cast<const i32x4 *>(g.q + row[i] * g.pitch + b * 64 + (lane >> 4) * 16);
         else load_values<PER>(in, row[i], (b * 4 + (lane >> 4)) * PER, v[u][i]);
       }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) fw[u][j] = w[(long)b * 256 + j * 64];
     };
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (kb0 + wave + u * W < kb1) ask(kb0 + wave + u * W, u);
+    // what comes behind the sums of 4 channels of a row a thread is asked for with them
+    const int c4 = (threadIdx.x & 15) * 4, mine = threadIdx.x >> 4;
+    const Channels<TYPE, BEHIND, 4> c(g, group, nb * 64 + c4);
+    unsigned int out_row[R];
+    float gate[R][4];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      const int q = min(first + mine + k * 4 * W, last - 1);
+      out_row[k] = row_out_of(g, q, group);
+      if (BEHIND == kAll && g.gate && c.left > 0) load_some(g.gate, g.gate_dtype, out_row[k] * g.out_stride + c.n, c.left, gate[k]);
+    }
     float up[MT];
     if constexpr (TYPE == BDH_INT8 && !PRE) {
       if (threadIdx.x < 16 * MT) s_top[threadIdx.x] = 0;
@@ -664,28 +696,23 @@ __global__ __launch_bounds__(64 * W) void k_packed_few(Product g, RowsIn in) {
       for (int j = 0; j < 4; ++j)
         *reinterpret_cast<acc_t *>(&s_sum[wave][i * 16 + (lane & 15)][32 * (j >> 1) + 8 * (lane >> 4) + 4 * (j & 1)]) = acc[i][j];
     __syncthreads();
-    for (int t = threadIdx.x; t < 16 * MT * 8; t += 64 * W) {
-      const int r = t >> 3, c8 = (t & 7) * 8;
-      if (first + r >= last) break;
-      acc_t lo = acc_t{}, hi = acc_t{};
 #pragma unroll
-      for (int k = 0; k < W; ++k) {
-        lo += *reinterpret_cast<const acc_t *>(&s_sum[k][r][c8]);
-        hi += *reinterpret_cast<const acc_t *>(&s_sum[k][r][c8 + 4]);
-      }
-      const long q = first + r, out_row = g.offsets || g.G == 1 ? q : (q / g.T * g.G + group) * g.T + q % g.T;
+    for (int k = 0; k < R; ++k) {
+      const int r = mine + k * 4 * W;
+      if (r >= 16 * MT || first + r >= last) break;
+      acc_t sum = *reinterpret_cast<const acc_t *>(&s_sum[0][r][c4]);
+#pragma unroll
+      for (int x = 1; x < W; ++x) sum += *reinterpret_cast<const acc_t *>(&s_sum[x][r][c4]);
       if constexpr (BEHIND == kParts) {
-        acc_t *out = reinterpret_cast<acc_t *>(static_cast<char *>(g.parts) + 4 * ((split * g.rows_out + out_row) * g.Nb + nb) * 64);
-        out[c8 / 4] = lo;
-        out[c8 / 4 + 1] = hi;
+        reinterpret_cast<acc_t *>(g.parts)[((split * g.rows_out + out_row[k]) * g.Nb + nb) * 16 + c4 / 4] = sum;
       } else {
         float scale = 1.0f, unused;
         if constexpr (TYPE == BDH_INT8) {
-          if constexpr (PRE) scale = g.row_scales[row_in(q)];
+          if constexpr (PRE) scale = g.row_scales[row_in_of(g, first + r, group)];
           else scale_of(s_top[r], scale, unused);
         }
-        const Channels<TYPE, BEHIND> c(g, group, nb * 64 + c8);
-        finish8<TYPE, BEHIND, false>(g, c, out_row * g.out_stride + c.n, lo, hi, scale, false);
+        float sums[4] = {(float)sum[0], (float)sum[1], (float)sum[2], (float)sum[3]};
+        finish<TYPE, BEHIND, false>(g, c, out_row[k] * g.out_stride + c.n, sums, gate[k], scale, false);
       }
     }
     if (first + 16 * MT < last) __syncthreads();
@@ -712,10 +739,14 @@ __global__ __launch_bounds__(256) void k_packed_finish(Product g) {
     for (int u = 0; u < 8; ++u) lo += a[u], hi += b[u];
   }
   for (; i < g.splits; ++i) lo += p[i * part], hi += p[i * part + 1];
-  const int group = (int)(row / g.T % g.G);
-  const long row_in = g.h_in == 1 ? row / ((long)g.T * g.G) * g.T + row % g.T : row;
-  const Channels<TYPE, BEHIND> c(g, group, n);
-  finish8<TYPE, BEHIND, false>(g, c, row * g.out_stride + n, lo, hi, TYPE == BDH_INT8 ? g.row_scales[row_in] : 1.0f, false);
+  const unsigned int r = (unsigned int)row, b = r / (unsigned int)g.T, head = b % (unsigned int)g.G;
+  const unsigned int row_in = g.h_in == 1 ? b / g.G * g.T + (r - b * g.T) : r;
+  const Channels<TYPE, BEHIND, 8> c(g, head, n);
+  float v[8], m[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = (float)(e < 4 ? lo[e] : hi[e - 4]);
+  if (BEHIND == kAll && g.gate) load_some(g.gate, g.gate_dtype, row * g.out_stride + n, c.left, m);
+  finish<TYPE, BEHIND, false>(g, c, row * g.out_stride + n, v, m, TYPE == BDH_INT8 ? g.row_scales[row_in] : 1.0f, false);
 }
 
 // ---- host ---------------------------------------------------------------------------------------
@@ -779,10 +810,22 @@ Plan plan_of(const bdh_ctx *ctx, const bdh_packed_weights &w, int64_t rows_in, i
   } else {
     p.prepared = !p.direct;
     const int64_t heads = grouped ? 1 : w.groups;
-    auto tiles = [&](int bm, int bn) { return (rows + bm - 1) / bm * heads * ((w.outer + bn - 1) / bn); };
-    if (tiles(128, 256) >= 2 * ctx->n_cu) p.bm = 128, p.bn = 256;
-    else if (tiles(64, 128) >= 2 * ctx->n_cu) p.bm = 64, p.bn = 128;
-    else p.bm = 64, p.bn = 64;
+    auto tiles = [&](int bm, int bn) {
+      const int64_t n = (w.outer + bn - 1) / bn;
+      return grouped ? ((rows + bm - 1) / bm + w.groups / 2) * n : (rows + bm - 1) / bm * heads * n;
+    };
+    // The tile whose rounds over the chip cost least: a round is as many as the CUs hold at a time, a value of a smaller tile costs more
+    // (8192 x 8192 x 8192 in 8 bits | bf16, us: 128x256 440 | 830, 64x128 640 | 1500, 64x64 more still).
+    const struct {
+      int bm, bn;
+      double value;
+    } shapes[] = {{128, 256, 1.0}, {64, 128, 1.3}, {64, 64, 2.0}};
+    double best = 0.0;
+    for (const auto &t : shapes) {
+      const int64_t each = tiles_a_cu(t.bm, t.bn), at_once = each * ctx->n_cu;
+      const double cost = (double)((tiles(t.bm, t.bn) + at_once - 1) / at_once) * each * t.bm * t.bn * t.value;
+      if (p.bm == 0 || cost < best) best = cost, p.bm = t.bm, p.bn = t.bn;
+    }
     if (!grouped && tiles(64, 64) < 2 * ctx->n_cu && Kb >= 32) {
       if (tiles(128, 256) * (Kb / 16) >= 2 * ctx->n_cu) p.bm = 128, p.bn = 256;
       const int64_t each = p.bm == 128 ? 2 : 5, want = (each * ctx->n_cu) / tiles(p.bm, p.bn), most = Kb / 16;
@@ -827,7 +870,7 @@ void with_behind(const Product &p, F launch) {
 template <int TYPE, int BM, int BN, int WM, int WN>
 int launch_tiles(bdh_ctx *ctx, Product p) {
   p.n_tiles = (p.N + BN - 1) / BN;
-  const long per_head = (p.rows + BM - 1) / BM, tiles = (p.offsets ? per_head + p.G : per_head * p.G) * p.n_tiles * p.splits;
+  const long per_head = ((long)p.rows + BM - 1) / BM, tiles = (p.offsets ? per_head + p.G : per_head * p.G) * p.n_tiles * p.splits;
   if (tiles > 0x7fffffffL) return bdh_fail(ctx, BDH_E_SHAPE, "%ld tiles: the call is too large", tiles);
   p.m_tiles = (int)per_head;
   const dim3 grid((unsigned)tiles), threads(64 * WM * WN);
@@ -883,7 +926,7 @@ int launch_product(bdh_ctx *ctx, const Call &c, const Plan &plan, Product p) {
   p.kb_each = plan.kb_each;
   char *workspace = static_cast<char *>(c.workspace);
   p.parts = workspace + plan.parts;
-  p.rows_out = p.rows * p.G;
+  p.rows_out = (long)p.rows * p.G;
   const RowsIn in{c.x, c.x_dtype, p.K, (long)c.rows_in, (long)c.x_stride};
   if (plan.prepared) {
     uint4 *q = reinterpret_cast<uint4 *>(workspace);
@@ -985,14 +1028,19 @@ int bdh_pack_weights(bdh_ctx *ctx, int type, int groups, int inner, int outer, c
   const size_t channels = type == BDH_INT8 ? sizeof(float) * (size_t)groups * outer : 0;
   if (overlap(weight, dense, data, bytes) || (channels && (overlap(weight, dense, scales, channels) || overlap(data, bytes, scales, channels))))
     return bdh_fail(ctx, BDH_E_INVAL, "weights, packed weights and scales overlap");
-  const dim3 grid((outer + 63) / 64, groups);
   const int Kb = blocks_of_k(type, inner);
+  const dim3 grid((outer + 63) / 64, groups, (Kb + kPackBlocks - 1) / kPackBlocks), threads(256);
+  unsigned int *tops = reinterpret_cast<unsigned int *>(scales);
+  uint4 *to = static_cast<uint4 *>(data);
   if (type == BDH_INT8) {
-    hipLaunchKernelGGL(k_pack_scales, grid, dim3(1024), 0, ctx->stream, weight, weight_dtype, inner, outer, scales);
-    BDH_LAUNCH_CHECK(ctx, "k_pack_scales");
-    hipLaunchKernelGGL(k_pack<BDH_INT8>, grid, dim3(256), 0, ctx->stream, weight, weight_dtype, inner, outer, Kb, static_cast<uint4 *>(data));
+    const long n = (long)groups * outer;
+    const dim3 every((unsigned)((n + 255) / 256));
+    hipLaunchKernelGGL(k_pack_scales, every, threads, 0, ctx->stream, tops, n, 1);
+    hipLaunchKernelGGL(k_pack_tops, grid, threads, 0, ctx->stream, weight, weight_dtype, inner, outer, tops);
+    hipLaunchKernelGGL(k_pack<BDH_INT8>, grid, threads, 0, ctx->stream, weight, weight_dtype, inner, outer, Kb, tops, to);
+    hipLaunchKernelGGL(k_pack_scales, every, threads, 0, ctx->stream, tops, n, 0);
   } else {
-    hipLaunchKernelGGL(k_pack<BDH_BF16>, grid, dim3(256), 0, ctx->stream, weight, weight_dtype, inner, outer, Kb, static_cast<uint4 *>(data));
+    hipLaunchKernelGGL(k_pack<BDH_BF16>, grid, threads, 0, ctx->stream, weight, weight_dtype, inner, outer, Kb, nullptr, to);
   }
   BDH_LAUNCH_CHECK(ctx, "k_pack");
   return BDH_OK;

@@ -6,7 +6,7 @@ from typing import Optional
 import torch
 
 from .. import ffi
-from ..packed import PackedWeights, _ROWS, _rows_type, _workspace
+from ..packed import _ROWS, PackedWeights, _new, _rows_type, _workspace
 from .block_sparse import BlockPattern1d
 
 
@@ -40,10 +40,10 @@ def packed_forward(input: torch.Tensor, weights: PackedWeights, bias: Optional[t
     [B,h,T,N] -> [B,h,T,N] = gate * relu(input . weight + bias - threshold), a new tensor of out_dtype or `out`.  Input, gate
     and out are f32 or bf16 each."""
     h, d, N, on = weights.groups, weights.inner, weights.outer, weights.on
-    kind = _rows_type("input", input, on)
-    if input.dim() != 4 or input.shape[1] not in (1, h) or input.shape[3] != d or not input.is_contiguous():
-        raise ValueError(f"input: expected contiguous [B, 1 or {h}, T, {d}], got {tuple(input.shape)} with strides {input.stride()}")
-    B, h_in, T = input.shape[:3]
+    kind, given = _rows_type("input", input, on), input.shape
+    if len(given) != 4 or given[3] != d or (given[1] != h and given[1] != 1) or not input.is_contiguous():
+        raise ValueError(f"input: expected contiguous [B, 1 or {h}, T, {d}], got {tuple(given)} with strides {input.stride()}")
+    B, h_in, T, _ = given
     if (B | T | B * T) >> 31:
         raise ValueError(f"{B} x {T} rows: a call carries numbers below 2^31")
     shape, gate_kind = (B, h, T, N), 0
@@ -56,14 +56,11 @@ def packed_forward(input: torch.Tensor, weights: PackedWeights, bias: Optional[t
             raise ValueError(f"gate: expected contiguous {shape}, got {tuple(gate.shape)}")
     ctx = ffi.context_on(on, ctx)
     if out is None:
-        if out_dtype not in _ROWS:
-            raise ValueError(f"out_dtype: f32 or bf16, not {out_dtype}")
-        with ctx.torch_stream():
-            out = torch.empty(shape, device=input.device, dtype=out_dtype)
+        out = _new(input, shape, out_dtype, ctx)
     elif out.dtype not in _ROWS or out.get_device() != on or out.shape != shape or not out.is_contiguous():
         raise ValueError(f"out: expected contiguous f32 or bf16 {shape}, got {out.dtype} {tuple(out.shape)}")
     held, workspace, size = _workspace(ctx, weights, B * h_in * T, B * T, input, kind, d)
     ctx.check(ctx._lib.bdh_packed_relu_lowrank(
-        ctx.handle, weights._ref, B, h_in, T, input.data_ptr(), kind, None if bias is None else bias.data_ptr(), float(threshold),
+        ctx.handle, weights._ref, B, h_in, T, input.data_ptr(), kind, None if bias is None else bias.data_ptr(), threshold,
         None if gate is None else gate.data_ptr(), gate_kind, out.data_ptr(), _ROWS[out.dtype], workspace, size))
     return out

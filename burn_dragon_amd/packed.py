@@ -13,6 +13,7 @@ from . import ffi
 
 _ROWS = {torch.float32: ffi.F32, torch.bfloat16: ffi.BF16}
 _WEIGHTS = {torch.int8: ffi.INT8, torch.bfloat16: ffi.BF16}
+FEW = 64  # rows that are streamed past the weights in one launch, where k is not so long that it is cut into parts
 MOST_INNER, MOST_OUTER, MOST_GROUPS = 131072, 1 << 24, 65535
 
 
@@ -38,20 +39,30 @@ class PackedWeights:
                                        self.data.data_ptr(), ffi.ptr(self.scales)))
         self._c = ffi.PackedWeightsC(kind, self.groups, self.inner, self.outer, self.data.data_ptr(), ffi.ptr(self.scales))
         self._ref = ctypes.byref(self._c)
+        # calls of up to this many rows a group need no workspace: asking for its size would cost a tenth of such a call
+        few = (lib.bdh_packed_workspace(ctx.handle, self._ref, n, n, None, ffi.F32, self.inner) for n in (1, 16, 32, FEW))
+        self.few = FEW if self.groups > 0 and not any(few) else 0
 
     @property
     def nbytes(self) -> int:
         return self.data.numel() + (0 if self.scales is None else 4 * self.scales.numel())
 
 
+def _refuse_rows(name: str, t: torch.Tensor, on: int) -> None:
+    raise ValueError(f"{name}: expected f32 or bf16 on device {on}, got {t.dtype} on {t.device}")
+
+
 def _rows_type(name: str, t: torch.Tensor, on: int) -> int:
-    if t.dtype not in _ROWS or t.get_device() != on:
-        raise ValueError(f"{name}: expected f32 or bf16 on device {on}, got {t.dtype} on {t.device}")
-    return _ROWS[t.dtype]
+    kind = _ROWS.get(t.dtype)
+    if kind is None or t.get_device() != on:
+        _refuse_rows(name, t, on)
+    return kind
 
 
 def _workspace(ctx: ffi.Context, weights: PackedWeights, rows: int, of_group: int, x: torch.Tensor, kind: int, stride: int):
     """What the call needs beside its arguments, from torch's allocator: a captured call keeps its own."""
+    if 0 <= of_group <= weights.few:
+        return None, None, 0
     size = ctx._lib.bdh_packed_workspace(ctx.handle, weights._ref, rows, of_group, x.data_ptr(), kind, stride)
     if size == 0:
         return None, None, 0
@@ -60,44 +71,43 @@ def _workspace(ctx: ffi.Context, weights: PackedWeights, rows: int, of_group: in
     return held, held.data_ptr(), size
 
 
-def _as_rows(x: torch.Tensor, K: int, ctx: ffi.Context) -> torch.Tensor:
-    """x as [M,K] rows of neighbouring values."""
-    if x.dim() == 2 and (K == 1 or x.stride(1) == 1) and (x.shape[0] < 2 or x.stride(0) >= K):
-        return x
-    with ctx.torch_stream():  # it may be a copy
-        return x.reshape(-1, K).contiguous()
+def _new(like: torch.Tensor, shape, dtype: torch.dtype, ctx: ffi.Context) -> torch.Tensor:
+    if dtype not in _ROWS:
+        raise ValueError(f"out_dtype: f32 or bf16, not {dtype}")
+    if ctx._follow:  # a tensor like another is a quarter faster to make than one from scratch
+        return like.new_empty(shape) if dtype is like.dtype else like.new_empty(shape, dtype=dtype)
+    with ctx.torch_stream():
+        return like.new_empty(shape, dtype=dtype)
 
 
-def _call(name: str, x: torch.Tensor, weights: PackedWeights, offsets, out_dtype, out, ctx):
+def _call(x: torch.Tensor, weights: PackedWeights, offsets, out_dtype, out, ctx):
     K, N, on = weights.inner, weights.outer, weights.on
-    kind = _rows_type("x", x, on)
-    if x.dim() < 1 or x.shape[-1] != K:
-        raise ValueError(f"x: expected rows of {K} values, got {tuple(x.shape)}")
+    kind, shape = _rows_type("x", x, on), x.shape
+    if not shape or shape[-1] != K:
+        raise ValueError(f"x: expected rows of {K} values, got {tuple(shape)}")
     ctx = ffi.context_on(on, ctx)
-    rows = _as_rows(x, K, ctx)
-    M = rows.shape[0]
+    if len(shape) != 2 or not x.is_contiguous():
+        if len(shape) != 2 or (K > 1 and x.stride(1) != 1) or (shape[0] > 1 and x.stride(0) < K):
+            with ctx.torch_stream():  # it may be a copy
+                x = x.reshape(-1, K).contiguous()
+    M = x.shape[0]
     if M >> 31:
         raise ValueError(f"{M} rows: a call carries numbers below 2^31")
-    shape = (*x.shape[:-1], N)
     if out is None:
-        if out_dtype not in _ROWS:
-            raise ValueError(f"out_dtype: f32 or bf16, not {out_dtype}")
-        with ctx.torch_stream():
-            out = torch.empty(shape, device=x.device, dtype=out_dtype)
-        out_stride = N
+        out, out_stride = _new(x, (M, N) if len(shape) == 2 else (*shape[:-1], N), out_dtype, ctx), N
     else:
         _rows_type("out", out, on)
         dense = out.is_contiguous()
-        if out.shape != shape or not (dense or (out.dim() == 2 and out.stride(1) == 1 and out.stride(0) >= N)):
-            raise ValueError(f"out: expected rows {shape}, got {tuple(out.shape)} with strides {out.stride()}")
+        if out.shape != (*shape[:-1], N) or not (dense or (out.dim() == 2 and out.stride(1) == 1 and out.stride(0) >= N)):
+            raise ValueError(f"out: expected rows {(*shape[:-1], N)}, got {tuple(out.shape)} with strides {out.stride()}")
         out_stride = N if dense else out.stride(0)
-    stride = rows.stride(0) if M > 1 else K
-    held, workspace, size = _workspace(ctx, weights, M, M if offsets is None else -1, rows, kind, stride)
+    stride = x.stride(0) if M > 1 else K
+    held, workspace, size = _workspace(ctx, weights, M, M if offsets is None or M <= weights.few else -1, x, kind, stride)
     if offsets is None:
-        ctx.check(ctx._lib.bdh_packed_product(ctx.handle, weights._ref, M, rows.data_ptr(), kind, stride, out.data_ptr(), _ROWS[out.dtype],
+        ctx.check(ctx._lib.bdh_packed_product(ctx.handle, weights._ref, M, x.data_ptr(), kind, stride, out.data_ptr(), _ROWS[out.dtype],
                                               out_stride, workspace, size))
     else:
-        ctx.check(ctx._lib.bdh_grouped_product(ctx.handle, weights._ref, M, offsets.data_ptr(), rows.data_ptr(), kind, stride,
+        ctx.check(ctx._lib.bdh_grouped_product(ctx.handle, weights._ref, M, offsets.data_ptr(), x.data_ptr(), kind, stride,
                                                out.data_ptr(), _ROWS[out.dtype], out_stride, workspace, size))
     return out
 
@@ -107,7 +117,7 @@ def product(x: torch.Tensor, weights: PackedWeights, out_dtype: torch.dtype = to
     """x [..., K] (f32 or bf16) times weights of one group -> [..., N], a new tensor of out_dtype (f32 or bf16) or `out`."""
     if weights.groups != 1:
         raise ValueError(f"weights of {weights.groups} groups: a product takes one (grouped_product takes them all)")
-    return _call("product", x, weights, None, out_dtype, out, ctx)
+    return _call(x, weights, None, out_dtype, out, ctx)
 
 
 def grouped_product(x: torch.Tensor, weights: PackedWeights, offsets: Union[torch.Tensor, Sequence[int]],
@@ -129,4 +139,4 @@ def grouped_product(x: torch.Tensor, weights: PackedWeights, offsets: Union[torc
             offsets = torch.tensor(offsets, dtype=torch.int32, device=x.device)
     if offsets.shape != (G + 1,) or offsets.dtype is not torch.int32 or offsets.get_device() != weights.on or not offsets.is_contiguous():
         raise ValueError(f"offsets: expected int32 [{G + 1}] on {weights.device}, got {offsets.dtype} {tuple(offsets.shape)} on {offsets.device}")
-    return _call("grouped_product", x, weights, offsets, out_dtype, out, ctx)
+    return _call(x, weights, offsets, out_dtype, out, ctx)
