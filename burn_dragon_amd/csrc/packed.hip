@@ -177,10 +177,10 @@ __device__ __forceinline__ uint4 packed16(const float (&v)[PER], float up) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Rows as the product takes them: [rows][Kb * 64 bytes], zeros behind K, and the scales of 8-bit rows.  THR threads a row, 16 bytes
+// Rows as the product takes them, `pitch` bytes apart: Kb * 64 bytes, zeros behind K, and the scales of 8-bit rows.  THR threads a row, 16 bytes
 // a thread at a time; 8-bit rows are read twice, the second time from a cache.
 template <int TYPE, int THR>
-__global__ __launch_bounds__(THR < 256 ? 256 : THR) void k_prepare_rows(RowsIn in, int Kb, uint4 *__restrict__ q, float *__restrict__ scales) {
+__global__ __launch_bounds__(THR < 256 ? 256 : THR) void k_prepare_rows(RowsIn in, int Kb, long pitch, uint4 *__restrict__ q, float *__restrict__ scales) {
   constexpr int ROWS = THR < 256 ? 256 / THR : 1, PER = TYPE == BDH_INT8 ? 16 : 8;
   __shared__ unsigned int s_top[THR < 256 ? 4 : THR / 64];
   const long row = (long)blockIdx.x * ROWS + threadIdx.x / THR;
@@ -205,7 +205,7 @@ __global__ __launch_bounds__(THR < 256 ? 256 : THR) void k_prepare_rows(RowsIn i
     if (live && t == 0) scales[row] = scale;
   }
   if (!live) return;
-  uint4 *out = q + row * Kb * 4;
+  uint4 *out = q + row * (pitch / 16);
   for (int k = t * PER; k < padded; k += THR * PER) {
     load_values<PER>(in, row, min(k, in.K), v);
     out[k / PER] = packed16<TYPE>(v, up);
@@ -219,7 +219,9 @@ struct Product {
   const float *scales;     // [G][N] of 8-bit weights
   int G, K, N, Kb, Nb;     // Kb blocks of 64 bytes of k, Nb blocks of 64 channels
   const unsigned char *q;  // rows [rows][pitch] bytes
-  const float *row_scales;
+  float *row_scales;
+  const unsigned int *tops;  // bits of the largest magnitudes of parts of the rows, top_parts of them a row
+  int top_parts;
   long pitch;
   // dense: G heads of B * T rows each; row r of head g is row (r / T * h_in + (h_in > 1 ? g : 0)) * T + r % T of q and row
   // (r / T * G + g) * T + r % T of out.  grouped (offsets): rows offsets[g] .. offsets[g + 1] of both.
@@ -305,6 +307,7 @@ template <int TYPE, int BEHIND, int E>
 struct Channels {
   int n, left;  // left <= 0: none of them exists
   float scale[E], bias[E];
+  __device__ __forceinline__ Channels(int first, int N) : n(first), left(N - first) {}
   __device__ __forceinline__ Channels(const Product &g, int group, int first) : n(first), left(g.N - first) {
     const long c0 = (long)group * g.N;
     if (TYPE == BDH_INT8) values(g.scales + c0, scale);
@@ -329,12 +332,6 @@ struct Channels {
 #pragma unroll
       for (int e = 0; e < E; ++e) v[e] = p[min(n + e, n + left - 1)];  // left <= 0: the group's last channel
     }
-  }
-  __device__ __forceinline__ bool plain() const {
-    bool all = true;
-#pragma unroll
-    for (int e = 0; e < E; ++e) all = all && plain_scale(scale[e]);
-    return all;
   }
 };
 
@@ -477,6 +474,14 @@ __global__ __launch_bounds__(64 * WM * WN, tiles_a_cu(BM, BN) * WM * WN / 4) voi
     first = (m_tile - group * g.m_tiles) * BM;
     last = g.rows;
   }
+  // What the finished sums are scaled by, a number a thread, on its way while the sums are made: BN channels, then BM rows.
+  static_assert(BM + BN <= 64 * W);
+  float mine = 1.0f, bias = 0.0f;
+  if (TYPE == BDH_INT8 && BEHIND != kParts) {
+    if (threadIdx.x < BN) mine = g.scales[(long)group * g.N + min(n_tile * BN + (int)threadIdx.x, g.N - 1)];
+    else if (threadIdx.x < BN + BM) mine = g.row_scales[row_in_of(g, min(first + (int)threadIdx.x - BN, last - 1), group)];
+  }
+  if (BEHIND == kAll && g.bias && threadIdx.x < BN) bias = g.bias[(long)group * g.N + min(n_tile * BN + (int)threadIdx.x, g.N - 1)];
   const unsigned char *from_w[CW], *from_r[CR];
 #pragma unroll
   for (int c = 0; c < CW; ++c) {
@@ -543,16 +548,9 @@ __global__ __launch_bounds__(64 * WM * WN, tiles_a_cu(BM, BN) * WM * WN / 4) voi
     step(1, rows);
   }
   long at[TM];
-  float row_scale[TM];
-  bool plain = true;
 #pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const int r = min(first + (wm * TM + i) * 16 + (lane & 15), last - 1);
-    at[i] = row_out_of(g, r, group) * (BEHIND == kParts ? g.Nb * 64L : g.out_stride);
-    if (BEHIND == kParts) continue;
-    row_scale[i] = TYPE == BDH_INT8 ? g.row_scales[row_in_of(g, r, group)] : 1.0f;
-    plain = plain && plain_scale(row_scale[i]);
-  }
+  for (int i = 0; i < TM; ++i)
+    at[i] = row_out_of(g, min(first + (wm * TM + i) * 16 + (lane & 15), last - 1), group) * (BEHIND == kParts ? g.Nb * 64L : g.out_stride);
   if (BEHIND == kParts) {
     acc_t *out = reinterpret_cast<acc_t *>(static_cast<char *>(g.parts) + 4 * split * g.rows_out * g.Nb * 64);
 #pragma unroll
@@ -565,10 +563,33 @@ __global__ __launch_bounds__(64 * WM * WN, tiles_a_cu(BM, BN) * WM * WN / 4) voi
     }
     return;
   }
+  float *s_scale = reinterpret_cast<float *>(s_w), *s_bias = s_scale + BM + BN;  // the ring is free
+  int *s_plain = reinterpret_cast<int *>(s_bias + BN);
+  if (TYPE == BDH_INT8 || BEHIND == kAll) {
+    __syncthreads();
+    if (threadIdx.x < BM + BN) s_scale[threadIdx.x] = mine;
+    if (threadIdx.x < BN) s_bias[threadIdx.x] = bias;
+    const bool all = __ballot(plain_scale(mine)) == ~0ull;
+    if (lane == 0) s_plain[wave] = all;
+    __syncthreads();
+  }
+  bool plain = true;
+  float row_scale[TM];
+  if (TYPE == BDH_INT8) {
+#pragma unroll
+    for (int w = 0; w < W; ++w) plain = plain && s_plain[w];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) row_scale[i] = s_scale[BN + (wm * TM + i) * 16 + (lane & 15)];
+  }
 #pragma unroll
   for (int j = 0; j < TN; j += 2) {
-    const Channels<TYPE, BEHIND, 8> c(g, group, n_tile * BN + (wn * TN + j) * 16 + 8 * (lane >> 4));
-    const bool simple = TYPE != BDH_INT8 || __ballot(plain && c.plain()) == ~0ull;
+    const int channel = (wn * TN + j) * 16 + 8 * (lane >> 4);
+    Channels<TYPE, BEHIND, 8> c(n_tile * BN + channel, g.N);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (TYPE == BDH_INT8) c.scale[e] = s_scale[channel + e];
+      if (BEHIND == kAll) c.bias[e] = s_bias[channel + e];
+    }
 #pragma unroll
     for (int i = 0; i < TM; ++i)
       if (first + (wm * TM + i) * 16 + (lane & 15) < last) {
@@ -576,7 +597,7 @@ __global__ __launch_bounds__(64 * WM * WN, tiles_a_cu(BM, BN) * WM * WN / 4) voi
         if (BEHIND == kAll && g.gate && c.left > 0) load_some(g.gate, g.gate_dtype, at[i] + c.n, c.left, m);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = (float)acc[i][j + (e >> 2)][e & 3];
-        finish<TYPE, BEHIND, PAST>(g, c, at[i] + c.n, v, m, row_scale[i], simple);
+        finish<TYPE, BEHIND, PAST>(g, c, at[i] + c.n, v, m, row_scale[i], plain);
       }
   }
 }
@@ -586,9 +607,9 @@ __global__ __launch_bounds__(64 * WM * WN, tiles_a_cu(BM, BN) * WM * WN / 4) voi
 // of k, up to U blocks of weights and rows, is asked for at once, and the largest magnitude of a row is a maximum over the
 // wavefronts in LDS; the wavefronts' sums are added up in LDS in their order.  PRE: the rows are prepared ones, for k so long that a row's
 // largest magnitude is looked for by a launch of its own and k is cut into parts.
-template <int TYPE, int BEHIND, int MT, int W, bool PRE>
+template <int TYPE, int BEHIND, int MT, int W, int U, bool PRE>
 __global__ __launch_bounds__(64 * W) void k_packed_few(Product g, RowsIn in) {
-  constexpr int U = MT == 1 ? 4 : MT == 2 ? 2 : 1, PER = TYPE == BDH_INT8 ? 16 : 8, LD = 68, ROUNDS = 16 * MT * 16 / (64 * W);
+  constexpr int PER = TYPE == BDH_INT8 ? 16 : 8, LD = 68, ROUNDS = 16 * MT * 16 / (64 * W);
   static_assert(ROUNDS * 64 * W == 16 * MT * 16 || ROUNDS == 0);
   constexpr int R = ROUNDS ? ROUNDS : 1;
   typedef typename Acc<TYPE>::type acc_t;
@@ -647,6 +668,20 @@ __global__ __launch_bounds__(64 * W) void k_packed_few(Product g, RowsIn in) {
     if constexpr (TYPE == BDH_INT8 && !PRE) {
       if (threadIdx.x < 16 * MT) s_top[threadIdx.x] = 0;
       __syncthreads();
+      if constexpr (BEHIND == kParts) {
+        const int n = min(last - first, 16 * MT);
+        for (int t = threadIdx.x; t < n * g.top_parts; t += 64 * W) {
+          const int r = t / g.top_parts;
+          atomicMax(&s_top[r], g.tops[(long)row_in_of(g, first + r, group) * g.top_parts + (t - r * g.top_parts)]);
+        }
+        __syncthreads();
+        if (split == 0 && nb == 0)  // for k_packed_finish
+          for (int t = threadIdx.x; t < n; t += 64 * W) {
+            float scale, unused;
+            scale_of(s_top[t], scale, unused);
+            g.row_scales[row_in_of(g, first + t, group)] = scale;
+          }
+      } else {
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         unsigned int top = 0;
@@ -663,10 +698,11 @@ __global__ __launch_bounds__(64 * W) void k_packed_few(Product g, RowsIn in) {
         if (lane < 16) atomicMax(&s_top[i * 16 + lane], top);
       }
       __syncthreads();
+      }
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         float scale;
-        scale_of(s_top[i * 16 + (lane & 15)], scale, up[i]);
+        scale_of(s_top[min(i * 16 + (lane & 15), last - first - 1)], scale, up[i]);
       }
     }
     acc_t acc[MT][4];
@@ -708,8 +744,7 @@ __global__ __launch_bounds__(64 * W) void k_packed_few(Product g, RowsIn in) {
       } else {
         float scale = 1.0f, unused;
         if constexpr (TYPE == BDH_INT8) {
-          if constexpr (PRE) scale = g.row_scales[row_in_of(g, first + r, group)];
-          else scale_of(s_top[r], scale, unused);
+          scale_of(s_top[r], scale, unused);
         }
         float sums[4] = {(float)sum[0], (float)sum[1], (float)sum[2], (float)sum[3]};
         finish<TYPE, BEHIND, false>(g, c, out_row[k] * g.out_stride + c.n, sums, gate[k], scale, false);
@@ -719,32 +754,56 @@ __global__ __launch_bounds__(64 * W) void k_packed_few(Product g, RowsIn in) {
   }
 }
 
-// The sums of the parts of k, and what comes behind them: 8 channels of a row a thread.
-template <int TYPE, int BEHIND>
+// The bits of the largest magnitudes of parts of rows, 4096 values each: for few and long rows, which one workgroup each would be long about.
+__global__ __launch_bounds__(256) void k_row_tops(RowsIn in, int parts, unsigned int *__restrict__ tops) {
+  __shared__ unsigned int s_top[4];
+  const unsigned int row = blockIdx.x / (unsigned int)parts, part = blockIdx.x - row * parts;
+  const int k = part * 4096 + threadIdx.x * 16;
+  unsigned int top = 0;
+  if (k < in.K) {
+    float v[16];
+    load_values<16>(in, row, k, v);
+    top = top_of<16>(v, 0);
+  }
+  for (int o = 32; o > 0; o >>= 1) top = max(top, (unsigned int)__shfl_xor((int)top, o));
+  if ((threadIdx.x & 63) == 0) s_top[threadIdx.x >> 6] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) tops[blockIdx.x] = max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3]));
+}
+
+// The sums of the parts of k, and what comes behind them: 4 channels of a row a thread; LANES threads share the parts where there are
+// few sums.
+template <int TYPE, int BEHIND, int LANES>
 __global__ __launch_bounds__(256) void k_packed_finish(Product g) {
   typedef typename Acc<TYPE>::type acc_t;
-  const int eighths = (g.N + 7) / 8;
-  const long t = (long)blockIdx.x * 256 + threadIdx.x, row = t / eighths;
-  if (row >= g.rows_out) return;
-  const int n = (int)(t - row * eighths) * 8;
+  __shared__ acc_t s_sum[LANES][256 / LANES];
+  const int fours = (g.N + 3) / 4, lane = threadIdx.x / (256 / LANES), at = threadIdx.x % (256 / LANES);
+  const long t = (long)blockIdx.x * (256 / LANES) + at, row = min(t / fours, g.rows_out - 1);
+  const int n = (int)(t % fours) * 4;
   const long part = g.rows_out * g.Nb * 16;
   const acc_t *p = static_cast<const acc_t *>(g.parts) + (row * g.Nb * 64 + n) / 4;
-  acc_t lo = acc_t{}, hi = acc_t{};
-  int i = 0;
-  for (; i + 8 <= g.splits; i += 8) {  // eight parts on their way at a time
-    acc_t a[8], b[8];
+  acc_t sum = acc_t{};
+  int i = lane;
+  for (; i + 7 * LANES < g.splits; i += 8 * LANES) {  // eight parts on their way at a time
+    acc_t a[8];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) a[u] = p[(i + u) * part], b[u] = p[(i + u) * part + 1];
+    for (int u = 0; u < 8; ++u) a[u] = p[(i + u * LANES) * part];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) lo += a[u], hi += b[u];
+    for (int u = 0; u < 8; ++u) sum += a[u];
   }
-  for (; i < g.splits; ++i) lo += p[i * part], hi += p[i * part + 1];
+  for (; i < g.splits; i += LANES) sum += p[i * part];
+  if (LANES > 1) {
+    s_sum[lane][at] = sum;
+    __syncthreads();
+    if (lane > 0) return;
+#pragma unroll
+    for (int l = 1; l < LANES; ++l) sum += s_sum[l][at];
+  }
+  if (t >= g.rows_out * fours) return;
   const unsigned int r = (unsigned int)row, b = r / (unsigned int)g.T, head = b % (unsigned int)g.G;
   const unsigned int row_in = g.h_in == 1 ? b / g.G * g.T + (r - b * g.T) : r;
-  const Channels<TYPE, BEHIND, 8> c(g, head, n);
-  float v[8], m[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = (float)(e < 4 ? lo[e] : hi[e - 4]);
+  const Channels<TYPE, BEHIND, 4> c(g, head, n);
+  float v[4] = {(float)sum[0], (float)sum[1], (float)sum[2], (float)sum[3]}, m[4];
   if (BEHIND == kAll && g.gate) load_some(g.gate, g.gate_dtype, row * g.out_stride + n, c.left, m);
   finish<TYPE, BEHIND, false>(g, c, row * g.out_stride + n, v, m, TYPE == BDH_INT8 ? g.row_scales[row_in] : 1.0f, false);
 }
@@ -767,6 +826,10 @@ int check_weights(bdh_ctx *ctx, const bdh_packed_weights *w) {
   return BDH_OK;
 }
 
+// Bytes from one prepared row to the next: rows that are multiples of 4 KiB would all lie at the same channels of the caches and memory
+// (2048 rows of 128 KiB 189 -> 142 us).
+long pitch_of(int Kb) { return Kb % 64 == 0 ? Kb * 64L + 128 : Kb * 64L; }
+
 bool is_rows_type(int t) { return t == BDH_F32 || t == BDH_BF16; }
 size_t value_bytes(int dtype) { return dtype == BDH_F32 ? 4 : 2; }
 
@@ -779,10 +842,12 @@ bool rows_as_they_are(int type, int K, const void *x, int x_dtype, int64_t x_str
 struct Plan {
   bool few;       // the weights are streamed by k_packed_few, for 16 * mt rows at a time by `waves` wavefronts
   int mt, waves;
+  bool one;       // a wavefront has one block of k at a time on its way
   int bm, bn;     // else tiles
   bool prepared, direct;  // the rows are prepared by a launch of their own; the product reads them where they are
   int splits, kb_each;
-  size_t scales, parts, bytes;  // where in the workspace the prepared rows' scales and the parts' sums lie, and its size
+  int top_parts;                      // parts of rows whose largest magnitudes a launch of its own looks for
+  size_t scales, tops, parts, bytes;  // where in the workspace the rows' scales, those magnitudes and the parts' sums lie, and its size
 };
 
 Plan plan_of(const bdh_ctx *ctx, const bdh_packed_weights &w, int64_t rows_in, int64_t rows_of_group, const void *x, int x_dtype,
@@ -799,14 +864,15 @@ Plan plan_of(const bdh_ctx *ctx, const bdh_packed_weights &w, int64_t rows_in, i
   if (p.few) {
     const int64_t a_group = grouped ? (rows + std::max(w.groups, 1) - 1) / std::max(w.groups, 1) : rows;
     p.mt = a_group <= 16 ? 1 : a_group <= 32 ? 2 : 4;
-    p.waves = p.mt < 4 && blocks < ctx->n_cu && Kb > 8 ? 8 : 4;
+    p.waves = p.mt < 4 && Kb > 4 && (Kb <= 8 || blocks < ctx->n_cu) ? 8 : 4;
     if (!grouped && Kb > 16 * p.waves && blocks < ctx->n_cu) {  // fewer workgroups than CUs, and more of k than they have on their way
-      const int64_t most = (Kb + p.waves - 1) / p.waves, want = (2 * ctx->n_cu + blocks - 1) / blocks;
       p.waves = 4;
-      p.kb_each = (int)((Kb + std::min(most, want) - 1) / std::min(most, want) + 7) / 8 * 8;
+      const int64_t most = (Kb + 3) / 4, want = (2 * ctx->n_cu + blocks - 1) / blocks, splits = std::min(most, want);
+      p.kb_each = (int)((Kb + splits - 1) / splits + 1) / 2 * 2;
       p.splits = (Kb + p.kb_each - 1) / p.kb_each;
-      p.prepared = !p.direct;
+      if (w.type == BDH_INT8) p.top_parts = (w.inner + 4095) / 4096;
     }
+    p.one = (p.splits > 1 ? p.kb_each : Kb) <= p.waves || p.mt == 4;
   } else {
     p.prepared = !p.direct;
     const int64_t heads = grouped ? 1 : w.groups;
@@ -819,25 +885,29 @@ Plan plan_of(const bdh_ctx *ctx, const bdh_packed_weights &w, int64_t rows_in, i
     const struct {
       int bm, bn;
       double value;
-    } shapes[] = {{128, 256, 1.0}, {64, 128, 1.3}, {64, 64, 2.0}};
+    } shapes[] = {{128, 256, 1.0}, {64, 128, 1.3}, {64, 64, 2.0}, {256, 256, 0.95}};
     double best = 0.0;
     for (const auto &t : shapes) {
       const int64_t each = tiles_a_cu(t.bm, t.bn), at_once = each * ctx->n_cu;
       const double cost = (double)((tiles(t.bm, t.bn) + at_once - 1) / at_once) * each * t.bm * t.bn * t.value;
+      if (t.bm == 256 && Kb < 128) continue;  // one workgroup a CU: nothing covers its beginning and end
       if (p.bm == 0 || cost < best) best = cost, p.bm = t.bm, p.bn = t.bn;
     }
     if (!grouped && tiles(64, 64) < 2 * ctx->n_cu && Kb >= 32) {
-      if (tiles(128, 256) * (Kb / 16) >= 2 * ctx->n_cu) p.bm = 128, p.bn = 256;
-      const int64_t each = p.bm == 128 ? 2 : 5, want = (each * ctx->n_cu) / tiles(p.bm, p.bn), most = Kb / 16;
+      if (tiles(256, 256) * (Kb / 64) >= ctx->n_cu) p.bm = 256, p.bn = 256;
+      else if (tiles(128, 256) * (Kb / 16) >= 2 * ctx->n_cu) p.bm = 128, p.bn = 256;
+      else p.bm = 64, p.bn = 64;
+      const int64_t each = tiles_a_cu(p.bm, p.bn), want = (each * ctx->n_cu) / tiles(p.bm, p.bn), most = Kb / 16;
       const int64_t splits = std::max<int64_t>(1, std::min(want, most));
       p.kb_each = (int)((Kb + splits - 1) / splits + 1) / 2 * 2;
       p.splits = (Kb + p.kb_each - 1) / p.kb_each;
     }
   }
   size_t at = 0;
-  if (p.prepared) {
-    p.scales = (size_t)rows_in * Kb * 64;
-    at = p.scales + bdh_align_up(sizeof(float) * (size_t)rows_in, 64);
+  if (p.prepared || p.top_parts) {
+    p.scales = p.prepared ? (size_t)rows_in * pitch_of(Kb) : 0;
+    p.tops = p.scales + bdh_align_up(sizeof(float) * (size_t)rows_in, 64);
+    at = p.tops + bdh_align_up(sizeof(float) * (size_t)rows_in * p.top_parts, 64);
   }
   if (p.splits > 1) {
     p.parts = at;
@@ -850,11 +920,11 @@ Plan plan_of(const bdh_ctx *ctx, const bdh_packed_weights &w, int64_t rows_in, i
 template <int TYPE>
 int launch_prepare(bdh_ctx *ctx, const RowsIn &in, int Kb, uint4 *q, float *scales) {
   if (in.K <= 2048)
-    hipLaunchKernelGGL((k_prepare_rows<TYPE, 64>), dim3((unsigned)((in.rows + 3) / 4)), dim3(256), 0, ctx->stream, in, Kb, q, scales);
+    hipLaunchKernelGGL((k_prepare_rows<TYPE, 64>), dim3((unsigned)((in.rows + 3) / 4)), dim3(256), 0, ctx->stream, in, Kb, pitch_of(Kb), q, scales);
   else if (in.K <= 16384)
-    hipLaunchKernelGGL((k_prepare_rows<TYPE, 256>), dim3((unsigned)in.rows), dim3(256), 0, ctx->stream, in, Kb, q, scales);
+    hipLaunchKernelGGL((k_prepare_rows<TYPE, 256>), dim3((unsigned)in.rows), dim3(256), 0, ctx->stream, in, Kb, pitch_of(Kb), q, scales);
   else
-    hipLaunchKernelGGL((k_prepare_rows<TYPE, 1024>), dim3((unsigned)in.rows), dim3(1024), 0, ctx->stream, in, Kb, q, scales);
+    hipLaunchKernelGGL((k_prepare_rows<TYPE, 1024>), dim3((unsigned)in.rows), dim3(1024), 0, ctx->stream, in, Kb, pitch_of(Kb), q, scales);
   BDH_LAUNCH_CHECK(ctx, "k_prepare_rows");
   return BDH_OK;
 }
@@ -887,16 +957,16 @@ int launch_tiles(bdh_ctx *ctx, Product p) {
   return BDH_OK;
 }
 
-template <int TYPE, int MT, int W, bool PRE>
+template <int TYPE, int MT, int W, int U, bool PRE>
 int launch_few(bdh_ctx *ctx, const Product &p, const RowsIn &in) {
   const long blocks = (long)p.Nb * p.G * p.splits;
   if (blocks > 0x7fffffffL) return bdh_fail(ctx, BDH_E_SHAPE, "%ld workgroups: the call is too large", blocks);
   const dim3 grid((unsigned)blocks), threads(64 * W);
   if (p.splits > 1) {
-    if constexpr (PRE && W == 4) hipLaunchKernelGGL((k_packed_few<TYPE, kParts, MT, W, true>), grid, threads, 0, ctx->stream, p, in);
-  } else if constexpr (!PRE || TYPE == BDH_BF16) {
+    if constexpr (W == 4) hipLaunchKernelGGL((k_packed_few<TYPE, kParts, MT, W, U, PRE>), grid, threads, 0, ctx->stream, p, in);
+  } else {
     with_behind(p, [&](auto behind) {
-      hipLaunchKernelGGL((k_packed_few<TYPE, decltype(behind)::value, MT, W, PRE>), grid, threads, 0, ctx->stream, p, in);
+      hipLaunchKernelGGL((k_packed_few<TYPE, decltype(behind)::value, MT, W, U, PRE>), grid, threads, 0, ctx->stream, p, in);
     });
   }
   BDH_LAUNCH_CHECK(ctx, "k_packed_few");
@@ -933,7 +1003,7 @@ int launch_product(bdh_ctx *ctx, const Call &c, const Plan &plan, Product p) {
     float *scales = reinterpret_cast<float *>(workspace + plan.scales);
     const int rc = launch_prepare<TYPE>(ctx, in, p.Kb, q, scales);
     if (rc != BDH_OK) return rc;
-    p.pitch = (long)p.Kb * 64;
+    p.pitch = pitch_of(p.Kb);
     p.q = reinterpret_cast<const unsigned char *>(q);
     p.row_scales = scales;
   } else {
@@ -944,22 +1014,39 @@ int launch_product(bdh_ctx *ctx, const Call &c, const Plan &plan, Product p) {
   if (plan.few) {
     auto launch = [&](auto pre) {
       constexpr bool PRE = decltype(pre)::value;
-      return plan.waves == 8 ? (plan.mt == 1 ? launch_few<TYPE, 1, 8, PRE>(ctx, p, in) : launch_few<TYPE, 2, 8, PRE>(ctx, p, in))
-             : plan.mt == 1  ? launch_few<TYPE, 1, 4, PRE>(ctx, p, in)
-             : plan.mt == 2  ? launch_few<TYPE, 2, 4, PRE>(ctx, p, in)
-                             : launch_few<TYPE, 4, 4, PRE>(ctx, p, in);
+      if (plan.waves == 8) {
+        if (plan.mt == 1) return plan.one ? launch_few<TYPE, 1, 8, 1, PRE>(ctx, p, in) : launch_few<TYPE, 1, 8, 4, PRE>(ctx, p, in);
+        return plan.one ? launch_few<TYPE, 2, 8, 1, PRE>(ctx, p, in) : launch_few<TYPE, 2, 8, 2, PRE>(ctx, p, in);
+      }
+      if (plan.mt == 1) return plan.one ? launch_few<TYPE, 1, 4, 1, PRE>(ctx, p, in) : launch_few<TYPE, 1, 4, 4, PRE>(ctx, p, in);
+      if (plan.mt == 2) return plan.one ? launch_few<TYPE, 2, 4, 1, PRE>(ctx, p, in) : launch_few<TYPE, 2, 4, 2, PRE>(ctx, p, in);
+      return launch_few<TYPE, 4, 4, 1, PRE>(ctx, p, in);
     };
-    rc = plan.splits > 1 || plan.direct ? launch(std::true_type{}) : launch(std::false_type{});
+    if (plan.top_parts) {
+      const long tops = (long)c.rows_in * plan.top_parts;
+      hipLaunchKernelGGL(k_row_tops, dim3((unsigned)tops), dim3(256), 0, ctx->stream, in, plan.top_parts, reinterpret_cast<unsigned int *>(workspace + plan.tops));
+      BDH_LAUNCH_CHECK(ctx, "k_row_tops");
+      p.tops = reinterpret_cast<const unsigned int *>(workspace + plan.tops);
+      p.top_parts = plan.top_parts;
+      p.row_scales = reinterpret_cast<float *>(workspace + plan.scales);
+    }
+    if constexpr (TYPE == BDH_BF16) rc = plan.direct ? launch(std::true_type{}) : launch(std::false_type{});
+    else rc = launch(std::false_type{});
   } else {
-    rc = plan.bm == 128  ? launch_tiles<TYPE, 128, 256, 2, 4>(ctx, p)
+    rc = plan.bm == 256   ? launch_tiles<TYPE, 256, 256, 4, 4>(ctx, p)
+         : plan.bm == 128 ? launch_tiles<TYPE, 128, 256, 2, 4>(ctx, p)
          : plan.bn == 128 ? launch_tiles<TYPE, 64, 128, 2, 2>(ctx, p)
                           : launch_tiles<TYPE, 64, 64, 2, 2>(ctx, p);
   }
   if (rc != BDH_OK || plan.splits == 1) return rc;
-  const long blocks = (p.rows_out * ((p.N + 7) / 8) + 255) / 256;
+  const long sums = p.rows_out * ((p.N + 3) / 4);
+  const bool shared = sums < 256L * ctx->n_cu;
+  const long blocks = (sums * (shared ? 8 : 1) + 255) / 256;
   if (blocks > 0x7fffffffL) return bdh_fail(ctx, BDH_E_SHAPE, "%ld workgroups: the call is too large", blocks);
   with_behind(p, [&](auto behind) {
-    hipLaunchKernelGGL((k_packed_finish<TYPE, decltype(behind)::value>), dim3((unsigned)blocks), dim3(256), 0, ctx->stream, p);
+    constexpr int BEHIND = decltype(behind)::value;
+    if (shared) hipLaunchKernelGGL((k_packed_finish<TYPE, BEHIND, 8>), dim3((unsigned)blocks), dim3(256), 0, ctx->stream, p);
+    else hipLaunchKernelGGL((k_packed_finish<TYPE, BEHIND, 1>), dim3((unsigned)blocks), dim3(256), 0, ctx->stream, p);
   });
   BDH_LAUNCH_CHECK(ctx, "k_packed_finish");
   return BDH_OK;
