@@ -177,23 +177,51 @@ __device__ __forceinline__ uint4 packed16(const float (&v)[PER], float up) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Rows as the product takes them, `pitch` bytes apart: Kb * 64 bytes, zeros behind K, and the scales of 8-bit rows.  THR threads a row, 16 bytes
-// a thread at a time; 8-bit rows are read twice, the second time from a cache.
-template <int TYPE, int THR>
+// Rows as the product takes them, `pitch` bytes apart: Kb * 64 bytes, zeros behind K, and the scales of 8-bit rows.  THR threads a row, 16
+// bytes a thread at a time.  An 8-bit row is read once, as far as HOLD values a thread hold it as they came (X: float or bf16's bits), and
+// what is behind them twice, the second time from a cache.
+template <int TYPE, typename X, int THR>
 __global__ __launch_bounds__(THR < 256 ? 256 : THR) void k_prepare_rows(RowsIn in, int Kb, long pitch, uint4 *__restrict__ q, float *__restrict__ scales) {
-  constexpr int ROWS = THR < 256 ? 256 / THR : 1, PER = TYPE == BDH_INT8 ? 16 : 8;
+  constexpr int ROWS = THR < 256 ? 256 / THR : 1, PER = TYPE == BDH_INT8 ? 16 : 8, HOLD = TYPE == BDH_INT8 ? (sizeof(X) == 2 ? 8 : 4) : 0;
+  typedef X piece __attribute__((ext_vector_type(PER), aligned(sizeof(X))));
   __shared__ unsigned int s_top[THR < 256 ? 4 : THR / 64];
   const long row = (long)blockIdx.x * ROWS + threadIdx.x / THR;
   const int t = threadIdx.x % THR, padded = Kb * (TYPE == BDH_INT8 ? 64 : 32);
   const bool live = row < in.rows;
+  const X *x = static_cast<const X *>(in.x) + (live ? row : 0) * in.stride;
+  auto values = [&](const piece &p, float (&v)[PER]) {
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      if constexpr (sizeof(X) == 2) v[e] = __uint_as_float((unsigned int)p[e] << 16);
+      else v[e] = p[e];
+    }
+  };
+  piece held[HOLD ? HOLD : 1];
   float v[PER], scale = 1.0f, up = 1.0f;
   if (TYPE == BDH_INT8) {
     unsigned int top = 0;
-    if (live)
-      for (int k = t * PER; k < in.K; k += THR * PER) {
+    if (live) {
+#pragma unroll
+      for (int h = 0; h < HOLD; ++h) {
+        const int k = (h * THR + t) * PER;
+        if (k + PER <= in.K) held[h] = *reinterpret_cast<const piece *>(x + k);
+      }
+#pragma unroll
+      for (int h = 0; h < HOLD; ++h) {
+        const int k = (h * THR + t) * PER;
+        if (k + PER <= in.K) {
+          values(held[h], v);
+          top = top_of<PER>(v, top);
+        } else if (k < in.K) {
+          load_values<PER>(in, row, k, v);
+          top = top_of<PER>(v, top);
+        }
+      }
+      for (int k = (HOLD * THR + t) * PER; k < in.K; k += THR * PER) {
         load_values<PER>(in, row, k, v);
         top = top_of<PER>(v, top);
       }
+    }
     for (int o = 32; o > 0; o >>= 1) top = max(top, (unsigned int)__shfl_xor((int)top, o));
     if (THR > 64) {
       if ((threadIdx.x & 63) == 0) s_top[threadIdx.x >> 6] = top;
@@ -206,7 +234,18 @@ __global__ __launch_bounds__(THR < 256 ? 256 : THR) void k_prepare_rows(RowsIn i
   }
   if (!live) return;
   uint4 *out = q + row * (pitch / 16);
-  for (int k = t * PER; k < padded; k += THR * PER) {
+#pragma unroll
+  for (int h = 0; h < HOLD; ++h) {
+    const int k = (h * THR + t) * PER;
+    if (k + PER <= in.K) {
+      values(held[h], v);
+      out[k / PER] = packed16<TYPE>(v, up);
+    } else if (k < padded) {
+      load_values<PER>(in, row, min(k, in.K), v);
+      out[k / PER] = packed16<TYPE>(v, up);
+    }
+  }
+  for (int k = (HOLD * THR + t) * PER; k < padded; k += THR * PER) {
     load_values<PER>(in, row, min(k, in.K), v);
     out[k / PER] = packed16<TYPE>(v, up);
   }
@@ -340,7 +379,9 @@ template <int E>
 __device__ __forceinline__ void load_some(const void *p, int dtype, long at, int left, float (&v)[E]) {
   if (left < E) {
     for (int e = 0; e < E; ++e) v[e] = load_value(p, dtype, at + min(e, left - 1));
-  } else if (dtype == BDH_F32) {
+    return;
+  }
+  if (dtype == BDH_F32) {
     const f32x4u *f = reinterpret_cast<const f32x4u *>(static_cast<const float *>(p) + at);
 #pragma unroll
     for (int q = 0; q < E / 4; ++q) {
@@ -590,14 +631,28 @@ __global__ __launch_bounds__(64 * WM * WN, tiles_a_cu(BM, BN) * WM * WN / 4) voi
       if (TYPE == BDH_INT8) c.scale[e] = s_scale[channel + e];
       if (BEHIND == kAll) c.bias[e] = s_bias[channel + e];
     }
+    float gate[BEHIND == kAll ? TM : 1][8];
+    if (BEHIND == kAll && g.gate) {
+      if ((n_tile + 1) * BN <= g.N) {  // all of them on their way before the first is used
+        if (g.gate_dtype == BDH_F32) {
+#pragma unroll
+          for (int i = 0; i < TM; ++i) load_some(g.gate, BDH_F32, at[i] + c.n, 8, gate[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < TM; ++i) load_some(g.gate, BDH_BF16, at[i] + c.n, 8, gate[i]);
+        }
+      } else if (c.left > 0) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) load_some(g.gate, g.gate_dtype, at[i] + c.n, c.left, gate[i]);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < TM; ++i)
       if (first + (wm * TM + i) * 16 + (lane & 15) < last) {
-        float v[8], m[8];
-        if (BEHIND == kAll && g.gate && c.left > 0) load_some(g.gate, g.gate_dtype, at[i] + c.n, c.left, m);
+        float v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = (float)acc[i][j + (e >> 2)][e & 3];
-        finish<TYPE, BEHIND, PAST>(g, c, at[i] + c.n, v, m, row_scale[i], plain);
+        finish<TYPE, BEHIND, PAST>(g, c, at[i] + c.n, v, gate[BEHIND == kAll ? i : 0], row_scale[i], plain);
       }
   }
 }
@@ -851,7 +906,7 @@ struct Plan {
 };
 
 Plan plan_of(const bdh_ctx *ctx, const bdh_packed_weights &w, int64_t rows_in, int64_t rows_of_group, const void *x, int x_dtype,
-             int64_t x_stride) {
+             int64_t x_stride, bool gated) {
   Plan p{};
   const bool grouped = rows_of_group < 0;
   p.direct = rows_as_they_are(w.type, w.inner, x, x_dtype, x_stride);
@@ -882,15 +937,18 @@ Plan plan_of(const bdh_ctx *ctx, const bdh_packed_weights &w, int64_t rows_in, i
     };
     // The tile whose rounds over the chip cost least: a round is as many as the CUs hold at a time, a value of a smaller tile costs more
     // (8192 x 8192 x 8192 in 8 bits | bf16, us: 128x256 440 | 830, 64x128 640 | 1500, 64x64 more still).
+    // Gates want registers beside the sums, all of them on their way at once: 128x128 by 8 wavefronts has them (1554 rows of 4 heads of
+    // 8192, bf16, K 256 118 -> 108; 1500 rows in 8 bits, K 512 131 -> 100), while k is so short that they count (bf16, K 1024 155 | 160).
+    const bool gates = gated && Kb < 32;
     const struct {
       int bm, bn;
       double value;
-    } shapes[] = {{128, 256, 1.0}, {64, 128, 1.3}, {64, 64, 2.0}, {256, 256, 0.95}};
+    } shapes[] = {{128, gates ? 128 : 256, 1.0}, {64, 128, 1.3}, {64, 64, 2.0}, {256, 256, 0.95}};
     double best = 0.0;
     for (const auto &t : shapes) {
       const int64_t each = tiles_a_cu(t.bm, t.bn), at_once = each * ctx->n_cu;
       const double cost = (double)((tiles(t.bm, t.bn) + at_once - 1) / at_once) * each * t.bm * t.bn * t.value;
-      if (t.bm == 256 && Kb < 128) continue;  // one workgroup a CU: nothing covers its beginning and end
+      if (t.bm == 256 && (Kb < 128 || gates)) continue;  // one workgroup a CU: nothing covers its beginning and end
       if (p.bm == 0 || cost < best) best = cost, p.bm = t.bm, p.bn = t.bn;
     }
     if (!grouped && tiles(64, 64) < 2 * ctx->n_cu && Kb >= 32) {
@@ -917,14 +975,15 @@ Plan plan_of(const bdh_ctx *ctx, const bdh_packed_weights &w, int64_t rows_in, i
   return p;
 }
 
-template <int TYPE>
+template <int TYPE, typename X>
 int launch_prepare(bdh_ctx *ctx, const RowsIn &in, int Kb, uint4 *q, float *scales) {
+  const unsigned int rows = (unsigned)in.rows;
   if (in.K <= 2048)
-    hipLaunchKernelGGL((k_prepare_rows<TYPE, 64>), dim3((unsigned)((in.rows + 3) / 4)), dim3(256), 0, ctx->stream, in, Kb, pitch_of(Kb), q, scales);
+    hipLaunchKernelGGL((k_prepare_rows<TYPE, X, 64>), dim3((rows + 3) / 4), dim3(256), 0, ctx->stream, in, Kb, pitch_of(Kb), q, scales);
   else if (in.K <= 16384)
-    hipLaunchKernelGGL((k_prepare_rows<TYPE, 256>), dim3((unsigned)in.rows), dim3(256), 0, ctx->stream, in, Kb, pitch_of(Kb), q, scales);
+    hipLaunchKernelGGL((k_prepare_rows<TYPE, X, 256>), dim3(rows), dim3(256), 0, ctx->stream, in, Kb, pitch_of(Kb), q, scales);
   else
-    hipLaunchKernelGGL((k_prepare_rows<TYPE, 1024>), dim3((unsigned)in.rows), dim3(1024), 0, ctx->stream, in, Kb, pitch_of(Kb), q, scales);
+    hipLaunchKernelGGL((k_prepare_rows<TYPE, X, 1024>), dim3(rows), dim3(1024), 0, ctx->stream, in, Kb, pitch_of(Kb), q, scales);
   BDH_LAUNCH_CHECK(ctx, "k_prepare_rows");
   return BDH_OK;
 }
@@ -945,14 +1004,16 @@ int launch_tiles(bdh_ctx *ctx, Product p) {
   p.m_tiles = (int)per_head;
   const dim3 grid((unsigned)tiles), threads(64 * WM * WN);
   const bool past = bdh_aligned(p.out, 16) && p.out_stride * value_bytes(p.out_dtype) % 16 == 0;
-  if (p.splits > 1)
-    hipLaunchKernelGGL((k_packed_tile<TYPE, kParts, false, BM, BN, WM, WN>), grid, threads, 0, ctx->stream, p);
-  else
+  if (p.splits > 1) {
+    if constexpr (BM != 128 || BN != 128) hipLaunchKernelGGL((k_packed_tile<TYPE, kParts, false, BM, BN, WM, WN>), grid, threads, 0, ctx->stream, p);
+  } else {
     with_behind(p, [&](auto behind) {
       constexpr int BEHIND = decltype(behind)::value;
-      if (past) hipLaunchKernelGGL((k_packed_tile<TYPE, BEHIND, true, BM, BN, WM, WN>), grid, threads, 0, ctx->stream, p);
+      if constexpr (BM == 128 && BN == 128 && BEHIND != kAll) return;  // for gates
+      else if (past) hipLaunchKernelGGL((k_packed_tile<TYPE, BEHIND, true, BM, BN, WM, WN>), grid, threads, 0, ctx->stream, p);
       else hipLaunchKernelGGL((k_packed_tile<TYPE, BEHIND, false, BM, BN, WM, WN>), grid, threads, 0, ctx->stream, p);
     });
+  }
   BDH_LAUNCH_CHECK(ctx, "k_packed_tile");
   return BDH_OK;
 }
@@ -1001,7 +1062,8 @@ int launch_product(bdh_ctx *ctx, const Call &c, const Plan &plan, Product p) {
   if (plan.prepared) {
     uint4 *q = reinterpret_cast<uint4 *>(workspace);
     float *scales = reinterpret_cast<float *>(workspace + plan.scales);
-    const int rc = launch_prepare<TYPE>(ctx, in, p.Kb, q, scales);
+    const int rc = in.dtype == BDH_F32 ? launch_prepare<TYPE, float>(ctx, in, p.Kb, q, scales)
+                                       : launch_prepare<TYPE, unsigned short>(ctx, in, p.Kb, q, scales);
     if (rc != BDH_OK) return rc;
     p.pitch = pitch_of(p.Kb);
     p.q = reinterpret_cast<const unsigned char *>(q);
@@ -1034,7 +1096,7 @@ int launch_product(bdh_ctx *ctx, const Call &c, const Plan &plan, Product p) {
     else rc = launch(std::false_type{});
   } else {
     rc = plan.bm == 256   ? launch_tiles<TYPE, 256, 256, 4, 4>(ctx, p)
-         : plan.bm == 128 ? launch_tiles<TYPE, 128, 256, 2, 4>(ctx, p)
+         : plan.bm == 128 ? (plan.bn == 256 ? launch_tiles<TYPE, 128, 256, 2, 4>(ctx, p) : launch_tiles<TYPE, 128, 128, 2, 4>(ctx, p))
          : plan.bn == 128 ? launch_tiles<TYPE, 64, 128, 2, 2>(ctx, p)
                           : launch_tiles<TYPE, 64, 64, 2, 2>(ctx, p);
   }
@@ -1070,7 +1132,7 @@ int run_product(bdh_ctx *ctx, const Call &c, const Product &p, int64_t rows_out)
   if (!bdh_aligned(c.x, value_bytes(c.x_dtype)) || !bdh_aligned(p.out, value_bytes(p.out_dtype)) ||
       (p.gate && !bdh_aligned(p.gate, value_bytes(p.gate_dtype))))
     return bdh_fail(ctx, BDH_E_ALIGN, "rows, gate and out need the alignment of their values");
-  const Plan plan = plan_of(ctx, w, c.rows_in, p.offsets ? -1 : p.rows, c.x, c.x_dtype, c.x_stride);
+  const Plan plan = plan_of(ctx, w, c.rows_in, p.offsets ? -1 : p.rows, c.x, c.x_dtype, c.x_stride, p.gate);
   const size_t need = plan.bytes;
   if (need > 0 && (!c.workspace || c.workspace_bytes < need))
     return bdh_fail(ctx, BDH_E_INVAL, "workspace of %zu bytes, %zu are needed", c.workspace ? c.workspace_bytes : 0, need);
@@ -1138,7 +1200,7 @@ size_t bdh_packed_workspace(const bdh_ctx *ctx, const bdh_packed_weights *w, int
   if (!ctx || !w || (w->type != BDH_INT8 && w->type != BDH_BF16) || w->inner < 1 || w->outer < 1 || w->groups < 1 || rows_in <= 0 ||
       rows_of_group == 0 || !is_rows_type(x_dtype))
     return 0;
-  return plan_of(ctx, *w, rows_in, rows_of_group, x, x_dtype, x_stride).bytes;
+  return plan_of(ctx, *w, rows_in, rows_of_group, x, x_dtype, x_stride, false).bytes;  // a gate changes no size
 }
 
 int bdh_packed_product(bdh_ctx *ctx, const bdh_packed_weights *w, int64_t rows, const void *x, int x_dtype, int64_t x_stride, void *out,
