@@ -64,6 +64,9 @@ struct bdh_model {
   // creation for every batch that form is taken for: a decode step of such a model never allocates, and a captured one keeps
   // its buffer whatever runs later.  One buffer a model: its steps follow one another, captured ones too.
   float *phase_act = nullptr;
+  // packed projections (bdh_model_set_packed); null data where the model runs with its f32 weights
+  bdh_packed_weights packed_encoder{}, packed_encoder_v{}, packed_decoder{};
+  bool packed() const { return packed_encoder.data != nullptr; }
 };
 
 int bdh_fail(bdh_ctx *ctx, int status, const char *fmt, ...);
@@ -198,6 +201,11 @@ int bdh_launch_shared_steps(bdh_ctx *ctx, const SharedStepParams &p);
 int bdh_check_shared(bdh_ctx *ctx, int G, const int32_t *counts_host, int B, int h, int T, int Nq, int d, int rotary,
                      const void *rho, int rho_dtype, int capacity, const int32_t *lens_dev, int longest, const float *keys,
                      const float *values);
+
+// packed.hip: the projections through packed weights.  token_major: out is [B,T,h,N], the rows of the encoder E.
+int bdh_packed_check(bdh_ctx *ctx, const bdh_packed_weights *w);
+int bdh_launch_packed_relu_lowrank(bdh_ctx *ctx, const bdh_packed_weights *w, int B, int h_in, int T, const float *in, float threshold,
+                                   const float *gate, float *out, bool token_major, void *workspace, size_t workspace_bytes);
 
 struct ReluLowrankParams {
   int B, h_in, T, d, h, N;

@@ -59,6 +59,45 @@ int model_forward_impl(bdh_model *m, const int64_t *tokens, int B, int T, StateR
                        const int32_t *positions_dev, float *logits, int64_t *next_tokens, float *x_tap, float *viz,
                        bdh_model_logs *logs, const SharedStepParams *shared = nullptr);
 
+// The projections of a layer: through the model's packed weights where it has them.
+struct Projections {
+  bdh_model *m;
+  int B, T;
+  void *workspace;
+  size_t bytes;
+  // floats of scratch for the packed products of B x T tokens: the largest of their workspaces, and the rows that E leaves
+  static size_t floats(const bdh_model *m, int B, int T) {
+    if (!m->packed()) return 0;
+    const int64_t M = (int64_t)B * T, h = m->cfg.n_head, d = m->cfg.n_embd, K = h * m->cfg.latent;
+    const bdh_ctx *ctx = m->ctx;
+    const size_t most = std::max({bdh_packed_workspace(ctx, &m->packed_encoder, M, M, nullptr, BDH_F32, d),
+                                  bdh_packed_workspace(ctx, &m->packed_encoder_v, M * h, M, nullptr, BDH_F32, d),
+                                  bdh_packed_workspace(ctx, &m->packed_decoder, M, M, nullptr, BDH_F32, K)});
+    return bdh_align_up(M * d, 64) + bdh_align_up(most, 256) / sizeof(float);
+  }
+  int encode(const ReluLowrankParams &p) const {
+    if (!m->packed()) return bdh_launch_relu_lowrank(m->ctx, p);
+    if (p.active_blocks_host) return bdh_fail(m->ctx, BDH_E_UNSUPPORTED, "packed projections have no latent block patterns");
+    return bdh_launch_packed_relu_lowrank(m->ctx, p.gate ? &m->packed_encoder_v : &m->packed_encoder, B, p.h_in, T, p.in, p.threshold, p.gate,
+                                          p.out, p.gate != nullptr, scratch(), scratch_bytes());
+  }
+  // cur = LN(cur + LN(xy . decoder)); xy as encode leaves it, [B,T,h,N] with packed weights
+  int decode(const float *xy, float *cur, const DecoderHead *head) const {
+    const bdh_model_config &c = m->cfg;
+    if (!m->packed()) return bdh_launch_decoder_residual(m->ctx, B, T, c.n_head, c.latent, c.n_embd, xy, m->w.decoder, cur, head);
+    const int64_t M = (int64_t)B * T, K = (int64_t)c.n_head * c.latent;
+    float *rows = static_cast<float *>(workspace);
+    const int rc = bdh_packed_product(m->ctx, &m->packed_decoder, M, xy, BDH_F32, K, rows, BDH_F32, c.n_embd, scratch(), scratch_bytes());
+    if (rc != BDH_OK) return rc;
+    return bdh_launch_decoder_finalize_head(m->ctx, rows, 1, (int)M, c.n_embd, cur, head);
+  }
+
+ private:
+  size_t row_floats() const { return bdh_align_up((size_t)B * T * m->cfg.n_embd, 64); }
+  void *scratch() const { return static_cast<float *>(workspace) + row_floats(); }
+  size_t scratch_bytes() const { return bytes - sizeof(float) * row_floats(); }
+};
+
 }  // namespace
 
 // the update logs of a model's layers (bdh_model_forward_deferred): one bdh_state_log per layer
@@ -132,6 +171,33 @@ int bdh_model_destroy(bdh_model *m) {
   if (m->act) (void)hipFree(m->act);
   if (m->phase_act) (void)hipFree(m->phase_act);
   delete m;
+  return BDH_OK;
+}
+
+int bdh_model_set_packed(bdh_model *m, const bdh_packed_weights *encoder, const bdh_packed_weights *encoder_v,
+                         const bdh_packed_weights *decoder) {
+  if (!m) return BDH_E_INVAL;
+  bdh_ctx *ctx = m->ctx;
+  if (!encoder && !encoder_v && !decoder) {
+    m->packed_encoder = m->packed_encoder_v = m->packed_decoder = bdh_packed_weights{};
+    return BDH_OK;
+  }
+  if (!encoder || !encoder_v || !decoder) return bdh_fail(ctx, BDH_E_INVAL, "a model's projections are packed together or not at all");
+  const bdh_model_config &c = m->cfg;
+  for (const bdh_packed_weights *w : {encoder, encoder_v, decoder}) {
+    const int rc = bdh_packed_check(ctx, w);
+    if (rc != BDH_OK) return rc;
+  }
+  for (const bdh_packed_weights *w : {encoder, encoder_v})
+    if (w->groups != c.n_head || w->inner != c.n_embd || w->outer != c.latent)
+      return bdh_fail(ctx, BDH_E_SHAPE, "packed encoder [%d, %d, %d], the model's is [%d, %d, %d]", w->groups, w->inner, w->outer, c.n_head,
+                      c.n_embd, c.latent);
+  if (decoder->groups != 1 || decoder->inner != (int64_t)c.n_head * c.latent || decoder->outer != c.n_embd)
+    return bdh_fail(ctx, BDH_E_SHAPE, "packed decoder [%d, %d, %d], the model's is [1, %lld, %d]", decoder->groups, decoder->inner, decoder->outer,
+                    (long long)c.n_head * c.latent, c.n_embd);
+  m->packed_encoder = *encoder;
+  m->packed_encoder_v = *encoder_v;
+  m->packed_decoder = *decoder;
   return BDH_OK;
 }
 
@@ -237,7 +303,7 @@ int model_forward_impl(bdh_model *m, const int64_t *tokens, int B, int T, StateR
   // us per step, half the neurons firing, one launch | two per layer | kernel by kernel: W = 3 MiB 76|41|103 at B=1, 80|56|121
   // at B=42, 87|81|137 at B=127; 6.75 MiB 129|55|130 at B=1, 143|116|195 at B=64; 12 MiB 211|47|100 at B=1, 232|149|175 at
   // B=64; 96 MiB -|114|308 at B=1, -|309|470 at B=16, -|576|607 at B=32.
-  if (T == 1 && !x_tap && !viz && !logs && !shared && contiguous && ctx->opt_model_one_launch != 0) {
+  if (T == 1 && !x_tap && !viz && !logs && !shared && !m->packed() && contiguous && ctx->opt_model_one_launch != 0) {
     const int one_from = bdh_model_one_launch_from(c);
     const bool small = has_phase_act(c);
     const bool forced = ctx->opt_model_one_launch == 2 && one_from > 0;
@@ -270,7 +336,7 @@ int model_forward_impl(bdh_model *m, const int64_t *tokens, int B, int T, StateR
   // partials per head (N/128 rows of d floats) and 128 KiB of encoder partials (h*N/KB rows); beyond that the redundant
   // sums cost more than the two launches they replace (measured at d=512, h=8, N=16384: 2.97 against 2.87 ms per token).
   const int fused_kb = ctx->opt_model_fused_kb;
-  if (B == 1 && T == 1 && !x_tap && !viz && !logs && !shared && ctx->opt_model_fused_rows != 0 && c.rotary == BDH_ROPE &&
+  if (B == 1 && T == 1 && !x_tap && !viz && !logs && !shared && !m->packed() && ctx->opt_model_fused_rows != 0 && c.rotary == BDH_ROPE &&
       (d == 256 || d == 512) && N >= 2 && (N % 2) == 0 && (long)N * d <= (2L << 20) &&
       (long)h * N * d <= (long)fused_kb * (1L << 15)) {
     const int KB = fused_kb;
@@ -314,7 +380,8 @@ int model_forward_impl(bdh_model *m, const int64_t *tokens, int B, int T, StateR
   // activation scratch: cur [M,d] | x [B,h,T,N] | xy [B,h,T,N] | attn [B,h,T,d] | attn_ln [B,h,T,d] | last [h,d]
   const size_t n_cur = bdh_align_up(M * d, 64), n_x = bdh_align_up(M * h * N, 64), n_a = bdh_align_up(M * h * d, 64);
   const size_t n_last = viz ? bdh_align_up((size_t)h * d, 64) : 0;
-  int rc = ensure_act(m, sizeof(float) * (n_cur + 2 * n_x + 2 * n_a + n_last));
+  const size_t n_packed = Projections::floats(m, B, T);
+  int rc = ensure_act(m, sizeof(float) * (n_cur + 2 * n_x + 2 * n_a + n_last + n_packed));
   if (rc != BDH_OK) return rc;
   float *cur = static_cast<float *>(m->act);
   float *x = cur + n_cur;
@@ -322,6 +389,7 @@ int model_forward_impl(bdh_model *m, const int64_t *tokens, int B, int T, StateR
   float *attn = xy + n_x;
   float *attn_ln = attn + n_a;
   float *last = attn_ln + n_a;
+  const Projections project{m, B, T, last + n_last, sizeof(float) * n_packed};
 
   rc = bdh_launch_embed_ln(ctx, tokens, (int64_t)M, d, V, m->w.embed, cur);  // :319-322
   if (rc != BDH_OK) return rc;
@@ -329,7 +397,7 @@ int model_forward_impl(bdh_model *m, const int64_t *tokens, int B, int T, StateR
     float *x_l = x_tap ? x_tap + (size_t)l * M * h * N : x;
     // :337-351  x = relu(cur . encoder - thr)
     ReluLowrankParams px{B, 1, T, d, h, N, cur, m->w.encoder, nullptr, c.relu_threshold, 1, nullptr, 0, nullptr, x_l};
-    rc = bdh_launch_relu_lowrank(ctx, px);
+    rc = project.encode(px);
     if (rc != BDH_OK) return rc;
     // :353-359  recurrent attention (value = cur) and LayerNorm of its output
     if (shared) {  // the prompt's state is only read, the tokens go to the sequences' own keys and values
@@ -355,7 +423,7 @@ int model_forward_impl(bdh_model *m, const int64_t *tokens, int B, int T, StateR
     // :361-381  xy = x * relu(LN(attn) . encoder_v - thr)
     ReluLowrankParams py{B, h, T, d, h, N, attn_ln, m->w.encoder_v, nullptr, c.relu_threshold, 1, nullptr, 0, x_l, xy,
                          T > 1 && !x_tap && !viz};
-    rc = bdh_launch_relu_lowrank(ctx, py);
+    rc = project.encode(py);
     if (rc != BDH_OK) return rc;
     if (viz) {  // :386-434: first sequence, last token; the state is already this call's updated one
       float *vz = viz + (size_t)l * 4 * h * N;
@@ -367,9 +435,11 @@ int model_forward_impl(bdh_model *m, const int64_t *tokens, int B, int T, StateR
       if (rc != BDH_OK) return rc;
       ReluLowrankParams pv{1, h, 1, d, h, N, last, m->w.encoder_v, nullptr, c.relu_threshold, 1, nullptr, 0, nullptr,
                            vz + (size_t)h * N};
-      rc = bdh_launch_relu_lowrank(ctx, pv);
+      rc = m->packed() ? bdh_launch_packed_relu_lowrank(ctx, &m->packed_encoder_v, 1, h, 1, last, c.relu_threshold, nullptr, pv.out, false,
+                                                        project.workspace, project.bytes)
+                       : bdh_launch_relu_lowrank(ctx, pv);
       if (rc != BDH_OK) return rc;
-      rc = bdh_launch_gather_head_rows(ctx, xy, h, hs, off, N, vz + (size_t)2 * h * N);
+      rc = bdh_launch_gather_head_rows(ctx, xy, h, m->packed() ? N : hs, m->packed() ? (long)(T - 1) * h * N : off, N, vz + (size_t)2 * h * N);
       if (rc != BDH_OK) return rc;
       if (Nq == (size_t)N)
         rc = bdh_launch_rho_energy(ctx, B, h, N, d, st.rho(l), rho_dtype, st.stamps(l), m->slopes, position + T,
@@ -380,7 +450,7 @@ int model_forward_impl(bdh_model *m, const int64_t *tokens, int B, int T, StateR
     }
     // :383,436-441  cur = LN(cur + LN(mixed . decoder)); the last layer's launch also runs the output head (:446-449)
     const DecoderHead head{m->w.lm_head, T, V, logits, next_tokens};
-    rc = bdh_launch_decoder_residual(ctx, B, T, h, N, d, xy, m->w.decoder, cur, l == L - 1 ? &head : nullptr);
+    rc = project.decode(xy, cur, l == L - 1 ? &head : nullptr);
     if (rc != BDH_OK) return rc;
   }
   return BDH_OK;
@@ -560,13 +630,15 @@ int bdh_model_forward_fast_ex(bdh_model *m, const int64_t *tokens, int B, int T,
   const size_t M = (size_t)B * T;
   // activation scratch: cur [M,d] | x [B,h,T,N] | xy [B,h,T,N] | attn [B,h,T,d] | attn_ln [B,h,T,d]
   const size_t n_cur = bdh_align_up(M * d, 64), n_x = bdh_align_up(M * h * N, 64), n_a = bdh_align_up(M * h * d, 64);
-  int rc = ensure_act(m, sizeof(float) * (n_cur + 2 * n_x + 2 * n_a));
+  const size_t n_packed = Projections::floats(m, B, T);
+  int rc = ensure_act(m, sizeof(float) * (n_cur + 2 * n_x + 2 * n_a + n_packed));
   if (rc != BDH_OK) return rc;
   float *cur = static_cast<float *>(m->act);
   float *x = cur + n_cur;
   float *xy = x + n_x;
   float *attn = xy + n_x;
   float *attn_ln = attn + n_a;
+  const Projections project{m, B, T, attn_ln + n_a, sizeof(float) * n_packed};
   rc = bdh_launch_embed_ln(ctx, tokens, (int64_t)M, d, V, m->w.embed, cur);  // :97-100
   if (rc != BDH_OK) return rc;
   const int block = time_block_size > 0 ? time_block_size : 1;  // plain branch: element-wise tril(-1)
@@ -578,7 +650,7 @@ int bdh_model_forward_fast_ex(bdh_model *m, const int64_t *tokens, int B, int T,
   for (int l = 0; l < L; ++l) {  // :113
     ReluLowrankParams px{B, 1, T, d, h, N, cur, m->w.encoder, nullptr, c.relu_threshold, lat_block, latent_blocks_host,
                          n_latent_blocks, nullptr, x};
-    rc = bdh_launch_relu_lowrank(ctx, px);  // :114-129
+    rc = project.encode(px);  // :114-129
     if (rc != BDH_OK) return rc;
     // :131  Attention::forward: all tokens at once from position 0, row-normalised
     rc = bdh_fused_state_aligned(ctx, B, h, T, N, d, x, cur, m->freqs, c.rotary == BDH_ALIBI ? m->slopes : nullptr, block,
@@ -588,9 +660,9 @@ int bdh_model_forward_fast_ex(bdh_model *m, const int64_t *tokens, int B, int T,
     if (rc != BDH_OK) return rc;
     ReluLowrankParams py{B, h, T, d, h, N, attn_ln, m->w.encoder_v, nullptr, c.relu_threshold, lat_block, latent_blocks_host,
                          n_latent_blocks, x, xy, true};
-    rc = bdh_launch_relu_lowrank(ctx, py);  // :134-151
+    rc = project.encode(py);  // :134-151
     if (rc != BDH_OK) return rc;
-    rc = bdh_launch_decoder_residual(ctx, B, T, h, N, d, xy, m->w.decoder, cur);  // :153-162
+    rc = project.decode(xy, cur, nullptr);  // :153-162
     if (rc != BDH_OK) return rc;
   }
   return bdh_launch_lm_head(ctx, B, T, d, V, cur, m->w.lm_head, logits, nullptr);  // :164-168

@@ -275,6 +275,7 @@ struct Product {
   void *out;
   int out_dtype;
   long out_stride;
+  bool token_major;  // out is [row][head][N], not [row / T][head][row % T][N]
   int m_tiles, n_tiles;  // of a head, or of all groups
   // k cut into `splits` parts of kb_each blocks: sums of part i at parts[i][row of out][Nb * 64], each 32 bits
   int splits, kb_each;
@@ -332,10 +333,14 @@ struct Acc<BDH_BF16> {
   }
 };
 
-// sum s t, the smaller scale first: what is in between neither leaves the range of f32 where the result does not, nor is subnormal.
-__device__ __forceinline__ float scaled(float sum, float s, float t) { return sum * (t < s ? t : s) * (t < s ? s : t); }
-// Where the scales are like these, (sum s) t does as well, for half the operations.
+// sum s t.  Where a scale is far from 1 the smaller one goes first: what is in between then neither leaves the range of f32 where the
+// result does not, nor is subnormal.  Elsewhere (sum s) t does as well, for half the operations; which of the two it is is each pair's
+// own matter, so that a result does not depend on its neighbours.
 __device__ __forceinline__ bool plain_scale(float s) { return s == 0.0f || (s > 0x1p-60f && s < 0x1p60f); }
+__device__ __forceinline__ float scaled(float sum, float s, float t) {
+  const bool first = (plain_scale(s) && plain_scale(t)) || !(t < s);
+  return sum * (first ? s : t) * (first ? t : s);
+}
 
 // What comes behind the sums: nothing but the scales; ReLU alone; bias, threshold, ReLU and gate as they are given; nothing, where
 // the sums are parts of a longer k.
@@ -474,6 +479,11 @@ __device__ __forceinline__ unsigned int row_in_of(const Product &g, unsigned int
 __device__ __forceinline__ unsigned int row_out_of(const Product &g, unsigned int r, int group) {
   return g.offsets ? r : row_of(r, g.T, g.G, group);
 }
+// Number of the first value of a row in out, and of its gate.
+__device__ __forceinline__ long out_at(const Product &g, unsigned int r, int group) {
+  return g.token_major ? r * g.out_stride + (long)group * g.N : row_out_of(g, r, group) * g.out_stride;
+}
+__device__ __forceinline__ long gate_at(const Product &g, unsigned int r, int group) { return (long)row_out_of(g, r, group) * g.N; }
 
 // Which tile a workgroup takes: workgroups go to the eight XCDs in turn, so XCD i gets every eighth; it takes the i-th eighth of
 // the tiles, which go through the channels by panels of kPanel tiles of rows, so that what an XCD works on at a time shares its
@@ -590,8 +600,10 @@ __global__ __launch_bounds__(64 * WM * WN, tiles_a_cu(BM, BN) * WM * WN / 4) voi
   }
   long at[TM];
 #pragma unroll
-  for (int i = 0; i < TM; ++i)
-    at[i] = row_out_of(g, min(first + (wm * TM + i) * 16 + (lane & 15), last - 1), group) * (BEHIND == kParts ? g.Nb * 64L : g.out_stride);
+  for (int i = 0; i < TM; ++i) {
+    const int r = min(first + (wm * TM + i) * 16 + (lane & 15), last - 1);
+    at[i] = BEHIND == kParts ? row_out_of(g, r, group) * (g.Nb * 64L) : out_at(g, r, group);
+  }
   if (BEHIND == kParts) {
     acc_t *out = reinterpret_cast<acc_t *>(static_cast<char *>(g.parts) + 4 * split * g.rows_out * g.Nb * 64);
 #pragma unroll
@@ -633,17 +645,18 @@ __global__ __launch_bounds__(64 * WM * WN, tiles_a_cu(BM, BN) * WM * WN / 4) voi
     }
     float gate[BEHIND == kAll ? TM : 1][8];
     if (BEHIND == kAll && g.gate) {
-      if ((n_tile + 1) * BN <= g.N) {  // all of them on their way before the first is used
-        if (g.gate_dtype == BDH_F32) {
+      auto load = [&](int dtype, int left) {
 #pragma unroll
-          for (int i = 0; i < TM; ++i) load_some(g.gate, BDH_F32, at[i] + c.n, 8, gate[i]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < TM; ++i) load_some(g.gate, BDH_BF16, at[i] + c.n, 8, gate[i]);
+        for (int i = 0; i < TM; ++i) {
+          const long from = g.token_major ? gate_at(g, min(first + (wm * TM + i) * 16 + (lane & 15), last - 1), group) : at[i];
+          load_some(g.gate, dtype, from + c.n, left, gate[i]);
         }
+      };
+      if ((n_tile + 1) * BN <= g.N) {  // all of them on their way before the first is used
+        if (g.gate_dtype == BDH_F32) load(BDH_F32, 8);
+        else load(BDH_BF16, 8);
       } else if (c.left > 0) {
-#pragma unroll
-        for (int i = 0; i < TM; ++i) load_some(g.gate, g.gate_dtype, at[i] + c.n, c.left, gate[i]);
+        load(g.gate_dtype, c.left);
       }
     }
 #pragma unroll
@@ -711,14 +724,11 @@ __global__ __launch_bounds__(64 * W) void k_packed_few(Product g, RowsIn in) {
     // what comes behind the sums of 4 channels of a row a thread is asked for with them
     const int c4 = (threadIdx.x & 15) * 4, mine = threadIdx.x >> 4;
     const Channels<TYPE, BEHIND, 4> c(g, group, nb * 64 + c4);
-    unsigned int out_row[R];
     float gate[R][4];
 #pragma unroll
-    for (int k = 0; k < R; ++k) {
-      const int q = min(first + mine + k * 4 * W, last - 1);
-      out_row[k] = row_out_of(g, q, group);
-      if (BEHIND == kAll && g.gate && c.left > 0) load_some(g.gate, g.gate_dtype, out_row[k] * g.out_stride + c.n, c.left, gate[k]);
-    }
+    for (int k = 0; k < R; ++k)
+      if (BEHIND == kAll && g.gate && c.left > 0)
+        load_some(g.gate, g.gate_dtype, gate_at(g, min(first + mine + k * 4 * W, last - 1), group) + c.n, c.left, gate[k]);
     float up[MT];
     if constexpr (TYPE == BDH_INT8 && !PRE) {
       if (threadIdx.x < 16 * MT) s_top[threadIdx.x] = 0;
@@ -795,14 +805,14 @@ __global__ __launch_bounds__(64 * W) void k_packed_few(Product g, RowsIn in) {
 #pragma unroll
       for (int x = 1; x < W; ++x) sum += *reinterpret_cast<const acc_t *>(&s_sum[x][r][c4]);
       if constexpr (BEHIND == kParts) {
-        reinterpret_cast<acc_t *>(g.parts)[((split * g.rows_out + out_row[k]) * g.Nb + nb) * 16 + c4 / 4] = sum;
+        reinterpret_cast<acc_t *>(g.parts)[((split * g.rows_out + row_out_of(g, first + r, group)) * g.Nb + nb) * 16 + c4 / 4] = sum;
       } else {
         float scale = 1.0f, unused;
         if constexpr (TYPE == BDH_INT8) {
           scale_of(s_top[r], scale, unused);
         }
         float sums[4] = {(float)sum[0], (float)sum[1], (float)sum[2], (float)sum[3]};
-        finish<TYPE, BEHIND, false>(g, c, out_row[k] * g.out_stride + c.n, sums, gate[k], scale, false);
+        finish<TYPE, BEHIND, false>(g, c, out_at(g, first + r, group) + c.n, sums, gate[k], scale, false);
       }
     }
     if (first + 16 * MT < last) __syncthreads();
@@ -859,8 +869,9 @@ __global__ __launch_bounds__(256) void k_packed_finish(Product g) {
   const unsigned int row_in = g.h_in == 1 ? b / g.G * g.T + (r - b * g.T) : r;
   const Channels<TYPE, BEHIND, 4> c(g, head, n);
   float v[4] = {(float)sum[0], (float)sum[1], (float)sum[2], (float)sum[3]}, m[4];
-  if (BEHIND == kAll && g.gate) load_some(g.gate, g.gate_dtype, row * g.out_stride + n, c.left, m);
-  finish<TYPE, BEHIND, false>(g, c, row * g.out_stride + n, v, m, TYPE == BDH_INT8 ? g.row_scales[row_in] : 1.0f, false);
+  if (BEHIND == kAll && g.gate) load_some(g.gate, g.gate_dtype, row * g.N + n, c.left, m);
+  const long out = g.token_major ? (b / g.G * g.T + (r - b * g.T)) * g.out_stride + (long)head * g.N : row * g.out_stride;
+  finish<TYPE, BEHIND, false>(g, c, out + n, v, m, TYPE == BDH_INT8 ? g.row_scales[row_in] : 1.0f, false);
 }
 
 // ---- host ---------------------------------------------------------------------------------------
@@ -1003,7 +1014,8 @@ int launch_tiles(bdh_ctx *ctx, Product p) {
   if (tiles > 0x7fffffffL) return bdh_fail(ctx, BDH_E_SHAPE, "%ld tiles: the call is too large", tiles);
   p.m_tiles = (int)per_head;
   const dim3 grid((unsigned)tiles), threads(64 * WM * WN);
-  const bool past = bdh_aligned(p.out, 16) && p.out_stride * value_bytes(p.out_dtype) % 16 == 0;
+  const size_t row = value_bytes(p.out_dtype) * (size_t)(p.token_major ? p.N : p.out_stride);
+  const bool past = bdh_aligned(p.out, 16) && row % 16 == 0;
   if (p.splits > 1) {
     if constexpr (BM != 128 || BN != 128) hipLaunchKernelGGL((k_packed_tile<TYPE, kParts, false, BM, BN, WM, WN>), grid, threads, 0, ctx->stream, p);
   } else {
@@ -1137,14 +1149,14 @@ int run_product(bdh_ctx *ctx, const Call &c, const Product &p, int64_t rows_out)
   if (need > 0 && (!c.workspace || c.workspace_bytes < need))
     return bdh_fail(ctx, BDH_E_INVAL, "workspace of %zu bytes, %zu are needed", c.workspace ? c.workspace_bytes : 0, need);
   if (need > 0 && !bdh_aligned(c.workspace, 16)) return bdh_fail(ctx, BDH_E_ALIGN, "the workspace needs 16-byte alignment");
-  const size_t out_bytes = value_bytes(p.out_dtype) * ((size_t)(rows_out - 1) * p.out_stride + w.outer);
+  const size_t out_bytes = value_bytes(p.out_dtype) * (p.token_major ? (size_t)rows_out * w.outer : (size_t)(rows_out - 1) * p.out_stride + w.outer);
   const size_t x_bytes = value_bytes(c.x_dtype) * ((size_t)(c.rows_in - 1) * c.x_stride + w.inner);
   const size_t channels = sizeof(float) * (size_t)w.groups * w.outer;
   const struct {
     const void *p;
     size_t bytes;
   } reads[] = {{c.x, x_bytes}, {w.data, bdh_packed_bytes(w.type, w.groups, w.inner, w.outer)}, {w.scales, channels}, {p.bias, channels},
-               {p.gate, value_bytes(p.gate_dtype) * ((size_t)(rows_out - 1) * p.out_stride + w.outer)},
+               {p.gate, value_bytes(p.gate_dtype) * (size_t)rows_out * w.outer},
                {p.offsets, sizeof(int32_t) * ((size_t)w.groups + 1)}};
   for (const auto &r : reads)
     if (overlap(r.p, r.bytes, p.out, out_bytes) || (need > 0 && overlap(r.p, r.bytes, c.workspace, need)))
@@ -1153,12 +1165,51 @@ int run_product(bdh_ctx *ctx, const Call &c, const Product &p, int64_t rows_out)
   return w.type == BDH_INT8 ? launch_product<BDH_INT8>(ctx, c, plan, p) : launch_product<BDH_BF16>(ctx, c, plan, p);
 }
 
+int relu_lowrank(bdh_ctx *ctx, const bdh_packed_weights *w, int B, int h_in, int T, const void *in, int in_dtype, const float *bias,
+                 float threshold, const void *gate, int gate_dtype, void *out, int out_dtype, bool token_major, void *workspace,
+                 size_t workspace_bytes) {
+  const int rc = check_weights(ctx, w);
+  if (rc != BDH_OK) return rc;
+  if (B < 0 || T < 0) return bdh_fail(ctx, BDH_E_INVAL, "negative batch or time");
+  if (h_in != 1 && h_in != w->groups) return bdh_fail(ctx, BDH_E_SHAPE, "input of %d heads for weights of %d", h_in, w->groups);
+  if (bias && !bdh_aligned(bias, 4)) return bdh_fail(ctx, BDH_E_ALIGN, "bias needs the alignment of its values");
+  const int64_t bt = (int64_t)B * T;
+  if (bt > 0x7fffffffLL) return bdh_fail(ctx, BDH_E_SHAPE, "rows >= 2^31");
+  Product p{};
+  p.rows = (int)bt;
+  p.T = std::max(T, 1);
+  p.h_in = h_in;
+  p.bias = bias;
+  p.threshold = threshold;
+  p.relu = 1;
+  p.gate = gate;
+  p.gate_dtype = gate_dtype;
+  p.out = out;
+  p.out_dtype = out_dtype;
+  p.out_stride = token_major ? (long)w->groups * w->outer : w->outer;
+  p.token_major = token_major;
+  return run_product(ctx, Call{w, bt * h_in, in, in_dtype, w->inner, workspace, workspace_bytes}, p, bt * w->groups);
+}
+
 }  // namespace
+
+int bdh_packed_check(bdh_ctx *ctx, const bdh_packed_weights *w) {
+  const int rc = check_weights(ctx, w);
+  if (rc != BDH_OK) return rc;
+  if (!w->data || (w->type == BDH_INT8 && !w->scales)) return bdh_fail(ctx, BDH_E_INVAL, "null data pointer");
+  return bdh_aligned(w->data, 16) ? BDH_OK : bdh_fail(ctx, BDH_E_ALIGN, "packed weights need 16-byte alignment");
+}
+
+int bdh_launch_packed_relu_lowrank(bdh_ctx *ctx, const bdh_packed_weights *w, int B, int h_in, int T, const float *in, float threshold,
+                                   const float *gate, float *out, bool token_major, void *workspace, size_t workspace_bytes) {
+  return relu_lowrank(ctx, w, B, h_in, T, in, BDH_F32, nullptr, threshold, gate, BDH_F32, out, BDH_F32, token_major, workspace, workspace_bytes);
+}
 
 extern "C" {
 
 size_t bdh_packed_bytes(int type, int groups, int inner, int outer) {
-  if ((type != BDH_INT8 && type != BDH_BF16) || groups < 0 || inner < 1 || outer < 1) return 0;
+  const bdh_packed_weights w{type, groups, inner, outer, nullptr, nullptr};
+  if (check_weights(nullptr, &w) != BDH_OK) return 0;
   return (size_t)groups * (((size_t)outer + 63) / 64) * blocks_of_k(type, inner) * 4096;
 }
 
@@ -1224,26 +1275,7 @@ int bdh_packed_relu_lowrank(bdh_ctx *ctx, const bdh_packed_weights *w, int B, in
                             const float *bias, float threshold, const void *gate, int gate_dtype, void *out, int out_dtype,
                             void *workspace, size_t workspace_bytes) {
   if (!ctx) return BDH_E_INVAL;
-  const int rc = check_weights(ctx, w);
-  if (rc != BDH_OK) return rc;
-  if (B < 0 || T < 0) return bdh_fail(ctx, BDH_E_INVAL, "negative batch or time");
-  if (h_in != 1 && h_in != w->groups) return bdh_fail(ctx, BDH_E_SHAPE, "input of %d heads for weights of %d", h_in, w->groups);
-  if (bias && !bdh_aligned(bias, 4)) return bdh_fail(ctx, BDH_E_ALIGN, "bias needs the alignment of its values");
-  Product p{};
-  const int64_t bt = (int64_t)B * T;
-  if (bt > 0x7fffffffLL) return bdh_fail(ctx, BDH_E_SHAPE, "rows >= 2^31");
-  p.rows = bt;
-  p.T = std::max(T, 1);
-  p.h_in = h_in;
-  p.bias = bias;
-  p.threshold = threshold;
-  p.relu = 1;
-  p.gate = gate;
-  p.gate_dtype = gate_dtype;
-  p.out = out;
-  p.out_dtype = out_dtype;
-  p.out_stride = w->outer;
-  return run_product(ctx, Call{w, bt * h_in, in, in_dtype, w->inner, workspace, workspace_bytes}, p, bt * w->groups);
+  return relu_lowrank(ctx, w, B, h_in, T, in, in_dtype, bias, threshold, gate, gate_dtype, out, out_dtype, false, workspace, workspace_bytes);
 }
 
 int bdh_grouped_product(bdh_ctx *ctx, const bdh_packed_weights *w, int64_t rows, const int32_t *offsets_dev, const void *x, int x_dtype,

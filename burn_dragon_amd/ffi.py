@@ -37,7 +37,7 @@ EXPORTS = [
     "bdh_model_logs_create", "bdh_model_logs_destroy", "bdh_model_logs_pending", "bdh_model_forward_deferred",
     "bdh_model_flush", "bdh_model_forward_deferred_layers", "bdh_model_flush_layers",
     "bdh_packed_bytes", "bdh_pack_weights", "bdh_packed_workspace", "bdh_packed_product", "bdh_packed_relu_lowrank",
-    "bdh_grouped_product",
+    "bdh_grouped_product", "bdh_model_set_packed",
 ]
 
 
@@ -165,6 +165,7 @@ def load_library(path: Optional[str] = None) -> ctypes.CDLL:
     lib.bdh_packed_workspace.argtypes = [P, W, c_int64, c_int64, P, c_int, c_int64]
     lib.bdh_packed_product.argtypes = [P, W, c_int64, P, c_int, c_int64, P, c_int, c_int64, P, c_size_t]
     lib.bdh_packed_relu_lowrank.argtypes = [P, W, c_int, c_int, c_int, P, c_int, P, c_float, P, c_int, P, c_int, P, c_size_t]
+    lib.bdh_model_set_packed.argtypes = [P, W, W, W]
     lib.bdh_grouped_product.argtypes = [P, W, c_int64, P, P, c_int, c_int64, P, c_int, c_int64, P, c_size_t]
     for name in EXPORTS:
         fn = getattr(lib, name)

@@ -70,6 +70,7 @@ class BDH:
                                                      ctypes.byref(handle)))
         self.handle = handle
         self.latent_q = 2 * N if rot == RotaryEmbedding.POPE else N
+        self.packed = None  # pack_projections
         if self.alibi_lazy and rot != RotaryEmbedding.ALIBI:
             raise ValueError("alibi_lazy needs rotary_embedding = alibi")
         self._slopes = slopes
@@ -97,6 +98,19 @@ class BDH:
                 self.handle = None
         except Exception:
             pass
+
+    def pack_projections(self, dtype: Optional[torch.dtype] = torch.int8) -> None:
+        """The projections of every layer (encoder, encoder_v, decoder) through weights packed for the matrix cores, torch.int8
+        or torch.bfloat16 (packed.PackedWeights); None goes back to the f32 weights, which are kept.  Every call made
+        afterwards takes them.  For prompts, batches and models whose weights are long; a model that runs a decode step in
+        one launch, or two a layer, is faster without."""
+        packed = None
+        if dtype is not None:
+            from ..packed import PackedWeights
+
+            packed = [PackedWeights(self.params[n], dtype, self.ctx) for n in ("encoder", "encoder_v", "decoder")]
+        self.ctx.check(self.ctx.lib.bdh_model_set_packed(self.handle, *([None] * 3 if packed is None else [w._ref for w in packed])))
+        self.packed = packed
 
     def init_state(self) -> ModelState:
         """src/model/bdh.rs:254-256."""
@@ -385,7 +399,7 @@ class DecodeGraph:
     def __init__(self, model: BDH, state: ModelState, tokens: torch.Tensor):
         assert state.storage is not None, "run the prefill before capturing the decode step"
         model.flush_state(state)  # the captured step writes the state itself (the pending count of a log lives on the host)
-        self.model, self.state = model, state
+        self.model, self.state, self.packed = model, state, model.packed  # the weights it was captured with
         B = state.storage.shape[1]
         dev = model.device
         self.tokens = tokens.to(dev, torch.int64).reshape(B).clone()

@@ -710,6 +710,14 @@ int bdh_grouped_product(bdh_ctx *ctx, const bdh_packed_weights *weights, int64_t
                         const void *x, int x_dtype, int64_t x_stride, void *out, int out_dtype, int64_t out_stride,
                         void *workspace, size_t workspace_bytes);
 
+/* The projections of a model through packed weights: encoder and encoder_v [h,d,N], decoder [1,h*N,d] (of one type or
+ * several), all three, or all NULL to go back to the model's f32 weights.  Every bdh_model_forward* call made afterwards takes
+ * them; embedding, output head, attention and LayerNorms stay as they are.  The structs are copied, the packed data is the
+ * caller's and stays where it is while the model (or a graph captured of it) uses it.  A decode step then runs kernel by kernel
+ * whatever the model's size.  Latent block patterns (bdh_model_forward_fast_ex) are refused. */
+int bdh_model_set_packed(bdh_model *model, const bdh_packed_weights *encoder, const bdh_packed_weights *encoder_v,
+                         const bdh_packed_weights *decoder);
+
 /* Draws the next token of every sequence on the device.  Replaces the temperature division of
  * sample_next_token (src/generation.rs:117) and sample_from_logits_values (src/generation.rs:26-72),
  * which copy the logits to the host for every token: values = logits / temperature; with

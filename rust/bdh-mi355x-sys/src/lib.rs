@@ -239,6 +239,8 @@ extern "C" {
     pub fn bdh_grouped_product(ctx: *mut bdh_ctx, weights: *const bdh_packed_weights, rows: i64, offsets_dev: *const i32,
         x: *const c_void, x_dtype: c_int, x_stride: i64, out: *mut c_void, out_dtype: c_int, out_stride: i64,
         workspace: *mut c_void, workspace_bytes: usize) -> c_int;
+    pub fn bdh_model_set_packed(model: *mut bdh_model, encoder: *const bdh_packed_weights,
+        encoder_v: *const bdh_packed_weights, decoder: *const bdh_packed_weights) -> c_int;
     pub fn bdh_sample_top_k(ctx: *mut bdh_ctx, b: c_int, v: c_int, logits: *const f32, row_stride: i64,
         temperature: f32, top_k: c_int, uniforms: *const f32, next_tokens: *mut i64) -> c_int;
     pub fn bdh_probe_chunks(ctx: *mut bdh_ctx, region: *mut c_void, region_bytes: usize,
