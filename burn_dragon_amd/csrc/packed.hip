@@ -23,6 +23,7 @@ namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // rows start at any multiple of their values' size
 typedef unsigned int u32x4u __attribute__((ext_vector_type(4), aligned(2)));
@@ -154,9 +155,11 @@ __device__ __forceinline__ void load_values(const RowsIn &in, long row, int k, f
         }
       }
     }
-  } else {
+  } else {  // all asked for at once; those past the end repeat the last one until they are cleared
 #pragma unroll
-    for (int e = 0; e < PER; ++e) v[e] = k + e < in.K ? load_value(in.x, in.dtype, at + e) : 0.0f;
+    for (int e = 0; e < PER; ++e) v[e] = load_value(in.x, in.dtype, at + min(e, in.K - 1 - k));
+#pragma unroll
+    for (int e = 0; e < PER; ++e) v[e] = k + e < in.K ? v[e] : 0.0f;
   }
 }
 template <int PER>
@@ -182,7 +185,7 @@ __device__ __forceinline__ uint4 packed16(const float (&v)[PER], float up) {
 // what is behind them twice, the second time from a cache.
 template <int TYPE, typename X, int THR>
 __global__ __launch_bounds__(THR < 256 ? 256 : THR) void k_prepare_rows(RowsIn in, int Kb, long pitch, uint4 *__restrict__ q, float *__restrict__ scales) {
-  constexpr int ROWS = THR < 256 ? 256 / THR : 1, PER = TYPE == BDH_INT8 ? 16 : 8, HOLD = TYPE == BDH_INT8 ? (sizeof(X) == 2 ? 8 : 4) : 0;
+  constexpr int ROWS = THR < 256 ? 256 / THR : 1, PER = TYPE == BDH_INT8 ? 16 : 8, HOLD = TYPE != BDH_INT8 ? 0 : THR < 1024 ? 2 : sizeof(X) == 2 ? 8 : 4;
   typedef X piece __attribute__((ext_vector_type(PER), aligned(sizeof(X))));
   __shared__ unsigned int s_top[THR < 256 ? 4 : THR / 64];
   const long row = (long)blockIdx.x * ROWS + threadIdx.x / THR;
@@ -222,7 +225,7 @@ __global__ __launch_bounds__(THR < 256 ? 256 : THR) void k_prepare_rows(RowsIn i
         top = top_of<PER>(v, top);
       }
     }
-    for (int o = 32; o > 0; o >>= 1) top = max(top, (unsigned int)__shfl_xor((int)top, o));
+    for (int o = THR < 64 ? THR / 2 : 32; o > 0; o >>= 1) top = max(top, (unsigned int)__shfl_xor((int)top, o));
     if (THR > 64) {
       if ((threadIdx.x & 63) == 0) s_top[threadIdx.x >> 6] = top;
       __syncthreads();
@@ -407,22 +410,12 @@ __device__ __forceinline__ void load_some(const void *p, int dtype, long at, int
     }
   }
 }
-// Results are stored with the streaming hint where every row starts on 16 bytes: they are written once and, where they are many,
-// gone from the caches before anyone reads them (1554 rows of 4 heads of 8192 in f32, gated, 122 -> 91 us; 8191 rows of 2816 in
-// bf16 47 -> 43).  Rows that start anywhere share their lines' ends: there the hint costs (192 rows of 65601 33 -> 59 us).
-template <bool PAST, typename V>
-__device__ __forceinline__ void store(V v, void *p) {
-  if (PAST) __builtin_nontemporal_store(v, static_cast<V *>(p));
-  else *static_cast<V *>(p) = v;
-}
-
-// E neighbouring channels of a row, whose first value is number `at` of out (and gate): scales, bias, threshold, gate (m, where there is
-// one), and the one rounding where out is bf16.  plain: plain_scale holds for all of them (uniform over the wavefront).  A large output
-// counts by the operations here: each one a value costs 5 us where 1500 rows of 131072 are written in 165.
-template <int TYPE, int BEHIND, bool PAST, int E>
-__device__ __forceinline__ void finish(const Product &g, const Channels<TYPE, BEHIND, E> &c, long at, float (&v)[E], const float (&m)[E],
+// What becomes of the sums of E neighbouring channels of a row: scales, bias, threshold, ReLU, gate (m, where there is one).  plain:
+// plain_scale holds for all of them (uniform over the wavefront).  A large output counts by the operations here: each one a value
+// costs 5 us where 1500 rows of 131072 are written in 150.
+template <int TYPE, int BEHIND, int E>
+__device__ __forceinline__ void finish(const Product &g, const Channels<TYPE, BEHIND, E> &c, float (&v)[E], const float (&m)[E],
                                        float row_scale, bool plain) {
-  if (c.left <= 0) return;
   if (TYPE == BDH_INT8) {
     if (plain) {
 #pragma unroll
@@ -444,22 +437,52 @@ __device__ __forceinline__ void finish(const Product &g, const Channels<TYPE, BE
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] *= m[e];
   }
+}
+
+// 8 neighbouring channels of a row to out, of which `left` exist; the one rounding where out is bf16.  LINES: rows start with a line of
+// memory, and a lane has 8 channels or none.  Such results are stored with the streaming hint: they are written once and, where they are
+// many, gone from the caches before anyone reads them (1554 rows of 4 heads of 8192 in f32, gated, 122 -> 91 us; 8191 rows of 2816 in
+// bf16 47 -> 43).  Elsewhere pieces share lines, which the caches put together, and the hint costs (192 rows of 65601 33 -> 59 us).
+template <bool LINES>
+__device__ __forceinline__ void store8(float *o, int left, const float (&v)[8]) {
+  const f32x4 a = {v[0], v[1], v[2], v[3]}, b = {v[4], v[5], v[6], v[7]};
+  if (LINES) {
+    __builtin_nontemporal_store(a, reinterpret_cast<f32x4 *>(o));
+    __builtin_nontemporal_store(b, reinterpret_cast<f32x4 *>(o) + 1);
+  } else if (left >= 8) {
+    *reinterpret_cast<f32x4u *>(o) = a;
+    *reinterpret_cast<f32x4u *>(o + 4) = b;
+  } else {
+    for (int e = 0; e < left; ++e) o[e] = v[e];
+  }
+}
+template <bool LINES>
+__device__ __forceinline__ void store8(unsigned short *o, int left, const float (&v)[8]) {
+  const u32x4 w = {half2(v[0], v[1]), half2(v[2], v[3]), half2(v[4], v[5]), half2(v[6], v[7])};
+  if (LINES) {
+    __builtin_nontemporal_store(w, reinterpret_cast<u32x4 *>(o));
+  } else if (left >= 8) {
+    *reinterpret_cast<u32x4u *>(o) = w;
+  } else {
+    for (int e = 0; e < left; ++e) o[e] = (unsigned short)(w[e >> 1] >> (16 * (e & 1)));
+  }
+}
+
+// 4 neighbouring channels of a row to out, from number `at` on; the one rounding where out is bf16.
+template <int TYPE, int BEHIND>
+__device__ __forceinline__ void store4(const Product &g, const Channels<TYPE, BEHIND, 4> &c, long at, const float (&v)[4]) {
   if (g.out_dtype == BDH_F32) {
     float *o = static_cast<float *>(g.out) + at;
-    if (c.left >= E) {
-#pragma unroll
-      for (int q = 0; q < E; q += 4) store<PAST>(f32x4u{v[q], v[q + 1], v[q + 2], v[q + 3]}, o + q);
+    if (c.left >= 4) {
+      *reinterpret_cast<f32x4u *>(o) = f32x4u{v[0], v[1], v[2], v[3]};
     } else {
       for (int e = 0; e < c.left; ++e) o[e] = v[e];
     }
   } else {
-    unsigned int w[E / 2];
-#pragma unroll
-    for (int e = 0; e < E / 2; ++e) w[e] = half2(v[2 * e], v[2 * e + 1]);
+    const unsigned int w[2] = {half2(v[0], v[1]), half2(v[2], v[3])};
     unsigned short *o = static_cast<unsigned short *>(g.out) + at;
-    if (c.left >= E) {
-      if constexpr (E == 8) store<PAST>(u32x4u{w[0], w[1], w[2], w[3]}, o);
-      else store<PAST>(u32x2u{w[0], w[1]}, o);
+    if (c.left >= 4) {
+      *reinterpret_cast<u32x2u *>(o) = u32x2u{w[0], w[1]};
     } else {
       for (int e = 0; e < c.left; ++e) o[e] = (unsigned short)(w[e >> 1] >> (16 * (e & 1)));
     }
@@ -507,11 +530,14 @@ __device__ __forceinline__ void place_of(const Product &g, int &m_tile, int &n_t
 // reads of a fragment, rows 128 bytes apart, meet no bank twice.
 constexpr int tile_lds(int BM, int BN) { return (3 * BN / 16 + 2 * BM / 8) * 1024; }
 constexpr int tiles_a_cu(int BM, int BN) { return 160 * 1024 / tile_lds(BM, BN); }
-template <int TYPE, int BEHIND, bool PAST, int BM, int BN, int WM, int WN>
+template <int TYPE, int BEHIND, bool LINES, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN, tiles_a_cu(BM, BN) * WM * WN / 4) void k_packed_tile(Product g) {
   constexpr int W = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, CB = BN / 16, RB = BM / 8, CW = CB / W, CR = RB / W;
   static_assert(CB % W == 0 && RB % W == 0 && TN % 2 == 0 && BN % 64 == 0);
-  __shared__ __attribute__((aligned(1024))) unsigned char s_w[3][CB * 1024], s_r[2][RB * 1024];
+  constexpr int RING = (3 * CB + 2 * RB) * 1024;
+  __shared__ __attribute__((aligned(1024))) unsigned char s_ring[RING];
+  auto s_w = [&](int stage) { return s_ring + stage * CB * 1024; };
+  auto s_r = [&](int stage) { return s_ring + (3 * CB + stage * RB) * 1024; };
   typedef typename Acc<TYPE>::type acc_t;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % WM, wn = wave / WM;
@@ -547,14 +573,14 @@ __global__ __launch_bounds__(64 * WM * WN, tiles_a_cu(BM, BN) * WM * WN / 4) voi
   auto copy_w = [&](int stage) {
 #pragma unroll
     for (int c = 0; c < CW; ++c) {
-      bdh_copy_to_lds(from_w[c], &s_w[stage][(wave + c * W) * 1024]);
+      bdh_copy_to_lds(from_w[c], s_w(stage) + (wave + c * W) * 1024);
       from_w[c] += 4096;
     }
   };
   auto copy_r = [&](int stage) {
 #pragma unroll
     for (int c = 0; c < CR; ++c) {
-      bdh_copy_to_lds(from_r[c], &s_r[stage][(wave + c * W) * 1024]);
+      bdh_copy_to_lds(from_r[c], s_r(stage) + (wave + c * W) * 1024);
       from_r[c] += 128;
     }
   };
@@ -573,10 +599,10 @@ __global__ __launch_bounds__(64 * WM * WN, tiles_a_cu(BM, BN) * WM * WN / 4) voi
   auto step = [&](int half, int rows) {
     i32x4 fw[TN], fr[TM];
 #pragma unroll
-    for (int j = 0; j < TN; ++j) fw[j] = *reinterpret_cast<const i32x4 *>(&s_w[stage][(wn * TN + j) * 1024 + lane * 16]);
+    for (int j = 0; j < TN; ++j) fw[j] = *reinterpret_cast<const i32x4 *>(s_w(stage) + (wn * TN + j) * 1024 + lane * 16);
 #pragma unroll
     for (int i = 0; i < TM; ++i)
-      fr[i] = *reinterpret_cast<const i32x4 *>(&s_r[rows][(wm * TM + i) * 2048 + (half ? at_r ^ 64 : at_r)]);
+      fr[i] = *reinterpret_cast<const i32x4 *>(s_r(rows) + (wm * TM + i) * 2048 + (half ? at_r ^ 64 : at_r));
 #pragma unroll
     for (int j = 0; j < TN; ++j)
 #pragma unroll
@@ -598,83 +624,88 @@ __global__ __launch_bounds__(64 * WM * WN, tiles_a_cu(BM, BN) * WM * WN / 4) voi
     if (more) copy_w(ahead);
     step(1, rows);
   }
-  long at[TM];
-#pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const int r = min(first + (wm * TM + i) * 16 + (lane & 15), last - 1);
-    at[i] = BEHIND == kParts ? row_out_of(g, r, group) * (g.Nb * 64L) : out_at(g, r, group);
-  }
   if (BEHIND == kParts) {
     acc_t *out = reinterpret_cast<acc_t *>(static_cast<char *>(g.parts) + 4 * split * g.rows_out * g.Nb * 64);
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const int channel = n_tile * BN + (wn * TN + (j & ~1)) * 16 + 8 * (lane >> 4) + 4 * (j & 1);
-      if (channel >= g.Nb * 64) continue;
+    for (int i = 0; i < TM; ++i) {
+      const int r = first + (wm * TM + i) * 16 + (lane & 15);
+      if (r >= last) continue;
+      const long at = row_out_of(g, r, group) * (g.Nb * 64L);
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
-        if (first + (wm * TM + i) * 16 + (lane & 15) < last) out[(at[i] + channel) >> 2] = acc[i][j];
+      for (int j = 0; j < TN; ++j) {
+        const int channel = n_tile * BN + (wn * TN + (j & ~1)) * 16 + 8 * (lane >> 4) + 4 * (j & 1);
+        if (channel < g.Nb * 64) out[(at + channel) >> 2] = acc[i][j];
+      }
     }
     return;
   }
-  float *s_scale = reinterpret_cast<float *>(s_w), *s_bias = s_scale + BM + BN;  // the ring is free
+  // The ring is free: scales, biases and places of the rows.
+  long *s_at = reinterpret_cast<long *>(s_ring);
+  float *s_scale = reinterpret_cast<float *>(s_at + BM), *s_bias = s_scale + BM + BN;
   int *s_plain = reinterpret_cast<int *>(s_bias + BN);
-  if (TYPE == BDH_INT8 || BEHIND == kAll) {
-    __syncthreads();
-    if (threadIdx.x < BM + BN) s_scale[threadIdx.x] = mine;
-    if (threadIdx.x < BN) s_bias[threadIdx.x] = bias;
-    const bool all = __ballot(plain_scale(mine)) == ~0ull;
-    if (lane == 0) s_plain[wave] = all;
-    __syncthreads();
-  }
+  __syncthreads();
+  if (threadIdx.x < BM + BN) s_scale[threadIdx.x] = mine;
+  if (threadIdx.x < BN) s_bias[threadIdx.x] = bias;
+  if (threadIdx.x < BM) s_at[threadIdx.x] = out_at(g, min(first + (int)threadIdx.x, last - 1), group) + n_tile * BN;
+  const bool all = __ballot(plain_scale(mine)) == ~0ull;
+  if (lane == 0) s_plain[wave] = all;
+  __syncthreads();
   bool plain = true;
+#pragma unroll
+  for (int w = 0; w < W; ++w) plain = plain && s_plain[w];
+  const long *place = s_at + wm * TM * 16 + (lane & 15);
   float row_scale[TM];
-  if (TYPE == BDH_INT8) {
 #pragma unroll
-    for (int w = 0; w < W; ++w) plain = plain && s_plain[w];
+  for (int i = 0; i < TM; ++i) row_scale[i] = TYPE == BDH_INT8 ? s_scale[BN + (wm * TM + i) * 16 + (lane & 15)] : 1.0f;
+  auto store = [&](auto type) {
+    typedef decltype(type) OUT;
 #pragma unroll
-    for (int i = 0; i < TM; ++i) row_scale[i] = s_scale[BN + (wm * TM + i) * 16 + (lane & 15)];
-  }
+    for (int j = 0; j < TN; j += 2) {
+      const int channel = (wn * TN + j) * 16 + 8 * (lane >> 4);
+      Channels<TYPE, BEHIND, 8> c(n_tile * BN + channel, g.N);
+      if (c.left <= 0) continue;
 #pragma unroll
-  for (int j = 0; j < TN; j += 2) {
-    const int channel = (wn * TN + j) * 16 + 8 * (lane >> 4);
-    Channels<TYPE, BEHIND, 8> c(n_tile * BN + channel, g.N);
+      for (int e = 0; e < 8; ++e) {
+        if (TYPE == BDH_INT8) c.scale[e] = s_scale[channel + e];
+        if (BEHIND == kAll) c.bias[e] = s_bias[channel + e];
+      }
+      constexpr int AT_ONCE = TM * TN < 16 ? TM : 1;  // gates on their way before the first is used: as the registers allow
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (TYPE == BDH_INT8) c.scale[e] = s_scale[channel + e];
-      if (BEHIND == kAll) c.bias[e] = s_bias[channel + e];
-    }
-    float gate[BEHIND == kAll ? TM : 1][8];
-    if (BEHIND == kAll && g.gate) {
-      auto load = [&](int dtype, int left) {
+      for (int i0 = 0; i0 < TM; i0 += AT_ONCE) {
+        float gate[BEHIND == kAll ? AT_ONCE : 1][8];
+        if (BEHIND == kAll && g.gate) {
+          auto load = [&](int dtype, int left) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-          const long from = g.token_major ? gate_at(g, min(first + (wm * TM + i) * 16 + (lane & 15), last - 1), group) : at[i];
-          load_some(g.gate, dtype, from + c.n, left, gate[i]);
+            for (int i = 0; i < AT_ONCE; ++i) {
+              const int r = min(first + (wm * TM + i0 + i) * 16 + (lane & 15), last - 1);
+              load_some(g.gate, dtype, (g.token_major ? gate_at(g, r, group) + n_tile * BN : place[(i0 + i) * 16]) + channel, left, gate[i]);
+            }
+          };
+          if (!LINES && c.left < 8) load(g.gate_dtype, c.left);
+          else if (g.gate_dtype == BDH_F32) load(BDH_F32, 8);
+          else load(BDH_BF16, 8);
         }
-      };
-      if ((n_tile + 1) * BN <= g.N) {  // all of them on their way before the first is used
-        if (g.gate_dtype == BDH_F32) load(BDH_F32, 8);
-        else load(BDH_BF16, 8);
-      } else if (c.left > 0) {
-        load(g.gate_dtype, c.left);
+#pragma unroll
+        for (int i = i0; i < i0 + AT_ONCE; ++i) {
+          if (first + (wm * TM + i) * 16 + (lane & 15) >= last) continue;
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = (float)acc[i][j + (e >> 2)][e & 3];
+          finish<TYPE, BEHIND>(g, c, v, gate[BEHIND == kAll ? i - i0 : 0], row_scale[i], plain);
+          store8<LINES>(static_cast<OUT *>(g.out) + place[i * 16] + channel, c.left, v);
+        }
       }
     }
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-      if (first + (wm * TM + i) * 16 + (lane & 15) < last) {
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = (float)acc[i][j + (e >> 2)][e & 3];
-        finish<TYPE, BEHIND, PAST>(g, c, at[i] + c.n, v, gate[BEHIND == kAll ? i : 0], row_scale[i], plain);
-      }
-  }
+  };
+  if (g.out_dtype == BDH_F32) store(float{});
+  else store((unsigned short)0);
 }
 
 // Few rows meet many weights: the weights are streamed, past LDS, and the rows are brought to 8 bits (or bf16) on their way.  A
-// workgroup takes 64 channels of a group, its W wavefronts every W-th block of k; 16 * MT rows at a time.  All that a wavefront has
-// of k, up to U blocks of weights and rows, is asked for at once, and the largest magnitude of a row is a maximum over the
-// wavefronts in LDS; the wavefronts' sums are added up in LDS in their order.  PRE: the rows are prepared ones, for k so long that a row's
-// largest magnitude is looked for by a launch of its own and k is cut into parts.
+// workgroup takes 16 * MT rows and 64 channels, its W wavefronts every W-th block of k.  All that a wavefront has of k, up to U blocks of
+// weights and rows, is asked for at once, and the largest magnitude of a row is a maximum over the wavefronts in LDS; the
+// wavefronts' sums are added up in LDS in their order.  PRE: the rows are prepared ones, or bf16 that needs no preparation.  With
+// kParts and 8 bits, the rows' largest magnitudes come from a launch before.
 template <int TYPE, int BEHIND, int MT, int W, int U, bool PRE>
 __global__ __launch_bounds__(64 * W) void k_packed_few(Product g, RowsIn in) {
   constexpr int PER = TYPE == BDH_INT8 ? 16 : 8, LD = 68, ROUNDS = 16 * MT * 16 / (64 * W);
@@ -684,26 +715,19 @@ __global__ __launch_bounds__(64 * W) void k_packed_few(Product g, RowsIn in) {
   __shared__ unsigned int s_top[16 * MT];
   __shared__ __attribute__((aligned(16))) int s_sum[W][16 * MT][LD];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const unsigned int rest = blockIdx.x / (unsigned int)g.Nb;
-  const int nb = blockIdx.x - rest * g.Nb, split = rest / (unsigned int)g.G, group = rest - split * g.G;
-  int first = 0, last = g.rows;
-  if (g.offsets) {  // the running maximum of the offsets up to the group's first and last row
-    int a = 0, b = 0;
-    for (int i = lane; i <= group + 1; i += 64) {
-      const int o = min(max(g.offsets[i], 0), g.rows);
-      b = max(b, o);
-      if (i <= group) a = max(a, o);
-    }
-    for (int o = 32; o > 0; o >>= 1) {
-      a = max(a, __shfl_xor(a, o));
-      b = max(b, __shfl_xor(b, o));
-    }
-    first = __builtin_amdgcn_readfirstlane(a);
-    last = __builtin_amdgcn_readfirstlane(b);
+  const unsigned int rest = blockIdx.x / (unsigned int)g.Nb, m_all = g.offsets ? g.m_tiles : g.m_tiles * g.G;
+  const int nb = blockIdx.x - rest * g.Nb, split = rest / m_all, m_tile = rest - split * m_all;
+  int group = 0, first, last;
+  if (g.offsets) {
+    if (!find_tile(g.offsets, g.G, g.rows, 16 * MT, m_tile, group, first, last)) return;
+  } else {
+    group = m_tile / g.m_tiles;
+    first = (m_tile - group * g.m_tiles) * 16 * MT;
+    last = g.rows;
   }
   const int kb0 = split * g.kb_each, kb1 = min(kb0 + g.kb_each, g.Kb);
   const i32x4 *w = reinterpret_cast<const i32x4 *>(g.w) + ((long)group * g.Nb + nb) * g.Kb * 256 + lane;
-  for (; first < last; first += 16 * MT) {
+  {
     unsigned int row[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) row[i] = row_in_of(g, min(first + i * 16 + (lane & 15), last - 1), group);
@@ -740,7 +764,7 @@ __global__ __launch_bounds__(64 * W) void k_packed_few(Product g, RowsIn in) {
           atomicMax(&s_top[r], g.tops[(long)row_in_of(g, first + r, group) * g.top_parts + (t - r * g.top_parts)]);
         }
         __syncthreads();
-        if (split == 0 && nb == 0)  // for k_packed_finish
+        if (split == 0 && nb == 0 && (g.h_in > 1 || group == 0))  // for k_packed_finish
           for (int t = threadIdx.x; t < n; t += 64 * W) {
             float scale, unused;
             scale_of(s_top[t], scale, unused);
@@ -809,13 +833,15 @@ __global__ __launch_bounds__(64 * W) void k_packed_few(Product g, RowsIn in) {
       } else {
         float scale = 1.0f, unused;
         if constexpr (TYPE == BDH_INT8) {
-          scale_of(s_top[r], scale, unused);
+          if constexpr (PRE) scale = g.row_scales[row_in_of(g, first + r, group)];
+          else scale_of(s_top[r], scale, unused);
         }
         float sums[4] = {(float)sum[0], (float)sum[1], (float)sum[2], (float)sum[3]};
-        finish<TYPE, BEHIND, false>(g, c, out_at(g, first + r, group) + c.n, sums, gate[k], scale, false);
+        if (c.left <= 0) continue;
+        finish<TYPE, BEHIND>(g, c, sums, gate[k], scale, false);
+        store4(g, c, out_at(g, first + r, group) + c.n, sums);
       }
     }
-    if (first + 16 * MT < last) __syncthreads();
   }
 }
 
@@ -848,15 +874,14 @@ __global__ __launch_bounds__(256) void k_packed_finish(Product g) {
   const long part = g.rows_out * g.Nb * 16;
   const acc_t *p = static_cast<const acc_t *>(g.parts) + (row * g.Nb * 64 + n) / 4;
   acc_t sum = acc_t{};
-  int i = lane;
-  for (; i + 7 * LANES < g.splits; i += 8 * LANES) {  // eight parts on their way at a time
+  for (int i = lane; i < g.splits; i += 8 * LANES) {  // eight parts on their way at a time
     acc_t a[8];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) a[u] = p[(i + u * LANES) * part];
+    for (int u = 0; u < 8; ++u) a[u] = p[min(i + u * LANES, g.splits - 1) * part];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) sum += a[u];
+    for (int u = 0; u < 8; ++u)
+      if (i + u * LANES < g.splits) sum += a[u];
   }
-  for (; i < g.splits; i += LANES) sum += p[i * part];
   if (LANES > 1) {
     s_sum[lane][at] = sum;
     __syncthreads();
@@ -871,7 +896,8 @@ __global__ __launch_bounds__(256) void k_packed_finish(Product g) {
   float v[4] = {(float)sum[0], (float)sum[1], (float)sum[2], (float)sum[3]}, m[4];
   if (BEHIND == kAll && g.gate) load_some(g.gate, g.gate_dtype, row * g.N + n, c.left, m);
   const long out = g.token_major ? (b / g.G * g.T + (r - b * g.T)) * g.out_stride + (long)head * g.N : row * g.out_stride;
-  finish<TYPE, BEHIND, false>(g, c, out + n, v, m, TYPE == BDH_INT8 ? g.row_scales[row_in] : 1.0f, false);
+  finish<TYPE, BEHIND>(g, c, v, m, TYPE == BDH_INT8 ? g.row_scales[row_in] : 1.0f, false);
+  store4(g, c, out + n, v);
 }
 
 // ---- host ---------------------------------------------------------------------------------------
@@ -916,61 +942,75 @@ struct Plan {
   size_t scales, tops, parts, bytes;  // where in the workspace the rows' scales, those magnitudes and the parts' sums lie, and its size
 };
 
+// The tiles that cost least, and the number of parts of k.  A round is as many tiles as the CUs hold at a time.  A step of it (64 bytes
+// of k) takes `step` us (8192 x 8192 x 8192 in 8 bits: 128x256 445 us, 4 rounds of 128 steps; 64x128 640, 64x64 825, 256x256 440,
+// 128x128 574), its beginning and end `ends` (1500 x 512 x 131072: 12 rounds of 8 steps of 128x256 155 us, of 256x256 177, 24 of 64x128
+// 207); a CU that has fewer tiles than it holds takes less.  Parts are written and read once.
+void choose_tiles(const bdh_ctx *ctx, const bdh_packed_weights &w, int64_t rows, bool grouped, bool gated, int Kb, Plan &p) {
+  // Gates want registers beside the sums, all of them on their way at once: 128x128 by 8 wavefronts has them (1554 rows of 4 heads of
+  // 8192, bf16, K 256 118 -> 108; 1500 rows in 8 bits, K 512 131 -> 100), while k is so short that they count (bf16, K 1024 155 | 160).
+  const bool gates = gated && Kb < 32;
+  const struct {
+    int bm, bn;
+    double step, ends;
+  } shapes[] = {{128, 256, 0.87, 6.0}, {64, 128, 0.70, 3.0}, {64, 64, 0.50, 2.0}, {256, 256, 0.80, 8.0}, {128, 128, 0.56, 3.0}};
+  double best = 0.0;
+  for (const auto &t : shapes) {
+    if (gates ? t.bn == 256 : t.bm == 128 && t.bn == 128) continue;
+    const int64_t n = (w.outer + t.bn - 1) / t.bn, m = (rows + t.bm - 1) / t.bm;
+    const int64_t tiles = grouped ? (m + w.groups / 2) * n : m * w.groups * n;
+    const int held = tiles_a_cu(t.bm, t.bn);
+    for (int splits : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32}) {
+      const int each = ((Kb + splits - 1) / splits + 1) / 2 * 2;
+      if (splits > 1 && (grouped || gates || each < 8)) break;
+      const double a_cu = (double)tiles * splits / ctx->n_cu, whole = floor(a_cu / held), rest = ceil(a_cu - whole * held);
+      double cost = (whole + (rest > 0 ? 0.2 + 0.8 * rest / held : 0.0)) * (each * t.step + t.ends);
+      if (splits > 1) cost += 4.0 + 8.0 * splits * rows * w.groups * w.outer / 4.6e6;
+      if (p.bm == 0 || cost < best) {
+        best = cost;
+        p.bm = t.bm;
+        p.bn = t.bn;
+        p.kb_each = each;
+        p.splits = (Kb + each - 1) / each;
+      }
+    }
+  }
+}
+
 Plan plan_of(const bdh_ctx *ctx, const bdh_packed_weights &w, int64_t rows_in, int64_t rows_of_group, const void *x, int x_dtype,
              int64_t x_stride, bool gated) {
   Plan p{};
   const bool grouped = rows_of_group < 0;
   p.direct = rows_as_they_are(w.type, w.inner, x, x_dtype, x_stride);
-  const int64_t rows = grouped ? rows_in : rows_of_group;
+  const int64_t rows = grouped ? rows_in : rows_of_group, groups = std::max(w.groups, 1);
   const int Kb = blocks_of_k(w.type, w.inner);
-  const int64_t Nb = (w.outer + 63) / 64, blocks = Nb * w.groups;
+  const int64_t Nb = (w.outer + 63) / 64, a_group = grouped ? (rows + groups - 1) / groups : rows;
   p.splits = 1;
   p.kb_each = Kb;
-  p.few = rows <= 64;
+  p.mt = a_group <= 16 ? 1 : a_group <= 32 ? 2 : 4;
+  const int64_t tiles = grouped ? rows / (16 * p.mt) + groups : (rows + 16 * p.mt - 1) / (16 * p.mt) * groups, blocks = tiles * Nb;
+  p.waves = Kb > 4 && (Kb <= 8 || p.mt == 4 || blocks < ctx->n_cu) ? 8 : 4;
+  const int at_once = p.waves * (p.mt == 1 ? 4 : p.mt == 2 ? 2 : 1);  // blocks of k that a workgroup has on their way
+  // Streamed: few rows (33 to 64 of them only where that takes one workgroup a CU: 56 rows of 96, 4 heads of 10501 27 us, prepared and in
+  // tiles 17), or so little work that a launch for the rows and one for tiles would be most of it (159 x 516 x 40 15 us | 16; with two
+  // turns of k no longer: 2904 x 932 x 104 24 | 17).
+  p.few = rows <= 32 || (rows <= 64 && blocks < ctx->n_cu) || (grouped && a_group <= 4) || (blocks <= 2 * ctx->n_cu && Kb <= at_once);
   if (p.few) {
-    const int64_t a_group = grouped ? (rows + std::max(w.groups, 1) - 1) / std::max(w.groups, 1) : rows;
-    p.mt = a_group <= 16 ? 1 : a_group <= 32 ? 2 : 4;
-    p.waves = p.mt < 4 && Kb > 4 && (Kb <= 8 || blocks < ctx->n_cu) ? 8 : 4;
-    if (!grouped && Kb > 16 * p.waves && blocks < ctx->n_cu) {  // fewer workgroups than CUs, and more of k than they have on their way
+    const int turns = (Kb + at_once - 1) / at_once;
+    if (turns > 2 && !grouped && blocks < ctx->n_cu) {
+      // parts of k, as many as fill the chip twice, at least a block of k a wavefront
       p.waves = 4;
       const int64_t most = (Kb + 3) / 4, want = (2 * ctx->n_cu + blocks - 1) / blocks, splits = std::min(most, want);
       p.kb_each = (int)((Kb + splits - 1) / splits + 1) / 2 * 2;
       p.splits = (Kb + p.kb_each - 1) / p.kb_each;
       if (w.type == BDH_INT8) p.top_parts = (w.inner + 4095) / 4096;
+    } else if (turns > 2 && p.mt > 1) {
+      p.prepared = !p.direct;  // every workgroup would bring the same rows to 8 bits
     }
     p.one = (p.splits > 1 ? p.kb_each : Kb) <= p.waves || p.mt == 4;
   } else {
     p.prepared = !p.direct;
-    const int64_t heads = grouped ? 1 : w.groups;
-    auto tiles = [&](int bm, int bn) {
-      const int64_t n = (w.outer + bn - 1) / bn;
-      return grouped ? ((rows + bm - 1) / bm + w.groups / 2) * n : (rows + bm - 1) / bm * heads * n;
-    };
-    // The tile whose rounds over the chip cost least: a round is as many as the CUs hold at a time, a value of a smaller tile costs more
-    // (8192 x 8192 x 8192 in 8 bits | bf16, us: 128x256 440 | 830, 64x128 640 | 1500, 64x64 more still).
-    // Gates want registers beside the sums, all of them on their way at once: 128x128 by 8 wavefronts has them (1554 rows of 4 heads of
-    // 8192, bf16, K 256 118 -> 108; 1500 rows in 8 bits, K 512 131 -> 100), while k is so short that they count (bf16, K 1024 155 | 160).
-    const bool gates = gated && Kb < 32;
-    const struct {
-      int bm, bn;
-      double value;
-    } shapes[] = {{128, gates ? 128 : 256, 1.0}, {64, 128, 1.3}, {64, 64, 2.0}, {256, 256, 0.95}};
-    double best = 0.0;
-    for (const auto &t : shapes) {
-      const int64_t each = tiles_a_cu(t.bm, t.bn), at_once = each * ctx->n_cu;
-      const double cost = (double)((tiles(t.bm, t.bn) + at_once - 1) / at_once) * each * t.bm * t.bn * t.value;
-      if (t.bm == 256 && (Kb < 128 || gates)) continue;  // one workgroup a CU: nothing covers its beginning and end
-      if (p.bm == 0 || cost < best) best = cost, p.bm = t.bm, p.bn = t.bn;
-    }
-    if (!grouped && tiles(64, 64) < 2 * ctx->n_cu && Kb >= 32) {
-      if (tiles(256, 256) * (Kb / 64) >= ctx->n_cu) p.bm = 256, p.bn = 256;
-      else if (tiles(128, 256) * (Kb / 16) >= 2 * ctx->n_cu) p.bm = 128, p.bn = 256;
-      else p.bm = 64, p.bn = 64;
-      const int64_t each = tiles_a_cu(p.bm, p.bn), want = (each * ctx->n_cu) / tiles(p.bm, p.bn), most = Kb / 16;
-      const int64_t splits = std::max<int64_t>(1, std::min(want, most));
-      p.kb_each = (int)((Kb + splits - 1) / splits + 1) / 2 * 2;
-      p.splits = (Kb + p.kb_each - 1) / p.kb_each;
-    }
+    choose_tiles(ctx, w, rows, grouped, gated, Kb, p);
   }
   size_t at = 0;
   if (p.prepared || p.top_parts) {
@@ -988,13 +1028,16 @@ Plan plan_of(const bdh_ctx *ctx, const bdh_packed_weights &w, int64_t rows_in, i
 
 template <int TYPE, typename X>
 int launch_prepare(bdh_ctx *ctx, const RowsIn &in, int Kb, uint4 *q, float *scales) {
-  const unsigned int rows = (unsigned)in.rows;
-  if (in.K <= 2048)
-    hipLaunchKernelGGL((k_prepare_rows<TYPE, X, 64>), dim3((rows + 3) / 4), dim3(256), 0, ctx->stream, in, Kb, pitch_of(Kb), q, scales);
-  else if (in.K <= 16384)
-    hipLaunchKernelGGL((k_prepare_rows<TYPE, X, 256>), dim3(rows), dim3(256), 0, ctx->stream, in, Kb, pitch_of(Kb), q, scales);
-  else
-    hipLaunchKernelGGL((k_prepare_rows<TYPE, X, 1024>), dim3(rows), dim3(1024), 0, ctx->stream, in, Kb, pitch_of(Kb), q, scales);
+  const unsigned int rows = (unsigned int)in.rows;
+  auto launch = [&](auto threads) {  // a row
+    constexpr int THR = decltype(threads)::value, ROWS = THR < 256 ? 256 / THR : 1;
+    hipLaunchKernelGGL((k_prepare_rows<TYPE, X, THR>), dim3((rows + ROWS - 1) / ROWS), dim3(THR < 256 ? 256 : THR), 0, ctx->stream, in, Kb,
+                       pitch_of(Kb), q, scales);
+  };
+  if (in.K <= 512) launch(std::integral_constant<int, 16>{});
+  else if (in.K <= 2048) launch(std::integral_constant<int, 64>{});
+  else if (in.K <= 8192) launch(std::integral_constant<int, 256>{});
+  else launch(std::integral_constant<int, 1024>{});
   BDH_LAUNCH_CHECK(ctx, "k_prepare_rows");
   return BDH_OK;
 }
@@ -1014,16 +1057,17 @@ int launch_tiles(bdh_ctx *ctx, Product p) {
   if (tiles > 0x7fffffffL) return bdh_fail(ctx, BDH_E_SHAPE, "%ld tiles: the call is too large", tiles);
   p.m_tiles = (int)per_head;
   const dim3 grid((unsigned)tiles), threads(64 * WM * WN);
-  const size_t row = value_bytes(p.out_dtype) * (size_t)(p.token_major ? p.N : p.out_stride);
-  const bool past = bdh_aligned(p.out, 16) && row % 16 == 0;
+  const size_t es = value_bytes(p.out_dtype);  // rows that are whole lines, of all 8 channels of a lane or none
+  const bool lines = bdh_aligned(p.out, 128) && p.out_stride * es % 128 == 0 && (!p.token_major || p.N * es % 128 == 0) && p.N % 8 == 0;
   if (p.splits > 1) {
-    if constexpr (BM != 128 || BN != 128) hipLaunchKernelGGL((k_packed_tile<TYPE, kParts, false, BM, BN, WM, WN>), grid, threads, 0, ctx->stream, p);
+    if constexpr (BM != 128 || BN != 128) hipLaunchKernelGGL((k_packed_tile<TYPE, kParts, true, BM, BN, WM, WN>), grid, threads, 0, ctx->stream, p);
   } else {
     with_behind(p, [&](auto behind) {
       constexpr int BEHIND = decltype(behind)::value;
-      if constexpr (BM == 128 && BN == 128 && BEHIND != kAll) return;  // for gates
-      else if (past) hipLaunchKernelGGL((k_packed_tile<TYPE, BEHIND, true, BM, BN, WM, WN>), grid, threads, 0, ctx->stream, p);
-      else hipLaunchKernelGGL((k_packed_tile<TYPE, BEHIND, false, BM, BN, WM, WN>), grid, threads, 0, ctx->stream, p);
+      if constexpr (BM != 128 || BN != 128 || BEHIND == kAll) {  // 128x128 is for gates
+        if (lines) hipLaunchKernelGGL((k_packed_tile<TYPE, BEHIND, true, BM, BN, WM, WN>), grid, threads, 0, ctx->stream, p);
+        else hipLaunchKernelGGL((k_packed_tile<TYPE, BEHIND, false, BM, BN, WM, WN>), grid, threads, 0, ctx->stream, p);
+      }
     });
   }
   BDH_LAUNCH_CHECK(ctx, "k_packed_tile");
@@ -1031,12 +1075,15 @@ int launch_tiles(bdh_ctx *ctx, Product p) {
 }
 
 template <int TYPE, int MT, int W, int U, bool PRE>
-int launch_few(bdh_ctx *ctx, const Product &p, const RowsIn &in) {
-  const long blocks = (long)p.Nb * p.G * p.splits;
+int launch_few(bdh_ctx *ctx, Product p, const RowsIn &in) {
+  const long per_head = ((long)p.rows + 16 * MT - 1) / (16 * MT), tiles = p.offsets ? p.rows / (16 * MT) + (long)p.G : per_head * p.G;
+  const long blocks = p.Nb * tiles * p.splits;
   if (blocks > 0x7fffffffL) return bdh_fail(ctx, BDH_E_SHAPE, "%ld workgroups: the call is too large", blocks);
+  p.m_tiles = (int)(p.offsets ? tiles : per_head);
   const dim3 grid((unsigned)blocks), threads(64 * W);
   if (p.splits > 1) {
-    if constexpr (W == 4) hipLaunchKernelGGL((k_packed_few<TYPE, kParts, MT, W, U, PRE>), grid, threads, 0, ctx->stream, p, in);
+    if constexpr (W == 4 && (!PRE || TYPE == BDH_BF16))
+      hipLaunchKernelGGL((k_packed_few<TYPE, kParts, MT, W, U, PRE>), grid, threads, 0, ctx->stream, p, in);
   } else {
     with_behind(p, [&](auto behind) {
       hipLaunchKernelGGL((k_packed_few<TYPE, decltype(behind)::value, MT, W, U, PRE>), grid, threads, 0, ctx->stream, p, in);
@@ -1090,7 +1137,8 @@ int launch_product(bdh_ctx *ctx, const Call &c, const Plan &plan, Product p) {
       constexpr bool PRE = decltype(pre)::value;
       if (plan.waves == 8) {
         if (plan.mt == 1) return plan.one ? launch_few<TYPE, 1, 8, 1, PRE>(ctx, p, in) : launch_few<TYPE, 1, 8, 4, PRE>(ctx, p, in);
-        return plan.one ? launch_few<TYPE, 2, 8, 1, PRE>(ctx, p, in) : launch_few<TYPE, 2, 8, 2, PRE>(ctx, p, in);
+        if (plan.mt == 2) return plan.one ? launch_few<TYPE, 2, 8, 1, PRE>(ctx, p, in) : launch_few<TYPE, 2, 8, 2, PRE>(ctx, p, in);
+        return launch_few<TYPE, 4, 8, 1, PRE>(ctx, p, in);
       }
       if (plan.mt == 1) return plan.one ? launch_few<TYPE, 1, 4, 1, PRE>(ctx, p, in) : launch_few<TYPE, 1, 4, 4, PRE>(ctx, p, in);
       if (plan.mt == 2) return plan.one ? launch_few<TYPE, 2, 4, 1, PRE>(ctx, p, in) : launch_few<TYPE, 2, 4, 2, PRE>(ctx, p, in);
@@ -1104,8 +1152,7 @@ int launch_product(bdh_ctx *ctx, const Call &c, const Plan &plan, Product p) {
       p.top_parts = plan.top_parts;
       p.row_scales = reinterpret_cast<float *>(workspace + plan.scales);
     }
-    if constexpr (TYPE == BDH_BF16) rc = plan.direct ? launch(std::true_type{}) : launch(std::false_type{});
-    else rc = launch(std::false_type{});
+    rc = plan.direct || plan.prepared ? launch(std::true_type{}) : launch(std::false_type{});
   } else {
     rc = plan.bm == 256   ? launch_tiles<TYPE, 256, 256, 4, 4>(ctx, p)
          : plan.bm == 128 ? (plan.bn == 256 ? launch_tiles<TYPE, 128, 256, 2, 4>(ctx, p) : launch_tiles<TYPE, 128, 128, 2, 4>(ctx, p))

@@ -40,8 +40,11 @@ class PackedWeights:
         self._c = ffi.PackedWeightsC(kind, self.groups, self.inner, self.outer, self.data.data_ptr(), ffi.ptr(self.scales))
         self._ref = ctypes.byref(self._c)
         # calls of up to this many rows a group need no workspace: asking for its size would cost a tenth of such a call
-        few = (lib.bdh_packed_workspace(ctx.handle, self._ref, n, n, None, ffi.F32, self.inner) for n in (1, 16, 32, FEW))
-        self.few = FEW if self.groups > 0 and not any(few) else 0
+        self.few = 0
+        for n in (16, 32, FEW):
+            if self.groups == 0 or lib.bdh_packed_workspace(ctx.handle, self._ref, n, n, None, ffi.F32, self.inner):
+                break
+            self.few = n
 
     @property
     def nbytes(self) -> int:
@@ -102,7 +105,9 @@ def _call(x: torch.Tensor, weights: PackedWeights, offsets, out_dtype, out, ctx)
             raise ValueError(f"out: expected rows {(*shape[:-1], N)}, got {tuple(out.shape)} with strides {out.stride()}")
         out_stride = N if dense else out.stride(0)
     stride = x.stride(0) if M > 1 else K
-    held, workspace, size = _workspace(ctx, weights, M, M if offsets is None or M <= weights.few else -1, x, kind, stride)
+    # (grouped rows that are few and on average at most 16 a group are streamed as they are)
+    of_group = M if offsets is None else 0 if M <= FEW and M <= 16 * weights.groups else -1
+    held, workspace, size = _workspace(ctx, weights, M, of_group, x, kind, stride)
     if offsets is None:
         ctx.check(ctx._lib.bdh_packed_product(ctx.handle, weights._ref, M, x.data_ptr(), kind, stride, out.data_ptr(), _ROWS[out.dtype],
                                               out_stride, workspace, size))

@@ -77,11 +77,12 @@ int main() {
   REFUSE(BDH_E_INVAL, product, a.x_stride = 63);
   REFUSE(BDH_E_INVAL, grouped, a.out_stride = 31);
   REFUSE(BDH_E_SHAPE, product, a.w.groups = 2);
-  REFUSE(BDH_E_INVAL, product, a.ws = nullptr);
-  REFUSE(BDH_E_INVAL, product, a.bytes = 1000);
-  REFUSE(BDH_E_ALIGN, product, a.ws = room + 4);
-  REFUSE(BDH_E_INVAL, product, a.ws = x);
-  REFUSE(BDH_E_INVAL, product, a.ws = out);
+  // (so many rows that they are prepared)
+  REFUSE(BDH_E_INVAL, product, a.rows = 1 << 20; a.ws = nullptr);
+  REFUSE(BDH_E_INVAL, product, a.rows = 1 << 20; a.bytes = 1000);
+  REFUSE(BDH_E_ALIGN, product, a.rows = 1 << 20; a.bytes = size_t(1) << 40; a.ws = room + 4);
+  REFUSE(BDH_E_INVAL, product, a.rows = 1 << 20; a.bytes = size_t(1) << 40; a.ws = x);
+  REFUSE(BDH_E_INVAL, product, a.rows = 1 << 20; a.bytes = size_t(1) << 40; a.ws = out);
   REFUSE(BDH_E_INVAL, grouped, a.off = nullptr);
   REFUSE(BDH_E_INVAL, grouped, a.off = reinterpret_cast<int32_t *>(reinterpret_cast<char *>(offsets) + 2));
   REFUSE(BDH_E_INVAL, grouped, a.off = reinterpret_cast<int32_t *>(out + 100));

@@ -73,7 +73,8 @@ def rows_of(g, M, K, dtype):
 
 
 SIZES = [(1, 1, 1), (1, 256, 256), (2, 15, 7), (3, 16, 8), (5, 63, 65), (16, 64, 64), (17, 65, 63), (4, 4096, 72), (33, 100, 200),
-         (64, 257, 129), (65, 128, 130), (130, 1000, 66), (200, 512, 321), (1, 32768, 256), (7, 5000, 9), (31, 9000, 40)]
+         (64, 257, 129), (65, 128, 130), (130, 1000, 66), (200, 512, 321), (1, 32768, 256), (7, 5000, 9), (31, 9000, 40),
+         (22, 3201, 203), (51, 1275, 92), (45, 2100, 700), (40, 1100, 17000), (500, 9, 324), (700, 70, 40), (300, 9000, 580), (90, 131072, 33)]
 
 
 @pytest.mark.parametrize("kind", [INT8, BF16])
@@ -126,7 +127,8 @@ def test_rows_with_strides_and_a_place_of_their_own(M, kind):
 
 @pytest.mark.parametrize("kind", [INT8, BF16])
 @pytest.mark.parametrize("B,h,T,d,N", [(1, 4, 1, 256, 256), (4, 4, 1, 256, 256), (3, 2, 5, 33, 70), (2, 3, 70, 64, 130), (1, 1, 1, 1, 1),
-                                       (2, 8, 33, 100, 129), (20, 2, 1, 40, 65), (1, 2, 300, 128, 64)])
+                                       (2, 8, 33, 100, 129), (20, 2, 1, 40, 65), (1, 2, 300, 128, 64), (2, 3, 20, 3000, 70),
+                                       (3, 2, 50, 4100, 66), (1, 3, 1, 5000, 130)])
 @pytest.mark.parametrize("shared", [True, False])
 @pytest.mark.parametrize("x_dtype,gate_dtype,out_dtype", [(F32, F32, F32), (BF16, BF16, BF16), (F32, None, BF16), (BF16, F32, F32)])
 def test_relu_lowrank(B, h, T, d, N, shared, kind, x_dtype, gate_dtype, out_dtype):
