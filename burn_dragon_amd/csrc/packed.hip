@@ -31,6 +31,8 @@ typedef unsigned int u32x2u __attribute__((ext_vector_type(2), aligned(2)));
 
 constexpr float kLeast = 0x1p-118f;  // below it a scale would be subnormal: such a row or channel counts as zeros
 constexpr int kMostInner = 131072;   // 127^2 K < 2^31
+constexpr int64_t kMostRows = 0x7fffff00;          // a tile's rows are counted in 32 bits past the last one
+constexpr int64_t kMostThreads = 0xffffffffLL;     // of a launch
 
 __device__ __forceinline__ int channel_of(int frag, int row) {
   return 32 * (frag >> 1) + 8 * (row >> 2) + 4 * (frag & 1) + (row & 3);
@@ -123,7 +125,7 @@ __global__ __launch_bounds__(256) void k_pack(const void *__restrict__ w, int dt
 
 // ---- rows ---------------------------------------------------------------------------------------
 
-// Where the values of a row lie: row r at base + (r / T) * outer + (r % T) * stride, its k in runs of `run` values, `jump` apart.
+// Rows of K values, `stride` values apart.
 struct RowsIn {
   const void *x;
   int dtype, K;
@@ -386,6 +388,7 @@ struct Channels {
 template <int E>
 __device__ __forceinline__ void load_some(const void *p, int dtype, long at, int left, float (&v)[E]) {
   if (left < E) {
+#pragma unroll
     for (int e = 0; e < E; ++e) v[e] = load_value(p, dtype, at + min(e, left - 1));
     return;
   }
@@ -727,50 +730,49 @@ __global__ __launch_bounds__(64 * W) void k_packed_few(Product g, RowsIn in) {
   }
   const int kb0 = split * g.kb_each, kb1 = min(kb0 + g.kb_each, g.Kb);
   const i32x4 *w = reinterpret_cast<const i32x4 *>(g.w) + ((long)group * g.Nb + nb) * g.Kb * 256 + lane;
-  {
-    unsigned int row[MT];
+  unsigned int row[MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) row[i] = row_in_of(g, min(first + i * 16 + (lane & 15), last - 1), group);
-    i32x4 fw[U][4], fr[U][MT];
-    float v[PRE ? 1 : U][PRE ? 1 : MT][PER];
-    auto ask = [&](int b, int u) {  // block b of the weights and rows
+  for (int i = 0; i < MT; ++i) row[i] = row_in_of(g, min(first + i * 16 + (lane & 15), last - 1), group);
+  i32x4 fw[U][4], fr[U][MT];
+  float v[PRE ? 1 : U][PRE ? 1 : MT][PER];
+  auto ask = [&](int b, int u) {  // block b of the weights and rows
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        if constexpr (PRE) fr[u][i] = *reinterpret_cast<const i32x4 *>(g.q + row[i] * g.pitch + b * 64 + (lane >> 4) * 16);
-        else load_values<PER>(in, row[i], (b * 4 + (lane >> 4)) * PER, v[u][i]);
+    for (int i = 0; i < MT; ++i) {
+      if constexpr (PRE) fr[u][i] = *reinterpret_cast<const i32x4 *>(g.q + row[i] * g.pitch + b * 64 + (lane >> 4) * 16);
+      else load_values<PER>(in, row[i], (b * 4 + (lane >> 4)) * PER, v[u][i]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) fw[u][j] = w[(long)b * 256 + j * 64];
+  };
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (kb0 + wave + u * W < kb1) ask(kb0 + wave + u * W, u);
+  // what comes behind the sums of 4 channels of a row a thread is asked for with them
+  const int c4 = (threadIdx.x & 15) * 4, mine = threadIdx.x >> 4;
+  const Channels<TYPE, BEHIND, 4> c(g, group, nb * 64 + c4);
+  float gate[R][4];
+#pragma unroll
+  for (int k = 0; k < R; ++k)
+    if (BEHIND == kAll && g.gate && c.left > 0)
+      load_some(g.gate, g.gate_dtype, gate_at(g, min(first + mine + k * 4 * W, last - 1), group) + c.n, c.left, gate[k]);
+  float up[MT];
+  if constexpr (TYPE == BDH_INT8 && !PRE) {
+    if (threadIdx.x < 16 * MT) s_top[threadIdx.x] = 0;
+    __syncthreads();
+    if constexpr (BEHIND == kParts) {
+      const int n = min(last - first, 16 * MT);
+      for (int t = threadIdx.x; t < n * g.top_parts; t += 64 * W) {
+        const int r = t / g.top_parts;
+        atomicMax(&s_top[r], g.tops[(long)row_in_of(g, first + r, group) * g.top_parts + (t - r * g.top_parts)]);
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) fw[u][j] = w[(long)b * 256 + j * 64];
-    };
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (kb0 + wave + u * W < kb1) ask(kb0 + wave + u * W, u);
-    // what comes behind the sums of 4 channels of a row a thread is asked for with them
-    const int c4 = (threadIdx.x & 15) * 4, mine = threadIdx.x >> 4;
-    const Channels<TYPE, BEHIND, 4> c(g, group, nb * 64 + c4);
-    float gate[R][4];
-#pragma unroll
-    for (int k = 0; k < R; ++k)
-      if (BEHIND == kAll && g.gate && c.left > 0)
-        load_some(g.gate, g.gate_dtype, gate_at(g, min(first + mine + k * 4 * W, last - 1), group) + c.n, c.left, gate[k]);
-    float up[MT];
-    if constexpr (TYPE == BDH_INT8 && !PRE) {
-      if (threadIdx.x < 16 * MT) s_top[threadIdx.x] = 0;
       __syncthreads();
-      if constexpr (BEHIND == kParts) {
-        const int n = min(last - first, 16 * MT);
-        for (int t = threadIdx.x; t < n * g.top_parts; t += 64 * W) {
-          const int r = t / g.top_parts;
-          atomicMax(&s_top[r], g.tops[(long)row_in_of(g, first + r, group) * g.top_parts + (t - r * g.top_parts)]);
+      if (split == 0 && nb == 0 && (g.h_in > 1 || group == 0))  // for k_packed_finish
+        for (int t = threadIdx.x; t < n; t += 64 * W) {
+          float scale, unused;
+          scale_of(s_top[t], scale, unused);
+          g.row_scales[row_in_of(g, first + t, group)] = scale;
         }
-        __syncthreads();
-        if (split == 0 && nb == 0 && (g.h_in > 1 || group == 0))  // for k_packed_finish
-          for (int t = threadIdx.x; t < n; t += 64 * W) {
-            float scale, unused;
-            scale_of(s_top[t], scale, unused);
-            g.row_scales[row_in_of(g, first + t, group)] = scale;
-          }
-      } else {
+    } else {
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         unsigned int top = 0;
@@ -787,60 +789,59 @@ __global__ __launch_bounds__(64 * W) void k_packed_few(Product g, RowsIn in) {
         if (lane < 16) atomicMax(&s_top[i * 16 + lane], top);
       }
       __syncthreads();
-      }
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        float scale;
-        scale_of(s_top[min(i * 16 + (lane & 15), last - first - 1)], scale, up[i]);
-      }
-    }
-    acc_t acc[MT][4];
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = acc_t{};
-    for (int kb = kb0 + wave; kb < kb1; kb += U * W) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (kb + u * W < kb1) {
-#pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            i32x4 r;
-            if constexpr (PRE) r = fr[u][i];
-            else r = __builtin_bit_cast(i32x4, packed16<TYPE>(v[u][i], up[i]));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = Acc<TYPE>::mac(fw[u][j], r, acc[i][j]);
-          }
-        }
-        if (kb + (u + U) * W < kb1) ask(kb + (u + U) * W, u);
-      }
     }
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < MT; ++i) {
+      float scale;
+      scale_of(s_top[min(i * 16 + (lane & 15), last - first - 1)], scale, up[i]);
+    }
+  }
+  acc_t acc[MT][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        *reinterpret_cast<acc_t *>(&s_sum[wave][i * 16 + (lane & 15)][32 * (j >> 1) + 8 * (lane >> 4) + 4 * (j & 1)]) = acc[i][j];
-    __syncthreads();
+  for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int k = 0; k < R; ++k) {
-      const int r = mine + k * 4 * W;
-      if (r >= 16 * MT || first + r >= last) break;
-      acc_t sum = *reinterpret_cast<const acc_t *>(&s_sum[0][r][c4]);
+    for (int j = 0; j < 4; ++j) acc[i][j] = acc_t{};
+  for (int kb = kb0 + wave; kb < kb1; kb += U * W) {
 #pragma unroll
-      for (int x = 1; x < W; ++x) sum += *reinterpret_cast<const acc_t *>(&s_sum[x][r][c4]);
-      if constexpr (BEHIND == kParts) {
-        reinterpret_cast<acc_t *>(g.parts)[((split * g.rows_out + row_out_of(g, first + r, group)) * g.Nb + nb) * 16 + c4 / 4] = sum;
-      } else {
-        float scale = 1.0f, unused;
-        if constexpr (TYPE == BDH_INT8) {
-          if constexpr (PRE) scale = g.row_scales[row_in_of(g, first + r, group)];
-          else scale_of(s_top[r], scale, unused);
+    for (int u = 0; u < U; ++u) {
+      if (kb + u * W < kb1) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          i32x4 r;
+          if constexpr (PRE) r = fr[u][i];
+          else r = __builtin_bit_cast(i32x4, packed16<TYPE>(v[u][i], up[i]));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j] = Acc<TYPE>::mac(fw[u][j], r, acc[i][j]);
         }
-        float sums[4] = {(float)sum[0], (float)sum[1], (float)sum[2], (float)sum[3]};
-        if (c.left <= 0) continue;
-        finish<TYPE, BEHIND>(g, c, sums, gate[k], scale, false);
-        store4(g, c, out_at(g, first + r, group) + c.n, sums);
       }
+      if (kb + (u + U) * W < kb1) ask(kb + (u + U) * W, u);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      *reinterpret_cast<acc_t *>(&s_sum[wave][i * 16 + (lane & 15)][32 * (j >> 1) + 8 * (lane >> 4) + 4 * (j & 1)]) = acc[i][j];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < R; ++k) {
+    const int r = mine + k * 4 * W;
+    if (r >= 16 * MT || first + r >= last) break;
+    acc_t sum = *reinterpret_cast<const acc_t *>(&s_sum[0][r][c4]);
+#pragma unroll
+    for (int x = 1; x < W; ++x) sum += *reinterpret_cast<const acc_t *>(&s_sum[x][r][c4]);
+    if constexpr (BEHIND == kParts) {
+      reinterpret_cast<acc_t *>(g.parts)[((split * g.rows_out + row_out_of(g, first + r, group)) * g.Nb + nb) * 16 + c4 / 4] = sum;
+    } else {
+      float scale = 1.0f, unused;
+      if constexpr (TYPE == BDH_INT8) {
+        if constexpr (PRE) scale = g.row_scales[row_in_of(g, first + r, group)];
+        else scale_of(s_top[r], scale, unused);
+      }
+      float sums[4] = {(float)sum[0], (float)sum[1], (float)sum[2], (float)sum[3]};
+      if (c.left <= 0) continue;
+      finish<TYPE, BEHIND>(g, c, sums, gate[k], scale, false);
+      store4(g, c, out_at(g, first + r, group) + c.n, sums);
     }
   }
 }
@@ -1026,6 +1027,9 @@ Plan plan_of(const bdh_ctx *ctx, const bdh_packed_weights &w, int64_t rows_in, i
   return p;
 }
 
+// Threads that prepare a row: it is held in registers, at most 64 values a thread.
+int threads_of_row(int K) { return K <= 512 ? 16 : K <= 2048 ? 64 : K <= 8192 ? 256 : 1024; }
+
 template <int TYPE, typename X>
 int launch_prepare(bdh_ctx *ctx, const RowsIn &in, int Kb, uint4 *q, float *scales) {
   const unsigned int rows = (unsigned int)in.rows;
@@ -1034,10 +1038,12 @@ int launch_prepare(bdh_ctx *ctx, const RowsIn &in, int Kb, uint4 *q, float *scal
     hipLaunchKernelGGL((k_prepare_rows<TYPE, X, THR>), dim3((rows + ROWS - 1) / ROWS), dim3(THR < 256 ? 256 : THR), 0, ctx->stream, in, Kb,
                        pitch_of(Kb), q, scales);
   };
-  if (in.K <= 512) launch(std::integral_constant<int, 16>{});
-  else if (in.K <= 2048) launch(std::integral_constant<int, 64>{});
-  else if (in.K <= 8192) launch(std::integral_constant<int, 256>{});
-  else launch(std::integral_constant<int, 1024>{});
+  switch (threads_of_row(in.K)) {
+    case 16: launch(std::integral_constant<int, 16>{}); break;
+    case 64: launch(std::integral_constant<int, 64>{}); break;
+    case 256: launch(std::integral_constant<int, 256>{}); break;
+    default: launch(std::integral_constant<int, 1024>{});
+  }
   BDH_LAUNCH_CHECK(ctx, "k_prepare_rows");
   return BDH_OK;
 }
@@ -1054,7 +1060,7 @@ template <int TYPE, int BM, int BN, int WM, int WN>
 int launch_tiles(bdh_ctx *ctx, Product p) {
   p.n_tiles = (p.N + BN - 1) / BN;
   const long per_head = ((long)p.rows + BM - 1) / BM, tiles = (p.offsets ? per_head + p.G : per_head * p.G) * p.n_tiles * p.splits;
-  if (tiles > 0x7fffffffL) return bdh_fail(ctx, BDH_E_SHAPE, "%ld tiles: the call is too large", tiles);
+  if (tiles * 64 * WM * WN > kMostThreads) return bdh_fail(ctx, BDH_E_SHAPE, "%ld tiles: the call is too large", tiles);
   p.m_tiles = (int)per_head;
   const dim3 grid((unsigned)tiles), threads(64 * WM * WN);
   const size_t es = value_bytes(p.out_dtype);  // rows that are whole lines, of all 8 channels of a lane or none
@@ -1078,7 +1084,7 @@ template <int TYPE, int MT, int W, int U, bool PRE>
 int launch_few(bdh_ctx *ctx, Product p, const RowsIn &in) {
   const long per_head = ((long)p.rows + 16 * MT - 1) / (16 * MT), tiles = p.offsets ? p.rows / (16 * MT) + (long)p.G : per_head * p.G;
   const long blocks = p.Nb * tiles * p.splits;
-  if (blocks > 0x7fffffffL) return bdh_fail(ctx, BDH_E_SHAPE, "%ld workgroups: the call is too large", blocks);
+  if (blocks * 64 * W > kMostThreads) return bdh_fail(ctx, BDH_E_SHAPE, "%ld workgroups: the call is too large", blocks);
   p.m_tiles = (int)(p.offsets ? tiles : per_head);
   const dim3 grid((unsigned)blocks), threads(64 * W);
   if (p.splits > 1) {
@@ -1163,7 +1169,7 @@ int launch_product(bdh_ctx *ctx, const Call &c, const Plan &plan, Product p) {
   const long sums = p.rows_out * ((p.N + 3) / 4);
   const bool shared = sums < 256L * ctx->n_cu;
   const long blocks = (sums * (shared ? 8 : 1) + 255) / 256;
-  if (blocks > 0x7fffffffL) return bdh_fail(ctx, BDH_E_SHAPE, "%ld workgroups: the call is too large", blocks);
+  if (blocks * 256 > kMostThreads) return bdh_fail(ctx, BDH_E_SHAPE, "%ld workgroups: the call is too large", blocks);
   with_behind(p, [&](auto behind) {
     constexpr int BEHIND = decltype(behind)::value;
     if (shared) hipLaunchKernelGGL((k_packed_finish<TYPE, BEHIND, 8>), dim3((unsigned)blocks), dim3(256), 0, ctx->stream, p);
@@ -1183,7 +1189,8 @@ int run_product(bdh_ctx *ctx, const Call &c, const Product &p, int64_t rows_out)
   const bdh_packed_weights &w = *c.w;
   if (!is_rows_type(c.x_dtype) || !is_rows_type(p.out_dtype) || (p.gate && !is_rows_type(p.gate_dtype)))
     return bdh_fail(ctx, BDH_E_INVAL, "rows, gate and out are f32 or bf16");
-  if (c.rows_in > 0x7fffffffLL || rows_out > 0x7fffffffLL) return bdh_fail(ctx, BDH_E_SHAPE, "rows >= 2^31");
+  if (c.rows_in > kMostRows || rows_out > kMostRows)
+    return bdh_fail(ctx, BDH_E_SHAPE, "%lld rows: a call takes up to %lld", (long long)std::max(c.rows_in, rows_out), (long long)kMostRows);
   if (c.x_stride < w.inner || p.out_stride < w.outer) return bdh_fail(ctx, BDH_E_INVAL, "row stride < row");
   if (rows_out == 0) return BDH_OK;
   if (!c.x || !p.out || !w.data || (w.type == BDH_INT8 && !w.scales)) return bdh_fail(ctx, BDH_E_INVAL, "null data pointer");
@@ -1192,6 +1199,8 @@ int run_product(bdh_ctx *ctx, const Call &c, const Product &p, int64_t rows_out)
       (p.gate && !bdh_aligned(p.gate, value_bytes(p.gate_dtype))))
     return bdh_fail(ctx, BDH_E_ALIGN, "rows, gate and out need the alignment of their values");
   const Plan plan = plan_of(ctx, w, c.rows_in, p.offsets ? -1 : p.rows, c.x, c.x_dtype, c.x_stride, p.gate);
+  if (plan.prepared && c.rows_in * threads_of_row(w.inner) > kMostThreads)
+    return bdh_fail(ctx, BDH_E_SHAPE, "%lld rows of %d values: the call is too large", (long long)c.rows_in, w.inner);
   const size_t need = plan.bytes;
   if (need > 0 && (!c.workspace || c.workspace_bytes < need))
     return bdh_fail(ctx, BDH_E_INVAL, "workspace of %zu bytes, %zu are needed", c.workspace ? c.workspace_bytes : 0, need);
@@ -1221,7 +1230,7 @@ int relu_lowrank(bdh_ctx *ctx, const bdh_packed_weights *w, int B, int h_in, int
   if (h_in != 1 && h_in != w->groups) return bdh_fail(ctx, BDH_E_SHAPE, "input of %d heads for weights of %d", h_in, w->groups);
   if (bias && !bdh_aligned(bias, 4)) return bdh_fail(ctx, BDH_E_ALIGN, "bias needs the alignment of its values");
   const int64_t bt = (int64_t)B * T;
-  if (bt > 0x7fffffffLL) return bdh_fail(ctx, BDH_E_SHAPE, "rows >= 2^31");
+  if (bt > kMostRows) return bdh_fail(ctx, BDH_E_SHAPE, "%lld rows: a call takes up to %lld", (long long)bt, (long long)kMostRows);
   Product p{};
   p.rows = (int)bt;
   p.T = std::max(T, 1);

@@ -13,7 +13,6 @@ from . import ffi
 
 _ROWS = {torch.float32: ffi.F32, torch.bfloat16: ffi.BF16}
 _WEIGHTS = {torch.int8: ffi.INT8, torch.bfloat16: ffi.BF16}
-FEW = 64  # rows that are streamed past the weights in one launch, where k is not so long that it is cut into parts
 MOST_INNER, MOST_OUTER, MOST_GROUPS = 131072, 1 << 24, 65535
 
 
@@ -41,7 +40,7 @@ class PackedWeights:
         self._ref = ctypes.byref(self._c)
         # calls of up to this many rows a group need no workspace: asking for its size would cost a tenth of such a call
         self.few = 0
-        for n in (16, 32, FEW):
+        for n in (16, 32, 64):
             if self.groups == 0 or lib.bdh_packed_workspace(ctx.handle, self._ref, n, n, None, ffi.F32, self.inner):
                 break
             self.few = n
@@ -94,8 +93,6 @@ def _call(x: torch.Tensor, weights: PackedWeights, offsets, out_dtype, out, ctx)
             with ctx.torch_stream():  # it may be a copy
                 x = x.reshape(-1, K).contiguous()
     M = x.shape[0]
-    if M >> 31:
-        raise ValueError(f"{M} rows: a call carries numbers below 2^31")
     if out is None:
         out, out_stride = _new(x, (M, N) if len(shape) == 2 else (*shape[:-1], N), out_dtype, ctx), N
     else:
@@ -105,8 +102,8 @@ def _call(x: torch.Tensor, weights: PackedWeights, offsets, out_dtype, out, ctx)
             raise ValueError(f"out: expected rows {(*shape[:-1], N)}, got {tuple(out.shape)} with strides {out.stride()}")
         out_stride = N if dense else out.stride(0)
     stride = x.stride(0) if M > 1 else K
-    # (grouped rows that are few and on average at most 16 a group are streamed as they are)
-    of_group = M if offsets is None else 0 if M <= FEW and M <= 16 * weights.groups else -1
+    # (up to 32 grouped rows, on average at most 16 a group, are streamed as they are)
+    of_group = M if offsets is None else 0 if M <= 32 and M <= 16 * weights.groups else -1
     held, workspace, size = _workspace(ctx, weights, M, of_group, x, kind, stride)
     if offsets is None:
         ctx.check(ctx._lib.bdh_packed_product(ctx.handle, weights._ref, M, x.data_ptr(), kind, stride, out.data_ptr(), _ROWS[out.dtype],

@@ -74,6 +74,11 @@ int main() {
   REFUSE(BDH_E_INVAL, grouped, a.rows = -1);
   REFUSE(BDH_E_SHAPE, product, a.rows = 1LL << 31);
   REFUSE(BDH_E_SHAPE, grouped, a.rows = 1LL << 31);
+  REFUSE(BDH_E_SHAPE, product, a.rows = 0x7fffff01);
+  REFUSE(BDH_E_SHAPE, grouped, a.rows = 0x7fffff01);
+  REFUSE(BDH_E_SHAPE, lowrank, a.B = 1; a.T = 0x7fffff01);
+  REFUSE(BDH_E_SHAPE, product, a.rows = 1 << 28);  // 16 threads a row
+  REFUSE(BDH_E_SHAPE, grouped, a.rows = 1 << 28);
   REFUSE(BDH_E_INVAL, product, a.x_stride = 63);
   REFUSE(BDH_E_INVAL, grouped, a.out_stride = 31);
   REFUSE(BDH_E_SHAPE, product, a.w.groups = 2);

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from .test_gpu_packed import BF16, DEV, F32, INT8, gen, pack
+from .test_gpu_packed import BF16, DEV, F32, INT8, close, definition, gen, pack, rows_of
 
 pytestmark = pytest.mark.gpu
 
@@ -134,3 +134,81 @@ def test_the_c_entry_refuses_a_workspace_that_is_too_small():
     assert run(x.data_ptr(), need) == ffi.E_INVAL and run(ws.data_ptr(), need, x) == ffi.E_INVAL
     assert (out == 7).all()
     assert run(ws.data_ptr(), need) == ffi.OK and (out == 0).all()
+
+
+@pytest.mark.parametrize("G", [1, 2, 8, 40])
+@pytest.mark.parametrize("M", [1, 16, 17, 32, 33, 48, 64, 65])
+def test_few_rows_of_wide_groups(M, G):
+    """Whatever a call needs beside its arguments it asks for, on both sides of every rule for few rows."""
+    from burn_dragon_amd.packed import grouped_product, product
+
+    K, N = 64, 1500 if G > 1 else 20000
+    g = gen(M + G)
+    x, w = rows_of(g, M, K, F32), torch.randn((G, K, N), generator=g)
+    for kind in (INT8, BF16):
+        limits = [i * M // G for i in range(G + 1)]
+        got = grouped_product(x.to(DEV), pack(w, kind), limits)
+        for k in range(G):
+            a, b = limits[k], limits[k + 1]
+            if b > a:
+                close(got[a:b], *definition(x[a:b], w[k], kind), k)
+        if G == 1:
+            close(product(x.to(DEV), pack(w, kind)), *definition(x, w[0], kind))
+
+
+def _room(gib):
+    if torch.cuda.mem_get_info()[0] < gib << 30:
+        pytest.skip(f"{gib} GiB of memory")
+
+
+def test_results_beyond_2_31_values():
+    """Rows repeat every 40 and 8-bit results do not depend on their neighbours: every block of 40 is the first one's."""
+    from burn_dragon_amd.kernel.relu_lowrank import packed_forward
+    from burn_dragon_amd.packed import product
+
+    _room(24)
+    g = gen(5)
+    M, K, N = 40000, 64, 65536
+    x, w = rows_of(g, 40, K, BF16), torch.randn((K, N), generator=g)
+    packed = pack(w, INT8)
+    out = product(x.to(DEV, BF16).repeat(M // 40, 1), packed, out_dtype=BF16)
+    assert out.numel() > 2**31
+    want, bound = definition(x, w, INT8)
+    close(out[:40], want, bound + 2.0**-8 * (abs(want) + bound))
+    assert all(torch.equal(out[i:i + 4000].view(-1, 40, N), out[:40].expand(100, 40, N)) for i in range(0, M, 4000))
+    del out
+    w4 = pack(w.view(K, 4, N // 4).transpose(0, 1).contiguous(), INT8)
+    gate = torch.randn((1, 4, 40, N // 4), generator=g).to(DEV, BF16)
+    out = packed_forward(x.to(DEV, BF16).repeat(M // 40, 1).view(1, 1, M, K), w4, gate=gate.repeat(1, 1, M // 40, 1), out_dtype=BF16)
+    first = packed_forward(x.to(DEV, BF16).view(1, 1, 40, K), w4, gate=gate, out_dtype=BF16)
+    assert torch.equal(out[:, :, :40], first)
+    for h in range(4):
+        assert all(torch.equal(out[0, h, i:i + 4000].view(-1, 40, N // 4), first[0, h].expand(100, 40, N // 4)) for i in range(0, M, 4000))
+
+
+def test_rows_beyond_2_31_values():
+    from burn_dragon_amd.packed import product
+
+    _room(16)
+    g = gen(6)
+    M, K, N = 16800, 131072, 40
+    x, w = rows_of(g, 40, K, BF16), torch.randn((K, N), generator=g)
+    out = product(x.to(DEV, BF16).repeat(M // 40, 1), pack(w, INT8))
+    close(out[:40], *definition(x, w, INT8))
+    assert torch.equal(out.view(-1, 40, N), out[:40].expand(M // 40, 40, N))
+
+
+@pytest.mark.parametrize("kind", [INT8, BF16])
+@pytest.mark.parametrize("M", [3, 90])
+def test_weights_beyond_2_31_bytes(M, kind):
+    from burn_dragon_amd.packed import PackedWeights, product
+
+    _room(24)
+    g = gen(7)
+    K, N = 8192, 64 * 4200
+    x, w = rows_of(g, M, K, F32), torch.randn((K, 64), generator=g)
+    packed = PackedWeights(w.to(DEV, BF16).repeat(1, N // 64), dtype=kind)
+    assert packed.data.numel() > 2**31
+    out = product(x.to(DEV), packed)
+    close(out[:, -64:], *definition(x, w.to(BF16).float(), kind))
+    assert torch.equal(out.view(M, -1, 64), out[:, None, :64].expand(M, N // 64, 64))
