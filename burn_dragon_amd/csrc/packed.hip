@@ -28,6 +28,8 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // rows start at any multiple of their values' size
 typedef unsigned int u32x4u __attribute__((ext_vector_type(4), aligned(2)));
 typedef unsigned int u32x2u __attribute__((ext_vector_type(2), aligned(2)));
+typedef unsigned int u32u __attribute__((aligned(2)));
+typedef float f32x2u __attribute__((ext_vector_type(2), aligned(4)));
 
 constexpr float kLeast = 0x1p-118f;  // below it a scale would be subnormal: such a row or channel counts as zeros
 constexpr int kMostInner = 131072;   // 127^2 K < 2^31
@@ -132,36 +134,81 @@ struct RowsIn {
   long rows, stride;
 };
 
+// N (8, 4, 2 or 1) neighbouring values.
+template <int N>
+__device__ __forceinline__ void load_near(const float *p, float *v) {
+  if constexpr (N >= 4) {
+#pragma unroll
+    for (int j = 0; j < N; j += 4) {
+      const f32x4 t = *reinterpret_cast<const f32x4u *>(p + j);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[j + e] = t[e];
+    }
+  } else if constexpr (N == 2) {
+    const f32x2u t = *reinterpret_cast<const f32x2u *>(p);
+    v[0] = t[0];
+    v[1] = t[1];
+  } else {
+    v[0] = p[0];
+  }
+}
+template <int N>
+__device__ __forceinline__ void load_near(const unsigned short *p, float *v) {
+  if constexpr (N == 1) {
+    v[0] = __uint_as_float((unsigned int)p[0] << 16);
+  } else {
+    unsigned int w[N / 2];
+    if constexpr (N == 8) *reinterpret_cast<u32x4u *>(w) = *reinterpret_cast<const u32x4u *>(p);
+    else if constexpr (N == 4) *reinterpret_cast<u32x2u *>(w) = *reinterpret_cast<const u32x2u *>(p);
+    else w[0] = *reinterpret_cast<const u32u *>(p);
+#pragma unroll
+    for (int e = 0; e < N / 2; ++e) {
+      v[2 * e] = __uint_as_float(w[e] << 16);
+      v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+    }
+  }
+}
+
+// The first `left` < 16 values of a piece, zeros behind them: a load for each bit of left, the longest first.  (A load for each value is
+// three times the instructions, which a workgroup that runs them once waits for: 64 rows of 64 bf16 values 12 us, so 8.)
+template <typename X>
+__device__ __forceinline__ void load_first(const X *p, int left, float (&t8)[8], float (&t4)[4], float (&t2)[2], float (&t1)[1]) {
+  if (left & 8) load_near<8>(p, t8);
+  if (left & 4) load_near<4>(p + (left & 8), t4);
+  if (left & 2) load_near<2>(p + (left & 12), t2);
+  if (left & 1) load_near<1>(p + (left & 14), t1);
+}
+
 // PER (8 or 16) neighbouring values of a row from k on; what lies past the end is 0.
 template <int PER>
 __device__ __forceinline__ void load_values(const RowsIn &in, long row, int k, float (&v)[PER]) {
   const long at = row * in.stride + k;
   if (k + PER <= in.K) {
-    if (in.dtype == BDH_F32) {
-      const float *p = static_cast<const float *>(in.x) + at;
 #pragma unroll
-      for (int j = 0; j < PER / 4; ++j) {
-        const f32x4 t = *reinterpret_cast<const f32x4u *>(p + 4 * j);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[4 * j + e] = t[e];
-      }
-    } else {
-      const unsigned short *p = static_cast<const unsigned short *>(in.x) + at;
-#pragma unroll
-      for (int j = 0; j < PER / 8; ++j) {
-        const u32x4u t = *reinterpret_cast<const u32x4u *>(p + 8 * j);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[8 * j + 2 * e] = __uint_as_float(t[e] << 16);
-          v[8 * j + 2 * e + 1] = __uint_as_float(t[e] & 0xffff0000u);
-        }
-      }
+    for (int j = 0; j < PER; j += 8) {
+      if (in.dtype == BDH_F32) load_near<8>(static_cast<const float *>(in.x) + at + j, v + j);
+      else load_near<8>(static_cast<const unsigned short *>(in.x) + at + j, v + j);
     }
-  } else {  // all asked for at once; those past the end repeat the last one until they are cleared
+    return;
+  }
 #pragma unroll
-    for (int e = 0; e < PER; ++e) v[e] = load_value(in.x, in.dtype, at + min(e, in.K - 1 - k));
+  for (int e = 0; e < PER; ++e) v[e] = 0.0f;
+  if (k >= in.K) return;
+  const int left = in.K - k;
+  float t8[8] = {}, t4[4] = {}, t2[2] = {}, t1[1] = {};
+  if (in.dtype == BDH_F32) load_first(static_cast<const float *>(in.x) + at, left, t8, t4, t2, t1);
+  else load_first(static_cast<const unsigned short *>(in.x) + at, left, t8, t4, t2, t1);
+  const bool b8 = PER > 8 && (left & 8), b4 = left & 4, b2 = left & 2;
+  const float w[4] = {b2 ? t2[0] : t1[0], t2[1], b2 ? t1[0] : 0.0f, 0.0f};
 #pragma unroll
-    for (int e = 0; e < PER; ++e) v[e] = k + e < in.K ? v[e] : 0.0f;
+  for (int e = 0; e < 4; ++e) {
+    const float low = b4 ? t4[e] : w[e], high = b4 ? w[e] : 0.0f;
+    v[e] = b8 ? t8[e] : low;
+    v[4 + e] = b8 ? t8[4 + e] : high;
+    if (PER > 8) {
+      v[PER - 8 + e] = b8 ? low : 0.0f;
+      v[PER - 4 + e] = b8 ? high : 0.0f;
+    }
   }
 }
 template <int PER>
@@ -183,8 +230,9 @@ __device__ __forceinline__ uint4 packed16(const float (&v)[PER], float up) {
 }
 
 // Rows as the product takes them, `pitch` bytes apart: Kb * 64 bytes, zeros behind K, and the scales of 8-bit rows.  THR threads a row, 16
-// bytes a thread at a time.  An 8-bit row is read once, as far as HOLD values a thread hold it as they came (X: float or bf16's bits), and
-// what is behind them twice, the second time from a cache.
+// bytes a thread at a time.  An 8-bit row is read once, as far as HOLD pieces a thread hold it as they came (X: float or bf16's bits; two
+// reads took 197 us for 2048 bf16 rows of 131072, one 154: 5.2 TB/s, what memory gives), and what is behind them twice, the second time
+// from a cache.  THR by the length of a row (threads_of_row): 256 a row throughout left most of them idle at 512 values and fewer.
 template <int TYPE, typename X, int THR>
 __global__ __launch_bounds__(THR < 256 ? 256 : THR) void k_prepare_rows(RowsIn in, int Kb, long pitch, uint4 *__restrict__ q, float *__restrict__ scales) {
   constexpr int ROWS = THR < 256 ? 256 / THR : 1, PER = TYPE == BDH_INT8 ? 16 : 8, HOLD = TYPE != BDH_INT8 ? 0 : THR < 1024 ? 2 : sizeof(X) == 2 ? 8 : 4;
@@ -246,12 +294,12 @@ __global__ __launch_bounds__(THR < 256 ? 256 : THR) void k_prepare_rows(RowsIn i
       values(held[h], v);
       out[k / PER] = packed16<TYPE>(v, up);
     } else if (k < padded) {
-      load_values<PER>(in, row, min(k, in.K), v);
+      load_values<PER>(in, row, k, v);
       out[k / PER] = packed16<TYPE>(v, up);
     }
   }
   for (int k = (HOLD * THR + t) * PER; k < padded; k += THR * PER) {
-    load_values<PER>(in, row, min(k, in.K), v);
+    load_values<PER>(in, row, k, v);
     out[k / PER] = packed16<TYPE>(v, up);
   }
 }
@@ -514,6 +562,7 @@ __device__ __forceinline__ long gate_at(const Product &g, unsigned int r, int gr
 // Which tile a workgroup takes: workgroups go to the eight XCDs in turn, so XCD i gets every eighth; it takes the i-th eighth of
 // the tiles, which go through the channels by panels of kPanel tiles of rows, so that what an XCD works on at a time shares its
 // rows and weights in the XCD's L2.
+// (kPanel 4 | 1 | 8 | 16: 1500 rows, 8 heads of 16384 from 512, 8 bits 152 | 187 | 160 | 162 us; 8192 x 8192 x 8192 478 | 502 | 495 | 498.)
 constexpr unsigned int kPanel = 4;
 __device__ __forceinline__ void place_of(const Product &g, int &m_tile, int &n_tile, int &split) {
   const unsigned int total = gridDim.x, xcd = blockIdx.x & 7, each = total >> 3, rest = total & 7;
@@ -531,6 +580,12 @@ __device__ __forceinline__ void place_of(const Product &g, int &m_tile, int &n_t
 // the rows' 128 bytes of k (whole lines of memory: half lines cost up to a fifth) through one of two; both are copied past the
 // registers and waited for by count.  A copy takes 128 bytes of 8 rows; piece p of row r lies at place p ^ (r & 7), so that the
 // reads of a fragment, rows 128 bytes apart, meet no bank twice.
+//
+// What bounds it: the copies, L2 to LDS.  8192 x 8192 x 8192 in 8 bits takes 440 to 455 us (2.45 POP/s), 335 without the matrix
+// instructions, 455 without the stores; in bf16 840 (1.3 PFLOP/s).  With short k the end counts: 1500 rows of 8 heads of 16384, K 512, take
+// 150 us, 108 of them without the loop over k and 92 without the end; two workgroups a CU cover each other in part.  Workgroups that stay
+// and take tile after tile, the next one's first copies before the last one's stores, were slower (167 -> 180 then, 90 -> 124 in bf16
+// with gates: registers), and so was a ring of four stages with fragments read a step ahead (453 -> 465).
 constexpr int tile_lds(int BM, int BN) { return (3 * BN / 16 + 2 * BM / 8) * 1024; }
 constexpr int tiles_a_cu(int BM, int BN) { return 160 * 1024 / tile_lds(BM, BN); }
 template <int TYPE, int BEHIND, bool LINES, int BM, int BN, int WM, int WN>
@@ -709,6 +764,11 @@ __global__ __launch_bounds__(64 * WM * WN, tiles_a_cu(BM, BN) * WM * WN / 4) voi
 // weights and rows, is asked for at once, and the largest magnitude of a row is a maximum over the wavefronts in LDS; the
 // wavefronts' sums are added up in LDS in their order.  PRE: the rows are prepared ones, or bf16 that needs no preparation.  With
 // kParts and 8 bits, the rows' largest magnitudes come from a launch before.
+//
+// What bounds it: a chain of trips to memory (the rows, the maximum, the products, the sums through LDS), so that as much as registers
+// hold is asked for before the first wait; 1 row of 256 x 256 3.6 us, 8 rows of 4 heads 256 x 8192, gated, 5.1, 32 rows of 32768 x 256
+// in 128 parts of k 7.1 (and 3 + 3.5 for the magnitudes and the sums' end).  Weights that fill the chip come at memory's rate: 64 rows that
+// meet 33 of 64 groups of 2048 x 1536 in bf16 35 us, 6 TB/s (a part of them from the last cache).
 template <int TYPE, int BEHIND, int MT, int W, int U, bool PRE>
 __global__ __launch_bounds__(64 * W) void k_packed_few(Product g, RowsIn in) {
   constexpr int PER = TYPE == BDH_INT8 ? 16 : 8, LD = 68, ROUNDS = 16 * MT * 16 / (64 * W);
@@ -846,7 +906,8 @@ __global__ __launch_bounds__(64 * W) void k_packed_few(Product g, RowsIn in) {
   }
 }
 
-// The bits of the largest magnitudes of parts of rows, 4096 values each: for few and long rows, which one workgroup each would be long about.
+// The bits of the largest magnitudes of parts of rows, 4096 values each: for few and long rows, which one workgroup each would be long about
+// (32 rows of 32768: 20 us a call, 15 with this launch of 3).
 __global__ __launch_bounds__(256) void k_row_tops(RowsIn in, int parts, unsigned int *__restrict__ tops) {
   __shared__ unsigned int s_top[4];
   const unsigned int row = blockIdx.x / (unsigned int)parts, part = blockIdx.x - row * parts;
@@ -863,8 +924,9 @@ __global__ __launch_bounds__(256) void k_row_tops(RowsIn in, int parts, unsigned
   if (threadIdx.x == 0) tops[blockIdx.x] = max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3]));
 }
 
-// The sums of the parts of k, and what comes behind them: 4 channels of a row a thread; LANES threads share the parts where there are
-// few sums.
+// The sums of the parts of k, in their order, and what comes behind them: 4 channels of a row a thread; 8 LANES share the parts where there
+// are fewer sums than threads that the chip holds.  Bound by the trip to memory, or by memory: 32 x 256 sums of 128 parts 3.4 us, 2048 x 512
+// of 16 parts 13 (71 MB, 5.5 TB/s, right behind the launch that wrote them).
 template <int TYPE, int BEHIND, int LANES>
 __global__ __launch_bounds__(256) void k_packed_finish(Product g) {
   typedef typename Acc<TYPE>::type acc_t;
@@ -992,9 +1054,9 @@ Plan plan_of(const bdh_ctx *ctx, const bdh_packed_weights &w, int64_t rows_in, i
   const int64_t tiles = grouped ? rows / (16 * p.mt) + groups : (rows + 16 * p.mt - 1) / (16 * p.mt) * groups, blocks = tiles * Nb;
   p.waves = Kb > 4 && (Kb <= 8 || p.mt == 4 || blocks < ctx->n_cu) ? 8 : 4;
   const int at_once = p.waves * (p.mt == 1 ? 4 : p.mt == 2 ? 2 : 1);  // blocks of k that a workgroup has on their way
-  // Streamed: few rows (33 to 64 of them only where that takes one workgroup a CU: 56 rows of 96, 4 heads of 10501 27 us, prepared and in
-  // tiles 17), or so little work that a launch for the rows and one for tiles would be most of it (159 x 516 x 40 15 us | 16; with two
-  // turns of k no longer: 2904 x 932 x 104 24 | 17).
+  // Streamed: few rows (33 to 64 of them only where that takes one workgroup a CU: 64 x 1024 x 20000 31 us, prepared and in tiles 14; 64 x
+  // 512 x 40000 in bf16 25 | 15), or so little work that a launch for the rows and one for tiles would be most of it (159 x 40 x 516 8.6 |
+  // 11; with four workgroups a CU no longer, 300 x 256 x 11000 in bf16 23 | 14, nor with two turns of k, 2904 x 932 x 104 24 | 17).
   p.few = rows <= 32 || (rows <= 64 && blocks < ctx->n_cu) || (grouped && a_group <= 4) || (blocks <= 2 * ctx->n_cu && Kb <= at_once);
   if (p.few) {
     const int turns = (Kb + at_once - 1) / at_once;
