@@ -1,4 +1,7 @@
-"""Packed products called from graphs, streams, contexts and threads."""
+"""Packed products called from graphs, streams and contexts.
+
+This file runs last: streams share a few hardware queues in the order in which they are first used, and the tests of contexts with
+a stream of their own, which hold one stream while another goes on, need the two on different queues."""
 import pytest
 import torch
 
