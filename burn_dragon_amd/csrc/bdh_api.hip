@@ -14,6 +14,54 @@ int bdh_fail(bdh_ctx *ctx, int status, const char *fmt, ...) {
   return status;
 }
 
+bool bdh_capturing(bdh_ctx *ctx) {
+  if (!ctx->stream) return false;  // the null stream is not captured
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(ctx->stream, &status) == hipSuccess) return status != hipStreamCaptureStatusNone;
+  (void)hipGetLastError();
+  return true;  // unknown: a buffer too many is kept
+}
+
+int bdh_grow(bdh_ctx *ctx, const char *what, size_t bytes, void **buffer, size_t *held, bool *captured, bdh_outgrown **kept) {
+  if (bytes <= *held) {
+    if (*buffer && !*captured) *captured = bdh_capturing(ctx);
+    return BDH_OK;
+  }
+  const bool now = bdh_capturing(ctx);
+  bytes = bdh_align_up(bytes, size_t(1) << 20);
+  if (*buffer) {
+    if (now || *captured) {  // (a capture may not wait for what came before it, either)
+      bdh_outgrown *o = new (std::nothrow) bdh_outgrown{*buffer, *kept};
+      if (!o) return bdh_fail(ctx, BDH_E_NOMEM, "host allocation failed");
+      *kept = o;
+    } else {
+      BDH_HIP_CHECK(ctx, hipStreamSynchronize(ctx->stream));
+      BDH_HIP_CHECK(ctx, hipFree(*buffer));
+    }
+    *buffer = nullptr;
+    *held = 0;
+    *captured = false;
+  }
+  const hipError_t e = hipMalloc(buffer, bytes);
+  if (e != hipSuccess) {
+    (void)hipGetLastError();
+    *buffer = nullptr;
+    return bdh_fail(ctx, BDH_E_NOMEM, "%s of %zu bytes: %s", what, bytes, hipGetErrorString(e));
+  }
+  *held = bytes;
+  *captured = now;
+  return BDH_OK;
+}
+
+void bdh_free_outgrown(bdh_outgrown **kept) {
+  while (*kept) {
+    bdh_outgrown *o = *kept;
+    *kept = o->next;
+    (void)hipFree(o->p);
+    delete o;
+  }
+}
+
 int bdh_ws_reserve(bdh_ctx *ctx, size_t bytes) {
   if (bytes <= ctx->ws_bytes) return BDH_OK;
   bytes = bdh_align_up(bytes, size_t(1) << 20);

@@ -12,6 +12,13 @@
 
 #include "../../include/bdh_mi355x.h"
 
+// Buffers that captured calls were given and later calls have outgrown: the graphs hold their addresses, so they stay until the
+// owner of the list (a context, a model) is destroyed.
+struct bdh_outgrown {
+  void *p;
+  bdh_outgrown *next;
+};
+
 struct bdh_ctx {
   int device = 0;
   hipStream_t stream = nullptr;
@@ -60,6 +67,8 @@ struct bdh_model {
   // activation scratch, grown on demand to the largest (B,T) seen
   void *act = nullptr;
   size_t act_bytes = 0;
+  bool act_captured = false;  // a captured call was given it
+  bdh_outgrown *outgrown = nullptr;
   // scratch of the two-launch layer of a model that fits the one-launch step, at most 4 MiB of projection weights; sized at
   // creation for every batch that form is taken for: a decode step of such a model never allocates, and a captured one keeps
   // its buffer whatever runs later.  One buffer a model: its steps follow one another, captured ones too.
@@ -88,6 +97,13 @@ bool bdh_model_small_fits(const bdh_model_config &c);
 int bdh_model_one_launch_from(const bdh_model_config &c);  // sequences; 0: never
 int bdh_launch_model_small(bdh_model *m, const int64_t *tokens, int B, void *rho, int rho_dtype, int32_t *stamps, int64_t position,
                            const int32_t *positions_dev, float *logits, int64_t *next_tokens);
+
+// Whether calls on the context's stream are being captured into a graph.
+bool bdh_capturing(bdh_ctx *ctx);
+// Makes room for `bytes` in a buffer that calls share, its size in `held`.  The one that was there is freed, behind a wait for the
+// stream, unless a captured call may have been given it: then it goes to `kept`.
+int bdh_grow(bdh_ctx *ctx, const char *what, size_t bytes, void **buffer, size_t *held, bool *captured, bdh_outgrown **kept);
+void bdh_free_outgrown(bdh_outgrown **kept);
 
 // Grows ctx->ws to at least `bytes` (synchronises the stream before freeing the old one).
 int bdh_ws_reserve(bdh_ctx *ctx, size_t bytes);

@@ -13,22 +13,7 @@ namespace {
 bool has_phase_act(const bdh_model_config &c) { return bdh_model_one_launch_from(c) == 1; }
 
 int ensure_act(bdh_model *m, size_t bytes) {
-  if (bytes <= m->act_bytes) return BDH_OK;
-  bdh_ctx *ctx = m->ctx;
-  if (m->act) {
-    BDH_HIP_CHECK(ctx, hipStreamSynchronize(ctx->stream));
-    BDH_HIP_CHECK(ctx, hipFree(m->act));
-    m->act = nullptr;
-    m->act_bytes = 0;
-  }
-  bytes = bdh_align_up(bytes, size_t(1) << 20);
-  hipError_t e = hipMalloc(&m->act, bytes);
-  if (e != hipSuccess) {
-    (void)hipGetLastError();
-    return bdh_fail(ctx, BDH_E_NOMEM, "activation scratch of %zu bytes: %s", bytes, hipGetErrorString(e));
-  }
-  m->act_bytes = bytes;
-  return BDH_OK;
+  return bdh_grow(m->ctx, "activation scratch", bytes, &m->act, &m->act_bytes, &m->act_captured, &m->outgrown);
 }
 
 // Where a call finds the recurrent state of layer l: one allocation [L,B,h,Nq,d] (the layers `layer_bytes` apart) or
@@ -169,6 +154,7 @@ int bdh_model_destroy(bdh_model *m) {
   if (m->ctx) (void)hipStreamSynchronize(m->ctx->stream);
   if (m->freqs) (void)hipFree(m->freqs);
   if (m->act) (void)hipFree(m->act);
+  bdh_free_outgrown(&m->outgrown);
   if (m->phase_act) (void)hipFree(m->phase_act);
   delete m;
   return BDH_OK;

@@ -1,0 +1,109 @@
+// What a captured call was given stays: a model's calls and a context's calls share buffers that grow, and a graph that holds the
+// address of one is replayed after later calls have needed more.  Whole models, on the host.
+#include "host_runtime.h"
+
+using host_runtime::memory;
+
+static int failures = 0;
+static void expect(int line, bool holds, const char *what) {
+  if (!holds) {
+    std::printf("line %d: %s\n", line, what);
+    ++failures;
+  }
+}
+#define EXPECT(holds) expect(__LINE__, holds, #holds)
+
+struct Model {
+  bdh_ctx *ctx = nullptr;
+  bdh_model *m = nullptr;
+  bdh_packed_weights encoder{}, encoder_v{}, decoder{};
+  std::vector<char *> held;  // what graphs hold
+  char *room = static_cast<char *>(host_runtime::device_address(size_t(1) << 40));
+  Model(int h, int N, int d, int type = BDH_INT8) {
+    EXPECT(bdh_ctx_create(0, host_runtime::stream(), &ctx) == BDH_OK);
+    bdh_model_config c{};
+    c.n_layer = 2;
+    c.n_embd = d;
+    c.n_head = h;
+    c.latent = N;
+    c.vocab = 256;
+    c.rotary = BDH_ROPE;
+    c.rope_theta = 65536.0f;
+    const float *w = reinterpret_cast<const float *>(room);
+    const bdh_model_weights weights{w, w, w, w, w};
+    EXPECT(bdh_model_create(ctx, &c, &weights, &m) == BDH_OK);
+    encoder = encoder_v = bdh_packed_weights{type, h, d, N, room + (1L << 36), w};
+    decoder = bdh_packed_weights{type, 1, h * N, d, room + (1L << 36), w};
+  }
+  ~Model() {
+    EXPECT(bdh_model_destroy(m) == BDH_OK && bdh_ctx_destroy(ctx) == BDH_OK);
+    EXPECT(memory().empty());
+  }
+  void pack() { EXPECT(bdh_model_set_packed(m, &encoder, &encoder_v, &decoder) == BDH_OK); }
+  void unpack() { EXPECT(bdh_model_set_packed(m, nullptr, nullptr, nullptr) == BDH_OK); }
+  void run(int B, int T) {
+    const int rc = bdh_model_forward(m, reinterpret_cast<int64_t *>(room), B, T, room + (1L << 37), BDH_F32, 0,
+                                     reinterpret_cast<float *>(room + (1L << 38)), nullptr, nullptr);
+    if (rc != BDH_OK) std::printf("%s\n", ctx->err);
+    EXPECT(rc == BDH_OK);
+  }
+  void fast(int B, int T) {
+    EXPECT(bdh_model_forward_fast(m, reinterpret_cast<int64_t *>(room), B, T, 0, reinterpret_cast<float *>(room + (1L << 38))) == BDH_OK);
+  }
+  void capture(int B) {
+    run(B, 1);  // sizes the buffers
+    host_runtime::capturing() = true;
+    run(B, 1);
+    host_runtime::capturing() = false;
+    held.push_back(static_cast<char *>(m->act));
+  }
+  bool kept() const {
+    for (char *b : held)
+      if (!memory().count(b)) return false;
+    return true;
+  }
+};
+
+int main() {
+  for (const int type : {int(BDH_INT8), int(BDH_BF16)}) {
+    {  // a step of f32 weights, then the prompt that ran before it, packed: it needs more than the one before
+      Model a(4, 8192, 256, type);
+      a.run(1, 64);
+      a.capture(1);
+      const void *act = a.m->act;
+      a.pack();
+      a.run(1, 64);
+      EXPECT(a.m->act != act);  // it did need more
+      EXPECT(a.kept());
+    }
+    {  // a small model's step, which had a buffer of its own in f32
+      Model a(4, 256, 256, type);
+      a.run(3, 20);
+      a.pack();
+      a.capture(3);
+      const void *act = a.m->act;
+      a.run(3, 400);
+      EXPECT(a.m->act != act);
+      EXPECT(a.kept());
+      a.capture(3);
+      a.fast(3, 900);
+      EXPECT(a.kept());
+    }
+  }
+  {  // f32 weights alone
+    Model a(4, 8192, 256);
+    a.capture(1);
+    a.run(2, 100);
+    a.run(2, 300);
+    EXPECT(a.kept());
+  }
+  {  // nothing captured: an outgrown buffer is let go of
+    Model a(4, 8192, 256);
+    a.run(1, 64);
+    const char *act = static_cast<const char *>(a.m->act);
+    a.run(1, 640);
+    EXPECT(a.m->act != act && !memory().count(const_cast<char *>(act)));
+  }
+  if (failures == 0) std::printf("ok\n");
+  return failures != 0;
+}
