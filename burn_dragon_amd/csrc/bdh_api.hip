@@ -22,26 +22,35 @@ bool bdh_capturing(bdh_ctx *ctx) {
   return true;  // unknown: a buffer too many is kept
 }
 
+namespace {
+
+// Lets go of a buffer: see bdh_grow.  (A capture may not wait for what came before it, so what it outgrows is kept too.)
+int let_go(bdh_ctx *ctx, void **buffer, size_t *held, bool *captured, bdh_outgrown **kept, bool capturing) {
+  if (*buffer && (capturing || *captured)) {
+    bdh_outgrown *o = new (std::nothrow) bdh_outgrown{*buffer, *kept};
+    if (!o) return bdh_fail(ctx, BDH_E_NOMEM, "host allocation failed");
+    *kept = o;
+  } else if (*buffer) {
+    BDH_HIP_CHECK(ctx, hipStreamSynchronize(ctx->stream));
+    BDH_HIP_CHECK(ctx, hipFree(*buffer));
+  }
+  *buffer = nullptr;
+  *held = 0;
+  *captured = false;
+  return BDH_OK;
+}
+
+}  // namespace
+
 int bdh_grow(bdh_ctx *ctx, const char *what, size_t bytes, void **buffer, size_t *held, bool *captured, bdh_outgrown **kept) {
   if (bytes <= *held) {
     if (*buffer && !*captured) *captured = bdh_capturing(ctx);
     return BDH_OK;
   }
-  const bool now = bdh_capturing(ctx);
+  const bool capturing = bdh_capturing(ctx);
   bytes = bdh_align_up(bytes, size_t(1) << 20);
-  if (*buffer) {
-    if (now || *captured) {  // (a capture may not wait for what came before it, either)
-      bdh_outgrown *o = new (std::nothrow) bdh_outgrown{*buffer, *kept};
-      if (!o) return bdh_fail(ctx, BDH_E_NOMEM, "host allocation failed");
-      *kept = o;
-    } else {
-      BDH_HIP_CHECK(ctx, hipStreamSynchronize(ctx->stream));
-      BDH_HIP_CHECK(ctx, hipFree(*buffer));
-    }
-    *buffer = nullptr;
-    *held = 0;
-    *captured = false;
-  }
+  const int rc = let_go(ctx, buffer, held, captured, kept, capturing);
+  if (rc != BDH_OK) return rc;
   const hipError_t e = hipMalloc(buffer, bytes);
   if (e != hipSuccess) {
     (void)hipGetLastError();
@@ -49,7 +58,7 @@ int bdh_grow(bdh_ctx *ctx, const char *what, size_t bytes, void **buffer, size_t
     return bdh_fail(ctx, BDH_E_NOMEM, "%s of %zu bytes: %s", what, bytes, hipGetErrorString(e));
   }
   *held = bytes;
-  *captured = now;
+  *captured = capturing;
   return BDH_OK;
 }
 
@@ -63,38 +72,23 @@ void bdh_free_outgrown(bdh_outgrown **kept) {
 }
 
 int bdh_ws_reserve(bdh_ctx *ctx, size_t bytes) {
-  if (bytes <= ctx->ws_bytes) return BDH_OK;
-  bytes = bdh_align_up(bytes, size_t(1) << 20);
-  if (ctx->opt_ws_max_mib > 0 && bytes > (size_t)ctx->opt_ws_max_mib << 20)
-    return bdh_fail(ctx, BDH_E_NOMEM, "workspace of %zu bytes: workspace.max_mib is %d", bytes, ctx->opt_ws_max_mib);
-  if (ctx->ws) {
-    BDH_HIP_CHECK(ctx, hipStreamSynchronize(ctx->stream));
-    BDH_HIP_CHECK(ctx, hipFree(ctx->ws));
-    ctx->ws = nullptr;
-    ctx->ws_bytes = 0;
-  }
-  hipError_t e = hipMalloc(&ctx->ws, bytes);
-  if (e != hipSuccess) {
-    (void)hipGetLastError();
-    return bdh_fail(ctx, BDH_E_NOMEM, "workspace of %zu bytes: %s", bytes, hipGetErrorString(e));
-  }
-  ctx->ws_bytes = bytes;
-  return BDH_OK;
+  const size_t whole = bdh_align_up(bytes, size_t(1) << 20);
+  if (bytes > ctx->ws_bytes && ctx->opt_ws_max_mib > 0 && whole > (size_t)ctx->opt_ws_max_mib << 20)
+    return bdh_fail(ctx, BDH_E_NOMEM, "workspace of %zu bytes: workspace.max_mib is %d", whole, ctx->opt_ws_max_mib);
+  return bdh_grow(ctx, "workspace", bytes, &ctx->ws, &ctx->ws_bytes, &ctx->ws_captured, &ctx->outgrown);
 }
 
 int bdh_ws_reserve_room(bdh_ctx *ctx, size_t bytes, size_t most) {
   most = bdh_align_up(most, size_t(1) << 20);
   if (most > ctx->ws_bytes && (ctx->ws_refused == 0 || most < ctx->ws_refused) &&
       (ctx->opt_ws_max_mib == 0 || most <= (size_t)ctx->opt_ws_max_mib << 20)) {
-    hipStreamCaptureStatus status = hipStreamCaptureStatusActive;  // a call that is captured takes what is there, if it is enough
-    const bool known = hipStreamIsCapturing(ctx->stream, &status) == hipSuccess;
-    if (!known) (void)hipGetLastError();
+    if (bdh_capturing(ctx)) return bdh_ws_reserve(ctx, bytes);  // a call that is captured takes what is there, if it is enough
     void *larger = nullptr;
-    if (!known || status != hipStreamCaptureStatusNone) return bdh_ws_reserve(ctx, bytes);
     if (hipMalloc(&larger, most) == hipSuccess) {
-      if (ctx->ws) {
-        BDH_HIP_CHECK(ctx, hipStreamSynchronize(ctx->stream));
-        BDH_HIP_CHECK(ctx, hipFree(ctx->ws));
+      const int rc = let_go(ctx, &ctx->ws, &ctx->ws_bytes, &ctx->ws_captured, &ctx->outgrown, false);
+      if (rc != BDH_OK) {
+        (void)hipFree(larger);
+        return rc;
       }
       ctx->ws = larger;
       ctx->ws_bytes = most;
@@ -107,21 +101,7 @@ int bdh_ws_reserve_room(bdh_ctx *ctx, size_t bytes, size_t most) {
 }
 
 int bdh_stage_reserve(bdh_ctx *ctx, size_t bytes) {
-  if (bytes <= ctx->stage_bytes) return BDH_OK;
-  bytes = bdh_align_up(bytes, size_t(1) << 20);
-  if (ctx->stage) {
-    BDH_HIP_CHECK(ctx, hipStreamSynchronize(ctx->stream));
-    BDH_HIP_CHECK(ctx, hipFree(ctx->stage));
-    ctx->stage = nullptr;
-    ctx->stage_bytes = 0;
-  }
-  hipError_t e = hipMalloc(&ctx->stage, bytes);
-  if (e != hipSuccess) {
-    (void)hipGetLastError();
-    return bdh_fail(ctx, BDH_E_NOMEM, "staging buffer of %zu bytes: %s", bytes, hipGetErrorString(e));
-  }
-  ctx->stage_bytes = bytes;
-  return BDH_OK;
+  return bdh_grow(ctx, "staging buffer", bytes, &ctx->stage, &ctx->stage_bytes, &ctx->stage_captured, &ctx->outgrown);
 }
 
 extern "C" {
@@ -175,9 +155,10 @@ int bdh_ctx_create(int device_id, void *hip_stream, bdh_ctx **out) {
 
 int bdh_ctx_destroy(bdh_ctx *ctx) {
   if (!ctx) return BDH_OK;
-  if (ctx->ws || ctx->fsa_mask || ctx->lat_mask || ctx->stage) (void)hipStreamSynchronize(ctx->stream);
+  if (ctx->ws || ctx->fsa_mask || ctx->lat_mask || ctx->stage || ctx->outgrown) (void)hipStreamSynchronize(ctx->stream);
   if (ctx->stage) (void)hipFree(ctx->stage);
   if (ctx->ws) (void)hipFree(ctx->ws);
+  bdh_free_outgrown(&ctx->outgrown);
   if (ctx->fsa_mask) (void)hipFree(ctx->fsa_mask);
   if (ctx->lat_mask) (void)hipFree(ctx->lat_mask);
   delete ctx;

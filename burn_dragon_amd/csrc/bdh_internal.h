@@ -26,9 +26,12 @@ struct bdh_ctx {
   void *ws = nullptr;
   size_t ws_bytes = 0;
   size_t ws_refused = 0;  // what bdh_ws_reserve_room last asked for in vain
+  bool ws_captured = false;  // a captured call was given it
   // a second growable buffer for inputs a launcher converts before it calls a path that sizes ctx->ws itself
   void *stage = nullptr;
   size_t stage_bytes = 0;
+  bool stage_captured = false;
+  bdh_outgrown *outgrown = nullptr;
   int n_cu = 0;
   int opt_step_split = -1;  // -1 choose by grid size, 0 / 1 force the 256- / 64-pair workgroup
   int opt_step_dense = -1;  // many-token state step as dense f32 products: -1 by dense_form_from, 0 never, 1 always
@@ -105,10 +108,10 @@ bool bdh_capturing(bdh_ctx *ctx);
 int bdh_grow(bdh_ctx *ctx, const char *what, size_t bytes, void **buffer, size_t *held, bool *captured, bdh_outgrown **kept);
 void bdh_free_outgrown(bdh_outgrown **kept);
 
-// Grows ctx->ws to at least `bytes` (synchronises the stream before freeing the old one).
+// Grows ctx->ws to at least `bytes`, by bdh_grow.
 int bdh_ws_reserve(bdh_ctx *ctx, size_t bytes);
 // The same for a call that needs `bytes` now, and `most` at the most where it is repeated with other arguments of the same shape:
-// room for all of them is made at once, so that the workspace stays where it is (a captured graph may hold its address).  Where
+// room for all of them is made at once, so that the workspace does not move from call to call.  Where
 // there is no memory for `most`, what is needed now is enough, and so much is not asked for again.
 int bdh_ws_reserve_room(bdh_ctx *ctx, size_t bytes, size_t most);
 // The same as bdh_ws_reserve for ctx->stage.

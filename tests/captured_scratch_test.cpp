@@ -17,7 +17,7 @@ struct Model {
   bdh_ctx *ctx = nullptr;
   bdh_model *m = nullptr;
   bdh_packed_weights encoder{}, encoder_v{}, decoder{};
-  std::vector<char *> held;  // what graphs hold
+  std::vector<char *> held;  // what graphs may hold
   char *room = static_cast<char *>(host_runtime::device_address(size_t(1) << 40));
   Model(int h, int N, int d, int type = BDH_INT8) {
     EXPECT(bdh_ctx_create(0, host_runtime::stream(), &ctx) == BDH_OK);
@@ -55,7 +55,7 @@ struct Model {
     host_runtime::capturing() = true;
     run(B, 1);
     host_runtime::capturing() = false;
-    held.push_back(static_cast<char *>(m->act));
+    for (const auto &b : memory()) held.push_back(b.first);
   }
   bool kept() const {
     for (char *b : held)
@@ -75,6 +75,8 @@ int main() {
       a.run(1, 64);
       EXPECT(a.m->act != act);  // it did need more
       EXPECT(a.kept());
+      for (int k = 3; k < 6; ++k) a.run(1, 64 * k);
+      EXPECT(a.kept());
     }
     {  // a small model's step, which had a buffer of its own in f32
       Model a(4, 256, 256, type);
@@ -90,19 +92,40 @@ int main() {
       EXPECT(a.kept());
     }
   }
-  {  // f32 weights alone
+  {  // f32 weights alone; and a packed step before f32 prompts, whose encoder takes parts in the context's workspace
     Model a(4, 8192, 256);
     a.capture(1);
+    const void *ws = a.ctx->ws;
     a.run(2, 100);
     a.run(2, 300);
+    EXPECT(a.ctx->ws != ws && a.kept());
+    a.pack();
+    a.capture(40);
+    a.unpack();
+    a.run(40, 1);
+    a.run(3, 500);
     EXPECT(a.kept());
+  }
+  {  // the room that shared states ask for, and the staging buffer
+    bdh_ctx *ctx = nullptr;
+    EXPECT(bdh_ctx_create(0, host_runtime::stream(), &ctx) == BDH_OK);
+    EXPECT(bdh_ws_reserve(ctx, 100) == BDH_OK && bdh_stage_reserve(ctx, 100) == BDH_OK);
+    host_runtime::capturing() = true;
+    EXPECT(bdh_ws_reserve(ctx, 50) == BDH_OK && bdh_stage_reserve(ctx, 50) == BDH_OK);
+    host_runtime::capturing() = false;
+    char *ws = static_cast<char *>(ctx->ws), *stage = static_cast<char *>(ctx->stage);
+    EXPECT(bdh_ws_reserve_room(ctx, 1 << 21, 1 << 23) == BDH_OK && ctx->ws != ws && memory().count(ws));
+    EXPECT(bdh_stage_reserve(ctx, 1 << 21) == BDH_OK && ctx->stage != stage && memory().count(stage));
+    ws = static_cast<char *>(ctx->ws);
+    EXPECT(bdh_ws_reserve_room(ctx, 1 << 24, 1 << 25) == BDH_OK && ctx->ws != ws && !memory().count(ws));  // never captured
+    EXPECT(bdh_ctx_destroy(ctx) == BDH_OK && memory().empty());
   }
   {  // nothing captured: an outgrown buffer is let go of
     Model a(4, 8192, 256);
     a.run(1, 64);
-    const char *act = static_cast<const char *>(a.m->act);
+    char *act = static_cast<char *>(a.m->act), *ws = static_cast<char *>(a.ctx->ws);
     a.run(1, 640);
-    EXPECT(a.m->act != act && !memory().count(const_cast<char *>(act)));
+    EXPECT(a.m->act != act && !memory().count(act) && a.ctx->ws != ws && !memory().count(ws));
   }
   if (failures == 0) std::printf("ok\n");
   return failures != 0;
