@@ -785,27 +785,18 @@ extern "C" int bdh_fused_state_aligned(bdh_ctx *ctx, int B, int h, int T, int N,
     key.reserve(2 * (size_t)n_pairs + 1);
     key.push_back(tb);
     key.insert(key.end(), block_pairs_host, block_pairs_host + 2 * (size_t)n_pairs);
-    if (!ctx->fsa_mask || ctx->fsa_mask_key != key) {
-      std::vector<unsigned char> m((size_t)tb * tb, 0);
+    const bool same = ctx->fsa_mask && ctx->fsa_mask_key == key;
+    std::vector<unsigned char> m;
+    if (!same) {
+      m.assign((size_t)tb * tb, 0);
       for (int p = 0; p < n_pairs; ++p) {
         const int r = block_pairs_host[2 * p], c = block_pairs_host[2 * p + 1];
         if (r >= 0 && r < tb && c >= 0 && c < tb) m[(size_t)r * tb + c] = 1;  // iter_cols drops c >= total_blocks
       }
-      BDH_HIP_CHECK(ctx, hipStreamSynchronize(ctx->stream));  // earlier calls may still read the old mask
-      if (ctx->fsa_mask_bytes < m.size()) {
-        if (ctx->fsa_mask) BDH_HIP_CHECK(ctx, hipFree(ctx->fsa_mask));
-        ctx->fsa_mask = nullptr;
-        ctx->fsa_mask_bytes = 0;
-        ctx->fsa_mask_key.clear();
-        if (hipMalloc(&ctx->fsa_mask, m.size()) != hipSuccess) {
-          (void)hipGetLastError();
-          return bdh_fail(ctx, BDH_E_NOMEM, "time-block mask of %zu bytes", m.size());
-        }
-        ctx->fsa_mask_bytes = m.size();
-      }
-      BDH_HIP_CHECK(ctx, hipMemcpy(ctx->fsa_mask, m.data(), m.size(), hipMemcpyHostToDevice));
-      ctx->fsa_mask_key = std::move(key);
     }
+    const int mask_rc = bdh_mask_on_device(ctx, m.data(), m.size(), same, &ctx->fsa_mask, &ctx->fsa_mask_bytes, &ctx->fsa_mask_captured);
+    if (mask_rc != BDH_OK) return mask_rc;
+    if (!same) ctx->fsa_mask_key = std::move(key);
     active = static_cast<unsigned char *>(ctx->fsa_mask);
   }
   const float *q = query;  // ALiBi does not rotate

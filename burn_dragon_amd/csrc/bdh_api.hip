@@ -62,6 +62,27 @@ int bdh_grow(bdh_ctx *ctx, const char *what, size_t bytes, void **buffer, size_t
   return BDH_OK;
 }
 
+int bdh_mask_on_device(bdh_ctx *ctx, const unsigned char *mask, size_t n, bool same, void **buffer, size_t *held, bool *captured) {
+  const bool capturing = bdh_capturing(ctx);
+  if (!same || !*buffer) {
+    if (capturing) return bdh_fail(ctx, BDH_E_UNSUPPORTED, "a block pattern is copied to the device: run the call once before capturing it");
+    if (*captured) {
+      const int rc = let_go(ctx, buffer, held, captured, &ctx->outgrown, false);
+      if (rc != BDH_OK) return rc;
+    }
+    BDH_HIP_CHECK(ctx, hipStreamSynchronize(ctx->stream));
+    const int rc = bdh_grow(ctx, "block mask", n + 256, buffer, held, captured, &ctx->outgrown);
+    if (rc != BDH_OK) return rc;
+    const hipError_t e = n > 0 ? hipMemcpy(*buffer, mask, n, hipMemcpyHostToDevice) : hipSuccess;
+    if (e != hipSuccess) {
+      (void)let_go(ctx, buffer, held, captured, &ctx->outgrown, false);  // no key names what it holds now
+      return bdh_fail(ctx, BDH_E_HIP, "block mask: %s", hipGetErrorString(e));
+    }
+  }
+  *captured = *captured || capturing;
+  return BDH_OK;
+}
+
 void bdh_free_outgrown(bdh_outgrown **kept) {
   while (*kept) {
     bdh_outgrown *o = *kept;

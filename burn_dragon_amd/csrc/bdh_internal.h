@@ -53,10 +53,12 @@ struct bdh_ctx {
   // time-block mask of the last sparse fused_state_aligned pattern (device) and the pattern it was built from
   void *fsa_mask = nullptr;
   size_t fsa_mask_bytes = 0;
+  bool fsa_mask_captured = false;
   std::vector<int> fsa_mask_key;
   // latent block mask of the last relu_lowrank call that had one (device) and the bytes it was built from
   void *lat_mask = nullptr;
   size_t lat_mask_bytes = 0;
+  bool lat_mask_captured = false;
   std::vector<uint8_t> lat_mask_key;
   char err[512] = {0};
 };
@@ -107,6 +109,9 @@ bool bdh_capturing(bdh_ctx *ctx);
 // stream, unless a captured call may have been given it: then it goes to `kept`.
 int bdh_grow(bdh_ctx *ctx, const char *what, size_t bytes, void **buffer, size_t *held, bool *captured, bdh_outgrown **kept);
 void bdh_free_outgrown(bdh_outgrown **kept);
+// The device copy of a mask of n bytes: the one that `key` was copied to, if that is this mask, or a new copy, behind a wait for
+// the calls that may still read the old one.  A copy that a captured call may have been given stays as it is.
+int bdh_mask_on_device(bdh_ctx *ctx, const unsigned char *mask, size_t n, bool same, void **buffer, size_t *held, bool *captured);
 
 // Grows ctx->ws to at least `bytes`, by bdh_grow.
 int bdh_ws_reserve(bdh_ctx *ctx, size_t bytes);

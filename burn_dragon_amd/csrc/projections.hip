@@ -1135,22 +1135,9 @@ int bdh_launch_relu_lowrank(bdh_ctx *ctx, const ReluLowrankParams &p) {
     const size_t nb = (size_t)std::max(p.n_blocks, 0);
     const bool same = ctx->lat_mask && ctx->lat_mask_key.size() == nb &&
                       (nb == 0 || memcmp(ctx->lat_mask_key.data(), p.active_blocks_host, nb) == 0);
-    if (!same) {
-      BDH_HIP_CHECK(ctx, hipStreamSynchronize(ctx->stream));
-      if (ctx->lat_mask_bytes < nb + 256) {
-        if (ctx->lat_mask) BDH_HIP_CHECK(ctx, hipFree(ctx->lat_mask));
-        ctx->lat_mask = nullptr;
-        ctx->lat_mask_bytes = 0;
-        ctx->lat_mask_key.clear();
-        if (hipMalloc(&ctx->lat_mask, nb + 256) != hipSuccess) {
-          (void)hipGetLastError();
-          return bdh_fail(ctx, BDH_E_NOMEM, "latent block mask of %zu bytes", nb);
-        }
-        ctx->lat_mask_bytes = nb + 256;
-      }
-      if (nb > 0) BDH_HIP_CHECK(ctx, hipMemcpy(ctx->lat_mask, p.active_blocks_host, nb, hipMemcpyHostToDevice));
-      ctx->lat_mask_key.assign(p.active_blocks_host, p.active_blocks_host + nb);
-    }
+    const int rc = bdh_mask_on_device(ctx, p.active_blocks_host, nb, same, &ctx->lat_mask, &ctx->lat_mask_bytes, &ctx->lat_mask_captured);
+    if (rc != BDH_OK) return rc;
+    if (!same) ctx->lat_mask_key.assign(p.active_blocks_host, p.active_blocks_host + nb);
     mask_dev = static_cast<const unsigned char *>(ctx->lat_mask);
   }
   // D_y of a prompt has no order to keep (it decides no active set): split-bf16 products where those are faster

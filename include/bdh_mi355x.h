@@ -22,7 +22,8 @@
  *     (hipSetDevice) on the calling thread for every call that takes the context or a model of it.
  *   - Entry points may grow the context's workspace (hipMalloc) the first time a shape is seen: run a
  *     step of each shape once before capturing calls in a HIP graph.  A workspace, or a model's scratch, that a captured
- *     call was given stays until the context, or the model, is destroyed, whatever later calls need.
+ *     call was given stays until the context, or the model, is destroyed, whatever later calls need.  So does the device's
+ *     copy of a block pattern; a pattern that the context has not just been called with is refused under capture.
  *   - There is no CPU fallback: without a HIP device every compute entry point fails.
  *   - State (`rho`) and output (`out`) buffers are ordinary device memory (hipMalloc: coarse-grained), the kind
  *     every kernel here is built and measured for.  Calls of many tokens read each element of the state, add the

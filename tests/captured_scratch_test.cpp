@@ -120,6 +120,38 @@ int main() {
     EXPECT(bdh_ws_reserve_room(ctx, 1 << 24, 1 << 25) == BDH_OK && ctx->ws != ws && !memory().count(ws));  // never captured
     EXPECT(bdh_ctx_destroy(ctx) == BDH_OK && memory().empty());
   }
+  {  // block masks: a captured one is neither freed nor written again, and none is made under capture
+    bdh_ctx *ctx = nullptr;
+    EXPECT(bdh_ctx_create(0, host_runtime::stream(), &ctx) == BDH_OK);
+    static uint8_t blocks[2000];
+    static int32_t pairs[2000];
+    float *f = static_cast<float *>(host_runtime::device_address(size_t(1) << 30));
+    auto lowrank = [&](int n, int active) {
+      for (int i = 0; i < n; ++i) blocks[i] = i == active;
+      return bdh_relu_lowrank(ctx, 1, 1, 2, 32, 1, 8 * n, f, f, nullptr, 0.0f, 8, blocks, n, nullptr, f + (1 << 24));
+    };
+    auto aligned = [&](int tb, int column) {
+      pairs[0] = tb - 1;
+      pairs[1] = column;
+      return bdh_fused_state_aligned(ctx, 1, 1, 4 * tb, 32, 16, f, f, f, nullptr, 4, pairs, 1, BDH_ROPE, 0, f + (1 << 24));
+    };
+    for (const bool time : {false, true}) {
+      auto call = [&](int n, int which) { return time ? aligned(n, which) : lowrank(n, which); };
+      void *&mask = time ? ctx->fsa_mask : ctx->lat_mask;
+      EXPECT(call(4, 1) == BDH_OK);
+      char *first = static_cast<char *>(mask);
+      EXPECT(call(4, 2) == BDH_OK && mask == first);  // no graph holds it
+      host_runtime::capturing() = true;
+      EXPECT(call(4, 2) == BDH_OK && mask == first);
+      EXPECT(call(4, 3) == BDH_E_UNSUPPORTED && mask == first);
+      host_runtime::capturing() = false;
+      EXPECT(call(4, 2) == BDH_OK && mask == first);
+      EXPECT(call(4, 1) == BDH_OK && mask != first && memory().count(first));
+      char *second = static_cast<char *>(mask);
+      EXPECT(call(time ? 40 : 900, 1) == BDH_OK && mask == second && memory().count(first));
+    }
+    EXPECT(bdh_ctx_destroy(ctx) == BDH_OK && memory().empty());
+  }
   {  // nothing captured: an outgrown buffer is let go of
     Model a(4, 8192, 256);
     a.run(1, 64);
