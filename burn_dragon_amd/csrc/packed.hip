@@ -1246,6 +1246,16 @@ bool overlap(const void *a, size_t na, const void *b, size_t nb) {
   return p && q && p < q + nb && q < p + na;
 }
 
+// Whether rows of `na` bytes from a on and rows of `nb` bytes from b on share a byte; where both lie `pitch` bytes apart they may be
+// columns of one buffer.
+bool rows_overlap(const void *a, size_t na, size_t pitch_a, const void *b, size_t nb, size_t pitch_b, size_t rows) {
+  if (!overlap(a, (rows - 1) * pitch_a + na, b, (rows - 1) * pitch_b + nb)) return false;
+  if (pitch_a != pitch_b || rows == 1) return true;
+  const uintptr_t p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b);
+  const size_t apart = q >= p ? (q - p) % pitch_a : (pitch_a - (p - q) % pitch_a) % pitch_a;  // from a row of a to the next of b
+  return apart < na || apart + nb > pitch_a;
+}
+
 // rows_out rows of out; what else of p is checked by the entry points
 int run_product(bdh_ctx *ctx, const Call &c, const Product &p, int64_t rows_out) {
   const bdh_packed_weights &w = *c.w;
@@ -1273,9 +1283,14 @@ int run_product(bdh_ctx *ctx, const Call &c, const Product &p, int64_t rows_out)
   const struct {
     const void *p;
     size_t bytes;
-  } reads[] = {{c.x, x_bytes}, {w.data, bdh_packed_bytes(w.type, w.groups, w.inner, w.outer)}, {w.scales, channels}, {p.bias, channels},
+  } reads[] = {{w.data, bdh_packed_bytes(w.type, w.groups, w.inner, w.outer)}, {w.scales, channels}, {p.bias, channels},
                {p.gate, value_bytes(p.gate_dtype) * (size_t)rows_out * w.outer},
                {p.offsets, sizeof(int32_t) * ((size_t)w.groups + 1)}};
+  const bool columns = c.rows_in == rows_out && !p.token_major &&
+                       !rows_overlap(c.x, value_bytes(c.x_dtype) * w.inner, value_bytes(c.x_dtype) * c.x_stride, p.out,
+                                     value_bytes(p.out_dtype) * w.outer, value_bytes(p.out_dtype) * p.out_stride, rows_out);
+  if ((!columns && overlap(c.x, x_bytes, p.out, out_bytes)) || (need > 0 && overlap(c.x, x_bytes, c.workspace, need)))
+    return bdh_fail(ctx, BDH_E_INVAL, "out or the workspace overlaps the rows");
   for (const auto &r : reads)
     if (overlap(r.p, r.bytes, p.out, out_bytes) || (need > 0 && overlap(r.p, r.bytes, c.workspace, need)))
       return bdh_fail(ctx, BDH_E_INVAL, "out or the workspace overlaps what the product reads");
