@@ -1152,6 +1152,9 @@ int launch_few(bdh_ctx *ctx, Product p, const RowsIn &in) {
   if (p.splits > 1) {
     if constexpr (W == 4 && (!PRE || TYPE == BDH_BF16))
       hipLaunchKernelGGL((k_packed_few<TYPE, kParts, MT, W, U, PRE>), grid, threads, 0, ctx->stream, p, in);
+  } else if constexpr (PRE && TYPE == BDH_INT8 && W == 8) {  // one group of a grouped product; other calls cut such a k into parts
+    if (p.relu) return bdh_fail(ctx, BDH_E_UNSUPPORTED, "prepared rows of 8 wavefronts have no ReLU");
+    hipLaunchKernelGGL((k_packed_few<TYPE, kScales, MT, W, U, PRE>), grid, threads, 0, ctx->stream, p, in);
   } else {
     with_behind(p, [&](auto behind) {
       hipLaunchKernelGGL((k_packed_few<TYPE, decltype(behind)::value, MT, W, U, PRE>), grid, threads, 0, ctx->stream, p, in);
@@ -1203,14 +1206,18 @@ int launch_product(bdh_ctx *ctx, const Call &c, const Plan &plan, Product p) {
   if (plan.few) {
     auto launch = [&](auto pre) {
       constexpr bool PRE = decltype(pre)::value;
-      if (plan.waves == 8) {
+      if constexpr (PRE && TYPE == BDH_INT8) {  // rows are prepared where there are more than 16 of them and k takes more than two turns
+        if (plan.mt == 4) return launch_few<TYPE, 4, 8, 1, PRE>(ctx, p, in);
+        return plan.waves == 8 ? launch_few<TYPE, 2, 8, 2, PRE>(ctx, p, in) : launch_few<TYPE, 2, 4, 2, PRE>(ctx, p, in);
+      } else if (plan.waves == 8) {
         if (plan.mt == 1) return plan.one ? launch_few<TYPE, 1, 8, 1, PRE>(ctx, p, in) : launch_few<TYPE, 1, 8, 4, PRE>(ctx, p, in);
         if (plan.mt == 2) return plan.one ? launch_few<TYPE, 2, 8, 1, PRE>(ctx, p, in) : launch_few<TYPE, 2, 8, 2, PRE>(ctx, p, in);
         return launch_few<TYPE, 4, 8, 1, PRE>(ctx, p, in);
+      } else {
+        if (plan.mt == 1) return plan.one ? launch_few<TYPE, 1, 4, 1, PRE>(ctx, p, in) : launch_few<TYPE, 1, 4, 4, PRE>(ctx, p, in);
+        if (plan.mt == 2) return plan.one ? launch_few<TYPE, 2, 4, 1, PRE>(ctx, p, in) : launch_few<TYPE, 2, 4, 2, PRE>(ctx, p, in);
+        return launch_few<TYPE, 4, 4, 1, PRE>(ctx, p, in);
       }
-      if (plan.mt == 1) return plan.one ? launch_few<TYPE, 1, 4, 1, PRE>(ctx, p, in) : launch_few<TYPE, 1, 4, 4, PRE>(ctx, p, in);
-      if (plan.mt == 2) return plan.one ? launch_few<TYPE, 2, 4, 1, PRE>(ctx, p, in) : launch_few<TYPE, 2, 4, 2, PRE>(ctx, p, in);
-      return launch_few<TYPE, 4, 4, 1, PRE>(ctx, p, in);
     };
     if (plan.top_parts) {
       const long tops = (long)c.rows_in * plan.top_parts;
