@@ -9,6 +9,8 @@ import pytest
 
 from burn_dragon_amd import build
 
+from .packed_shapes import COMPANY, PROMPTS, TILES, prompt_lines
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 
 
@@ -80,3 +82,37 @@ def test_what_comes_behind_the_sums_is_the_calls(plan):
         a = line.split()
         want = 0 if a[0] != "lowrank" else 2 if a[9] != "-1" or a[11] == "1" or float(a[12]) else 1
         assert behind == want, (line, kernels)
+
+
+def _short(kernels):
+    return [k.replace(", ", ",").replace("unsigned short", "bf16") for k in kernels]
+
+
+def test_the_sizes_of_the_tests_take_the_kernels_they_are_for(plan):
+    launched, compiled = plan([line for line, _ in TILES])
+    assert [(line, " ".join(_short(k))) for (line, _), k in zip(TILES, launched)] == TILES
+    ends = {k for k in compiled if re.match(r"k_packed_tile|k_packed_finish|k_packed_few<2, \d, \d, \d, \d, true>", k)}
+    assert ends - {k for ks in launched for k in ks} == set()
+
+
+def test_rows_that_are_compared_take_different_kernels(plan):
+    kernels = set()
+    for K, N, rows in COMPANY:
+        launched = plan([f"product 2 {K} {N} {M} 0 {K} 0 {N}" for M in rows])[0]
+        assert len({k for ks in launched for k in ks}) >= len(rows) // 2
+        kernels |= {re.sub(r"<2,(\d),.*?((\d+),(\d+),\d,\d)?>", r"\1 \3x\4", k) for ks in launched for k in _short(ks)}
+    assert {"k_packed_tile0 64x64", "k_packed_tile0 64x128", "k_packed_tile0 128x256", "k_packed_tile0 256x256", "k_packed_tile3 64x64",
+            "k_packed_tile3 128x256"} <= kernels
+    assert any(k.startswith("k_packed_few0") for k in kernels) and any(k.startswith("k_packed_few3") for k in kernels)
+
+
+def test_prompts_of_models_go_through_tiles_and_parts(plan):
+    lines = [l for p in PROMPTS for l in prompt_lines(*p)]
+    launched = [" ".join(_short(k)) for k in plan(lines)[0]]
+    for name, which in (("D_y in tiles for gates", [re.search(r"tile<\d,2,\w+,128,128", k) for k in launched[1::3]]),
+                        ("D_y in other tiles", [re.search(r"tile<\d,2,\w+,64,64", k) for k in launched[1::3]]),
+                        ("D_y in parts", [re.search(r"finish<\d,2", k) for k in launched[1::3]]),
+                        ("D_x in tiles", [re.search(r"tile<\d,1", k) for k in launched[::3]]),
+                        ("E in tiles", [re.search(r"tile<\d,0", k) for k in launched[2::3]]),
+                        ("E in parts", [re.search(r"finish<\d,0", k) for k in launched[2::3]])):
+        assert any(which), name
