@@ -110,6 +110,9 @@ class BDH:
 
             packed = [PackedWeights(self.params[n], dtype, self.ctx) for n in ("encoder", "encoder_v", "decoder")]
         self.ctx.check(self.ctx.lib.bdh_model_set_packed(self.handle, *([None] * 3 if packed is None else [w._ref for w in packed])))
+        with self.ctx.torch_stream():  # calls queued there may still read the old ones, which another stream may have made
+            for w in self.packed or ():
+                w.used_on(torch.cuda.current_stream(self.device))
         self.packed = packed
 
     def init_state(self) -> ModelState:

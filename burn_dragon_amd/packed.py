@@ -45,6 +45,13 @@ class PackedWeights:
                 break
             self.few = n
 
+    def used_on(self, stream: torch.cuda.Stream) -> None:
+        """Calls on `stream` use these weights: when they are dropped, their memory is given to others behind what is queued there
+        by then (Tensor.record_stream).  For weights that are dropped while another stream than the one that made them works."""
+        for t in (self.data, self.scales):
+            if t is not None:
+                t.record_stream(stream)
+
     @property
     def nbytes(self) -> int:
         return self.data.numel() + (0 if self.scales is None else 4 * self.scales.numel())

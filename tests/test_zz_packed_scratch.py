@@ -1,11 +1,13 @@
-"""Captured steps of models whose later calls need more scratch than the ones before the capture."""
+"""Captured steps of models whose later calls need more scratch than the ones before the capture, and packed weights that are replaced while
+a stream reads them."""
 import pytest
 import torch
 
 from oracle import bdh_oracle as orc
 
-from .test_gpu_packed import BF16, INT8, gen
+from .test_gpu_packed import BF16, DEV, INT8, gen
 from .test_zz_packed_model import _copied, build
+from .test_zz_packed_prompts import _model
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +57,27 @@ def test_a_captured_step_of_a_small_packed_model_goes_on_beside_longer_prompts()
     state = model.init_state()
     _, token = model.forward_with_state(tokens, state, want_next=True)
     _goes_on(model, state, token, lambda k: model.forward_with_state(tokens.repeat(1, 1 + 10 * k), model.init_state()))
+
+
+def test_weights_that_are_replaced_while_a_stream_reads_them():
+    """Memory of the old packed weights is not given to the stream that made them while another one's calls are queued."""
+    model = _model(INT8, 4, 256, 1024)
+    tokens = torch.randint(0, 50, (2, 100), device=DEV)
+    want = model.forward_with_state(tokens, model.init_state())
+    torch.cuda.synchronize()
+    old = [(w.data.data_ptr(), w.data.numel()) for w in model.packed]
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        model.forward_with_state(tokens, model.init_state())
+        torch.cuda.synchronize()
+        torch.cuda._sleep(1_000_000_000)
+        held = torch.cuda.Event()
+        held.record()
+        got = model.forward_with_state(tokens, model.init_state())
+        model.pack_projections(None)
+    taken = [torch.full((n,), 99, device=DEV, dtype=torch.uint8) for _, n in old for _ in range(2)]
+    places = {t.data_ptr() for t in taken}
+    assert not held.query(), "the wait was too short to show anything"
+    torch.cuda.synchronize()
+    assert not places & {p for p, _ in old}
+    assert torch.equal(got, want)
