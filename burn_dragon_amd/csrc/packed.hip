@@ -978,6 +978,7 @@ int check_weights(bdh_ctx *ctx, const bdh_packed_weights *w) {
   if (w->groups > kMostGroups) return bdh_fail(ctx, BDH_E_SHAPE, "%d groups > %d", w->groups, kMostGroups);
   if (w->inner > kMostInner) return bdh_fail(ctx, BDH_E_SHAPE, "inner dimension %d > %d", w->inner, kMostInner);
   if (w->outer > (1 << 24)) return bdh_fail(ctx, BDH_E_SHAPE, "outer dimension %d > 2^24", w->outer);
+  if (!bdh_aligned(w->scales, 4)) return bdh_fail(ctx, BDH_E_ALIGN, "scales need the alignment of their values");  // atomics make them
   return BDH_OK;
 }
 

@@ -116,3 +116,8 @@ def test_prompts_of_models_go_through_tiles_and_parts(plan):
                         ("E in tiles", [re.search(r"tile<\d,0", k) for k in launched[2::3]]),
                         ("E in parts", [re.search(r"finish<\d,0", k) for k in launched[2::3]])):
         assert any(which), name
+
+
+def test_scales_are_aligned(tmp_path):
+    done = subprocess.run([program(tmp_path, "packed_alignment_test")], capture_output=True, text=True)
+    assert done.returncode == 0 and done.stdout == "ok\n", (done.returncode, done.stdout, done.stderr)
