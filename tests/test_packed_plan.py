@@ -31,14 +31,16 @@ INT8, BF16, F32 = 2, 1, 0
 
 @pytest.fixture(scope="module")
 def plan(tmp_path_factory):
-    """Lines of packed_plan.cpp -> the kernels that each call launches, and all there are."""
+    """Lines of packed_plan.cpp -> the kernels that each call launches (with their grids, if asked), and all there are."""
     exe = program(tmp_path_factory.mktemp("plan"), "packed_plan")
 
-    def run(lines):
+    def run(lines, grids=False):
         done = subprocess.run([exe], input="\n".join([*lines, "kernels"]) + "\n", capture_output=True, text=True)
         out = done.stdout.split("\n")
         assert done.returncode == 0 and len(out) > len(lines), done.stderr
         compiled = {k for k in out[len(lines):] if re.match("k_packed|k_prepare_rows|k_row_tops", k)}
+        if grids:
+            return out[:len(lines)]
         return [l if l.startswith("refused") else [re.sub(r" x\d+$", "", k) for k in l.split(" + ")] for l in out[:len(lines)]], compiled
 
     return run
@@ -121,3 +123,13 @@ def test_prompts_of_models_go_through_tiles_and_parts(plan):
 def test_scales_are_aligned(tmp_path):
     done = subprocess.run([program(tmp_path, "packed_alignment_test")], capture_output=True, text=True)
     assert done.returncode == 0 and done.stdout == "ok\n", (done.returncode, done.stdout, done.stderr)
+
+
+def test_groups_without_rows_have_no_workgroups(plan):
+    """At most a tile for each whole 16, 32, 64, 128 or 256 rows and one more for each group that can have rows."""
+    cases = [(G, M, N) for G in (1, 7, 64, 1000, 65535) for M in (1, 5, 16, 40, 300, 5000) for N in (64, 200)]
+    for (G, M, N), line in zip(cases, plan([f"grouped 2 {G} 64 {N} {M} 0 64 0 {N}" for G, M, N in cases], grids=True)):
+        kernel, grid = re.match(r"(?:.* \+ )?k_packed_(.*) x(\d+)$", line).groups()
+        few = re.match(r"few<2, 0, (\d)", kernel)
+        rows, wide = (16 * int(few.group(1)), 64) if few else map(int, re.search(r"(\d+), (\d+), \d, \d>", kernel).groups())
+        assert int(grid) == (M // rows + min(M, G)) * -(-N // wide), (G, M, N, line)

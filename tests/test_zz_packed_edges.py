@@ -91,3 +91,27 @@ def test_groups_whatever_the_offsets(line):
         if limits[k + 1] > limits[k]:
             _near(out[limits[k]:limits[k + 1]], *_wide(x[limits[k]:limits[k + 1]], w[k], kind), F32, k)
     assert (out[:limits[0]] == 7).all() and (out[limits[-1]:] == 7).all()
+
+
+@pytest.mark.parametrize("kind", [INT8, BF16])
+@pytest.mark.parametrize("G,M", [(1000, 16), (3000, 40), (200, 200), (201, 200), (64, 63), (130, 900)])
+def test_groups_that_are_mostly_empty(G, M, kind):
+    """Every row another group's, all rows the last group's, the first one's, and rows dealt at random."""
+    from burn_dragon_amd.packed import PackedWeights, grouped_product
+
+    K, N = 130, 70
+    g = _dev_gen(G + M)
+    x, w = torch.randn((M, K), generator=g, device=DEV), torch.randn((G, K, N), generator=g, device=DEV)
+    packed = PackedWeights(w, dtype=kind)
+    spread = torch.zeros(G, dtype=torch.int64)
+    spread[torch.randperm(G)[:min(G, M)]] = 1
+    spread[G // 2] += M - int(spread.sum())
+    ends = {"spread": spread, "last": torch.tensor([0] * (G - 1) + [M]), "first": torch.tensor([M] + [0] * (G - 1)),
+            "random": torch.bincount(torch.randint(0, G, (M,), generator=torch.Generator().manual_seed(G)), minlength=G)}
+    for name, sizes in ends.items():
+        limits = [0, *sizes.cumsum(0).tolist()]
+        out = grouped_product(x, packed, torch.tensor(limits, dtype=torch.int32, device=DEV))
+        group = torch.repeat_interleave(torch.arange(G), sizes).tolist()
+        for k in set(group):
+            a, b = limits[k], limits[k + 1]
+            _near(out[a:b], *_wide(x[a:b], w[k], kind), F32, (name, k))
