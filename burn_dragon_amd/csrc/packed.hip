@@ -1397,7 +1397,7 @@ size_t bdh_packed_workspace(const bdh_ctx *ctx, const bdh_packed_weights *w, int
   if (!ctx || !w || (w->type != BDH_INT8 && w->type != BDH_BF16) || w->inner < 1 || w->outer < 1 || w->groups < 1 || rows_in <= 0 ||
       rows_of_group == 0 || !is_rows_type(x_dtype))
     return 0;
-  return plan_of(ctx, *w, rows_in, rows_of_group, x, x_dtype, x_stride, false).bytes;  // a gate changes no size
+  return plan_of(ctx, *w, rows_in, rows_of_group, x, x_dtype, x_stride, false).bytes;  // a gate never needs more
 }
 
 int bdh_packed_product(bdh_ctx *ctx, const bdh_packed_weights *w, int64_t rows, const void *x, int x_dtype, int64_t x_stride, void *out,

@@ -103,7 +103,8 @@ class BDH:
         """The projections of every layer (encoder, encoder_v, decoder) through weights packed for the matrix cores, torch.int8
         or torch.bfloat16 (packed.PackedWeights); None goes back to the f32 weights, which are kept.  Every call made
         afterwards takes them.  For prompts, batches and models whose weights are long; a model that runs a decode step in
-        one launch, or two a layer, is faster without."""
+        one launch, or two a layer, is faster without.  Both types change the logits: on a trained checkpoint of 4 layers of 4 x 128
+        neurons int8 costs 3e-4 nats a token (KL from f32; the likeliest token is another in 1.1 % of places), bf16 1.5e-5 (0.25 %)."""
         packed = None
         if dtype is not None:
             from ..packed import PackedWeights
