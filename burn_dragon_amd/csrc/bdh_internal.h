@@ -109,8 +109,8 @@ bool bdh_capturing(bdh_ctx *ctx);
 // stream, unless a captured call may have been given it: then it goes to `kept`.
 int bdh_grow(bdh_ctx *ctx, const char *what, size_t bytes, void **buffer, size_t *held, bool *captured, bdh_outgrown **kept);
 void bdh_free_outgrown(bdh_outgrown **kept);
-// The device copy of a mask of n bytes: the one that `key` was copied to, if that is this mask, or a new copy, behind a wait for
-// the calls that may still read the old one.  A copy that a captured call may have been given stays as it is.
+// The device copy of a block mask of n bytes: the one that is there, if it is the `same` mask, or a new copy, behind a wait for the
+// calls that may still read the old one.  A copy that a captured call may have been given stays as it is.
 int bdh_mask_on_device(bdh_ctx *ctx, const unsigned char *mask, size_t n, bool same, void **buffer, size_t *held, bool *captured);
 
 // Grows ctx->ws to at least `bytes`, by bdh_grow.

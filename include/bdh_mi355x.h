@@ -688,10 +688,11 @@ int bdh_count_tokens(bdh_ctx *ctx, int B, int T, int V, const int64_t *tokens, i
  *   are in out.  Offsets that decrease or leave 0 .. rows count as their running maximum within 0 .. rows.
  * A call takes up to 2^31 - 256 rows, of x and of out, and 2^32 threads a launch (2^28 rows of up to 512 values, 2^22 of more than 8192).
  * x, in, gate and out are BDH_F32 or BDH_BF16 each, strides in values; an f32 result is rounded once where out is BDH_BF16.  out
- * shares no value with what is read (the rows of x and of out may be columns of one buffer).  The workspace is the caller's, bdh_packed_workspace bytes of it (0: none; on 16 bytes) for the
- * same weights, rows and place of the rows: rows_in = the rows of x or in, rows_of_group = rows that meet each group (B * T of
- * bdh_packed_relu_lowrank), -1 for bdh_grouped_product.  Nothing is copied to or from the host, no result depends on the order of
- * atomics, and a call in a HIP graph uses the workspace it was captured with.
+ * shares no value with what is read (the rows of x and of out may be columns of one buffer).  The workspace is the caller's,
+ * bdh_packed_workspace bytes of it (0: none; on 16 bytes) for the same weights, rows and place of the rows: rows_in = the rows of x
+ * or in, rows_of_group = rows that meet each group (B * T of bdh_packed_relu_lowrank), -1 for bdh_grouped_product.  Nothing is
+ * copied to or from the host, no result depends on the order of atomics, and a call in a HIP graph uses the workspace it was
+ * captured with.
  */
 typedef struct bdh_packed_weights {
   int32_t type, groups, inner, outer;
